@@ -1,6 +1,6 @@
 """In-tree builds of the native libraries (no JIT cache, no pip install).
 
-libdfgpu.so         CUDA kernels + the C ABI of include/dfgpu.h, compiled for sm_100a only.
+libdfgpu.so         CUDA kernels + the C ABI of include/dfgpu.h and include/dfgpu_cache.h, compiled for sm_100a only.
 libdeepforge_b200.so  C++20 host side (importer, graph analysis, workspace planner,
                     kernel-selection lowering, runtime) + the flat C API of
                     include/deepforge_b200.h. It links libdfgpu.so.
@@ -66,7 +66,7 @@ def nlohmann_include() -> Path:
 def build_kernels(force: bool = False, verbose: bool = False) -> Path:
     OUT.mkdir(exist_ok=True)
     sources = sorted((PKG / "csrc").glob("*.cu"))
-    headers = sorted((PKG / "csrc").glob("*.cuh")) + [ROOT / "include" / "dfgpu.h"]
+    headers = sorted((PKG / "csrc").glob("*.cuh")) + [ROOT / "include" / "dfgpu.h", ROOT / "include" / "dfgpu_cache.h"]
     target = OUT / "libdfgpu.so"
     stamp = _stamp(sources + headers, " ".join(NVCC_FLAGS))
     if not force and _up_to_date(target, stamp):
