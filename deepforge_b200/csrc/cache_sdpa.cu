@@ -8,60 +8,57 @@
 // With 16 rows the tensor cores have 16 multiply-adds for each code, 384 a clock and SM at HBM speed.
 //   * Q is not rounded: each row is scaled by a power of two that puts its largest magnitude at 2^14, and is exact in f16 down to
 //     2^-38 of that (below, within 2^-39 of it).
-//   * 16 consecutive keys share a page and a scale (both are multiples of 16 tokens): the K scale multiplies scores, the V scale
-//     the product of 16 or 32 keys before it is added up in f32, so that no scale however far from its neighbours costs bits.
-//   * Probabilities are rounded to f16 as p * 2^15: 11 bits down to 2^-29, where p is measured against the largest score so far.
+//   * 16 consecutive keys share a page and a scale (both are multiples of 16 tokens). The K scale multiplies their scores. O is
+//     held in units of a power of two, 2^unit: the V scale of 16 keys goes into their probabilities, as 2^(scale - unit), where that is from 2^-10
+//     to 1, and else the unit moves and O with it (exactly, as far as scales within 2^80 of one another go).
+//   * Probabilities are rounded to f16 as p * 2^15: 11 bits down to 2^-29 (2^-19 beside a V scale of 2^-10 units), where p is measured
+//     against the largest score so far.
 // Channels and keys may go to any k index of a product as long as both operands agree; the ones taken here give each thread 16-byte
 // reads without bank conflicts: of K 32 consecutive channels of a key, of V 16 consecutive channels of four keys, and of O 32
 // consecutive channels of a row.
-// CTA: one (sequence, KV head, block of rows), a run of key tiles; four warps share each tile's keys out between them, or its rows where there are
-// more than 16, or both. Tiles come by cp.async into a ring of three stages; two CTAs fit on an SM. More than one run of key tiles a
-// sequence leaves partial results that a second kernel merges.
+// CTA: one (sequence, KV head, block of rows), a run of key tiles; a fifth warp brings the tiles by TMA (whole pages or runs of them,
+// swizzled) into a ring, four share each tile's keys out between them, or its rows where there are more than 16, or
+// both. Two CTAs fit on an SM. More than one run of key tiles a sequence leaves partial results that a second kernel merges.
 #include <algorithm>
 #include <cmath>
 
 #include "cache_sdpa.cuh"
-#include "common.cuh"
 #include "dfgpu_cache.h"
+#include "umma_ptx.cuh"
 
 namespace dfgpu {
 namespace {
 
-constexpr int kWarps = 4, kThreads = 128;
+constexpr int kWarps = 4, kConsumers = 128, kThreads = 160;
 constexpr int kMostTiles = 32;     // key tiles a CTA
 constexpr float kUp = 15.0f;       // probabilities are held as p * 2^15
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kNoUnit = -100000;   // O is zero and has no unit yet
+constexpr int kNaN = 0x7fc00000;
 
 template <int D>
 struct Shape {
     static constexpr int kKeys = D == 256 ? 64 : 128;     // keys a tile
     static constexpr int kRuns = kKeys / 16;
     static constexpr int kTile = kKeys * D;               // bytes of a K or V tile
-    static constexpr int kStages = D == 64 ? 4 : 3;
-    static constexpr int kChunks = D / 16;                // 16-byte chunks a row
+    static constexpr int kCtas = D == 256 ? 1 : 2;        // on an SM: a D of 256 takes 255 registers a thread
+    static constexpr int kStages = D == 64 ? 4 : 3 * (3 - kCtas);
     static constexpr int kRing = kStages * 2 * kTile;
-    static constexpr int kOffsets = kRing;                // [K | V][runs] int64: of the first code of a run, -1: reads as zeros
-    static constexpr int kScales = kOffsets + 2 * kMostTiles * kRuns * 8;   // [K | V][runs] f32
-    static constexpr int kTotal = kScales + 2 * kMostTiles * kRuns * 4;
+    static constexpr int kKScales = kRing;                                    // [runs] f32, -1: the page's rows read as zeros
+    static constexpr int kVScales = kKScales + kMostTiles * kRuns * 4;        // [runs] the code, -1 likewise
+    static constexpr int kBarriers = kVScales + kMostTiles * kRuns * 4;       // full[stages], empty[stages]
+    static constexpr int kTotal = kBarriers + 2 * kStages * 8;
+    static constexpr int kDynamic = kTotal + 1024;
 };
 
-// Byte offset of a 16-byte chunk of a tile's row: rows are spread so that the reads above meet each bank once.
+// Byte offset of a 16-byte chunk of a tile's row, as TMA lays rows of 128 or 64 bytes out (a D of 256: two halves): the reads above meet each bank once.
 template <int D>
 __device__ __forceinline__ uint32_t at_chunk(int row, int chunk) {
-    return D == 64 ? row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4) : row * D + ((chunk ^ (row & 7)) << 4);
+    return D == 64 ? row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4) : (chunk >> 3) * (Shape<D>::kKeys * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
 }
 
-__device__ __forceinline__ void copy_16(uint32_t to, const void* from, bool live) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-__device__ __forceinline__ uint32_t two_codes(uint32_t codes16) {   // the low two codes as f16
-    uint32_t v;
-    asm("{\n\t.reg .b16 c;\n\tcvt.u16.u32 c, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, c;\n\t}" : "=r"(v) : "r"(codes16));
-    return v;
+__device__ __forceinline__ void four_codes(uint32_t codes, uint32_t& low, uint32_t& high) {   // as f16
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(low), "=r"(high) : "r"(codes));
 }
 __device__ __forceinline__ uint32_t two_halves(float lo, float hi) {
     uint32_t v;
@@ -77,7 +74,17 @@ __device__ __forceinline__ void multiply(float (&c)[4], const uint32_t (&a)[4], 
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void multiply_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+__device__ __forceinline__ uint32_t times(uint32_t pair, uint32_t factor) {
+    uint32_t v;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(v) : "r"(pair), "r"(factor));
+    return v;
+}
 __device__ __forceinline__ uint4 read_16(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
+__device__ __forceinline__ float power_of_two(int n) { return __uint_as_float(static_cast<uint32_t>(n + 127) << 23); }   // -126 to 127
 
 __device__ __forceinline__ float value_of(__half v) { return __half2float(v); }
 __device__ __forceinline__ float value_of(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -104,236 +111,141 @@ __device__ __forceinline__ void store_values(const CacheSdpaArgs& a, int64_t at,
     for (int i = 0; i < COUNT; ++i) store_from_f32(a.o, a.o_type, at + i, v[i]);
 }
 
-template <typename T, int D, int MT>
-__global__ void __launch_bounds__(kThreads, D == 64 ? 3 : 2)
-cache_sdpa_stream_kernel(CacheSdpaArgs a) {
-    using S = Shape<D>;
-    constexpr int kGroups = kWarps / MT;              // warps that share an M tile's keys
-    constexpr int kOwn = S::kKeys / kGroups;          // keys a warp and tile
-    constexpr int kStep = kOwn < 32 ? kOwn : 32;      // keys at a time
-    constexpr int kStepRuns = kStep / 16;
-    constexpr int kDeep = D / 16;                     // products along the channels
-    constexpr int kWide = D / 8;                      // products along the channels of V: thread value j
-    constexpr int kReach = D == 64 ? 8 : 16;          // consecutive channels that a thread reads of a V row
-    extern __shared__ __align__(16) uint8_t smem[];
-    int64_t* run_offset = reinterpret_cast<int64_t*>(smem + S::kOffsets);
-    float* run_scale = reinterpret_cast<float*>(smem + S::kScales);
-    const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem));
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane & 3, eighth = lane >> 2;
-    const int mt = warp % MT, group = warp / MT;
-    const int head = blockIdx.y % a.heads_kv, row_block = blockIdx.y / a.heads_kv;
-    const int64_t batch = blockIdx.z;
-    const int row_first = row_block * (MT * 16);
-    chain_begin();
+// The page of a tile's key in a side's table, -1 where there is none.
+__device__ __forceinline__ int page_of(const CacheSdpaArgs& a, const CacheSide& s, int64_t batch, int slot) {
+    if (slot >= s.table_len) return -1;
+    const int page = s.table[batch * s.table_batch + slot * s.table_slot];
+    return page >= 0 && page < s.pages ? page : -1;
+}
 
-    // The keys that any row of the CTA sees, and this CTA's tiles among them.
-    const SequenceWindow window = sequence_window(a, batch);
-    const int token_first = row_first / a.group, token_last = min(row_first + MT * 16, a.rows) - 1;
-    int lo, hi;
-    window_of_tokens(a, window, token_first, token_last / a.group, lo, hi);
-    const int chunk_first = static_cast<int>(blockIdx.x) * a.tiles_per_cta;
-    const int tile_first = max(chunk_first, lo / S::kKeys), tile_end = hi > lo ? min(chunk_first + a.tiles_per_cta, (hi + S::kKeys - 1) / S::kKeys) : 0;
-    const int tiles = tile_end - tile_first;
-    if (tiles <= 0 && a.chunks > 1) return;   // (the merge knows which chunks a row has)
-
-    // Where the runs of 16 keys lie, and their scales.
-    constexpr int kLookups = 2 * kMostTiles * S::kRuns / kThreads;
-    const int runs = max(tiles, 0) * S::kRuns;
-    int64_t scale_at[kLookups];
-#pragma unroll
-    for (int k = 0; k < kLookups; ++k) {
-        scale_at[k] = -1;
-        const int i = threadIdx.x + k * kThreads;
-        if (i >= 2 * runs) continue;
-        const CacheSide& s = a.side[i >= runs ? 1 : 0];
-        const int key = tile_first * S::kKeys + (i >= runs ? i - runs : i) * 16;
-        const int slot = static_cast<int>(fast_divide(static_cast<uint32_t>(key >> 4), a.by_page)), in_page = key - slot * a.page;
-        int64_t offset = -1;
-        if (key < hi && key + 16 > lo && slot < s.table_len) {
-            const int64_t page = s.table[batch * s.table_batch + slot * s.table_slot];
-            if (page >= 0 && page < s.pages) {
-                offset = page * s.stride[0] + head * s.stride[1] + in_page * s.stride[2];
-                scale_at[k] = page * s.scale_stride[0] + head * s.scale_stride[1] + static_cast<int64_t>(fast_divide(static_cast<uint32_t>(in_page >> 4), a.by_tokens)) * s.scale_stride[2];
-            }
-        }
-        run_offset[i >= runs ? i - runs + kMostTiles * S::kRuns : i] = offset;
-    }
-    __syncthreads();
-    auto fetch = [&](int t) {
-        if (t < tiles) {
-            constexpr int kRowsAtOnce = kThreads / S::kChunks;
-            const int chunk = threadIdx.x % S::kChunks, row0 = threadIdx.x / S::kChunks;
-            const uint32_t stage = ring + (t % S::kStages) * (2 * S::kTile);
-            const int key0 = (tile_first + t) * S::kKeys;
-#pragma unroll
-            for (int which = 0; which < 2; ++which) {
-                const CacheSide& s = a.side[which];
-#pragma unroll
-                for (int r = 0; r < S::kKeys; r += kRowsAtOnce) {
-                    const int row = r + row0;
-                    const int64_t offset = run_offset[which * (kMostTiles * S::kRuns) + t * S::kRuns + (row >> 4)];
-                    const bool live = offset >= 0 && key0 + row >= lo && key0 + row < hi;   // (others read as zeros: no stale NaN meets a zero probability)
-                    copy_16(stage + which * S::kTile + at_chunk<D>(row, chunk), s.codes + (live ? offset + (row & 15) * s.stride[2] + chunk * 16 : 0), live);
-                }
-            }
-        }
-        copies_commit();
-    };
-#pragma unroll
-    for (int t = 0; t < S::kStages - 1; ++t) fetch(t);
-#pragma unroll
-    for (int k = 0; k < kLookups; ++k) {
-        const int i = threadIdx.x + k * kThreads;
-        if (i >= 2 * runs) continue;
-        const bool is_v = i >= runs;
-        run_scale[is_v ? i - runs + kMostTiles * S::kRuns : i] = scale_at[k] >= 0 ? decode_e8m0(a.side[is_v ? 1 : 0].scales[scale_at[k]]) : 1.0f;
-    }
-
-    // This thread's two rows: their windows and their share of Q.
+// 16 rows of one M tile against the codes of K and V that its warp takes.
+template <int D>
+struct RowTile {
+    static constexpr int kDeep = D / 16;                     // products along the channels
+    static constexpr int kWide = D / 8;                      // products along the channels of V: thread value j
+    static constexpr int kReach = D == 64 ? 8 : 16;          // consecutive channels that a thread reads of a V row
     uint32_t q[kDeep][4];
     float factor[2];            // of a score: 1 / the row's power of two, attention scale, log2(e)
-    int row_lo[2], row_hi[2];
-    int64_t token_of[2];
-    int head_of[2];
-    bool live_row[2];           // has a place in O
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        const int row = row_first + mt * 16 + half * 8 + eighth;
-        live_row[half] = row < a.rows;
-        const int token = live_row[half] ? row / a.group : 0;
-        token_of[half] = token;
-        head_of[half] = head * a.group + (live_row[half] ? row - token * a.group : 0);
-        const bool takes_part = live_row[half] && token < window.len_q;
-        row_lo[half] = lo, row_hi[half] = hi;                // (rows without a part see what the others see; their results go nowhere)
-        if (takes_part) window_of_tokens(a, window, token, token, row_lo[half], row_hi[half]);
-        row_hi[half] = max(row_hi[half], row_lo[half]);
-        const T* from = static_cast<const T*>(a.q) + batch * a.q_stride[0] + head_of[half] * a.q_stride[1] + token * a.q_stride[2];
-        float v[kDeep][4];
-        float largest = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kDeep; ++i) {
-            const int channel = D == 64 ? quad * 16 + i * 4 : (quad * 2 + ((i >> 2) & 1) + (i >> 3) * 8) * 16 + (i & 3) * 4;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                v[i][e] = live_row[half] ? value_of(from[channel + e]) : 0.0f;
-                largest = fmaxf(largest, fabsf(v[i][e]));
-            }
-        }
-        largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-        largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-        int up = 14 - (static_cast<int>(__float_as_uint(largest) >> 23) - 127);
-        up = largest == 0.0f ? 0 : min(max(up, -126), 126);
-        const float power = __uint_as_float(static_cast<uint32_t>(up + 127) << 23);
-        factor[half] = __uint_as_float(static_cast<uint32_t>(127 - up) << 23) * a.scale_log2;
-#pragma unroll
-        for (int i = 0; i < kDeep; ++i) {
-            q[i][half] = two_halves(v[i][0] * power, v[i][1] * power);
-            q[i][2 + half] = two_halves(v[i][2] * power, v[i][3] * power);
-        }
-    }
-    // What the warp's rows see in common, and what any of them sees.
-    const int common_lo = __reduce_max_sync(0xffffffffu, max(row_lo[0], row_lo[1])), common_hi = __reduce_min_sync(0xffffffffu, min(row_hi[0], row_hi[1]));
-    const int any_lo = __reduce_min_sync(0xffffffffu, min(row_lo[0], row_lo[1])), any_hi = __reduce_max_sync(0xffffffffu, max(row_hi[0], row_hi[1]));
-
-    float largest[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+    int row_lo[2], row_hi[2];   // keys that the thread's two rows see
+    float largest[2], sum[2];
     float o[kWide][4];
-#pragma unroll
-    for (int j = 0; j < kWide; ++j)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) o[j][c] = 0.0f;
+    int unit;
 
-    for (int t = 0; t < tiles; ++t) {
-        copies_wait<S::kStages - 2>();
-        __syncthreads();
-        fetch(t + S::kStages - 1);
-        const uint8_t* k_tile = smem + (t % S::kStages) * (2 * S::kTile);
-        const uint8_t* v_tile = k_tile + S::kTile;
-#pragma unroll 1
-        for (int step = group * kOwn; step < (group + 1) * kOwn; step += kStep) {
-            const int key0 = (tile_first + t) * S::kKeys + step;
-            if (key0 >= any_hi || key0 + kStep <= any_lo) continue;
-            const bool masked = key0 < common_lo || key0 + kStep > common_hi;
-            const float* scales = run_scale + t * S::kRuns + (step >> 4);
-            // scores: 8 keys a product, keys along its columns
-            float s[kStep / 8][4];
+    // KEYS keys from row `row` of a tile, key0 of the sequence. SPECIAL: some row does not see all of them, or a page or scale is none.
+    template <bool SPECIAL, int KEYS>
+    __device__ __forceinline__ void step(const uint8_t* k_tile, const uint8_t* v_tile, const float* k_scales, const int* v_scales, int row, int key0, int lo, int hi, bool mixed) {
+        const int lane = threadIdx.x & 31, quad = lane & 3, eighth = lane >> 2;
+        constexpr int kRuns = KEYS / 16;
+        float s[KEYS / 8][4];   // scores: 8 keys a product, keys along its columns
 #pragma unroll
-            for (int n = 0; n < kStep / 8; ++n) {
+        for (int n = 0; n < KEYS / 8; ++n) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c) s[n][c] = 0.0f;
-                const int row = step + n * 8 + eighth;
+            for (int u = 0; u < kDeep / 4; ++u) {
+                const uint4 raw = read_16(k_tile + at_chunk<D>(row + n * 8 + eighth, D == 64 ? quad : quad * 2 + (u & 1) + (u >> 1) * 8));
+                const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-                for (int u = 0; u < kDeep / 4; ++u) {
-                    const uint4 raw = read_16(k_tile + at_chunk<D>(row, D == 64 ? quad : quad * 2 + (u & 1) + (u >> 1) * 8));
-                    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) multiply(s[n], q[u * 4 + i], two_codes(w[i]), two_codes(w[i] >> 16));
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t b0, b1;
+                    four_codes(w[i], b0, b1);
+                    if (u + i == 0) multiply_first(s[n], q[0], b0, b1);
+                    else multiply(s[n], q[u * 4 + i], b0, b1);
                 }
             }
-            bool above = false;
+        }
+        bool above = false;
 #pragma unroll
-            for (int n = 0; n < kStep / 8; ++n) {
-                const float k_scale = scales[n >> 1];
-                const float f0 = factor[0] * k_scale, f1 = factor[1] * k_scale;
-                s[n][0] *= f0, s[n][1] *= f0, s[n][2] *= f1, s[n][3] *= f1;
-                if (masked) {
+        for (int n = 0; n < KEYS / 8; ++n) {
+            const float k_scale = k_scales[n >> 1];
+            const float f0 = factor[0] * k_scale, f1 = factor[1] * k_scale;
+            s[n][0] *= f0, s[n][1] *= f0, s[n][2] *= f1, s[n][3] *= f1;
+            if (SPECIAL) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const int key = key0 + n * 8 + quad * 2 + (c & 1);
-                        if (static_cast<uint32_t>(key - row_lo[c >> 1]) >= static_cast<uint32_t>(row_hi[c >> 1] - row_lo[c >> 1])) s[n][c] = -INFINITY;
+                for (int c = 0; c < 4; ++c) {
+                    const int key = key0 + n * 8 + quad * 2 + (c & 1);
+                    if (k_scale < 0.0f) s[n][c] = 0.0f;
+                    if (static_cast<uint32_t>(key - row_lo[c >> 1]) >= static_cast<uint32_t>(row_hi[c >> 1] - row_lo[c >> 1])) s[n][c] = -INFINITY;
+                }
+            }
+            above = above || fmaxf(s[n][0], s[n][1]) > largest[0] || fmaxf(s[n][2], s[n][3]) > largest[1];
+        }
+        if (__any_sync(0xffffffffu, above)) {   // a new largest score in some row (rare after the first tiles)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                float top = largest[half];
+#pragma unroll
+                for (int n = 0; n < KEYS / 8; ++n) top = fmaxf(top, fmaxf(s[n][2 * half], s[n][2 * half + 1]));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const float down = top == -INFINITY ? 1.0f : exp2_of(largest[half] - top);
+                largest[half] = top;
+                sum[half] *= down;
+#pragma unroll
+                for (int j = 0; j < kWide; ++j) o[j][2 * half] *= down, o[j][2 * half + 1] *= down;
+            }
+        }
+        const float from0 = largest[0] == -INFINITY ? 0.0f : kUp - largest[0], from1 = largest[1] == -INFINITY ? 0.0f : kUp - largest[1];
+        uint32_t p[kRuns][4];
+#pragma unroll
+        for (int n = 0; n < KEYS / 8; ++n) {
+            const float p0 = exp2_of(s[n][0] + from0), p1 = exp2_of(s[n][1] + from0), p2 = exp2_of(s[n][2] + from1), p3 = exp2_of(s[n][3] + from1);
+            sum[0] += p0 + p1;
+            sum[1] += p2 + p3;
+            p[n >> 1][(n & 1) * 2] = two_halves(p0, p1);
+            p[n >> 1][(n & 1) * 2 + 1] = two_halves(p2, p3);
+        }
+#pragma unroll
+        for (int r = 0; r < kRuns; ++r) {
+            const int code = v_scales[r], apart = code - unit;   // (the same in all threads)
+            if ((!SPECIAL || (code >= 0 && code != 255)) && apart != 0) {
+                if (apart < 0 && (apart >= -10 || apart < -80)) {
+                    const uint32_t less = apart < -80 ? 0u : static_cast<uint32_t>(15 + apart) << 10, both = less | less << 16;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) p[r][c] = times(p[r][c], both);
+                } else {
+                    const float to = unit == kNoUnit ? 1.0f : power_of_two(max(-apart, -126));
+#pragma unroll
+                    for (int j = 0; j < kWide; ++j)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) o[j][c] *= to;
+                    unit = code;
+                }
+            }
+            // V: thread value j of a run is channel 16 * eighth + j of keys 2 quad, 2 quad + 1 and those plus 8
+            uint32_t w[4][kWide / 4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int at = row + r * 16 + quad * 2 + (k & 1) + (k >> 1) * 8;
+                if constexpr (D == 64) {
+                    const uint2 raw = *reinterpret_cast<const uint2*>(v_tile + at_chunk<D>(at, eighth >> 1) + (eighth & 1) * 8);
+                    w[k][0] = raw.x, w[k][1] = raw.y;
+                } else {
+#pragma unroll
+                    for (int u = 0; u < kWide / 16; ++u) {
+                        const uint4 raw = read_16(v_tile + at_chunk<D>(at, eighth + u * 8));
+                        w[k][u * 4] = raw.x, w[k][u * 4 + 1] = raw.y, w[k][u * 4 + 2] = raw.z, w[k][u * 4 + 3] = raw.w;
                     }
                 }
-                above = above || fmaxf(s[n][0], s[n][1]) > largest[0] || fmaxf(s[n][2], s[n][3]) > largest[1];
-            }
-            if (__any_sync(0xffffffffu, above)) {   // a new largest score in some row (rare after the first tiles)
+                if (SPECIAL) {   // rows that nothing was brought to, or that no row sees: anything may lie there, NaN codes too
+                    const int key = key0 + r * 16 + quad * 2 + (k & 1) + (k >> 1) * 8;
+                    if (code < 0 || key < lo || key >= hi) {
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    float top = largest[half];
-#pragma unroll
-                    for (int n = 0; n < kStep / 8; ++n) top = fmaxf(top, fmaxf(s[n][2 * half], s[n][2 * half + 1]));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                    const float down = top == -INFINITY ? 1.0f : exp2_of(largest[half] - top);
-                    largest[half] = top;
-                    sum[half] *= down;
-#pragma unroll
-                    for (int j = 0; j < kWide; ++j) o[j][2 * half] *= down, o[j][2 * half + 1] *= down;
-                }
-            }
-            const float from0 = largest[0] == -INFINITY ? 0.0f : kUp - largest[0], from1 = largest[1] == -INFINITY ? 0.0f : kUp - largest[1];
-            uint32_t p[kStepRuns][4];
-#pragma unroll
-            for (int n = 0; n < kStep / 8; ++n) {
-                const float p0 = exp2_of(s[n][0] + from0), p1 = exp2_of(s[n][1] + from0), p2 = exp2_of(s[n][2] + from1), p3 = exp2_of(s[n][3] + from1);
-                sum[0] += p0 + p1;
-                sum[1] += p2 + p3;
-                p[n >> 1][(n & 1) * 2] = two_halves(p0, p1);
-                p[n >> 1][(n & 1) * 2 + 1] = two_halves(p2, p3);
-            }
-            const bool mixed = masked && a.seq_q > 1;   // some rows see a key that others do not
-#pragma unroll
-            for (int r = 0; r < kStepRuns; ++r) {
-                // V: thread value j of a run is channel 16 * eighth + j of keys 2 quad, 2 quad + 1 and those plus 8
-                uint32_t w[4][kWide / 4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int row = step + r * 16 + quad * 2 + (k & 1) + (k >> 1) * 8;
-                    if constexpr (D == 64) {
-                        const uint2 raw = *reinterpret_cast<const uint2*>(v_tile + at_chunk<D>(row, eighth >> 1) + (eighth & 1) * 8);
-                        w[k][0] = raw.x, w[k][1] = raw.y;
-                    } else {
-#pragma unroll
-                        for (int u = 0; u < kWide / 16; ++u) {
-                            const uint4 raw = read_16(v_tile + at_chunk<D>(row, eighth + u * 8));
-                            w[k][u * 4] = raw.x, w[k][u * 4 + 1] = raw.y, w[k][u * 4 + 2] = raw.z, w[k][u * 4 + 3] = raw.w;
-                        }
+                        for (int i = 0; i < kWide / 4; ++i) w[k][i] = 0;
                     }
                 }
-                float v_scale[2] = {scales[kMostTiles * S::kRuns + r], 0.0f};
-                v_scale[1] = v_scale[0];
+            }
+            if (SPECIAL) {
+                const int run0 = key0 + r * 16;
+                const bool sees[2] = {run0 < row_hi[0] && run0 + 16 > row_lo[0], run0 < row_hi[1] && run0 + 16 > row_lo[1]};
+                if (code == 255) {   // a scale that is a NaN: for the rows that see one of its keys
+#pragma unroll
+                    for (int j = 0; j < kWide; ++j)
+#pragma unroll
+                        for (int c = 0; c < 4; ++c)
+                            if (sees[c >> 1]) o[j][c] = __int_as_float(kNaN);
+                }
                 if (mixed) {
-                    // A NaN code or scale must reach the rows that see its key and no others, whose probability for it is 0: NaN codes become zeros in the
+                    // A NaN code must reach the rows that see its key and no others, whose probability for it is 0: such codes become zeros in the
                     // products, and NaNs in the sums of the rows that they belong to.
-                    const int run0 = key0 + r * 16;
                     uint32_t nan = 0;
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
@@ -346,68 +258,227 @@ cache_sdpa_stream_kernel(CacheSdpaArgs a) {
                     if (__any_sync(0xffffffffu, nan != 0)) {
 #pragma unroll 1
                         for (int k = 0; k < 16; ++k) {
-                            const bool sees0 = run0 + k >= row_lo[0] && run0 + k < row_hi[0], sees1 = run0 + k >= row_lo[1] && run0 + k < row_hi[1];
+                            const bool in0 = run0 + k >= row_lo[0] && run0 + k < row_hi[0], in1 = run0 + k >= row_lo[1] && run0 + k < row_hi[1];
 #pragma unroll
                             for (int j = 0; j < kWide; ++j)
 #pragma unroll
                                 for (int c = 0; c < 2; ++c) {
-                                    const int column = quad * 2 + c, channel = column * kReach + (j & (kReach - 1)) + (j / kReach) * 128;
-                                    const uint8_t code = v_tile[at_chunk<D>(step + r * 16 + k, channel >> 4) + (channel & 15)];
-                                    if ((code & 0x7fu) == 0x7fu) {
-                                        if (sees0) o[j][c] = __int_as_float(0x7fc00000);
-                                        if (sees1) o[j][2 + c] = __int_as_float(0x7fc00000);
+                                    const int channel = (quad * 2 + c) * kReach + (j & (kReach - 1)) + (j / kReach) * 128;
+                                    const uint8_t found = v_tile[at_chunk<D>(row + r * 16 + k, channel >> 4) + (channel & 15)];
+                                    if ((found & 0x7fu) == 0x7fu) {
+                                        if (in0) o[j][c] = __int_as_float(kNaN);
+                                        if (in1) o[j][2 + c] = __int_as_float(kNaN);
                                     }
                                 }
                         }
                     }
-#pragma unroll
-                    for (int half = 0; half < 2; ++half)
-                        if (!(run0 < row_hi[half] && run0 + 16 > row_lo[half])) v_scale[half] = 0.0f;
                 }
+            }
 #pragma unroll
-                for (int i = 0; i < kWide / 4; ++i) {
-                    const uint32_t a01 = __byte_perm(w[0][i], w[1][i], 0x5140), a23 = __byte_perm(w[0][i], w[1][i], 0x7362);
-                    const uint32_t b01 = __byte_perm(w[2][i], w[3][i], 0x5140), b23 = __byte_perm(w[2][i], w[3][i], 0x7362);
-                    const uint32_t first[4] = {two_codes(a01), two_codes(a01 >> 16), two_codes(a23), two_codes(a23 >> 16)};
-                    const uint32_t second[4] = {two_codes(b01), two_codes(b01 >> 16), two_codes(b23), two_codes(b23 >> 16)};
+            for (int i = 0; i < kWide / 4; ++i) {
+                uint32_t first[4], second[4];
+                four_codes(__byte_perm(w[0][i], w[1][i], 0x5140), first[0], first[1]);
+                four_codes(__byte_perm(w[0][i], w[1][i], 0x7362), first[2], first[3]);
+                four_codes(__byte_perm(w[2][i], w[3][i], 0x5140), second[0], second[1]);
+                four_codes(__byte_perm(w[2][i], w[3][i], 0x7362), second[2], second[3]);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                        multiply(c, p[r], first[e], second[e]);
-                        float(&to)[4] = o[i * 4 + e];
-                        to[0] = fmaf(c[0], v_scale[0], to[0]);
-                        to[1] = fmaf(c[1], v_scale[0], to[1]);
-                        to[2] = fmaf(c[2], v_scale[1], to[2]);
-                        to[3] = fmaf(c[3], v_scale[1], to[3]);
-                    }
-                }
+                for (int e = 0; e < 4; ++e) multiply(o[i * 4 + e], p[r], first[e], second[e]);
             }
         }
     }
+};
+
+template <typename T, int D, int MT>
+__global__ void __launch_bounds__(kThreads, Shape<D>::kCtas)
+cache_sdpa_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CacheSdpaArgs a) {
+    using S = Shape<D>;
+    using Rows = RowTile<D>;
+    constexpr int kGroups = kWarps / MT;              // warps that share an M tile's keys
+    constexpr int kOwn = S::kKeys / kGroups;          // keys a warp and tile
+    constexpr int kStep = kOwn < 32 ? kOwn : 32;      // keys at a time
+    constexpr int kWide = Rows::kWide, kReach = Rows::kReach;
+    extern __shared__ uint8_t raw_smem[];
+    const uint32_t ring = (smem_u32(raw_smem) + 1023u) & ~1023u;
+    uint8_t* smem = raw_smem + (ring - smem_u32(raw_smem));
+    float* k_scales = reinterpret_cast<float*>(smem + S::kKScales);
+    int* v_scales = reinterpret_cast<int*>(smem + S::kVScales);
+    auto full = [&](int s) { return ring + S::kBarriers + 8u * s; };
+    auto empty = [&](int s) { return ring + S::kBarriers + 8u * (S::kStages + s); };
+    const int warp = uniform_warp_index(), lane = threadIdx.x & 31;
+    const int head = blockIdx.y % a.heads_kv, row_block = blockIdx.y / a.heads_kv;
+    const int64_t batch = blockIdx.z;
+    const int row_first = row_block * (MT * 16);
+    if (threadIdx.x == 0) {
+        prefetch_tensormap(&map_k);
+        prefetch_tensormap(&map_v);
+        for (int s = 0; s < S::kStages; ++s) {
+            mbar_init(full(s), 1);
+            mbar_init(empty(s), kWarps);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    chain_begin();
+
+    const int chunk_first = static_cast<int>(blockIdx.x) * a.tiles_per_cta;
+    if (warp == kWarps) {
+        // The loader: lane l brings one box of a tile, `box` rows (a page or a part of one) of K or V by 128 or 64 bytes. Page ids are read a tile ahead of
+        // their use, and the first ones before the lengths are known.
+        constexpr int kHalves = D == 256 ? 2 : 1;
+        const int boxes = S::kKeys / a.box, side = lane / (boxes * kHalves), within = lane % (boxes * kHalves);
+        const bool has_box = side < 2;
+        const CacheSide& s = a.side[has_box ? side : 0];
+        const int box_row = (within / kHalves) * a.box, half = within % kHalves;
+        const uint32_t box_bytes = static_cast<uint32_t>(a.box) * (D == 64 ? 64u : 128u);
+        const uint32_t to = side * S::kTile + half * (S::kKeys * 128) + box_row * (D == 64 ? 64 : 128);
+        auto locate = [&](int tile, int& page, int& token) {
+            const int key = tile * S::kKeys + box_row, slot = static_cast<int>(fast_divide(static_cast<uint32_t>(key >> 4), a.by_page));
+            token = key - slot * a.page;
+            page = has_box ? page_of(a, s, batch, slot) : -1;
+        };
+        int page, token;
+        locate(chunk_first, page, token);
+        const SequenceWindow window = sequence_window(a, batch);
+        int lo, hi;
+        window_of_tokens(a, window, row_first / a.group, (min(row_first + MT * 16, a.rows) - 1) / a.group, lo, hi);
+        const int tile_first = max(chunk_first, lo / S::kKeys), tile_end = hi > lo ? min(chunk_first + a.tiles_per_cta, (hi + S::kKeys - 1) / S::kKeys) : 0;
+        if (tile_first != chunk_first && tile_first < tile_end) locate(tile_first, page, token);
+        for (int t = 0; t < tile_end - tile_first; ++t) {
+            const int key = (tile_first + t) * S::kKeys + box_row;
+            const bool live = page >= 0 && key < hi && key + a.box > lo;
+            const int now_page = page, now_token = token;
+            if (tile_first + t + 1 < tile_end) locate(tile_first + t + 1, page, token);
+            const int slot = t % S::kStages;
+            if (!mbar_wait_warp(empty(slot), ((t / S::kStages) & 1) ^ 1, 701)) break;
+            const uint32_t count = __popc(__ballot_sync(0xffffffffu, live));
+            if (lane == 0) mbar_expect_tx(full(slot), count * box_bytes);   // (also the arrival; no byte where no page is)
+            __syncwarp();
+            if (live) tma_load_4d(ring + slot * (2 * S::kTile) + to, side ? &map_v : &map_k, half * 128, now_token, head, now_page, full(slot));
+        }
+        return;
+    }
+
+    const int quad = lane & 3, eighth = lane >> 2, mt = warp % MT, group = warp / MT;
+    const SequenceWindow window = sequence_window(a, batch);
+    // The keys that any row of the CTA sees, and this CTA's tiles among them.
+    int lo, hi;
+    window_of_tokens(a, window, row_first / a.group, (min(row_first + MT * 16, a.rows) - 1) / a.group, lo, hi);
+    const int tile_first = max(chunk_first, lo / S::kKeys), tile_end = hi > lo ? min(chunk_first + a.tiles_per_cta, (hi + S::kKeys - 1) / S::kKeys) : 0;
+    const int tiles = tile_end - tile_first;
+    if (tiles <= 0 && a.chunks > 1) return;   // (the merge knows which chunks a row has)
+
+    // The scales of the runs of 16 keys.
+    for (int i = threadIdx.x; i < 2 * tiles * S::kRuns; i += kConsumers) {
+        const bool is_v = i >= tiles * S::kRuns;
+        const CacheSide& s = a.side[is_v ? 1 : 0];
+        const int run = is_v ? i - tiles * S::kRuns : i, key = tile_first * S::kKeys + run * 16;
+        const int slot = static_cast<int>(fast_divide(static_cast<uint32_t>(key >> 4), a.by_page)), block = static_cast<int>(fast_divide(static_cast<uint32_t>((key - slot * a.page) >> 4), a.by_tokens));
+        const int page = key < hi && key + 16 > lo ? page_of(a, s, batch, slot) : -1;
+        const int code = page >= 0 ? s.scales[page * s.scale_stride[0] + head * s.scale_stride[1] + block * s.scale_stride[2]] : -1;
+        if (is_v) v_scales[run] = code;
+        else k_scales[run] = page >= 0 ? decode_e8m0(static_cast<uint32_t>(code)) : -1.0f;
+    }
+
+    Rows rows;
+    int64_t token_of[2];
+    int head_of[2];
+    bool live_row[2];           // has a place in O
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        const int row = row_first + mt * 16 + half * 8 + eighth;
+        live_row[half] = row < a.rows;
+        const int token = live_row[half] ? row / a.group : 0;
+        token_of[half] = token;
+        head_of[half] = head * a.group + (live_row[half] ? row - token * a.group : 0);
+        const bool takes_part = live_row[half] && token < window.len_q;
+        rows.row_lo[half] = lo, rows.row_hi[half] = hi;      // (rows without a part see what the others see; their results go nowhere)
+        if (takes_part) window_of_tokens(a, window, token, token, rows.row_lo[half], rows.row_hi[half]);
+        rows.row_hi[half] = max(rows.row_hi[half], rows.row_lo[half]);
+        const T* from = static_cast<const T*>(a.q) + batch * a.q_stride[0] + head_of[half] * a.q_stride[1] + token * a.q_stride[2];
+        float v[Rows::kDeep][4];
+        float largest = 0.0f;
+#pragma unroll
+        for (int i = 0; i < Rows::kDeep; ++i) {
+            const int channel = D == 64 ? quad * 16 + i * 4 : (quad * 2 + ((i >> 2) & 1) + (i >> 3) * 8) * 16 + (i & 3) * 4;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[i][e] = live_row[half] ? value_of(from[channel + e]) : 0.0f;
+                largest = fmaxf(largest, fabsf(v[i][e]));
+            }
+        }
+        largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+        largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+        int up = 14 - (static_cast<int>(__float_as_uint(largest) >> 23) - 127);
+        up = largest == 0.0f ? 0 : min(max(up, -126), 126);
+        const float power = power_of_two(up);
+        rows.factor[half] = power_of_two(-up) * a.scale_log2;
+#pragma unroll
+        for (int i = 0; i < Rows::kDeep; ++i) {
+            rows.q[i][half] = two_halves(v[i][0] * power, v[i][1] * power);
+            rows.q[i][2 + half] = two_halves(v[i][2] * power, v[i][3] * power);
+        }
+        rows.largest[half] = -INFINITY;
+        rows.sum[half] = 0.0f;
+    }
+    rows.unit = kNoUnit;
+#pragma unroll
+    for (int j = 0; j < kWide; ++j)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) rows.o[j][c] = 0.0f;
+    // What the warp's rows see in common, and what any of them sees.
+    const int common_lo = __reduce_max_sync(0xffffffffu, max(rows.row_lo[0], rows.row_lo[1])), common_hi = __reduce_min_sync(0xffffffffu, min(rows.row_hi[0], rows.row_hi[1]));
+    const int any_lo = __reduce_min_sync(0xffffffffu, min(rows.row_lo[0], rows.row_lo[1])), any_hi = __reduce_max_sync(0xffffffffu, max(rows.row_hi[0], rows.row_hi[1]));
+    asm volatile("bar.sync 1, 128;" ::: "memory");   // the scales are there
+
+    bool ok = true;
+    for (int t = 0; t < tiles; ++t) {
+        const int slot = t % S::kStages;
+        if (ok) ok = mbar_wait_warp(full(slot), (t / S::kStages) & 1, 702);
+        if (!ok) break;
+        const uint8_t* k_tile = smem + slot * (2 * S::kTile);
+        const uint8_t* v_tile = k_tile + S::kTile;
+#pragma unroll 1
+        for (int at = group * kOwn; at < (group + 1) * kOwn; at += kStep) {
+            const int key0 = (tile_first + t) * S::kKeys + at, run = t * S::kRuns + (at >> 4);
+            if (key0 >= any_hi || key0 + kStep <= any_lo) continue;
+            bool special = key0 < common_lo || key0 + kStep > common_hi;
+#pragma unroll
+            for (int r = 0; r < kStep / 16; ++r) special = special || k_scales[run + r] < 0.0f || static_cast<uint32_t>(v_scales[run + r]) > 254u;
+            if (special) rows.template step<true, kStep>(k_tile, v_tile, k_scales + run, v_scales + run, at, key0, lo, hi, a.seq_q > 1);
+            else rows.template step<false, kStep>(k_tile, v_tile, k_scales + run, v_scales + run, at, key0, lo, hi, false);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty(slot));
+    }
+    ok = ok && g_device_status == 0;
 
     // The warps of an M tile meet: (largest score, sum, O) triples by shared memory, in the order of the fragments, so that each bank
     // is met once. Warp g then has rows and columns of its own: fragment values c with c * groups / 4 == g.
-    copies_wait<0>();
+    const float absolute = rows.unit == kNoUnit ? 1.0f : decode_e8m0(static_cast<uint32_t>(rows.unit));
+#pragma unroll
+    for (int j = 0; j < kWide; ++j)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) rows.o[j][c] *= absolute;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-        sum[half] += __shfl_xor_sync(0xffffffffu, sum[half], 1);
-        sum[half] += __shfl_xor_sync(0xffffffffu, sum[half], 2);
+        rows.sum[half] += __shfl_xor_sync(0xffffffffu, rows.sum[half], 1);
+        rows.sum[half] += __shfl_xor_sync(0xffffffffu, rows.sum[half], 2);
     }
-    float top[2] = {largest[0], largest[1]}, total[2] = {sum[0], sum[1]};
+    float top[2] = {rows.largest[0], rows.largest[1]}, total[2] = {rows.sum[0], rows.sum[1]};
     if constexpr (kGroups > 1) {
-        __syncthreads();
-        float* fragments = reinterpret_cast<float*>(smem);                          // [warp][4 * kWide][32]
-        float* meeting = reinterpret_cast<float*>(smem + S::kOffsets);              // [warp][half][32][2]
+        asm volatile("bar.sync 1, 128;" ::: "memory");   // (every tile has come and been read)
+        float* fragments = reinterpret_cast<float*>(smem);                 // [warp][4 * kWide][32]
+        float* meeting = reinterpret_cast<float*>(smem + S::kKScales);     // [warp][half][32][2]
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            meeting[((warp * 2 + half) * 32 + lane) * 2] = largest[half];
-            meeting[((warp * 2 + half) * 32 + lane) * 2 + 1] = sum[half];
+            meeting[((warp * 2 + half) * 32 + lane) * 2] = rows.largest[half];
+            meeting[((warp * 2 + half) * 32 + lane) * 2 + 1] = rows.sum[half];
         }
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
-            for (int j = 0; j < kWide; ++j) fragments[((warp * 4 + c) * kWide + j) * 32 + lane] = o[j][c];
-        __syncthreads();
+            for (int j = 0; j < kWide; ++j) fragments[((warp * 4 + c) * kWide + j) * 32 + lane] = rows.o[j][c];
+        asm volatile("bar.sync 1, 128;" ::: "memory");
         float weight[kGroups][2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
@@ -429,10 +500,11 @@ cache_sdpa_stream_kernel(CacheSdpaArgs a) {
                 float v = 0.0f;
 #pragma unroll
                 for (int g = 0; g < kGroups; ++g) v = fmaf(fragments[(((g * MT + mt) * 4 + c) * kWide + j) * 32 + lane], weight[g][c >> 1], v);
-                o[j][c] = v;
+                rows.o[j][c] = v;
             }
         }
     }
+    if (!ok) return;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         if (c * kGroups / 4 != group) continue;
@@ -446,7 +518,7 @@ cache_sdpa_stream_kernel(CacheSdpaArgs a) {
 #pragma unroll
             for (int j = 0; j < kWide; j += 2) {
                 const int channel = column * kReach + (j & (kReach - 1)) + (j / kReach) * 128;
-                *reinterpret_cast<float2*>(partial + channel) = make_float2(o[j][c], o[j + 1][c]);
+                *reinterpret_cast<float2*>(partial + channel) = make_float2(rows.o[j][c], rows.o[j + 1][c]);
             }
             if (first_of_row) *reinterpret_cast<float2*>(partial + D) = make_float2(top[half], total[half]);
         } else {
@@ -456,7 +528,7 @@ cache_sdpa_stream_kernel(CacheSdpaArgs a) {
             for (int j0 = 0; j0 < kWide; j0 += kReach) {
                 float v[kReach];
 #pragma unroll
-                for (int j = 0; j < kReach; ++j) v[j] = none ? 0.0f : o[j0 + j][c] * inverse;
+                for (int j = 0; j < kReach; ++j) v[j] = none ? 0.0f : rows.o[j0 + j][c] * inverse;
                 store_values(a, batch * a.o_stride[0] + head_of[half] * a.o_stride[1] + token_of[half] * a.o_stride[2] + column * kReach + (j0 / kReach) * 128, v);
             }
             if (first_of_row && a.stats)
@@ -466,60 +538,61 @@ cache_sdpa_stream_kernel(CacheSdpaArgs a) {
     }
 }
 
-// One warp a row: the chunks that hold keys of it, all their maxima and sums first, a chunk a lane, then their values.
+// A CTA a row, a thread a channel. Latency-bound: maxima and sums of the first 32 chunks, a chunk a lane in every warp, and the values of
+// the first eight are on their way before the lengths say which of them the row has.
 template <int D>
-__global__ void __launch_bounds__(128)
-cache_sdpa_merge_kernel(CacheSdpaArgs a, int64_t all_rows) {
-    constexpr int kOwn = D / 32;   // channels a lane
-    chain_begin();
+__global__ void __launch_bounds__(D)
+cache_sdpa_merge_kernel(const __grid_constant__ CacheSdpaArgs a) {
+    constexpr int kAhead = 8;
     const int lane = threadIdx.x & 31;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-    if (row >= all_rows) return;
-    const int64_t list = row / a.rows, batch = list / a.heads_kv;
+    const int64_t row = blockIdx.x, list = row / a.rows, batch = list / a.heads_kv;
     const int in_list = static_cast<int>(row - list * a.rows), token = in_list / a.group;
     const int head = static_cast<int>(list - batch * a.heads_kv) * a.group + (in_list - token * a.group);
+    const float* base = a.partial + row * a.chunks * (D + 2);
+    chain_begin();
+    float ahead[kAhead];
+#pragma unroll
+    for (int c = 0; c < kAhead; ++c) ahead[c] = c < a.chunks ? base[c * (D + 2) + threadIdx.x] : 0.0f;
+    float2 first_pair = lane < a.chunks ? *reinterpret_cast<const float2*>(base + lane * (D + 2) + D) : make_float2(-INFINITY, 0.0f);
     const SequenceWindow window = sequence_window(a, batch);
     int lo = 0, hi = 0;
     if (token < window.len_q) window_of_tokens(a, window, token, token, lo, hi);
     const int keys = a.tiles_per_cta * a.tile_keys;
     const int first = lo / keys, end = hi > lo ? (hi + keys - 1) / keys : first;
-    const float* base = a.partial + row * a.chunks * (D + 2);
+    auto pair_of = [&](int c) {   // (largest score, sum); a chunk without keys of the row was perhaps not written
+        if (c < first || c >= end) return make_float2(-INFINITY, 0.0f);
+        return c == lane ? first_pair : *reinterpret_cast<const float2*>(base + c * (D + 2) + D);
+    };
     float top = -INFINITY;
-    for (int c = first + lane; c < end; c += 32) top = fmaxf(top, base[c * (D + 2) + D]);
+    for (int c = lane; c < end; c += 32) top = fmaxf(top, pair_of(c).x);
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-    float total = 0.0f, value[kOwn];
-#pragma unroll
-    for (int i = 0; i < kOwn; ++i) value[i] = 0.0f;
-    for (int c0 = first; c0 < end; c0 += 32) {
-        float weight = 0.0f, part = 0.0f;
-        if (c0 + lane < end) {
-            const float m = base[(c0 + lane) * (D + 2) + D];
-            weight = m == -INFINITY ? 1.0f : exp2_of(m - top);   // (no score above -inf: its values are zeros, or NaNs that are to be seen)
-            part = base[(c0 + lane) * (D + 2) + D + 1] * weight;
-        }
+    float total = 0.0f, value = 0.0f;
+    for (int c0 = 0; c0 < end; c0 += 32) {
+        const float2 pair = pair_of(c0 + lane);
+        const float weight = pair.x == -INFINITY ? 1.0f : exp2_of(pair.x - top);   // (no score above -inf: its values are zeros, or NaNs that are to be seen)
+        float part = pair.y * weight;
 #pragma unroll
         for (int s = 16; s > 0; s >>= 1) part += __shfl_xor_sync(0xffffffffu, part, s);
         total += part;
-        const int count = min(32, end - c0);
-#pragma unroll 4
-        for (int c = 0; c < count; ++c) {
-            const float w = __shfl_sync(0xffffffffu, weight, c);
-            const float2* from = reinterpret_cast<const float2*>(base + (c0 + c) * (D + 2) + lane * kOwn);
 #pragma unroll
-            for (int i = 0; i < kOwn / 2; ++i) {
-                const float2 v = from[i];
-                value[2 * i] = fmaf(v.x, w, value[2 * i]);
-                value[2 * i + 1] = fmaf(v.y, w, value[2 * i + 1]);
+        for (int c = 0; c < 32; c += kAhead) {
+            if (c0 + c >= end) break;
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const float w = __shfl_sync(0xffffffffu, weight, c + k);
+                if (c0 + c + k >= first && c0 + c + k < end) value = fmaf(ahead[k], w, value);
+            }
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const int next = c0 + c + kAhead + k;
+                if (next >= first && next < end) ahead[k] = base[next * (D + 2) + threadIdx.x];
             }
         }
     }
     const bool none = total == 0.0f;
-    const float inverse = 1.0f / total;
-    const int64_t at = batch * a.o_stride[0] + head * a.o_stride[1] + token * a.o_stride[2] + lane * kOwn;
-#pragma unroll
-    for (int i = 0; i < kOwn; ++i) store_from_f32(a.o, a.o_type, at + i, none ? 0.0f : value[i] * inverse);
-    if (lane == 0 && a.stats) a.stats[batch * a.stats_stride[0] + head * a.stats_stride[1] + token * a.stats_stride[2]] = none ? -INFINITY : top * kLn2 + logf(total * 0x1p-15f);
+    store_from_f32(a.o, a.o_type, batch * a.o_stride[0] + head * a.o_stride[1] + token * a.o_stride[2] + threadIdx.x, none ? 0.0f : value / total);
+    if (threadIdx.x == 0 && a.stats) a.stats[batch * a.stats_stride[0] + head * a.stats_stride[1] + token * a.stats_stride[2]] = none ? -INFINITY : top * kLn2 + logf(total * 0x1p-15f);
 }
 
 struct StreamPlan {
@@ -535,10 +608,10 @@ StreamPlan plan_stream(const dfgpu_cache_sdpa_params& p) {
     plan.row_blocks = static_cast<int>((plan.rows + plan.row_tiles * 16 - 1) / (plan.row_tiles * 16));
     plan.tile_keys = d == 256 ? 64 : 128;
     const int64_t tiles = (p.s_kv + plan.tile_keys - 1) / plan.tile_keys, lists = p.q.dim[0] * p.k.dim[1] * plan.row_blocks;
-    // Long runs of tiles save prologues and partial results, short ones give a small batch more CTAs: as long as there are three for
-    // every two SMs' worth (148: a function of the shape alone, as the scratch is).
-    int per_cta = kMostTiles;
-    while (per_cta > 1 && lists * ((tiles + per_cta - 1) / per_cta) < 4 * 148) per_cta /= 2;
+    // Long runs of tiles save prologues and partial results (the more the more rows there are), short ones give a small batch more
+    // CTAs: as long as there are three for every two SMs (148: a function of the shape alone, as the scratch is).
+    int per_cta = 8 * plan.row_tiles;
+    while (per_cta > 1 && 2 * lists * ((tiles + per_cta - 1) / per_cta) < 3 * 148) per_cta /= 2;
     plan.tiles_per_cta = per_cta;
     plan.chunks = static_cast<int>((tiles + per_cta - 1) / per_cta);
     plan.scratch = plan.chunks > 1 ? p.q.dim[0] * p.k.dim[1] * plan.rows * plan.chunks * (d + 2) * 4 : 0;
@@ -552,7 +625,7 @@ int check_side(const dfgpu_cache_sdpa_params& p, const dfgpu_tensor& cache, cons
     if (cache.dim[1] != p.k.dim[1] || cache.dim[2] != p.k.dim[2]) return fail(kInvalidShape, "CACHE_SDPA: the containers differ in heads or tokens a page");
     if (cache.stride[3] != 1) return fail(kInvalidLayout, "CACHE_SDPA: the head dimension of a container must have unit stride");
     for (int i = 0; i < 3; ++i)
-        if (cache.dim[i] > 1 && cache.stride[i] % 16 != 0) return fail(kInvalidLayout, "CACHE_SDPA: the strides of the container of %s must be multiples of 16", name);
+        if (cache.dim[i] > 1 && (cache.stride[i] % 16 != 0 || cache.stride[i] >= (1ll << 40))) return fail(kInvalidLayout, "CACHE_SDPA: the strides of the container of %s must be multiples of 16", name);
     if (!valid_tensor(scale) || scale.rank != 4 || scale.dtype != DFGPU_E8M0 || scale.reorder != DFGPU_REORDER_NONE || scale.dim[0] != cache.dim[0] || scale.dim[1] != cache.dim[1] ||
         scale.dim[3] != 1 || cache.dim[2] % scale.dim[2] != 0 || scale.dim[2] != p.k_scale.dim[2])
         return fail(kInvalidShape, "CACHE_SDPA: the scales of %s must be FP8_E8M0 [pages, Hk, T / t, 1], t a divisor of T and one for K and V", name);
@@ -589,24 +662,38 @@ int check_cache_sdpa(const dfgpu_cache_sdpa_params& p, int& kernel) {
         return fail(kInvalidShape, "CACHE_SDPA: Stats must be FLOAT [B, Hq, Sq, 1]");
     if (!std::isfinite(p.attn_scale)) return fail(kInvalidValue, "CACHE_SDPA: the attention scale must be finite");
     const StreamPlan plan = plan_stream(p);
-    if (p.q.dim[0] > 65535 || p.k.dim[1] * plan.row_blocks > 65535 || p.q.dim[2] >= (1ll << 30) || plan.rows >= (1ll << 31)) return fail(kUnsupported, "CACHE_SDPA: too many sequences, heads or query rows");
+    if (p.q.dim[0] > 65535 || p.k.dim[1] * plan.row_blocks > 65535 || p.q.dim[2] >= (1ll << 30) || p.q.dim[0] * p.k.dim[1] * plan.rows >= (1ll << 31)) return fail(kUnsupported, "CACHE_SDPA: too many sequences, heads or query rows");
     if (p.kernel < DFGPU_CACHE_SDPA_AUTO || p.kernel > DFGPU_CACHE_SDPA_STREAM) return fail(kInvalidArgument, "CACHE_SDPA: unknown kernel id %d", p.kernel);
     kernel = DFGPU_CACHE_SDPA_STREAM;
     return kOk;
 }
 
+// Codes as [pages, Hk, T, D] boxes of `box` tokens by 128 or 64 bytes.
+int make_side_map(CUtensorMap* map, const dfgpu_tensor& cache, const void* base, int box_rows) {
+    EncodeTiled encode = encode_tiled();
+    if (!encode) return fail(kExecutionFailed, "CACHE_SDPA: cuTensorMapEncodeTiled is unavailable");
+    const bool narrow = cache.dim[3] == 64;
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(cache.dim[3]), static_cast<cuuint64_t>(cache.dim[2]), static_cast<cuuint64_t>(cache.dim[1]), static_cast<cuuint64_t>(cache.dim[0])};
+    cuuint64_t strides[3];
+    for (int i = 0; i < 3; ++i) strides[i] = static_cast<cuuint64_t>(cache.dim[2 - i] > 1 ? cache.stride[2 - i] : cache.dim[3]);
+    const cuuint32_t box[4] = {narrow ? 64u : 128u, static_cast<cuuint32_t>(box_rows), 1, 1}, steps[4] = {1, 1, 1, 1};
+    const CUresult result = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                   narrow ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (result != CUDA_SUCCESS) return fail(kExecutionFailed, "CACHE_SDPA: tensor map encode failed (CUresult %d)", static_cast<int>(result));
+    return kOk;
+}
+
 template <typename T, int D>
-int launch_stream(const CacheSdpaArgs& a, const StreamPlan& plan, dim3 grid, cudaStream_t stream) {
+int launch_stream(const CUtensorMap& map_k, const CUtensorMap& map_v, const CacheSdpaArgs& a, const StreamPlan& plan, dim3 grid, cudaStream_t stream) {
     auto run = [&](auto kernel) -> int {
-        const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kTotal);
-        if (error != cudaSuccess) return fail(kExecutionFailed, "CACHE_SDPA: cannot reserve %d bytes of shared memory: %s", Shape<D>::kTotal, cudaGetErrorString(error));
-        launch_chained(kernel, grid, dim3(kThreads), Shape<D>::kTotal, stream, a);
+        const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kDynamic);
+        if (error != cudaSuccess) return fail(kExecutionFailed, "CACHE_SDPA: cannot reserve %d bytes of shared memory: %s", Shape<D>::kDynamic, cudaGetErrorString(error));
+        launch_chained(kernel, grid, dim3(kThreads), Shape<D>::kDynamic, stream, map_k, map_v, a);
         return check_launch("CACHE_SDPA");
     };
     const int status = plan.row_tiles == 1 ? run(cache_sdpa_stream_kernel<T, D, 1>) : plan.row_tiles == 2 ? run(cache_sdpa_stream_kernel<T, D, 2>) : run(cache_sdpa_stream_kernel<T, D, 4>);
     if (status || plan.chunks == 1) return status;
-    const int64_t all_rows = static_cast<int64_t>(grid.z) * a.heads_kv * a.rows;
-    launch_chained(cache_sdpa_merge_kernel<D>, dim3(static_cast<unsigned>((all_rows + 3) / 4)), dim3(128), 0, stream, a, all_rows);
+    launch_chained(cache_sdpa_merge_kernel<D>, dim3(static_cast<unsigned>(static_cast<int64_t>(grid.z) * a.heads_kv * a.rows)), dim3(D), 0, stream, a);
     return check_launch("CACHE_SDPA merge");
 }
 
@@ -694,12 +781,22 @@ extern "C" int dfgpu_cache_sdpa(const dfgpu_cache_sdpa_params* p, void* const* t
     a.tiles_per_cta = plan.tiles_per_cta;
     a.tile_keys = plan.tile_keys;
     a.partial = static_cast<float*>(scratch);
+    // TMA boxes: the most tokens up to 64 that divide a page's
+    a.box = a.page % 64 == 0 ? 64 : a.page % 32 == 0 ? 32 : 16;
+    CUtensorMap map_k, map_v;
+    int made = make_side_map(&map_k, p->k, tensors[1], a.box);
+    if (!made) made = make_side_map(&map_v, p->v, tensors[2], a.box);
+    if (made) return made;
     const dim3 grid(static_cast<unsigned>(plan.chunks), static_cast<unsigned>(a.heads_kv * plan.row_blocks), static_cast<unsigned>(p->q.dim[0]));
     cudaStream_t on = as_stream(stream);
     const bool half = p->q.dtype == DFGPU_F16;
     switch (p->q.dim[3]) {
-        case 64: return half ? launch_stream<__half, 64>(a, plan, grid, on) : launch_stream<__nv_bfloat16, 64>(a, plan, grid, on);
-        case 128: return half ? launch_stream<__half, 128>(a, plan, grid, on) : launch_stream<__nv_bfloat16, 128>(a, plan, grid, on);
-        default: return half ? launch_stream<__half, 256>(a, plan, grid, on) : launch_stream<__nv_bfloat16, 256>(a, plan, grid, on);
+        case 64: return half ? launch_stream<__half, 64>(map_k, map_v, a, plan, grid, on) : launch_stream<__nv_bfloat16, 64>(map_k, map_v, a, plan, grid, on);
+        case 128: return half ? launch_stream<__half, 128>(map_k, map_v, a, plan, grid, on) : launch_stream<__nv_bfloat16, 128>(map_k, map_v, a, plan, grid, on);
+        default: return half ? launch_stream<__half, 256>(map_k, map_v, a, plan, grid, on) : launch_stream<__nv_bfloat16, 256>(map_k, map_v, a, plan, grid, on);
     }
 }
+
+namespace dfgpu {
+int cache_sdpa_device_status(int* status) { return read_and_clear_device_status(status); }
+}  // namespace dfgpu

@@ -26,7 +26,7 @@ struct CacheSdpaArgs {
     int64_t left, right;
     int32_t o_type, o_vector;
     int32_t heads_kv, group, rows, seq_q, s_kv;   // rows: (token, head of the group) pairs of a KV head
-    int32_t page;
+    int32_t page, box;                            // tokens a page, and of one TMA copy
     FastDivisor by_page, by_tokens;               // of numbers of 16 tokens
     int32_t has_left, has_right, bottom_right;
     int32_t chunks, tiles_per_cta, tile_keys;

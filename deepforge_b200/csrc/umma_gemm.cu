@@ -1128,6 +1128,10 @@ extern "C" int dfgpu_device_status(int* status) {
     code = sdpa_device_status(&prefix);
     if (code) return code;
     if (!decode) decode = prefix;
+    int cache = 0;
+    code = cache_sdpa_device_status(&cache);
+    if (code) return code;
+    if (!decode) decode = cache;
     *status = gemm ? gemm : (sdpa ? sdpa : decode);
     return kOk;
 }
