@@ -1,11 +1,12 @@
 // Attention over a paged cache of E4M3 codes with E8M0 scales: the streaming form, for few query rows a KV head (single tokens,
 // drafted tokens) and for every type and head dimension.
 //
-// Bound by HBM: each held code is read once for all query heads of its KV head. A row of the products is a (token, head) pair,
-// 16 rows an M tile. Codes are exact in f16 (448 to 2^-9), so K and V go from shared memory through one convert for two codes
-// straight into the register operands of mma.sync.m16n8k16: a tcgen05 product wants its operands in shared memory, and writing the
-// converted tile there and reading it back is 144 bytes of shared-memory traffic a clock at HBM speed, where the port moves 128.
-// With 16 rows the tensor cores have 16 multiply-adds for each code, 384 a clock and SM at HBM speed.
+// Bound by HBM: each held code is read once for all query heads of its KV head. A row of the products is a (token, head) pair.
+// Codes are exact in f16 (448 to 2^-9), so K and V go from shared memory through one convert for two codes straight into the
+// register operands of mma.sync.m16n8k16: a tcgen05 product wants its operands in shared memory, and writing the converted tile there
+// and reading it back is 144 bytes of shared-memory traffic a clock at HBM speed, where the port moves 128. Both products are taken
+// transposed, S^T = K Q^T and O^T = V^T P^T, so that rows come in eights (most groups of query heads are no larger) and 16 keys or
+// channels share an instruction; P^T turns from the first one's result into the second one's operand by movmatrix.
 //   * Q is not rounded: each row is scaled by a power of two that puts its largest magnitude at 2^14, and is exact in f16 down to
 //     2^-38 of that (below, within 2^-39 of it).
 //   * 16 consecutive keys share a page and a scale (both are multiples of 16 tokens). The K scale multiplies their scores. O is
@@ -13,12 +14,12 @@
 //     to 1, and else the unit moves and O with it (exactly, as far as scales within 2^80 of one another go).
 //   * Probabilities are rounded to f16 as p * 2^15: 11 bits down to 2^-29 (2^-19 beside a V scale of 2^-10 units), where p is measured
 //     against the largest score so far.
-// Channels and keys may go to any k index of a product as long as both operands agree; the ones taken here give each thread 16-byte
-// reads without bank conflicts: of K 32 consecutive channels of a key, of V 16 consecutive channels of four keys, and of O 32
+// Channels and keys may go to any index of a product as long as both operands agree; the ones taken here give each thread 16-byte
+// reads without bank conflicts: of K 32 consecutive channels of a key, of V 16 consecutive channels of four keys, and of O 16
 // consecutive channels of a row.
-// CTA: one (sequence, KV head, block of rows), a run of key tiles; a fifth warp brings the tiles by TMA (whole pages or runs of them,
-// swizzled) into a ring, four share each tile's keys out between them, or its rows where there are more than 16, or
-// both. Two CTAs fit on an SM. More than one run of key tiles a sequence leaves partial results that a second kernel merges.
+// CTA: one (sequence, KV head, block of rows), a run of units of 32 keys; a fifth warp brings them by TMA (pages or parts of them,
+// swizzled) into a ring, four take them in turn, or in pairs or all of them with rows of their own where there are more than 16.
+// Single tokens leave three CTAs on an SM. More than one run of units a sequence leaves partial results that a second kernel merges.
 #include <algorithm>
 #include <cmath>
 
@@ -30,31 +31,31 @@ namespace dfgpu {
 namespace {
 
 constexpr int kWarps = 4, kConsumers = 128, kThreads = 160;
-constexpr int kMostTiles = 32;     // key tiles a CTA
+constexpr int kUnit = 32;          // keys that a warp takes at a time
+constexpr int kMostUnits = 128;    // of a CTA
 constexpr float kUp = 15.0f;       // probabilities are held as p * 2^15
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kNoUnit = -100000;   // O is zero and has no unit yet
 constexpr int kNaN = 0x7fc00000;
 
-template <int D>
+// EIGHTS: eights of rows that a warp takes.
+template <int D, int EIGHTS>
 struct Shape {
-    static constexpr int kKeys = D == 256 ? 64 : 128;     // keys a tile
-    static constexpr int kRuns = kKeys / 16;
-    static constexpr int kTile = kKeys * D;               // bytes of a K or V tile
-    static constexpr int kCtas = D == 256 ? 1 : 2;        // on an SM: a D of 256 takes 255 registers a thread
-    static constexpr int kStages = D == 64 ? 4 : 3 * (3 - kCtas);
-    static constexpr int kRing = kStages * 2 * kTile;
-    static constexpr int kKScales = kRing;                                    // [runs] f32, -1: the page's rows read as zeros
-    static constexpr int kVScales = kKScales + kMostTiles * kRuns * 4;        // [runs] the code, -1 likewise
-    static constexpr int kBarriers = kVScales + kMostTiles * kRuns * 4;       // full[stages], empty[stages]
-    static constexpr int kTotal = kBarriers + 2 * kStages * 8;
+    static constexpr int kCtas = D == 256 ? (EIGHTS == 1 ? 2 : 1) : EIGHTS == 1 ? 3 : 2;   // on an SM
+    static constexpr int kSide = kUnit * D;                                                // bytes of a unit's K or V
+    static constexpr int kSlots = (kCtas == 3 ? 64 : kCtas == 2 ? 96 : 192) * 1024 / (2 * kSide);
+    static constexpr int kRing = kSlots * 2 * kSide;
+    static constexpr int kKScales = kRing;                                    // [runs of 16 keys] f32, -1: the page's rows read as zeros
+    static constexpr int kVScales = kKScales + kMostUnits * 2 * 4;            // [runs] the code, -1 likewise
+    static constexpr int kBarriers = kVScales + kMostUnits * 2 * 4;           // full[slots], empty[slots]
+    static constexpr int kTotal = kBarriers + 2 * kSlots * 8;
     static constexpr int kDynamic = kTotal + 1024;
 };
 
-// Byte offset of a 16-byte chunk of a tile's row, as TMA lays rows of 128 or 64 bytes out (a D of 256: two halves): the reads above meet each bank once.
+// Byte offset of a 16-byte chunk of a unit's row, as TMA lays rows of 128 or 64 bytes out (a D of 256: two halves): the reads above meet each bank once.
 template <int D>
 __device__ __forceinline__ uint32_t at_chunk(int row, int chunk) {
-    return D == 64 ? row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4) : (chunk >> 3) * (Shape<D>::kKeys * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
+    return D == 64 ? row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4) : (chunk >> 3) * (kUnit * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
 }
 
 __device__ __forceinline__ void four_codes(uint32_t codes, uint32_t& low, uint32_t& high) {   // as f16
@@ -70,13 +71,18 @@ __device__ __forceinline__ float exp2_of(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ void multiply(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+__device__ __forceinline__ void multiply(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, const uint32_t (&b)[2]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]));
 }
-__device__ __forceinline__ void multiply_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
-                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+__device__ __forceinline__ void multiply_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, const uint32_t (&b)[2]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b[0]), "r"(b[1]), "f"(0.0f));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t pair) {   // of an 8 x 8 matrix of f16 over the warp
+    uint32_t v;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(v) : "r"(pair));
+    return v;
 }
 __device__ __forceinline__ uint32_t times(uint32_t pair, uint32_t factor) {
     uint32_t v;
@@ -89,159 +95,166 @@ __device__ __forceinline__ float power_of_two(int n) { return __uint_as_float(st
 __device__ __forceinline__ float value_of(__half v) { return __half2float(v); }
 __device__ __forceinline__ float value_of(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// `count` (8 or 16) neighbouring values of a row of O.
-template <int COUNT>
-__device__ __forceinline__ void store_values(const CacheSdpaArgs& a, int64_t at, const float (&v)[COUNT]) {
+// Two neighbouring values of a row of O.
+__device__ __forceinline__ void store_pair(const CacheSdpaArgs& a, int64_t at, float first, float second) {
     if (a.o_vector) {
-        if (a.o_type == DFGPU_F32) {
-#pragma unroll
-            for (int i = 0; i < COUNT; i += 4) *reinterpret_cast<float4*>(static_cast<float*>(a.o) + at + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-        } else {
-            uint32_t words[COUNT / 2];
-#pragma unroll
-            for (int i = 0; i < COUNT; i += 2)
-                words[i / 2] = a.o_type == DFGPU_F16 ? two_halves(v[i], v[i + 1]) : static_cast<uint32_t>(f32_to_bf16_bits(v[i])) | static_cast<uint32_t>(f32_to_bf16_bits(v[i + 1])) << 16;
-#pragma unroll
-            for (int i = 0; i < COUNT / 2; i += 4)
-                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.o) + at + 2 * i) = make_uint4(words[i], words[i + 1], words[i + 2], words[i + 3]);
-        }
+        if (a.o_type == DFGPU_F32) *reinterpret_cast<float2*>(static_cast<float*>(a.o) + at) = make_float2(first, second);
+        else *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.o) + at) =
+                 a.o_type == DFGPU_F16 ? two_halves(first, second) : static_cast<uint32_t>(f32_to_bf16_bits(first)) | static_cast<uint32_t>(f32_to_bf16_bits(second)) << 16;
         return;
     }
-#pragma unroll
-    for (int i = 0; i < COUNT; ++i) store_from_f32(a.o, a.o_type, at + i, v[i]);
+    store_from_f32(a.o, a.o_type, at, first);
+    store_from_f32(a.o, a.o_type, at + 1, second);
 }
 
-// The page of a tile's key in a side's table, -1 where there is none.
+// The page of a slot in a side's table, -1 where there is none.
 __device__ __forceinline__ int page_of(const CacheSdpaArgs& a, const CacheSide& s, int64_t batch, int slot) {
     if (slot >= s.table_len) return -1;
     const int page = s.table[batch * s.table_batch + slot * s.table_slot];
     return page >= 0 && page < s.pages ? page : -1;
 }
 
-// 16 rows of one M tile against the codes of K and V that its warp takes.
-template <int D>
+// EIGHTS * 8 rows against the codes of K and V that their warp takes. Thread (eighth, quad) = (lane / 4, lane % 4) has scores of keys
+// eighth and eighth + 8 of each 16, and O's channels channel_of(j) and the next one, both for rows 2 quad and 2 quad + 1 of each eight.
+template <int D, int EIGHTS>
 struct RowTile {
-    static constexpr int kDeep = D / 16;                     // products along the channels
-    static constexpr int kWide = D / 8;                      // products along the channels of V: thread value j
-    static constexpr int kReach = D == 64 ? 8 : 16;          // consecutive channels that a thread reads of a V row
-    uint32_t q[kDeep][4];
-    float factor[2];            // of a score: 1 / the row's power of two, attention scale, log2(e)
-    int row_lo[2], row_hi[2];   // keys that the thread's two rows see
-    float largest[2], sum[2];
-    float o[kWide][4];
+    static constexpr int kDeep = D / 16;                     // products along the channels of K
+    static constexpr int kWide = D / 16;                     // pairs of channels of V
+    uint32_t q[kDeep][EIGHTS][2];
+    float factor[EIGHTS][2];            // of a score: 1 / the row's power of two, attention scale, log2(e)
+    int row_lo[EIGHTS][2], row_hi[EIGHTS][2];   // keys that a row sees
+    float largest[EIGHTS][2], sum[EIGHTS][2];
+    float o[kWide][EIGHTS][4];          // (channel, row), (channel, next row), (next channel, row), (next channel, next row)
     int unit;
 
-    // KEYS keys from row `row` of a tile, key0 of the sequence. SPECIAL: some row does not see all of them, or a page or scale is none.
-    template <bool SPECIAL, int KEYS>
-    __device__ __forceinline__ void step(const uint8_t* k_tile, const uint8_t* v_tile, const float* k_scales, const int* v_scales, int row, int key0, int lo, int hi, bool mixed) {
+    __device__ static __forceinline__ int channel_of(int j, int eighth) { return D == 64 ? eighth * 8 + 2 * j : (j >> 3) * 128 + eighth * 16 + 2 * (j & 7); }
+
+    // A unit of keys from key0 of the sequence on. SPECIAL: some row does not see all of them, or a page or scale is none.
+    template <bool SPECIAL>
+    __device__ __forceinline__ void step(const uint8_t* k_unit, const uint8_t* v_unit, const float* k_scales, const int* v_scales, int key0, int lo, int hi, bool mixed) {
         const int lane = threadIdx.x & 31, quad = lane & 3, eighth = lane >> 2;
-        constexpr int kRuns = KEYS / 16;
-        float s[KEYS / 8][4];   // scores: 8 keys a product, keys along its columns
+        float s[2][EIGHTS][4];   // neighbouring products add to different ones
 #pragma unroll
-        for (int n = 0; n < KEYS / 8; ++n) {
+        for (int u = 0; u < kDeep / 4; ++u) {
+            uint32_t w[4][4];    // of keys eighth, + 8, + 16, + 24
 #pragma unroll
-            for (int u = 0; u < kDeep / 4; ++u) {
-                const uint4 raw = read_16(k_tile + at_chunk<D>(row + n * 8 + eighth, D == 64 ? quad : quad * 2 + (u & 1) + (u >> 1) * 8));
-                const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t b0, b1;
-                    four_codes(w[i], b0, b1);
-                    if (u + i == 0) multiply_first(s[n], q[0], b0, b1);
-                    else multiply(s[n], q[u * 4 + i], b0, b1);
-                }
+            for (int r = 0; r < 4; ++r) {
+                const uint4 raw = read_16(k_unit + at_chunk<D>(r * 8 + eighth, D == 64 ? quad : quad * 2 + (u & 1) + (u >> 1) * 8));
+                w[r][0] = raw.x, w[r][1] = raw.y, w[r][2] = raw.z, w[r][3] = raw.w;
             }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    uint32_t a0, a1, a2, a3;
+                    four_codes(w[2 * r][i], a0, a2);
+                    four_codes(w[2 * r + 1][i], a1, a3);
+#pragma unroll
+                    for (int n = 0; n < EIGHTS; ++n) {
+                        if (u + i == 0) multiply_first(s[r][n], a0, a1, a2, a3, q[0][n]);
+                        else multiply(s[r][n], a0, a1, a2, a3, q[u * 4 + i][n]);
+                    }
+                }
         }
         bool above = false;
 #pragma unroll
-        for (int n = 0; n < KEYS / 8; ++n) {
-            const float k_scale = k_scales[n >> 1];
-            const float f0 = factor[0] * k_scale, f1 = factor[1] * k_scale;
-            s[n][0] *= f0, s[n][1] *= f0, s[n][2] *= f1, s[n][3] *= f1;
-            if (SPECIAL) {
+        for (int r = 0; r < 2; ++r) {
+            const float k_scale = k_scales[r];
+#pragma unroll
+            for (int n = 0; n < EIGHTS; ++n)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    const int key = key0 + n * 8 + quad * 2 + (c & 1);
-                    if (k_scale < 0.0f) s[n][c] = 0.0f;
-                    if (static_cast<uint32_t>(key - row_lo[c >> 1]) >= static_cast<uint32_t>(row_hi[c >> 1] - row_lo[c >> 1])) s[n][c] = -INFINITY;
+                    float& x = s[r][n][c];
+                    x *= factor[n][c & 1] * k_scale;
+                    if (SPECIAL) {
+                        const int key = key0 + r * 16 + eighth + (c >> 1) * 8;
+                        if (k_scale < 0.0f) x = 0.0f;
+                        if (static_cast<uint32_t>(key - row_lo[n][c & 1]) >= static_cast<uint32_t>(row_hi[n][c & 1] - row_lo[n][c & 1])) x = -INFINITY;
+                    }
+                    above = above || x > largest[n][c & 1];
                 }
+        }
+        if (__any_sync(0xffffffffu, above)) {   // a new largest score in some row (rare after the first units)
+#pragma unroll
+            for (int n = 0; n < EIGHTS; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float top = fmaxf(fmaxf(fmaxf(s[0][n][c], s[0][n][c + 2]), fmaxf(s[1][n][c], s[1][n][c + 2])), largest[n][c]);
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                    const float down = top == -INFINITY ? 1.0f : exp2_of(largest[n][c] - top);
+                    largest[n][c] = top;
+                    sum[n][c] *= down;
+#pragma unroll
+                    for (int j = 0; j < kWide; ++j) o[j][n][c] *= down, o[j][n][c + 2] *= down;
+                }
+        }
+        uint32_t p[2][EIGHTS][2];
+#pragma unroll
+        for (int n = 0; n < EIGHTS; ++n) {
+            const float from0 = largest[n][0] == -INFINITY ? 0.0f : kUp - largest[n][0], from1 = largest[n][1] == -INFINITY ? 0.0f : kUp - largest[n][1];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const float p0 = exp2_of(s[r][n][0] + from0), p1 = exp2_of(s[r][n][1] + from1), p2 = exp2_of(s[r][n][2] + from0), p3 = exp2_of(s[r][n][3] + from1);
+                sum[n][0] += p0 + p2;
+                sum[n][1] += p1 + p3;
+                p[r][n][0] = transposed(two_halves(p0, p1));
+                p[r][n][1] = transposed(two_halves(p2, p3));
             }
-            above = above || fmaxf(s[n][0], s[n][1]) > largest[0] || fmaxf(s[n][2], s[n][3]) > largest[1];
-        }
-        if (__any_sync(0xffffffffu, above)) {   // a new largest score in some row (rare after the first tiles)
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                float top = largest[half];
-#pragma unroll
-                for (int n = 0; n < KEYS / 8; ++n) top = fmaxf(top, fmaxf(s[n][2 * half], s[n][2 * half + 1]));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const float down = top == -INFINITY ? 1.0f : exp2_of(largest[half] - top);
-                largest[half] = top;
-                sum[half] *= down;
-#pragma unroll
-                for (int j = 0; j < kWide; ++j) o[j][2 * half] *= down, o[j][2 * half + 1] *= down;
-            }
-        }
-        const float from0 = largest[0] == -INFINITY ? 0.0f : kUp - largest[0], from1 = largest[1] == -INFINITY ? 0.0f : kUp - largest[1];
-        uint32_t p[kRuns][4];
-#pragma unroll
-        for (int n = 0; n < KEYS / 8; ++n) {
-            const float p0 = exp2_of(s[n][0] + from0), p1 = exp2_of(s[n][1] + from0), p2 = exp2_of(s[n][2] + from1), p3 = exp2_of(s[n][3] + from1);
-            sum[0] += p0 + p1;
-            sum[1] += p2 + p3;
-            p[n >> 1][(n & 1) * 2] = two_halves(p0, p1);
-            p[n >> 1][(n & 1) * 2 + 1] = two_halves(p2, p3);
         }
 #pragma unroll
-        for (int r = 0; r < kRuns; ++r) {
+        for (int r = 0; r < 2; ++r) {
             const int code = v_scales[r], apart = code - unit;   // (the same in all threads)
             if ((!SPECIAL || (code >= 0 && code != 255)) && apart != 0) {
                 if (apart < 0 && (apart >= -10 || apart < -80)) {
                     const uint32_t less = apart < -80 ? 0u : static_cast<uint32_t>(15 + apart) << 10, both = less | less << 16;
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) p[r][c] = times(p[r][c], both);
+                    for (int n = 0; n < EIGHTS; ++n) p[r][n][0] = times(p[r][n][0], both), p[r][n][1] = times(p[r][n][1], both);
                 } else {
                     const float to = unit == kNoUnit ? 1.0f : power_of_two(max(-apart, -126));
 #pragma unroll
                     for (int j = 0; j < kWide; ++j)
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) o[j][c] *= to;
+                        for (int n = 0; n < EIGHTS; ++n)
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) o[j][n][c] *= to;
                     unit = code;
                 }
             }
-            // V: thread value j of a run is channel 16 * eighth + j of keys 2 quad, 2 quad + 1 and those plus 8
-            uint32_t w[4][kWide / 4];
+            // V: channels from 16 * eighth on (8 * eighth for a D of 64) of keys 2 quad, 2 quad + 1 and those plus 8
+            uint32_t w[4][kWide / 2];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const int at = row + r * 16 + quad * 2 + (k & 1) + (k >> 1) * 8;
+                const int at = r * 16 + quad * 2 + (k & 1) + (k >> 1) * 8;
                 if constexpr (D == 64) {
-                    const uint2 raw = *reinterpret_cast<const uint2*>(v_tile + at_chunk<D>(at, eighth >> 1) + (eighth & 1) * 8);
+                    const uint2 raw = *reinterpret_cast<const uint2*>(v_unit + at_chunk<D>(at, eighth >> 1) + (eighth & 1) * 8);
                     w[k][0] = raw.x, w[k][1] = raw.y;
                 } else {
 #pragma unroll
-                    for (int u = 0; u < kWide / 16; ++u) {
-                        const uint4 raw = read_16(v_tile + at_chunk<D>(at, eighth + u * 8));
+                    for (int u = 0; u < kWide / 8; ++u) {
+                        const uint4 raw = read_16(v_unit + at_chunk<D>(at, eighth + u * 8));
                         w[k][u * 4] = raw.x, w[k][u * 4 + 1] = raw.y, w[k][u * 4 + 2] = raw.z, w[k][u * 4 + 3] = raw.w;
                     }
                 }
-                if (SPECIAL) {   // rows that nothing was brought to, or that no row sees: anything may lie there, NaN codes too
-                    const int key = key0 + r * 16 + quad * 2 + (k & 1) + (k >> 1) * 8;
+                if (SPECIAL) {   // rows that nothing was brought to, or that no query sees: anything may lie there, NaN codes too
+                    const int key = key0 + at;
                     if (code < 0 || key < lo || key >= hi) {
 #pragma unroll
-                        for (int i = 0; i < kWide / 4; ++i) w[k][i] = 0;
+                        for (int i = 0; i < kWide / 2; ++i) w[k][i] = 0;
                     }
                 }
             }
             if (SPECIAL) {
                 const int run0 = key0 + r * 16;
-                const bool sees[2] = {run0 < row_hi[0] && run0 + 16 > row_lo[0], run0 < row_hi[1] && run0 + 16 > row_lo[1]};
                 if (code == 255) {   // a scale that is a NaN: for the rows that see one of its keys
 #pragma unroll
-                    for (int j = 0; j < kWide; ++j)
+                    for (int n = 0; n < EIGHTS; ++n)
 #pragma unroll
                         for (int c = 0; c < 4; ++c)
-                            if (sees[c >> 1]) o[j][c] = __int_as_float(kNaN);
+                            if (run0 < row_hi[n][c & 1] && run0 + 16 > row_lo[n][c & 1]) {
+#pragma unroll
+                                for (int j = 0; j < kWide; ++j) o[j][n][c] = __int_as_float(kNaN);
+                            }
                 }
                 if (mixed) {
                     // A NaN code must reach the rows that see its key and no others, whose probability for it is 0: such codes become zeros in the
@@ -250,89 +263,90 @@ struct RowTile {
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
 #pragma unroll
-                        for (int i = 0; i < kWide / 4; ++i) {
+                        for (int i = 0; i < kWide / 2; ++i) {
                             const uint32_t found = ((w[k][i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
                             w[k][i] &= ~((found >> 7) * 0xffu);
                             nan |= found;
                         }
                     if (__any_sync(0xffffffffu, nan != 0)) {
 #pragma unroll 1
-                        for (int k = 0; k < 16; ++k) {
-                            const bool in0 = run0 + k >= row_lo[0] && run0 + k < row_hi[0], in1 = run0 + k >= row_lo[1] && run0 + k < row_hi[1];
+                        for (int k = 0; k < 16; ++k)
 #pragma unroll
                             for (int j = 0; j < kWide; ++j)
 #pragma unroll
-                                for (int c = 0; c < 2; ++c) {
-                                    const int channel = (quad * 2 + c) * kReach + (j & (kReach - 1)) + (j / kReach) * 128;
-                                    const uint8_t found = v_tile[at_chunk<D>(row + r * 16 + k, channel >> 4) + (channel & 15)];
-                                    if ((found & 0x7fu) == 0x7fu) {
-                                        if (in0) o[j][c] = __int_as_float(kNaN);
-                                        if (in1) o[j][2 + c] = __int_as_float(kNaN);
-                                    }
+                                for (int e = 0; e < 2; ++e) {
+                                    const int channel = channel_of(j, eighth) + e;
+                                    const uint8_t found = v_unit[at_chunk<D>(r * 16 + k, channel >> 4) + (channel & 15)];
+                                    if ((found & 0x7fu) != 0x7fu) continue;
+#pragma unroll
+                                    for (int n = 0; n < EIGHTS; ++n)
+#pragma unroll
+                                        for (int c = 0; c < 2; ++c)
+                                            if (run0 + k >= row_lo[n][c] && run0 + k < row_hi[n][c]) o[j][n][e * 2 + c] = __int_as_float(kNaN);
                                 }
-                        }
                     }
                 }
             }
 #pragma unroll
-            for (int i = 0; i < kWide / 4; ++i) {
-                uint32_t first[4], second[4];
-                four_codes(__byte_perm(w[0][i], w[1][i], 0x5140), first[0], first[1]);
-                four_codes(__byte_perm(w[0][i], w[1][i], 0x7362), first[2], first[3]);
-                four_codes(__byte_perm(w[2][i], w[3][i], 0x5140), second[0], second[1]);
-                four_codes(__byte_perm(w[2][i], w[3][i], 0x7362), second[2], second[3]);
+            for (int i = 0; i < kWide / 2; ++i) {   // four channels: two products
+                uint32_t near[4], far[4];
+                four_codes(__byte_perm(w[0][i], w[1][i], 0x5140), near[0], near[1]);
+                four_codes(__byte_perm(w[0][i], w[1][i], 0x7362), near[2], near[3]);
+                four_codes(__byte_perm(w[2][i], w[3][i], 0x5140), far[0], far[1]);
+                four_codes(__byte_perm(w[2][i], w[3][i], 0x7362), far[2], far[3]);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) multiply(o[i * 4 + e], p[r], first[e], second[e]);
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int n = 0; n < EIGHTS; ++n) multiply(o[i * 2 + e][n], near[2 * e], near[2 * e + 1], far[2 * e], far[2 * e + 1], p[r][n]);
             }
         }
     }
 };
 
-template <typename T, int D, int MT>
-__global__ void __launch_bounds__(kThreads, Shape<D>::kCtas)
+// ROW_WARPS: warps with rows of their own.
+template <typename T, int D, int EIGHTS, int ROW_WARPS>
+__global__ void __launch_bounds__(kThreads, Shape<D, EIGHTS>::kCtas)
 cache_sdpa_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CacheSdpaArgs a) {
-    using S = Shape<D>;
-    using Rows = RowTile<D>;
-    constexpr int kGroups = kWarps / MT;              // warps that share an M tile's keys
-    constexpr int kOwn = S::kKeys / kGroups;          // keys a warp and tile
-    constexpr int kStep = kOwn < 32 ? kOwn : 32;      // keys at a time
-    constexpr int kWide = Rows::kWide, kReach = Rows::kReach;
+    using S = Shape<D, EIGHTS>;
+    using Rows = RowTile<D, EIGHTS>;
+    constexpr int kGroups = kWarps / ROW_WARPS;       // warps that take units in turn
+    constexpr int kWide = Rows::kWide, kRows = EIGHTS * 8;
     extern __shared__ uint8_t raw_smem[];
     const uint32_t ring = (smem_u32(raw_smem) + 1023u) & ~1023u;
     uint8_t* smem = raw_smem + (ring - smem_u32(raw_smem));
     float* k_scales = reinterpret_cast<float*>(smem + S::kKScales);
     int* v_scales = reinterpret_cast<int*>(smem + S::kVScales);
     auto full = [&](int s) { return ring + S::kBarriers + 8u * s; };
-    auto empty = [&](int s) { return ring + S::kBarriers + 8u * (S::kStages + s); };
+    auto empty = [&](int s) { return ring + S::kBarriers + 8u * (S::kSlots + s); };
     const int warp = uniform_warp_index(), lane = threadIdx.x & 31;
     const int head = blockIdx.y % a.heads_kv, row_block = blockIdx.y / a.heads_kv;
     const int64_t batch = blockIdx.z;
-    const int row_first = row_block * (MT * 16);
+    const int row_first = row_block * (ROW_WARPS * kRows);
     if (threadIdx.x == 0) {
         prefetch_tensormap(&map_k);
         prefetch_tensormap(&map_v);
-        for (int s = 0; s < S::kStages; ++s) {
+        for (int s = 0; s < S::kSlots; ++s) {
             mbar_init(full(s), 1);
-            mbar_init(empty(s), kWarps);
+            mbar_init(empty(s), ROW_WARPS);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
     chain_begin();
 
-    const int chunk_first = static_cast<int>(blockIdx.x) * a.tiles_per_cta;
+    const int chunk_first = static_cast<int>(blockIdx.x) * a.units_per_cta;
     if (warp == kWarps) {
-        // The loader: lane l brings one box of a tile, `box` rows (a page or a part of one) of K or V by 128 or 64 bytes. Page ids are read a tile ahead of
+        // The loader: lane l brings one box of a unit, `box` rows (16 or 32 of a page) of K or V by 128 or 64 bytes. Page ids are read a unit ahead of
         // their use, and the first ones before the lengths are known.
         constexpr int kHalves = D == 256 ? 2 : 1;
-        const int boxes = S::kKeys / a.box, side = lane / (boxes * kHalves), within = lane % (boxes * kHalves);
+        const int boxes = kUnit / a.box, side = lane / (boxes * kHalves), within = lane % (boxes * kHalves);
         const bool has_box = side < 2;
         const CacheSide& s = a.side[has_box ? side : 0];
         const int box_row = (within / kHalves) * a.box, half = within % kHalves;
         const uint32_t box_bytes = static_cast<uint32_t>(a.box) * (D == 64 ? 64u : 128u);
-        const uint32_t to = side * S::kTile + half * (S::kKeys * 128) + box_row * (D == 64 ? 64 : 128);
-        auto locate = [&](int tile, int& page, int& token) {
-            const int key = tile * S::kKeys + box_row, slot = static_cast<int>(fast_divide(static_cast<uint32_t>(key >> 4), a.by_page));
+        const uint32_t to = side * S::kSide + half * (kUnit * 128) + box_row * (D == 64 ? 64 : 128);
+        auto locate = [&](int unit, int& page, int& token) {
+            const int key = unit * kUnit + box_row, slot = static_cast<int>(fast_divide(static_cast<uint32_t>(key >> 4), a.by_page));
             token = key - slot * a.page;
             page = has_box ? page_of(a, s, batch, slot) : -1;
         };
@@ -340,38 +354,40 @@ cache_sdpa_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
         locate(chunk_first, page, token);
         const SequenceWindow window = sequence_window(a, batch);
         int lo, hi;
-        window_of_tokens(a, window, row_first / a.group, (min(row_first + MT * 16, a.rows) - 1) / a.group, lo, hi);
-        const int tile_first = max(chunk_first, lo / S::kKeys), tile_end = hi > lo ? min(chunk_first + a.tiles_per_cta, (hi + S::kKeys - 1) / S::kKeys) : 0;
-        if (tile_first != chunk_first && tile_first < tile_end) locate(tile_first, page, token);
-        for (int t = 0; t < tile_end - tile_first; ++t) {
-            const int key = (tile_first + t) * S::kKeys + box_row;
+        window_of_tokens(a, window, row_first / a.group, (min(row_first + ROW_WARPS * kRows, a.rows) - 1) / a.group, lo, hi);
+        const int first = max(chunk_first, lo / kUnit), end = hi > lo ? min(chunk_first + a.units_per_cta, (hi + kUnit - 1) / kUnit) : 0;
+        if (first != chunk_first && first < end) locate(first, page, token);
+        int slot = 0;
+        uint32_t turn = 1;
+        for (int u = first; u < end; ++u) {
+            const int key = u * kUnit + box_row;
             const bool live = page >= 0 && key < hi && key + a.box > lo;
             const int now_page = page, now_token = token;
-            if (tile_first + t + 1 < tile_end) locate(tile_first + t + 1, page, token);
-            const int slot = t % S::kStages;
-            if (!mbar_wait_warp(empty(slot), ((t / S::kStages) & 1) ^ 1, 701)) break;
+            if (u + 1 < end) locate(u + 1, page, token);
+            if (!mbar_wait_warp(empty(slot), turn, 701)) break;
             const uint32_t count = __popc(__ballot_sync(0xffffffffu, live));
             if (lane == 0) mbar_expect_tx(full(slot), count * box_bytes);   // (also the arrival; no byte where no page is)
             __syncwarp();
-            if (live) tma_load_4d(ring + slot * (2 * S::kTile) + to, side ? &map_v : &map_k, half * 128, now_token, head, now_page, full(slot));
+            if (live) tma_load_4d(ring + slot * (2 * S::kSide) + to, side ? &map_v : &map_k, half * 128, now_token, head, now_page, full(slot));
+            if (++slot == S::kSlots) slot = 0, turn ^= 1;
         }
         return;
     }
 
-    const int quad = lane & 3, eighth = lane >> 2, mt = warp % MT, group = warp / MT;
+    const int quad = lane & 3, eighth = lane >> 2, row_warp = warp % ROW_WARPS, group = warp / ROW_WARPS;
     const SequenceWindow window = sequence_window(a, batch);
-    // The keys that any row of the CTA sees, and this CTA's tiles among them.
+    // The keys that any row of the CTA sees, and this CTA's units among them.
     int lo, hi;
-    window_of_tokens(a, window, row_first / a.group, (min(row_first + MT * 16, a.rows) - 1) / a.group, lo, hi);
-    const int tile_first = max(chunk_first, lo / S::kKeys), tile_end = hi > lo ? min(chunk_first + a.tiles_per_cta, (hi + S::kKeys - 1) / S::kKeys) : 0;
-    const int tiles = tile_end - tile_first;
-    if (tiles <= 0 && a.chunks > 1) return;   // (the merge knows which chunks a row has)
+    window_of_tokens(a, window, row_first / a.group, (min(row_first + ROW_WARPS * kRows, a.rows) - 1) / a.group, lo, hi);
+    const int first_unit = max(chunk_first, lo / kUnit), end_unit = hi > lo ? min(chunk_first + a.units_per_cta, (hi + kUnit - 1) / kUnit) : 0;
+    const int units = end_unit - first_unit;
+    if (units <= 0 && a.chunks > 1) return;   // (the merge knows which chunks a row has)
 
     // The scales of the runs of 16 keys.
-    for (int i = threadIdx.x; i < 2 * tiles * S::kRuns; i += kConsumers) {
-        const bool is_v = i >= tiles * S::kRuns;
+    for (int i = threadIdx.x; i < 4 * units; i += kConsumers) {
+        const bool is_v = i >= 2 * units;
         const CacheSide& s = a.side[is_v ? 1 : 0];
-        const int run = is_v ? i - tiles * S::kRuns : i, key = tile_first * S::kKeys + run * 16;
+        const int run = is_v ? i - 2 * units : i, key = first_unit * kUnit + run * 16;
         const int slot = static_cast<int>(fast_divide(static_cast<uint32_t>(key >> 4), a.by_page)), block = static_cast<int>(fast_divide(static_cast<uint32_t>((key - slot * a.page) >> 4), a.by_tokens));
         const int page = key < hi && key + 16 > lo ? page_of(a, s, batch, slot) : -1;
         const int code = page >= 0 ? s.scales[page * s.scale_stride[0] + head * s.scale_stride[1] + block * s.scale_stride[2]] : -1;
@@ -380,29 +396,32 @@ cache_sdpa_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     }
 
     Rows rows;
-    int64_t token_of[2];
-    int head_of[2];
-    bool live_row[2];           // has a place in O
+    const int own_row = row_first + row_warp * kRows;
+    auto place_of = [&](int row, int& token, int& head_q) {   // of a row that there is
+        token = row / a.group;
+        head_q = head * a.group + (row - token * a.group);
+    };
+    int common_lo = lo, common_hi = hi, any_lo = hi, any_hi = lo;   // what the warp's rows see in common, and what any of them sees
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        const int row = row_first + mt * 16 + half * 8 + eighth;
-        live_row[half] = row < a.rows;
-        const int token = live_row[half] ? row / a.group : 0;
-        token_of[half] = token;
-        head_of[half] = head * a.group + (live_row[half] ? row - token * a.group : 0);
-        const bool takes_part = live_row[half] && token < window.len_q;
-        rows.row_lo[half] = lo, rows.row_hi[half] = hi;      // (rows without a part see what the others see; their results go nowhere)
-        if (takes_part) window_of_tokens(a, window, token, token, rows.row_lo[half], rows.row_hi[half]);
-        rows.row_hi[half] = max(rows.row_hi[half], rows.row_lo[half]);
-        const T* from = static_cast<const T*>(a.q) + batch * a.q_stride[0] + head_of[half] * a.q_stride[1] + token * a.q_stride[2];
+    for (int n = 0; n < EIGHTS; ++n) {
+        // Q of row `eighth`: this quarter of its channels
+        const int row = own_row + n * 8 + eighth;
+        int token = 0, head_q = 0;
+        if (row < a.rows) place_of(row, token, head_q);
+        const T* from = static_cast<const T*>(a.q) + batch * a.q_stride[0] + head_q * a.q_stride[1] + token * a.q_stride[2];
         float v[Rows::kDeep][4];
         float largest = 0.0f;
 #pragma unroll
         for (int i = 0; i < Rows::kDeep; ++i) {
             const int channel = D == 64 ? quad * 16 + i * 4 : (quad * 2 + ((i >> 2) & 1) + (i >> 3) * 8) * 16 + (i & 3) * 4;
+            struct alignas(8) Four { T v[4]; } four{};
+            if (row < a.rows) {
+                if (a.q_vector) four = *reinterpret_cast<const Four*>(from + channel);
+                else four = Four{{from[channel], from[channel + 1], from[channel + 2], from[channel + 3]}};
+            }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                v[i][e] = live_row[half] ? value_of(from[channel + e]) : 0.0f;
+                v[i][e] = value_of(four.v[e]);
                 largest = fmaxf(largest, fabsf(v[i][e]));
             }
         }
@@ -410,132 +429,150 @@ cache_sdpa_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
         largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
         int up = 14 - (static_cast<int>(__float_as_uint(largest) >> 23) - 127);
         up = largest == 0.0f ? 0 : min(max(up, -126), 126);
-        const float power = power_of_two(up);
-        rows.factor[half] = power_of_two(-up) * a.scale_log2;
+        const float power = power_of_two(up), factor = power_of_two(-up) * a.scale_log2;
 #pragma unroll
         for (int i = 0; i < Rows::kDeep; ++i) {
-            rows.q[i][half] = two_halves(v[i][0] * power, v[i][1] * power);
-            rows.q[i][2 + half] = two_halves(v[i][2] * power, v[i][3] * power);
+            rows.q[i][n][0] = two_halves(v[i][0] * power, v[i][1] * power);
+            rows.q[i][n][1] = two_halves(v[i][2] * power, v[i][3] * power);
         }
-        rows.largest[half] = -INFINITY;
-        rows.sum[half] = 0.0f;
+        // rows 2 quad and 2 quad + 1
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            rows.factor[n][c] = __shfl_sync(0xffffffffu, factor, (quad * 2 + c) * 4);
+            const int column = own_row + n * 8 + quad * 2 + c;
+            const bool there = column < a.rows && column / a.group < window.len_q;
+            rows.row_lo[n][c] = lo, rows.row_hi[n][c] = hi;      // (rows without a part see what the others see; their results go nowhere)
+            if (there) {
+                window_of_tokens(a, window, column / a.group, column / a.group, rows.row_lo[n][c], rows.row_hi[n][c]);
+                any_lo = min(any_lo, rows.row_lo[n][c]);
+                any_hi = max(any_hi, rows.row_hi[n][c]);
+            }
+            rows.row_hi[n][c] = max(rows.row_hi[n][c], rows.row_lo[n][c]);
+            common_lo = max(common_lo, rows.row_lo[n][c]);
+            common_hi = min(common_hi, rows.row_hi[n][c]);
+            rows.largest[n][c] = -INFINITY;
+            rows.sum[n][c] = 0.0f;
+        }
     }
     rows.unit = kNoUnit;
 #pragma unroll
     for (int j = 0; j < kWide; ++j)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) rows.o[j][c] = 0.0f;
-    // What the warp's rows see in common, and what any of them sees.
-    const int common_lo = __reduce_max_sync(0xffffffffu, max(rows.row_lo[0], rows.row_lo[1])), common_hi = __reduce_min_sync(0xffffffffu, min(rows.row_hi[0], rows.row_hi[1]));
-    const int any_lo = __reduce_min_sync(0xffffffffu, min(rows.row_lo[0], rows.row_lo[1])), any_hi = __reduce_max_sync(0xffffffffu, max(rows.row_hi[0], rows.row_hi[1]));
+        for (int n = 0; n < EIGHTS; ++n)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) rows.o[j][n][c] = 0.0f;
+    common_lo = __reduce_max_sync(0xffffffffu, common_lo), common_hi = __reduce_min_sync(0xffffffffu, common_hi);
+    any_lo = __reduce_min_sync(0xffffffffu, any_lo), any_hi = __reduce_max_sync(0xffffffffu, any_hi);
     asm volatile("bar.sync 1, 128;" ::: "memory");   // the scales are there
 
     bool ok = true;
-    for (int t = 0; t < tiles; ++t) {
-        const int slot = t % S::kStages;
-        if (ok) ok = mbar_wait_warp(full(slot), (t / S::kStages) & 1, 702);
+    for (int u = group; u < units; u += kGroups) {
+        const int slot = u % S::kSlots;
+        ok = mbar_wait_warp(full(slot), (u / S::kSlots) & 1, 702);
         if (!ok) break;
-        const uint8_t* k_tile = smem + slot * (2 * S::kTile);
-        const uint8_t* v_tile = k_tile + S::kTile;
-#pragma unroll 1
-        for (int at = group * kOwn; at < (group + 1) * kOwn; at += kStep) {
-            const int key0 = (tile_first + t) * S::kKeys + at, run = t * S::kRuns + (at >> 4);
-            if (key0 >= any_hi || key0 + kStep <= any_lo) continue;
-            bool special = key0 < common_lo || key0 + kStep > common_hi;
-#pragma unroll
-            for (int r = 0; r < kStep / 16; ++r) special = special || k_scales[run + r] < 0.0f || static_cast<uint32_t>(v_scales[run + r]) > 254u;
-            if (special) rows.template step<true, kStep>(k_tile, v_tile, k_scales + run, v_scales + run, at, key0, lo, hi, a.seq_q > 1);
-            else rows.template step<false, kStep>(k_tile, v_tile, k_scales + run, v_scales + run, at, key0, lo, hi, false);
+        const uint8_t* k_unit = smem + slot * (2 * S::kSide);
+        const int key0 = (first_unit + u) * kUnit;
+        const float* k_scale = k_scales + 2 * u;
+        const int* v_scale = v_scales + 2 * u;
+        if (key0 < any_hi && key0 + kUnit > any_lo) {
+            const bool special = key0 < common_lo || key0 + kUnit > common_hi || fminf(k_scale[0], k_scale[1]) < 0.0f ||
+                                 max(static_cast<uint32_t>(v_scale[0]), static_cast<uint32_t>(v_scale[1])) > 254u;
+            if (special) rows.template step<true>(k_unit, k_unit + S::kSide, k_scale, v_scale, key0, lo, hi, a.seq_q > 1);
+            else rows.template step<false>(k_unit, k_unit + S::kSide, k_scale, v_scale, key0, lo, hi, false);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(empty(slot));
     }
     ok = ok && g_device_status == 0;
 
-    // The warps of an M tile meet: (largest score, sum, O) triples by shared memory, in the order of the fragments, so that each bank
-    // is met once. Warp g then has rows and columns of its own: fragment values c with c * groups / 4 == g.
+    // The warps with the same rows meet: (largest score, sum, O) triples by shared memory, in the order of the fragments, so that each bank
+    // is met once. Each of them then has pairs of channels of its own: place i of [eight][row of two][pair] with i * groups / places == group.
+    constexpr int kPlaces = EIGHTS * 2 * kWide;
     const float absolute = rows.unit == kNoUnit ? 1.0f : decode_e8m0(static_cast<uint32_t>(rows.unit));
 #pragma unroll
-    for (int j = 0; j < kWide; ++j)
+    for (int n = 0; n < EIGHTS; ++n) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) rows.o[j][c] *= absolute;
+        for (int j = 0; j < kWide; ++j)
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        rows.sum[half] += __shfl_xor_sync(0xffffffffu, rows.sum[half], 1);
-        rows.sum[half] += __shfl_xor_sync(0xffffffffu, rows.sum[half], 2);
+            for (int c = 0; c < 4; ++c) rows.o[j][n][c] *= absolute;
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) rows.sum[n][c] += __shfl_xor_sync(0xffffffffu, rows.sum[n][c], x);
     }
-    float top[2] = {rows.largest[0], rows.largest[1]}, total[2] = {rows.sum[0], rows.sum[1]};
     if constexpr (kGroups > 1) {
-        asm volatile("bar.sync 1, 128;" ::: "memory");   // (every tile has come and been read)
-        float* fragments = reinterpret_cast<float*>(smem);                 // [warp][4 * kWide][32]
-        float* meeting = reinterpret_cast<float*>(smem + S::kKScales);     // [warp][half][32][2]
+        asm volatile("bar.sync 1, 128;" ::: "memory");   // (every unit has come and been read)
+        float2* fragments = reinterpret_cast<float2*>(smem);                 // [warp][places][32]
+        float2* meeting = reinterpret_cast<float2*>(smem + S::kKScales);     // [warp][eight][row of two][quad]
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            meeting[((warp * 2 + half) * 32 + lane) * 2] = rows.largest[half];
-            meeting[((warp * 2 + half) * 32 + lane) * 2 + 1] = rows.sum[half];
-        }
+        for (int n = 0; n < EIGHTS; ++n)
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+            for (int c = 0; c < 2; ++c) {
+                if (eighth == 0) meeting[((warp * EIGHTS + n) * 2 + c) * 4 + quad] = make_float2(rows.largest[n][c], rows.sum[n][c]);
 #pragma unroll
-            for (int j = 0; j < kWide; ++j) fragments[((warp * 4 + c) * kWide + j) * 32 + lane] = rows.o[j][c];
+                for (int j = 0; j < kWide; ++j) fragments[((warp * EIGHTS * 2 + n * 2 + c) * kWide + j) * 32 + lane] = make_float2(rows.o[j][n][c], rows.o[j][n][c + 2]);
+            }
         asm volatile("bar.sync 1, 128;" ::: "memory");
-        float weight[kGroups][2];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            top[half] = -INFINITY, total[half] = 0.0f;
+        for (int n = 0; n < EIGHTS; ++n)
 #pragma unroll
-            for (int g = 0; g < kGroups; ++g) top[half] = fmaxf(top[half], meeting[(((g * MT + mt) * 2 + half) * 32 + lane) * 2]);
+            for (int c = 0; c < 2; ++c) {
+                float2 other[kGroups];
+                float top = -INFINITY, total = 0.0f;
 #pragma unroll
-            for (int g = 0; g < kGroups; ++g) {
-                const float* other = meeting + (((g * MT + mt) * 2 + half) * 32 + lane) * 2;
-                weight[g][half] = other[0] == -INFINITY ? 1.0f : exp2_of(other[0] - top[half]);   // (a group without keys has zeros)
-                total[half] = fmaf(other[1], weight[g][half], total[half]);
+                for (int g = 0; g < kGroups; ++g) {
+                    other[g] = meeting[(((g * ROW_WARPS + row_warp) * EIGHTS + n) * 2 + c) * 4 + quad];
+                    top = fmaxf(top, other[g].x);
+                }
+#pragma unroll
+                for (int g = 0; g < kGroups; ++g) {
+                    other[g].x = other[g].x == -INFINITY ? 1.0f : exp2_of(other[g].x - top);   // (a group without keys has zeros)
+                    total = fmaf(other[g].y, other[g].x, total);
+                }
+                rows.largest[n][c] = top, rows.sum[n][c] = total;
+#pragma unroll
+                for (int j = 0; j < kWide; ++j) {
+                    if (((n * 2 + c) * kWide + j) * kGroups / kPlaces != group) continue;
+                    float2 v = make_float2(0.0f, 0.0f);
+#pragma unroll
+                    for (int g = 0; g < kGroups; ++g) {
+                        const float2 part = fragments[(((g * ROW_WARPS + row_warp) * EIGHTS * 2 + n * 2 + c) * kWide + j) * 32 + lane];
+                        v.x = fmaf(part.x, other[g].x, v.x);
+                        v.y = fmaf(part.y, other[g].x, v.y);
+                    }
+                    rows.o[j][n][c] = v.x, rows.o[j][n][c + 2] = v.y;
+                }
             }
-        }
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            if (c * kGroups / 4 != group) continue;
-#pragma unroll
-            for (int j = 0; j < kWide; ++j) {
-                float v = 0.0f;
-#pragma unroll
-                for (int g = 0; g < kGroups; ++g) v = fmaf(fragments[(((g * MT + mt) * 4 + c) * kWide + j) * 32 + lane], weight[g][c >> 1], v);
-                rows.o[j][c] = v;
-            }
-        }
     }
     if (!ok) return;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-        if (c * kGroups / 4 != group) continue;
-        const int half = c >> 1, column = quad * 2 + (c & 1);
-        if (!live_row[half]) continue;
-        const bool first_of_row = column == 0;
-        const bool takes_part = token_of[half] < window.len_q;
-        if (a.chunks > 1) {
-            const int64_t row = (batch * a.heads_kv + head) * a.rows + row_first + mt * 16 + half * 8 + eighth;
-            float* partial = a.partial + (row * a.chunks + blockIdx.x) * (D + 2);
+    for (int n = 0; n < EIGHTS; ++n)
 #pragma unroll
-            for (int j = 0; j < kWide; j += 2) {
-                const int channel = column * kReach + (j & (kReach - 1)) + (j / kReach) * 128;
-                *reinterpret_cast<float2*>(partial + channel) = make_float2(rows.o[j][c], rows.o[j + 1][c]);
+        for (int c = 0; c < 2; ++c) {
+            const int row = own_row + n * 8 + quad * 2 + c;
+            if (row >= a.rows) continue;
+            const float top = rows.largest[n][c], total = rows.sum[n][c];
+            if (a.chunks > 1) {
+                float* partial = a.partial + (((batch * a.heads_kv + head) * a.rows + row) * a.chunks + blockIdx.x) * (D + 2);
+#pragma unroll
+                for (int j = 0; j < kWide; ++j)
+                    if (((n * 2 + c) * kWide + j) * kGroups / kPlaces == group)
+                        *reinterpret_cast<float2*>(partial + Rows::channel_of(j, eighth)) = make_float2(rows.o[j][n][c], rows.o[j][n][c + 2]);
+                if (eighth == 0 && group == 0) *reinterpret_cast<float2*>(partial + D) = make_float2(top, total);
+            } else {
+                int token, head_q;
+                place_of(row, token, head_q);
+                const bool none = token >= window.len_q || total == 0.0f;   // (a NaN sum is a NaN result)
+                const float inverse = 1.0f / total;
+                const int64_t at = batch * a.o_stride[0] + head_q * a.o_stride[1] + token * a.o_stride[2];
+#pragma unroll
+                for (int j = 0; j < kWide; ++j)
+                    if (((n * 2 + c) * kWide + j) * kGroups / kPlaces == group)
+                        store_pair(a, at + Rows::channel_of(j, eighth), none ? 0.0f : rows.o[j][n][c] * inverse, none ? 0.0f : rows.o[j][n][c + 2] * inverse);
+                if (eighth == 0 && group == 0 && a.stats)
+                    a.stats[batch * a.stats_stride[0] + head_q * a.stats_stride[1] + token * a.stats_stride[2]] = none ? -INFINITY : top * kLn2 + logf(total * 0x1p-15f);
             }
-            if (first_of_row) *reinterpret_cast<float2*>(partial + D) = make_float2(top[half], total[half]);
-        } else {
-            const bool none = !takes_part || total[half] == 0.0f;   // (a NaN sum is a NaN result)
-            const float inverse = 1.0f / total[half];
-#pragma unroll
-            for (int j0 = 0; j0 < kWide; j0 += kReach) {
-                float v[kReach];
-#pragma unroll
-                for (int j = 0; j < kReach; ++j) v[j] = none ? 0.0f : rows.o[j0 + j][c] * inverse;
-                store_values(a, batch * a.o_stride[0] + head_of[half] * a.o_stride[1] + token_of[half] * a.o_stride[2] + column * kReach + (j0 / kReach) * 128, v);
-            }
-            if (first_of_row && a.stats)
-                a.stats[batch * a.stats_stride[0] + head_of[half] * a.stats_stride[1] + token_of[half] * a.stats_stride[2]] =
-                    none ? -INFINITY : top[half] * kLn2 + logf(total[half] * 0x1p-15f);
         }
-    }
 }
 
 // A CTA a row, a thread a channel. Latency-bound: maxima and sums of the first 32 chunks, a chunk a lane in every warp, and the values of
@@ -557,7 +594,7 @@ cache_sdpa_merge_kernel(const __grid_constant__ CacheSdpaArgs a) {
     const SequenceWindow window = sequence_window(a, batch);
     int lo = 0, hi = 0;
     if (token < window.len_q) window_of_tokens(a, window, token, token, lo, hi);
-    const int keys = a.tiles_per_cta * a.tile_keys;
+    const int keys = a.units_per_cta * kUnit;
     const int first = lo / keys, end = hi > lo ? (hi + keys - 1) / keys : first;
     auto pair_of = [&](int c) {   // (largest score, sum); a chunk without keys of the row was perhaps not written
         if (c < first || c >= end) return make_float2(-INFINITY, 0.0f);
@@ -596,7 +633,7 @@ cache_sdpa_merge_kernel(const __grid_constant__ CacheSdpaArgs a) {
 }
 
 struct StreamPlan {
-    int row_tiles, row_blocks, tile_keys, tiles_per_cta, chunks;
+    int eights, row_warps, row_blocks, units_per_cta, chunks;
     int64_t rows, scratch;
 };
 
@@ -604,16 +641,21 @@ StreamPlan plan_stream(const dfgpu_cache_sdpa_params& p) {
     StreamPlan plan{};
     const int64_t d = p.q.dim[3], group = p.q.dim[1] / p.k.dim[1];
     plan.rows = group * p.q.dim[2];
-    plan.row_tiles = plan.rows <= 16 ? 1 : plan.rows <= 32 ? 2 : 4;
-    plan.row_blocks = static_cast<int>((plan.rows + plan.row_tiles * 16 - 1) / (plan.row_tiles * 16));
-    plan.tile_keys = d == 256 ? 64 : 128;
-    const int64_t tiles = (p.s_kv + plan.tile_keys - 1) / plan.tile_keys, lists = p.q.dim[0] * p.k.dim[1] * plan.row_blocks;
-    // Long runs of tiles save prologues and partial results (the more the more rows there are), short ones give a small batch more
+    plan.eights = plan.rows <= 8 ? 1 : 2;
+    plan.row_warps = plan.rows <= 16 ? 1 : plan.rows <= 32 ? 2 : 4;
+    const int block = plan.eights * 8 * plan.row_warps;
+    plan.row_blocks = static_cast<int>((plan.rows + block - 1) / block);
+    const int64_t units = (p.s_kv + kUnit - 1) / kUnit, lists = p.q.dim[0] * p.k.dim[1] * plan.row_blocks;
+    // Units that a CTA's rows can see: a left bound and its last row's right one leave a band of them.
+    int64_t seen = units;
+    if (p.has_left_bound && p.has_right_bound && p.left_bound + p.right_bound >= 0 && p.left_bound < p.s_kv && p.right_bound < p.s_kv)
+        seen = std::min(units, (p.left_bound + p.right_bound + std::min<int64_t>(p.q.dim[2], block)) / kUnit + 1);
+    // Long runs of units save prologues and partial results (the more the more rows there are), short ones give a small batch more
     // CTAs: as long as there are three for every two SMs (148: a function of the shape alone, as the scratch is).
-    int per_cta = 8 * plan.row_tiles;
-    while (per_cta > 1 && 2 * lists * ((tiles + per_cta - 1) / per_cta) < 3 * 148) per_cta /= 2;
-    plan.tiles_per_cta = per_cta;
-    plan.chunks = static_cast<int>((tiles + per_cta - 1) / per_cta);
+    int per_cta = std::min(kMostUnits, 32 * plan.row_warps);
+    while (per_cta > 4 && 2 * lists * ((seen + per_cta - 1) / per_cta) < 3 * 148) per_cta /= 2;
+    plan.units_per_cta = per_cta;
+    plan.chunks = static_cast<int>((units + per_cta - 1) / per_cta);
     plan.scratch = plan.chunks > 1 ? p.q.dim[0] * p.k.dim[1] * plan.rows * plan.chunks * (d + 2) * 4 : 0;
     return plan;
 }
@@ -683,15 +725,22 @@ int make_side_map(CUtensorMap* map, const dfgpu_tensor& cache, const void* base,
     return kOk;
 }
 
+template <typename T, int D, int EIGHTS, int ROW_WARPS>
+int launch_rows(const CUtensorMap& map_k, const CUtensorMap& map_v, const CacheSdpaArgs& a, dim3 grid, cudaStream_t stream) {
+    constexpr int kBytes = Shape<D, EIGHTS>::kDynamic;
+    const auto kernel = cache_sdpa_stream_kernel<T, D, EIGHTS, ROW_WARPS>;
+    const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+    if (error != cudaSuccess) return fail(kExecutionFailed, "CACHE_SDPA: cannot reserve %d bytes of shared memory: %s", kBytes, cudaGetErrorString(error));
+    launch_chained(kernel, grid, dim3(kThreads), kBytes, stream, map_k, map_v, a);
+    return check_launch("CACHE_SDPA");
+}
+
 template <typename T, int D>
 int launch_stream(const CUtensorMap& map_k, const CUtensorMap& map_v, const CacheSdpaArgs& a, const StreamPlan& plan, dim3 grid, cudaStream_t stream) {
-    auto run = [&](auto kernel) -> int {
-        const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kDynamic);
-        if (error != cudaSuccess) return fail(kExecutionFailed, "CACHE_SDPA: cannot reserve %d bytes of shared memory: %s", Shape<D>::kDynamic, cudaGetErrorString(error));
-        launch_chained(kernel, grid, dim3(kThreads), Shape<D>::kDynamic, stream, map_k, map_v, a);
-        return check_launch("CACHE_SDPA");
-    };
-    const int status = plan.row_tiles == 1 ? run(cache_sdpa_stream_kernel<T, D, 1>) : plan.row_tiles == 2 ? run(cache_sdpa_stream_kernel<T, D, 2>) : run(cache_sdpa_stream_kernel<T, D, 4>);
+    const int status = plan.eights == 1      ? launch_rows<T, D, 1, 1>(map_k, map_v, a, grid, stream)
+                       : plan.row_warps == 1 ? launch_rows<T, D, 2, 1>(map_k, map_v, a, grid, stream)
+                       : plan.row_warps == 2 ? launch_rows<T, D, 2, 2>(map_k, map_v, a, grid, stream)
+                                             : launch_rows<T, D, 2, 4>(map_k, map_v, a, grid, stream);
     if (status || plan.chunks == 1) return status;
     launch_chained(cache_sdpa_merge_kernel<D>, dim3(static_cast<unsigned>(static_cast<int64_t>(grid.z) * a.heads_kv * a.rows)), dim3(D), 0, stream, a);
     return check_launch("CACHE_SDPA merge");
@@ -755,9 +804,12 @@ extern "C" int dfgpu_cache_sdpa(const dfgpu_cache_sdpa_params* p, void* const* t
         a.stats_stride[i] = p->stats.rank ? p->stats.stride[i] : 0;
     }
     a.o_type = p->o.dtype;
-    const int64_t o_row = 16 / dtype_bytes(p->o.dtype);
-    a.o_vector = on_16(a.o);
-    for (int i = 0; i < 3; ++i) a.o_vector = a.o_vector && (p->o.dim[i] == 1 || p->o.stride[i] % o_row == 0);
+    a.o_vector = (reinterpret_cast<uintptr_t>(a.o) & static_cast<uintptr_t>(2 * dtype_bytes(p->o.dtype) - 1)) == 0;   // pairs of O, fours of Q
+    a.q_vector = (reinterpret_cast<uintptr_t>(a.q) & 7u) == 0;
+    for (int i = 0; i < 3; ++i) {
+        a.o_vector = a.o_vector && (p->o.dim[i] == 1 || p->o.stride[i] % 2 == 0);
+        a.q_vector = a.q_vector && (p->q.dim[i] == 1 || p->q.stride[i] % 4 == 0);
+    }
     a.seq_q_data = p->seq_q.rank ? static_cast<const int32_t*>(tensors[7]) : nullptr;
     a.seq_kv_data = static_cast<const int32_t*>(tensors[8]);
     a.seq_q_stride = p->seq_q.rank ? p->seq_q.stride[0] : 0;
@@ -778,11 +830,9 @@ extern "C" int dfgpu_cache_sdpa(const dfgpu_cache_sdpa_params* p, void* const* t
     a.right = std::min(std::max(p->right_bound, -far), far);
     a.scale_log2 = p->attn_scale * 1.4426950408889634f;
     a.chunks = plan.chunks;
-    a.tiles_per_cta = plan.tiles_per_cta;
-    a.tile_keys = plan.tile_keys;
+    a.units_per_cta = plan.units_per_cta;
     a.partial = static_cast<float*>(scratch);
-    // TMA boxes: the most tokens up to 64 that divide a page's
-    a.box = a.page % 64 == 0 ? 64 : a.page % 32 == 0 ? 32 : 16;
+    a.box = a.page % 32 == 0 ? 32 : 16;
     CUtensorMap map_k, map_v;
     int made = make_side_map(&map_k, p->k, tensors[1], a.box);
     if (!made) made = make_side_map(&map_v, p->v, tensors[2], a.box);

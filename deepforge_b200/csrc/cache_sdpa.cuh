@@ -24,12 +24,12 @@ struct CacheSdpaArgs {
     float* partial;       // [row][chunk][D + 2]: O against the chunk's own largest score, that score, sum
     int64_t q_stride[3], o_stride[3], stats_stride[3], seq_q_stride, seq_kv_stride;
     int64_t left, right;
-    int32_t o_type, o_vector;
+    int32_t o_type, o_vector, q_vector;
     int32_t heads_kv, group, rows, seq_q, s_kv;   // rows: (token, head of the group) pairs of a KV head
     int32_t page, box;                            // tokens a page, and of one TMA copy
     FastDivisor by_page, by_tokens;               // of numbers of 16 tokens
     int32_t has_left, has_right, bottom_right;
-    int32_t chunks, tiles_per_cta, tile_keys;
+    int32_t chunks, units_per_cta;
     float scale_log2;
 };
 
