@@ -17,9 +17,11 @@
 // Channels and keys may go to any index of a product as long as both operands agree; the ones taken here give each thread 16-byte
 // reads without bank conflicts: of K 32 consecutive channels of a key, of V 16 consecutive channels of four keys, and of O 16
 // consecutive channels of a row.
-// CTA: one (sequence, KV head, block of rows), a run of units of 32 keys; a fifth warp brings them by TMA (pages or parts of them,
-// swizzled) into a ring, four take them in turn, or in pairs or all of them with rows of their own where there are more than 16.
-// Single tokens leave three CTAs on an SM. More than one run of units a sequence leaves partial results that a second kernel merges.
+// The work is one row of units of 32 keys, list by list (a sequence's block of rows, a KV head), cut into equal parts for the CTAs that are on
+// the chip together (three an SM for single tokens): lengths differ, and a grid of lists or of pieces of them pays for it with idle SMs
+// at the end and with a prologue for each piece. A fifth warp brings a CTA's units by TMA into a ring, across lists, so that the
+// next list's codes are on their way while O of the last one is written; four take them in turn, or in pairs or all of them with rows
+// of their own where there are more than 16. Lists that were cut leave partial results, which a second kernel merges.
 #include <algorithm>
 #include <cmath>
 
@@ -30,9 +32,11 @@
 namespace dfgpu {
 namespace {
 
-constexpr int kWarps = 4, kConsumers = 128, kThreads = 160;
+constexpr int kWarps = 4, kThreads = 160;
 constexpr int kUnit = 32;          // keys that a warp takes at a time
-constexpr int kMostUnits = 128;    // of a CTA
+constexpr int kBatch = 4;          // units that the loader looks up at a time
+constexpr int kLeastUnits = 8;     // of a CTA: fewer cost more in prologues and partial results than they gain
+constexpr int kSms = 148;          // (the cut is a function of the shape and the lengths alone, as the scratch is of the shape)
 constexpr float kUp = 15.0f;       // probabilities are held as p * 2^15
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kNoUnit = -100000;   // O is zero and has no unit yet
@@ -43,12 +47,17 @@ template <int D, int EIGHTS>
 struct Shape {
     static constexpr int kCtas = D == 256 ? (EIGHTS == 1 ? 2 : 1) : EIGHTS == 1 ? 3 : 2;   // on an SM
     static constexpr int kSide = kUnit * D;                                                // bytes of a unit's K or V
-    static constexpr int kSlots = (kCtas == 3 ? 64 : kCtas == 2 ? 96 : 192) * 1024 / (2 * kSide);
+    // A multiple of the warps, so that a slot's units are always the same warp's: it then knows one phase of the slot's barrier from the
+    // next. (With six slots a warp that was ahead took the phase before last, of another warp's unit, for its own.)
+    static constexpr int kSlots = (kCtas == 3 ? 64 : D == 256 ? (EIGHTS == 1 ? 64 : 192) : 96) * 1024 / (2 * kSide);
+    static_assert(kSlots % kWarps == 0, "a slot belongs to one warp");
     static constexpr int kRing = kSlots * 2 * kSide;
-    static constexpr int kKScales = kRing;                                    // [runs of 16 keys] f32, -1: the page's rows read as zeros
-    static constexpr int kVScales = kKScales + kMostUnits * 2 * 4;            // [runs] the code, -1 likewise
-    static constexpr int kBarriers = kVScales + kMostUnits * 2 * 4;           // full[slots], empty[slots]
-    static constexpr int kTotal = kBarriers + 2 * kSlots * 8;
+    static constexpr int kFragments = kRing;                                  // [warp][pairs of O][32] float2, of one row of two of an eight
+    static constexpr int kMeeting = kFragments + kWarps * (D / 16) * 32 * 8;  // [warp][eight][row of two][quad] float2
+    static constexpr int kScales = kMeeting + kWarps * EIGHTS * 2 * 4 * 8;    // [slot] K scales of its two runs of 16 keys as f32 (-1: the page's rows read as zeros), V's as codes (-1 likewise)
+    static constexpr int kBarriers = kScales + kSlots * 16;                   // full[slots], empty[slots]
+    static constexpr int kScan = kBarriers + 2 * kSlots * 8;                  // [warps] int64, then where the CTA begins
+    static constexpr int kTotal = kScan + 64 + 32;
     static constexpr int kDynamic = kTotal + 1024;
 };
 
@@ -303,6 +312,48 @@ struct RowTile {
     }
 };
 
+// Units of keys of an entry (a sequence's block of rows), the same for each of its KV heads.
+__device__ __forceinline__ int units_of(const CacheSdpaArgs& a, int entry, int& lo, int& hi) {
+    const int sequence = entry / a.row_blocks, row_first = (entry - sequence * a.row_blocks) * a.block_rows;
+    window_of_tokens(a, sequence_window(a, sequence), row_first / a.group, (min(row_first + a.block_rows, a.rows) - 1) / a.group, lo, hi);
+    return hi > lo ? (hi + kUnit - 1) / kUnit - lo / kUnit : 0;
+}
+
+// A CTA's way through the lists: entry, KV head, the next unit of the list and how many of the CTA's are left.
+struct Walk {
+    int entry, head, offset, left;
+    int lo, hi, units;      // of the entry
+    bool first;             // nothing has been taken yet
+
+    // The next piece of a list, `take` units from unit `offset` on; false after the last. Every lane of a warp walks alike. Entries without
+    // keys are passed over 32 at a time.
+    __device__ __forceinline__ bool next(const CacheSdpaArgs& a, int& take) {
+        if (left <= 0) return false;
+        while (units == 0) {
+            const int lane = threadIdx.x & 31;
+            int from = 0, until = 0;
+            const int n = entry + lane < a.entries ? units_of(a, entry + lane, from, until) : 0;
+            const uint32_t some = __ballot_sync(0xffffffffu, n > 0);
+            if (some == 0) {
+                entry += 32;
+                if (entry >= a.entries) return false;
+                continue;
+            }
+            const int found = __ffs(some) - 1;
+            entry += found;
+            lo = __shfl_sync(0xffffffffu, from, found), hi = __shfl_sync(0xffffffffu, until, found), units = __shfl_sync(0xffffffffu, n, found);
+        }
+        take = min(units - offset, left);
+        return true;
+    }
+    __device__ __forceinline__ void taken(const CacheSdpaArgs& a, int take) {
+        left -= take;
+        offset = 0;
+        first = false;
+        if (++head == a.heads_kv) head = 0, ++entry, units = 0;
+    }
+};
+
 // ROW_WARPS: warps with rows of their own.
 template <typename T, int D, int EIGHTS, int ROW_WARPS>
 __global__ void __launch_bounds__(kThreads, Shape<D, EIGHTS>::kCtas)
@@ -314,327 +365,375 @@ cache_sdpa_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     extern __shared__ uint8_t raw_smem[];
     const uint32_t ring = (smem_u32(raw_smem) + 1023u) & ~1023u;
     uint8_t* smem = raw_smem + (ring - smem_u32(raw_smem));
-    float* k_scales = reinterpret_cast<float*>(smem + S::kKScales);
-    int* v_scales = reinterpret_cast<int*>(smem + S::kVScales);
     auto full = [&](int s) { return ring + S::kBarriers + 8u * s; };
     auto empty = [&](int s) { return ring + S::kBarriers + 8u * (S::kSlots + s); };
     const int warp = uniform_warp_index(), lane = threadIdx.x & 31;
-    const int head = blockIdx.y % a.heads_kv, row_block = blockIdx.y / a.heads_kv;
-    const int64_t batch = blockIdx.z;
-    const int row_first = row_block * (ROW_WARPS * kRows);
     if (threadIdx.x == 0) {
         prefetch_tensormap(&map_k);
         prefetch_tensormap(&map_v);
         for (int s = 0; s < S::kSlots; ++s) {
-            mbar_init(full(s), 1);
+            mbar_init(full(s), 5);            // the loader's bytes, four scales
             mbar_init(empty(s), ROW_WARPS);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    __syncthreads();
     chain_begin();
 
-    const int chunk_first = static_cast<int>(blockIdx.x) * a.units_per_cta;
+    // All units before those of this thread's entries, and their number: where this CTA's part begins.
+    Walk walk{};
+    int per;
+    {
+        int64_t* sums = reinterpret_cast<int64_t*>(smem + S::kScan);
+        int* begin = reinterpret_cast<int*>(smem + S::kScan + 64);
+        const int each = (a.entries + kThreads - 1) / kThreads, from = min(static_cast<int>(threadIdx.x) * each, a.entries), until = min(from + each, a.entries);
+        int64_t own = 0;
+        int lo, hi;
+        for (int e = from; e < until; ++e) own += units_of(a, e, lo, hi);
+        own *= a.heads_kv;
+        int64_t up_to = own;
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) {
+            const int64_t other = __shfl_up_sync(0xffffffffu, up_to, x);
+            if (lane >= x) up_to += other;
+        }
+        if (lane == 31) sums[warp] = up_to;
+        __syncthreads();
+        int64_t all = 0, before = up_to - own;
+#pragma unroll
+        for (int w = 0; w <= kWarps; ++w) {
+            if (w < warp) before += sums[w];
+            all += sums[w];
+        }
+        per = max(static_cast<int>((all + gridDim.x - 1) / gridDim.x), kLeastUnits);
+        if (blockIdx.x == 0 && threadIdx.x == 0) a.starts[0] = per;
+        int64_t start = static_cast<int64_t>(blockIdx.x) * per;
+        walk.left = static_cast<int>(max(min(static_cast<int64_t>(per), all - start), static_cast<int64_t>(0)));
+        if (walk.left > 0 && start >= before && start < before + own) {
+            start -= before;
+            for (int e = from; e < until; ++e) {
+                const int n = units_of(a, e, lo, hi);
+                if (start < static_cast<int64_t>(n) * a.heads_kv) {
+                    begin[0] = e, begin[1] = static_cast<int>(start / n), begin[2] = static_cast<int>(start % n);
+                    break;
+                }
+                start -= static_cast<int64_t>(n) * a.heads_kv;
+            }
+        }
+        __syncthreads();
+        if (walk.left <= 0) return;
+        walk.entry = begin[0], walk.head = begin[1], walk.offset = begin[2];
+        walk.first = true;
+    }
+
     if (warp == kWarps) {
-        // The loader: lane l brings one box of a unit, `box` rows (16 or 32 of a page) of K or V by 128 or 64 bytes. Page ids are read a unit ahead of
-        // their use, and the first ones before the lengths are known.
+        // The loader looks up four units at a time: lane l has one box of one of them, `box` rows (16 or 32 of a page) of K or V by 128 or 64 bytes, and
+        // the first sixteen lanes one of their scales each. Page ids are read two batches ahead of their use, scales one.
         constexpr int kHalves = D == 256 ? 2 : 1;
-        const int boxes = kUnit / a.box, side = lane / (boxes * kHalves), within = lane % (boxes * kHalves);
-        const bool has_box = side < 2;
-        const CacheSide& s = a.side[has_box ? side : 0];
-        const int box_row = (within / kHalves) * a.box, half = within % kHalves;
+        const int boxes = kUnit / a.box * kHalves, box = lane % boxes, side = lane / boxes & 1, own_unit = lane / boxes >> 1;
+        const int box_row = box / kHalves * a.box, half = box % kHalves;
         const uint32_t box_bytes = static_cast<uint32_t>(a.box) * (D == 64 ? 64u : 128u);
         const uint32_t to = side * S::kSide + half * (kUnit * 128) + box_row * (D == 64 ? 64 : 128);
-        auto locate = [&](int unit, int& page, int& token) {
-            const int key = unit * kUnit + box_row, slot = static_cast<int>(fast_divide(static_cast<uint32_t>(key >> 4), a.by_page));
-            token = key - slot * a.page;
-            page = has_box ? page_of(a, s, batch, slot) : -1;
+        const int scale_unit = lane >> 2 & 3, scale_side = lane >> 1 & 1, scale_run = lane & 1;
+        const int scale_from = (scale_unit * 2 + scale_side) * boxes + scale_run * 16 / a.box * kHalves;   // the lane that has the scale's page
+        struct Batch {
+            int entry, head, unit, count, lo, hi;   // count: 0 after the last
+            int page, token;                        // of this lane's box
         };
-        int page, token;
-        locate(chunk_first, page, token);
-        const SequenceWindow window = sequence_window(a, batch);
-        int lo, hi;
-        window_of_tokens(a, window, row_first / a.group, (min(row_first + ROW_WARPS * kRows, a.rows) - 1) / a.group, lo, hi);
-        const int first = max(chunk_first, lo / kUnit), end = hi > lo ? min(chunk_first + a.units_per_cta, (hi + kUnit - 1) / kUnit) : 0;
-        if (first != chunk_first && first < end) locate(first, page, token);
+        int u = 0, take = 0;
+        auto following = [&](Batch& b) {   // the next four units, or what is left of their list
+            if (u >= take) {
+                if (take > 0) walk.taken(a, take);
+                u = 0;
+                if (!walk.next(a, take)) take = 0;
+            }
+            b.count = min(kBatch, take - u);
+            b.entry = walk.entry, b.head = walk.head, b.lo = walk.lo, b.hi = walk.hi;
+            b.unit = walk.lo / kUnit + walk.offset + u;
+            b.page = -1, b.token = 0;
+            if (own_unit < b.count) {
+                const int key = (b.unit + own_unit) * kUnit + box_row, at = static_cast<int>(fast_divide(static_cast<uint32_t>(key >> 4), a.by_page));
+                b.token = key - at * a.page;
+                if (key < b.hi && key + a.box > b.lo) b.page = page_of(a, a.side[side], b.entry / a.row_blocks, at);
+            }
+            u += kBatch;
+        };
+        auto scale_of = [&](const Batch& b) {
+            const int page = __shfl_sync(0xffffffffu, b.page, scale_from), token = __shfl_sync(0xffffffffu, b.token, scale_from) + scale_run * 16 % a.box;
+            const int key = (b.unit + scale_unit) * kUnit + scale_run * 16;
+            if (lane >= 16 || page < 0 || key >= b.hi || key + 16 <= b.lo) return -1;
+            const CacheSide& s = a.side[scale_side];
+            return static_cast<int>(s.scales[page * s.scale_stride[0] + b.head * s.scale_stride[1] + fast_divide(static_cast<uint32_t>(token >> 4), a.by_tokens) * s.scale_stride[2]]);
+        };
+        Batch now, next, later;
+        following(now);
+        following(next);
+        int code = scale_of(now);
         int slot = 0;
         uint32_t turn = 1;
-        for (int u = first; u < end; ++u) {
-            const int key = u * kUnit + box_row;
-            const bool live = page >= 0 && key < hi && key + a.box > lo;
-            const int now_page = page, now_token = token;
-            if (u + 1 < end) locate(u + 1, page, token);
-            if (!mbar_wait_warp(empty(slot), turn, 701)) break;
-            const uint32_t count = __popc(__ballot_sync(0xffffffffu, live));
-            if (lane == 0) mbar_expect_tx(full(slot), count * box_bytes);   // (also the arrival; no byte where no page is)
+        const uint32_t of_unit = own_unit < kBatch ? ((1u << (2 * boxes)) - 1u) << (2 * boxes * own_unit) : 0u;   // the lanes with this unit's boxes (2, 4 or 8)
+        const bool first_of_unit = own_unit < kBatch && lane % (2 * boxes) == 0;
+        while (now.count > 0) {
+            following(later);
+            const int next_code = scale_of(next);
+            // the slots of this lane's box and of its scale, free when all four units' are
+            const int box_slot = slot + own_unit < S::kSlots ? slot + own_unit : slot + own_unit - S::kSlots, scale_slot = slot + scale_unit < S::kSlots ? slot + scale_unit : slot + scale_unit - S::kSlots;
+            const bool mine = own_unit < now.count;
+            const uint32_t bar = full(mine ? box_slot : slot), living = __ballot_sync(0xffffffffu, now.page >= 0);
+            if (!mbar_wait_warp(mine ? empty(box_slot) : empty(slot), mine && slot + own_unit >= S::kSlots ? turn ^ 1 : turn, 701)) break;
+            if (first_of_unit && mine) mbar_expect_tx(bar, __popc(living & of_unit) * box_bytes);   // (also the first arrival; no byte where no page is)
             __syncwarp();
-            if (live) tma_load_4d(ring + slot * (2 * S::kSide) + to, side ? &map_v : &map_k, half * 128, now_token, head, now_page, full(slot));
-            if (++slot == S::kSlots) slot = 0, turn ^= 1;
+            if (now.page >= 0) tma_load_4d(ring + box_slot * (2 * S::kSide) + to, side ? &map_v : &map_k, half * 128, now.token, now.head, now.page, bar);
+            if (lane < 16 && scale_unit < now.count) {   // the other arrivals, behind the scales
+                reinterpret_cast<float*>(smem + S::kScales + scale_slot * 16)[lane & 3] = scale_side ? __int_as_float(code) : code < 0 ? -1.0f : decode_e8m0(static_cast<uint32_t>(code));
+                mbar_arrive(full(scale_slot));
+            }
+            __syncwarp();
+            slot += now.count;
+            if (slot >= S::kSlots) slot -= S::kSlots, turn ^= 1;
+            now = next, next = later, code = next_code;
         }
         return;
     }
 
     const int quad = lane & 3, eighth = lane >> 2, row_warp = warp % ROW_WARPS, group = warp / ROW_WARPS;
-    const SequenceWindow window = sequence_window(a, batch);
-    // The keys that any row of the CTA sees, and this CTA's units among them.
-    int lo, hi;
-    window_of_tokens(a, window, row_first / a.group, (min(row_first + ROW_WARPS * kRows, a.rows) - 1) / a.group, lo, hi);
-    const int first_unit = max(chunk_first, lo / kUnit), end_unit = hi > lo ? min(chunk_first + a.units_per_cta, (hi + kUnit - 1) / kUnit) : 0;
-    const int units = end_unit - first_unit;
-    if (units <= 0 && a.chunks > 1) return;   // (the merge knows which chunks a row has)
-
-    // The scales of the runs of 16 keys.
-    for (int i = threadIdx.x; i < 4 * units; i += kConsumers) {
-        const bool is_v = i >= 2 * units;
-        const CacheSide& s = a.side[is_v ? 1 : 0];
-        const int run = is_v ? i - 2 * units : i, key = first_unit * kUnit + run * 16;
-        const int slot = static_cast<int>(fast_divide(static_cast<uint32_t>(key >> 4), a.by_page)), block = static_cast<int>(fast_divide(static_cast<uint32_t>((key - slot * a.page) >> 4), a.by_tokens));
-        const int page = key < hi && key + 16 > lo ? page_of(a, s, batch, slot) : -1;
-        const int code = page >= 0 ? s.scales[page * s.scale_stride[0] + head * s.scale_stride[1] + block * s.scale_stride[2]] : -1;
-        if (is_v) v_scales[run] = code;
-        else k_scales[run] = page >= 0 ? decode_e8m0(static_cast<uint32_t>(code)) : -1.0f;
-    }
-
-    Rows rows;
-    const int own_row = row_first + row_warp * kRows;
-    auto place_of = [&](int row, int& token, int& head_q) {   // of a row that there is
-        token = row / a.group;
-        head_q = head * a.group + (row - token * a.group);
-    };
-    int common_lo = lo, common_hi = hi, any_lo = hi, any_hi = lo;   // what the warp's rows see in common, and what any of them sees
-#pragma unroll
-    for (int n = 0; n < EIGHTS; ++n) {
-        // Q of row `eighth`: this quarter of its channels
-        const int row = own_row + n * 8 + eighth;
-        int token = 0, head_q = 0;
-        if (row < a.rows) place_of(row, token, head_q);
-        const T* from = static_cast<const T*>(a.q) + batch * a.q_stride[0] + head_q * a.q_stride[1] + token * a.q_stride[2];
-        float v[Rows::kDeep][4];
-        float largest = 0.0f;
-#pragma unroll
-        for (int i = 0; i < Rows::kDeep; ++i) {
-            const int channel = D == 64 ? quad * 16 + i * 4 : (quad * 2 + ((i >> 2) & 1) + (i >> 3) * 8) * 16 + (i & 3) * 4;
-            struct alignas(8) Four { T v[4]; } four{};
-            if (row < a.rows) {
-                if (a.q_vector) four = *reinterpret_cast<const Four*>(from + channel);
-                else four = Four{{from[channel], from[channel + 1], from[channel + 2], from[channel + 3]}};
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                v[i][e] = value_of(four.v[e]);
-                largest = fmaxf(largest, fabsf(v[i][e]));
-            }
-        }
-        largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-        largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-        int up = 14 - (static_cast<int>(__float_as_uint(largest) >> 23) - 127);
-        up = largest == 0.0f ? 0 : min(max(up, -126), 126);
-        const float power = power_of_two(up), factor = power_of_two(-up) * a.scale_log2;
-#pragma unroll
-        for (int i = 0; i < Rows::kDeep; ++i) {
-            rows.q[i][n][0] = two_halves(v[i][0] * power, v[i][1] * power);
-            rows.q[i][n][1] = two_halves(v[i][2] * power, v[i][3] * power);
-        }
-        // rows 2 quad and 2 quad + 1
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            rows.factor[n][c] = __shfl_sync(0xffffffffu, factor, (quad * 2 + c) * 4);
-            const int column = own_row + n * 8 + quad * 2 + c;
-            const bool there = column < a.rows && column / a.group < window.len_q;
-            rows.row_lo[n][c] = lo, rows.row_hi[n][c] = hi;      // (rows without a part see what the others see; their results go nowhere)
-            if (there) {
-                window_of_tokens(a, window, column / a.group, column / a.group, rows.row_lo[n][c], rows.row_hi[n][c]);
-                any_lo = min(any_lo, rows.row_lo[n][c]);
-                any_hi = max(any_hi, rows.row_hi[n][c]);
-            }
-            rows.row_hi[n][c] = max(rows.row_hi[n][c], rows.row_lo[n][c]);
-            common_lo = max(common_lo, rows.row_lo[n][c]);
-            common_hi = min(common_hi, rows.row_hi[n][c]);
-            rows.largest[n][c] = -INFINITY;
-            rows.sum[n][c] = 0.0f;
-        }
-    }
-    rows.unit = kNoUnit;
-#pragma unroll
-    for (int j = 0; j < kWide; ++j)
-#pragma unroll
-        for (int n = 0; n < EIGHTS; ++n)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) rows.o[j][n][c] = 0.0f;
-    common_lo = __reduce_max_sync(0xffffffffu, common_lo), common_hi = __reduce_min_sync(0xffffffffu, common_hi);
-    any_lo = __reduce_min_sync(0xffffffffu, any_lo), any_hi = __reduce_max_sync(0xffffffffu, any_hi);
-    asm volatile("bar.sync 1, 128;" ::: "memory");   // the scales are there
-
     bool ok = true;
-    for (int u = group; u < units; u += kGroups) {
-        const int slot = u % S::kSlots;
-        ok = mbar_wait_warp(full(slot), (u / S::kSlots) & 1, 702);
-        if (!ok) break;
-        const uint8_t* k_unit = smem + slot * (2 * S::kSide);
-        const int key0 = (first_unit + u) * kUnit;
-        const float* k_scale = k_scales + 2 * u;
-        const int* v_scale = v_scales + 2 * u;
-        if (key0 < any_hi && key0 + kUnit > any_lo) {
-            const bool special = key0 < common_lo || key0 + kUnit > common_hi || fminf(k_scale[0], k_scale[1]) < 0.0f ||
-                                 max(static_cast<uint32_t>(v_scale[0]), static_cast<uint32_t>(v_scale[1])) > 254u;
-            if (special) rows.template step<true>(k_unit, k_unit + S::kSide, k_scale, v_scale, key0, lo, hi, a.seq_q > 1);
-            else rows.template step<false>(k_unit, k_unit + S::kSide, k_scale, v_scale, key0, lo, hi, false);
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(empty(slot));
-    }
-    ok = ok && g_device_status == 0;
-
-    // The warps with the same rows meet: (largest score, sum, O) triples by shared memory, in the order of the fragments, so that each bank
-    // is met once. Each of them then has pairs of channels of its own: place i of [eight][row of two][pair] with i * groups / places == group.
-    constexpr int kPlaces = EIGHTS * 2 * kWide;
-    const float absolute = rows.unit == kNoUnit ? 1.0f : decode_e8m0(static_cast<uint32_t>(rows.unit));
+    int behind = 0, take;      // units of the lists before
+    for (; walk.next(a, take); behind += take, walk.taken(a, take)) {
+        const int64_t batch = walk.entry / a.row_blocks;
+        const int row_first = (walk.entry - static_cast<int>(batch) * a.row_blocks) * a.block_rows, lo = walk.lo, hi = walk.hi, head = walk.head;
+        const SequenceWindow window = sequence_window(a, batch);
+        const bool whole = walk.offset == 0 && take == walk.units;
+        if (threadIdx.x == 0 && walk.offset == 0) a.starts[1 + static_cast<int64_t>(walk.entry) * a.heads_kv + head] = whole ? -1 : static_cast<int64_t>(blockIdx.x) * per + behind;
+        Rows rows;
+        const int own_row = row_first + row_warp * kRows;
+        auto place_of = [&](int row, int& token, int& head_q) {   // of a row that there is
+            token = row / a.group;
+            head_q = head * a.group + (row - token * a.group);
+        };
+        int common_lo = lo, common_hi = hi, any_lo = hi, any_hi = lo;   // what the warp's rows see in common, and what any of them sees
 #pragma unroll
-    for (int n = 0; n < EIGHTS; ++n) {
+        for (int n = 0; n < EIGHTS; ++n) {
+            // Q of row `eighth`: this quarter of its channels
+            const int row = own_row + n * 8 + eighth;
+            int token = 0, head_q = 0;
+            if (row < a.rows) place_of(row, token, head_q);
+            const T* from = static_cast<const T*>(a.q) + batch * a.q_stride[0] + head_q * a.q_stride[1] + token * a.q_stride[2];
+            float v[Rows::kDeep][4];
+            float largest = 0.0f;
+#pragma unroll
+            for (int i = 0; i < Rows::kDeep; ++i) {
+                const int channel = D == 64 ? quad * 16 + i * 4 : (quad * 2 + ((i >> 2) & 1) + (i >> 3) * 8) * 16 + (i & 3) * 4;
+                struct alignas(8) Four { T v[4]; } four{};
+                if (row < a.rows) {
+                    if (a.q_vector) four = *reinterpret_cast<const Four*>(from + channel);
+                    else four = Four{{from[channel], from[channel + 1], from[channel + 2], from[channel + 3]}};
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    v[i][e] = value_of(four.v[e]);
+                    largest = fmaxf(largest, fabsf(v[i][e]));
+                }
+            }
+            largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+            largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+            int up = 14 - (static_cast<int>(__float_as_uint(largest) >> 23) - 127);
+            up = largest == 0.0f ? 0 : min(max(up, -126), 126);
+            const float power = power_of_two(up), factor = power_of_two(-up) * a.scale_log2;
+#pragma unroll
+            for (int i = 0; i < Rows::kDeep; ++i) {
+                rows.q[i][n][0] = two_halves(v[i][0] * power, v[i][1] * power);
+                rows.q[i][n][1] = two_halves(v[i][2] * power, v[i][3] * power);
+            }
+            // rows 2 quad and 2 quad + 1
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                rows.factor[n][c] = __shfl_sync(0xffffffffu, factor, (quad * 2 + c) * 4);
+                const int column = own_row + n * 8 + quad * 2 + c;
+                const bool there = column < a.rows && column / a.group < window.len_q;
+                rows.row_lo[n][c] = lo, rows.row_hi[n][c] = hi;      // (rows without a part see what the others see; their results go nowhere)
+                if (there) {
+                    window_of_tokens(a, window, column / a.group, column / a.group, rows.row_lo[n][c], rows.row_hi[n][c]);
+                    any_lo = min(any_lo, rows.row_lo[n][c]);
+                    any_hi = max(any_hi, rows.row_hi[n][c]);
+                }
+                rows.row_hi[n][c] = max(rows.row_hi[n][c], rows.row_lo[n][c]);
+                common_lo = max(common_lo, rows.row_lo[n][c]);
+                common_hi = min(common_hi, rows.row_hi[n][c]);
+                rows.largest[n][c] = -INFINITY;
+                rows.sum[n][c] = 0.0f;
+            }
+        }
+        rows.unit = kNoUnit;
 #pragma unroll
         for (int j = 0; j < kWide; ++j)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) rows.o[j][n][c] *= absolute;
+            for (int n = 0; n < EIGHTS; ++n)
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int x = 4; x < 32; x <<= 1) rows.sum[n][c] += __shfl_xor_sync(0xffffffffu, rows.sum[n][c], x);
-    }
-    if constexpr (kGroups > 1) {
-        asm volatile("bar.sync 1, 128;" ::: "memory");   // (every unit has come and been read)
-        float2* fragments = reinterpret_cast<float2*>(smem);                 // [warp][places][32]
-        float2* meeting = reinterpret_cast<float2*>(smem + S::kKScales);     // [warp][eight][row of two][quad]
-#pragma unroll
-        for (int n = 0; n < EIGHTS; ++n)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                if (eighth == 0) meeting[((warp * EIGHTS + n) * 2 + c) * 4 + quad] = make_float2(rows.largest[n][c], rows.sum[n][c]);
-#pragma unroll
-                for (int j = 0; j < kWide; ++j) fragments[((warp * EIGHTS * 2 + n * 2 + c) * kWide + j) * 32 + lane] = make_float2(rows.o[j][n][c], rows.o[j][n][c + 2]);
+                for (int c = 0; c < 4; ++c) rows.o[j][n][c] = 0.0f;
+        common_lo = __reduce_max_sync(0xffffffffu, common_lo), common_hi = __reduce_min_sync(0xffffffffu, common_hi);
+        any_lo = __reduce_min_sync(0xffffffffu, any_lo), any_hi = __reduce_max_sync(0xffffffffu, any_hi);
+
+        // (on a wait that gave up, walk on without units: the warps meet at their barriers)
+        for (int u = (group - behind) & (kGroups - 1); u < take; u += kGroups) {
+            const int nth = behind + u, slot = nth % S::kSlots;
+            if (ok) ok = mbar_wait_warp(full(slot), (nth / S::kSlots) & 1, 702);
+            if (!ok) continue;
+            const uint8_t* k_unit = smem + slot * (2 * S::kSide);
+            const float* k_scale = reinterpret_cast<const float*>(smem + S::kScales + slot * 16);
+            const int* v_scale = reinterpret_cast<const int*>(k_scale + 2);
+            const int key0 = (lo / kUnit + walk.offset + u) * kUnit;
+            if (key0 < any_hi && key0 + kUnit > any_lo) {
+                const bool special = key0 < common_lo || key0 + kUnit > common_hi || fminf(k_scale[0], k_scale[1]) < 0.0f ||
+                                     max(static_cast<uint32_t>(v_scale[0]), static_cast<uint32_t>(v_scale[1])) > 254u;
+                if (special) rows.template step<true>(k_unit, k_unit + S::kSide, k_scale, v_scale, key0, lo, hi, a.seq_q > 1);
+                else rows.template step<false>(k_unit, k_unit + S::kSide, k_scale, v_scale, key0, lo, hi, false);
             }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(empty(slot));
+        }
+
+        // The warps with the same rows meet: (largest score, sum, O) triples by shared memory, one row of two of an eight at a time, in the
+        // order of the fragments, so that each bank is met once. Each warp then has pairs of channels of its own: j * groups / pairs == group.
+        const float absolute = rows.unit == kNoUnit ? 1.0f : decode_e8m0(static_cast<uint32_t>(rows.unit));
 #pragma unroll
-        for (int n = 0; n < EIGHTS; ++n)
+        for (int n = 0; n < EIGHTS; ++n) {
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                float2 other[kGroups];
-                float top = -INFINITY, total = 0.0f;
+            for (int j = 0; j < kWide; ++j)
 #pragma unroll
-                for (int g = 0; g < kGroups; ++g) {
-                    other[g] = meeting[(((g * ROW_WARPS + row_warp) * EIGHTS + n) * 2 + c) * 4 + quad];
-                    top = fmaxf(top, other[g].x);
-                }
+                for (int c = 0; c < 4; ++c) rows.o[j][n][c] *= absolute;
 #pragma unroll
-                for (int g = 0; g < kGroups; ++g) {
-                    other[g].x = other[g].x == -INFINITY ? 1.0f : exp2_of(other[g].x - top);   // (a group without keys has zeros)
-                    total = fmaf(other[g].y, other[g].x, total);
-                }
-                rows.largest[n][c] = top, rows.sum[n][c] = total;
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
-                for (int j = 0; j < kWide; ++j) {
-                    if (((n * 2 + c) * kWide + j) * kGroups / kPlaces != group) continue;
-                    float2 v = make_float2(0.0f, 0.0f);
+                for (int x = 4; x < 32; x <<= 1) rows.sum[n][c] += __shfl_xor_sync(0xffffffffu, rows.sum[n][c], x);
+        }
+        if constexpr (kGroups > 1) {
+            float2* fragments = reinterpret_cast<float2*>(smem + S::kFragments);
+            float2* meeting = reinterpret_cast<float2*>(smem + S::kMeeting);
+#pragma unroll
+            for (int n = 0; n < EIGHTS; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    asm volatile("bar.sync 1, 128;" ::: "memory");   // (what was there before has been read)
+                    if (eighth == 0) meeting[((warp * EIGHTS + n) * 2 + c) * 4 + quad] = make_float2(rows.largest[n][c], rows.sum[n][c]);
+#pragma unroll
+                    for (int j = 0; j < kWide; ++j)
+                        if (j * kGroups / kWide != group) fragments[(warp * kWide + j) * 32 + lane] = make_float2(rows.o[j][n][c], rows.o[j][n][c + 2]);
+                    asm volatile("bar.sync 1, 128;" ::: "memory");
+                    float2 other[kGroups];
+                    float top = -INFINITY, total = 0.0f, own_weight = 0.0f;
 #pragma unroll
                     for (int g = 0; g < kGroups; ++g) {
-                        const float2 part = fragments[(((g * ROW_WARPS + row_warp) * EIGHTS * 2 + n * 2 + c) * kWide + j) * 32 + lane];
-                        v.x = fmaf(part.x, other[g].x, v.x);
-                        v.y = fmaf(part.y, other[g].x, v.y);
+                        other[g] = meeting[(((g * ROW_WARPS + row_warp) * EIGHTS + n) * 2 + c) * 4 + quad];
+                        top = fmaxf(top, other[g].x);
                     }
-                    rows.o[j][n][c] = v.x, rows.o[j][n][c + 2] = v.y;
+#pragma unroll
+                    for (int g = 0; g < kGroups; ++g) {
+                        other[g].x = other[g].x == -INFINITY ? 1.0f : exp2_of(other[g].x - top);   // (a group without keys has zeros)
+                        total = fmaf(other[g].y, other[g].x, total);
+                        if (g == group) own_weight = other[g].x;
+                    }
+                    rows.largest[n][c] = top, rows.sum[n][c] = total;
+#pragma unroll
+                    for (int j = 0; j < kWide; ++j) {
+                        if (j * kGroups / kWide != group) continue;
+                        float2 v = make_float2(rows.o[j][n][c] * own_weight, rows.o[j][n][c + 2] * own_weight);
+#pragma unroll
+                        for (int g = 0; g < kGroups; ++g) {
+                            if (g == group) continue;
+                            const float2 part = fragments[((g * ROW_WARPS + row_warp) * kWide + j) * 32 + lane];
+                            v.x = fmaf(part.x, other[g].x, v.x);
+                            v.y = fmaf(part.y, other[g].x, v.y);
+                        }
+                        rows.o[j][n][c] = v.x, rows.o[j][n][c + 2] = v.y;
+                    }
+                }
+        }
+        if (!ok || g_device_status != 0) continue;
+#pragma unroll
+        for (int n = 0; n < EIGHTS; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int row = own_row + n * 8 + quad * 2 + c;
+                if (row >= a.rows) continue;
+                const float top = rows.largest[n][c], total = rows.sum[n][c];
+                if (!whole) {
+                    float* partial = a.partial + ((static_cast<int64_t>(blockIdx.x) * 2 + (walk.first ? 0 : 1)) * a.block_rows + (row - row_first)) * (D + 2);
+#pragma unroll
+                    for (int j = 0; j < kWide; ++j)
+                        if (j * kGroups / kWide == group)
+                            *reinterpret_cast<float2*>(partial + Rows::channel_of(j, eighth)) = make_float2(rows.o[j][n][c], rows.o[j][n][c + 2]);
+                    if (eighth == 0 && group == 0) *reinterpret_cast<float2*>(partial + D) = make_float2(top, total);
+                } else {
+                    int token, head_q;
+                    place_of(row, token, head_q);
+                    const bool none = token >= window.len_q || total == 0.0f;   // (a NaN sum is a NaN result)
+                    const float inverse = 1.0f / total;
+                    const int64_t at = batch * a.o_stride[0] + head_q * a.o_stride[1] + token * a.o_stride[2];
+#pragma unroll
+                    for (int j = 0; j < kWide; ++j)
+                        if (j * kGroups / kWide == group)
+                            store_pair(a, at + Rows::channel_of(j, eighth), none ? 0.0f : rows.o[j][n][c] * inverse, none ? 0.0f : rows.o[j][n][c + 2] * inverse);
+                    if (eighth == 0 && group == 0 && a.stats)
+                        a.stats[batch * a.stats_stride[0] + head_q * a.stats_stride[1] + token * a.stats_stride[2]] = none ? -INFINITY : top * kLn2 + logf(total * 0x1p-15f);
                 }
             }
     }
-    if (!ok) return;
-#pragma unroll
-    for (int n = 0; n < EIGHTS; ++n)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            const int row = own_row + n * 8 + quad * 2 + c;
-            if (row >= a.rows) continue;
-            const float top = rows.largest[n][c], total = rows.sum[n][c];
-            if (a.chunks > 1) {
-                float* partial = a.partial + (((batch * a.heads_kv + head) * a.rows + row) * a.chunks + blockIdx.x) * (D + 2);
-#pragma unroll
-                for (int j = 0; j < kWide; ++j)
-                    if (((n * 2 + c) * kWide + j) * kGroups / kPlaces == group)
-                        *reinterpret_cast<float2*>(partial + Rows::channel_of(j, eighth)) = make_float2(rows.o[j][n][c], rows.o[j][n][c + 2]);
-                if (eighth == 0 && group == 0) *reinterpret_cast<float2*>(partial + D) = make_float2(top, total);
-            } else {
-                int token, head_q;
-                place_of(row, token, head_q);
-                const bool none = token >= window.len_q || total == 0.0f;   // (a NaN sum is a NaN result)
-                const float inverse = 1.0f / total;
-                const int64_t at = batch * a.o_stride[0] + head_q * a.o_stride[1] + token * a.o_stride[2];
-#pragma unroll
-                for (int j = 0; j < kWide; ++j)
-                    if (((n * 2 + c) * kWide + j) * kGroups / kPlaces == group)
-                        store_pair(a, at + Rows::channel_of(j, eighth), none ? 0.0f : rows.o[j][n][c] * inverse, none ? 0.0f : rows.o[j][n][c + 2] * inverse);
-                if (eighth == 0 && group == 0 && a.stats)
-                    a.stats[batch * a.stats_stride[0] + head_q * a.stats_stride[1] + token * a.stats_stride[2]] = none ? -INFINITY : top * kLn2 + logf(total * 0x1p-15f);
-            }
-        }
 }
 
-// A CTA a row, a thread a channel. Latency-bound: maxima and sums of the first 32 chunks, a chunk a lane in every warp, and the values of
-// the first eight are on their way before the lengths say which of them the row has.
+// A CTA a row, a thread a channel: the rows of lists that were cut, and of those without keys. Latency-bound: the maxima and sums of 32 parts come at
+// once, a part a lane in every warp, together with their values.
 template <int D>
 __global__ void __launch_bounds__(D)
 cache_sdpa_merge_kernel(const __grid_constant__ CacheSdpaArgs a) {
-    constexpr int kAhead = 8;
     const int lane = threadIdx.x & 31;
-    const int64_t row = blockIdx.x, list = row / a.rows, batch = list / a.heads_kv;
-    const int in_list = static_cast<int>(row - list * a.rows), token = in_list / a.group;
-    const int head = static_cast<int>(list - batch * a.heads_kv) * a.group + (in_list - token * a.group);
-    const float* base = a.partial + row * a.chunks * (D + 2);
+    const int in_rows = static_cast<int>(blockIdx.x % a.rows), token = in_rows / a.group;
+    const int64_t list = blockIdx.x / a.rows, batch = list / a.heads_kv;
+    const int head_kv = static_cast<int>(list - batch * a.heads_kv), head = head_kv * a.group + (in_rows - token * a.group);
+    const int block = in_rows / a.block_rows, row = in_rows - block * a.block_rows, entry = static_cast<int>(batch) * a.row_blocks + block;
     chain_begin();
-    float ahead[kAhead];
+    const int64_t per = a.starts[0], start = a.starts[1 + static_cast<int64_t>(entry) * a.heads_kv + head_kv];   // (written where the list has keys)
+    int lo, hi;
+    const int units = units_of(a, entry, lo, hi);
+    const bool takes_part = token < sequence_window(a, batch).len_q;
+    float top = -INFINITY, total = 0.0f, value = 0.0f;
+    if (units > 0) {
+        if (start < 0) return;   // not cut: its CTA has written O
+        const int64_t first = start / per;
+        const int parts = static_cast<int>((start + units - 1) / per - first) + 1;
+        const bool second_place = start != first * per;   // of the first part in its CTA
+        auto part_of = [&](int i) { return a.partial + (((first + i) * 2 + (i == 0 && second_place ? 1 : 0)) * a.block_rows + row) * (D + 2); };
+        for (int i0 = 0; i0 < parts; i0 += 32) {
+            float ahead[32];
 #pragma unroll
-    for (int c = 0; c < kAhead; ++c) ahead[c] = c < a.chunks ? base[c * (D + 2) + threadIdx.x] : 0.0f;
-    float2 first_pair = lane < a.chunks ? *reinterpret_cast<const float2*>(base + lane * (D + 2) + D) : make_float2(-INFINITY, 0.0f);
-    const SequenceWindow window = sequence_window(a, batch);
-    int lo = 0, hi = 0;
-    if (token < window.len_q) window_of_tokens(a, window, token, token, lo, hi);
-    const int keys = a.units_per_cta * kUnit;
-    const int first = lo / keys, end = hi > lo ? (hi + keys - 1) / keys : first;
-    auto pair_of = [&](int c) {   // (largest score, sum); a chunk without keys of the row was perhaps not written
-        if (c < first || c >= end) return make_float2(-INFINITY, 0.0f);
-        return c == lane ? first_pair : *reinterpret_cast<const float2*>(base + c * (D + 2) + D);
-    };
-    float top = -INFINITY;
-    for (int c = lane; c < end; c += 32) top = fmaxf(top, pair_of(c).x);
+            for (int k = 0; k < 32; ++k) ahead[k] = i0 + k < parts ? part_of(i0 + k)[threadIdx.x] : 0.0f;
+            float2 pair = make_float2(-INFINITY, 0.0f);
+            if (i0 + lane < parts) pair = *reinterpret_cast<const float2*>(part_of(i0 + lane) + D);
+            float largest = fmaxf(top, pair.x);
 #pragma unroll
-    for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-    float total = 0.0f, value = 0.0f;
-    for (int c0 = 0; c0 < end; c0 += 32) {
-        const float2 pair = pair_of(c0 + lane);
-        const float weight = pair.x == -INFINITY ? 1.0f : exp2_of(pair.x - top);   // (no score above -inf: its values are zeros, or NaNs that are to be seen)
-        float part = pair.y * weight;
+            for (int s = 16; s > 0; s >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, s));
+            const float down = top == -INFINITY ? 1.0f : exp2_of(top - largest);   // (no score above -inf: zeros, or NaNs that are to be seen)
+            const float weight = pair.x == -INFINITY ? 1.0f : exp2_of(pair.x - largest);
+            top = largest;
+            float part = pair.y * weight;
 #pragma unroll
-        for (int s = 16; s > 0; s >>= 1) part += __shfl_xor_sync(0xffffffffu, part, s);
-        total += part;
+            for (int s = 16; s > 0; s >>= 1) part += __shfl_xor_sync(0xffffffffu, part, s);
+            total = fmaf(total, down, part);
+            value *= down;
 #pragma unroll
-        for (int c = 0; c < 32; c += kAhead) {
-            if (c0 + c >= end) break;
-#pragma unroll
-            for (int k = 0; k < kAhead; ++k) {
-                const float w = __shfl_sync(0xffffffffu, weight, c + k);
-                if (c0 + c + k >= first && c0 + c + k < end) value = fmaf(ahead[k], w, value);
-            }
-#pragma unroll
-            for (int k = 0; k < kAhead; ++k) {
-                const int next = c0 + c + kAhead + k;
-                if (next >= first && next < end) ahead[k] = base[next * (D + 2) + threadIdx.x];
+            for (int k = 0; k < 32; ++k) {
+                const float w = __shfl_sync(0xffffffffu, weight, k);
+                if (i0 + k < parts) value = fmaf(ahead[k], w, value);
             }
         }
     }
-    const bool none = total == 0.0f;
+    const bool none = !takes_part || total == 0.0f;
     store_from_f32(a.o, a.o_type, batch * a.o_stride[0] + head * a.o_stride[1] + token * a.o_stride[2] + threadIdx.x, none ? 0.0f : value / total);
     if (threadIdx.x == 0 && a.stats) a.stats[batch * a.stats_stride[0] + head * a.stats_stride[1] + token * a.stats_stride[2]] = none ? -INFINITY : top * kLn2 + logf(total * 0x1p-15f);
 }
 
 struct StreamPlan {
-    int eights, row_warps, row_blocks, units_per_cta, chunks;
-    int64_t rows, scratch;
+    int eights, row_warps, block_rows, row_blocks;
+    int64_t rows, grid, starts, scratch;   // starts: integers before the partial results
 };
 
 StreamPlan plan_stream(const dfgpu_cache_sdpa_params& p) {
@@ -643,20 +742,13 @@ StreamPlan plan_stream(const dfgpu_cache_sdpa_params& p) {
     plan.rows = group * p.q.dim[2];
     plan.eights = plan.rows <= 8 ? 1 : 2;
     plan.row_warps = plan.rows <= 16 ? 1 : plan.rows <= 32 ? 2 : 4;
-    const int block = plan.eights * 8 * plan.row_warps;
-    plan.row_blocks = static_cast<int>((plan.rows + block - 1) / block);
-    const int64_t units = (p.s_kv + kUnit - 1) / kUnit, lists = p.q.dim[0] * p.k.dim[1] * plan.row_blocks;
-    // Units that a CTA's rows can see: a left bound and its last row's right one leave a band of them.
-    int64_t seen = units;
-    if (p.has_left_bound && p.has_right_bound && p.left_bound + p.right_bound >= 0 && p.left_bound < p.s_kv && p.right_bound < p.s_kv)
-        seen = std::min(units, (p.left_bound + p.right_bound + std::min<int64_t>(p.q.dim[2], block)) / kUnit + 1);
-    // Long runs of units save prologues and partial results (the more the more rows there are), short ones give a small batch more
-    // CTAs: as long as there are three for every two SMs (148: a function of the shape alone, as the scratch is).
-    int per_cta = std::min(kMostUnits, 32 * plan.row_warps);
-    while (per_cta > 4 && 2 * lists * ((seen + per_cta - 1) / per_cta) < 3 * 148) per_cta /= 2;
-    plan.units_per_cta = per_cta;
-    plan.chunks = static_cast<int>((units + per_cta - 1) / per_cta);
-    plan.scratch = plan.chunks > 1 ? p.q.dim[0] * p.k.dim[1] * plan.rows * plan.chunks * (d + 2) * 4 : 0;
+    plan.block_rows = plan.eights * 8 * plan.row_warps;
+    plan.row_blocks = static_cast<int>((plan.rows + plan.block_rows - 1) / plan.block_rows);
+    const int64_t lists = p.q.dim[0] * p.k.dim[1] * plan.row_blocks, units = (p.s_kv + kUnit - 1) / kUnit;
+    const int64_t ctas = kSms * (d == 256 ? (plan.eights == 1 ? 2 : 1) : plan.eights == 1 ? 3 : 2);   // (Shape::kCtas)
+    plan.grid = std::min(ctas, (lists * units + kLeastUnits - 1) / kLeastUnits);
+    plan.starts = (1 + lists + 1) / 2 * 2;
+    plan.scratch = plan.starts * 8 + plan.grid * 2 * plan.block_rows * (d + 2) * 4;
     return plan;
 }
 
@@ -704,7 +796,7 @@ int check_cache_sdpa(const dfgpu_cache_sdpa_params& p, int& kernel) {
         return fail(kInvalidShape, "CACHE_SDPA: Stats must be FLOAT [B, Hq, Sq, 1]");
     if (!std::isfinite(p.attn_scale)) return fail(kInvalidValue, "CACHE_SDPA: the attention scale must be finite");
     const StreamPlan plan = plan_stream(p);
-    if (p.q.dim[0] > 65535 || p.k.dim[1] * plan.row_blocks > 65535 || p.q.dim[2] >= (1ll << 30) || p.q.dim[0] * p.k.dim[1] * plan.rows >= (1ll << 31)) return fail(kUnsupported, "CACHE_SDPA: too many sequences, heads or query rows");
+    if (p.q.dim[2] >= (1ll << 30) || p.q.dim[0] * p.k.dim[1] * plan.rows >= (1ll << 31)) return fail(kUnsupported, "CACHE_SDPA: too many sequences, heads or query rows");
     if (p.kernel < DFGPU_CACHE_SDPA_AUTO || p.kernel > DFGPU_CACHE_SDPA_STREAM) return fail(kInvalidArgument, "CACHE_SDPA: unknown kernel id %d", p.kernel);
     kernel = DFGPU_CACHE_SDPA_STREAM;
     return kOk;
@@ -741,8 +833,8 @@ int launch_stream(const CUtensorMap& map_k, const CUtensorMap& map_v, const Cach
                        : plan.row_warps == 1 ? launch_rows<T, D, 2, 1>(map_k, map_v, a, grid, stream)
                        : plan.row_warps == 2 ? launch_rows<T, D, 2, 2>(map_k, map_v, a, grid, stream)
                                              : launch_rows<T, D, 2, 4>(map_k, map_v, a, grid, stream);
-    if (status || plan.chunks == 1) return status;
-    launch_chained(cache_sdpa_merge_kernel<D>, dim3(static_cast<unsigned>(static_cast<int64_t>(grid.z) * a.heads_kv * a.rows)), dim3(D), 0, stream, a);
+    if (status) return status;
+    launch_chained(cache_sdpa_merge_kernel<D>, dim3(static_cast<unsigned>(static_cast<int64_t>(a.entries / a.row_blocks) * a.heads_kv * a.rows)), dim3(D), 0, stream, a);
     return check_launch("CACHE_SDPA merge");
 }
 
@@ -758,7 +850,7 @@ extern "C" int dfgpu_query_cache_sdpa(const dfgpu_cache_sdpa_params* p, dfgpu_pl
     if (status) return status;
     const StreamPlan plan = plan_stream(*p);
     info->kernel = kernel;
-    info->launches = plan.chunks > 1 ? 2 : 1;
+    info->launches = 2;
     info->scratch_bytes = plan.scratch;
     return kOk;
 }
@@ -778,7 +870,7 @@ extern "C" int dfgpu_cache_sdpa(const dfgpu_cache_sdpa_params* p, void* const* t
         return fail(kInvalidArgument, "CACHE_SDPA: Q or O is not aligned to its type");
     for (int i : {4, 7, 8, 9, 10})
         if ((reinterpret_cast<uintptr_t>(tensors[i]) & 3u) != 0) return fail(kInvalidArgument, "CACHE_SDPA: port %d is not aligned to its type", i);
-    if (plan.scratch && (!scratch || !on_16(scratch))) return fail(kInvalidArgument, "CACHE_SDPA: needs the 16-byte aligned scratch dfgpu_query_cache_sdpa reports");
+    if (!scratch || !on_16(scratch)) return fail(kInvalidArgument, "CACHE_SDPA: needs the 16-byte aligned scratch dfgpu_query_cache_sdpa reports");
     CacheSdpaArgs a{};
     a.q = tensors[0];
     a.o = tensors[3];
@@ -829,15 +921,17 @@ extern "C" int dfgpu_cache_sdpa(const dfgpu_cache_sdpa_params* p, void* const* t
     a.left = std::min(std::max(p->left_bound, -far), far);
     a.right = std::min(std::max(p->right_bound, -far), far);
     a.scale_log2 = p->attn_scale * 1.4426950408889634f;
-    a.chunks = plan.chunks;
-    a.units_per_cta = plan.units_per_cta;
-    a.partial = static_cast<float*>(scratch);
+    a.row_blocks = plan.row_blocks;
+    a.block_rows = plan.block_rows;
+    a.entries = static_cast<int>(p->q.dim[0] * plan.row_blocks);
+    a.starts = static_cast<int64_t*>(scratch);
+    a.partial = reinterpret_cast<float*>(a.starts + plan.starts);
     a.box = a.page % 32 == 0 ? 32 : 16;
     CUtensorMap map_k, map_v;
     int made = make_side_map(&map_k, p->k, tensors[1], a.box);
     if (!made) made = make_side_map(&map_v, p->v, tensors[2], a.box);
     if (made) return made;
-    const dim3 grid(static_cast<unsigned>(plan.chunks), static_cast<unsigned>(a.heads_kv * plan.row_blocks), static_cast<unsigned>(p->q.dim[0]));
+    const dim3 grid(static_cast<unsigned>(plan.grid));
     cudaStream_t on = as_stream(stream);
     const bool half = p->q.dtype == DFGPU_F16;
     switch (p->q.dim[3]) {

@@ -155,10 +155,9 @@ def test_sdpa_refusals():
         assert error.value.code == 1 and f"port {i}" in str(error.value)
     with pytest.raises(dfgpu.DfgpuError):
         cache.cache_sdpa(sdpa_params(), [16, 24] + good[2:], 256)
-    long = sdpa_params(s_kv=128 * 64, page_table_k=tensor(I32, [2, 1, 256, 1]), page_table_v=tensor(I32, [2, 1, 256, 1]))
-    assert cache.query("cache_sdpa", long).scratch_bytes > 0
+    assert cache.query("cache_sdpa", sdpa_params()).scratch_bytes > 0
     with pytest.raises(dfgpu.DfgpuError) as error:
-        cache.cache_sdpa(long, good, None)
+        cache.cache_sdpa(sdpa_params(), good, None)
     assert "scratch" in str(error.value)
 
 

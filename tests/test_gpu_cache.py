@@ -348,6 +348,12 @@ def test_long_contexts_and_many_chunks(lengths, hk):
     attend_case(len(lengths), F16, 64, hk, 2, 3, 64, 16, lengths, right=0, bottom_right=True, left=3000)
 
 
+@pytest.mark.parametrize("d,g,dtype", [(128, 2, BF16), (128, 12, BF16), (64, 4, F16), (256, 3, BF16), (256, 16, F16)])
+def test_many_units_for_each_cta(d, g, dtype):
+    """Every CTA's ring goes round several times, over the ends of lists of very different lengths."""
+    attend_case(d + g, dtype, d, 8, g, 1, 64, 64, [9000, 100, 6000, 0, 12000, 33, 7000, 2000], right=0, bottom_right=True)
+
+
 def test_scales_far_apart():
     """Neighbouring blocks of V 2^60 apart, one of zeros with a scale of 1 beside tiny ones: nothing is lost to the larger scale."""
     def spoil(q, caches, scales, tables):
