@@ -17,11 +17,12 @@
 // Channels and keys may go to any index of a product as long as both operands agree; the ones taken here give each thread 16-byte
 // reads without bank conflicts: of K 32 consecutive channels of a key, of V 16 consecutive channels of four keys, and of O 16
 // consecutive channels of a row.
-// The work is one row of units of 32 keys, list by list (a sequence's block of rows, a KV head), cut into equal parts for the CTAs that are on
-// the chip together (three an SM for single tokens): lengths differ, and a grid of lists or of pieces of them pays for it with idle SMs
-// at the end and with a prologue for each piece. A fifth warp brings a CTA's units by TMA into a ring, across lists, so that the
-// next list's codes are on their way while O of the last one is written; four take them in turn, or in pairs or all of them with rows
-// of their own where there are more than 16. Lists that were cut leave partial results, which a second kernel merges.
+// The work is one row of units of 32 keys, list by list (a sequence, a KV head, a block of 8 or 16 rows), cut into equal parts for the WARPS that
+// are on the chip together, sixteen an SM for single tokens. A warp is on its own: it brings its units by TMA into a private ring of K and V
+// tiles, computes on them and refills each as soon as it has read it, so that nothing is shared and nobody waits for another warp. (CTAs
+// whose warps shared each list's units spent a third of their time on meeting and on beginning lists; a loading warp for four
+// others was what they waited for.) Lists that were cut leave partial results, which a second kernel merges. Rows beyond 16 are
+// lists of their own, whose keys come from L2.
 #include <algorithm>
 #include <cmath>
 
@@ -32,10 +33,9 @@
 namespace dfgpu {
 namespace {
 
-constexpr int kWarps = 4, kThreads = 160;
+constexpr int kWarps = 4, kThreads = 128;
 constexpr int kUnit = 32;          // keys that a warp takes at a time
-constexpr int kBatch = 4;          // units that the loader looks up at a time
-constexpr int kLeastUnits = 8;     // of a CTA: fewer cost more in prologues and partial results than they gain
+constexpr int kLeastUnits = 4;     // of a part: fewer cost more in prologues and partial results than they gain
 constexpr int kSms = 148;          // (the cut is a function of the shape and the lengths alone, as the scratch is of the shape)
 constexpr float kUp = 15.0f;       // probabilities are held as p * 2^15
 constexpr float kLn2 = 0.6931471805599453f;
@@ -45,20 +45,14 @@ constexpr int kNaN = 0x7fc00000;
 // EIGHTS: eights of rows that a warp takes.
 template <int D, int EIGHTS>
 struct Shape {
-    static constexpr int kCtas = D == 256 ? (EIGHTS == 1 ? 2 : 1) : EIGHTS == 1 ? 3 : 2;   // on an SM
-    static constexpr int kSide = kUnit * D;                                                // bytes of a unit's K or V
-    // A multiple of the warps, so that a slot's units are always the same warp's: it then knows one phase of the slot's barrier from the
-    // next. (With six slots a warp that was ahead took the phase before last, of another warp's unit, for its own.)
-    static constexpr int kSlots = (kCtas == 3 ? 64 : D == 256 ? (EIGHTS == 1 ? 64 : 192) : 96) * 1024 / (2 * kSide);
-    static_assert(kSlots % kWarps == 0, "a slot belongs to one warp");
-    static constexpr int kRing = kSlots * 2 * kSide;
-    static constexpr int kFragments = kRing;                                  // [warp][pairs of O][32] float2, of one row of two of an eight
-    static constexpr int kMeeting = kFragments + kWarps * (D / 16) * 32 * 8;  // [warp][eight][row of two][quad] float2
-    static constexpr int kScales = kMeeting + kWarps * EIGHTS * 2 * 4 * 8;    // [slot] K scales of its two runs of 16 keys as f32 (-1: the page's rows read as zeros), V's as codes (-1 likewise)
-    static constexpr int kBarriers = kScales + kSlots * 16;                   // full[slots], empty[slots]
-    static constexpr int kScan = kBarriers + 2 * kSlots * 8;                  // [warps] int64, then where the CTA begins
-    static constexpr int kTotal = kScan + 64 + 32;
+    static constexpr int kCtas = D == 256 ? 2 : EIGHTS == 1 ? 4 : 3;          // on an SM, by registers
+    static constexpr int kSide = kUnit * D;                                   // bytes of a unit's K or V
+    static constexpr int kSlots = D == 64 ? (EIGHTS == 1 ? 6 : 8) : D == 128 && EIGHTS == 2 ? 4 : 3;   // K and V tiles of a warp's ring
+    static constexpr int kRing = kWarps * kSlots * kSide;
+    static constexpr int kBarriers = kRing;                                   // [warp][slot]
+    static constexpr int kTotal = kBarriers + kWarps * kSlots * 8;
     static constexpr int kDynamic = kTotal + 1024;
+    static_assert(kCtas * (kDynamic + 1024) <= 228 * 1024, "CTAs an SM");
 };
 
 // Byte offset of a 16-byte chunk of a unit's row, as TMA lays rows of 128 or 64 bytes out (a D of 256: two halves): the reads above meet each bank once.
@@ -116,13 +110,6 @@ __device__ __forceinline__ void store_pair(const CacheSdpaArgs& a, int64_t at, f
     store_from_f32(a.o, a.o_type, at + 1, second);
 }
 
-// The page of a slot in a side's table, -1 where there is none.
-__device__ __forceinline__ int page_of(const CacheSdpaArgs& a, const CacheSide& s, int64_t batch, int slot) {
-    if (slot >= s.table_len) return -1;
-    const int page = s.table[batch * s.table_batch + slot * s.table_slot];
-    return page >= 0 && page < s.pages ? page : -1;
-}
-
 // EIGHTS * 8 rows against the codes of K and V that their warp takes. Thread (eighth, quad) = (lane / 4, lane % 4) has scores of keys
 // eighth and eighth + 8 of each 16, and O's channels channel_of(j) and the next one, both for rows 2 quad and 2 quad + 1 of each eight.
 template <int D, int EIGHTS>
@@ -138,9 +125,10 @@ struct RowTile {
 
     __device__ static __forceinline__ int channel_of(int j, int eighth) { return D == 64 ? eighth * 8 + 2 * j : (j >> 3) * 128 + eighth * 16 + 2 * (j & 7); }
 
-    // A unit of keys from key0 of the sequence on. SPECIAL: some row does not see all of them, or a page or scale is none.
+    // Probabilities of a unit of keys, from key0 of the sequence on. SPECIAL: some row does not see all of them, or a page or scale is none (k_scales of
+    // 16 keys each, -1 where the page's rows read as zeros).
     template <bool SPECIAL>
-    __device__ __forceinline__ void step(const uint8_t* k_unit, const uint8_t* v_unit, const float* k_scales, const int* v_scales, int key0, int lo, int hi, bool mixed) {
+    __device__ __forceinline__ void scores(const uint8_t* k_unit, const float (&k_scales)[2], int key0, uint32_t (&p)[2][EIGHTS][2]) {
         const int lane = threadIdx.x & 31, quad = lane & 3, eighth = lane >> 2;
         float s[2][EIGHTS][4];   // neighbouring products add to different ones
 #pragma unroll
@@ -198,7 +186,6 @@ struct RowTile {
                     for (int j = 0; j < kWide; ++j) o[j][n][c] *= down, o[j][n][c + 2] *= down;
                 }
         }
-        uint32_t p[2][EIGHTS][2];
 #pragma unroll
         for (int n = 0; n < EIGHTS; ++n) {
             const float from0 = largest[n][0] == -INFINITY ? 0.0f : kUp - largest[n][0], from1 = largest[n][1] == -INFINITY ? 0.0f : kUp - largest[n][1];
@@ -211,6 +198,12 @@ struct RowTile {
                 p[r][n][1] = transposed(two_halves(p2, p3));
             }
         }
+    }
+
+    // Their values to O (v_scales: codes, -1 likewise). [lo, hi): the keys that any row sees.
+    template <bool SPECIAL>
+    __device__ __forceinline__ void values(const uint8_t* v_unit, const int (&v_scales)[2], int key0, int lo, int hi, bool mixed, uint32_t (&p)[2][EIGHTS][2]) {
+        const int lane = threadIdx.x & 31, quad = lane & 3, eighth = lane >> 2;
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
             const int code = v_scales[r], apart = code - unit;   // (the same in all threads)
@@ -319,221 +312,158 @@ __device__ __forceinline__ int units_of(const CacheSdpaArgs& a, int entry, int& 
     return hi > lo ? (hi + kUnit - 1) / kUnit - lo / kUnit : 0;
 }
 
-// A CTA's way through the lists: entry, KV head, the next unit of the list and how many of the CTA's are left.
-struct Walk {
-    int entry, head, offset, left;
-    int lo, hi, units;      // of the entry
-    bool first;             // nothing has been taken yet
-
-    // The next piece of a list, `take` units from unit `offset` on; false after the last. Every lane of a warp walks alike. Entries without
-    // keys are passed over 32 at a time.
-    __device__ __forceinline__ bool next(const CacheSdpaArgs& a, int& take) {
-        if (left <= 0) return false;
-        while (units == 0) {
-            const int lane = threadIdx.x & 31;
-            int from = 0, until = 0;
-            const int n = entry + lane < a.entries ? units_of(a, entry + lane, from, until) : 0;
-            const uint32_t some = __ballot_sync(0xffffffffu, n > 0);
-            if (some == 0) {
-                entry += 32;
-                if (entry >= a.entries) return false;
-                continue;
-            }
-            const int found = __ffs(some) - 1;
-            entry += found;
-            lo = __shfl_sync(0xffffffffu, from, found), hi = __shfl_sync(0xffffffffu, until, found), units = __shfl_sync(0xffffffffu, n, found);
-        }
-        take = min(units - offset, left);
-        return true;
-    }
-    __device__ __forceinline__ void taken(const CacheSdpaArgs& a, int take) {
-        left -= take;
-        offset = 0;
-        first = false;
-        if (++head == a.heads_kv) head = 0, ++entry, units = 0;
-    }
-};
-
-// ROW_WARPS: warps with rows of their own.
-template <typename T, int D, int EIGHTS, int ROW_WARPS>
+template <typename T, int D, int EIGHTS>
 __global__ void __launch_bounds__(kThreads, Shape<D, EIGHTS>::kCtas)
 cache_sdpa_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CacheSdpaArgs a) {
     using S = Shape<D, EIGHTS>;
     using Rows = RowTile<D, EIGHTS>;
-    constexpr int kGroups = kWarps / ROW_WARPS;       // warps that take units in turn
     constexpr int kWide = Rows::kWide, kRows = EIGHTS * 8;
     extern __shared__ uint8_t raw_smem[];
-    const uint32_t ring = (smem_u32(raw_smem) + 1023u) & ~1023u;
-    uint8_t* smem = raw_smem + (ring - smem_u32(raw_smem));
-    auto full = [&](int s) { return ring + S::kBarriers + 8u * s; };
-    auto empty = [&](int s) { return ring + S::kBarriers + 8u * (S::kSlots + s); };
-    const int warp = uniform_warp_index(), lane = threadIdx.x & 31;
-    if (threadIdx.x == 0) {
+    const uint32_t base = (smem_u32(raw_smem) + 1023u) & ~1023u;
+    uint8_t* smem = raw_smem + (base - smem_u32(raw_smem));
+    const int warp = uniform_warp_index(), lane = threadIdx.x & 31, quad = lane & 3, eighth = lane >> 2;
+    const uint32_t bars = base + S::kBarriers + warp * (S::kSlots * 8), ring = base + warp * (S::kSlots * S::kSide);
+    const uint8_t* ring_data = smem + warp * (S::kSlots * S::kSide);
+    if (lane == 0) {
         prefetch_tensormap(&map_k);
         prefetch_tensormap(&map_v);
-        for (int s = 0; s < S::kSlots; ++s) {
-            mbar_init(full(s), 5);            // the loader's bytes, four scales
-            mbar_init(empty(s), ROW_WARPS);
-        }
+        for (int s = 0; s < S::kSlots; ++s) mbar_init(bars + 8u * s, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     chain_begin();
 
-    // All units before those of this thread's entries, and their number: where this CTA's part begins.
-    Walk walk{};
-    int per;
+    // The units before each lane's entries, and all of them (fewer than 2^30): where the warp's part begins. (Every warp for itself: the lengths come
+    // from L1 for the later ones, and a pass over a few of them is shorter than a barrier of the CTA.)
+    const int each = (a.entries + 31) / 32, from = min(lane * each, a.entries), until = min(from + each, a.entries);
+    int own = 0, lo = 0, hi = 0;
+    for (int e = from; e < until; ++e) own += units_of(a, e, lo, hi);
+    own *= a.heads_kv;
+    int up_to = own;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+        const int other = __shfl_up_sync(0xffffffffu, up_to, x);
+        if (lane >= x) up_to += other;
+    }
+    const int all = __shfl_sync(0xffffffffu, up_to, 31);
+    const int warps = static_cast<int>(gridDim.x) * kWarps, per = max((all + warps - 1) / warps, kLeastUnits);
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.starts[0] = per;
+    // Neighbouring parts go to different SMs: with fewer parts than warps all SMs have some.
+    const int part = warp * static_cast<int>(gridDim.x) + static_cast<int>(blockIdx.x);
+    if (part >= (all + per - 1) / per) return;
+    int left = min(per, all - part * per), entry, head, offset, units = 0;
+    bool first_piece = true;
     {
-        int64_t* sums = reinterpret_cast<int64_t*>(smem + S::kScan);
-        int* begin = reinterpret_cast<int*>(smem + S::kScan + 64);
-        const int each = (a.entries + kThreads - 1) / kThreads, from = min(static_cast<int>(threadIdx.x) * each, a.entries), until = min(from + each, a.entries);
-        int64_t own = 0;
-        int lo, hi;
-        for (int e = from; e < until; ++e) own += units_of(a, e, lo, hi);
-        own *= a.heads_kv;
-        int64_t up_to = own;
-#pragma unroll
-        for (int x = 1; x < 32; x <<= 1) {
-            const int64_t other = __shfl_up_sync(0xffffffffu, up_to, x);
-            if (lane >= x) up_to += other;
-        }
-        if (lane == 31) sums[warp] = up_to;
-        __syncthreads();
-        int64_t all = 0, before = up_to - own;
-#pragma unroll
-        for (int w = 0; w <= kWarps; ++w) {
-            if (w < warp) before += sums[w];
-            all += sums[w];
-        }
-        per = max(static_cast<int>((all + gridDim.x - 1) / gridDim.x), kLeastUnits);
-        if (blockIdx.x == 0 && threadIdx.x == 0) a.starts[0] = per;
-        int64_t start = static_cast<int64_t>(blockIdx.x) * per;
-        walk.left = static_cast<int>(max(min(static_cast<int64_t>(per), all - start), static_cast<int64_t>(0)));
-        if (walk.left > 0 && start >= before && start < before + own) {
-            start -= before;
-            for (int e = from; e < until; ++e) {
-                const int n = units_of(a, e, lo, hi);
-                if (start < static_cast<int64_t>(n) * a.heads_kv) {
-                    begin[0] = e, begin[1] = static_cast<int>(start / n), begin[2] = static_cast<int>(start % n);
-                    break;
-                }
-                start -= static_cast<int64_t>(n) * a.heads_kv;
+        const int start = part * per, found = __ffs(__ballot_sync(0xffffffffu, up_to > start)) - 1;   // the lane with the part's first entry
+        int rest = start - (up_to - own);
+        entry = from;
+        if (lane == found)
+            for (;; ++entry) {
+                units = units_of(a, entry, lo, hi);
+                if (rest < units * a.heads_kv) break;
+                rest -= units * a.heads_kv;
             }
-        }
-        __syncthreads();
-        if (walk.left <= 0) return;
-        walk.entry = begin[0], walk.head = begin[1], walk.offset = begin[2];
-        walk.first = true;
+        entry = __shfl_sync(0xffffffffu, entry, found), units = __shfl_sync(0xffffffffu, units, found), rest = __shfl_sync(0xffffffffu, rest, found);
+        lo = __shfl_sync(0xffffffffu, lo, found), hi = __shfl_sync(0xffffffffu, hi, found);
+        head = rest / units;
+        offset = rest - head * units;
     }
 
-    if (warp == kWarps) {
-        // The loader looks up four units at a time: lane l has one box of one of them, `box` rows (16 or 32 of a page) of K or V by 128 or 64 bytes, and
-        // the first sixteen lanes one of their scales each. Page ids are read two batches ahead of their use, scales one.
-        constexpr int kHalves = D == 256 ? 2 : 1;
-        const int boxes = kUnit / a.box * kHalves, box = lane % boxes, side = lane / boxes & 1, own_unit = lane / boxes >> 1;
-        const int box_row = box / kHalves * a.box, half = box % kHalves;
-        const uint32_t box_bytes = static_cast<uint32_t>(a.box) * (D == 64 ? 64u : 128u);
-        const uint32_t to = side * S::kSide + half * (kUnit * 128) + box_row * (D == 64 ? 64 : 128);
-        const int scale_unit = lane >> 2 & 3, scale_side = lane >> 1 & 1, scale_run = lane & 1;
-        const int scale_from = (scale_unit * 2 + scale_side) * boxes + scale_run * 16 / a.box * kHalves;   // the lane that has the scale's page
-        struct Batch {
-            int entry, head, unit, count, lo, hi;   // count: 0 after the last
-            int page, token;                        // of this lane's box
-        };
-        int u = 0, take = 0;
-        auto following = [&](Batch& b) {   // the next four units, or what is left of their list
-            if (u >= take) {
-                if (take > 0) walk.taken(a, take);
-                u = 0;
-                if (!walk.next(a, take)) take = 0;
-            }
-            b.count = min(kBatch, take - u);
-            b.entry = walk.entry, b.head = walk.head, b.lo = walk.lo, b.hi = walk.hi;
-            b.unit = walk.lo / kUnit + walk.offset + u;
-            b.page = -1, b.token = 0;
-            if (own_unit < b.count) {
-                const int key = (b.unit + own_unit) * kUnit + box_row, at = static_cast<int>(fast_divide(static_cast<uint32_t>(key >> 4), a.by_page));
-                b.token = key - at * a.page;
-                if (key < b.hi && key + a.box > b.lo) b.page = page_of(a, a.side[side], b.entry / a.row_blocks, at);
-            }
-            u += kBatch;
-        };
-        auto scale_of = [&](const Batch& b) {
-            const int page = __shfl_sync(0xffffffffu, b.page, scale_from), token = __shfl_sync(0xffffffffu, b.token, scale_from) + scale_run * 16 % a.box;
-            const int key = (b.unit + scale_unit) * kUnit + scale_run * 16;
-            if (lane >= 16 || page < 0 || key >= b.hi || key + 16 <= b.lo) return -1;
-            const CacheSide& s = a.side[scale_side];
-            return static_cast<int>(s.scales[page * s.scale_stride[0] + b.head * s.scale_stride[1] + fast_divide(static_cast<uint32_t>(token >> 4), a.by_tokens) * s.scale_stride[2]]);
-        };
-        Batch now, next, later;
-        following(now);
-        following(next);
-        int code = scale_of(now);
-        int slot = 0;
-        uint32_t turn = 1;
-        const uint32_t of_unit = own_unit < kBatch ? ((1u << (2 * boxes)) - 1u) << (2 * boxes * own_unit) : 0u;   // the lanes with this unit's boxes (2, 4 or 8)
-        const bool first_of_unit = own_unit < kBatch && lane % (2 * boxes) == 0;
-        while (now.count > 0) {
-            following(later);
-            const int next_code = scale_of(next);
-            // the slots of this lane's box and of its scale, free when all four units' are
-            const int box_slot = slot + own_unit < S::kSlots ? slot + own_unit : slot + own_unit - S::kSlots, scale_slot = slot + scale_unit < S::kSlots ? slot + scale_unit : slot + scale_unit - S::kSlots;
-            const bool mine = own_unit < now.count;
-            const uint32_t bar = full(mine ? box_slot : slot), living = __ballot_sync(0xffffffffu, now.page >= 0);
-            if (!mbar_wait_warp(mine ? empty(box_slot) : empty(slot), mine && slot + own_unit >= S::kSlots ? turn ^ 1 : turn, 701)) break;
-            if (first_of_unit && mine) mbar_expect_tx(bar, __popc(living & of_unit) * box_bytes);   // (also the first arrival; no byte where no page is)
-            __syncwarp();
-            if (now.page >= 0) tma_load_4d(ring + box_slot * (2 * S::kSide) + to, side ? &map_v : &map_k, half * 128, now.token, now.head, now.page, bar);
-            if (lane < 16 && scale_unit < now.count) {   // the other arrivals, behind the scales
-                reinterpret_cast<float*>(smem + S::kScales + scale_slot * 16)[lane & 3] = scale_side ? __int_as_float(code) : code < 0 ? -1.0f : decode_e8m0(static_cast<uint32_t>(code));
-                mbar_arrive(full(scale_slot));
-            }
-            __syncwarp();
-            slot += now.count;
-            if (slot >= S::kSlots) slot -= S::kSlots, turn ^= 1;
-            now = next, next = later, code = next_code;
+    constexpr int kHalves = D == 256 ? 2 : 1, kAhead = 16;   // units a look-up
+    const int boxes = kUnit / a.box;                         // of `box` keys, 16 or 32 of a page
+    const uint32_t box_bytes = static_cast<uint32_t>(a.box) * (D == 64 ? 64u : 128u);
+    int tiles = 0;   // K and V tiles of the pieces before: tile t is in slot t % kSlots, in phase t / kSlots of its barrier
+    for (;;) {
+        while (units == 0) {   // entries without keys, 32 at a time
+            int from = 0, until = 0;
+            const int n = entry + lane < a.entries ? units_of(a, entry + lane, from, until) : 0;
+            const uint32_t some = __ballot_sync(0xffffffffu, n > 0);
+            const int which = some ? __ffs(some) - 1 : 32;
+            entry += which;
+            if (some) units = __shfl_sync(0xffffffffu, n, which), lo = __shfl_sync(0xffffffffu, from, which), hi = __shfl_sync(0xffffffffu, until, which);
         }
-        return;
-    }
+        const int take = min(units - offset, left), unit0 = lo / kUnit + offset;
+        const int64_t batch = entry / a.row_blocks;
+        const int row_first = (entry - static_cast<int>(batch) * a.row_blocks) * a.block_rows;
+        const bool whole = offset == 0 && take == units;
+        if (lane == 0 && offset == 0) a.starts[1 + static_cast<int64_t>(entry) * a.heads_kv + head] = whole ? -1 : min((part + 1) * per, all) - left;
 
-    const int quad = lane & 3, eighth = lane >> 2, row_warp = warp % ROW_WARPS, group = warp / ROW_WARPS;
-    bool ok = true;
-    int behind = 0, take;      // units of the lists before
-    for (; walk.next(a, take); behind += take, walk.taken(a, take)) {
-        const int64_t batch = walk.entry / a.row_blocks;
-        const int row_first = (walk.entry - static_cast<int>(batch) * a.row_blocks) * a.block_rows, lo = walk.lo, hi = walk.hi, head = walk.head;
-        const SequenceWindow window = sequence_window(a, batch);
-        const bool whole = walk.offset == 0 && take == walk.units;
-        if (threadIdx.x == 0 && walk.offset == 0) a.starts[1 + static_cast<int64_t>(walk.entry) * a.heads_kv + head] = whole ? -1 : static_cast<int64_t>(blockIdx.x) * per + behind;
+        // Of sixteen units, lane l has the table's entries of box l and the scales of the l-th 16 keys. Whether an entry is a page is asked when
+        // it is used: a comparison here would wait for it.
+        int page[2], page_next[2] = {-1, -1}, code[2] = {-1, -1}, code_next[2];   // K, V
+        auto look_up = [&](int from, int (&to)[2]) {
+            const int key = (unit0 + from) * kUnit + lane * a.box, slot = static_cast<int>(fast_divide(static_cast<uint32_t>(key >> 4), a.by_page));
+            const bool in = lane < kAhead * boxes && from + lane / boxes < take && key < hi && key + a.box > lo;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) to[w] = in && slot < a.side[w].table_len ? a.side[w].table[batch * a.side[w].table_batch + slot * a.side[w].table_slot] : -1;
+        };
+        auto is_page = [&](int id, int w) { return id >= 0 && id < a.side[w].pages; };
+        auto look_up_scales = [&](int from) {
+            const int key = (unit0 + from) * kUnit + lane * 16, token = key - static_cast<int>(fast_divide(static_cast<uint32_t>(key >> 4), a.by_page)) * a.page;
+            const int64_t block = fast_divide(static_cast<uint32_t>(token >> 4), a.by_tokens);
+            const bool in = from + (lane >> 1) < take && key < hi && key + 16 > lo;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+                const CacheSide& s = a.side[w];
+                const int id = __shfl_sync(0xffffffffu, page[w], lane * 16 / a.box);
+                code_next[w] = in && is_page(id, w) ? s.scales[id * s.scale_stride[0] + head * s.scale_stride[1] + block * s.scale_stride[2]] : -1;
+            }
+        };
+        // Brings tile t of the piece, K (t even) or V of unit t / 2: in order, each as soon as its slot has been read.
+        auto fetch = [&](int t) {
+            if (t >= 2 * take) return;
+            const int u = t >> 1, w = t & 1, slot = (tiles + t) % S::kSlots;
+            if (w == 0 && u > 0 && u % kAhead == 0) {
+                page[0] = page_next[0], page[1] = page_next[1];
+                look_up(u + kAhead, page_next);
+                look_up_scales(u);
+            }
+            const int box = lane / kHalves, half = lane % kHalves, key = (unit0 + u) * kUnit + box * a.box;
+            const int id = __shfl_sync(0xffffffffu, page[w], (u % kAhead) * boxes + (box & 1));
+            const bool live = box < boxes && is_page(id, w);
+            const uint32_t count = __popc(__ballot_sync(0xffffffffu, live)), bar = bars + 8u * slot;
+            if (lane == 0) mbar_expect_tx(bar, count * box_bytes);   // (also the arrival; no byte where no page is)
+            __syncwarp();
+            if (live) {
+                const int token = key - static_cast<int>(fast_divide(static_cast<uint32_t>(key >> 4), a.by_page)) * a.page;
+                tma_load_4d(ring + slot * S::kSide + half * (kUnit * 128) + box * a.box * (D == 64 ? 64 : 128), w ? &map_v : &map_k, half * 128, token, head, id, bar);
+            }
+            __syncwarp();
+        };
+        look_up(0, page);
+        look_up(kAhead, page_next);
+        look_up_scales(0);
+#pragma unroll 1
+        for (int t = 0; t < S::kSlots; ++t) fetch(t);
+
         Rows rows;
-        const int own_row = row_first + row_warp * kRows;
+        const SequenceWindow window = sequence_window(a, batch);
         auto place_of = [&](int row, int& token, int& head_q) {   // of a row that there is
-            token = row / a.group;
+            token = static_cast<int>(fast_divide(static_cast<uint32_t>(row), a.by_group));
             head_q = head * a.group + (row - token * a.group);
         };
-        int common_lo = lo, common_hi = hi, any_lo = hi, any_hi = lo;   // what the warp's rows see in common, and what any of them sees
+        int common_lo = lo, common_hi = hi, any_lo = hi, any_hi = lo;   // what the rows see in common, and what any of them sees
 #pragma unroll
         for (int n = 0; n < EIGHTS; ++n) {
             // Q of row `eighth`: this quarter of its channels
-            const int row = own_row + n * 8 + eighth;
+            const int row = row_first + n * 8 + eighth;
             int token = 0, head_q = 0;
             if (row < a.rows) place_of(row, token, head_q);
             const T* from = static_cast<const T*>(a.q) + batch * a.q_stride[0] + head_q * a.q_stride[1] + token * a.q_stride[2];
-            float v[Rows::kDeep][4];
-            float largest = 0.0f;
+            struct alignas(8) Four { T v[4]; } v[Rows::kDeep];
 #pragma unroll
             for (int i = 0; i < Rows::kDeep; ++i) {
                 const int channel = D == 64 ? quad * 16 + i * 4 : (quad * 2 + ((i >> 2) & 1) + (i >> 3) * 8) * 16 + (i & 3) * 4;
-                struct alignas(8) Four { T v[4]; } four{};
+                v[i] = Four{};
                 if (row < a.rows) {
-                    if (a.q_vector) four = *reinterpret_cast<const Four*>(from + channel);
-                    else four = Four{{from[channel], from[channel + 1], from[channel + 2], from[channel + 3]}};
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    v[i][e] = value_of(four.v[e]);
-                    largest = fmaxf(largest, fabsf(v[i][e]));
+                    if (a.q_vector) v[i] = *reinterpret_cast<const Four*>(from + channel);
+                    else v[i] = Four{{from[channel], from[channel + 1], from[channel + 2], from[channel + 3]}};
                 }
             }
+            float largest = 0.0f;
+#pragma unroll
+            for (int i = 0; i < Rows::kDeep; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) largest = fmaxf(largest, fabsf(value_of(v[i].v[e])));
             largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
             largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
             int up = 14 - (static_cast<int>(__float_as_uint(largest) >> 23) - 127);
@@ -541,27 +471,36 @@ cache_sdpa_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
             const float power = power_of_two(up), factor = power_of_two(-up) * a.scale_log2;
 #pragma unroll
             for (int i = 0; i < Rows::kDeep; ++i) {
-                rows.q[i][n][0] = two_halves(v[i][0] * power, v[i][1] * power);
-                rows.q[i][n][1] = two_halves(v[i][2] * power, v[i][3] * power);
+                rows.q[i][n][0] = two_halves(value_of(v[i].v[0]) * power, value_of(v[i].v[1]) * power);
+                rows.q[i][n][1] = two_halves(value_of(v[i].v[2]) * power, value_of(v[i].v[3]) * power);
             }
             // rows 2 quad and 2 quad + 1
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 rows.factor[n][c] = __shfl_sync(0xffffffffu, factor, (quad * 2 + c) * 4);
-                const int column = own_row + n * 8 + quad * 2 + c;
-                const bool there = column < a.rows && column / a.group < window.len_q;
+                const int column = row_first + n * 8 + quad * 2 + c;
                 rows.row_lo[n][c] = lo, rows.row_hi[n][c] = hi;      // (rows without a part see what the others see; their results go nowhere)
-                if (there) {
-                    window_of_tokens(a, window, column / a.group, column / a.group, rows.row_lo[n][c], rows.row_hi[n][c]);
-                    any_lo = min(any_lo, rows.row_lo[n][c]);
-                    any_hi = max(any_hi, rows.row_hi[n][c]);
+                if (a.seq_q > 1) {
+                    int of, head_of;
+                    place_of(column, of, head_of);
+                    if (column < a.rows && of < window.len_q) {
+                        window_of_tokens(a, window, of, of, rows.row_lo[n][c], rows.row_hi[n][c]);
+                        any_lo = min(any_lo, rows.row_lo[n][c]);
+                        any_hi = max(any_hi, rows.row_hi[n][c]);
+                    }
+                    rows.row_hi[n][c] = max(rows.row_hi[n][c], rows.row_lo[n][c]);
+                    common_lo = max(common_lo, rows.row_lo[n][c]);
+                    common_hi = min(common_hi, rows.row_hi[n][c]);
                 }
-                rows.row_hi[n][c] = max(rows.row_hi[n][c], rows.row_lo[n][c]);
-                common_lo = max(common_lo, rows.row_lo[n][c]);
-                common_hi = min(common_hi, rows.row_hi[n][c]);
                 rows.largest[n][c] = -INFINITY;
                 rows.sum[n][c] = 0.0f;
             }
+        }
+        if (a.seq_q > 1) {
+            common_lo = __reduce_max_sync(0xffffffffu, common_lo), common_hi = __reduce_min_sync(0xffffffffu, common_hi);
+            any_lo = __reduce_min_sync(0xffffffffu, any_lo), any_hi = __reduce_max_sync(0xffffffffu, any_hi);
+        } else {
+            any_lo = lo, any_hi = hi;
         }
         rows.unit = kNoUnit;
 #pragma unroll
@@ -570,99 +509,67 @@ cache_sdpa_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
             for (int n = 0; n < EIGHTS; ++n)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) rows.o[j][n][c] = 0.0f;
-        common_lo = __reduce_max_sync(0xffffffffu, common_lo), common_hi = __reduce_min_sync(0xffffffffu, common_hi);
-        any_lo = __reduce_min_sync(0xffffffffu, any_lo), any_hi = __reduce_max_sync(0xffffffffu, any_hi);
 
-        // (on a wait that gave up, walk on without units: the warps meet at their barriers)
-        for (int u = (group - behind) & (kGroups - 1); u < take; u += kGroups) {
-            const int nth = behind + u, slot = nth % S::kSlots;
-            if (ok) ok = mbar_wait_warp(full(slot), (nth / S::kSlots) & 1, 702);
-            if (!ok) continue;
-            const uint8_t* k_unit = smem + slot * (2 * S::kSide);
-            const float* k_scale = reinterpret_cast<const float*>(smem + S::kScales + slot * 16);
-            const int* v_scale = reinterpret_cast<const int*>(k_scale + 2);
-            const int key0 = (lo / kUnit + walk.offset + u) * kUnit;
-            if (key0 < any_hi && key0 + kUnit > any_lo) {
-                const bool special = key0 < common_lo || key0 + kUnit > common_hi || fminf(k_scale[0], k_scale[1]) < 0.0f ||
-                                     max(static_cast<uint32_t>(v_scale[0]), static_cast<uint32_t>(v_scale[1])) > 254u;
-                if (special) rows.template step<true>(k_unit, k_unit + S::kSide, k_scale, v_scale, key0, lo, hi, a.seq_q > 1);
-                else rows.template step<false>(k_unit, k_unit + S::kSide, k_scale, v_scale, key0, lo, hi, false);
+        bool ok = true;
+#pragma unroll 1
+        for (int u = 0; u < take; ++u) {
+            if (u % kAhead == 0) code[0] = code_next[0], code[1] = code_next[1];
+            float k_scale[2];
+            int v_scale[2];
+            const int key0 = (unit0 + u) * kUnit;
+            bool special = key0 < common_lo || key0 + kUnit > common_hi;
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                const int k_code = __shfl_sync(0xffffffffu, code[0], (u % kAhead) * 2 + r);
+                v_scale[r] = __shfl_sync(0xffffffffu, code[1], (u % kAhead) * 2 + r);
+                k_scale[r] = k_code < 0 ? -1.0f : decode_e8m0(static_cast<uint32_t>(k_code));
+                special = special || k_code < 0 || static_cast<uint32_t>(v_scale[r]) > 254u;
+            }
+            const bool seen = key0 < any_hi && key0 + kUnit > any_lo;
+            uint32_t p[2][EIGHTS][2];
+            const int k_slot = (tiles + 2 * u) % S::kSlots, v_slot = (tiles + 2 * u + 1) % S::kSlots;
+            ok = mbar_wait_warp(bars + 8u * k_slot, ((tiles + 2 * u) / S::kSlots) & 1, 702);
+            if (!ok) break;
+            if (seen) {
+                if (special) rows.template scores<true>(ring_data + k_slot * S::kSide, k_scale, key0, p);
+                else rows.template scores<false>(ring_data + k_slot * S::kSide, k_scale, key0, p);
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(empty(slot));
+            fetch(2 * u + S::kSlots);
+            ok = mbar_wait_warp(bars + 8u * v_slot, ((tiles + 2 * u + 1) / S::kSlots) & 1, 703);
+            if (!ok) break;
+            if (seen) {
+                if (special) rows.template values<true>(ring_data + v_slot * S::kSide, v_scale, key0, lo, hi, a.seq_q > 1, p);
+                else rows.template values<false>(ring_data + v_slot * S::kSide, v_scale, key0, lo, hi, false, p);
+            }
+            __syncwarp();
+            fetch(2 * u + 1 + S::kSlots);
+        }
+        if (!ok || g_device_status != 0) {
+            // A wait gave up, here or elsewhere: what is on its way comes first, so that nothing lands in another CTA's shared memory (each of these waits is
+            // bounded too).
+            for (int s = 0; s < S::kSlots && !ok; ++s) {
+                mbar_wait_warp(bars + 8u * s, 0, 704);
+                mbar_wait_warp(bars + 8u * s, 1, 704);
+            }
+            return;
         }
 
-        // The warps with the same rows meet: (largest score, sum, O) triples by shared memory, one row of two of an eight at a time, in the
-        // order of the fragments, so that each bank is met once. Each warp then has pairs of channels of its own: j * groups / pairs == group.
         const float absolute = rows.unit == kNoUnit ? 1.0f : decode_e8m0(static_cast<uint32_t>(rows.unit));
-#pragma unroll
-        for (int n = 0; n < EIGHTS; ++n) {
-#pragma unroll
-            for (int j = 0; j < kWide; ++j)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) rows.o[j][n][c] *= absolute;
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-                for (int x = 4; x < 32; x <<= 1) rows.sum[n][c] += __shfl_xor_sync(0xffffffffu, rows.sum[n][c], x);
-        }
-        if constexpr (kGroups > 1) {
-            float2* fragments = reinterpret_cast<float2*>(smem + S::kFragments);
-            float2* meeting = reinterpret_cast<float2*>(smem + S::kMeeting);
-#pragma unroll
-            for (int n = 0; n < EIGHTS; ++n)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    asm volatile("bar.sync 1, 128;" ::: "memory");   // (what was there before has been read)
-                    if (eighth == 0) meeting[((warp * EIGHTS + n) * 2 + c) * 4 + quad] = make_float2(rows.largest[n][c], rows.sum[n][c]);
-#pragma unroll
-                    for (int j = 0; j < kWide; ++j)
-                        if (j * kGroups / kWide != group) fragments[(warp * kWide + j) * 32 + lane] = make_float2(rows.o[j][n][c], rows.o[j][n][c + 2]);
-                    asm volatile("bar.sync 1, 128;" ::: "memory");
-                    float2 other[kGroups];
-                    float top = -INFINITY, total = 0.0f, own_weight = 0.0f;
-#pragma unroll
-                    for (int g = 0; g < kGroups; ++g) {
-                        other[g] = meeting[(((g * ROW_WARPS + row_warp) * EIGHTS + n) * 2 + c) * 4 + quad];
-                        top = fmaxf(top, other[g].x);
-                    }
-#pragma unroll
-                    for (int g = 0; g < kGroups; ++g) {
-                        other[g].x = other[g].x == -INFINITY ? 1.0f : exp2_of(other[g].x - top);   // (a group without keys has zeros)
-                        total = fmaf(other[g].y, other[g].x, total);
-                        if (g == group) own_weight = other[g].x;
-                    }
-                    rows.largest[n][c] = top, rows.sum[n][c] = total;
-#pragma unroll
-                    for (int j = 0; j < kWide; ++j) {
-                        if (j * kGroups / kWide != group) continue;
-                        float2 v = make_float2(rows.o[j][n][c] * own_weight, rows.o[j][n][c + 2] * own_weight);
-#pragma unroll
-                        for (int g = 0; g < kGroups; ++g) {
-                            if (g == group) continue;
-                            const float2 part = fragments[((g * ROW_WARPS + row_warp) * kWide + j) * 32 + lane];
-                            v.x = fmaf(part.x, other[g].x, v.x);
-                            v.y = fmaf(part.y, other[g].x, v.y);
-                        }
-                        rows.o[j][n][c] = v.x, rows.o[j][n][c + 2] = v.y;
-                    }
-                }
-        }
-        if (!ok || g_device_status != 0) continue;
 #pragma unroll
         for (int n = 0; n < EIGHTS; ++n)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const int row = own_row + n * 8 + quad * 2 + c;
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) rows.sum[n][c] += __shfl_xor_sync(0xffffffffu, rows.sum[n][c], x);
+                const int row = row_first + n * 8 + quad * 2 + c;
                 if (row >= a.rows) continue;
                 const float top = rows.largest[n][c], total = rows.sum[n][c];
                 if (!whole) {
-                    float* partial = a.partial + ((static_cast<int64_t>(blockIdx.x) * 2 + (walk.first ? 0 : 1)) * a.block_rows + (row - row_first)) * (D + 2);
+                    float* partial = a.partial + (static_cast<int64_t>(part * 2 + (first_piece ? 0 : 1)) * a.block_rows + (row - row_first)) * (D + 2);
 #pragma unroll
-                    for (int j = 0; j < kWide; ++j)
-                        if (j * kGroups / kWide == group)
-                            *reinterpret_cast<float2*>(partial + Rows::channel_of(j, eighth)) = make_float2(rows.o[j][n][c], rows.o[j][n][c + 2]);
-                    if (eighth == 0 && group == 0) *reinterpret_cast<float2*>(partial + D) = make_float2(top, total);
+                    for (int j = 0; j < kWide; ++j) *reinterpret_cast<float2*>(partial + Rows::channel_of(j, eighth)) = make_float2(rows.o[j][n][c] * absolute, rows.o[j][n][c + 2] * absolute);
+                    if (eighth == 0) *reinterpret_cast<float2*>(partial + D) = make_float2(top, total);
                 } else {
                     int token, head_q;
                     place_of(row, token, head_q);
@@ -671,69 +578,107 @@ cache_sdpa_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
                     const int64_t at = batch * a.o_stride[0] + head_q * a.o_stride[1] + token * a.o_stride[2];
 #pragma unroll
                     for (int j = 0; j < kWide; ++j)
-                        if (j * kGroups / kWide == group)
-                            store_pair(a, at + Rows::channel_of(j, eighth), none ? 0.0f : rows.o[j][n][c] * inverse, none ? 0.0f : rows.o[j][n][c + 2] * inverse);
-                    if (eighth == 0 && group == 0 && a.stats)
+                        store_pair(a, at + Rows::channel_of(j, eighth), none ? 0.0f : rows.o[j][n][c] * absolute * inverse, none ? 0.0f : rows.o[j][n][c + 2] * absolute * inverse);
+                    if (eighth == 0 && a.stats)
                         a.stats[batch * a.stats_stride[0] + head_q * a.stats_stride[1] + token * a.stats_stride[2]] = none ? -INFINITY : top * kLn2 + logf(total * 0x1p-15f);
                 }
             }
+        tiles += 2 * take;
+        left -= take;
+        if (left == 0) return;
+        offset = 0;
+        first_piece = false;
+        if (++head == a.heads_kv) head = 0, ++entry, units = 0;
     }
 }
 
-// A CTA a row, a thread a channel: the rows of lists that were cut, and of those without keys. Latency-bound: the maxima and sums of 32 parts come at
-// once, a part a lane in every warp, together with their values.
+// Loads where it stands: left to itself, the compiler moves each load of a run of them down to its use, and they come one after the other.
+__device__ __forceinline__ float2 load_now(const float* p) {
+    float2 v;
+    asm volatile("ld.global.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(__cvta_generic_to_global(p)) : "memory");
+    return v;
+}
+
+// A CTA a row: the rows of lists that were cut, and of those without keys. Latency-bound, so each warp has eight parts on their way at a time.
 template <int D>
 __global__ void __launch_bounds__(D)
 cache_sdpa_merge_kernel(const __grid_constant__ CacheSdpaArgs a) {
-    const int lane = threadIdx.x & 31;
+    constexpr int kWarpsHere = D / 32, kOwn = D / 32, kAhead = D == 256 ? 4 : 8;   // channels a lane, parts on their way a warp
+    __shared__ float2 meeting[kWarpsHere];
+    __shared__ __align__(16) float values[kWarpsHere][D];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int in_rows = static_cast<int>(blockIdx.x % a.rows), token = in_rows / a.group;
     const int64_t list = blockIdx.x / a.rows, batch = list / a.heads_kv;
     const int head_kv = static_cast<int>(list - batch * a.heads_kv), head = head_kv * a.group + (in_rows - token * a.group);
     const int block = in_rows / a.block_rows, row = in_rows - block * a.block_rows, entry = static_cast<int>(batch) * a.row_blocks + block;
     chain_begin();
-    const int64_t per = a.starts[0], start = a.starts[1 + static_cast<int64_t>(entry) * a.heads_kv + head_kv];   // (written where the list has keys)
+    const int per = a.starts[0], start = a.starts[1 + static_cast<int64_t>(entry) * a.heads_kv + head_kv];   // (written where the list has keys)
     int lo, hi;
     const int units = units_of(a, entry, lo, hi);
     const bool takes_part = token < sequence_window(a, batch).len_q;
-    float top = -INFINITY, total = 0.0f, value = 0.0f;
+    float top = -INFINITY, total = 0.0f, value[kOwn];
+#pragma unroll
+    for (int e = 0; e < kOwn; ++e) value[e] = 0.0f;
     if (units > 0) {
         if (start < 0) return;   // not cut: its CTA has written O
-        const int64_t first = start / per;
-        const int parts = static_cast<int>((start + units - 1) / per - first) + 1;
+        const int first = start / per, parts = (start + units - 1) / per - first + 1;
         const bool second_place = start != first * per;   // of the first part in its CTA
-        auto part_of = [&](int i) { return a.partial + (((first + i) * 2 + (i == 0 && second_place ? 1 : 0)) * a.block_rows + row) * (D + 2); };
-        for (int i0 = 0; i0 < parts; i0 += 32) {
-            float ahead[32];
+        // Each warp takes every fourth (eighth) part, with all channels; they meet below.
+        for (int i0 = warp; i0 < parts; i0 += kWarpsHere * kAhead) {
+            float2 pair[kAhead];
+            float ahead[kAhead][kOwn];
 #pragma unroll
-            for (int k = 0; k < 32; ++k) ahead[k] = i0 + k < parts ? part_of(i0 + k)[threadIdx.x] : 0.0f;
-            float2 pair = make_float2(-INFINITY, 0.0f);
-            if (i0 + lane < parts) pair = *reinterpret_cast<const float2*>(part_of(i0 + lane) + D);
-            float largest = fmaxf(top, pair.x);
+            for (int k = 0; k < kAhead; ++k) {
+                const int i = min(i0 + k * kWarpsHere, parts - 1);
+                const float* part = a.partial + (static_cast<int64_t>((first + i) * 2 + (i == 0 && second_place ? 1 : 0)) * a.block_rows + row) * (D + 2);
+                pair[k] = load_now(part + D);
 #pragma unroll
-            for (int s = 16; s > 0; s >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, s));
+                for (int e = 0; e < kOwn; e += 2) {
+                    const float2 v = load_now(part + lane * kOwn + e);
+                    ahead[k][e] = v.x, ahead[k][e + 1] = v.y;
+                }
+            }
+            float largest = top;
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k)
+                if (i0 + k * kWarpsHere < parts) largest = fmaxf(largest, pair[k].x);
             const float down = top == -INFINITY ? 1.0f : exp2_of(top - largest);   // (no score above -inf: zeros, or NaNs that are to be seen)
-            const float weight = pair.x == -INFINITY ? 1.0f : exp2_of(pair.x - largest);
+            total *= down;
+#pragma unroll
+            for (int e = 0; e < kOwn; ++e) value[e] *= down;
             top = largest;
-            float part = pair.y * weight;
 #pragma unroll
-            for (int s = 16; s > 0; s >>= 1) part += __shfl_xor_sync(0xffffffffu, part, s);
-            total = fmaf(total, down, part);
-            value *= down;
+            for (int k = 0; k < kAhead; ++k) {
+                if (i0 + k * kWarpsHere >= parts) continue;
+                const float weight = pair[k].x == -INFINITY ? 1.0f : exp2_of(pair[k].x - largest);
+                total = fmaf(pair[k].y, weight, total);
 #pragma unroll
-            for (int k = 0; k < 32; ++k) {
-                const float w = __shfl_sync(0xffffffffu, weight, k);
-                if (i0 + k < parts) value = fmaf(ahead[k], w, value);
+                for (int e = 0; e < kOwn; ++e) value[e] = fmaf(ahead[k][e], weight, value[e]);
             }
         }
     }
+    if (lane == 0) meeting[warp] = make_float2(top, total);
+#pragma unroll
+    for (int e = 0; e < kOwn; e += 2) *reinterpret_cast<float2*>(&values[warp][lane * kOwn + e]) = make_float2(value[e], value[e + 1]);
+    __syncthreads();
+    float result = 0.0f;
+    top = -INFINITY, total = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWarpsHere; ++w) top = fmaxf(top, meeting[w].x);
+#pragma unroll
+    for (int w = 0; w < kWarpsHere; ++w) {
+        const float weight = meeting[w].x == -INFINITY ? 1.0f : exp2_of(meeting[w].x - top);
+        total = fmaf(meeting[w].y, weight, total);
+        result = fmaf(values[w][threadIdx.x], weight, result);
+    }
     const bool none = !takes_part || total == 0.0f;
-    store_from_f32(a.o, a.o_type, batch * a.o_stride[0] + head * a.o_stride[1] + token * a.o_stride[2] + threadIdx.x, none ? 0.0f : value / total);
+    store_from_f32(a.o, a.o_type, batch * a.o_stride[0] + head * a.o_stride[1] + token * a.o_stride[2] + threadIdx.x, none ? 0.0f : result / total);
     if (threadIdx.x == 0 && a.stats) a.stats[batch * a.stats_stride[0] + head * a.stats_stride[1] + token * a.stats_stride[2]] = none ? -INFINITY : top * kLn2 + logf(total * 0x1p-15f);
 }
 
 struct StreamPlan {
-    int eights, row_warps, block_rows, row_blocks;
-    int64_t rows, grid, starts, scratch;   // starts: integers before the partial results
+    int eights, block_rows, row_blocks;
+    int64_t rows, units, grid, starts, scratch;   // units: the most there can be; starts: integers before the partial results
 };
 
 StreamPlan plan_stream(const dfgpu_cache_sdpa_params& p) {
@@ -741,14 +686,14 @@ StreamPlan plan_stream(const dfgpu_cache_sdpa_params& p) {
     const int64_t d = p.q.dim[3], group = p.q.dim[1] / p.k.dim[1];
     plan.rows = group * p.q.dim[2];
     plan.eights = plan.rows <= 8 ? 1 : 2;
-    plan.row_warps = plan.rows <= 16 ? 1 : plan.rows <= 32 ? 2 : 4;
-    plan.block_rows = plan.eights * 8 * plan.row_warps;
+    plan.block_rows = plan.eights * 8;
     plan.row_blocks = static_cast<int>((plan.rows + plan.block_rows - 1) / plan.block_rows);
     const int64_t lists = p.q.dim[0] * p.k.dim[1] * plan.row_blocks, units = (p.s_kv + kUnit - 1) / kUnit;
-    const int64_t ctas = kSms * (d == 256 ? (plan.eights == 1 ? 2 : 1) : plan.eights == 1 ? 3 : 2);   // (Shape::kCtas)
-    plan.grid = std::min(ctas, (lists * units + kLeastUnits - 1) / kLeastUnits);
-    plan.starts = (1 + lists + 1) / 2 * 2;
-    plan.scratch = plan.starts * 8 + plan.grid * 2 * plan.block_rows * (d + 2) * 4;
+    plan.units = lists * units;
+    const int64_t ctas = kSms * (d == 256 ? 2 : plan.eights == 1 ? 4 : 3);   // (Shape::kCtas)
+    plan.grid = std::min(ctas, (plan.units + kLeastUnits - 1) / kLeastUnits);
+    plan.starts = (1 + lists + 3) / 4 * 4;
+    plan.scratch = plan.starts * 4 + plan.grid * kWarps * 2 * plan.block_rows * (d + 2) * 4;
     return plan;
 }
 
@@ -796,7 +741,7 @@ int check_cache_sdpa(const dfgpu_cache_sdpa_params& p, int& kernel) {
         return fail(kInvalidShape, "CACHE_SDPA: Stats must be FLOAT [B, Hq, Sq, 1]");
     if (!std::isfinite(p.attn_scale)) return fail(kInvalidValue, "CACHE_SDPA: the attention scale must be finite");
     const StreamPlan plan = plan_stream(p);
-    if (p.q.dim[2] >= (1ll << 30) || p.q.dim[0] * p.k.dim[1] * plan.rows >= (1ll << 31)) return fail(kUnsupported, "CACHE_SDPA: too many sequences, heads or query rows");
+    if (p.q.dim[2] >= (1ll << 30) || p.q.dim[0] * p.k.dim[1] * plan.rows >= (1ll << 31) || plan.units >= (1ll << 30)) return fail(kUnsupported, "CACHE_SDPA: too many sequences, heads or query rows");
     if (p.kernel < DFGPU_CACHE_SDPA_AUTO || p.kernel > DFGPU_CACHE_SDPA_STREAM) return fail(kInvalidArgument, "CACHE_SDPA: unknown kernel id %d", p.kernel);
     kernel = DFGPU_CACHE_SDPA_STREAM;
     return kOk;
@@ -817,10 +762,10 @@ int make_side_map(CUtensorMap* map, const dfgpu_tensor& cache, const void* base,
     return kOk;
 }
 
-template <typename T, int D, int EIGHTS, int ROW_WARPS>
+template <typename T, int D, int EIGHTS>
 int launch_rows(const CUtensorMap& map_k, const CUtensorMap& map_v, const CacheSdpaArgs& a, dim3 grid, cudaStream_t stream) {
     constexpr int kBytes = Shape<D, EIGHTS>::kDynamic;
-    const auto kernel = cache_sdpa_stream_kernel<T, D, EIGHTS, ROW_WARPS>;
+    const auto kernel = cache_sdpa_stream_kernel<T, D, EIGHTS>;
     const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
     if (error != cudaSuccess) return fail(kExecutionFailed, "CACHE_SDPA: cannot reserve %d bytes of shared memory: %s", kBytes, cudaGetErrorString(error));
     launch_chained(kernel, grid, dim3(kThreads), kBytes, stream, map_k, map_v, a);
@@ -829,10 +774,7 @@ int launch_rows(const CUtensorMap& map_k, const CUtensorMap& map_v, const CacheS
 
 template <typename T, int D>
 int launch_stream(const CUtensorMap& map_k, const CUtensorMap& map_v, const CacheSdpaArgs& a, const StreamPlan& plan, dim3 grid, cudaStream_t stream) {
-    const int status = plan.eights == 1      ? launch_rows<T, D, 1, 1>(map_k, map_v, a, grid, stream)
-                       : plan.row_warps == 1 ? launch_rows<T, D, 2, 1>(map_k, map_v, a, grid, stream)
-                       : plan.row_warps == 2 ? launch_rows<T, D, 2, 2>(map_k, map_v, a, grid, stream)
-                                             : launch_rows<T, D, 2, 4>(map_k, map_v, a, grid, stream);
+    const int status = plan.eights == 1 ? launch_rows<T, D, 1>(map_k, map_v, a, grid, stream) : launch_rows<T, D, 2>(map_k, map_v, a, grid, stream);
     if (status) return status;
     launch_chained(cache_sdpa_merge_kernel<D>, dim3(static_cast<unsigned>(static_cast<int64_t>(a.entries / a.row_blocks) * a.heads_kv * a.rows)), dim3(D), 0, stream, a);
     return check_launch("CACHE_SDPA merge");
@@ -914,6 +856,7 @@ extern "C" int dfgpu_cache_sdpa(const dfgpu_cache_sdpa_params* p, void* const* t
     a.page = static_cast<int>(p->k.dim[2]);
     a.by_page = make_fast_divisor(static_cast<uint32_t>(a.page / 16));
     a.by_tokens = make_fast_divisor(static_cast<uint32_t>(p->k.dim[2] / p->k_scale.dim[2] / 16));
+    a.by_group = make_fast_divisor(static_cast<uint32_t>(a.group));
     a.has_left = p->has_left_bound;
     a.has_right = p->has_right_bound;
     a.bottom_right = p->bottom_right;
@@ -924,7 +867,7 @@ extern "C" int dfgpu_cache_sdpa(const dfgpu_cache_sdpa_params* p, void* const* t
     a.row_blocks = plan.row_blocks;
     a.block_rows = plan.block_rows;
     a.entries = static_cast<int>(p->q.dim[0] * plan.row_blocks);
-    a.starts = static_cast<int64_t*>(scratch);
+    a.starts = static_cast<int32_t*>(scratch);
     a.partial = reinterpret_cast<float*>(a.starts + plan.starts);
     a.box = a.page % 32 == 0 ? 32 : 16;
     CUtensorMap map_k, map_v;

@@ -21,14 +21,14 @@ struct CacheSdpaArgs {
     float* stats;
     const int32_t* seq_q_data;
     const int32_t* seq_kv_data;
-    float* partial;       // [CTA][first list, last list][row][D + 2]: O against the part's own largest score, that score, sum
-    int64_t* starts;      // [0] units a CTA, [1 + list] the list's first unit among all, -1: one CTA has all of it
+    float* partial;       // [part][first list, last list][row][D + 2]: O against the part's own largest score, that score, sum
+    int32_t* starts;      // [0] units a part, [1 + list] the list's first unit among all, -1: one part has all of it
     int64_t q_stride[3], o_stride[3], stats_stride[3], seq_q_stride, seq_kv_stride;
     int64_t left, right;
     int32_t o_type, o_vector, q_vector;
     int32_t heads_kv, group, rows, seq_q, s_kv;   // rows: (token, head of the group) pairs of a KV head
     int32_t page, box;                            // tokens a page, and of one TMA copy
-    FastDivisor by_page, by_tokens;               // of numbers of 16 tokens
+    FastDivisor by_page, by_tokens, by_group;     // the first two of numbers of 16 tokens
     int32_t has_left, has_right, bottom_right;
     int32_t row_blocks, block_rows, entries;      // entries: (sequence, block of rows)
     float scale_log2;
