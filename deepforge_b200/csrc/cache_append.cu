@@ -2,8 +2,9 @@
 //
 // Bound by HBM where prompts are written (2 or 4 bytes in, 1 out for a value), by latency where a step adds one token. The unit of work is
 // what one call adds to one scale block of K or V: its largest magnitude has to be known before its first code, so a unit's vectors stay in
-// registers between the two (up to eight of 16 bytes a thread; what a larger block has more is read again, from the cache). Small
-// blocks take a warp each, larger ones a CTA; nothing is shared between units, and no atomic is needed.
+// registers between the two (what a block has beyond the last variant's is read again, from the cache). Small blocks take a warp each, larger
+// ones a CTA of as many threads as hold it in four vectors of 16 bytes each; nothing is shared between units, and no atomic is needed. The
+// chain of a unit is length -> new tokens -> largest -> codes, with the page's id on its way beside the tokens.
 #include <algorithm>
 
 #include "common.cuh"
@@ -13,7 +14,8 @@
 namespace dfgpu {
 namespace {
 
-constexpr int kHeld = 8;   // vectors that a thread keeps
+// Vectors that a thread keeps.
+__host__ __device__ constexpr int held_by(int threads) { return threads == 32 ? 8 : 4; }
 
 struct AppendSide {
     const void* x;
@@ -33,7 +35,7 @@ struct AppendArgs {
     int32_t page, tokens, row;      // tokens a page and a scale block; vectors a row
     int32_t capacity;               // K's, what lengths_out is clamped to
     int64_t units;
-    FastDivisor by_row;
+    FastDivisor by_row, by_blocks, by_heads;
 };
 
 template <typename T, int V>
@@ -76,38 +78,32 @@ __device__ __forceinline__ AppendCodes<V> encode(const AppendVector<T, V>& x, fl
 template <typename T, int V, int NT>
 __global__ void __launch_bounds__(NT < 128 ? 128 : NT)
 cache_append_kernel(AppendArgs a) {
-    constexpr int kPerCta = NT < 128 ? 128 / NT : 1;
+    constexpr int kPerCta = NT < 128 ? 128 / NT : 1, kHeld = held_by(NT);
     __shared__ uint32_t largest_of[NT < 128 ? 1 : NT / 32];
     chain_begin();
     const int64_t unit = static_cast<int64_t>(blockIdx.x) * kPerCta + (kPerCta > 1 ? threadIdx.x / NT : 0);
     if (unit >= a.units) return;
     const int thread = kPerCta > 1 ? threadIdx.x % NT : threadIdx.x;
-    int64_t rest = unit;
-    const int which = static_cast<int>(rest & 1);
-    rest >>= 1;
-    const int nth = static_cast<int>(rest % a.blocks);
-    rest /= a.blocks;
-    const int head = static_cast<int>(rest % a.heads);
-    const int64_t batch = rest / a.heads;
+    const int which = static_cast<int>(unit & 1);
+    const uint32_t list = fast_divide(static_cast<uint32_t>(unit >> 1), a.by_blocks);
+    const int nth = static_cast<int>(unit >> 1) - static_cast<int>(list) * a.blocks;
+    const int64_t batch = fast_divide(list, a.by_heads);
+    const int head = static_cast<int>(list) - static_cast<int>(batch) * a.heads;
     const AppendSide& s = a.side[which];
 
-    const int64_t length = max(a.lengths[batch * a.lengths_stride], 0);
-    const int64_t added = a.added ? min(max(a.added[batch * a.added_stride], 0), a.seq) : a.seq;
-    if (unit % (2ll * a.blocks * a.heads) == 0 && thread == 0 && a.lengths_out)
-        a.lengths_out[batch * a.out_stride] = static_cast<int32_t>(min(length + added, static_cast<int64_t>(a.capacity)));
+    const int length = min(max(a.lengths[batch * a.lengths_stride], 0), 1 << 30);   // (a table's capacity is below)
+    const int added = a.added ? min(max(a.added[batch * a.added_stride], 0), a.seq) : a.seq;
+    if (which == 0 && nth == 0 && head == 0 && thread == 0 && a.lengths_out)
+        a.lengths_out[batch * a.out_stride] = min(length + added, a.capacity);
     // (a sequence that is as long as its table has no block here: the slot below is behind it)
-    const int64_t begin = (length / a.tokens + nth) * a.tokens, first = max(begin, length), end = min(begin + a.tokens, length + added);
+    const int begin = (length / a.tokens + nth) * a.tokens, first = max(begin, length), end = min(begin + a.tokens, length + added);
     if (first >= end) return;
-    const int64_t slot = begin / a.page;
+    const int slot = begin / a.page;
     if (slot >= s.table_len) return;
-    const int64_t page = s.table[batch * s.table_batch + slot * s.table_slot];
-    if (page < 0 || page >= s.pages) return;
-
-    const int in_page = static_cast<int>(begin - slot * a.page);
+    const int page = s.table[batch * s.table_batch + slot * s.table_slot];   // (asked whether it is one below, when the tokens are on their way)
+    const int in_page = begin - slot * a.page;
     const T* x = static_cast<const T*>(s.x) + batch * s.x_stride[0] + head * s.x_stride[1] + (first - length) * s.x_stride[2];
-    uint8_t* codes = s.codes + page * s.code_stride[0] + head * s.code_stride[1] + (in_page + (first - begin)) * s.code_stride[2];
-    uint8_t* scale = s.scales + page * s.scale_stride[0] + head * s.scale_stride[1] + (in_page / a.tokens) * s.scale_stride[2];
-    const int count = static_cast<int>(end - first) * a.row;   // vectors
+    const int count = (end - first) * a.row;   // vectors
     auto load = [&](int i) {
         const int row = static_cast<int>(fast_divide(static_cast<uint32_t>(i), a.by_row));
         return *reinterpret_cast<const AppendVector<T, V>*>(x + row * s.x_stride[2] + (i - row * a.row) * V);
@@ -117,6 +113,9 @@ cache_append_kernel(AppendArgs a) {
 #pragma unroll
     for (int k = 0; k < kHeld; ++k)
         if (thread + k * NT < count) held[k] = load(thread + k * NT);
+    if (page < 0 || page >= s.pages) return;
+    uint8_t* codes = s.codes + page * s.code_stride[0] + head * s.code_stride[1] + (in_page + (first - begin)) * s.code_stride[2];
+    uint8_t* scale = s.scales + page * s.scale_stride[0] + head * s.scale_stride[1] + (in_page / a.tokens) * s.scale_stride[2];
     const bool holds = first > begin;
     const uint32_t old = holds ? *scale : 0u;
 #pragma unroll
@@ -147,7 +146,7 @@ cache_append_kernel(AppendArgs a) {
         uint8_t* before = s.codes + page * s.code_stride[0] + head * s.code_stride[1] + in_page * s.code_stride[2];
         // (Scales more than 2^60 apart leave no code but zeros, as 2^-60 does; their quotient may leave f32's range. A NaN stays one.)
         const float shrink = code != 0xffu && code - old > 60u ? 0x1p-60f : decode_e8m0(old) * inverse;
-        for (int i = thread; i < static_cast<int>(first - begin) * a.row; i += NT) {
+        for (int i = thread; i < (first - begin) * a.row; i += NT) {
             const int row = static_cast<int>(fast_divide(static_cast<uint32_t>(i), a.by_row));
             AppendCodes<V>& at = *reinterpret_cast<AppendCodes<V>*>(before + row * s.code_stride[2] + (i - row * a.row) * V);
             AppendCodes<V> c = at;
@@ -164,9 +163,9 @@ __global__ void __launch_bounds__(256) cache_lengths_kernel(AppendArgs a, int64_
     chain_begin();
     const int64_t batch = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     if (batch >= batches) return;
-    const int64_t length = max(a.lengths[batch * a.lengths_stride], 0);
-    const int64_t added = a.added ? min(max(a.added[batch * a.added_stride], 0), a.seq) : a.seq;
-    a.lengths_out[batch * a.out_stride] = static_cast<int32_t>(min(length + added, static_cast<int64_t>(a.capacity)));
+    const int length = min(max(a.lengths[batch * a.lengths_stride], 0), 1 << 30);
+    const int added = a.added ? min(max(a.added[batch * a.added_stride], 0), a.seq) : a.seq;
+    a.lengths_out[batch * a.out_stride] = min(length + added, a.capacity);
 }
 
 bool on_boundary(const void* pointer, int64_t bytes) { return (reinterpret_cast<uintptr_t>(pointer) & static_cast<uintptr_t>(bytes - 1)) == 0; }
@@ -222,6 +221,7 @@ template <typename T, int V>
 void launch_append(const AppendArgs& a, int threads, cudaStream_t stream) {
     if (threads == 32) launch_chained(cache_append_kernel<T, V, 32>, dim3(static_cast<unsigned>((a.units + 3) / 4)), dim3(128), 0, stream, a);
     else if (threads == 128) launch_chained(cache_append_kernel<T, V, 128>, dim3(static_cast<unsigned>(a.units)), dim3(128), 0, stream, a);
+    else if (threads == 256) launch_chained(cache_append_kernel<T, V, 256>, dim3(static_cast<unsigned>(a.units)), dim3(256), 0, stream, a);
     else launch_chained(cache_append_kernel<T, V, 512>, dim3(static_cast<unsigned>(a.units)), dim3(512), 0, stream, a);
 }
 
@@ -295,10 +295,14 @@ extern "C" int dfgpu_cache_append(const dfgpu_cache_append_params* p, void* cons
     a.units = 2ll * a.blocks * a.heads * p->k.dim[0];
     a.row = static_cast<int>(p->k.dim[3]) / (vector ? width : 1);
     a.by_row = make_fast_divisor(static_cast<uint32_t>(a.row));
+    a.by_blocks = make_fast_divisor(static_cast<uint32_t>(a.blocks));
+    a.by_heads = make_fast_divisor(static_cast<uint32_t>(a.heads));
     if (a.units >= (1ll << 31)) return fail(kUnsupported, "CACHE_APPEND: too many blocks in one call");
     // As few threads as hold a whole block of new tokens in their registers.
     const int64_t vectors = static_cast<int64_t>(std::min(a.tokens, a.seq)) * a.row;
-    const int threads = vectors <= 32 * kHeld ? 32 : vectors <= 128 * kHeld ? 128 : 512;
+    int threads = 32;
+    if (vectors > 32 * held_by(32))
+        for (threads = 128; threads < 512 && vectors > threads * held_by(threads);) threads *= 2;
     cudaStream_t on = as_stream(stream);
     if (p->k.dtype == DFGPU_F32) vector ? launch_append<float, 4>(a, threads, on) : launch_append<float, 1>(a, threads, on);
     else if (p->k.dtype == DFGPU_F16) vector ? launch_append<__half, 8>(a, threads, on) : launch_append<__half, 1>(a, threads, on);
