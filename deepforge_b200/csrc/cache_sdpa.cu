@@ -312,6 +312,14 @@ __device__ __forceinline__ int units_of(const CacheSdpaArgs& a, int entry, int& 
     return hi > lo ? (hi + kUnit - 1) / kUnit - lo / kUnit : 0;
 }
 
+// Whether the kernel has anything to do (whole warps).
+__device__ __forceinline__ bool wanted(const CacheSdpaArgs& a) {
+    if (!a.only_if) return true;
+    bool some = false;
+    for (int i = threadIdx.x & 31; i < a.only_if_count; i += 32) some = some || a.only_if[i] != 0;
+    return __any_sync(0xffffffffu, some);
+}
+
 template <typename T, int D, int EIGHTS>
 __global__ void __launch_bounds__(kThreads, Shape<D, EIGHTS>::kCtas)
 cache_sdpa_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CacheSdpaArgs a) {
@@ -331,6 +339,7 @@ cache_sdpa_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     chain_begin();
+    if (!wanted(a)) return;
 
     // The units before each lane's entries, and all of them (fewer than 2^30): where the warp's part begins. (Every warp for itself: the lengths come
     // from L1 for the later ones, and a pass over a few of them is shorter than a barrier of the CTA.)
@@ -612,6 +621,7 @@ cache_sdpa_merge_kernel(const __grid_constant__ CacheSdpaArgs a) {
     const int head_kv = static_cast<int>(list - batch * a.heads_kv), head = head_kv * a.group + (in_rows - token * a.group);
     const int block = in_rows / a.block_rows, row = in_rows - block * a.block_rows, entry = static_cast<int>(batch) * a.row_blocks + block;
     chain_begin();
+    if (!wanted(a)) return;
     const int per = a.starts[0], start = a.starts[1 + static_cast<int64_t>(entry) * a.heads_kv + head_kv];   // (written where the list has keys)
     int lo, hi;
     const int units = units_of(a, entry, lo, hi);
@@ -697,6 +707,10 @@ StreamPlan plan_stream(const dfgpu_cache_sdpa_params& p) {
     return plan;
 }
 
+// The tcgen05 form has blocks of 256 rows, an SM each; the streaming form cuts any shape evenly but runs at a seventh of its rate.
+bool umma_pays(const dfgpu_cache_sdpa_params& p, const StreamPlan& plan) { return plan.rows >= 128 && 7 * cache_sdpa_umma_items(p) >= kSms; }
+int64_t flag_bytes(const dfgpu_cache_sdpa_params& p, int kernel) { return kernel == DFGPU_CACHE_SDPA_UMMA ? (cache_sdpa_umma_items(p) + 3) / 4 * 16 : 0; }
+
 bool on_16(const void* pointer) { return (reinterpret_cast<uintptr_t>(pointer) & 15u) == 0; }
 
 int check_side(const dfgpu_cache_sdpa_params& p, const dfgpu_tensor& cache, const dfgpu_tensor& scale, const dfgpu_tensor& table, const char* name) {
@@ -742,8 +756,10 @@ int check_cache_sdpa(const dfgpu_cache_sdpa_params& p, int& kernel) {
     if (!std::isfinite(p.attn_scale)) return fail(kInvalidValue, "CACHE_SDPA: the attention scale must be finite");
     const StreamPlan plan = plan_stream(p);
     if (p.q.dim[2] >= (1ll << 30) || p.q.dim[0] * p.k.dim[1] * plan.rows >= (1ll << 31) || plan.units >= (1ll << 30)) return fail(kUnsupported, "CACHE_SDPA: too many sequences, heads or query rows");
-    if (p.kernel < DFGPU_CACHE_SDPA_AUTO || p.kernel > DFGPU_CACHE_SDPA_STREAM) return fail(kInvalidArgument, "CACHE_SDPA: unknown kernel id %d", p.kernel);
-    kernel = DFGPU_CACHE_SDPA_STREAM;
+    if (p.kernel < DFGPU_CACHE_SDPA_AUTO || p.kernel > DFGPU_CACHE_SDPA_UMMA) return fail(kInvalidArgument, "CACHE_SDPA: unknown kernel id %d", p.kernel);
+    const bool umma = cache_sdpa_umma_supported(p);
+    if (p.kernel == DFGPU_CACHE_SDPA_UMMA && !umma) return fail(kUnsupported, "CACHE_SDPA: the tcgen05 kernel needs a head dimension of 64 or 128 and at most 128 query heads a KV head");
+    kernel = p.kernel != DFGPU_CACHE_SDPA_AUTO ? p.kernel : umma && umma_pays(p, plan) ? DFGPU_CACHE_SDPA_UMMA : DFGPU_CACHE_SDPA_STREAM;
     return kOk;
 }
 
@@ -792,8 +808,8 @@ extern "C" int dfgpu_query_cache_sdpa(const dfgpu_cache_sdpa_params* p, dfgpu_pl
     if (status) return status;
     const StreamPlan plan = plan_stream(*p);
     info->kernel = kernel;
-    info->launches = 2;
-    info->scratch_bytes = plan.scratch;
+    info->launches = kernel == DFGPU_CACHE_SDPA_UMMA ? 3 : 2;
+    info->scratch_bytes = plan.scratch + flag_bytes(*p, kernel);
     return kOk;
 }
 
@@ -867,7 +883,8 @@ extern "C" int dfgpu_cache_sdpa(const dfgpu_cache_sdpa_params* p, void* const* t
     a.row_blocks = plan.row_blocks;
     a.block_rows = plan.block_rows;
     a.entries = static_cast<int>(p->q.dim[0] * plan.row_blocks);
-    a.starts = static_cast<int32_t*>(scratch);
+    const int64_t flags = flag_bytes(*p, kernel);
+    a.starts = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(scratch) + flags);
     a.partial = reinterpret_cast<float*>(a.starts + plan.starts);
     a.box = a.page % 32 == 0 ? 32 : 16;
     CUtensorMap map_k, map_v;
@@ -876,6 +893,12 @@ extern "C" int dfgpu_cache_sdpa(const dfgpu_cache_sdpa_params* p, void* const* t
     if (made) return made;
     const dim3 grid(static_cast<unsigned>(plan.grid));
     cudaStream_t on = as_stream(stream);
+    if (kernel == DFGPU_CACHE_SDPA_UMMA) {
+        const int launched = launch_cache_sdpa_umma(*p, a, static_cast<int32_t*>(scratch), on);
+        if (launched) return launched;
+        a.only_if = static_cast<const int32_t*>(scratch);
+        a.only_if_count = static_cast<int>(cache_sdpa_umma_items(*p));
+    }
     const bool half = p->q.dtype == DFGPU_F16;
     switch (p->q.dim[3]) {
         case 64: return half ? launch_stream<__half, 64>(map_k, map_v, a, plan, grid, on) : launch_stream<__nv_bfloat16, 64>(map_k, map_v, a, plan, grid, on);
@@ -885,5 +908,11 @@ extern "C" int dfgpu_cache_sdpa(const dfgpu_cache_sdpa_params* p, void* const* t
 }
 
 namespace dfgpu {
-int cache_sdpa_device_status(int* status) { return read_and_clear_device_status(status); }
+int cache_sdpa_device_status(int* status) {
+    int own = 0, umma = 0;
+    int code = read_and_clear_device_status(&own);
+    if (!code) code = cache_sdpa_umma_device_status(&umma);
+    *status = own ? own : umma;
+    return code;
+}
 }  // namespace dfgpu

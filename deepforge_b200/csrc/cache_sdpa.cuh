@@ -2,6 +2,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "dfgpu_cache.h"
 
 namespace dfgpu {
 
@@ -32,7 +33,14 @@ struct CacheSdpaArgs {
     int32_t has_left, has_right, bottom_right;
     int32_t row_blocks, block_rows, entries;      // entries: (sequence, block of rows)
     float scale_log2;
+    const int32_t* only_if;   // the streaming form returns at once unless one of these only_if_count integers is set; null: always runs
+    int32_t only_if_count;
 };
+
+// The tcgen05 form (cache_sdpa_umma.cu). What it leaves to the streaming form it says in `flags`, one integer an item.
+bool cache_sdpa_umma_supported(const dfgpu_cache_sdpa_params& p);
+int64_t cache_sdpa_umma_items(const dfgpu_cache_sdpa_params& p);
+int launch_cache_sdpa_umma(const dfgpu_cache_sdpa_params& p, const CacheSdpaArgs& a, int32_t* flags, cudaStream_t stream);
 
 struct SequenceWindow {
     int64_t shift;    // key minus query position on the diagonal

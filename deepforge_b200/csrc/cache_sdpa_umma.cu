@@ -1,0 +1,539 @@
+// Attention over the 8-bit paged cache for many query rows a KV head (chunks of prompts), on tcgen05.
+//
+// Bound by the tensor pipe and the exponentials, about 1024 clocks each for 128 rows x 128 keys of 128 channels. The codes have to become f16
+// (exactly) before the tensor core can take them, and that is paid once for 256 rows: a CTA has two query tiles of 128 rows, (token, head of the
+// group) pairs of one KV head, and both read the same converted K and V tiles.
+//   warps 0-3, 4-7   softmax of query tile 0 and 1, a thread a row; Q to f16 at the start, O out of tensor memory at the end
+//   warps 8-11       codes from global memory (looked up and loaded a tile ahead, in registers) to f16 tiles in shared memory, two K and two V
+//   warp 12          issues the products: S = Q K^T, then O += P V with P from tensor memory, the two query tiles in turn
+// Tensor memory: S (then P, in its place) of the query tiles at 0 and 128, O at 256 and 384.
+// Q is exact as in the streaming form (a power of two a row). The K scale of 16 keys is a factor of their scores. The V scale is
+// part of the exponent: with t = score + log2(V scale), a row's reference r follows the largest t, P = 2^(t - r + 11) in f16 multiplies codes, and the
+// row's sum adds up P / (V scale), so nothing but the final division knows of either. r is raised when t passes it by 2^4 (O
+// is rescaled in tensor memory then, which is rare).
+// What this cannot do exactly it says in a flag of the item, and the streaming form then computes the whole call again (its kernels return at
+// once otherwise): a NaN among V codes of a tile that some rows do not see all of (their zero probability times it is NaN), a V
+// scale of 2^126 or more or a NaN, V scales more than 2^16
+// apart or below 2^-80 over codes that are not zero, scores beyond 2^10.
+#include <algorithm>
+
+#include "cache_sdpa.cuh"
+#include "dfgpu_cache.h"
+#include "umma_ptx.cuh"
+
+namespace dfgpu {
+namespace {
+
+constexpr int kRows = 128, kKeys = 128, kRuns = kKeys / 16;
+constexpr int kThreads = 13 * 32, kConverters = 128;
+constexpr int kScaleStages = 4;      // (three are enough: a tile's K slot is free when both query tiles are done with the tile before)
+constexpr float kUp = 11.0f;         // P = 2^(t - r + 11): at most 2^15 while t is within 4 of r
+constexpr float kRaise = 4.0f;
+constexpr int kLeastCode = 47;       // V scales below 2^-80 count as that (over zeros; else a flag)
+constexpr int kMostApart = 16;
+constexpr float kMostReference = 1024.0f;   // |r|: the exponent's one rounding, of score * factor + (scale - r), is below 2^-14 up to there
+constexpr int kMostRanked = 128;     // sequences that are put in order of length
+constexpr float kLn2 = 0.6931471805599453f;
+
+struct CachePrefillArgs {
+    CacheSdpaArgs a;
+    int32_t* flags;       // by item
+    int32_t tokens;       // of a query tile: 128 / group
+    int32_t blocks;       // of two query tiles
+    int32_t batches;
+};
+
+template <int D>
+struct Smem {
+    static constexpr int kHalves = D / 64, kHalf = kRows * 128;
+    static constexpr int kTile = kHalves * kHalf;              // of f16: 128 rows by 64 channels, swizzled, once or twice
+    static constexpr int kQ = 0, kK = 2 * kTile, kV = 4 * kTile;
+    static constexpr int kScales = 6 * kTile;                  // [stage][run]{K factor, log2 of V's, 1 / V's, -}
+    static constexpr int kBarriers = kScales + kScaleStages * kRuns * 16;
+    // q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], scale_full[4]
+    static constexpr int kBarrierCount = 1 + 14 + kScaleStages;
+    static constexpr int kMisc = kBarriers + kBarrierCount * 8;    // tensor memory's address, flag, {least, largest} V scale by converter warp
+    static constexpr int kTotal = kMisc + 64;
+    static constexpr int kDynamic = kTotal + 1024;
+};
+
+__device__ __forceinline__ void tmem_load_32_now(uint32_t taddr, uint32_t (&r)[32]) {
+    tmem_load_32(taddr, r);
+    tmem_load_wait();
+}
+__device__ __forceinline__ void tmem_store_16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_store_32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+          "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+          "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// D[tmem] (+)= A[tmem] * B[smem]: A are pairs of f16, one row per lane.
+__device__ __forceinline__ void umma_a_tmem(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ float exp2_of(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t two_halves(float lo, float hi) {
+    uint32_t v;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(hi), "f"(lo));
+    return v;
+}
+__device__ __forceinline__ void four_codes(uint32_t codes, uint32_t& low, uint32_t& high) {   // as f16
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(low), "=r"(high) : "r"(codes));
+}
+__device__ __forceinline__ float power_of_two(int n) { return __uint_as_float(static_cast<uint32_t>(n + 127) << 23); }   // -126 to 127
+__device__ __forceinline__ float value_of(__half v) { return __half2float(v); }
+__device__ __forceinline__ float value_of(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+cache_sdpa_umma_kernel(const __grid_constant__ CachePrefillArgs args) {
+    using S = Smem<D>;
+    constexpr int kChunks = D / 16, kAtOnce = kConverters / kChunks, kPasses = kKeys / kAtOnce;   // a converter's 16 codes at a time
+    const CacheSdpaArgs& a = args.a;
+    extern __shared__ uint8_t raw_smem[];
+    const uint32_t base = (smem_u32(raw_smem) + 1023u) & ~1023u;
+    uint8_t* smem = raw_smem + (base - smem_u32(raw_smem));
+    const uint32_t bars = base + S::kBarriers;
+    const uint32_t q_full = bars;
+    auto k_full = [&](int s) { return bars + 8u * (1 + s); };
+    auto k_empty = [&](int s) { return bars + 8u * (3 + s); };
+    auto v_full = [&](int s) { return bars + 8u * (5 + s); };
+    auto v_empty = [&](int s) { return bars + 8u * (7 + s); };
+    auto s_full = [&](int i) { return bars + 8u * (9 + i); };
+    auto p_full = [&](int i) { return bars + 8u * (11 + i); };
+    auto o_full = [&](int i) { return bars + 8u * (13 + i); };
+    auto scale_full = [&](int s) { return bars + 8u * (15 + s); };
+    int* misc = reinterpret_cast<int*>(smem + S::kMisc);
+    const int warp = uniform_warp_index(), lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, 8);
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(k_full(s), 4), mbar_init(k_empty(s), 1);
+            mbar_init(v_full(s), 4), mbar_init(v_empty(s), 1);
+            mbar_init(s_full(s), 1), mbar_init(p_full(s), 4), mbar_init(o_full(s), 1);
+        }
+        for (int s = 0; s < kScaleStages; ++s) mbar_init(scale_full(s), 4);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        misc[1] = 0;
+    }
+    if (warp == 12) {
+        tmem_alloc(base + S::kMisc, 512);
+        tmem_relinquish();
+        tc_fence_before();
+    }
+    chain_wait();
+
+    // The item: sequences by falling length (those beyond the first 128 as they are stored), their last query blocks first, a block's heads side by side.
+    const int per_batch = a.heads_kv * args.blocks;
+    int nth = static_cast<int>(blockIdx.x) / per_batch;
+    if (args.batches <= kMostRanked) {
+        if (static_cast<int>(threadIdx.x) < args.batches) {
+            const int own = a.seq_kv_data[threadIdx.x * a.seq_kv_stride];
+            int rank = 0;
+            for (int b = 0; b < args.batches; ++b) {
+                const int other = a.seq_kv_data[b * a.seq_kv_stride];
+                rank += other > own || (other == own && b < static_cast<int>(threadIdx.x));
+            }
+            if (rank == nth) misc[2] = threadIdx.x;
+        }
+    } else if (threadIdx.x == 0) {
+        misc[2] = nth;
+    }
+    __syncthreads();
+    tc_fence_after();
+    chain_release();
+    const uint32_t tmem = static_cast<uint32_t>(misc[0]);
+    const int64_t batch = misc[2];
+    const int in_batch = static_cast<int>(blockIdx.x) % per_batch, head = in_batch % a.heads_kv, block = args.blocks - 1 - in_batch / a.heads_kv;
+    const SequenceWindow window = sequence_window(a, batch);
+    const int token0 = block * 2 * args.tokens;
+    // Keys that the query tiles see; the first key tile is common.
+    int lo[2], hi[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) window_of_tokens(a, window, token0 + i * args.tokens, min(token0 + (i + 1) * args.tokens, a.seq_q) - 1, lo[i], hi[i]);
+    const bool some[2] = {hi[0] > lo[0], hi[1] > lo[1]};
+    const int all_lo = some[0] && some[1] ? min(lo[0], lo[1]) : some[0] ? lo[0] : lo[1], all_hi = max(hi[0], hi[1]);
+    const int first = all_lo / kKeys;
+    const int n[2] = {some[0] ? (hi[0] + kKeys - 1) / kKeys - first : 0, some[1] ? (hi[1] + kKeys - 1) / kKeys - first : 0};
+    const int tiles = max(n[0], n[1]);
+    bool ok = true;
+
+    if (warp == 12) {
+        // ---- the products
+        const bool leader = elect_one();
+        constexpr uint32_t idesc_s = (1u << 4) | (static_cast<uint32_t>(kKeys >> 3) << 17) | (static_cast<uint32_t>(kRows >> 4) << 24);   // f16 operands, f32 sums
+        constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | (static_cast<uint32_t>(D >> 3) << 17) | (static_cast<uint32_t>(kRows >> 4) << 24);   // V read MN-major
+        const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
+        if (tiles > 0) ok = mbar_wait_warp(q_full, 0, 721);
+        auto scores = [&](int i, int j) {
+            if (ok) ok = mbar_wait_warp(k_full(j & 1), (j >> 1) & 1, 722);
+            tc_fence_after();
+            if (leader && ok) {
+                const uint32_t q_lo = smem_desc_lo(base + S::kQ + i * S::kTile, 16), k_lo = smem_desc_lo(base + S::kK + (j & 1) * S::kTile, 16);
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint32_t at = ((k >> 2) * S::kHalf + (k & 3) * 32) >> 4;
+                    umma_bf16(tmem_u + i * 128, desc_words(q_lo + at, smem_desc_hi(1024)), desc_words(k_lo + at, smem_desc_hi(1024)), idesc_s, k != 0 ? 1u : 0u);
+                }
+                umma_commit(s_full(i));
+            }
+            __syncwarp();
+        };
+        for (int i = 0; i < 2; ++i)
+            if (n[i] > 0) scores(i, 0);
+        if (leader && ok && tiles > 0) umma_commit(k_empty(0));
+        for (int j = 0; j < tiles && ok; ++j) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (j >= n[i]) continue;
+                if (ok) ok = mbar_wait_warp(p_full(i), j & 1, 723);
+                if (ok) ok = mbar_wait_warp(v_full(j & 1), (j >> 1) & 1, 724);
+                tc_fence_after();
+                if (leader && ok) {
+                    const uint32_t v_lo = smem_desc_lo(base + S::kV + (j & 1) * S::kTile, S::kHalf);
+#pragma unroll
+                    for (int k = 0; k < kKeys / 16; ++k)
+                        umma_a_tmem(tmem_u + 256 + i * 128, tmem_u + i * 128 + k * 8, desc_words(v_lo + ((k * 2048) >> 4), smem_desc_hi(1024)), idesc_o, (j | k) != 0 ? 1u : 0u);
+                    if (j + 1 == n[i]) umma_commit(o_full(i));
+                }
+                __syncwarp();
+                if (j + 1 < n[i]) scores(i, j + 1);   // (over P, which the products before have read: they run in order)
+            }
+            if (leader && ok) {
+                umma_commit(v_empty(j & 1));
+                if (j + 1 < tiles) umma_commit(k_empty((j + 1) & 1));
+            }
+            __syncwarp();
+        }
+    } else if (warp >= 8) {
+        // ---- codes to f16
+        const int thread = threadIdx.x - 256, chunk = thread % kChunks, row0 = thread / kChunks;
+        int common_lo, common_hi;   // what all rows see
+        {
+            int l0, h0, l1, h1;
+            window_of_tokens(a, window, token0, token0, l0, h0);
+            const int last = min(min(token0 + 2 * args.tokens, a.seq_q), window.len_q) - 1;
+            window_of_tokens(a, window, last, last, l1, h1);
+            common_lo = max(l0, l1), common_hi = min(h0, h1);
+        }
+        int v_least = 1 << 20, v_most = -1;
+        bool flag = false;
+        // Lane l < 16 has run l % 8 of K (l < 8) or V: its page (as the table has it), where it begins in it, and its scale.
+        const int side = lane >> 3 & 1, run = lane & 7;
+        auto look_up = [&](int j, int& page, int& token) {
+            const int key = (first + j) * kKeys + run * 16, slot = static_cast<int>(fast_divide(static_cast<uint32_t>(key >> 4), a.by_page));
+            token = key - slot * a.page;
+            const CacheSide& s = a.side[side];
+            page = j < tiles && key < all_hi && key + 16 > all_lo && slot < s.table_len ? s.table[batch * s.table_batch + slot * s.table_slot] : -1;
+        };
+        auto checked = [&](int page) { return page >= 0 && page < a.side[side].pages ? page : -1; };
+        auto look_up_scale = [&](int page, int token) {
+            const CacheSide& s = a.side[side];
+            return page >= 0 ? static_cast<int>(s.scales[page * s.scale_stride[0] + head * s.scale_stride[1] + fast_divide(static_cast<uint32_t>(token >> 4), a.by_tokens) * s.scale_stride[2]]) : -1;
+        };
+        // A tile's codes, 16 of a row at a time; zeros where there is no page and where no row sees the key.
+        auto load = [&](int which, int j, int page, int token, uint4 (&to)[kPasses]) {
+            const CacheSide& s = a.side[which];
+#pragma unroll
+            for (int i = 0; i < kPasses; ++i) {
+                const int row = i * kAtOnce + row0, from = which * 8 + (row >> 4), key = (first + j) * kKeys + row;
+                const int id = __shfl_sync(0xffffffffu, page, from), at = __shfl_sync(0xffffffffu, token, from) + (row & 15);
+                to[i] = make_uint4(0, 0, 0, 0);
+                if (id >= 0 && key >= all_lo && key < all_hi) to[i] = __ldcg(reinterpret_cast<const uint4*>(s.codes + id * s.stride[0] + head * s.stride[1] + at * s.stride[2] + chunk * 16));
+            }
+        };
+        auto convert = [&](uint32_t to, const uint4 (&from)[kPasses]) {
+#pragma unroll
+            for (int i = 0; i < kPasses; ++i) {
+                const int row = i * kAtOnce + row0;
+                uint32_t h[8];
+                four_codes(from[i].x, h[0], h[1]), four_codes(from[i].y, h[2], h[3]), four_codes(from[i].z, h[4], h[5]), four_codes(from[i].w, h[6], h[7]);
+                const uint32_t at = to + (chunk >> 2) * S::kHalf + row * 128, place = chunk * 2 & 7;
+                const int odd = chunk >> 2;   // (the halves lie in the same banks: their chunks go in opposite order)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int which = e ^ odd;
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + (((place + which) ^ (row & 7)) << 4)), "r"(which ? h[4] : h[0]), "r"(which ? h[5] : h[1]),
+                                 "r"(which ? h[6] : h[2]), "r"(which ? h[7] : h[3])
+                                 : "memory");
+                }
+            }
+        };
+        int page, token, page_next, token_next, code;
+        uint4 k_raw[kPasses], v_raw[kPasses];
+        look_up(0, page, token);
+        look_up(1, page_next, token_next);
+        page = checked(page);
+        code = look_up_scale(page, token);
+        load(0, 0, page, token, k_raw);
+        load(1, 0, page, token, v_raw);
+        for (int j = 0; j < tiles; ++j) {
+            const int now = j & 1;
+            page = checked(page_next), token = token_next;   // of tile j + 1
+            look_up(j + 2, page_next, token_next);
+            const int code_next = look_up_scale(page, token);
+            if (ok) ok = mbar_wait_warp(k_empty(now), ((j >> 1) & 1) ^ 1, 725);
+            if (!ok) break;
+            convert(base + S::kK + now * S::kTile, k_raw);
+            if (warp == 8) {
+                // (lanes 0-7 the K scales, 8-15 V's; a V scale that the exponent does not take counts as the least)
+                float* scale = reinterpret_cast<float*>(smem + S::kScales + ((j & (kScaleStages - 1)) * kRuns + run) * 16);
+                if (lane < 8) {
+                    scale[0] = code < 0 ? 1.0f : decode_e8m0(static_cast<uint32_t>(code));
+                } else if (lane < 16) {
+                    const int exponent = max(code < 0 ? 127 : code, kLeastCode) - 127;
+                    scale[1] = static_cast<float>(exponent);
+                    scale[2] = power_of_two(max(-exponent, -126));
+                    if (code >= kLeastCode) v_least = min(v_least, code), v_most = max(v_most, code);
+                    flag = flag || code >= 253;   // (a NaN among them)
+                }
+            }
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(k_full(now));
+                mbar_arrive(scale_full(j & (kScaleStages - 1)));
+            }
+            load(0, j + 1, page, token, k_raw);
+            const int key0 = (first + j) * kKeys;
+            const bool mixed = key0 < common_lo || key0 + kKeys > common_hi;
+            const bool low = __any_sync(0xffffffffu, lane >= 8 && lane < 16 && code >= 0 && code < kLeastCode);
+            if (mixed || low) {
+#pragma unroll
+                for (int i = 0; i < kPasses; ++i) {
+                    const uint32_t w[4] = {v_raw[i].x, v_raw[i].y, v_raw[i].z, v_raw[i].w};
+                    const int run_code = __shfl_sync(0xffffffffu, code, 8 + ((i * kAtOnce + row0) >> 4));
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        flag = flag || (mixed && (((w[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0) || (run_code >= 0 && run_code < kLeastCode && (w[e] & 0x7f7f7f7fu) != 0);
+                }
+            }
+            if (ok) ok = mbar_wait_warp(v_empty(now), ((j >> 1) & 1) ^ 1, 726);
+            if (!ok) break;
+            convert(base + S::kV + now * S::kTile, v_raw);
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(v_full(now));
+            load(1, j + 1, page, token, v_raw);
+            code = code_next;
+        }
+        v_least = __reduce_min_sync(0xffffffffu, v_least), v_most = __reduce_max_sync(0xffffffffu, v_most);
+        if (flag || v_most - v_least > kMostApart) misc[1] = 1;
+    } else {
+        // ---- a row a thread
+        const int i = warp >> 2, row = threadIdx.x & 127, quarter = warp & 3;
+        const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16, s_tmem = tmem + lanes + i * 128, o_tmem = tmem + lanes + 256 + i * 128;
+        const int in_group = row / args.tokens, token = token0 + i * args.tokens + (row - in_group * args.tokens);
+        const bool there = in_group < a.group && token < a.seq_q;   // has a place in O
+        const int head_q = head * a.group + (there ? in_group : 0);
+        int row_lo = 0, row_hi = 0;
+        if (there && token < window.len_q) window_of_tokens(a, window, token, token, row_lo, row_hi);
+        float factor;
+        {
+            const T* from = static_cast<const T*>(a.q) + batch * a.q_stride[0] + head_q * a.q_stride[1] + (there ? token : 0) * a.q_stride[2];
+            struct alignas(8) Four { T v[4]; };
+            auto four_of = [&](int c) {
+                if (!there) return Four{};
+                if (a.q_vector) return *reinterpret_cast<const Four*>(from + c);
+                return Four{{from[c], from[c + 1], from[c + 2], from[c + 3]}};
+            };
+            float largest = 0.0f;
+#pragma unroll 8
+            for (int c = 0; c < D; c += 4) {
+                const Four v = four_of(c);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) largest = fmaxf(largest, fabsf(value_of(v.v[e])));
+            }
+            int up = 14 - (static_cast<int>(__float_as_uint(largest) >> 23) - 127);
+            up = largest == 0.0f ? 0 : min(max(up, -126), 126);
+            const float power = a.scale_log2 < 0.0f ? -power_of_two(up) : power_of_two(up);   // (a negative scale turns Q about: larger products are larger scores)
+            factor = power_of_two(-up) * fabsf(a.scale_log2);
+#pragma unroll 4
+            for (int c = 0; c < D; c += 8) {
+                const Four v = four_of(c), w = four_of(c + 4);
+                const uint32_t at = base + S::kQ + i * S::kTile + (c >> 6) * S::kHalf + row * 128 + ((((c >> 3) & 7) ^ (row & 7)) << 4);
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(two_halves(value_of(v.v[0]) * power, value_of(v.v[1]) * power)),
+                             "r"(two_halves(value_of(v.v[2]) * power, value_of(v.v[3]) * power)), "r"(two_halves(value_of(w.v[0]) * power, value_of(w.v[1]) * power)),
+                             "r"(two_halves(value_of(w.v[2]) * power, value_of(w.v[3]) * power))
+                             : "memory");
+            }
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_full);
+        }
+        const int common_lo = __reduce_max_sync(0xffffffffu, there ? row_lo : 0), common_hi = __reduce_min_sync(0xffffffffu, there ? row_hi : 0x7fffffff);
+        float r = -INFINITY, sum = 0.0f;
+        for (int j = 0; j < n[i]; ++j) {
+            const float4* scale = reinterpret_cast<const float4*>(smem + S::kScales + (j & (kScaleStages - 1)) * kRuns * 16);
+            if (ok) ok = mbar_wait_warp(scale_full(j & (kScaleStages - 1)), (j / kScaleStages) & 1, 727);
+            if (ok) ok = mbar_wait_warp(s_full(i), j & 1, 728);
+            if (!ok) break;
+            tc_fence_after();
+            const int key0 = (first + j) * kKeys;
+            const bool masked = key0 < common_lo || key0 + kKeys > common_hi;
+            const uint32_t from = static_cast<uint32_t>(row_lo - key0), span = static_cast<uint32_t>(row_hi - row_lo);   // column c is seen where c - from < span
+            float top = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint32_t raw[32];
+                tmem_load_32_now(s_tmem + c * 32, raw);
+                if (masked) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        if (static_cast<uint32_t>(c * 32 + e) - from >= span) raw[e] = 0xff800000u;
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float part[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2)
+                        asm("max.f32 %0, %0, %1, %2;" : "+f"(part[(e >> 1) & 1]) : "f"(__uint_as_float(raw[h * 16 + e])), "f"(__uint_as_float(raw[h * 16 + e + 1])));
+                    const float4 run = scale[c * 2 + h];
+                    top = fmaxf(top, fmaf(fmaxf(part[0], part[1]), factor * run.x, run.y));
+                }
+            }
+            const bool raise = top > r + kRaise || (r == -INFINITY && top > -INFINITY);
+            if (__any_sync(0xffffffffu, raise)) {
+                const float next = raise ? top : r, down = raise ? exp2_of(r - next) : 1.0f;
+                r = next;
+                sum *= down;
+                if (j > 0) {   // (the products before S are done: they run in order)
+#pragma unroll
+                    for (int c = 0; c < D; c += 32) {
+                        uint32_t acc[32];
+                        tmem_load_32_now(o_tmem + c, acc);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) acc[e] = __float_as_uint(__uint_as_float(acc[e]) * down);
+                        tmem_store_32(o_tmem + c, acc);
+                    }
+                    tmem_store_wait();
+                }
+            }
+            const float reference = r == -INFINITY ? 0.0f : r - kUp;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                uint32_t raw[32], p[16];
+                tmem_load_32_now(s_tmem + c * 32, raw);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float4 run = scale[c * 2 + h];
+                    const float f = factor * run.x, bias = run.y - reference;
+                    const uint64_t f2 = pack2(f, f), bias2 = pack2(bias, bias);
+                    uint64_t sums = pack2(0.0f, 0.0f);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        float x0, x1;
+                        unpack2(fma2(pack2(__uint_as_float(raw[h * 16 + 2 * e]), __uint_as_float(raw[h * 16 + 2 * e + 1])), f2, bias2), x0, x1);
+                        if (masked) {
+                            if (static_cast<uint32_t>(c * 32 + h * 16 + 2 * e) - from >= span) x0 = -INFINITY;
+                            if (static_cast<uint32_t>(c * 32 + h * 16 + 2 * e + 1) - from >= span) x1 = -INFINITY;
+                        }
+                        const float p0 = exp2_of(x0), p1 = exp2_of(x1);
+                        sums = add2(sums, pack2(p0, p1));
+                        p[h * 8 + e] = two_halves(p0, p1);
+                    }
+                    float s0, s1;
+                    unpack2(sums, s0, s1);
+                    sum = fmaf(s0 + s1, run.z, sum);
+                }
+                tmem_store_16(s_tmem + c * 16, p);
+            }
+            tmem_store_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full(i));
+        }
+        if (fabsf(r) > kMostReference && r != -INFINITY) misc[1] = 1;
+        // O, normalised
+        if (ok && n[i] > 0) ok = mbar_wait_warp(o_full(i), 0, 729);
+        tc_fence_after();
+        const bool healthy = ok && g_device_status == 0, none = !(sum != 0.0f);   // (a NaN sum is a NaN result)
+        const float inverse = 1.0f / sum;
+        const int64_t at = batch * a.o_stride[0] + head_q * a.o_stride[1] + token * a.o_stride[2];
+        if (ok) {
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+                uint32_t acc[32];
+                __syncwarp();
+                if (n[i] > 0) tmem_load_32_now(o_tmem + c, acc);
+                if (!there || !healthy) continue;
+#pragma unroll
+                for (int e = 0; e < 32; ++e) acc[e] = n[i] == 0 || none ? 0u : __float_as_uint(__uint_as_float(acc[e]) * inverse);
+                if (a.o_vector && a.o_type != DFGPU_F32) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        const float v0 = __uint_as_float(acc[e]), v1 = __uint_as_float(acc[e + 1]);
+                        *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.o) + at + c + e) =
+                            a.o_type == DFGPU_F16 ? two_halves(v0, v1) : static_cast<uint32_t>(f32_to_bf16_bits(v0)) | static_cast<uint32_t>(f32_to_bf16_bits(v1)) << 16;
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) store_from_f32(a.o, a.o_type, at + c + e, __uint_as_float(acc[e]));
+                }
+            }
+            if (there && healthy && a.stats)
+                a.stats[batch * a.stats_stride[0] + head_q * a.stats_stride[1] + token * a.stats_stride[2]] = none ? -INFINITY : kLn2 * (r - kUp) + logf(sum);
+        }
+        tc_fence_before();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (threadIdx.x == 0) args.flags[blockIdx.x] = misc[1];
+    if (warp == 12) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+}  // namespace
+
+bool cache_sdpa_umma_supported(const dfgpu_cache_sdpa_params& p) {
+    return (p.q.dim[3] == 64 || p.q.dim[3] == 128) && p.q.dim[1] / p.k.dim[1] <= kRows && cache_sdpa_umma_items(p) < (1ll << 30);
+}
+int64_t cache_sdpa_umma_items(const dfgpu_cache_sdpa_params& p) {
+    const int64_t tokens = kRows / (p.q.dim[1] / p.k.dim[1]);
+    return p.q.dim[0] * p.k.dim[1] * ((p.q.dim[2] + 2 * tokens - 1) / (2 * tokens));
+}
+
+int launch_cache_sdpa_umma(const dfgpu_cache_sdpa_params& p, const CacheSdpaArgs& a, int32_t* flags, cudaStream_t stream) {
+    CachePrefillArgs args{};
+    args.a = a;
+    args.flags = flags;
+    args.tokens = kRows / a.group;
+    args.blocks = (a.seq_q + 2 * args.tokens - 1) / (2 * args.tokens);
+    args.batches = static_cast<int>(p.q.dim[0]);
+    const dim3 grid(static_cast<unsigned>(cache_sdpa_umma_items(p)));
+    auto run = [&](auto kernel, int bytes) -> int {
+        const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (error != cudaSuccess) return fail(kExecutionFailed, "CACHE_SDPA: cannot reserve %d bytes of shared memory: %s", bytes, cudaGetErrorString(error));
+        launch_chained(kernel, grid, dim3(kThreads), bytes, stream, args);
+        return check_launch("CACHE_SDPA (tcgen05)");
+    };
+    const bool half = p.q.dtype == DFGPU_F16;
+    if (p.q.dim[3] == 64) return half ? run(cache_sdpa_umma_kernel<__half, 64>, Smem<64>::kDynamic) : run(cache_sdpa_umma_kernel<__nv_bfloat16, 64>, Smem<64>::kDynamic);
+    return half ? run(cache_sdpa_umma_kernel<__half, 128>, Smem<128>::kDynamic) : run(cache_sdpa_umma_kernel<__nv_bfloat16, 128>, Smem<128>::kDynamic);
+}
+
+int cache_sdpa_umma_device_status(int* status) { return read_and_clear_device_status(status); }
+
+}  // namespace dfgpu

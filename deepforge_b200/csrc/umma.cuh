@@ -117,6 +117,7 @@ int64_t decode_umma_scratch_bytes(const dfgpu_sdpa_params& p);
 int launch_decode_umma(const dfgpu_sdpa_params& p, void* const* tensors, void* scratch, const int* prefix_ok, cudaStream_t stream);  // prefix_ok: the validation result of compact page tables (null without them)
 int sdpa_device_status(int* status);  // (sdpa.cu: compact page table validation)
 int decode_umma_device_status(int* status);
-int cache_sdpa_device_status(int* status);   // (cache_sdpa.cu: attention over the 8-bit cache)
+int cache_sdpa_device_status(int* status);        // (cache_sdpa.cu: attention over the 8-bit cache)
+int cache_sdpa_umma_device_status(int* status);
 
 }  // namespace dfgpu

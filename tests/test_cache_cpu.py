@@ -130,6 +130,8 @@ def sdpa_params(**change):
 
 def test_sdpa_refusals():
     assert cache.query("cache_sdpa", sdpa_params()).kernel == cache.SDPA_STREAM
+    info = cache.query("cache_sdpa", sdpa_params(kernel=cache.SDPA_UMMA))
+    assert (info.kernel, info.launches) == (cache.SDPA_UMMA, 3) and info.scratch_bytes > cache.query("cache_sdpa", sdpa_params()).scratch_bytes
     refused(20, "cache_sdpa", sdpa_params(q=tensor(F32, [2, 8, 3, 64])))
     refused(20, "cache_sdpa", sdpa_params(o=tensor(F16, [2, 8, 3, 64])))
     refused(15, "cache_sdpa", sdpa_params(o=tensor(BF16, [2, 8, 2, 64])))
@@ -148,6 +150,10 @@ def test_sdpa_refusals():
     refused(1, "cache_sdpa", sdpa_params(kernel=9))
     d = 96
     refused(20, "cache_sdpa", sdpa_params(q=tensor(BF16, [2, 8, 3, d]), o=tensor(BF16, [2, 8, 3, d]), k=tensor(E4M3, [9, 4, 32, d]), v=tensor(E4M3, [9, 4, 32, d])))
+    d = 256
+    wide = dict(q=tensor(BF16, [2, 8, 3, d]), o=tensor(BF16, [2, 8, 3, d]), k=tensor(E4M3, [9, 4, 32, d]), v=tensor(E4M3, [9, 4, 32, d]))
+    assert cache.query("cache_sdpa", sdpa_params(**wide)).kernel == cache.SDPA_STREAM
+    refused(20, "cache_sdpa", sdpa_params(kernel=cache.SDPA_UMMA, **wide))
     good = [16, 16, 16, 16, None, 16, 16, None, 16, 16, 16]
     for i in (0, 1, 2, 3, 5, 6, 8, 9, 10):
         with pytest.raises(dfgpu.DfgpuError) as error:

@@ -317,6 +317,41 @@ def test_several_tokens(dtype, d, hk, g, sq, page, t, lengths, left):
     attend_case(d + sq, dtype, d, hk, g, sq, page, t, lengths, right=0, left=left, bottom_right=True)
 
 
+UMMA = cache.SDPA_UMMA
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("d,hk,g,sq,page,t,lengths,left", [
+    (128, 1, 1, 128, 64, 16, [128], None),
+    (128, 1, 4, 64, 64, 64, [300, 64], None),
+    (64, 2, 2, 200, 48, 16, [200, 333], None),
+    (128, 2, 5, 60, 32, 32, [500, 61, 60], None),
+    (64, 1, 16, 30, 16, 16, [129, 31], 40),
+    (128, 1, 3, 150, 256, 128, [1000], 200),
+    (128, 1, 70, 3, 64, 64, [260, 2], None),
+    (64, 1, 128, 2, 64, 16, [100], None),
+    (128, 2, 8, 1, 64, 16, [700, 0, 1], None),
+])
+def test_chunks_of_prompts_on_tcgen05(dtype, d, hk, g, sq, page, t, lengths, left):
+    _, _, info = attend_case(d + sq, dtype, d, hk, g, sq, page, t, lengths, right=0, left=left, bottom_right=True, kernel=UMMA)
+    assert info.kernel == UMMA
+
+
+def test_tcgen05_form_masks_and_types():
+    attend_case(1, BF16, 128, 2, 2, 70, 64, 16, [200, 90, 5], seq_q=[70, 3, 0], right=0, bottom_right=True, kernel=UMMA)
+    attend_case(2, BF16, 128, 1, 2, 70, 64, 16, [200, 90, 5], seq_q=[6, 90, -2], right=0, bottom_right=True, kernel=UMMA)
+    attend_case(3, BF16, 64, 2, 2, 150, 32, 16, [100, 8], right=0, kernel=UMMA)                                  # aligned to the top left
+    attend_case(4, F16, 64, 2, 2, 90, 32, 16, [100, 8], right=-2, left=50, bottom_right=True, kernel=UMMA)       # rows without keys
+    attend_case(5, BF16, 64, 1, 2, 90, 32, 16, [400, 8], left=0, kernel=UMMA)                                   # no right bound
+    attend_case(6, BF16, 128, 1, 4, 40, 64, 64, [700, 300], s_kv=450, kernel=UMMA)
+    attend_case(7, BF16, 128, 1, 4, 40, 64, 64, [700, -3], slots=11, right=2 ** 62, left=2 ** 62, kernel=UMMA)
+    attend_case(8, BF16, 128, 2, 4, 40, 64, 16, [300, 70], o_type=F32, right=0, bottom_right=True, kernel=UMMA)
+    attend_case(10, F16, 128, 2, 4, 40, 48, 16, [300, 77], layout="tokens", bad_pages=True, right=0, bottom_right=True, kernel=UMMA)
+    attend_case(13, BF16, 128, 1, 4, 40, 64, 16, [300, 70], q_scale=2.0 ** 70, kernel=UMMA)
+    attend_case(14, BF16, 128, 1, 4, 40, 64, 16, [300, 70], q_scale=2.0 ** -90, stats=False, kernel=UMMA)
+    attend_case(15, BF16, 128, 2, 2, 33, 64, 16, [40] * 130, right=0, bottom_right=True, kernel=UMMA)            # more sequences than are ranked
+
+
 def test_masks_lengths_and_types():
     attend_case(1, BF16, 128, 2, 2, 6, 64, 16, [200, 90, 5], seq_q=[6, 3, 0], right=0, bottom_right=True)       # padded query rows
     attend_case(2, BF16, 128, 2, 2, 6, 64, 16, [200, 90, 5], seq_q=[6, 9, -2], right=0, bottom_right=True)      # and lengths out of range
@@ -363,6 +398,21 @@ def test_scales_far_apart():
         caches[1][:, :, 48:] = 0
     attend_case(3, BF16, 128, 2, 4, 1, 64, 16, [300, 70], spoil=spoil)
     attend_case(3, BF16, 64, 2, 4, 5, 64, 16, [300, 70], spoil=spoil, right=0, bottom_right=True)
+    attend_case(3, BF16, 128, 1, 4, 50, 64, 16, [300, 70], spoil=spoil, right=0, bottom_right=True, kernel=UMMA)   # (left to the streaming form)
+
+
+def test_zeros_with_the_least_scale():
+    """Blocks of zeros as an append writes them, among others and alone."""
+    def spoil(q, caches, scales, tables):
+        caches[1][:, :, :16] = 0
+        scales[1][:, :, 0] = 0
+
+    def all_zero(q, caches, scales, tables):
+        caches[1].zero_()
+        scales[1].zero_()
+    for kernel, sq in ((0, 1), (0, 6), (UMMA, 40)):
+        attend_case(6, BF16, 128, 1, 4, sq, 64, 16, [300, 70], spoil=spoil, right=0, bottom_right=True, kernel=kernel)
+        attend_case(6, BF16, 64, 1, 4, sq, 64, 16, [300, 70], spoil=all_zero, right=0, bottom_right=True, kernel=kernel)
 
 
 @pytest.mark.parametrize("d", [64, 128, 256])
@@ -386,6 +436,8 @@ def test_nan_in_masked_places(d, sq):
             scales[which][table[1, last // page].item(), :, -1] = 255                 # a block that nobody reaches
     attend_case(d, BF16, d, 2, 2, sq, page, 16, lengths, spoil=spoil, right=0, bottom_right=True)
     attend_case(d, BF16, d, 2, 2, sq, page, 16, lengths, spoil=spoil, right=0, left=40, bottom_right=True)
+    if d < 256:
+        attend_case(d, BF16, d, 2, 2, sq, page, 16, lengths, spoil=spoil, right=0, bottom_right=True, kernel=UMMA)
 
 
 def test_a_block_above_the_diagonal_has_no_scale():
@@ -393,8 +445,9 @@ def test_a_block_above_the_diagonal_has_no_scale():
     def spoil(q, caches, scales, tables):
         scales[1][tables[1][0, 1].item(), :, 1] = 255
         scales[0][tables[0][0, 1].item(), :, 1] = 255
-    got, rows, _ = attend_case(1, BF16, 128, 1, 2, 20, 32, 16, [64], spoil=spoil, right=0, bottom_right=True)
-    assert bool(torch.isfinite(got[:, :, :4].float()).all()) and bool(torch.isnan(got[:, :, 4:].float()).all())
+    for kernel in (0, UMMA):
+        got, rows, _ = attend_case(1, BF16, 128, 1, 2, 20, 32, 16, [64], spoil=spoil, right=0, bottom_right=True, kernel=kernel)
+        assert bool(torch.isfinite(got[:, :, :4].float()).all()) and bool(torch.isnan(got[:, :, 4:].float()).all())
 
 
 def test_offsets_past_32_bits():
