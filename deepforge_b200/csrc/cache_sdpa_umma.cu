@@ -4,8 +4,9 @@
 // (exactly) before the tensor core can take them, and that is paid once for 256 rows: a CTA has two query tiles of 128 rows, (token, head of the
 // group) pairs of one KV head, and both read the same converted K and V tiles.
 //   warps 0-3, 4-7   softmax of query tile 0 and 1, a thread a row; Q to f16 at the start, O out of tensor memory at the end
-//   warps 8-11       codes from global memory (looked up and loaded a tile ahead, in registers) to f16 tiles in shared memory, two K and two V
-//   warp 12          issues the products: S = Q K^T, then O += P V with P from tensor memory, the two query tiles in turn
+//   warps 8-11, 12-15  codes of K and of V from global memory (looked up and loaded a tile ahead, in registers) to f16 tiles in shared memory, two of each
+//   warp 16          issues the products: S = Q K^T, then O += P V with P from tensor memory, the two query tiles in turn
+// (With four converting warps for both, these set the pace: 6500 clocks a pair of score tiles.)
 // Tensor memory: S (then P, in its place) of the query tiles at 0 and 128, O at 256 and 384.
 // Q is exact as in the streaming form (a power of two a row). The K scale of 16 keys is a factor of their scores. The V scale is
 // part of the exponent: with t = score + log2(V scale), a row's reference r follows the largest t, P = 2^(t - r + 11) in f16 multiplies codes, and the
@@ -13,7 +14,7 @@
 // is rescaled in tensor memory then, which is rare).
 // What this cannot do exactly it says in a flag of the item, and the streaming form then computes the whole call again (its kernels return at
 // once otherwise): a NaN among V codes of a tile that some rows do not see all of (their zero probability times it is NaN), a V
-// scale of 2^126 or more or a NaN, V scales more than 2^16
+// scale of 2^126 or more, a scale that is a NaN, V scales more than 2^16
 // apart or below 2^-80 over codes that are not zero, scores beyond 2^10.
 #include <algorithm>
 
@@ -25,12 +26,13 @@ namespace dfgpu {
 namespace {
 
 constexpr int kRows = 128, kKeys = 128, kRuns = kKeys / 16;
-constexpr int kThreads = 13 * 32, kConverters = 128;
+constexpr int kThreads = 17 * 32, kConverters = 128, kIssuer = 16;
 constexpr int kScaleStages = 4;      // (three are enough: a tile's K slot is free when both query tiles are done with the tile before)
 constexpr float kUp = 11.0f;         // P = 2^(t - r + 11): at most 2^15 while t is within 4 of r
 constexpr float kRaise = 4.0f;
 constexpr int kLeastCode = 47;       // V scales below 2^-80 count as that (over zeros; else a flag)
 constexpr int kMostApart = 16;
+constexpr float kLeastFactor = 1.17549435e-38f;   // (of a score: not zero, so that -inf stays -inf)
 constexpr float kMostReference = 1024.0f;   // |r|: the exponent's one rounding, of score * factor + (scale - r), is below 2^-14 up to there
 constexpr int kMostRanked = 128;     // sequences that are put in order of length
 constexpr float kLn2 = 0.6931471805599453f;
@@ -48,7 +50,7 @@ struct Smem {
     static constexpr int kHalves = D / 64, kHalf = kRows * 128;
     static constexpr int kTile = kHalves * kHalf;              // of f16: 128 rows by 64 channels, swizzled, once or twice
     static constexpr int kQ = 0, kK = 2 * kTile, kV = 4 * kTile;
-    static constexpr int kScales = 6 * kTile;                  // [stage][run]{K factor, log2 of V's, 1 / V's, -}
+    static constexpr int kScales = 6 * kTile;                  // [stage][run]{K factor, -, log2 of V's, 1 / V's}
     static constexpr int kBarriers = kScales + kScaleStages * kRuns * 16;
     // q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], scale_full[4]
     static constexpr int kBarrierCount = 1 + 14 + kScaleStages;
@@ -132,11 +134,11 @@ cache_sdpa_umma_kernel(const __grid_constant__ CachePrefillArgs args) {
             mbar_init(v_full(s), 4), mbar_init(v_empty(s), 1);
             mbar_init(s_full(s), 1), mbar_init(p_full(s), 4), mbar_init(o_full(s), 1);
         }
-        for (int s = 0; s < kScaleStages; ++s) mbar_init(scale_full(s), 4);
+        for (int s = 0; s < kScaleStages; ++s) mbar_init(scale_full(s), 2);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         misc[1] = 0;
     }
-    if (warp == 12) {
+    if (warp == kIssuer) {
         tmem_alloc(base + S::kMisc, 512);
         tmem_relinquish();
         tc_fence_before();
@@ -178,7 +180,7 @@ cache_sdpa_umma_kernel(const __grid_constant__ CachePrefillArgs args) {
     const int tiles = max(n[0], n[1]);
     bool ok = true;
 
-    if (warp == 12) {
+    if (warp == kIssuer) {
         // ---- the products
         const bool leader = elect_one();
         constexpr uint32_t idesc_s = (1u << 4) | (static_cast<uint32_t>(kKeys >> 3) << 17) | (static_cast<uint32_t>(kRows >> 4) << 24);   // f16 operands, f32 sums
@@ -227,7 +229,9 @@ cache_sdpa_umma_kernel(const __grid_constant__ CachePrefillArgs args) {
         }
     } else if (warp >= 8) {
         // ---- codes to f16
-        const int thread = threadIdx.x - 256, chunk = thread % kChunks, row0 = thread / kChunks;
+        const int which = warp >= 12 ? 1 : 0, thread = threadIdx.x - 256 - which * kConverters, chunk = thread % kChunks, row0 = thread / kChunks;
+        const bool writer = (warp & 3) == 0;   // of the scales
+        const CacheSide& side = a.side[which];
         int common_lo, common_hi;   // what all rows see
         {
             int l0, h0, l1, h1;
@@ -238,103 +242,94 @@ cache_sdpa_umma_kernel(const __grid_constant__ CachePrefillArgs args) {
         }
         int v_least = 1 << 20, v_most = -1;
         bool flag = false;
-        // Lane l < 16 has run l % 8 of K (l < 8) or V: its page (as the table has it), where it begins in it, and its scale.
-        const int side = lane >> 3 & 1, run = lane & 7;
+        // Lane l has run l % 8: its page (as the table has it), where it begins in it, and its scale.
+        const int run = lane & 7;
         auto look_up = [&](int j, int& page, int& token) {
             const int key = (first + j) * kKeys + run * 16, slot = static_cast<int>(fast_divide(static_cast<uint32_t>(key >> 4), a.by_page));
             token = key - slot * a.page;
-            const CacheSide& s = a.side[side];
-            page = j < tiles && key < all_hi && key + 16 > all_lo && slot < s.table_len ? s.table[batch * s.table_batch + slot * s.table_slot] : -1;
+            page = j < tiles && key < all_hi && key + 16 > all_lo && slot < side.table_len ? side.table[batch * side.table_batch + slot * side.table_slot] : -1;
         };
-        auto checked = [&](int page) { return page >= 0 && page < a.side[side].pages ? page : -1; };
+        auto checked = [&](int page) { return page >= 0 && page < side.pages ? page : -1; };
         auto look_up_scale = [&](int page, int token) {
-            const CacheSide& s = a.side[side];
-            return page >= 0 ? static_cast<int>(s.scales[page * s.scale_stride[0] + head * s.scale_stride[1] + fast_divide(static_cast<uint32_t>(token >> 4), a.by_tokens) * s.scale_stride[2]]) : -1;
+            return page >= 0 ? static_cast<int>(side.scales[page * side.scale_stride[0] + head * side.scale_stride[1] + fast_divide(static_cast<uint32_t>(token >> 4), a.by_tokens) * side.scale_stride[2]]) : -1;
         };
+        // Where a lane's run begins, -1 where there is no page.
+        auto offset_of = [&](int page, int token) { return page >= 0 ? page * side.stride[0] + head * side.stride[1] + token * side.stride[2] : -1ll; };
         // A tile's codes, 16 of a row at a time; zeros where there is no page and where no row sees the key.
-        auto load = [&](int which, int j, int page, int token, uint4 (&to)[kPasses]) {
-            const CacheSide& s = a.side[which];
-#pragma unroll
-            for (int i = 0; i < kPasses; ++i) {
-                const int row = i * kAtOnce + row0, from = which * 8 + (row >> 4), key = (first + j) * kKeys + row;
-                const int id = __shfl_sync(0xffffffffu, page, from), at = __shfl_sync(0xffffffffu, token, from) + (row & 15);
-                to[i] = make_uint4(0, 0, 0, 0);
-                if (id >= 0 && key >= all_lo && key < all_hi) to[i] = __ldcg(reinterpret_cast<const uint4*>(s.codes + id * s.stride[0] + head * s.stride[1] + at * s.stride[2] + chunk * 16));
-            }
-        };
-        auto convert = [&](uint32_t to, const uint4 (&from)[kPasses]) {
+        const uint8_t* own = side.codes + (row0 & 15) * side.stride[2] + chunk * 16;
+        uint4 raw[kPasses];
+        auto load = [&](int j, int64_t offset) {
+            const int key0 = (first + j) * kKeys;
+            const bool edge = key0 < all_lo || key0 + kKeys > all_hi;
 #pragma unroll
             for (int i = 0; i < kPasses; ++i) {
                 const int row = i * kAtOnce + row0;
-                uint32_t h[8];
-                four_codes(from[i].x, h[0], h[1]), four_codes(from[i].y, h[2], h[3]), four_codes(from[i].z, h[4], h[5]), four_codes(from[i].w, h[6], h[7]);
-                const uint32_t at = to + (chunk >> 2) * S::kHalf + row * 128, place = chunk * 2 & 7;
-                const int odd = chunk >> 2;   // (the halves lie in the same banks: their chunks go in opposite order)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int which = e ^ odd;
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + (((place + which) ^ (row & 7)) << 4)), "r"(which ? h[4] : h[0]), "r"(which ? h[5] : h[1]),
-                                 "r"(which ? h[6] : h[2]), "r"(which ? h[7] : h[3])
-                                 : "memory");
-                }
+                const int64_t at = __shfl_sync(0xffffffffu, offset, row >> 4);
+                raw[i] = make_uint4(0, 0, 0, 0);
+                if (at >= 0 && (!edge || (key0 + row >= all_lo && key0 + row < all_hi))) raw[i] = __ldcg(reinterpret_cast<const uint4*>(own + at));
             }
         };
+        const uint32_t tile_at = base + (which ? S::kV : S::kK), row_at = (chunk >> 2) * S::kHalf + row0 * 128, place = chunk * 2 & 7;
+        const bool odd = (chunk >> 2) != 0;   // (the halves lie in the same banks: their chunks go in opposite order)
+        const uint32_t first_at = row_at + (((place + (odd ? 1 : 0)) ^ (row0 & 7)) << 4), second_at = row_at + (((place + (odd ? 0 : 1)) ^ (row0 & 7)) << 4);   // (rows of later passes are 16 or 32 on: the same swizzle)
         int page, token, page_next, token_next, code;
-        uint4 k_raw[kPasses], v_raw[kPasses];
         look_up(0, page, token);
         look_up(1, page_next, token_next);
         page = checked(page);
         code = look_up_scale(page, token);
-        load(0, 0, page, token, k_raw);
-        load(1, 0, page, token, v_raw);
+        load(0, offset_of(page, token));
         for (int j = 0; j < tiles; ++j) {
             const int now = j & 1;
             page = checked(page_next), token = token_next;   // of tile j + 1
             look_up(j + 2, page_next, token_next);
             const int code_next = look_up_scale(page, token);
-            if (ok) ok = mbar_wait_warp(k_empty(now), ((j >> 1) & 1) ^ 1, 725);
-            if (!ok) break;
-            convert(base + S::kK + now * S::kTile, k_raw);
-            if (warp == 8) {
-                // (lanes 0-7 the K scales, 8-15 V's; a V scale that the exponent does not take counts as the least)
-                float* scale = reinterpret_cast<float*>(smem + S::kScales + ((j & (kScaleStages - 1)) * kRuns + run) * 16);
+            const int64_t offset = offset_of(page, token);
+            if (writer) {
                 if (lane < 8) {
-                    scale[0] = code < 0 ? 1.0f : decode_e8m0(static_cast<uint32_t>(code));
-                } else if (lane < 16) {
-                    const int exponent = max(code < 0 ? 127 : code, kLeastCode) - 127;
-                    scale[1] = static_cast<float>(exponent);
-                    scale[2] = power_of_two(max(-exponent, -126));
-                    if (code >= kLeastCode) v_least = min(v_least, code), v_most = max(v_most, code);
-                    flag = flag || code >= 253;   // (a NaN among them)
+                    // (a V scale that the exponent does not take counts as the least)
+                    float* scale = reinterpret_cast<float*>(smem + S::kScales + ((j & (kScaleStages - 1)) * kRuns + run) * 16);
+                    if (which == 0) {
+                        scale[0] = code < 0 ? 1.0f : decode_e8m0(static_cast<uint32_t>(code));
+                        flag = flag || code == 255;
+                    } else {
+                        const int exponent = max(code < 0 ? 127 : code, kLeastCode) - 127;
+                        *reinterpret_cast<float2*>(scale + 2) = make_float2(static_cast<float>(exponent), power_of_two(max(-exponent, -126)));
+                        if (code >= kLeastCode) v_least = min(v_least, code), v_most = max(v_most, code);
+                        flag = flag || code >= 253;   // (a NaN among them)
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(scale_full(j & (kScaleStages - 1)));
+            }
+            if (which == 1) {
+                const int key0 = (first + j) * kKeys;
+                const bool mixed = key0 < common_lo || key0 + kKeys > common_hi;
+                if (mixed || __any_sync(0xffffffffu, code >= 0 && code < kLeastCode)) {
+#pragma unroll
+                    for (int i = 0; i < kPasses; ++i) {
+                        const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+                        const int run_code = __shfl_sync(0xffffffffu, code, (i * kAtOnce + row0) >> 4);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            flag = flag || (mixed && (((w[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0) || (run_code >= 0 && run_code < kLeastCode && (w[e] & 0x7f7f7f7fu) != 0);
+                    }
                 }
             }
-            fence_async_shared();
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(k_full(now));
-                mbar_arrive(scale_full(j & (kScaleStages - 1)));
-            }
-            load(0, j + 1, page, token, k_raw);
-            const int key0 = (first + j) * kKeys;
-            const bool mixed = key0 < common_lo || key0 + kKeys > common_hi;
-            const bool low = __any_sync(0xffffffffu, lane >= 8 && lane < 16 && code >= 0 && code < kLeastCode);
-            if (mixed || low) {
-#pragma unroll
-                for (int i = 0; i < kPasses; ++i) {
-                    const uint32_t w[4] = {v_raw[i].x, v_raw[i].y, v_raw[i].z, v_raw[i].w};
-                    const int run_code = __shfl_sync(0xffffffffu, code, 8 + ((i * kAtOnce + row0) >> 4));
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        flag = flag || (mixed && (((w[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) != 0) || (run_code >= 0 && run_code < kLeastCode && (w[e] & 0x7f7f7f7fu) != 0);
-                }
-            }
-            if (ok) ok = mbar_wait_warp(v_empty(now), ((j >> 1) & 1) ^ 1, 726);
+            if (ok) ok = mbar_wait_warp(which ? v_empty(now) : k_empty(now), ((j >> 1) & 1) ^ 1, 725 + which);
             if (!ok) break;
-            convert(base + S::kV + now * S::kTile, v_raw);
+            const uint32_t to = tile_at + now * S::kTile;
+#pragma unroll
+            for (int i = 0; i < kPasses; ++i) {
+                uint32_t h[8];
+                four_codes(odd ? raw[i].z : raw[i].x, h[0], h[1]), four_codes(odd ? raw[i].w : raw[i].y, h[2], h[3]);
+                four_codes(odd ? raw[i].x : raw[i].z, h[4], h[5]), four_codes(odd ? raw[i].y : raw[i].w, h[6], h[7]);
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + first_at + i * (kAtOnce * 128)), "r"(h[0]), "r"(h[1]), "r"(h[2]), "r"(h[3]) : "memory");
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + second_at + i * (kAtOnce * 128)), "r"(h[4]), "r"(h[5]), "r"(h[6]), "r"(h[7]) : "memory");
+            }
             fence_async_shared();
             __syncwarp();
-            if (lane == 0) mbar_arrive(v_full(now));
-            load(1, j + 1, page, token, v_raw);
+            if (lane == 0) mbar_arrive(which ? v_full(now) : k_full(now));
+            load(j + 1, offset);
             code = code_next;
         }
         v_least = __reduce_min_sync(0xffffffffu, v_least), v_most = __reduce_max_sync(0xffffffffu, v_most);
@@ -392,6 +387,7 @@ cache_sdpa_umma_kernel(const __grid_constant__ CachePrefillArgs args) {
             const int key0 = (first + j) * kKeys;
             const bool masked = key0 < common_lo || key0 + kKeys > common_hi;
             const uint32_t from = static_cast<uint32_t>(row_lo - key0), span = static_cast<uint32_t>(row_hi - row_lo);   // column c is seen where c - from < span
+            // The largest t first, by runs of 16 keys (the scores are read a second time for their exponentials: 96 registers do not hold a row of them)
             float top = -INFINITY;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
@@ -409,7 +405,7 @@ cache_sdpa_umma_kernel(const __grid_constant__ CachePrefillArgs args) {
                     for (int e = 0; e < 16; e += 2)
                         asm("max.f32 %0, %0, %1, %2;" : "+f"(part[(e >> 1) & 1]) : "f"(__uint_as_float(raw[h * 16 + e])), "f"(__uint_as_float(raw[h * 16 + e + 1])));
                     const float4 run = scale[c * 2 + h];
-                    top = fmaxf(top, fmaf(fmaxf(part[0], part[1]), factor * run.x, run.y));
+                    top = fmaxf(top, fmaf(fmaxf(part[0], part[1]), fmaxf(factor * run.x, kLeastFactor), run.z));
                 }
             }
             const bool raise = top > r + kRaise || (r == -INFINITY && top > -INFINITY);
@@ -418,7 +414,7 @@ cache_sdpa_umma_kernel(const __grid_constant__ CachePrefillArgs args) {
                 r = next;
                 sum *= down;
                 if (j > 0) {   // (the products before S are done: they run in order)
-#pragma unroll
+#pragma unroll 1
                     for (int c = 0; c < D; c += 32) {
                         uint32_t acc[32];
                         tmem_load_32_now(o_tmem + c, acc);
@@ -426,7 +422,6 @@ cache_sdpa_umma_kernel(const __grid_constant__ CachePrefillArgs args) {
                         for (int e = 0; e < 32; ++e) acc[e] = __float_as_uint(__uint_as_float(acc[e]) * down);
                         tmem_store_32(o_tmem + c, acc);
                     }
-                    tmem_store_wait();
                 }
             }
             const float reference = r == -INFINITY ? 0.0f : r - kUp;
@@ -434,29 +429,30 @@ cache_sdpa_umma_kernel(const __grid_constant__ CachePrefillArgs args) {
             for (int c = 0; c < 4; ++c) {
                 uint32_t raw[32], p[16];
                 tmem_load_32_now(s_tmem + c * 32, raw);
+                if (masked) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e)
+                        if (static_cast<uint32_t>(c * 32 + e) - from >= span) raw[e] = 0xff800000u;
+                }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const float4 run = scale[c * 2 + h];
-                    const float f = factor * run.x, bias = run.y - reference;
+                    const float f = fmaxf(factor * run.x, kLeastFactor), bias = run.z - reference;
                     const uint64_t f2 = pack2(f, f), bias2 = pack2(bias, bias);
                     uint64_t sums = pack2(0.0f, 0.0f);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         float x0, x1;
                         unpack2(fma2(pack2(__uint_as_float(raw[h * 16 + 2 * e]), __uint_as_float(raw[h * 16 + 2 * e + 1])), f2, bias2), x0, x1);
-                        if (masked) {
-                            if (static_cast<uint32_t>(c * 32 + h * 16 + 2 * e) - from >= span) x0 = -INFINITY;
-                            if (static_cast<uint32_t>(c * 32 + h * 16 + 2 * e + 1) - from >= span) x1 = -INFINITY;
-                        }
                         const float p0 = exp2_of(x0), p1 = exp2_of(x1);
                         sums = add2(sums, pack2(p0, p1));
                         p[h * 8 + e] = two_halves(p0, p1);
                     }
-                    float s0, s1;
-                    unpack2(sums, s0, s1);
-                    sum = fmaf(s0 + s1, run.z, sum);
+                    float sum0, sum1;
+                    unpack2(sums, sum0, sum1);
+                    sum = fmaf(sum0 + sum1, run.w, sum);
                 }
-                tmem_store_16(s_tmem + c * 16, p);
+                tmem_store_16(s_tmem + c * 16, p);   // (over scores that have been read)
             }
             tmem_store_wait();
             tc_fence_before();
@@ -499,7 +495,7 @@ cache_sdpa_umma_kernel(const __grid_constant__ CachePrefillArgs args) {
     tc_fence_before();
     __syncthreads();
     if (threadIdx.x == 0) args.flags[blockIdx.x] = misc[1];
-    if (warp == 12) {
+    if (warp == kIssuer) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
     }
