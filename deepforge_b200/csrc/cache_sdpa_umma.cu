@@ -7,7 +7,9 @@
 //   warps 8-11, 12-15  codes of K and of V from global memory (looked up and loaded a tile ahead, in registers) to f16 tiles in shared memory, two of each
 //   warp 16          issues the products: S = Q K^T, then O += P V with P from tensor memory, the two query tiles in turn
 // (With four converting warps for both, these set the pace: 6500 clocks a pair of score tiles.)
-// Tensor memory: S (then P, in its place) of the query tiles at 0 and 128, O at 256 and 384.
+// Tensor memory: S (then P, in its place) of the query tiles at 0 and 128, O at 256 and 384. S comes in halves of 64 keys, two a query
+// tile: the next half's scores are made while a half's softmax is under way, so that no softmax waits for a product (with whole tiles each waited
+// 1250 of 4900 clocks), and a half of a row fits a thread's registers, so that scores are read once.
 // Q is exact as in the streaming form (a power of two a row). The K scale of 16 keys is a factor of their scores. The V scale is
 // part of the exponent: with t = score + log2(V scale), a row's reference r follows the largest t, P = 2^(t - r + 11) in f16 multiplies codes, and the
 // row's sum adds up P / (V scale), so nothing but the final division knows of either. r is raised when t passes it by 2^4 (O
@@ -25,7 +27,7 @@
 namespace dfgpu {
 namespace {
 
-constexpr int kRows = 128, kKeys = 128, kRuns = kKeys / 16;
+constexpr int kRows = 128, kKeys = 128, kHalfKeys = 64, kRuns = kKeys / 16;
 constexpr int kThreads = 17 * 32, kConverters = 128, kIssuer = 16;
 constexpr int kScaleStages = 4;      // (three are enough: a tile's K slot is free when both query tiles are done with the tile before)
 constexpr float kUp = 11.0f;         // P = 2^(t - r + 11): at most 2^15 while t is within 4 of r
@@ -52,8 +54,8 @@ struct Smem {
     static constexpr int kQ = 0, kK = 2 * kTile, kV = 4 * kTile;
     static constexpr int kScales = 6 * kTile;                  // [stage][run]{K factor, -, log2 of V's, 1 / V's}
     static constexpr int kBarriers = kScales + kScaleStages * kRuns * 16;
-    // q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_full[2], scale_full[4]
-    static constexpr int kBarrierCount = 1 + 14 + kScaleStages;
+    // q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], o_full[2], pv_done[2], s_full[tile][half], p_full[tile][half], scale_full[4]
+    static constexpr int kBarrierCount = 1 + 20 + kScaleStages;
     static constexpr int kMisc = kBarriers + kBarrierCount * 8;    // tensor memory's address, flag, {least, largest} V scale by converter warp
     static constexpr int kTotal = kMisc + 64;
     static constexpr int kDynamic = kTotal + 1024;
@@ -70,16 +72,18 @@ __device__ __forceinline__ void tmem_store_16(uint32_t taddr, const uint32_t (&r
           "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
-__device__ __forceinline__ void tmem_store_32(uint32_t taddr, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_load_16_now(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
-        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-          "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
-          "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr) : "memory");
+}
+// Waits for the loads in flight; their registers pass through, so that nothing that reads them stands above the wait.
+__device__ __forceinline__ void tmem_load_wait_both(uint32_t (&a)[32], uint32_t (&b)[32]) {
+    tmem_load_wait();
+#pragma unroll
+    for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(a[i]), "+r"(b[i])::"memory");
 }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // D[tmem] (+)= A[tmem] * B[smem]: A are pairs of f16, one row per lane.
@@ -121,10 +125,11 @@ cache_sdpa_umma_kernel(const __grid_constant__ CachePrefillArgs args) {
     auto k_empty = [&](int s) { return bars + 8u * (3 + s); };
     auto v_full = [&](int s) { return bars + 8u * (5 + s); };
     auto v_empty = [&](int s) { return bars + 8u * (7 + s); };
-    auto s_full = [&](int i) { return bars + 8u * (9 + i); };
-    auto p_full = [&](int i) { return bars + 8u * (11 + i); };
-    auto o_full = [&](int i) { return bars + 8u * (13 + i); };
-    auto scale_full = [&](int s) { return bars + 8u * (15 + s); };
+    auto o_full = [&](int i) { return bars + 8u * (9 + i); };
+    auto pv_done = [&](int i) { return bars + 8u * (11 + i); };
+    auto s_full = [&](int i, int h) { return bars + 8u * (13 + 2 * i + (h & 1)); };
+    auto p_full = [&](int i, int h) { return bars + 8u * (17 + 2 * i + (h & 1)); };
+    auto scale_full = [&](int s) { return bars + 8u * (21 + s); };
     int* misc = reinterpret_cast<int*>(smem + S::kMisc);
     const int warp = uniform_warp_index(), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -132,7 +137,8 @@ cache_sdpa_umma_kernel(const __grid_constant__ CachePrefillArgs args) {
         for (int s = 0; s < 2; ++s) {
             mbar_init(k_full(s), 4), mbar_init(k_empty(s), 1);
             mbar_init(v_full(s), 4), mbar_init(v_empty(s), 1);
-            mbar_init(s_full(s), 1), mbar_init(p_full(s), 4), mbar_init(o_full(s), 1);
+            mbar_init(o_full(s), 1), mbar_init(pv_done(s), 1);
+            for (int h = 0; h < 2; ++h) mbar_init(s_full(s, h), 1), mbar_init(p_full(s, h), 4);
         }
         for (int s = 0; s < kScaleStages; ++s) mbar_init(scale_full(s), 2);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -176,56 +182,65 @@ cache_sdpa_umma_kernel(const __grid_constant__ CachePrefillArgs args) {
     const bool some[2] = {hi[0] > lo[0], hi[1] > lo[1]};
     const int all_lo = some[0] && some[1] ? min(lo[0], lo[1]) : some[0] ? lo[0] : lo[1], all_hi = max(hi[0], hi[1]);
     const int first = all_lo / kKeys;
-    const int n[2] = {some[0] ? (hi[0] + kKeys - 1) / kKeys - first : 0, some[1] ? (hi[1] + kKeys - 1) / kKeys - first : 0};
-    const int tiles = max(n[0], n[1]);
+    // halves of key tiles that a query tile walks
+    const int n[2] = {some[0] ? (hi[0] - first * kKeys + kHalfKeys - 1) / kHalfKeys : 0, some[1] ? (hi[1] - first * kKeys + kHalfKeys - 1) / kHalfKeys : 0};
+    const int halves = max(n[0], n[1]), tiles = (halves + 1) / 2;
     bool ok = true;
 
     if (warp == kIssuer) {
         // ---- the products
         const bool leader = elect_one();
-        constexpr uint32_t idesc_s = (1u << 4) | (static_cast<uint32_t>(kKeys >> 3) << 17) | (static_cast<uint32_t>(kRows >> 4) << 24);   // f16 operands, f32 sums
+        constexpr uint32_t idesc_s = (1u << 4) | (static_cast<uint32_t>(kHalfKeys >> 3) << 17) | (static_cast<uint32_t>(kRows >> 4) << 24);   // f16 operands, f32 sums
         constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | (static_cast<uint32_t>(D >> 3) << 17) | (static_cast<uint32_t>(kRows >> 4) << 24);   // V read MN-major
         const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
         if (tiles > 0) ok = mbar_wait_warp(q_full, 0, 721);
-        auto scores = [&](int i, int j) {
+        // S of half h of query tile i, over P of half h - 2, which the products before it have read: they run in order.
+        auto scores = [&](int i, int h) {
+            const int j = h >> 1;
             if (ok) ok = mbar_wait_warp(k_full(j & 1), (j >> 1) & 1, 722);
             tc_fence_after();
             if (leader && ok) {
-                const uint32_t q_lo = smem_desc_lo(base + S::kQ + i * S::kTile, 16), k_lo = smem_desc_lo(base + S::kK + (j & 1) * S::kTile, 16);
+                const uint32_t q_lo = smem_desc_lo(base + S::kQ + i * S::kTile, 16), k_lo = smem_desc_lo(base + S::kK + (j & 1) * S::kTile + (h & 1) * (kHalfKeys * 128), 16);
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {
                     const uint32_t at = ((k >> 2) * S::kHalf + (k & 3) * 32) >> 4;
-                    umma_bf16(tmem_u + i * 128, desc_words(q_lo + at, smem_desc_hi(1024)), desc_words(k_lo + at, smem_desc_hi(1024)), idesc_s, k != 0 ? 1u : 0u);
+                    umma_bf16(tmem_u + i * 128 + (h & 1) * kHalfKeys, desc_words(q_lo + at, smem_desc_hi(1024)), desc_words(k_lo + at, smem_desc_hi(1024)), idesc_s, k != 0 ? 1u : 0u);
                 }
-                umma_commit(s_full(i));
+                umma_commit(s_full(i, h));
             }
             __syncwarp();
         };
-        for (int i = 0; i < 2; ++i)
-            if (n[i] > 0) scores(i, 0);
-        if (leader && ok && tiles > 0) umma_commit(k_empty(0));
-        for (int j = 0; j < tiles && ok; ++j) {
+        // K of a tile is free behind its last scores, of the second half, or of the first where that is the last there is.
+        auto release_k = [&](int h) {
+            if (leader && ok && h < halves && ((h & 1) != 0 || h + 1 == halves)) umma_commit(k_empty((h >> 1) & 1));
+            __syncwarp();
+        };
+        for (int h = 0; h < 2; ++h) {
+            for (int i = 0; i < 2; ++i)
+                if (h < n[i]) scores(i, h);
+            release_k(h);
+        }
+        for (int h = 0; h < halves && ok; ++h) {
+            const int j = h >> 1;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                if (j >= n[i]) continue;
-                if (ok) ok = mbar_wait_warp(p_full(i), j & 1, 723);
+                if (h >= n[i]) continue;
+                if (ok) ok = mbar_wait_warp(p_full(i, h), (h >> 1) & 1, 723);
                 if (ok) ok = mbar_wait_warp(v_full(j & 1), (j >> 1) & 1, 724);
                 tc_fence_after();
                 if (leader && ok) {
-                    const uint32_t v_lo = smem_desc_lo(base + S::kV + (j & 1) * S::kTile, S::kHalf);
+                    const uint32_t v_lo = smem_desc_lo(base + S::kV + (j & 1) * S::kTile + (h & 1) * (kHalfKeys * 128), S::kHalf);
 #pragma unroll
-                    for (int k = 0; k < kKeys / 16; ++k)
-                        umma_a_tmem(tmem_u + 256 + i * 128, tmem_u + i * 128 + k * 8, desc_words(v_lo + ((k * 2048) >> 4), smem_desc_hi(1024)), idesc_o, (j | k) != 0 ? 1u : 0u);
-                    if (j + 1 == n[i]) umma_commit(o_full(i));
+                    for (int k = 0; k < kHalfKeys / 16; ++k)
+                        umma_a_tmem(tmem_u + 256 + i * 128, tmem_u + i * 128 + (h & 1) * kHalfKeys + k * 8, desc_words(v_lo + ((k * 2048) >> 4), smem_desc_hi(1024)), idesc_o, (h | k) != 0 ? 1u : 0u);
+                    umma_commit(pv_done(i));
+                    if (h + 1 == n[i]) umma_commit(o_full(i));
                 }
                 __syncwarp();
-                if (j + 1 < n[i]) scores(i, j + 1);   // (over P, which the products before have read: they run in order)
+                if (h + 2 < n[i]) scores(i, h + 2);
             }
-            if (leader && ok) {
-                umma_commit(v_empty(j & 1));
-                if (j + 1 < tiles) umma_commit(k_empty((j + 1) & 1));
-            }
-            __syncwarp();
+            if (leader && ok && ((h & 1) != 0 || h + 1 == halves)) umma_commit(v_empty(j & 1));
+            release_k(h + 2);
         }
     } else if (warp >= 8) {
         // ---- codes to f16
@@ -378,86 +393,86 @@ cache_sdpa_umma_kernel(const __grid_constant__ CachePrefillArgs args) {
         }
         const int common_lo = __reduce_max_sync(0xffffffffu, there ? row_lo : 0), common_hi = __reduce_min_sync(0xffffffffu, there ? row_hi : 0x7fffffff);
         float r = -INFINITY, sum = 0.0f;
-        for (int j = 0; j < n[i]; ++j) {
-            const float4* scale = reinterpret_cast<const float4*>(smem + S::kScales + (j & (kScaleStages - 1)) * kRuns * 16);
+        for (int h = 0; h < n[i]; ++h) {
+            const int j = h >> 1;
+            const float4* scale = reinterpret_cast<const float4*>(smem + S::kScales + ((j & (kScaleStages - 1)) * kRuns + (h & 1) * (kRuns / 2)) * 16);
             if (ok) ok = mbar_wait_warp(scale_full(j & (kScaleStages - 1)), (j / kScaleStages) & 1, 727);
-            if (ok) ok = mbar_wait_warp(s_full(i), j & 1, 728);
+            if (ok) ok = mbar_wait_warp(s_full(i, h), (h >> 1) & 1, 728);
             if (!ok) break;
             tc_fence_after();
-            const int key0 = (first + j) * kKeys;
-            const bool masked = key0 < common_lo || key0 + kKeys > common_hi;
-            const uint32_t from = static_cast<uint32_t>(row_lo - key0), span = static_cast<uint32_t>(row_hi - row_lo);   // column c is seen where c - from < span
-            // The largest t first, by runs of 16 keys (the scores are read a second time for their exponentials: 96 registers do not hold a row of them)
+            const int key0 = first * kKeys + h * kHalfKeys;
+            const bool masked = key0 < common_lo || key0 + kHalfKeys > common_hi;
+            const uint32_t own_s = s_tmem + (h & 1) * kHalfKeys;
+            uint32_t raw[2][32];
+            tmem_load_32(own_s, raw[0]);
+            tmem_load_32(own_s + 32, raw[1]);
+            tmem_load_wait_both(raw[0], raw[1]);
+            if (masked) {
+                const uint32_t from = static_cast<uint32_t>(row_lo - key0), span = static_cast<uint32_t>(row_hi - row_lo);   // column c is seen where c - from < span
+#pragma unroll
+                for (int c = 0; c < 64; ++c)
+                    if (static_cast<uint32_t>(c) - from >= span) raw[c >> 5][c & 31] = 0xff800000u;
+            }
+            // the largest t, by runs of 16 keys
             float top = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t raw[32];
-                tmem_load_32_now(s_tmem + c * 32, raw);
-                if (masked) {
+            for (int run = 0; run < 4; ++run) {
+                float part[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if (static_cast<uint32_t>(c * 32 + e) - from >= span) raw[e] = 0xff800000u;
-                }
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float part[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-                    for (int e = 0; e < 16; e += 2)
-                        asm("max.f32 %0, %0, %1, %2;" : "+f"(part[(e >> 1) & 1]) : "f"(__uint_as_float(raw[h * 16 + e])), "f"(__uint_as_float(raw[h * 16 + e + 1])));
-                    const float4 run = scale[c * 2 + h];
-                    top = fmaxf(top, fmaf(fmaxf(part[0], part[1]), fmaxf(factor * run.x, kLeastFactor), run.z));
-                }
+                for (int e = 0; e < 16; e += 2)
+                    asm("max.f32 %0, %0, %1, %2;" : "+f"(part[(e >> 1) & 1]) : "f"(__uint_as_float(raw[run >> 1][(run & 1) * 16 + e])), "f"(__uint_as_float(raw[run >> 1][(run & 1) * 16 + e + 1])));
+                const float4 of = scale[run];
+                top = fmaxf(top, fmaf(fmaxf(part[0], part[1]), fmaxf(factor * of.x, kLeastFactor), of.z));
             }
             const bool raise = top > r + kRaise || (r == -INFINITY && top > -INFINITY);
             if (__any_sync(0xffffffffu, raise)) {
                 const float next = raise ? top : r, down = raise ? exp2_of(r - next) : 1.0f;
                 r = next;
                 sum *= down;
-                if (j > 0) {   // (the products before S are done: they run in order)
+                if (h > 0) {   // (S of this half came behind the products of all halves but the last)
+                    if (ok) ok = mbar_wait_warp(pv_done(i), (h - 1) & 1, 730);
+                    tc_fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < D; c += 32) {
-                        uint32_t acc[32];
-                        tmem_load_32_now(o_tmem + c, acc);
+                    for (int c = 0; c < D; c += 16) {
+                        uint32_t acc[16];
+                        tmem_load_16_now(o_tmem + c, acc);
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) acc[e] = __float_as_uint(__uint_as_float(acc[e]) * down);
-                        tmem_store_32(o_tmem + c, acc);
+                        for (int e = 0; e < 16; ++e) acc[e] = __float_as_uint(__uint_as_float(acc[e]) * down);
+                        tmem_store_16(o_tmem + c, acc);
                     }
                 }
             }
             const float reference = r == -INFINITY ? 0.0f : r - kUp;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t raw[32], p[16];
-                tmem_load_32_now(s_tmem + c * 32, raw);
-                if (masked) {
+            for (int run = 0; run < 4; ++run) {
+                const float4 of = scale[run];
+                const float f = fmaxf(factor * of.x, kLeastFactor), bias = of.z - reference;
+                const uint64_t f2 = pack2(f, f), bias2 = pack2(bias, bias);
+                uint64_t sums = pack2(0.0f, 0.0f);
 #pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        if (static_cast<uint32_t>(c * 32 + e) - from >= span) raw[e] = 0xff800000u;
+                for (int e = 0; e < 8; ++e) {
+                    const int at = (run & 1) * 16 + 2 * e;
+                    float x0, x1;
+                    unpack2(fma2(pack2(__uint_as_float(raw[run >> 1][at]), __uint_as_float(raw[run >> 1][at + 1])), f2, bias2), x0, x1);
+                    const float p0 = exp2_of(x0), p1 = exp2_of(x1);
+                    sums = add2(sums, pack2(p0, p1));
+                    raw[run >> 1][(run & 1) * 8 + e] = two_halves(p0, p1);   // (the first halves of the array take the pairs: what lay there has been read)
                 }
+                float sum0, sum1;
+                unpack2(sums, sum0, sum1);
+                sum = fmaf(sum0 + sum1, of.w, sum);
+            }
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float4 run = scale[c * 2 + h];
-                    const float f = fmaxf(factor * run.x, kLeastFactor), bias = run.z - reference;
-                    const uint64_t f2 = pack2(f, f), bias2 = pack2(bias, bias);
-                    uint64_t sums = pack2(0.0f, 0.0f);
+            for (int c = 0; c < 2; ++c) {
+                uint32_t p[16];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        float x0, x1;
-                        unpack2(fma2(pack2(__uint_as_float(raw[h * 16 + 2 * e]), __uint_as_float(raw[h * 16 + 2 * e + 1])), f2, bias2), x0, x1);
-                        const float p0 = exp2_of(x0), p1 = exp2_of(x1);
-                        sums = add2(sums, pack2(p0, p1));
-                        p[h * 8 + e] = two_halves(p0, p1);
-                    }
-                    float sum0, sum1;
-                    unpack2(sums, sum0, sum1);
-                    sum = fmaf(sum0 + sum1, run.w, sum);
-                }
-                tmem_store_16(s_tmem + c * 16, p);   // (over scores that have been read)
+                for (int e = 0; e < 16; ++e) p[e] = raw[c][e];
+                tmem_store_16(own_s + c * 16, p);
             }
             tmem_store_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(p_full(i));
+            if (lane == 0) mbar_arrive(p_full(i, h));
         }
         if (fabsf(r) > kMostReference && r != -INFINITY) misc[1] = 1;
         // O, normalised

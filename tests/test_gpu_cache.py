@@ -415,6 +415,15 @@ def test_zeros_with_the_least_scale():
         attend_case(6, BF16, 64, 1, 4, sq, 64, 16, [300, 70], spoil=all_zero, right=0, bottom_right=True, kernel=kernel)
 
 
+@pytest.mark.parametrize("kernel,sq", [(0, 1), (0, 9), (UMMA, 50)])
+def test_nan_and_infinity_in_queries_and_seen_keys(kernel, sq):
+    def spoil(q, caches, scales, tables):
+        q[0, 1, 0, 5], q[1, 2, -1, 100] = float("inf"), float("nan")
+        caches[0][tables[0][0, 1].item(), 0, 7, ::9] = 0xFF       # key 71: seen by every row of its sequence but the first
+        caches[1][tables[1][1, 0].item(), 0, 9, 3] = 0x7F
+    got, _, _ = attend_case(2, BF16, 128, 1, 4, sq, 64, 16, [60 + sq + 11, 150], spoil=spoil, right=0, bottom_right=True, kernel=kernel)
+
+
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("sq", [1, 6, 30])
 def test_nan_in_masked_places(d, sq):
