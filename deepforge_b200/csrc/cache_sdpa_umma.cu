@@ -5,8 +5,8 @@
 // group) pairs of one KV head, and both read the same converted K and V tiles.
 //   warps 0-3, 4-7   softmax of query tile 0 and 1, a thread a row; Q to f16 at the start, O out of tensor memory at the end
 //   warps 8-11, 12-15  codes of K and of V from global memory (looked up and loaded a tile ahead, in registers) to f16 tiles in shared memory, two of each
-//   warp 16          issues the products: S = Q K^T, then O += P V with P from tensor memory, the two query tiles in turn
-// (With four converting warps for both, these set the pace: 6500 clocks a pair of score tiles.)
+//   warp 16, 17      issue the products, S = Q K^T and O += P V with P from tensor memory, the two query tiles in turn
+// (With four converting warps for both, these set the pace: 6500 clocks a pair of score tiles; with one issuing warp, it did: 75 clocks a product, 3600.)
 // Tensor memory: S (then P, in its place) of the query tiles at 0 and 128, O at 256 and 384. S comes in halves of 64 keys, two a query
 // tile: the next half's scores are made while a half's softmax is under way, so that no softmax waits for a product (with whole tiles each waited
 // 1250 of 4900 clocks), and a half of a row fits a thread's registers, so that scores are read once.
@@ -28,8 +28,8 @@ namespace dfgpu {
 namespace {
 
 constexpr int kRows = 128, kKeys = 128, kHalfKeys = 64, kRuns = kKeys / 16;
-constexpr int kThreads = 17 * 32, kConverters = 128, kIssuer = 16;
-constexpr int kScaleStages = 4;      // (three are enough: a tile's K slot is free when both query tiles are done with the tile before)
+constexpr int kThreads = 18 * 32, kConverters = 128, kIssuer = 16;   // (the first of the issuing warps has the tensor memory)
+constexpr int kScaleStages = 4;      // (K's converters write tile j's with K of j - 3 used up: its last scores came behind the products with V of j - 4, and those behind all softmax of j - 4, as the second query tile, which comes last, sees as many halves as the first or none)
 constexpr float kUp = 11.0f;         // P = 2^(t - r + 11): at most 2^15 while t is within 4 of r
 constexpr float kRaise = 4.0f;
 constexpr int kLeastCode = 47;       // V scales below 2^-80 count as that (over zeros; else a flag)
@@ -54,8 +54,8 @@ struct Smem {
     static constexpr int kQ = 0, kK = 2 * kTile, kV = 4 * kTile;
     static constexpr int kScales = 6 * kTile;                  // [stage][run]{K factor, -, log2 of V's, 1 / V's}
     static constexpr int kBarriers = kScales + kScaleStages * kRuns * 16;
-    // q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], o_full[2], pv_done[2], s_full[tile][half], p_full[tile][half], scale_full[4]
-    static constexpr int kBarrierCount = 1 + 20 + kScaleStages;
+    // q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], o_full[2], pv_done[tile][half], s_full[tile][half], p_full[tile][half], scale_full[4]
+    static constexpr int kBarrierCount = 1 + 22 + kScaleStages;
     static constexpr int kMisc = kBarriers + kBarrierCount * 8;    // tensor memory's address, flag, {least, largest} V scale by converter warp
     static constexpr int kTotal = kMisc + 64;
     static constexpr int kDynamic = kTotal + 1024;
@@ -126,10 +126,10 @@ cache_sdpa_umma_kernel(const __grid_constant__ CachePrefillArgs args) {
     auto v_full = [&](int s) { return bars + 8u * (5 + s); };
     auto v_empty = [&](int s) { return bars + 8u * (7 + s); };
     auto o_full = [&](int i) { return bars + 8u * (9 + i); };
-    auto pv_done = [&](int i) { return bars + 8u * (11 + i); };
-    auto s_full = [&](int i, int h) { return bars + 8u * (13 + 2 * i + (h & 1)); };
-    auto p_full = [&](int i, int h) { return bars + 8u * (17 + 2 * i + (h & 1)); };
-    auto scale_full = [&](int s) { return bars + 8u * (21 + s); };
+    auto pv_done = [&](int i, int h) { return bars + 8u * (11 + 2 * i + (h & 1)); };   // (by half: a late look at one barrier for both could find half h - 1 done and take it for h - 3)
+    auto s_full = [&](int i, int h) { return bars + 8u * (15 + 2 * i + (h & 1)); };
+    auto p_full = [&](int i, int h) { return bars + 8u * (19 + 2 * i + (h & 1)); };
+    auto scale_full = [&](int s) { return bars + 8u * (23 + s); };
     int* misc = reinterpret_cast<int*>(smem + S::kMisc);
     const int warp = uniform_warp_index(), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -137,8 +137,8 @@ cache_sdpa_umma_kernel(const __grid_constant__ CachePrefillArgs args) {
         for (int s = 0; s < 2; ++s) {
             mbar_init(k_full(s), 4), mbar_init(k_empty(s), 1);
             mbar_init(v_full(s), 4), mbar_init(v_empty(s), 1);
-            mbar_init(o_full(s), 1), mbar_init(pv_done(s), 1);
-            for (int h = 0; h < 2; ++h) mbar_init(s_full(s, h), 1), mbar_init(p_full(s, h), 4);
+            mbar_init(o_full(s), 1);
+            for (int h = 0; h < 2; ++h) mbar_init(s_full(s, h), 1), mbar_init(p_full(s, h), 4), mbar_init(pv_done(s, h), 1);
         }
         for (int s = 0; s < kScaleStages; ++s) mbar_init(scale_full(s), 2);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -187,60 +187,59 @@ cache_sdpa_umma_kernel(const __grid_constant__ CachePrefillArgs args) {
     const int halves = max(n[0], n[1]), tiles = (halves + 1) / 2;
     bool ok = true;
 
-    if (warp == kIssuer) {
+    if (warp >= kIssuer) {
         // ---- the products
         const bool leader = elect_one();
         constexpr uint32_t idesc_s = (1u << 4) | (static_cast<uint32_t>(kHalfKeys >> 3) << 17) | (static_cast<uint32_t>(kRows >> 4) << 24);   // f16 operands, f32 sums
         constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | (static_cast<uint32_t>(D >> 3) << 17) | (static_cast<uint32_t>(kRows >> 4) << 24);   // V read MN-major
         const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
-        if (tiles > 0) ok = mbar_wait_warp(q_full, 0, 721);
-        // S of half h of query tile i, over P of half h - 2, which the products before it have read: they run in order.
-        auto scores = [&](int i, int h) {
-            const int j = h >> 1;
-            if (ok) ok = mbar_wait_warp(k_full(j & 1), (j >> 1) & 1, 722);
-            tc_fence_after();
-            if (leader && ok) {
-                const uint32_t q_lo = smem_desc_lo(base + S::kQ + i * S::kTile, 16), k_lo = smem_desc_lo(base + S::kK + (j & 1) * S::kTile + (h & 1) * (kHalfKeys * 128), 16);
+        if (warp == kIssuer) {
+            if (tiles > 0) ok = mbar_wait_warp(q_full, 0, 721);
+            for (int h = 0; h < halves && ok; ++h) {
+                const int j = h >> 1;
+                if (ok) ok = mbar_wait_warp(k_full(j & 1), (j >> 1) & 1, 722);
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const uint32_t at = ((k >> 2) * S::kHalf + (k & 3) * 32) >> 4;
-                    umma_bf16(tmem_u + i * 128 + (h & 1) * kHalfKeys, desc_words(q_lo + at, smem_desc_hi(1024)), desc_words(k_lo + at, smem_desc_hi(1024)), idesc_s, k != 0 ? 1u : 0u);
+                for (int i = 0; i < 2; ++i) {
+                    if (h >= n[i]) continue;
+                    if (ok && h >= 2) ok = mbar_wait_warp(pv_done(i, h), ((h >> 1) & 1) ^ 1, 731);   // S goes over P of half h - 2
+                    tc_fence_after();
+                    if (leader && ok) {
+                        const uint32_t q_lo = smem_desc_lo(base + S::kQ + i * S::kTile, 16), k_lo = smem_desc_lo(base + S::kK + (j & 1) * S::kTile + (h & 1) * (kHalfKeys * 128), 16);
+#pragma unroll
+                        for (int k = 0; k < D / 16; ++k) {
+                            const uint32_t at = ((k >> 2) * S::kHalf + (k & 3) * 32) >> 4;
+                            umma_bf16(tmem_u + i * 128 + (h & 1) * kHalfKeys, desc_words(q_lo + at, smem_desc_hi(1024)), desc_words(k_lo + at, smem_desc_hi(1024)), idesc_s, k != 0 ? 1u : 0u);
+                        }
+                        umma_commit(s_full(i, h));
+                    }
+                    __syncwarp();
                 }
-                umma_commit(s_full(i, h));
-            }
-            __syncwarp();
-        };
-        // K of a tile is free behind its last scores, of the second half, or of the first where that is the last there is.
-        auto release_k = [&](int h) {
-            if (leader && ok && h < halves && ((h & 1) != 0 || h + 1 == halves)) umma_commit(k_empty((h >> 1) & 1));
-            __syncwarp();
-        };
-        for (int h = 0; h < 2; ++h) {
-            for (int i = 0; i < 2; ++i)
-                if (h < n[i]) scores(i, h);
-            release_k(h);
-        }
-        for (int h = 0; h < halves && ok; ++h) {
-            const int j = h >> 1;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if (h >= n[i]) continue;
-                if (ok) ok = mbar_wait_warp(p_full(i, h), (h >> 1) & 1, 723);
-                if (ok) ok = mbar_wait_warp(v_full(j & 1), (j >> 1) & 1, 724);
-                tc_fence_after();
-                if (leader && ok) {
-                    const uint32_t v_lo = smem_desc_lo(base + S::kV + (j & 1) * S::kTile + (h & 1) * (kHalfKeys * 128), S::kHalf);
-#pragma unroll
-                    for (int k = 0; k < kHalfKeys / 16; ++k)
-                        umma_a_tmem(tmem_u + 256 + i * 128, tmem_u + i * 128 + (h & 1) * kHalfKeys + k * 8, desc_words(v_lo + ((k * 2048) >> 4), smem_desc_hi(1024)), idesc_o, (h | k) != 0 ? 1u : 0u);
-                    umma_commit(pv_done(i));
-                    if (h + 1 == n[i]) umma_commit(o_full(i));
-                }
+                // K of a tile is free behind its last scores, of the second half, or of the first where that is the last there is.
+                if (leader && ok && ((h & 1) != 0 || h + 1 == halves)) umma_commit(k_empty(j & 1));
                 __syncwarp();
-                if (h + 2 < n[i]) scores(i, h + 2);
             }
-            if (leader && ok && ((h & 1) != 0 || h + 1 == halves)) umma_commit(v_empty(j & 1));
-            release_k(h + 2);
+        } else {
+            for (int h = 0; h < halves && ok; ++h) {
+                const int j = h >> 1;
+                if (ok) ok = mbar_wait_warp(v_full(j & 1), (j >> 1) & 1, 724);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    if (h >= n[i]) continue;
+                    if (ok) ok = mbar_wait_warp(p_full(i, h), (h >> 1) & 1, 723);
+                    tc_fence_after();
+                    if (leader && ok) {
+                        const uint32_t v_lo = smem_desc_lo(base + S::kV + (j & 1) * S::kTile + (h & 1) * (kHalfKeys * 128), S::kHalf);
+#pragma unroll
+                        for (int k = 0; k < kHalfKeys / 16; ++k)
+                            umma_a_tmem(tmem_u + 256 + i * 128, tmem_u + i * 128 + (h & 1) * kHalfKeys + k * 8, desc_words(v_lo + ((k * 2048) >> 4), smem_desc_hi(1024)), idesc_o, (h | k) != 0 ? 1u : 0u);
+                        umma_commit(pv_done(i, h));
+                        if (h + 1 == n[i]) umma_commit(o_full(i));
+                    }
+                    __syncwarp();
+                }
+                if (leader && ok && ((h & 1) != 0 || h + 1 == halves)) umma_commit(v_empty(j & 1));
+                __syncwarp();
+            }
         }
     } else if (warp >= 8) {
         // ---- codes to f16
@@ -429,8 +428,8 @@ cache_sdpa_umma_kernel(const __grid_constant__ CachePrefillArgs args) {
                 const float next = raise ? top : r, down = raise ? exp2_of(r - next) : 1.0f;
                 r = next;
                 sum *= down;
-                if (h > 0) {   // (S of this half came behind the products of all halves but the last)
-                    if (ok) ok = mbar_wait_warp(pv_done(i), (h - 1) & 1, 730);
+                if (h > 0) {   // (S of this half came behind the products with V of all halves but the last)
+                    if (ok) ok = mbar_wait_warp(pv_done(i, h - 1), ((h - 1) >> 1) & 1, 730);
                     tc_fence_after();
 #pragma unroll 1
                     for (int c = 0; c < D; c += 16) {
