@@ -10,6 +10,7 @@
 #include "common.cuh"
 #include "dfgpu_cache.h"
 #include "scale_rule.cuh"
+#include "umma_ptx.cuh"
 
 namespace dfgpu {
 namespace {
@@ -35,6 +36,7 @@ struct AppendArgs {
     int32_t page, tokens, row;      // tokens a page and a scale block; vectors a row
     int32_t capacity;               // K's, what lengths_out is clamped to
     int64_t units;
+    int32_t rows, rest;             // of a unit's threads: whole rows of vectors, and the vectors beyond
     FastDivisor by_row, by_blocks, by_heads;
 };
 
@@ -46,13 +48,32 @@ __device__ __forceinline__ float value_of(float v) { return v; }
 __device__ __forceinline__ float value_of(__half v) { return __half2float(v); }
 __device__ __forceinline__ float value_of(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// |x| as f32 bits: ordered like whole numbers, a NaN above all.
-template <typename T, int V>
-__device__ __forceinline__ uint32_t magnitude_bits(const AppendVector<T, V>& x, uint32_t largest) {
+// The largest |x|, of 16-bit values two at a time: without their signs they are ordered like whole numbers, a NaN above all.
+template <typename T>
+struct Largest {
+    uint32_t bits = 0;
+    template <int V>
+    __device__ __forceinline__ void take(const AppendVector<T, V>& x) {
+        if constexpr (sizeof(T) == 2 && V > 1) {
+            const uint32_t* pairs = reinterpret_cast<const uint32_t*>(&x);
 #pragma unroll
-    for (int i = 0; i < V; ++i) largest = max(largest, __float_as_uint(value_of(x.v[i])) & 0x7fffffffu);
-    return largest;
-}
+            for (int i = 0; i < V / 2; ++i) bits = __vmaxu2(bits, pairs[i] & 0x7fff7fffu);
+        } else if constexpr (sizeof(T) == 2) {
+            bits = max(bits, *reinterpret_cast<const uint16_t*>(&x) & 0x7fffu);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) bits = max(bits, __float_as_uint(x.v[i]) & 0x7fffffffu);
+        }
+    }
+    __device__ __forceinline__ uint32_t as_f32() const {
+        if constexpr (sizeof(T) == 2) {
+            const uint16_t top = static_cast<uint16_t>(max(bits & 0xffffu, bits >> 16));
+            return __float_as_uint(value_of(*reinterpret_cast<const T*>(&top))) & 0x7fffffffu;
+        } else {
+            return bits;
+        }
+    }
+};
 
 template <int V>
 struct alignas(V) AppendCodes {
@@ -64,15 +85,43 @@ __device__ __forceinline__ AppendCodes<V> encode(const AppendVector<T, V>& x, fl
     if constexpr (V == 1) {
         codes.v[0] = static_cast<uint8_t>(encode_e4m3_scalar(value_of(x.v[0]) * inverse));
     } else {
+        uint32_t* words = reinterpret_cast<uint32_t*>(&codes);
+        bool zeros = false;   // a code of -0: of a value that is one, or of one that rounds to it, whose code is +0
 #pragma unroll
-        for (int i = 0; i < V; i += 2) {
-            const uint32_t pair = encode_e4m3_pair(value_of(x.v[i]) * inverse, value_of(x.v[i + 1]) * inverse);
-            codes.v[i] = static_cast<uint8_t>(pair);
-            codes.v[i + 1] = static_cast<uint8_t>(pair >> 8);
+        for (int i = 0; i < V; i += 4) {
+            float v[4];
+            const uint64_t by = pack2(inverse, inverse);
+            unpack2(mul2(pack2(value_of(x.v[i]), value_of(x.v[i + 1])), by), v[0], v[1]);
+            unpack2(mul2(pack2(value_of(x.v[i + 2]), value_of(x.v[i + 3])), by), v[2], v[3]);
+            const uint32_t word = cvt_e4m3_pair(v[0], v[1]) | cvt_e4m3_pair(v[2], v[3]) << 16, turned = word ^ 0x80808080u;
+            zeros = zeros || ((turned - 0x01010101u) & ~turned & 0x80808080u) != 0;
+            words[i / 4] = word;
+        }
+        if (zeros) {   // (one value in 10^5 of normal ones)
+#pragma unroll
+            for (int i = 0; i < V; i += 4)
+                words[i / 4] = encode_e4m3_pair(value_of(x.v[i]) * inverse, value_of(x.v[i + 1]) * inverse) | encode_e4m3_pair(value_of(x.v[i + 2]) * inverse, value_of(x.v[i + 3]) * inverse) << 16;
         }
     }
     return codes;
 }
+
+// The places of a thread's vectors in rows of `row` vectors, NT vectors apart.
+struct AppendWalk {
+    int column;
+    int64_t at;
+    __device__ __forceinline__ AppendWalk(int thread, int64_t stride, int width, const FastDivisor& by_row, int row) {
+        const int first = static_cast<int>(fast_divide(static_cast<uint32_t>(thread), by_row));
+        column = thread - first * row;
+        at = first * stride + column * width;
+    }
+    // rows: NT / row of them and rest = NT % row vectors on
+    __device__ __forceinline__ void next(int64_t step, int64_t wrap, int rest, int row) {
+        column += rest;
+        at += step;
+        if (column >= row) column -= row, at += wrap;
+    }
+};
 
 // NT threads a unit.
 template <typename T, int V, int NT>
@@ -104,25 +153,30 @@ cache_append_kernel(AppendArgs a) {
     const int in_page = begin - slot * a.page;
     const T* x = static_cast<const T*>(s.x) + batch * s.x_stride[0] + head * s.x_stride[1] + (first - length) * s.x_stride[2];
     const int count = (end - first) * a.row;   // vectors
-    auto load = [&](int i) {
-        const int row = static_cast<int>(fast_divide(static_cast<uint32_t>(i), a.by_row));
-        return *reinterpret_cast<const AppendVector<T, V>*>(x + row * s.x_stride[2] + (i - row * a.row) * V);
-    };
+    AppendWalk from(thread, s.x_stride[2], V, a.by_row, a.row);
+    const int64_t from_step = a.rows * s.x_stride[2] + a.rest * V, from_wrap = s.x_stride[2] - a.row * V;
+    auto load = [&](const AppendWalk& walk) { return *reinterpret_cast<const AppendVector<T, V>*>(x + walk.at); };
     AppendVector<T, V> held[kHeld];
-    uint32_t largest = 0;
 #pragma unroll
-    for (int k = 0; k < kHeld; ++k)
-        if (thread + k * NT < count) held[k] = load(thread + k * NT);
+    for (int k = 0; k < kHeld; ++k) {
+        if (thread + k * NT < count) held[k] = load(from);
+        from.next(from_step, from_wrap, a.rest, a.row);
+    }
     if (page < 0 || page >= s.pages) return;
     uint8_t* codes = s.codes + page * s.code_stride[0] + head * s.code_stride[1] + (in_page + (first - begin)) * s.code_stride[2];
     uint8_t* scale = s.scales + page * s.scale_stride[0] + head * s.scale_stride[1] + (in_page / a.tokens) * s.scale_stride[2];
     const bool holds = first > begin;
     const uint32_t old = holds ? *scale : 0u;
+    Largest<T> own;
 #pragma unroll
     for (int k = 0; k < kHeld; ++k)
-        if (thread + k * NT < count) largest = magnitude_bits(held[k], largest);
-    for (int i = thread + kHeld * NT; i < count; i += NT) largest = magnitude_bits(load(i), largest);
-    largest = __reduce_max_sync(0xffffffffu, largest);
+        if (thread + k * NT < count) own.take(held[k]);
+    AppendWalk beyond = from;
+    for (int i = thread + kHeld * NT; i < count; i += NT) {
+        own.take(load(beyond));
+        beyond.next(from_step, from_wrap, a.rest, a.row);
+    }
+    uint32_t largest = __reduce_max_sync(0xffffffffu, own.as_f32());
     if constexpr (NT > 32) {
         if ((threadIdx.x & 31) == 0) largest_of[threadIdx.x >> 5] = largest;
         __syncthreads();
@@ -133,14 +187,17 @@ cache_append_kernel(AppendArgs a) {
     // rounds to zero, at most 224 of f32's smallest steps.)
     const uint32_t code = max(largest <= 224u ? 0u : scale_code_from_amax_bits(largest), old);
     const float inverse = reciprocal_e8m0(code);
-    auto store = [&](int i, const AppendVector<T, V>& v) {
-        const int row = static_cast<int>(fast_divide(static_cast<uint32_t>(i), a.by_row));
-        *reinterpret_cast<AppendCodes<V>*>(codes + row * s.code_stride[2] + (i - row * a.row) * V) = encode(v, inverse);
-    };
+    AppendWalk to(thread, s.code_stride[2], V, a.by_row, a.row);
+    const int64_t to_step = a.rows * s.code_stride[2] + a.rest * V, to_wrap = s.code_stride[2] - a.row * V;
 #pragma unroll
-    for (int k = 0; k < kHeld; ++k)
-        if (thread + k * NT < count) store(thread + k * NT, held[k]);
-    for (int i = thread + kHeld * NT; i < count; i += NT) store(i, load(i));
+    for (int k = 0; k < kHeld; ++k) {
+        if (thread + k * NT < count) *reinterpret_cast<AppendCodes<V>*>(codes + to.at) = encode(held[k], inverse);
+        to.next(to_step, to_wrap, a.rest, a.row);
+    }
+    for (int i = thread + kHeld * NT; i < count; i += NT) {
+        *reinterpret_cast<AppendCodes<V>*>(codes + to.at) = encode(load(from), inverse);
+        from.next(from_step, from_wrap, a.rest, a.row), to.next(to_step, to_wrap, a.rest, a.row);
+    }
     if (holds && code != old) {
         // What the block holds already, in the new scale: both are powers of two (or NaN), so that the value before the rounding is exact.
         uint8_t* before = s.codes + page * s.code_stride[0] + head * s.code_stride[1] + in_page * s.code_stride[2];
@@ -303,6 +360,7 @@ extern "C" int dfgpu_cache_append(const dfgpu_cache_append_params* p, void* cons
     int threads = 32;
     if (vectors > 32 * held_by(32))
         for (threads = 128; threads < 512 && vectors > threads * held_by(threads);) threads *= 2;
+    a.rows = threads / a.row, a.rest = threads % a.row;
     cudaStream_t on = as_stream(stream);
     if (p->k.dtype == DFGPU_F32) vector ? launch_append<float, 4>(a, threads, on) : launch_append<float, 1>(a, threads, on);
     else if (p->k.dtype == DFGPU_F16) vector ? launch_append<__half, 8>(a, threads, on) : launch_append<__half, 1>(a, threads, on);
