@@ -132,7 +132,9 @@ cache_pages_kernel(PagesArgs a) {
         copy_ints(a.refs_out, a.refs, a.pages, thread);
         copy_ints(a.table_out, a.table, static_cast<int64_t>(a.batch) * a.slots, thread);
         if constexpr (kFork) {
-            for (int i = thread; i < a.batch; i += kPagesAll) a.sequence_a[i] = 0x7fffffff;   // the first entry that names a target
+            // the first entry that names a target; the lengths, which a target's new one may go over before its source's is asked for
+            for (int i = thread; i < a.batch; i += kPagesAll) a.sequence_a[i] = 0x7fffffff, a.sequence_b[i] = length_of(a, i);
+            copy_ints(a.lengths_out, a.lengths, a.batch, thread);
             cluster_sync();
             for (int i = thread; i < a.entries; i += kPagesAll) {
                 const int source = a.list[2 * i], target = a.list[2 * i + 1];
@@ -171,6 +173,7 @@ cache_pages_kernel(PagesArgs a) {
             if (a.refs[i] <= 0) a.pages_a[rank++] = i;
         int ahead = before.y;
         int2 taken = make_int2(0, 0);   // pages, refused
+        int copied = 0;
         for (int i = from; i < until; ++i) {
             bool fine;
             const int wanted = demand(i, fine);
@@ -178,6 +181,10 @@ cache_pages_kernel(PagesArgs a) {
             if constexpr (kFork) {
                 a.entry_a[i] = served ? ahead : -1;
                 taken.y += !served && a.list[2 * i] >= 0;
+                if (served && wanted) {
+                    const int source = a.list[2 * i];
+                    copied += names_page(a, a.table[static_cast<int64_t>(source) * a.slots + length_of(a, source) / a.block]);
+                }
             } else {
                 a.sequence_a[i] = ahead;
                 a.sequence_b[i] = served ? wanted : 0;
@@ -186,15 +193,16 @@ cache_pages_kernel(PagesArgs a) {
             taken.x += served ? wanted : 0;
             ahead += wanted;
         }
+        if (kFork && copied) atomicAdd(&a.header[1], copied);
         cluster_scan(shared, 1, taken, total);   // (its barrier: the lists are there, and the inputs have been copied)
         if constexpr (kFork) {
-            int copied = 0;
             for (int i = warp; i < a.entries; i += kPagesAll / 32) {
                 const int place = a.entry_a[i];
                 if (place < 0) continue;
                 const int source = a.list[2 * i], target = a.list[2 * i + 1];
-                const int length = length_of(a, source), full = length / a.block;
+                const int length = a.sequence_b[source], full = length / a.block;
                 const bool partial = length % a.block != 0;
+                if (lane == 0) a.lengths_out[target] = length;
                 for (int s = lane; s < a.slots; s += 32) {
                     int id = -1;
                     if (s < full || (s == full && partial)) {
@@ -202,7 +210,6 @@ cache_pages_kernel(PagesArgs a) {
                         if (s == full) {
                             const int fresh = a.pages_a[place];
                             a.copies[place] = make_int2(names_page(a, id) ? id : -1, fresh);
-                            copied += names_page(a, id);
                             id = fresh;
                         }
                         if (names_page(a, id)) atomicAdd(&a.refs_out[id], 1);
@@ -210,17 +217,6 @@ cache_pages_kernel(PagesArgs a) {
                     a.table_out[static_cast<int64_t>(target) * a.slots + s] = id;
                 }
             }
-            copied = __reduce_add_sync(0xffffffffu, copied);
-            if (lane == 0 && copied) atomicAdd(&a.header[1], copied);
-            // lengths after everybody has read them: a target's new length is not yet another entry's business
-            cluster_sync();
-            copy_ints(a.lengths_out, a.lengths, a.batch, thread);
-            if (a.lengths_out != a.lengths) cluster_sync();
-            for (int i = thread; i < a.entries; i += kPagesAll)
-                if (a.entry_a[i] >= 0) a.sequence_b[a.list[2 * i + 1]] = length_of(a, a.list[2 * i]);
-            cluster_sync();
-            for (int i = thread; i < a.entries; i += kPagesAll)
-                if (a.entry_a[i] >= 0) a.lengths_out[a.list[2 * i + 1]] = a.sequence_b[a.list[2 * i + 1]];
             if (thread == 0) a.header[0] = total.x;
             if (thread == 0 && a.report) {
                 a.report[0] = available - total.x;
