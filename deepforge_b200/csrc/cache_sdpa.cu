@@ -305,17 +305,20 @@ struct RowTile {
     }
 };
 
+__device__ __forceinline__ int divided(int n, const FastDivisor& by) { return static_cast<int>(fast_divide(static_cast<uint32_t>(n), by)); }
+
 // Units of keys of an entry (a sequence's block of rows), the same for each of its KV heads.
 __device__ __forceinline__ int units_of(const CacheSdpaArgs& a, int entry, int& lo, int& hi) {
-    const int sequence = entry / a.row_blocks, row_first = (entry - sequence * a.row_blocks) * a.block_rows;
-    window_of_tokens(a, sequence_window(a, sequence), row_first / a.group, (min(row_first + a.block_rows, a.rows) - 1) / a.group, lo, hi);
+    const int sequence = divided(entry, a.by_row_blocks), row_first = (entry - sequence * a.row_blocks) * a.block_rows;
+    window_of_tokens(a, sequence_window(a, sequence), divided(row_first, a.by_group), divided(min(row_first + a.block_rows, a.rows) - 1, a.by_group), lo, hi);
     return hi > lo ? (hi + kUnit - 1) / kUnit - lo / kUnit : 0;
 }
 
 // Whether the kernel has anything to do (whole warps).
 __device__ __forceinline__ bool wanted(const CacheSdpaArgs& a) {
-    if (!a.only_if) return true;
+    if (__builtin_expect(a.only_if == nullptr, 1)) return true;
     bool some = false;
+#pragma unroll 1
     for (int i = threadIdx.x & 31; i < a.only_if_count; i += 32) some = some || a.only_if[i] != 0;
     return __any_sync(0xffffffffu, some);
 }
@@ -391,7 +394,7 @@ cache_sdpa_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
             if (some) units = __shfl_sync(0xffffffffu, n, which), lo = __shfl_sync(0xffffffffu, from, which), hi = __shfl_sync(0xffffffffu, until, which);
         }
         const int take = min(units - offset, left), unit0 = lo / kUnit + offset;
-        const int64_t batch = entry / a.row_blocks;
+        const int64_t batch = divided(entry, a.by_row_blocks);
         const int row_first = (entry - static_cast<int>(batch) * a.row_blocks) * a.block_rows;
         const bool whole = offset == 0 && take == units;
         if (lane == 0 && offset == 0) a.starts[1 + static_cast<int64_t>(entry) * a.heads_kv + head] = whole ? -1 : min((part + 1) * per, all) - left;
@@ -616,10 +619,10 @@ cache_sdpa_merge_kernel(const __grid_constant__ CacheSdpaArgs a) {
     __shared__ float2 meeting[kWarpsHere];
     __shared__ __align__(16) float values[kWarpsHere][D];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int in_rows = static_cast<int>(blockIdx.x % a.rows), token = in_rows / a.group;
-    const int64_t list = blockIdx.x / a.rows, batch = list / a.heads_kv;
-    const int head_kv = static_cast<int>(list - batch * a.heads_kv), head = head_kv * a.group + (in_rows - token * a.group);
-    const int block = in_rows / a.block_rows, row = in_rows - block * a.block_rows, entry = static_cast<int>(batch) * a.row_blocks + block;
+    const int list = divided(static_cast<int>(blockIdx.x), a.by_rows), in_rows = static_cast<int>(blockIdx.x) - list * a.rows, token = divided(in_rows, a.by_group);
+    const int64_t batch = divided(list, a.by_heads);
+    const int head_kv = list - static_cast<int>(batch) * a.heads_kv, head = head_kv * a.group + (in_rows - token * a.group);
+    const int block = in_rows >> (a.block_rows == 8 ? 3 : 4), row = in_rows - block * a.block_rows, entry = static_cast<int>(batch) * a.row_blocks + block;
     chain_begin();
     if (!wanted(a)) return;
     const int per = a.starts[0], start = a.starts[1 + static_cast<int64_t>(entry) * a.heads_kv + head_kv];   // (written where the list has keys)
@@ -883,6 +886,9 @@ extern "C" int dfgpu_cache_sdpa(const dfgpu_cache_sdpa_params* p, void* const* t
     a.row_blocks = plan.row_blocks;
     a.block_rows = plan.block_rows;
     a.entries = static_cast<int>(p->q.dim[0] * plan.row_blocks);
+    a.by_rows = make_fast_divisor(static_cast<uint32_t>(a.rows));
+    a.by_heads = make_fast_divisor(static_cast<uint32_t>(a.heads_kv));
+    a.by_row_blocks = make_fast_divisor(static_cast<uint32_t>(a.row_blocks));
     const int64_t flags = flag_bytes(*p, kernel);
     a.starts = reinterpret_cast<int32_t*>(static_cast<uint8_t*>(scratch) + flags);
     a.partial = reinterpret_cast<float*>(a.starts + plan.starts);

@@ -30,6 +30,7 @@ struct CacheSdpaArgs {
     int32_t heads_kv, group, rows, seq_q, s_kv;   // rows: (token, head of the group) pairs of a KV head
     int32_t page, box;                            // tokens a page, and of one TMA copy
     FastDivisor by_page, by_tokens, by_group;     // the first two of numbers of 16 tokens
+    FastDivisor by_rows, by_heads, by_row_blocks;
     int32_t has_left, has_right, bottom_right;
     int32_t row_blocks, block_rows, entries;      // entries: (sequence, block of rows)
     float scale_log2;
