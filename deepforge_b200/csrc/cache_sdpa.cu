@@ -710,9 +710,12 @@ StreamPlan plan_stream(const dfgpu_cache_sdpa_params& p) {
     return plan;
 }
 
-// The tcgen05 form has blocks of 256 rows, an SM each; the streaming form cuts any shape evenly but runs at a seventh of its rate.
-bool umma_pays(const dfgpu_cache_sdpa_params& p, const StreamPlan& plan) { return plan.rows >= 128 && 7 * cache_sdpa_umma_items(p) >= kSms; }
-int64_t flag_bytes(const dfgpu_cache_sdpa_params& p, int kernel) { return kernel == DFGPU_CACHE_SDPA_UMMA ? (cache_sdpa_umma_items(p) + 3) / 4 * 16 : 0; }
+// The tcgen05 form has blocks of 256 rows, an SM for each piece of their keys; the streaming form cuts any shape evenly but runs at a fourth to a seventh of
+// its rate. Streaming and tcgen05: 1000 tokens, 8 KV heads, 2000 keys, 128 pieces: 270 and 104 us; 40 tokens, 8 heads, 2000 keys, 32 pieces: 49 and 41;
+// 64 tokens, 2 heads, 4000 keys, 6 pieces: 38 and 49; 32 tokens, one head, 1100 keys, one piece: 28 and 37.
+bool umma_pays(const dfgpu_cache_sdpa_params& p, const StreamPlan& plan) { return plan.rows >= 128 && 7 * cache_sdpa_umma_items(p) * cache_sdpa_umma_pieces(p) >= kSms; }
+int64_t flag_count(const dfgpu_cache_sdpa_params& p) { return cache_sdpa_umma_items(p) * cache_sdpa_umma_pieces(p); }
+int64_t flag_bytes(const dfgpu_cache_sdpa_params& p, int kernel) { return kernel == DFGPU_CACHE_SDPA_UMMA ? (flag_count(p) + 3) / 4 * 16 : 0; }
 
 bool on_16(const void* pointer) { return (reinterpret_cast<uintptr_t>(pointer) & 15u) == 0; }
 
@@ -811,8 +814,9 @@ extern "C" int dfgpu_query_cache_sdpa(const dfgpu_cache_sdpa_params* p, dfgpu_pl
     if (status) return status;
     const StreamPlan plan = plan_stream(*p);
     info->kernel = kernel;
-    info->launches = kernel == DFGPU_CACHE_SDPA_UMMA ? 3 : 2;
-    info->scratch_bytes = plan.scratch + flag_bytes(*p, kernel);
+    info->launches = kernel != DFGPU_CACHE_SDPA_UMMA ? 2 : cache_sdpa_umma_pieces(*p) == 1 ? 3 : 4;
+    // (the two forms' partial results take turns)
+    info->scratch_bytes = flag_bytes(*p, kernel) + std::max(plan.scratch, kernel == DFGPU_CACHE_SDPA_UMMA ? cache_sdpa_umma_partial_bytes(*p) : 0);
     return kOk;
 }
 
@@ -900,10 +904,10 @@ extern "C" int dfgpu_cache_sdpa(const dfgpu_cache_sdpa_params* p, void* const* t
     const dim3 grid(static_cast<unsigned>(plan.grid));
     cudaStream_t on = as_stream(stream);
     if (kernel == DFGPU_CACHE_SDPA_UMMA) {
-        const int launched = launch_cache_sdpa_umma(*p, a, static_cast<int32_t*>(scratch), on);
+        const int launched = launch_cache_sdpa_umma(*p, a, static_cast<int32_t*>(scratch), reinterpret_cast<float*>(static_cast<uint8_t*>(scratch) + flags), on);
         if (launched) return launched;
         a.only_if = static_cast<const int32_t*>(scratch);
-        a.only_if_count = static_cast<int>(cache_sdpa_umma_items(*p));
+        a.only_if_count = static_cast<int>(flag_count(*p));
     }
     const bool half = p->q.dtype == DFGPU_F16;
     switch (p->q.dim[3]) {

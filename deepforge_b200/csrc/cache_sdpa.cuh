@@ -38,10 +38,12 @@ struct CacheSdpaArgs {
     int32_t only_if_count;
 };
 
-// The tcgen05 form (cache_sdpa_umma.cu). What it leaves to the streaming form it says in `flags`, one integer an item.
+// The tcgen05 form (cache_sdpa_umma.cu). What it leaves to the streaming form it says in `flags`, one integer a piece of an item.
 bool cache_sdpa_umma_supported(const dfgpu_cache_sdpa_params& p);
 int64_t cache_sdpa_umma_items(const dfgpu_cache_sdpa_params& p);
-int launch_cache_sdpa_umma(const dfgpu_cache_sdpa_params& p, const CacheSdpaArgs& a, int32_t* flags, cudaStream_t stream);
+int cache_sdpa_umma_pieces(const dfgpu_cache_sdpa_params& p);   // of an item
+int64_t cache_sdpa_umma_partial_bytes(const dfgpu_cache_sdpa_params& p);
+int launch_cache_sdpa_umma(const dfgpu_cache_sdpa_params& p, const CacheSdpaArgs& a, int32_t* flags, float* partial, cudaStream_t stream);
 
 struct SequenceWindow {
     int64_t shift;    // key minus query position on the diagonal

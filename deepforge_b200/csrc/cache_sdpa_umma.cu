@@ -19,6 +19,7 @@
 // scale of 2^126 or more, a scale that is a NaN, V scales more than 2^16
 // apart or below 2^-80 over codes that are not zero, scores beyond 2^10.
 #include <algorithm>
+#include <type_traits>
 
 #include "cache_sdpa.cuh"
 #include "dfgpu_cache.h"
@@ -36,15 +37,18 @@ constexpr int kLeastCode = 47;       // V scales below 2^-80 count as that (over
 constexpr int kMostApart = 16;
 constexpr float kLeastFactor = 1.17549435e-38f;   // (of a score: not zero, so that -inf stays -inf)
 constexpr float kMostReference = 1024.0f;   // |r|: the exponent's one rounding, of score * factor + (scale - r), is below 2^-14 up to there
+constexpr int kSms = 148, kLeastTiles = 4;   // of key tiles that a piece has
 constexpr int kMostRanked = 128;     // sequences that are put in order of length
 constexpr float kLn2 = 0.6931471805599453f;
 
 struct CachePrefillArgs {
     CacheSdpaArgs a;
-    int32_t* flags;       // by item
+    int32_t* flags;       // by CTA
+    float* partial;       // [item in the order of O][piece][row]{O, not divided by its sum; its reference, its sum}, where there are pieces
     int32_t tokens;       // of a query tile: 128 / group
     int32_t blocks;       // of two query tiles
     int32_t batches;
+    int32_t pieces;       // of an item's keys
 };
 
 template <int D>
@@ -110,7 +114,8 @@ __device__ __forceinline__ float power_of_two(int n) { return __uint_as_float(st
 __device__ __forceinline__ float value_of(__half v) { return __half2float(v); }
 __device__ __forceinline__ float value_of(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-template <typename T, int D>
+// PIECES: an item's keys are cut (3 % slower where they are not).
+template <typename T, int D, bool PIECES>
 __global__ void __launch_bounds__(kThreads, 1)
 cache_sdpa_umma_kernel(const __grid_constant__ CachePrefillArgs args) {
     using S = Smem<D>;
@@ -151,9 +156,10 @@ cache_sdpa_umma_kernel(const __grid_constant__ CachePrefillArgs args) {
     }
     chain_wait();
 
-    // The item: sequences by falling length (those beyond the first 128 as they are stored), their last query blocks first, a block's heads side by side.
+    // The piece of an item: sequences by falling length (those beyond the first 128 as they are stored), their last query blocks first, a block's heads side by side.
     const int per_batch = a.heads_kv * args.blocks;
-    int nth = static_cast<int>(blockIdx.x) / per_batch;
+    const int item = PIECES ? static_cast<int>(blockIdx.x) / args.pieces : static_cast<int>(blockIdx.x), piece = PIECES ? static_cast<int>(blockIdx.x) - item * args.pieces : 0;
+    int nth = item / per_batch;
     if (args.batches <= kMostRanked) {
         if (static_cast<int>(threadIdx.x) < args.batches) {
             const int own = a.seq_kv_data[threadIdx.x * a.seq_kv_stride];
@@ -172,7 +178,7 @@ cache_sdpa_umma_kernel(const __grid_constant__ CachePrefillArgs args) {
     chain_release();
     const uint32_t tmem = static_cast<uint32_t>(misc[0]);
     const int64_t batch = misc[2];
-    const int in_batch = static_cast<int>(blockIdx.x) % per_batch, head = in_batch % a.heads_kv, block = args.blocks - 1 - in_batch / a.heads_kv;
+    const int in_batch = item % per_batch, head = in_batch % a.heads_kv, block = args.blocks - 1 - in_batch / a.heads_kv;
     const SequenceWindow window = sequence_window(a, batch);
     const int token0 = block * 2 * args.tokens;
     // Keys that the query tiles see; the first key tile is common.
@@ -180,10 +186,16 @@ cache_sdpa_umma_kernel(const __grid_constant__ CachePrefillArgs args) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) window_of_tokens(a, window, token0 + i * args.tokens, min(token0 + (i + 1) * args.tokens, a.seq_q) - 1, lo[i], hi[i]);
     const bool some[2] = {hi[0] > lo[0], hi[1] > lo[1]};
-    const int all_lo = some[0] && some[1] ? min(lo[0], lo[1]) : some[0] ? lo[0] : lo[1], all_hi = max(hi[0], hi[1]);
-    const int first = all_lo / kKeys;
+    const int all_lo = some[0] && some[1] ? min(lo[0], lo[1]) : some[0] ? lo[0] : lo[1];
+    int all_hi = max(hi[0], hi[1]), first = all_lo / kKeys;
+    if constexpr (PIECES) {
+        const int each = ((all_hi + kKeys - 1) / kKeys - first + args.pieces - 1) / args.pieces;   // key tiles of a piece
+        first += piece * each;
+        all_hi = min(all_hi, (first + each) * kKeys);
+    }
     // halves of key tiles that a query tile walks
-    const int n[2] = {some[0] ? (hi[0] - first * kKeys + kHalfKeys - 1) / kHalfKeys : 0, some[1] ? (hi[1] - first * kKeys + kHalfKeys - 1) / kHalfKeys : 0};
+    auto halves_to = [&](bool any, int until) { return any ? max(min(until, all_hi) - first * kKeys + kHalfKeys - 1, 0) / kHalfKeys : 0; };
+    const int n[2] = {halves_to(some[0], hi[0]), halves_to(some[1], hi[1])};
     const int halves = max(n[0], n[1]), tiles = (halves + 1) / 2;
     bool ok = true;
 
@@ -477,6 +489,26 @@ cache_sdpa_umma_kernel(const __grid_constant__ CachePrefillArgs args) {
         // O, normalised
         if (ok && n[i] > 0) ok = mbar_wait_warp(o_full(i), 0, 729);
         tc_fence_after();
+        if constexpr (PIECES) {
+            float* to = args.partial + ((static_cast<int64_t>((batch * a.heads_kv + head) * args.blocks + block) * args.pieces + piece) * (2 * kRows) + i * kRows + row) * (D + 4);
+            if (ok) {
+#pragma unroll 1
+                for (int c = 0; c < D; c += 16) {
+                    uint32_t acc[16];
+                    __syncwarp();
+                    if (n[i] > 0) tmem_load_16_now(o_tmem + c, acc);
+                    if (!there) continue;
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) {
+                        uint4 v = make_uint4(acc[e], acc[e + 1], acc[e + 2], acc[e + 3]);
+                        if (n[i] == 0) v = make_uint4(0, 0, 0, 0);
+                        *reinterpret_cast<uint4*>(to + c + e) = v;
+                    }
+                }
+                if (there) *reinterpret_cast<float4*>(to + D) = make_float4(r, sum, 0.0f, 0.0f);
+            }
+            ok = false;   // (nothing more to do)
+        }
         const bool healthy = ok && g_device_status == 0, none = !(sum != 0.0f);   // (a NaN sum is a NaN result)
         const float inverse = 1.0f / sum;
         const int64_t at = batch * a.o_stride[0] + head_q * a.o_stride[1] + token * a.o_stride[2];
@@ -515,6 +547,39 @@ cache_sdpa_umma_kernel(const __grid_constant__ CachePrefillArgs args) {
     }
 }
 
+// A warp a row of O: its pieces.
+template <int D>
+__global__ void __launch_bounds__(128)
+cache_sdpa_pieces_kernel(const __grid_constant__ CachePrefillArgs args) {
+    constexpr int kOwn = D / 32;
+    const CacheSdpaArgs& a = args.a;
+    const int lane = threadIdx.x & 31;
+    const int64_t nth = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5), item = nth / (2 * kRows);
+    const int row = static_cast<int>(nth % (2 * kRows)), tile = row / kRows, in_group = row % kRows / args.tokens;
+    const int block = static_cast<int>(item % args.blocks), token = (block * 2 + tile) * args.tokens + (row % kRows - in_group * args.tokens);
+    const int64_t list = item / args.blocks, batch = list / a.heads_kv;
+    const int head = static_cast<int>(list % a.heads_kv) * a.group + in_group;
+    chain_begin();
+    if (in_group >= a.group || token >= a.seq_q || g_device_status != 0) return;
+    const float* from = args.partial + (item * args.pieces * (2 * kRows) + row) * (D + 4);
+    constexpr int64_t kNext = 2 * kRows * (D + 4);
+    float top = -INFINITY, total = 0.0f, value[kOwn] = {};
+    for (int i = 0; i < args.pieces; ++i) top = fmaxf(top, from[i * kNext + D]);
+#pragma unroll 4
+    for (int i = 0; i < args.pieces; ++i) {
+        const float2 of = *reinterpret_cast<const float2*>(from + i * kNext + D);
+        const float weight = of.x == -INFINITY ? 1.0f : exp2_of(of.x - top);   // (no score above -inf: zeros, or NaNs that are to be seen)
+        total = fmaf(of.y, weight, total);
+#pragma unroll
+        for (int e = 0; e < kOwn; ++e) value[e] = fmaf(from[i * kNext + lane * kOwn + e], weight, value[e]);
+    }
+    const bool none = total == 0.0f;
+    const int64_t at = batch * a.o_stride[0] + head * a.o_stride[1] + token * a.o_stride[2] + lane * kOwn;
+#pragma unroll
+    for (int e = 0; e < kOwn; ++e) store_from_f32(a.o, a.o_type, at + e, none ? 0.0f : value[e] / total);
+    if (lane == 0 && a.stats) a.stats[batch * a.stats_stride[0] + head * a.stats_stride[1] + token * a.stats_stride[2]] = none ? -INFINITY : kLn2 * (top - kUp) + logf(total);
+}
+
 }  // namespace
 
 bool cache_sdpa_umma_supported(const dfgpu_cache_sdpa_params& p) {
@@ -525,23 +590,53 @@ int64_t cache_sdpa_umma_items(const dfgpu_cache_sdpa_params& p) {
     return p.q.dim[0] * p.k.dim[1] * ((p.q.dim[2] + 2 * tokens - 1) / (2 * tokens));
 }
 
-int launch_cache_sdpa_umma(const dfgpu_cache_sdpa_params& p, const CacheSdpaArgs& a, int32_t* flags, cudaStream_t stream) {
+// Items that do not fill the SMs evenly have their keys cut into pieces. The time of a wave of CTAs is that of a piece's key tiles and about four more, for
+// its beginning and its results (pieces of fewer than four tiles gain nothing, of eight and more they are up to a third slower), if all sequences
+// are as long as they may be; it has to fall by 15 % at least, and the partial results are those of three waves at most, 60 MB.
+// 256 tokens, 8 KV heads, 16000 keys (32 items): 123 us in four pieces, 329 in one.
+int cache_sdpa_umma_pieces(const dfgpu_cache_sdpa_params& p) {
+    const int64_t tiles = (p.s_kv + kKeys - 1) / kKeys, items = cache_sdpa_umma_items(p);
+    auto cost = [&](int64_t pieces) { return (items * pieces + kSms - 1) / kSms * ((tiles + pieces - 1) / pieces + kLeastTiles); };
+    int64_t best = 1;
+    for (int64_t pieces = 2; pieces * kLeastTiles <= tiles && items * pieces <= 3 * kSms; ++pieces)
+        if (cost(pieces) * 115 < cost(1) * 100 && cost(pieces) < cost(best)) best = pieces;
+    return static_cast<int>(best);
+}
+int64_t cache_sdpa_umma_partial_bytes(const dfgpu_cache_sdpa_params& p) {
+    const int pieces = cache_sdpa_umma_pieces(p);
+    return pieces > 1 ? cache_sdpa_umma_items(p) * pieces * (2 * kRows) * (p.q.dim[3] + 4) * 4 : 0;
+}
+
+int launch_cache_sdpa_umma(const dfgpu_cache_sdpa_params& p, const CacheSdpaArgs& a, int32_t* flags, float* partial, cudaStream_t stream) {
     CachePrefillArgs args{};
     args.a = a;
     args.flags = flags;
+    args.partial = partial;
     args.tokens = kRows / a.group;
     args.blocks = (a.seq_q + 2 * args.tokens - 1) / (2 * args.tokens);
     args.batches = static_cast<int>(p.q.dim[0]);
-    const dim3 grid(static_cast<unsigned>(cache_sdpa_umma_items(p)));
+    args.pieces = cache_sdpa_umma_pieces(p);
+    const int64_t items = cache_sdpa_umma_items(p);
     auto run = [&](auto kernel, int bytes) -> int {
         const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
         if (error != cudaSuccess) return fail(kExecutionFailed, "CACHE_SDPA: cannot reserve %d bytes of shared memory: %s", bytes, cudaGetErrorString(error));
-        launch_chained(kernel, grid, dim3(kThreads), bytes, stream, args);
+        launch_chained(kernel, dim3(static_cast<unsigned>(items * args.pieces)), dim3(kThreads), bytes, stream, args);
         return check_launch("CACHE_SDPA (tcgen05)");
     };
+    auto run_type = [&](auto type, auto merge, auto d) -> int {
+        using T = decltype(type);
+        constexpr int D = decltype(d)::value;
+        if (args.pieces == 1) return run(cache_sdpa_umma_kernel<T, D, false>, Smem<D>::kDynamic);
+        const int status = run(cache_sdpa_umma_kernel<T, D, true>, Smem<D>::kDynamic);
+        if (status) return status;
+        launch_chained(merge, dim3(static_cast<unsigned>(items * (2 * kRows / 4))), dim3(128), 0, stream, args);
+        return check_launch("CACHE_SDPA pieces");
+    };
     const bool half = p.q.dtype == DFGPU_F16;
-    if (p.q.dim[3] == 64) return half ? run(cache_sdpa_umma_kernel<__half, 64>, Smem<64>::kDynamic) : run(cache_sdpa_umma_kernel<__nv_bfloat16, 64>, Smem<64>::kDynamic);
-    return half ? run(cache_sdpa_umma_kernel<__half, 128>, Smem<128>::kDynamic) : run(cache_sdpa_umma_kernel<__nv_bfloat16, 128>, Smem<128>::kDynamic);
+    const std::integral_constant<int, 64> narrow;
+    const std::integral_constant<int, 128> wide;
+    if (p.q.dim[3] == 64) return half ? run_type(__half(), cache_sdpa_pieces_kernel<64>, narrow) : run_type(__nv_bfloat16(), cache_sdpa_pieces_kernel<64>, narrow);
+    return half ? run_type(__half(), cache_sdpa_pieces_kernel<128>, wide) : run_type(__nv_bfloat16(), cache_sdpa_pieces_kernel<128>, wide);
 }
 
 int cache_sdpa_umma_device_status(int* status) { return read_and_clear_device_status(status); }

@@ -747,3 +747,26 @@ def test_results_do_not_depend_on_timing():
     for _ in range(5):
         again = run_attend(q, caches, scales, (table, table), lengths)[:2]
         assert all(torch.equal(x, y) for x, y in zip(first, again))
+
+
+@pytest.mark.parametrize("dtype,d,hk,g,sq,page,t,lengths,left", [
+    (BF16, 128, 1, 4, 64, 64, 64, [5000], None),                  # many pieces
+    (F16, 64, 2, 2, 90, 48, 16, [2200, 130, 0, 91], None),        # short sequences: pieces without keys
+    (BF16, 128, 1, 3, 130, 256, 128, [4097, 1025], 700),          # a window inside some of the pieces
+    (F16, 128, 1, 128, 2, 64, 16, [3000], None),
+])
+def test_tcgen05_form_in_pieces(dtype, d, hk, g, sq, page, t, lengths, left):
+    _, _, info = attend_case(d + sq, dtype, d, hk, g, sq, page, t, lengths, right=0, left=left, bottom_right=True, kernel=UMMA)
+    assert info.kernel == UMMA and info.launches == 4
+
+
+def test_tcgen05_form_in_pieces_without_a_bound():
+    attend_case(7, BF16, 128, 1, 2, 150, 64, 64, [2500, 1200], seq_q=[150, 7], kernel=UMMA)
+
+
+def test_tcgen05_form_in_pieces_over_special_values():
+    def nan_code(q, caches, scales, tables):   # for the rows that see it alone: the streaming form has the call
+        page = int(tables[1][0, 2400 // 64])
+        caches[1].view(torch.uint8)[page, 0, 2400 % 64, 5] = 0x7f
+
+    attend_case(8, BF16, 128, 1, 2, 150, 64, 64, [2500], right=0, bottom_right=True, kernel=UMMA, spoil=nan_code)
