@@ -724,7 +724,8 @@ int check_side(const dfgpu_cache_sdpa_params& p, const dfgpu_tensor& cache, cons
     if (cache.dim[1] != p.k.dim[1] || cache.dim[2] != p.k.dim[2]) return fail(kInvalidShape, "CACHE_SDPA: the containers differ in heads or tokens a page");
     if (cache.stride[3] != 1) return fail(kInvalidLayout, "CACHE_SDPA: the head dimension of a container must have unit stride");
     for (int i = 0; i < 3; ++i)
-        if (cache.dim[i] > 1 && (cache.stride[i] % 16 != 0 || cache.stride[i] >= (1ll << 40))) return fail(kInvalidLayout, "CACHE_SDPA: the strides of the container of %s must be multiples of 16", name);
+        if (cache.dim[i] > 1 && (cache.stride[i] <= 0 || cache.stride[i] % 16 != 0 || cache.stride[i] >= (1ll << 40)))
+            return fail(kInvalidLayout, "CACHE_SDPA: the strides of the container of %s must be positive multiples of 16", name);
     if (!valid_tensor(scale) || scale.rank != 4 || scale.dtype != DFGPU_E8M0 || scale.reorder != DFGPU_REORDER_NONE || scale.dim[0] != cache.dim[0] || scale.dim[1] != cache.dim[1] ||
         scale.dim[3] != 1 || cache.dim[2] % scale.dim[2] != 0 || scale.dim[2] != p.k_scale.dim[2])
         return fail(kInvalidShape, "CACHE_SDPA: the scales of %s must be FP8_E8M0 [pages, Hk, T / t, 1], t a divisor of T and one for K and V", name);
@@ -759,6 +760,8 @@ int check_cache_sdpa(const dfgpu_cache_sdpa_params& p, int& kernel) {
     if (p.stats.rank && (!valid_tensor(p.stats) || p.stats.rank != 4 || p.stats.dtype != DFGPU_F32 || p.stats.dim[0] != p.q.dim[0] || p.stats.dim[1] != p.q.dim[1] ||
                          p.stats.dim[2] != p.q.dim[2] || p.stats.dim[3] != 1))
         return fail(kInvalidShape, "CACHE_SDPA: Stats must be FLOAT [B, Hq, Sq, 1]");
+    for (int i = 0; i < 3 && p.stats.rank; ++i)
+        if (p.stats.dim[i] > 1 && p.stats.stride[i] == 0) return fail(kInvalidLayout, "CACHE_SDPA: Stats overlaps itself");
     if (!std::isfinite(p.attn_scale)) return fail(kInvalidValue, "CACHE_SDPA: the attention scale must be finite");
     const StreamPlan plan = plan_stream(p);
     if (p.q.dim[2] >= (1ll << 30) || p.q.dim[0] * p.k.dim[1] * plan.rows >= (1ll << 31) || plan.units >= (1ll << 30)) return fail(kUnsupported, "CACHE_SDPA: too many sequences, heads or query rows");

@@ -140,6 +140,8 @@ int check_side(const dfgpu_tensor& x, const dfgpu_tensor& y, const dfgpu_tensor&
     if (x.dtype != DFGPU_F32 && x.dtype != DFGPU_F16 && x.dtype != DFGPU_BF16) return fail(kUnsupported, "ROPE: %s must be FLOAT, HALF or BFLOAT16", name);
     if (x.dtype != y.dtype || x.dtype != reference.dtype) return fail(kUnsupported, "ROPE: all tensors that are turned have one type");
     if (x.stride[3] != 1 || y.stride[3] != 1) return fail(kInvalidLayout, "ROPE: the head dimension must have unit stride");
+    for (int i = 0; i < 3; ++i)
+        if (y.dim[i] > 1 && y.stride[i] == 0) return fail(kInvalidLayout, "ROPE: the output of %s overlaps itself", name);
     return kOk;
 }
 
@@ -207,6 +209,7 @@ extern "C" int dfgpu_rope(const dfgpu_rope_params* p, void* const* tensors, void
     const bool two = p->x2.rank != 0;
     for (int i = 0; i < (two ? 6 : 4); ++i)
         if (!tensors[i]) return fail(kInvalidArgument, "ROPE: port %d is null", i);
+    if (two && (tensors[1] == tensors[5] || tensors[0] == tensors[5] || tensors[1] == tensors[4])) return fail(kInvalidArgument, "ROPE: the output of one pair is a tensor of the other");
     const int bytes = dtype_bytes(p->x.dtype);
     RopeArgs a{};
     for (int s = 0; s < (two ? 2 : 1); ++s) {

@@ -32,7 +32,7 @@ int dfgpu_cache_abi_version(void);
    64 bits, so far positions keep f32 accuracy; products and sums are f32, rounded once to Y's type.
    tensors: {X, Y, positions, frequencies, X2 or null, Y2 or null}. X, Y [B, H, S, D] FLOAT, HALF or BFLOAT16, the same type
    (any strides; D contiguous); X2, Y2 [B, H2, S, D], a second pair of tensors turned in the same launch (keys beside queries),
-   rank 0: absent. Y may be X itself (same pointer, same strides) and must not overlap it otherwise. positions INT32 or INT64
+   rank 0: absent. Y may be X itself (same pointer, same strides) and must not overlap it, X2 or Y2 otherwise. positions INT32 or INT64
    [B or 1, 1, S, 1]; frequencies FLOAT [1, 1, 1, R/2], R = 2 * that extent <= D. The largest D is 1024. */
 enum { DFGPU_ROPE_AUTO = 0, DFGPU_ROPE_VECTOR = 1, DFGPU_ROPE_SCALAR = 2 };
 typedef struct dfgpu_rope_params {
@@ -93,10 +93,11 @@ int dfgpu_cache_append(const dfgpu_cache_append_params*, void* const* tensors, v
    kv > q + shift - left_bound (with has_left_bound). Query rows from SEQ_LEN_Q on, and rows without keys, give O = 0 and
    Stats = -inf. A key whose page id is out of range reads as zeros, as in SDPA. Products take the codes as they are
    (exact in f16), scales and everything else are f32; the probabilities that weight V are rounded to f16, and Q is not
-   rounded. A code or scale of a masked key, NaN or not, has no effect.
+   rounded. A code or scale of a masked key, NaN or not, has no effect. Values under a V scale more than 2^80 below
+   that of an earlier key of the sequence count as zeros.
    tensors: {Q, K container, V container, O, Stats or null, K scale, V scale, SEQ_LEN_Q or null, SEQ_LEN_KV, Page_table_K,
    Page_table_V}. Q, O [B, Hq, Sq, D] HALF or BFLOAT16, the same type (O may be FLOAT); D contiguous, 64, 128 or 256; Hq a
-   multiple of Hk. Containers with D contiguous, their other strides multiples of 16 and 16-byte aligned; T and t multiples of 16. Stats FLOAT
+   multiple of Hk. Containers with D contiguous, their other strides positive multiples of 16 and 16-byte aligned; T and t multiples of 16. Stats FLOAT
    [B, Hq, Sq, 1]: max + ln(sum). SEQ_LEN_Q absent: all Sq rows. s_kv bounds the keys of every sequence (at most P * T). */
 enum { DFGPU_CACHE_SDPA_AUTO = 0, DFGPU_CACHE_SDPA_STREAM = 1, DFGPU_CACHE_SDPA_UMMA = 2 };
 typedef struct dfgpu_cache_sdpa_params {

@@ -270,3 +270,29 @@ def test_the_restatement_encodes_as_a_search_does():
         assert len({abs(ref.E4M3[c]) for c in ties}) == 1 or code % 2 == 0
     assert ref.encode_e4m3(-0.0) == 0x80 and ref.encode_e4m3(-(2.0 ** -11)) == 0
     assert [ref.scale_code(x) for x in (0.0, 448.0, 448.0001, 896.0, 1.0, np.inf, np.nan)] == [0, 127, 128, 128, 119, 254, 255]
+
+
+def test_outputs_that_overlap_are_refused():
+    refused(14, "rope", rope_params(y=tensor(BF16, [2, 4, 3, 64], [768, 0, 64, 1])), "overlaps")
+    assert cache.query("rope", rope_params(x=tensor(BF16, [2, 4, 3, 64], [768, 0, 64, 1]))).launches == 1   # (a broadcast input is none)
+    both = rope_params(x2=tensor(BF16, [2, 4, 3, 64]), y2=tensor(BF16, [2, 4, 3, 64]))
+    for pointers in ([16, 32, 16, 16, 64, 32], [16, 32, 16, 16, 64, 16], [16, 64, 16, 16, 64, 48]):
+        with pytest.raises(dfgpu.DfgpuError) as error:
+            cache.rope(both, pointers)
+        assert error.value.code == 1 and "other" in str(error.value)
+    refused(14, "cache_sdpa", sdpa_params(stats=tensor(F32, [2, 8, 3, 1], [24, 0, 1, 1])), "overlaps")
+
+
+def test_containers_without_a_stride_are_refused():
+    refused(14, "cache_sdpa", sdpa_params(k=tensor(E4M3, [9, 4, 32, 64], [2048, 0, 64, 1])), "positive")
+    refused(14, "cache_sdpa", sdpa_params(v=tensor(E4M3, [9, 4, 32, 64], [8192, 2048, 0, 1])), "positive")
+
+
+def test_pieces_of_long_sequences():
+    """Few query blocks before many keys: pieces, a merge and scratch for their results; as many blocks as SMs: none."""
+    long = dict(kernel=cache.SDPA_UMMA, page_table_k=tensor(I32, [2, 1, 400, 1]), page_table_v=tensor(I32, [2, 1, 400, 1]))
+    short, cut = (cache.query("cache_sdpa", sdpa_params(**{**long, "s_kv": s_kv})) for s_kv in (500, 12800))
+    assert (short.launches, cut.launches) == (3, 4) and cut.scratch_bytes > short.scratch_bytes
+    rows = [2, 8, 2000, 64]
+    many = cache.query("cache_sdpa", sdpa_params(**{**long, "s_kv": 12800, "q": tensor(BF16, rows), "o": tensor(BF16, rows)}))
+    assert many.launches == 3
