@@ -355,7 +355,8 @@ extern "C" int dfgpu_cache_append(const dfgpu_cache_append_params* p, void* cons
     a.by_blocks = make_fast_divisor(static_cast<uint32_t>(a.blocks));
     a.by_heads = make_fast_divisor(static_cast<uint32_t>(a.heads));
     if (a.units >= (1ll << 31)) return fail(kUnsupported, "CACHE_APPEND: too many blocks in one call");
-    // As few threads as hold a whole block of new tokens in their registers.
+    // As few threads as hold a whole block of new tokens in their registers. 8 x 2048 tokens of 8 heads of 128 bf16 channels: blocks of 16 tokens, a warp 16.4 us,
+    // 128 threads 27.6; of 64, 256 threads 17.9, 512 32.1, a warp 19.8; of 256, 512 threads 20.2, 128 33.1, a warp 58.
     const int64_t vectors = static_cast<int64_t>(std::min(a.tokens, a.seq)) * a.row;
     int threads = 32;
     if (vectors > 32 * held_by(32))

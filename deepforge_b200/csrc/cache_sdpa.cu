@@ -45,9 +45,10 @@ constexpr int kNaN = 0x7fc00000;
 // EIGHTS: eights of rows that a warp takes.
 template <int D, int EIGHTS>
 struct Shape {
+    static_assert(EIGHTS == 1 || D == 64, "see plan_stream");
     static constexpr int kCtas = D == 256 ? 2 : EIGHTS == 1 ? 4 : 3;          // on an SM, by registers
     static constexpr int kSide = kUnit * D;                                   // bytes of a unit's K or V
-    static constexpr int kSlots = D == 64 ? (EIGHTS == 1 ? 6 : 8) : D == 128 && EIGHTS == 2 ? 4 : 3;   // K and V tiles of a warp's ring
+    static constexpr int kSlots = D == 64 ? (EIGHTS == 1 ? 6 : 8) : 3;   // K and V tiles of a warp's ring
     static constexpr int kRing = kWarps * kSlots * kSide;
     static constexpr int kBarriers = kRing;                                   // [warp][slot]
     static constexpr int kTotal = kBarriers + kWarps * kSlots * 8;
@@ -698,7 +699,10 @@ StreamPlan plan_stream(const dfgpu_cache_sdpa_params& p) {
     StreamPlan plan{};
     const int64_t d = p.q.dim[3], group = p.q.dim[1] / p.k.dim[1];
     plan.rows = group * p.q.dim[2];
-    plan.eights = plan.rows <= 8 ? 1 : 2;
+    // With 64 channels two eights of rows share the conversions of a unit (16 rows, 64 sequences, 8 KV heads, 2000 keys: 54 us, 65 in eights; 40 rows: 33 and 32);
+    // with more their registers cost what that gains (128 channels, 16 rows, 24 sequences, 4000 keys: 73 and 70 us, 40 rows: 66 and 60, 64 rows: 81 and 83;
+    // 256 channels, 2000 rows: 831 and 773).
+    plan.eights = plan.rows > 8 && d == 64 ? 2 : 1;
     plan.block_rows = plan.eights * 8;
     plan.row_blocks = static_cast<int>((plan.rows + plan.block_rows - 1) / plan.block_rows);
     const int64_t lists = p.q.dim[0] * p.k.dim[1] * plan.row_blocks, units = (p.s_kv + kUnit - 1) / kUnit;
@@ -711,8 +715,8 @@ StreamPlan plan_stream(const dfgpu_cache_sdpa_params& p) {
 }
 
 // The tcgen05 form has blocks of 256 rows, an SM for each piece of their keys; the streaming form cuts any shape evenly but runs at a fourth to a seventh of
-// its rate. Streaming and tcgen05: 1000 tokens, 8 KV heads, 2000 keys, 128 pieces: 270 and 104 us; 40 tokens, 8 heads, 2000 keys, 32 pieces: 49 and 41;
-// 64 tokens, 2 heads, 4000 keys, 6 pieces: 38 and 49; 32 tokens, one head, 1100 keys, one piece: 28 and 37.
+// its rate. Streaming and tcgen05: 1000 tokens of 4 query heads, 8 KV heads, 2000 keys, 128 pieces: 283 and 102 us; 40 of 8, 8 heads, 2000 keys, 32 pieces: 46 and 40;
+// 64 of 4, 2 heads, 4000 keys, 14 pieces: 34 and 38; 32 of 4, one head, 1100 keys, 2 pieces: 22 and 28.
 bool umma_pays(const dfgpu_cache_sdpa_params& p, const StreamPlan& plan) { return plan.rows >= 128 && 7 * cache_sdpa_umma_items(p) * cache_sdpa_umma_pieces(p) >= kSms; }
 int64_t flag_count(const dfgpu_cache_sdpa_params& p) { return cache_sdpa_umma_items(p) * cache_sdpa_umma_pieces(p); }
 int64_t flag_bytes(const dfgpu_cache_sdpa_params& p, int kernel) { return kernel == DFGPU_CACHE_SDPA_UMMA ? (flag_count(p) + 3) / 4 * 16 : 0; }
@@ -799,7 +803,9 @@ int launch_rows(const CUtensorMap& map_k, const CUtensorMap& map_v, const CacheS
 
 template <typename T, int D>
 int launch_stream(const CUtensorMap& map_k, const CUtensorMap& map_v, const CacheSdpaArgs& a, const StreamPlan& plan, dim3 grid, cudaStream_t stream) {
-    const int status = plan.eights == 1 ? launch_rows<T, D, 1>(map_k, map_v, a, grid, stream) : launch_rows<T, D, 2>(map_k, map_v, a, grid, stream);
+    int status;
+    if constexpr (D == 64) status = plan.eights == 1 ? launch_rows<T, D, 1>(map_k, map_v, a, grid, stream) : launch_rows<T, D, 2>(map_k, map_v, a, grid, stream);
+    else status = launch_rows<T, D, 1>(map_k, map_v, a, grid, stream);
     if (status) return status;
     launch_chained(cache_sdpa_merge_kernel<D>, dim3(static_cast<unsigned>(static_cast<int64_t>(a.entries / a.row_blocks) * a.heads_kv * a.rows)), dim3(D), 0, stream, a);
     return check_launch("CACHE_SDPA merge");

@@ -249,15 +249,14 @@ extern "C" int dfgpu_rope(const dfgpu_rope_params* p, void* const* tensors, void
     a.units = a.turning + (static_cast<int>(p->x.dim[3]) - 2 * a.half) / width;
     a.by_units = make_fast_divisor(static_cast<uint32_t>(a.units));
     a.pitch = a.half + a.turning;   // (eight units of a token and the next token's do not meet in the same banks)
-    // Up to eight tokens a CTA, so that a long run of heads shares each token's sines; then as few heads as give each thread eight units
-    // (fewer, and the sines cost more than the turning), or one where that leaves an SM fewer than sixteen CTAs.
+    // Up to eight tokens a CTA, so that a long run of heads shares each token's sines; then as few heads as give each thread eight units.
+    // (One unit a thread: 108 us for 60 with 2 x 8192 tokens of 40 heads of 128 bf16 channels, 16.1 for 13.2 with 2048, 7.5 for 7.6 with 512: the sines cost more
+    // than the CTAs gain.)
     while (a.token_shift < 3 && (1 << a.token_shift) < a.seq && (a.pitch << (a.token_shift + 1)) <= kRopeTable) ++a.token_shift;
     a.tiles = (a.seq + (1 << a.token_shift) - 1) >> a.token_shift;
     a.by_tiles = make_fast_divisor(static_cast<uint32_t>(a.tiles));
     const int64_t tiles = p->x.dim[0] * a.tiles;
-    auto heads_for = [&](int units) { return std::min(a.heads, (units * kRopeThreads - 1) / (a.units << a.token_shift) + 1); };
-    a.heads_per_cta = heads_for(8);
-    if (tiles * ((a.heads + a.heads_per_cta - 1) / a.heads_per_cta) < 16 * sm_count()) a.heads_per_cta = heads_for(1);
+    a.heads_per_cta = std::min(a.heads, (8 * kRopeThreads - 1) / (a.units << a.token_shift) + 1);
     const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>((a.heads + a.heads_per_cta - 1) / a.heads_per_cta));
     const size_t shared = sizeof(float2) * static_cast<size_t>(a.pitch << a.token_shift);
     const bool interleaved = p->interleaved != 0;
