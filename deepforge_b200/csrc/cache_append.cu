@@ -4,7 +4,9 @@
 // what one call adds to one scale block of K or V: its largest magnitude has to be known before its first code, so a unit's vectors stay in
 // registers between the two (what a block has beyond the last variant's is read again, from the cache). Small blocks take a warp each, larger
 // ones a CTA of as many threads as hold it in four vectors of 16 bytes each; nothing is shared between units, and no atomic is needed. The
-// chain of a unit is length -> new tokens -> largest -> codes, with the page's id on its way beside the tokens.
+// chain of a unit is length -> new tokens -> largest -> codes, with the page's id on its way beside the tokens. Long prompts are next bound by
+// issue slots, so that largest magnitudes go two at a time, codes four, and places are stepped to, not divided (28 to 18 us together).
+// 8 sequences of up to 2048 tokens, 8 heads of 128 bf16 channels, blocks of 64: 17.9 us, 3.2 TB/s, 49 % of the copy rate; one token of 64 sequences: 7.2 us.
 #include <algorithm>
 
 #include "common.cuh"

@@ -1,5 +1,5 @@
-// Attention over a paged cache of E4M3 codes with E8M0 scales: the streaming form, for few query rows a KV head (single tokens,
-// drafted tokens) and for every type and head dimension.
+// Attention over a paged cache of E4M3 codes with E8M0 scales: the streaming form, for few query rows a KV head (single tokens, a few
+// drafted ones) and for every type and head dimension.
 //
 // Bound by HBM: each held code is read once for all query heads of its KV head. A row of the products is a (token, head) pair.
 // Codes are exact in f16 (448 to 2^-9), so K and V go from shared memory through one convert for two codes straight into the
@@ -7,8 +7,8 @@
 // and reading it back is 144 bytes of shared-memory traffic a clock at HBM speed, where the port moves 128. Both products are taken
 // transposed, S^T = K Q^T and O^T = V^T P^T, so that rows come in eights (most groups of query heads are no larger) and 16 keys or
 // channels share an instruction; P^T turns from the first one's result into the second one's operand by movmatrix.
-//   * Q is not rounded: each row is scaled by a power of two that puts its largest magnitude at 2^14, and is exact in f16 down to
-//     2^-38 of that (below, within 2^-39 of it).
+//   * Q is scaled row by row by a power of two that puts its largest magnitude at 2^14: f16 holds it exactly down to 2^-28 of that (bf16:
+//     2^-31), and to within 2^-39 of that below.
 //   * 16 consecutive keys share a page and a scale (both are multiples of 16 tokens). The K scale multiplies their scores. O is
 //     held in units of a power of two, 2^unit: the V scale of 16 keys goes into their probabilities, as 2^(scale - unit), where that is from 2^-10
 //     to 1, and else the unit moves and O with it (exactly, as far as scales within 2^80 of one another go).
@@ -21,8 +21,10 @@
 // are on the chip together, sixteen an SM for single tokens. A warp is on its own: it brings its units by TMA into a private ring of K and V
 // tiles, computes on them and refills each as soon as it has read it, so that nothing is shared and nobody waits for another warp. (CTAs
 // whose warps shared each list's units spent a third of their time on meeting and on beginning lists; a loading warp for four
-// others was what they waited for.) Lists that were cut leave partial results, which a second kernel merges. Rows beyond 16 are
+// others was what they waited for.) Lists that were cut leave partial results, which a second kernel merges. Rows beyond 16 (8) are
 // lists of their own, whose keys come from L2.
+// 64 sequences of 512 to 8192 keys, 8 KV heads of 128 channels, 4 query heads each: 122 us, 4.7 TB/s, 71 % of the copy rate (110 without the arithmetic); two
+// such sequences: 19 us, of which 15 are look-ups, launches and the merge; 16 sequences of 32 or 40 rows: at the choice of a form below.
 #include <algorithm>
 #include <cmath>
 
@@ -717,7 +719,9 @@ StreamPlan plan_stream(const dfgpu_cache_sdpa_params& p) {
 // The tcgen05 form has blocks of 256 rows, an SM for each piece of their keys; the streaming form cuts any shape evenly but runs at a fourth to a seventh of
 // its rate. Streaming and tcgen05: 1000 tokens of 4 query heads, 8 KV heads, 2000 keys, 128 pieces: 283 and 102 us; 40 of 8, 8 heads, 2000 keys, 32 pieces: 46 and 40;
 // 64 of 4, 2 heads, 4000 keys, 14 pieces: 34 and 38; 32 of 4, one head, 1100 keys, 2 pieces: 22 and 28.
-bool umma_pays(const dfgpu_cache_sdpa_params& p, const StreamPlan& plan) { return plan.rows >= 128 && 7 * cache_sdpa_umma_items(p) * cache_sdpa_umma_pieces(p) >= kSms; }
+// Of 256 rows few may be there: 16 rows, 24 sequences, 8 heads, 4000 keys: 70 and 121 us; 32 rows, 16 sequences: 84 and 82; 40 rows, 16 sequences, 4 heads: 60 and 53; 64 rows: 83 and
+// 57; 96 rows, 4 sequences, 8 heads, 8000 keys: 104 and 56.
+bool umma_pays(const dfgpu_cache_sdpa_params& p, const StreamPlan& plan) { return plan.rows >= 32 && 7 * cache_sdpa_umma_items(p) * cache_sdpa_umma_pieces(p) >= kSms; }
 int64_t flag_count(const dfgpu_cache_sdpa_params& p) { return cache_sdpa_umma_items(p) * cache_sdpa_umma_pieces(p); }
 int64_t flag_bytes(const dfgpu_cache_sdpa_params& p, int kernel) { return kernel == DFGPU_CACHE_SDPA_UMMA ? (flag_count(p) + 3) / 4 * 16 : 0; }
 

@@ -92,8 +92,8 @@ int dfgpu_cache_append(const dfgpu_cache_append_params*, void* const* tensors, v
    shift = bottom_right ? SEQ_LEN_KV - SEQ_LEN_Q : 0, kv <= q + shift + right_bound (with has_right_bound) and
    kv > q + shift - left_bound (with has_left_bound). Query rows from SEQ_LEN_Q on, and rows without keys, give O = 0 and
    Stats = -inf. A key whose page id is out of range reads as zeros, as in SDPA. Products take the codes as they are
-   (exact in f16), scales and everything else are f32; the probabilities that weight V are rounded to f16, and Q is not
-   rounded. A code or scale of a masked key, NaN or not, has no effect. Values under a V scale more than 2^80 below
+   (exact in f16), scales and everything else are f32; the probabilities that weight V are rounded to f16, and Q is
+   taken to within 2^-39 of its row's largest magnitude. A code or scale of a masked key, NaN or not, has no effect. Values under a V scale more than 2^80 below
    that of an earlier key of the sequence count as zeros.
    tensors: {Q, K container, V container, O, Stats or null, K scale, V scale, SEQ_LEN_Q or null, SEQ_LEN_KV, Page_table_K,
    Page_table_V}. Q, O [B, Hq, Sq, D] HALF or BFLOAT16, the same type (O may be FLOAT); D contiguous, 64, 128 or 256; Hq a

@@ -770,3 +770,11 @@ def test_tcgen05_form_in_pieces_over_special_values():
         caches[1].view(torch.uint8)[page, 0, 2400 % 64, 5] = 0x7f
 
     attend_case(8, BF16, 128, 1, 2, 150, 64, 64, [2500], right=0, bottom_right=True, kernel=UMMA, spoil=nan_code)
+
+
+@pytest.mark.parametrize("dtype,d,hk,g,sq,left", [(F16, 64, 4, 8, 5, 300), (BF16, 128, 4, 16, 2, None)])
+def test_drafted_tokens_of_large_groups_take_tcgen05(dtype, d, hk, g, sq, left):
+    _, _, info = attend_case(d, dtype, d, hk, g, sq, 48, 16, [700, 5, 9, 1030, 100, 33, 64, 500], right=0, left=left, bottom_right=True)
+    assert info.kernel == UMMA
+    _, _, info = attend_case(d, dtype, d, hk, 7, 4, 48, 16, [700, 5, 9, 1030, 100, 33, 64, 500], right=0, left=left, bottom_right=True)
+    assert info.kernel == cache.SDPA_STREAM
