@@ -53,6 +53,7 @@ struct CachePrefillArgs {
     int32_t blocks;       // of two query tiles
     int32_t batches;
     int32_t pieces;       // of an item's keys
+    int32_t rows;         // of O
 };
 
 template <int D>
@@ -558,13 +559,15 @@ cache_sdpa_pieces_kernel(const __grid_constant__ CachePrefillArgs args) {
     constexpr int kOwn = D / 32;
     const CacheSdpaArgs& a = args.a;
     const int lane = threadIdx.x & 31;
-    const int64_t nth = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5), item = nth / (2 * kRows);
-    const int row = static_cast<int>(nth % (2 * kRows)), tile = row / kRows, in_group = row % kRows / args.tokens;
-    const int block = static_cast<int>(item % args.blocks), token = (block * 2 + tile) * args.tokens + (row % kRows - in_group * args.tokens);
-    const int64_t list = item / args.blocks, batch = list / a.heads_kv;
-    const int head = static_cast<int>(list % a.heads_kv) * a.group + in_group;
+    auto divided = [](int n, const FastDivisor& by) { return static_cast<int>(fast_divide(static_cast<uint32_t>(n), by)); };
+    const int nth = static_cast<int>(blockIdx.x) * 4 + static_cast<int>(threadIdx.x >> 5);   // (sequence, KV head, token, head of the group)
+    const int list = divided(nth, a.by_rows), in_list = nth - list * a.rows, token = divided(in_list, a.by_group), in_group = in_list - token * a.group;
+    const int64_t batch = divided(list, a.by_heads);
+    const int head = (list - static_cast<int>(batch) * a.heads_kv) * a.group + in_group;
+    const int tile = token / args.tokens, row = (tile & 1) * kRows + in_group * args.tokens + (token - tile * args.tokens);
+    const int64_t item = static_cast<int64_t>(list) * args.blocks + (tile >> 1);
     chain_begin();
-    if (in_group >= a.group || token >= a.seq_q || g_device_status != 0) return;
+    if (nth >= args.rows || g_device_status != 0) return;
     const float* from = args.partial + (item * args.pieces * (2 * kRows) + row) * (D + 4);
     constexpr int64_t kNext = 2 * kRows * (D + 4);
     float top = -INFINITY, total = 0.0f, value[kOwn] = {};
@@ -620,6 +623,7 @@ int launch_cache_sdpa_umma(const dfgpu_cache_sdpa_params& p, const CacheSdpaArgs
     args.blocks = (a.seq_q + 2 * args.tokens - 1) / (2 * args.tokens);
     args.batches = static_cast<int>(p.q.dim[0]);
     args.pieces = cache_sdpa_umma_pieces(p);
+    args.rows = static_cast<int>(p.q.dim[0] * p.q.dim[1] * p.q.dim[2]);   // (below 2^31, as the streaming form's merge needs)
     const int64_t items = cache_sdpa_umma_items(p);
     auto run = [&](auto kernel, int bytes) -> int {
         const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
@@ -633,7 +637,7 @@ int launch_cache_sdpa_umma(const dfgpu_cache_sdpa_params& p, const CacheSdpaArgs
         if (args.pieces == 1) return run(cache_sdpa_umma_kernel<T, D, false>, Smem<D>::kDynamic);
         const int status = run(cache_sdpa_umma_kernel<T, D, true>, Smem<D>::kDynamic);
         if (status) return status;
-        launch_chained(merge, dim3(static_cast<unsigned>(items * (2 * kRows / 4))), dim3(128), 0, stream, args);
+        launch_chained(merge, dim3(static_cast<unsigned>((args.rows + 3) / 4)), dim3(128), 0, stream, args);
         return check_launch("CACHE_SDPA pieces");
     };
     const bool half = p.q.dtype == DFGPU_F16;
