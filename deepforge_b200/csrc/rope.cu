@@ -4,8 +4,9 @@
 // tokens and a run of heads, works out the tokens' sines and cosines once into shared memory and turns all the heads' rows by them.
 // position * frequency passes 2^24 for far positions, where f32 has lost the angle: the product and its reduction to one turn are
 // made in f64 (one product, rint and difference a pair and token), the sine and cosine of what is left, within half a turn, in f32.
-// 2 x 8192 tokens, 32 + 8 heads of 128 bf16 channels: 60 to 62 us, 5.4 TB/s, 83 % of the copy rate, with 71 % of the issue slots taken; 3 x 1001 f32 tokens, 16 + 16
-// heads, half of each turned: 23.7 us, 4.1 TB/s; one token of 32 sequences: 5.4 us, a launch.
+// Next come the issue slots (two thirds taken): rows and units are stepped to, and a CTA's heads are of one pair of tensors (3 us less of 59).
+// 2 x 8192 tokens, 32 + 8 heads of 128 bf16 channels: 56 us, 6.0 TB/s, 91 % of the copy rate; 3 x 1001 f32 tokens, 16 + 16 heads, half of each
+// turned: 21 us, 4.7 TB/s; one token of 32 sequences: 5.4 us, a launch.
 #include <algorithm>
 #include <cmath>
 
@@ -31,7 +32,8 @@ struct RopeArgs {
     const float* frequencies;
     int64_t position_batch, position_token, frequency_stride;
     int32_t positions_wide, seq, tiles, token_shift;   // a CTA's tokens: 1 << token_shift
-    int32_t heads, heads_per_cta, half, turning, units, pitch;   // units of V pairs (half) or V channels (interleaved) a row; pitch: of a token in the table
+    int32_t first_side, heads_per_cta, half, turning, units, pitch;   // first_side: runs of heads of the first pair of tensors; units of V pairs (half) or V channels (interleaved) a row; pitch: of a token in the table
+    int32_t rows_on, units_on;                         // kRopeThreads units on: whole rows, and the units beyond
     FastDivisor by_units, by_tiles;
     float scale, sign;
 };
@@ -59,22 +61,16 @@ struct RopeUnit {
     int32_t table;     // the first pair's place in the table; -1: channels to copy, -2: nothing
     int32_t apart;     // elements from the first vector to the second
 
-    __device__ __forceinline__ void load(const RopeArgs& a, int item, int items, int64_t batch, int token0, int head0) {
+    // row: (head of the run, token of the CTA); x, y: of the run's first head and the CTA's first token
+    __device__ __forceinline__ void load(const RopeArgs& a, const RopeSide& s, const T* x, T* y, int row, int rows, int unit, int tokens) {
         table = -2;
-        if (item >= items) return;
-        const int row = static_cast<int>(fast_divide(static_cast<uint32_t>(item), a.by_units)), unit = item - row * a.units;
-        const int local = row & ((1 << a.token_shift) - 1), token = token0 + local;
-        int head = head0 + (row >> a.token_shift);
-        if (token >= a.seq || head >= a.heads) return;
-        const bool second_side = head >= a.side[0].heads;
-        const RopeSide& s = a.side[second_side ? 1 : 0];
-        if (second_side) head -= a.side[0].heads;
+        const int local = row & ((1 << a.token_shift) - 1), head = row >> a.token_shift;
         const bool turns = unit < a.turning;
-        if (!turns && s.in_place) return;
+        if (row >= rows || local >= tokens || (!turns && s.in_place)) return;
         const int channel = turns ? (INTERLEAVED ? unit * (V == 1 ? 2 : V) : unit * V) : 2 * a.half + (unit - a.turning) * V;
         apart = INTERLEAVED ? 1 : a.half;
-        const T* from = static_cast<const T*>(s.x) + batch * s.x_stride[0] + head * s.x_stride[1] + token * s.x_stride[2] + channel;
-        to = static_cast<T*>(s.y) + batch * s.y_stride[0] + head * s.y_stride[1] + token * s.y_stride[2] + channel;
+        const T* from = x + head * s.x_stride[1] + local * s.x_stride[2] + channel;
+        to = y + head * s.y_stride[1] + local * s.y_stride[2] + channel;
         table = turns ? local * a.pitch + unit : -1;
         first = *reinterpret_cast<const Pack<T, V>*>(from);
         if (kTwo && turns) second = *reinterpret_cast<const Pack<T, V>*>(from + apart);
@@ -105,12 +101,17 @@ rope_kernel(RopeArgs a) {
     const int tile = static_cast<int>(blockIdx.x);
     const int batch_index = static_cast<int>(fast_divide(static_cast<uint32_t>(tile), a.by_tiles));
     const int token0 = (tile - batch_index * a.tiles) << a.token_shift;
-    const int head0 = static_cast<int>(blockIdx.y) * a.heads_per_cta;
-    const int heads = min(a.heads_per_cta, a.heads - head0);
-    const int items = (heads << a.token_shift) * a.units;
+    // A CTA's heads are of one pair of tensors, so that all of its addresses share their strides.
+    const bool second_side = static_cast<int>(blockIdx.y) >= a.first_side;
+    const RopeSide s = second_side ? a.side[1] : a.side[0];
+    const int head0 = (static_cast<int>(blockIdx.y) - (second_side ? a.first_side : 0)) * a.heads_per_cta;
+    const int rows = min(a.heads_per_cta, s.heads - head0) << a.token_shift, tokens = a.seq - token0;
+    const T* x = static_cast<const T*>(s.x) + batch_index * s.x_stride[0] + head0 * s.x_stride[1] + token0 * s.x_stride[2];
+    T* y = static_cast<T*>(s.y) + batch_index * s.y_stride[0] + head0 * s.y_stride[1] + token0 * s.y_stride[2];
     chain_begin();
+    int row = static_cast<int>(fast_divide(threadIdx.x, a.by_units)), unit = static_cast<int>(threadIdx.x) - row * a.units;
     Unit now, next;
-    now.load(a, threadIdx.x, items, batch_index, token0, head0);   // (on its way while the angles are worked out)
+    now.load(a, s, x, y, row, rows, unit, tokens);   // (on its way while the angles are worked out)
     for (int i = threadIdx.x; i < a.half << a.token_shift; i += kRopeThreads) {
         const int local = i & ((1 << a.token_shift) - 1), pair = i >> a.token_shift;
         if (token0 + local < a.seq) {
@@ -124,8 +125,10 @@ rope_kernel(RopeArgs a) {
         }
     }
     __syncthreads();
-    for (int item = threadIdx.x; item < items; item += kRopeThreads) {
-        next.load(a, item + kRopeThreads, items, batch_index, token0, head0);
+    while (row < rows) {
+        row += a.rows_on, unit += a.units_on;
+        if (unit >= a.units) unit -= a.units, ++row;
+        next.load(a, s, x, y, row, rows, unit, tokens);
         now.turn_and_store(a, angles);
         now = next;
     }
@@ -244,7 +247,6 @@ extern "C" int dfgpu_rope(const dfgpu_rope_params* p, void* const* tensors, void
     a.scale = p->scale;
     a.sign = p->inverse ? -1.0f : 1.0f;
     a.seq = static_cast<int>(p->x.dim[2]);
-    a.heads = a.side[0].heads + a.side[1].heads;
     a.half = static_cast<int>(p->frequencies.dim[3]);
     const int pairs = p->interleaved && width > 1 ? width / 2 : width;   // of a unit
     a.turning = a.half / pairs;
@@ -252,14 +254,16 @@ extern "C" int dfgpu_rope(const dfgpu_rope_params* p, void* const* tensors, void
     a.by_units = make_fast_divisor(static_cast<uint32_t>(a.units));
     a.pitch = a.half + a.turning;   // (eight units of a token and the next token's do not meet in the same banks)
     // Up to eight tokens a CTA, so that a long run of heads shares each token's sines; then as few heads as give each thread eight units.
-    // (One unit a thread: 108 us for 60 with 2 x 8192 tokens of 40 heads of 128 bf16 channels, 16.1 for 13.2 with 2048, 7.5 for 7.6 with 512: the sines cost more
-    // than the CTAs gain.)
+    // (One unit a thread, all else being equal: 108 us for 60 with 2 x 8192 tokens of 40 heads of 128 bf16 channels, 16.1 for 13.2 with 2048, 7.5 for 7.6 with
+    // 512: the sines cost more than the CTAs gain.)
     while (a.token_shift < 3 && (1 << a.token_shift) < a.seq && (a.pitch << (a.token_shift + 1)) <= kRopeTable) ++a.token_shift;
     a.tiles = (a.seq + (1 << a.token_shift) - 1) >> a.token_shift;
     a.by_tiles = make_fast_divisor(static_cast<uint32_t>(a.tiles));
     const int64_t tiles = p->x.dim[0] * a.tiles;
-    a.heads_per_cta = std::min(a.heads, (8 * kRopeThreads - 1) / (a.units << a.token_shift) + 1);
-    const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>((a.heads + a.heads_per_cta - 1) / a.heads_per_cta));
+    a.heads_per_cta = std::min(std::max(a.side[0].heads, a.side[1].heads), (8 * kRopeThreads - 1) / (a.units << a.token_shift) + 1);
+    a.first_side = (a.side[0].heads + a.heads_per_cta - 1) / a.heads_per_cta;
+    a.rows_on = kRopeThreads / a.units, a.units_on = kRopeThreads % a.units;
+    const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(a.first_side + (a.side[1].heads + a.heads_per_cta - 1) / a.heads_per_cta));
     const size_t shared = sizeof(float2) * static_cast<size_t>(a.pitch << a.token_shift);
     const bool interleaved = p->interleaved != 0;
     cudaStream_t on = as_stream(stream);
