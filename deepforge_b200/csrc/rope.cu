@@ -5,7 +5,7 @@
 // position * frequency passes 2^24 for far positions, where f32 has lost the angle: the product and its reduction to one turn are
 // made in f64 (one product, rint and difference a pair and token), the sine and cosine of what is left, within half a turn, in f32.
 // Next come the issue slots (two thirds taken): rows and units are stepped to, and a CTA's heads are of one pair of tensors (3 us less of 59).
-// 2 x 8192 tokens, 32 + 8 heads of 128 bf16 channels: 56 us, 6.0 TB/s, 91 % of the copy rate; 3 x 1001 f32 tokens, 16 + 16 heads, half of each
+// 2 x 8192 tokens, 32 + 8 heads of 128 bf16 channels: 56 to 59 us, 5.7 to 6.0 TB/s, 86 to 91 % of the copy rate; 3 x 1001 f32 tokens, 16 + 16 heads, half of each
 // turned: 21 us, 4.7 TB/s; one token of 32 sequences: 5.4 us, a launch.
 #include <algorithm>
 #include <cmath>
