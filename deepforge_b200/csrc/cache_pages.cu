@@ -44,6 +44,9 @@ struct PagesArgs {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// Once at the kernel's beginning, the two halves apart: nobody writes into another CTA's shared memory before that CTA is running.
+__device__ __forceinline__ void cluster_arrive_first() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait_first() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t rank;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
@@ -125,7 +128,9 @@ cache_pages_kernel(PagesArgs a) {
     __shared__ PagesShared shared;
     const int thread = static_cast<int>(cluster_rank()) * kPagesThreads + threadIdx.x;
     const int warp = thread >> 5, lane = thread & 31;
+    cluster_arrive_first();
     chain_begin();
+    cluster_wait_first();   // (behind the wait for the kernel before, where the others arrive too)
     if (thread < 8) a.header[thread] = 0;
     int2 total;
 
