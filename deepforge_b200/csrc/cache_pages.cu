@@ -469,6 +469,8 @@ int check_pages(const dfgpu_cache_pages_params& p, PagesSizes& sizes) {
     if (!copy && p.block <= 0) return fail(kInvalidShape, "CACHE_PAGES: tokens per page must be positive");
     if (sizes.pages >= (1ll << 28) || sizes.batch >= (1ll << 28) || (!copy && (p.block >= (1ll << 30) || sizes.slots * p.block >= (1ll << 30))) || sizes.batch * sizes.slots >= (1ll << 40))
         return fail(kUnsupported, "CACHE_PAGES: too many pages, sequences or tokens");
+    // (RESERVE adds up what all sequences lack, those that are refused too, in 32 bits: at most all slots)
+    if (p.op == DFGPU_CACHE_PAGES_RESERVE && sizes.batch * sizes.slots >= (1ll << 31)) return fail(kUnsupported, "CACHE_PAGES: RESERVE over a page table of 2^31 slots or more");
     sizes.entries = 0;
     if (p.op != DFGPU_CACHE_PAGES_COMPACT) {
         const int64_t width = p.op == DFGPU_CACHE_PAGES_FORK || copy ? 2 : 1;

@@ -121,7 +121,7 @@ int dfgpu_cache_sdpa(const dfgpu_cache_sdpa_params*, void* const* tensors, void*
    lowest id first. Results do not depend on timing.
      RESERVE  list [B, 1]: tokens that each sequence is going to add (negative: 0). Sequences get the pages that they lack for that,
               in order; one whose tokens pass P * block, or whose pages and those of all before it that fit their rows are more
-              than the free ones, is refused and keeps its row. Lengths stay.
+              than the free ones, is refused and keeps its row. Lengths stay. The table has fewer than 2^31 slots.
      FORK     list [n, 2]: (source, target) sequences. The target, which must be empty and named by no earlier entry of the kind,
               gets the source's length and shares its full pages (counts grow by one); a last page that is partly filled is copied
               into a free one. Refused: ids out of range, source == target, a target with tokens, and entries for whose copies, and those of all

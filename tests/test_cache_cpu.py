@@ -296,3 +296,12 @@ def test_pieces_of_long_sequences():
     rows = [2, 8, 2000, 64]
     many = cache.query("cache_sdpa", sdpa_params(**{**long, "s_kv": 12800, "q": tensor(BF16, rows), "o": tensor(BF16, rows)}))
     assert many.launches == 3
+
+
+def test_reserve_refuses_tables_whose_demand_could_pass_32_bits():
+    def table(b, slots):
+        return dict(page_table=tensor(I32, [b, 1, slots, 1]), lengths=tensor(I32, [b, 1, 1, 1]), list=tensor(I32, [b, 1]))
+    refused(20, "cache_pages", pages_params("reserve", **table(1 << 14, 1 << 17)), "2^31")
+    refused(20, "cache_pages", pages_params("reserve", **table(1 << 27, 16)), "2^31")
+    assert cache.query("cache_pages", pages_params("reserve", **table((1 << 14) - 1, 1 << 17))).launches == 1
+    assert cache.query("cache_pages", pages_params("free", **table(1 << 14, 1 << 17))).launches == 1   # (counts pages, of which there are fewer than 2^28)
