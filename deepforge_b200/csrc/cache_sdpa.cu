@@ -11,7 +11,7 @@
 //     2^-31), and to within 2^-39 of that below.
 //   * 16 consecutive keys share a page and a scale (both are multiples of 16 tokens). The K scale multiplies their scores. O is
 //     held in units of a power of two, 2^unit: the V scale of 16 keys goes into their probabilities, as 2^(scale - unit), where that is from 2^-10
-//     to 1, and else the unit moves and O with it (exactly, as far as scales within 2^80 of one another go).
+//     to 1, and else the unit moves and O with it (exactly, as far as scales within 2^80 of one another go: what lies further below the largest so far counts as zeros).
 //   * Probabilities are rounded to f16 as p * 2^15: 11 bits down to 2^-29 (2^-19 beside a V scale of 2^-10 units), where p is measured
 //     against the largest score so far.
 // Channels and keys may go to any index of a product as long as both operands agree; the ones taken here give each thread 16-byte
@@ -42,6 +42,7 @@ constexpr int kSms = 148;          // (the cut is a function of the shape and th
 constexpr float kUp = 15.0f;       // probabilities are held as p * 2^15
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kNoUnit = -100000;   // O is zero and has no unit yet
+constexpr int kMostDown = 80;      // O's unit goes down no further below its largest: n keys make at most 2^(15 + 9 + 80) n of it, below f32's range up to 2^24 keys of a warp's part
 constexpr int kNaN = 0x7fc00000;
 
 // EIGHTS: eights of rows that a warp takes.
@@ -124,7 +125,7 @@ struct RowTile {
     int row_lo[EIGHTS][2], row_hi[EIGHTS][2];   // keys that a row sees
     float largest[EIGHTS][2], sum[EIGHTS][2];
     float o[kWide][EIGHTS][4];          // (channel, row), (channel, next row), (next channel, row), (next channel, next row)
-    int unit;
+    int unit, most;                     // most: the largest unit that O has had, over which its values may stand at most 2^80 up (kNoUnit: none)
 
     __device__ static __forceinline__ int channel_of(int j, int eighth) { return D == 64 ? eighth * 8 + 2 * j : (j >> 3) * 128 + eighth * 16 + 2 * (j & 7); }
 
@@ -211,8 +212,9 @@ struct RowTile {
         for (int r = 0; r < 2; ++r) {
             const int code = v_scales[r], apart = code - unit;   // (the same in all threads)
             if ((!SPECIAL || (code >= 0 && code != 255)) && apart != 0) {
-                if (apart < 0 && (apart >= -10 || apart < -80)) {
-                    const uint32_t less = apart < -80 ? 0u : static_cast<uint32_t>(15 + apart) << 10, both = less | less << 16;
+                const bool least = code < most - kMostDown;   // (against all that O holds, not against the last unit: steps down add up)
+                if (apart < 0 && (apart >= -10 || least)) {
+                    const uint32_t less = least ? 0u : static_cast<uint32_t>(15 + apart) << 10, both = less | less << 16;
 #pragma unroll
                     for (int n = 0; n < EIGHTS; ++n) p[r][n][0] = times(p[r][n][0], both), p[r][n][1] = times(p[r][n][1], both);
                 } else {
@@ -223,7 +225,7 @@ struct RowTile {
                         for (int n = 0; n < EIGHTS; ++n)
 #pragma unroll
                             for (int c = 0; c < 4; ++c) o[j][n][c] *= to;
-                    unit = code;
+                    unit = code, most = max(most, code);
                 }
             }
             // V: channels from 16 * eighth on (8 * eighth for a D of 64) of keys 2 quad, 2 quad + 1 and those plus 8
@@ -517,7 +519,7 @@ cache_sdpa_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
         } else {
             any_lo = lo, any_hi = hi;
         }
-        rows.unit = kNoUnit;
+        rows.unit = rows.most = kNoUnit;
 #pragma unroll
         for (int j = 0; j < kWide; ++j)
 #pragma unroll

@@ -4,8 +4,8 @@ import pytest
 
 import cache_reference as ref
 from deepforge_b200 import cache
-from deepforge_b200.dfgpu import I32, tensor
-from test_gpu_cache import ints, pages_state
+from deepforge_b200.dfgpu import BF16, F16, F32, I32, tensor
+from test_gpu_cache import UMMA, attend_case, ints, pages_state
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -34,3 +34,35 @@ def test_page_operations_one_behind_the_other(op):
     torch.cuda.synchronize()
     for got, expected in zip(outs, (want.table, want.lengths, want.refs, report)):
         assert bool((got == ints(expected)).all())
+
+
+# ---- attention: V scales and values far apart
+
+def scales_in_turn(codes):
+    """V scales of neighbouring runs of 16 tokens; under the least scale only zeros, as an append writes them."""
+    def spoil(q, caches, scales, tables):
+        for run in range(scales[1].shape[2]):
+            code = codes[run % len(codes)]
+            scales[1][:, :, run] = code
+            if code == 0:
+                caches[1][:, :, run * 16:run * 16 + 16] = 0
+    return spoil
+
+
+FALLING = [[118, 60, 0, 118], [127, 70, 20, 3], [120, 80, 0, 120], [200, 140, 80, 20], [127, 116, 105, 46]]
+
+
+def check_falling(d, codes):
+    for sq, g in ((1, 4), (6, 2), (1, 20)):
+        attend_case(d + sq, BF16, d, 2, g, sq, 64, 16, [300, 70, 1000], spoil=scales_in_turn(codes), right=0, bottom_right=True)
+    attend_case(d, F16, d, 8, 4, 1, 64, 16, [9000, 100, 6000, 0, 12000, 33, 7000, 2000], spoil=scales_in_turn(codes), o_type=F32)      # all parts
+    if d < 256:
+        attend_case(d, BF16, d, 1, 4, 50, 64, 16, [300, 70], spoil=scales_in_turn(codes), right=0, bottom_right=True, kernel=UMMA)
+        attend_case(d, BF16, d, 1, 4, 50, 64, 16, [3000], spoil=scales_in_turn(codes), right=0, bottom_right=True, kernel=UMMA)         # in pieces
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("codes", FALLING)
+def test_scales_that_fall_in_steps(d, codes):
+    """V scales that fall by less than 2^80 each and by more together: what was made of the larger ones stays finite."""
+    check_falling(d, codes)
