@@ -581,21 +581,22 @@ cache_sdpa_stream_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
                 for (int x = 4; x < 32; x <<= 1) rows.sum[n][c] += __shfl_xor_sync(0xffffffffu, rows.sum[n][c], x);
                 const int row = row_first + n * 8 + quad * 2 + c;
                 if (row >= a.rows) continue;
-                const float top = rows.largest[n][c], total = rows.sum[n][c];
+                // The sum goes first: O alone carries the probabilities' 2^15 and as many values as there are keys, which V far above one takes past f32's range.
+                const float top = rows.largest[n][c], total = rows.sum[n][c], inverse = total == 0.0f ? 1.0f : 1.0f / total;
                 if (!whole) {
                     float* partial = a.partial + (static_cast<int64_t>(part * 2 + (first_piece ? 0 : 1)) * a.block_rows + (row - row_first)) * (D + 2);
 #pragma unroll
-                    for (int j = 0; j < kWide; ++j) *reinterpret_cast<float2*>(partial + Rows::channel_of(j, eighth)) = make_float2(rows.o[j][n][c] * absolute, rows.o[j][n][c + 2] * absolute);
+                    for (int j = 0; j < kWide; ++j)
+                        *reinterpret_cast<float2*>(partial + Rows::channel_of(j, eighth)) = make_float2(rows.o[j][n][c] * inverse * absolute, rows.o[j][n][c + 2] * inverse * absolute);
                     if (eighth == 0) *reinterpret_cast<float2*>(partial + D) = make_float2(top, total);
                 } else {
                     int token, head_q;
                     place_of(row, token, head_q);
                     const bool none = token >= window.len_q || total == 0.0f;   // (a NaN sum is a NaN result)
-                    const float inverse = 1.0f / total;
                     const int64_t at = batch * a.o_stride[0] + head_q * a.o_stride[1] + token * a.o_stride[2];
 #pragma unroll
                     for (int j = 0; j < kWide; ++j)
-                        store_pair(a, at + Rows::channel_of(j, eighth), none ? 0.0f : rows.o[j][n][c] * absolute * inverse, none ? 0.0f : rows.o[j][n][c + 2] * absolute * inverse);
+                        store_pair(a, at + Rows::channel_of(j, eighth), none ? 0.0f : rows.o[j][n][c] * inverse * absolute, none ? 0.0f : rows.o[j][n][c + 2] * inverse * absolute);
                     if (eighth == 0 && a.stats)
                         a.stats[batch * a.stats_stride[0] + head_q * a.stats_stride[1] + token * a.stats_stride[2]] = none ? -INFINITY : top * kLn2 + logf(total * 0x1p-15f);
                 }
@@ -660,19 +661,25 @@ cache_sdpa_merge_kernel(const __grid_constant__ CacheSdpaArgs a) {
 #pragma unroll
             for (int k = 0; k < kAhead; ++k)
                 if (i0 + k * kWarpsHere < parts) largest = fmaxf(largest, pair[k].x);
-            const float down = top == -INFINITY ? 1.0f : exp2_of(top - largest);   // (no score above -inf: zeros, or NaNs that are to be seen)
-            total *= down;
+            // A part has the mean of its values, a weight its share of the sum so far: no sum of values that could pass f32's range.
+            float weight[kAhead], sum = total * (top == -INFINITY ? 1.0f : exp2_of(top - largest));   // (no score above -inf: zeros, or NaNs that are to be seen)
+            const float before = sum;
 #pragma unroll
-            for (int e = 0; e < kOwn; ++e) value[e] *= down;
-            top = largest;
+            for (int k = 0; k < kAhead; ++k) {
+                weight[k] = i0 + k * kWarpsHere < parts ? pair[k].y * (pair[k].x == -INFINITY ? 1.0f : exp2_of(pair[k].x - largest)) : 0.0f;
+                sum += weight[k];
+            }
+            const float inverse = sum == 0.0f ? 1.0f : 1.0f / sum, keep = before * inverse;
+#pragma unroll
+            for (int e = 0; e < kOwn; ++e) value[e] *= keep;
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
                 if (i0 + k * kWarpsHere >= parts) continue;
-                const float weight = pair[k].x == -INFINITY ? 1.0f : exp2_of(pair[k].x - largest);
-                total = fmaf(pair[k].y, weight, total);
+                const float share = weight[k] * inverse;
 #pragma unroll
-                for (int e = 0; e < kOwn; ++e) value[e] = fmaf(ahead[k][e], weight, value[e]);
+                for (int e = 0; e < kOwn; ++e) value[e] = fmaf(ahead[k][e], share, value[e]);
             }
+            top = largest, total = sum;
         }
     }
     if (lane == 0) meeting[warp] = make_float2(top, total);
@@ -683,14 +690,17 @@ cache_sdpa_merge_kernel(const __grid_constant__ CacheSdpaArgs a) {
     top = -INFINITY, total = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWarpsHere; ++w) top = fmaxf(top, meeting[w].x);
+    float weight[kWarpsHere];
 #pragma unroll
     for (int w = 0; w < kWarpsHere; ++w) {
-        const float weight = meeting[w].x == -INFINITY ? 1.0f : exp2_of(meeting[w].x - top);
-        total = fmaf(meeting[w].y, weight, total);
-        result = fmaf(values[w][threadIdx.x], weight, result);
+        weight[w] = meeting[w].y * (meeting[w].x == -INFINITY ? 1.0f : exp2_of(meeting[w].x - top));
+        total += weight[w];
     }
+    const float inverse = 1.0f / total;
+#pragma unroll
+    for (int w = 0; w < kWarpsHere; ++w) result = fmaf(values[w][threadIdx.x], weight[w] * inverse, result);
     const bool none = !takes_part || total == 0.0f;
-    store_from_f32(a.o, a.o_type, batch * a.o_stride[0] + head * a.o_stride[1] + token * a.o_stride[2] + threadIdx.x, none ? 0.0f : result / total);
+    store_from_f32(a.o, a.o_type, batch * a.o_stride[0] + head * a.o_stride[1] + token * a.o_stride[2] + threadIdx.x, none ? 0.0f : result);
     if (threadIdx.x == 0 && a.stats) a.stats[batch * a.stats_stride[0] + head * a.stats_stride[1] + token * a.stats_stride[2]] = none ? -INFINITY : top * kLn2 + logf(total * 0x1p-15f);
 }
 

@@ -22,7 +22,7 @@ struct CacheSdpaArgs {
     float* stats;
     const int32_t* seq_q_data;
     const int32_t* seq_kv_data;
-    float* partial;       // [part][first list, last list][row][D + 2]: O against the part's own largest score, that score, sum
+    float* partial;       // [part][first list, last list][row][D + 2]: the part's own O, the largest score in it, the sum against that
     int32_t* starts;      // [0] units a part, [1 + list] the list's first unit among all, -1: one part has all of it
     int64_t q_stride[3], o_stride[3], stats_stride[3], seq_q_stride, seq_kv_stride;
     int64_t left, right;

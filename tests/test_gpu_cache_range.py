@@ -52,6 +52,9 @@ def scales_in_turn(codes):
 FALLING = [[118, 60, 0, 118], [127, 70, 20, 3], [120, 80, 0, 120], [200, 140, 80, 20], [127, 116, 105, 46]]
 
 
+FALLING_FROM_FAR = [[240, 170, 100, 30], [241, 161, 81, 1]]      # (448 * 2^114 is below f32's largest)
+
+
 def check_falling(d, codes):
     for sq, g in ((1, 4), (6, 2), (1, 20)):
         attend_case(d + sq, BF16, d, 2, g, sq, 64, 16, [300, 70, 1000], spoil=scales_in_turn(codes), right=0, bottom_right=True)
@@ -66,3 +69,27 @@ def check_falling(d, codes):
 def test_scales_that_fall_in_steps(d, codes):
     """V scales that fall by less than 2^80 each and by more together: what was made of the larger ones stays finite."""
     check_falling(d, codes)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("codes", FALLING_FROM_FAR)
+def test_scales_that_fall_in_steps_from_far_above_one(d, codes):
+    check_falling(d, codes)
+
+
+def large_values(code):
+    def spoil(q, caches, scales, tables):
+        caches[1][:] = 0x7E        # 448
+        scales[1][:] = code
+    return spoil
+
+
+@pytest.mark.parametrize("code", [218, 228, 244])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_values_far_above_one(d, code):
+    """V of 1e30, 2^110 and 2^126 under long sequences: the weights' scale and the number of keys do not reach the results."""
+    for lengths, hk, sq in (([16000], 1, 1), ([5000, 16000, 700], 2, 3), ([60] * 512, 8, 1)):      # cut lists, and whole ones
+        attend_case(d, BF16, d, hk, 2, sq, 64, 64, lengths, spoil=large_values(code), right=0, bottom_right=True)
+    if d < 256:
+        attend_case(d, BF16, d, 1, 4, 64, 64, 64, [5000], spoil=large_values(code), right=0, bottom_right=True, kernel=UMMA)
+        attend_case(d, BF16, d, 2, 4, 64, 64, 64, [200, 130], spoil=large_values(code), right=0, bottom_right=True, kernel=UMMA)
