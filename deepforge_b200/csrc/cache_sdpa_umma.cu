@@ -323,7 +323,7 @@ cache_sdpa_umma_kernel(const __grid_constant__ CachePrefillArgs args) {
                         scale[0] = code < 0 ? 1.0f : decode_e8m0(static_cast<uint32_t>(code));
                         flag = flag || code == 255;
                     } else {
-                        const int exponent = max(code < 0 ? 127 : code, kLeastCode) - 127;
+                        const int exponent = max(code, kLeastCode) - 127;   // (the least where there is no page: its zeros must not lift the reference above the scales beside them)
                         *reinterpret_cast<float2*>(scale + 2) = make_float2(static_cast<float>(exponent), power_of_two(max(-exponent, -126)));
                         if (code >= kLeastCode) v_least = min(v_least, code), v_most = max(v_most, code);
                         flag = flag || code >= 253;   // (a NaN among them)

@@ -93,3 +93,12 @@ def test_values_far_above_one(d, code):
     if d < 256:
         attend_case(d, BF16, d, 1, 4, 64, 64, 64, [5000], spoil=large_values(code), right=0, bottom_right=True, kernel=UMMA)
         attend_case(d, BF16, d, 2, 4, 64, 64, 64, [200, 130], spoil=large_values(code), right=0, bottom_right=True, kernel=UMMA)
+
+
+def test_absent_pages_beside_small_scales_on_tcgen05():
+    """Keys whose V page is none count in the sum alone, however small the scales beside them."""
+    def spoil(q, caches, scales, tables):
+        scales[1][:] = torch.randint(85, 100, scales[1].shape, device="cuda").to(torch.uint8)
+    for d in (64, 128):
+        attend_case(d, BF16, d, 2, 4, 40, 64, 16, [300, 170], bad_pages=True, spoil=spoil, right=0, bottom_right=True, kernel=UMMA)
+        attend_case(d, F16, d, 1, 4, 64, 64, 16, [3000], bad_pages=True, spoil=spoil, o_type=F32, right=0, bottom_right=True, kernel=UMMA)     # in pieces
