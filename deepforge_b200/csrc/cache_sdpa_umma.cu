@@ -17,7 +17,7 @@
 // What this cannot do exactly it says in a flag of the item, and the streaming form then computes the whole call again (its kernels return at
 // once otherwise): a NaN among V codes of a tile that some rows do not see all of (their zero probability times it is NaN), a V
 // scale of 2^126 or more, a scale that is a NaN, V scales more than 2^16
-// apart or below 2^-80 over codes that are not zero, scores beyond 2^10.
+// apart or below 2^-80 over codes that are not zero, V scales above 2^16 beside zeros under the least one or pages that are none, scores beyond 2^10.
 // 1000 tokens behind 3000 and 16000 keys, 8 KV heads of 128 channels, 4 query heads each: 440 to 446 us, 670 TFLOP/s, 41 % of the bf16 rate; a pair of score
 // tiles every 5000 clocks, where the products take 2048. Without the exponentials 443 of 457 us then: the chain of a half's scores, maxima,
 // exponentials and store, on two warps a scheduler, and the last items' end (148 of 128 tiles' time on 148 SMs).
@@ -39,6 +39,7 @@ constexpr float kUp = 11.0f;         // P = 2^(t - r + 11): at most 2^15 while t
 constexpr float kRaise = 4.0f;
 constexpr int kLeastCode = 47;       // V scales below 2^-80 count as that (over zeros; else a flag)
 constexpr int kMostApart = 16;
+constexpr int kMostAboveLeast = 96;  // beside zeros under the least scale: P of these, 2^(-80 - r + 11) where r is up to 96 - 80, has to stay in f32's range for the sum, down to 2^-30 of the row's largest weight, where the sum made so far is taken down to a new r
 constexpr float kLeastFactor = 1.17549435e-38f;   // (of a score: not zero, so that -inf stays -inf)
 constexpr float kMostReference = 1024.0f;   // |r|: the exponent's one rounding, of score * factor + (scale - r), is below 2^-14 up to there
 constexpr int kSms = 148, kLeastTiles = 4;   // of key tiles that a piece has
@@ -272,7 +273,7 @@ cache_sdpa_umma_kernel(const __grid_constant__ CachePrefillArgs args) {
             common_lo = max(l0, l1), common_hi = min(h0, h1);
         }
         int v_least = 1 << 20, v_most = -1;
-        bool flag = false;
+        bool flag = false, least = false;   // least: some key that is seen has the least V scale, or no page
         // Lane l has run l % 8: its page (as the table has it), where it begins in it, and its scale.
         const int run = lane & 7;
         auto look_up = [&](int j, int& page, int& token) {
@@ -325,7 +326,9 @@ cache_sdpa_umma_kernel(const __grid_constant__ CachePrefillArgs args) {
                     } else {
                         const int exponent = max(code, kLeastCode) - 127;   // (the least where there is no page: its zeros must not lift the reference above the scales beside them)
                         *reinterpret_cast<float2*>(scale + 2) = make_float2(static_cast<float>(exponent), power_of_two(max(-exponent, -126)));
+                        const int key = (first + j) * kKeys + run * 16;
                         if (code >= kLeastCode) v_least = min(v_least, code), v_most = max(v_most, code);
+                        else least = least || (key < all_hi && key + 16 > all_lo);
                         flag = flag || code >= 253;   // (a NaN among them)
                     }
                 }
@@ -364,7 +367,7 @@ cache_sdpa_umma_kernel(const __grid_constant__ CachePrefillArgs args) {
             code = code_next;
         }
         v_least = __reduce_min_sync(0xffffffffu, v_least), v_most = __reduce_max_sync(0xffffffffu, v_most);
-        if (flag || v_most - v_least > kMostApart) misc[1] = 1;
+        if (flag || v_most - v_least > kMostApart || (least && v_most > kLeastCode + kMostAboveLeast)) misc[1] = 1;
     } else {
         // ---- a row a thread
         const int i = warp >> 2, row = threadIdx.x & 127, quarter = warp & 3;

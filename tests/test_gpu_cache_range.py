@@ -102,3 +102,15 @@ def test_absent_pages_beside_small_scales_on_tcgen05():
     for d in (64, 128):
         attend_case(d, BF16, d, 2, 4, 40, 64, 16, [300, 170], bad_pages=True, spoil=spoil, right=0, bottom_right=True, kernel=UMMA)
         attend_case(d, F16, d, 1, 4, 64, 64, 16, [3000], bad_pages=True, spoil=spoil, o_type=F32, right=0, bottom_right=True, kernel=UMMA)     # in pieces
+
+
+@pytest.mark.parametrize("code", [140, 150, 180, 202, 245])
+def test_zero_blocks_beside_large_values_on_tcgen05(code):
+    """Blocks of zeros with the least scale, and pages that are none, beside V scales far above one: their weights stay in the sum."""
+    def spoil(q, caches, scales, tables):
+        scales[1][:] = code
+        scales[1][:, :, ::2] = 0
+        caches[1].view(*caches[1].shape[:2], -1, 2, 16, caches[1].shape[3])[:, :, :, 0] = 0
+    for lengths in ([300, 170], [3000]):
+        for bad_pages in (False, True):
+            attend_case(code, BF16, 128, 1, 4, 64, 64, 16, lengths, bad_pages=bad_pages, spoil=spoil, right=0, bottom_right=True, kernel=UMMA)
