@@ -578,10 +578,11 @@ cache_sdpa_pieces_kernel(const __grid_constant__ CachePrefillArgs args) {
 #pragma unroll 4
     for (int i = 0; i < args.pieces; ++i) {
         const float2 of = *reinterpret_cast<const float2*>(from + i * kNext + D);
-        const float weight = of.x == -INFINITY ? 1.0f : exp2_of(of.x - top);   // (no score above -inf: zeros, or NaNs that are to be seen)
-        total = fmaf(of.y, weight, total);
+        // In two halves: under V scales far apart the references are so too, by up to 2^205, and a small weight may meet a large sum.
+        const float root = of.x == -INFINITY ? 1.0f : exp2_of(0.5f * (of.x - top));   // (no score above -inf: zeros, or NaNs that are to be seen)
+        total = fmaf(of.y * root, root, total);
 #pragma unroll
-        for (int e = 0; e < kOwn; ++e) value[e] = fmaf(from[i * kNext + lane * kOwn + e], weight, value[e]);
+        for (int e = 0; e < kOwn; ++e) value[e] = fmaf(from[i * kNext + lane * kOwn + e] * root, root, value[e]);
     }
     const bool none = total == 0.0f;
     const int64_t at = batch * a.o_stride[0] + head * a.o_stride[1] + token * a.o_stride[2] + lane * kOwn;

@@ -114,3 +114,14 @@ def test_zero_blocks_beside_large_values_on_tcgen05(code):
     for lengths in ([300, 170], [3000]):
         for bad_pages in (False, True):
             attend_case(code, BF16, 128, 1, 4, 64, 64, 16, lengths, bad_pages=bad_pages, spoil=spoil, right=0, bottom_right=True, kernel=UMMA)
+
+
+@pytest.mark.parametrize("first,second", [(217, 52), (52, 217), (127, 52), (240, 90)])
+def test_pieces_of_scales_far_apart_on_tcgen05(first, second):
+    """One half of the keys under a V scale far above the other's, neighbours within each piece alike: the sum has the weights of both."""
+    def spoil(q, caches, scales, tables):
+        scales[1][tables[1][0, :40].long()] = first
+        scales[1][tables[1][0, 40:].long()] = second
+    for d in (64, 128):
+        _, _, info = attend_case(d, BF16, d, 1, 4, 64, 64, 64, [5120], spoil=spoil, kernel=UMMA)
+        assert info.launches == 4
