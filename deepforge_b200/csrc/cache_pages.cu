@@ -176,8 +176,12 @@ cache_pages_kernel(PagesArgs a) {
         const int available = total.x;
         wanted_most = min(total.y, available);
         int rank = before.x;
-        for (int i = page0; i < page1 && rank < wanted_most; ++i)
-            if (a.refs[i] <= 0) a.pages_a[rank++] = i;
+        for (int i = page0; i < page1 && rank < wanted_most; ++i) {
+            const int count = a.refs[i];
+            if (count > 0) continue;
+            a.pages_a[rank++] = i;
+            if (kFork && count < 0) a.refs_out[i] = 0;   // (what is added to it below makes it one)
+        }
         int ahead = before.y;
         int2 taken = make_int2(0, 0);   // pages, refused
         int copied = 0;

@@ -115,7 +115,7 @@ int dfgpu_query_cache_sdpa(const dfgpu_cache_sdpa_params*, dfgpu_plan_info*);
 int dfgpu_cache_sdpa(const dfgpu_cache_sdpa_params*, void* const* tensors, void* scratch, void* stream);
 
 /* ---- pages -------------------------------------------------------------------------------------
-   A page is free where its reference count is 0. Every operation reads {page table, lengths, refs} and writes whole tables of
+   A page is free where its reference count is 0 (or less; one that is taken has a count of 1). Every operation reads {page table, lengths, refs} and writes whole tables of
    what they are afterwards to {table_out, lengths_out, refs_out}, each of which may be its input itself. A sequence of n tokens uses its
    first ceil(n / block) slots (lengths are clamped to [0, P * block]); ids outside [0, pages) there count for nothing. Free pages are taken
    lowest id first. Results do not depend on timing.

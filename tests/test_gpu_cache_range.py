@@ -4,8 +4,8 @@ import pytest
 
 import cache_reference as ref
 from deepforge_b200 import cache
-from deepforge_b200.dfgpu import BF16, F16, F32, I32, tensor
-from test_gpu_cache import UMMA, attend_case, ints, pages_state
+from deepforge_b200.dfgpu import BF16, F16, F32, I32, U8, tensor
+from test_gpu_cache import UMMA, attend_case, ints, pages_state, run_pages
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -125,3 +125,17 @@ def test_pieces_of_scales_far_apart_on_tcgen05(first, second):
     for d in (64, 128):
         _, _, info = attend_case(d, BF16, d, 1, 4, 64, 64, 64, [5120], spoil=spoil, kernel=UMMA)
         assert info.launches == 4
+
+
+# ---- lists and counts that contradict themselves
+
+@pytest.mark.parametrize("in_place", [False, True])
+def test_fork_into_pages_with_negative_counts(in_place):
+    """A page whose count fell below 0 is free; a fork that takes it leaves it with a count of one."""
+    table, lengths, refs = np.full((3, 4), -1, np.int32), np.array([20, 0, 0], np.int32), np.array([-3, -1, 0, 1, 0, 1], np.int32)
+    table[0, :2] = 3, 5
+    state = ref.Pages(table, lengths, refs, [np.arange(6 * 8, dtype=np.uint8).reshape(1, 6, 8)], 16)
+    (got, got_lengths, got_refs), report, pools = run_pages("fork", state, [[0, 1], [0, 2]], [(1, 8, U8)], in_place=in_place)
+    assert got.tolist() == [[3, 5, -1, -1], [3, 0, -1, -1], [3, 1, -1, -1]] and got_lengths.tolist() == [20, 20, 20]
+    assert got_refs.tolist() == [1, 1, 0, 3, 0, 1] and report == [2, 2, 2, 0]
+    assert np.array_equal(pools[0][0, 0], state.pools[0][0, 5]) and np.array_equal(pools[0][0, 1], state.pools[0][0, 5])
