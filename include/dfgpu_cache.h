@@ -130,8 +130,9 @@ int dfgpu_cache_sdpa(const dfgpu_cache_sdpa_params*, void* const* tensors, void*
               not below 0; their rows become -1 and their lengths 0.
      COMPACT  no list. With L pages in use, those with ids >= L move to the free ids < L, in order: contents, counts and the
               used slots of all tables follow.
-     COPY     list [n, 2]: (source, target) pages. A target named twice receives the last of its sources. Refused: ids out of range,
-              source == target, and entries whose source is another entry's target. Table, lengths and counts stay.
+     COPY     list [n, 2]: (source, target) pages. Refused: ids out of range, source == target, and entries whose source is another entry's
+              target (one of ids in range that differ, refused or not). Of the entries that name a target, ids out of range and equal ones apart, only the last
+              counts: it is copied, or where it is refused for its source, nothing is; the others are neither copied nor refused. Table, lengths and counts stay.
    Entries of a list whose first id is negative are skipped without being refused (FORK, FREE, COPY), so a list may be longer than what it says.
    report INT32 [4] (or null): free pages afterwards; pages taken, given back or moved (COPY: copied); page copies; entries refused.
    tensors: {page table, lengths, refs, list or null, table_out, lengths_out, refs_out, report or null, pool 0, ...}. page table

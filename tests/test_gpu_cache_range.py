@@ -139,3 +139,21 @@ def test_fork_into_pages_with_negative_counts(in_place):
     assert got.tolist() == [[3, 5, -1, -1], [3, 0, -1, -1], [3, 1, -1, -1]] and got_lengths.tolist() == [20, 20, 20]
     assert got_refs.tolist() == [1, 1, 0, 3, 0, 1] and report == [2, 2, 2, 0]
     assert np.array_equal(pools[0][0, 0], state.pools[0][0, 5]) and np.array_equal(pools[0][0, 1], state.pools[0][0, 5])
+
+
+@pytest.mark.parametrize("entries,pairs,refused", [
+    ([(0, 5), (1, 5), (2, 1)], [(2, 1)], 1),                # the last entry for 5 is refused, its source being a target: 5 receives nothing
+    ([(1, 5), (2, 1), (0, 5)], [(2, 1), (0, 5)], 1),        # the last one stands
+    ([(0, 5), (1, 5), (1, 5)], [(1, 5)], 0),                # the same twice
+    ([(0, 5), (9, 5), (5, 5)], [(0, 5)], 2),                # ids out of range and equal ones name no target
+    ([(0, 5), (5, 0), (1, 0)], [(1, 0)], 2),
+    ([(-1, 5), (0, 5), (-2, 5)], [(0, 5)], 0),
+])
+def test_copy_takes_the_last_entry_of_a_target_alone(entries, pairs, refused):
+    rng = np.random.default_rng(0)
+    state = ref.Pages(np.full((1, 2), -1, np.int32), np.zeros(1, np.int32), np.array([1, 1, 1, 1, 1, 0, 0, 0], np.int32), [rng.integers(0, 256, (2, 8, 24)).astype(np.uint8)], 16)
+    _, report, pools = run_pages("copy", state, entries, [(2, 24, U8)])
+    want = state.pools[0].copy()
+    for source, target in pairs:
+        want[:, target] = state.pools[0][:, source]
+    assert np.array_equal(pools[0], want) and report == [3, len(pairs), len(pairs), refused]
