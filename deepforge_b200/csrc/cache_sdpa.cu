@@ -861,6 +861,8 @@ extern "C" int dfgpu_cache_sdpa(const dfgpu_cache_sdpa_params* p, void* const* t
     for (int i : {4, 7, 8, 9, 10})
         if ((reinterpret_cast<uintptr_t>(tensors[i]) & 3u) != 0) return fail(kInvalidArgument, "CACHE_SDPA: port %d is not aligned to its type", i);
     if (!scratch || !on_16(scratch)) return fail(kInvalidArgument, "CACHE_SDPA: needs the 16-byte aligned scratch dfgpu_query_cache_sdpa reports");
+    // (what the tcgen05 form leaves to the streaming form reads Q again after O has been written)
+    if (tensors[0] == tensors[3]) return fail(kInvalidArgument, "CACHE_SDPA: O is Q");
     CacheSdpaArgs a{};
     a.q = tensors[0];
     a.o = tensors[3];

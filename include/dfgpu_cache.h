@@ -97,7 +97,7 @@ int dfgpu_cache_append(const dfgpu_cache_append_params*, void* const* tensors, v
    that of an earlier key of the sequence count as zeros.
    tensors: {Q, K container, V container, O, Stats or null, K scale, V scale, SEQ_LEN_Q or null, SEQ_LEN_KV, Page_table_K,
    Page_table_V}. Q, O [B, Hq, Sq, D] HALF or BFLOAT16, the same type (O may be FLOAT); D contiguous, 64, 128 or 256; Hq a
-   multiple of Hk. Containers with D contiguous, their other strides positive multiples of 16 and 16-byte aligned; T and t multiples of 16. Stats FLOAT
+   multiple of Hk. O must not overlap Q or any other input. Containers with D contiguous, their other strides positive multiples of 16 and 16-byte aligned; T and t multiples of 16. Stats FLOAT
    [B, Hq, Sq, 1]: max + ln(sum). SEQ_LEN_Q absent: all Sq rows. s_kv bounds the keys of every sequence (at most P * T). */
 enum { DFGPU_CACHE_SDPA_AUTO = 0, DFGPU_CACHE_SDPA_STREAM = 1, DFGPU_CACHE_SDPA_UMMA = 2 };
 typedef struct dfgpu_cache_sdpa_params {

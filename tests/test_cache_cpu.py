@@ -305,3 +305,10 @@ def test_reserve_refuses_tables_whose_demand_could_pass_32_bits():
     refused(20, "cache_pages", pages_params("reserve", **table(1 << 27, 16)), "2^31")
     assert cache.query("cache_pages", pages_params("reserve", **table((1 << 14) - 1, 1 << 17))).launches == 1
     assert cache.query("cache_pages", pages_params("free", **table(1 << 14, 1 << 17))).launches == 1   # (counts pages, of which there are fewer than 2^28)
+
+
+def test_attention_does_not_write_over_its_queries():
+    for kernel in (cache.SDPA_AUTO, cache.SDPA_STREAM, cache.SDPA_UMMA):
+        with pytest.raises(dfgpu.DfgpuError) as error:
+            cache.cache_sdpa(sdpa_params(kernel=kernel), [4096, 16, 16, 4096, None, 16, 16, None, 16, 16, 16], 256)
+        assert error.value.code == 1 and "O is Q" in str(error.value)
