@@ -341,6 +341,8 @@ extern "C" int dfgpu_cache_append(const dfgpu_cache_append_params* p, void* cons
     int32_t* lengths_out = p->lengths_out.rank ? static_cast<int32_t*>(tensors[10]) : nullptr;
     const bool in_place = lengths_out == a.lengths;
     a.lengths_out = in_place ? nullptr : lengths_out;
+    // (`added` is still read while lengths_out is written; in place the lengths come in a launch of their own)
+    if (lengths_out && !in_place && lengths_out == a.added) return fail(kInvalidArgument, "CACHE_APPEND: lengths_out is added");
     a.lengths_stride = p->lengths.stride[0];
     a.added_stride = p->added.rank ? p->added.stride[0] : 0;
     a.out_stride = p->lengths_out.rank ? p->lengths_out.stride[0] : 0;

@@ -74,7 +74,7 @@ int dfgpu_rope_frequencies(const dfgpu_rope_scaling*, float* frequencies, float*
    tensors: {K, V, K container, V container, K scale, V scale, page table of K, page table of V, lengths, added or null,
    lengths_out or null}. K, V [B, Hk, S, D] FLOAT, HALF or BFLOAT16 (any strides, D contiguous); page tables INT32 [B,1,P,1]
    (both may be the same); lengths, added, lengths_out INT32 [B,1,1,1]: tokens before the call (a negative one counts as 0), new
-   tokens (absent: S; clamped to [0, S]), and their sum (clamped to P * T of the K table), which may be `lengths` itself. Positions past a table's P * T are not
+   tokens (absent: S; clamped to [0, S]), and their sum (clamped to P * T of the K table), which may be `lengths` itself, but not `added`. Positions past a table's P * T are not
    written. A page that two sequences share must not be written: fork first. */
 enum { DFGPU_CACHE_APPEND_AUTO = 0, DFGPU_CACHE_APPEND_VECTOR = 1, DFGPU_CACHE_APPEND_SCALAR = 2 };
 typedef struct dfgpu_cache_append_params {

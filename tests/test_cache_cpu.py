@@ -312,3 +312,10 @@ def test_attention_does_not_write_over_its_queries():
         with pytest.raises(dfgpu.DfgpuError) as error:
             cache.cache_sdpa(sdpa_params(kernel=kernel), [4096, 16, 16, 4096, None, 16, 16, None, 16, 16, 16], 256)
         assert error.value.code == 1 and "O is Q" in str(error.value)
+
+
+def test_append_does_not_write_lengths_over_the_counts_it_reads():
+    vector = tensor(I32, [2, 1, 1, 1])
+    with pytest.raises(dfgpu.DfgpuError) as error:
+        cache.cache_append(append_params(added=vector, lengths_out=vector), [16, 16, 16, 32, 16, 32, 16, 16, 64, 128, 128])
+    assert error.value.code == 1 and "lengths_out is added" in str(error.value)
