@@ -117,6 +117,12 @@ __device__ __forceinline__ void four_codes(uint32_t codes, uint32_t& low, uint32
     asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(low), "=r"(high) : "r"(codes));
 }
 __device__ __forceinline__ float power_of_two(int n) { return __uint_as_float(static_cast<uint32_t>(n + 127) << 23); }   // -126 to 127
+// ln(2^reference * sum). The V scales stand in both, against each other: the powers of two meet first, as exact differences.
+__device__ __forceinline__ float log_of_sum(float reference, float sum) {
+    const uint32_t bits = __float_as_uint(sum);
+    if (bits - 0x00800000u >= 0x7f000000u) return kLn2 * reference + logf(sum);   // (not a normal number above zero)
+    return fmaf(kLn2, reference + static_cast<float>(static_cast<int>(bits >> 23) - 127), logf(__uint_as_float((bits & 0x007fffffu) | 0x3f800000u)));
+}
 __device__ __forceinline__ float value_of(__half v) { return __half2float(v); }
 __device__ __forceinline__ float value_of(__nv_bfloat16 v) { return __bfloat162float(v); }
 
@@ -542,7 +548,7 @@ cache_sdpa_umma_kernel(const __grid_constant__ CachePrefillArgs args) {
                 }
             }
             if (there && healthy && a.stats)
-                a.stats[batch * a.stats_stride[0] + head_q * a.stats_stride[1] + token * a.stats_stride[2]] = none ? -INFINITY : kLn2 * (r - kUp) + logf(sum);
+                a.stats[batch * a.stats_stride[0] + head_q * a.stats_stride[1] + token * a.stats_stride[2]] = none ? -INFINITY : log_of_sum(r - kUp, sum);
         }
         tc_fence_before();
     }
@@ -588,7 +594,7 @@ cache_sdpa_pieces_kernel(const __grid_constant__ CachePrefillArgs args) {
     const int64_t at = batch * a.o_stride[0] + head * a.o_stride[1] + token * a.o_stride[2] + lane * kOwn;
 #pragma unroll
     for (int e = 0; e < kOwn; ++e) store_from_f32(a.o, a.o_type, at + e, none ? 0.0f : value[e] / total);
-    if (lane == 0 && a.stats) a.stats[batch * a.stats_stride[0] + head * a.stats_stride[1] + token * a.stats_stride[2]] = none ? -INFINITY : kLn2 * (top - kUp) + logf(total);
+    if (lane == 0 && a.stats) a.stats[batch * a.stats_stride[0] + head * a.stats_stride[1] + token * a.stats_stride[2]] = none ? -INFINITY : log_of_sum(top - kUp, total);
 }
 
 }  // namespace

@@ -127,6 +127,16 @@ def test_pieces_of_scales_far_apart_on_tcgen05(first, second):
         assert info.launches == 4
 
 
+@pytest.mark.parametrize("code", [47, 73, 92, 160, 200, 238])
+@pytest.mark.parametrize("lengths", [[1, 1, 2, 1, 3, 1, 1, 2], [2100, 1900]])
+def test_stats_under_v_scales_far_from_one_on_tcgen05(code, lengths):
+    """Stats have nothing to do with V's scales, and no digit is lost to them."""
+    def spoil(q, caches, scales, tables):
+        scales[1][:] = code
+    for seed in range(4):
+        attend_case(seed, BF16, 64, 3, 4, 64, 64, 16, lengths, spoil=spoil, right=0, bottom_right=True, kernel=UMMA)
+
+
 # ---- lists and counts that contradict themselves
 
 @pytest.mark.parametrize("in_place", [False, True])
