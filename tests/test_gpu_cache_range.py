@@ -3,9 +3,9 @@ import numpy as np
 import pytest
 
 import cache_reference as ref
-from deepforge_b200 import cache
+from deepforge_b200 import cache, dfgpu
 from deepforge_b200.dfgpu import BF16, F16, F32, I32, U8, tensor
-from test_gpu_cache import UMMA, attend_case, ints, pages_state, run_pages
+from test_gpu_cache import UMMA, attend_case, cache_of, ints, pages_state, randn, run_attend, run_pages, table_of
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -167,3 +167,29 @@ def test_copy_takes_the_last_entry_of_a_target_alone(entries, pairs, refused):
     for source, target in pairs:
         want[:, target] = state.pools[0][:, source]
     assert np.array_equal(pools[0], want) and report == [3, len(pairs), len(pairs), refused]
+
+
+# ---- calls beside one another
+
+@pytest.mark.parametrize("kernel,sq", [(cache.SDPA_STREAM, 1), (UMMA, 40)])
+def test_two_streams_at_once(kernel, sq):
+    """Each with scratch of its own; what one computes does not depend on the other."""
+    rng = np.random.default_rng(5)
+    calls = []
+    for i in range(2):
+        caches, scales = zip(*(cache_of(rng, 300, 4, 64, 16, 128) for _ in range(2)))
+        table = torch.from_numpy(table_of(rng, 4, 48, 300)).cuda()
+        calls.append((randn(rng, (4, 16, sq, 128), BF16), caches, scales, (table, table), ints(rng.integers(sq, 48 * 64, 4))))
+    want = [run_attend(*call, kernel=kernel, attn_scale=2.0 ** -10, right=0, bottom_right=True) for call in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    scratch = [torch.empty(info.scratch_bytes, device="cuda", dtype=torch.uint8) for _, _, info in want]
+    outs = [[torch.full_like(o, 77.0) for _ in range(30)] for o, _, _ in want]
+    torch.cuda.synchronize()
+    for turn in range(30):
+        for i, call in enumerate(calls):
+            run_attend(*call, kernel=kernel, attn_scale=2.0 ** -10, right=0, bottom_right=True, stream=streams[i].cuda_stream, o=outs[i][turn], stats=False, scratch=scratch[i])
+    torch.cuda.synchronize()
+    assert dfgpu.device_status() == 0
+    for (o, _, _), made in zip(want, outs):
+        assert bool(torch.isfinite(o).all()) and all(torch.equal(o, x) for x in made)
