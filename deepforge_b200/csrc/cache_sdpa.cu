@@ -635,6 +635,9 @@ cache_sdpa_merge_kernel(const __grid_constant__ CacheSdpaArgs a) {
     int lo, hi;
     const int units = units_of(a, entry, lo, hi);
     const bool takes_part = token < sequence_window(a, batch).len_q;
+    // A part has its own O, which counts by its sum. Sums are at most 2^15 for each key: taken by a power of two above them all, no sum of values passes the largest of V.
+    const int keys_log2 = 32 - __clz(units * kUnit);
+    const float share = power_of_two(-15 - keys_log2);
     float top = -INFINITY, total = 0.0f, value[kOwn];
 #pragma unroll
     for (int e = 0; e < kOwn; ++e) value[e] = 0.0f;
@@ -661,25 +664,19 @@ cache_sdpa_merge_kernel(const __grid_constant__ CacheSdpaArgs a) {
 #pragma unroll
             for (int k = 0; k < kAhead; ++k)
                 if (i0 + k * kWarpsHere < parts) largest = fmaxf(largest, pair[k].x);
-            // A part has the mean of its values, a weight its share of the sum so far: no sum of values that could pass f32's range.
-            float weight[kAhead], sum = total * (top == -INFINITY ? 1.0f : exp2_of(top - largest));   // (no score above -inf: zeros, or NaNs that are to be seen)
-            const float before = sum;
+            const float down = top == -INFINITY ? 1.0f : exp2_of(top - largest);   // (no score above -inf: zeros, or NaNs that are to be seen)
+            total *= down;
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) {
-                weight[k] = i0 + k * kWarpsHere < parts ? pair[k].y * (pair[k].x == -INFINITY ? 1.0f : exp2_of(pair[k].x - largest)) : 0.0f;
-                sum += weight[k];
-            }
-            const float inverse = sum == 0.0f ? 1.0f : 1.0f / sum, keep = before * inverse;
-#pragma unroll
-            for (int e = 0; e < kOwn; ++e) value[e] *= keep;
+            for (int e = 0; e < kOwn; ++e) value[e] *= down;
+            top = largest;
 #pragma unroll
             for (int k = 0; k < kAhead; ++k) {
                 if (i0 + k * kWarpsHere >= parts) continue;
-                const float share = weight[k] * inverse;
+                const float weight = pair[k].y * share * (pair[k].x == -INFINITY ? 1.0f : exp2_of(pair[k].x - largest));
+                total += weight;
 #pragma unroll
-                for (int e = 0; e < kOwn; ++e) value[e] = fmaf(ahead[k][e], share, value[e]);
+                for (int e = 0; e < kOwn; ++e) value[e] = fmaf(ahead[k][e], weight, value[e]);
             }
-            top = largest, total = sum;
         }
     }
     if (lane == 0) meeting[warp] = make_float2(top, total);
@@ -690,18 +687,15 @@ cache_sdpa_merge_kernel(const __grid_constant__ CacheSdpaArgs a) {
     top = -INFINITY, total = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWarpsHere; ++w) top = fmaxf(top, meeting[w].x);
-    float weight[kWarpsHere];
 #pragma unroll
     for (int w = 0; w < kWarpsHere; ++w) {
-        weight[w] = meeting[w].y * (meeting[w].x == -INFINITY ? 1.0f : exp2_of(meeting[w].x - top));
-        total += weight[w];
+        const float weight = meeting[w].x == -INFINITY ? 1.0f : exp2_of(meeting[w].x - top);
+        total = fmaf(meeting[w].y, weight, total);
+        result = fmaf(values[w][threadIdx.x], weight, result);
     }
-    const float inverse = 1.0f / total;
-#pragma unroll
-    for (int w = 0; w < kWarpsHere; ++w) result = fmaf(values[w][threadIdx.x], weight[w] * inverse, result);
     const bool none = !takes_part || total == 0.0f;
-    store_from_f32(a.o, a.o_type, batch * a.o_stride[0] + head * a.o_stride[1] + token * a.o_stride[2] + threadIdx.x, none ? 0.0f : result);
-    if (threadIdx.x == 0 && a.stats) a.stats[batch * a.stats_stride[0] + head * a.stats_stride[1] + token * a.stats_stride[2]] = none ? -INFINITY : top * kLn2 + logf(total * 0x1p-15f);
+    store_from_f32(a.o, a.o_type, batch * a.o_stride[0] + head * a.o_stride[1] + token * a.o_stride[2] + threadIdx.x, none ? 0.0f : result / total);
+    if (threadIdx.x == 0 && a.stats) a.stats[batch * a.stats_stride[0] + head * a.stats_stride[1] + token * a.stats_stride[2]] = none ? -INFINITY : top * kLn2 + logf(total * power_of_two(keys_log2));
 }
 
 struct StreamPlan {

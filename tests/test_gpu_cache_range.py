@@ -95,6 +95,21 @@ def test_values_far_above_one(d, code):
         attend_case(d, BF16, d, 2, 4, 64, 64, 64, [200, 130], spoil=large_values(code), right=0, bottom_right=True, kernel=UMMA)
 
 
+@pytest.mark.parametrize("code", [1, 20])
+def test_values_far_below_one(code):
+    """V of 2^-117 and 2^-98, all alike: O is that, to the weights' rounding (2^-11) and, of the smallest, f32's last digits below its normal range (2^-18)."""
+    rng = np.random.default_rng(code)
+    for d, lengths, hk in ((128, [16000], 1), (64, [60] * 512, 8), (256, [3000, 700], 2)):
+        slots = -(-max(lengths) // 64)
+        caches, scales = zip(*(cache_of(rng, len(lengths) * slots, hk, 64, 64, d) for _ in range(2)))
+        caches[1][:], scales[1][:] = 0x7E, code
+        table = torch.from_numpy(table_of(rng, len(lengths), slots, len(lengths) * slots)).cuda()
+        q = randn(rng, (len(lengths), hk * 2, 1, d), BF16)
+        o, _, _ = run_attend(q, caches, scales, (table, table), ints(lengths), o_type=F32, attn_scale=d ** -0.5 / 64)
+        off = (o.double() / (448.0 * 2.0 ** (code - 127)) - 1.0).abs().max().item()
+        assert off <= 2.0 ** -11 * 1.01 + 2.0 ** -16, off
+
+
 def test_absent_pages_beside_small_scales_on_tcgen05():
     """Keys whose V page is none count in the sum alone, however small the scales beside them."""
     def spoil(q, caches, scales, tables):
