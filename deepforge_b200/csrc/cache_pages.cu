@@ -400,7 +400,6 @@ struct CopyArgs {
     const int32_t* header;
     const int2* copies;
     int32_t pools, per_copy;
-    FastDivisor by_copy;
 };
 
 template <typename T>
