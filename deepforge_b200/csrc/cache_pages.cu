@@ -7,8 +7,10 @@
 // order, repeated entries from atomic minima and maxima of list positions, reference counts from integer sums: nothing depends on
 // the order in which threads run. Contents move in a second launch (two bytes over HBM for each byte of a page), over
 // a list of (source, target) pages that the first one leaves in the scratch memory; no page is both.
-// Reserving for 256 sequences among 40000 pages 8.0 us; 32 forks of 64 sequences, 8.6 MB copied, 13.4 us (three more barriers: 15.7); compacting 8192 pages, 337 MB
-// moved, 65 us, of which the copy's 53 run at 6.4 TB/s, 98 % of the copy rate.
+// Reserving for 256 sequences among 40000 pages 8.1 us; 32 forks of 64 sequences, 8.6 MB copied, 13.5 us (three more barriers: 15.7; without the one at the
+// beginning, which orders the first writes into other CTAs' shared memory, 13.3); compacting 8192 pages, 337 MB moved, 65.6 us, of which the copy's 53 run at
+// 6.4 TB/s, 98 % of the copy rate. With the L2 flushed before every four calls: freeing 32 of 64 sequences among 8192 pages 10.2 us, 128 of 256 among 70000 pages
+// 16.4; copying 544 pages of 131 KB 37 us (143 MB: 3.8 TB/s), 4192 pages of 8 KB 30 us.
 #include <algorithm>
 
 #include "common.cuh"

@@ -23,8 +23,8 @@
 // whose warps shared each list's units spent a third of their time on meeting and on beginning lists; a loading warp for four
 // others was what they waited for.) Lists that were cut leave partial results, which a second kernel merges. Rows beyond 16 (8) are
 // lists of their own, whose keys come from L2.
-// 64 sequences of 512 to 8192 keys, 8 KV heads of 128 channels, 4 query heads each: 122 us, 4.7 TB/s, 71 % of the copy rate (110 without the arithmetic); two
-// such sequences: 19 us, of which 15 are look-ups, launches and the merge. More rows: at the choice of a form below.
+// 64 sequences of 512 to 8192 keys, 8 KV heads of 128 channels, 4 query heads each: 122 us, 4.7 TB/s, 71 % of the copy rate (110 without the arithmetic; as long
+// with the pages in order as with pages anywhere); two such sequences: 19 us, of which 15 are look-ups, launches and the merge. More rows: at the choice of a form below.
 #include <algorithm>
 #include <cmath>
 

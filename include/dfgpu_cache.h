@@ -2,8 +2,9 @@
  * dfgpu_cache -- C ABI of the operators around a paged key/value cache in 8 bits: rotary positions, writing new tokens into the
  * cache, attention over it, and the bookkeeping of its pages. Part of libdfgpu.so; types, status codes, dfgpu_last_error()
  * and the shape of every launcher are those of dfgpu.h (device pointers in port order, caller-owned scratch, no allocation and
- * no synchronisation inside a launcher, launches capture into CUDA graphs). The reference has no counterpart of these: it reads
- * paged K/V containers (SDPA) but neither writes nor quantises nor moves them.
+ * no synchronisation inside a launcher, launches capture into CUDA graphs). They are calls beside the graph:
+ * the importer refuses graphs with the reference's own rotary nodes (ROPE, ROPE_BWD; lib/Compiler/SequenceGraph.cpp) and its PAGED_CACHE_LOAD
+ * as before. Writing to a paged cache, holding it in 8 bits and moving its pages have no counterpart there.
  *
  * The cache. K and V are containers [pages, Hk, T, D] of FP8_E4M3 codes, T tokens a page, as the SDPA node's paged containers
  * are, and each has a tensor of FP8_E8M0 scales [pages, Hk, T / t, 1]: one power of two for every t consecutive tokens of a page
@@ -48,12 +49,12 @@ int dfgpu_rope(const dfgpu_rope_params*, void* const* tensors, void* scratch, vo
 /* Fills HOST memory frequencies[rotary / 2] with base^(-2i / rotary), scaled for contexts `factor` times as long as the
    `original` one, in 64 bits and rounded once; *magnitude receives the factor for dfgpu_rope_params.scale (may be null).
      NONE    as they are; magnitude 1
-     LINEAR  all divided by factor
-     BASE    the base becomes base * factor^(rotary / (rotary - 2)): the last pair's frequency is divided by factor, the first's kept
-     RAMP    a pair that makes more than `high` turns over the original length is kept, one that makes fewer than `low` is divided
-             by factor, and between the pair numbers at which that is so (rounded outwards, within [0, R - 1]) a linear ramp blends the two;
-             magnitude 0.1 ln(factor) + 1
-     BANDS   the same borders with a blend linear in the number of turns; magnitude 1 */
+     LINEAR  all divided by factor (position interpolation)
+     BASE    ("NTK-aware") the base becomes base * factor^(rotary / (rotary - 2)): the last pair's frequency is divided by factor, the first's kept
+     RAMP    ("NTK by parts", YaRN) a pair that makes more than `high` turns over the original length is kept, one that makes fewer than `low` is divided
+             by factor, and between the pair numbers at which that is so (rounded outwards, within [0, R - 1], a step of 0.001 where they
+             meet: that method's conventions, which its users' frequencies follow) a linear ramp blends the two; magnitude 0.1 ln(factor) + 1
+     BANDS   the same borders with a blend linear in the number of turns (bands of wavelengths); magnitude 1 */
 enum { DFGPU_ROPE_SCALING_NONE = 0, DFGPU_ROPE_SCALING_LINEAR = 1, DFGPU_ROPE_SCALING_BASE = 2, DFGPU_ROPE_SCALING_RAMP = 3, DFGPU_ROPE_SCALING_BANDS = 4 };
 typedef struct dfgpu_rope_scaling {
     int32_t kind;
@@ -92,8 +93,8 @@ int dfgpu_cache_append(const dfgpu_cache_append_params*, void* const* tensors, v
    shift = bottom_right ? SEQ_LEN_KV - SEQ_LEN_Q : 0, kv <= q + shift + right_bound (with has_right_bound) and
    kv > q + shift - left_bound (with has_left_bound). Query rows from SEQ_LEN_Q on, and rows without keys, give O = 0 and
    Stats = -inf. A key whose page id is out of range reads as zeros, as in SDPA. Products take the codes as they are
-   (exact in f16), scales and everything else are f32; the probabilities that weight V are rounded to f16, and Q is
-   taken to within 2^-39 of its row's largest magnitude. A code or scale of a masked key, NaN or not, has no effect. Values under a V scale more than 2^80 below
+   (exact in f16), scales and everything else are f32; the probabilities that weight V are rounded to f16 (2^-11 of each, 2^-36 of
+   the row's largest where that is more), and Q is taken to within 2^-39 of its row's largest magnitude. A code or scale of a masked key, NaN or not, has no effect. Values under a V scale more than 2^80 below
    that of an earlier key of the sequence count as zeros.
    tensors: {Q, K container, V container, O, Stats or null, K scale, V scale, SEQ_LEN_Q or null, SEQ_LEN_KV, Page_table_K,
    Page_table_V}. Q, O [B, Hq, Sq, D] HALF or BFLOAT16, the same type (O may be FLOAT); D contiguous, 64, 128 or 256; Hq a
