@@ -452,7 +452,7 @@ cache_sdpa_umma_kernel(const __grid_constant__ CachePrefillArgs args) {
             }
             const bool raise = top > r + kRaise || (r == -INFINITY && top > -INFINITY);
             if (__any_sync(0xffffffffu, raise)) {
-                const float next = raise ? top : r, down = raise ? exp2_of(r - next) : 1.0f;
+                const float next = raise ? rintf(top) : r, down = raise ? exp2_of(r - next) : 1.0f;   // (whole numbers: r - kUp and the difference of two are exact)
                 r = next;
                 sum *= down;
                 if (h > 0) {   // (S of this half came behind the products with V of all halves but the last)

@@ -152,6 +152,19 @@ def test_stats_under_v_scales_far_from_one_on_tcgen05(code, lengths):
         attend_case(seed, BF16, 64, 3, 4, 64, 64, 16, lengths, spoil=spoil, right=0, bottom_right=True, kernel=UMMA)
 
 
+@pytest.mark.parametrize("near,far", [(66, 74), (200, 206), (50, 60)])
+def test_stats_over_pieces_under_v_scales_that_differ_on_tcgen05(near, far):
+    """Few keys, the last ones in a piece of their own: where the references of two pieces are far from zero, their difference is exact."""
+    for behind in (4, 8, 14):
+        def spoil(q, caches, scales, tables):
+            scales[0][:] = 114
+            scales[1][:] = far
+            scales[1][tables[1][0, 5248 // 32:].long()] = near
+        for seed in range(8):
+            _, _, info = attend_case(seed, BF16, 128, 1, 4, 33, 32, 16, [5248 + behind], spoil=spoil, left=10, bottom_right=True, kernel=UMMA)
+        assert info.launches == 4
+
+
 # ---- lists and counts that contradict themselves
 
 @pytest.mark.parametrize("in_place", [False, True])
