@@ -18,9 +18,9 @@
 // once otherwise): a NaN among V codes of a tile that some rows do not see all of (their zero probability times it is NaN), a V
 // scale of 2^126 or more, a scale that is a NaN, V scales more than 2^16
 // apart or below 2^-80 over codes that are not zero, V scales above 2^16 beside zeros under the least one or pages that are none, scores beyond 2^10.
-// 1000 tokens behind 3000 and 16000 keys, 8 KV heads of 128 channels, 4 query heads each: 440 to 446 us, 670 TFLOP/s, 41 % of the bf16 rate. Under the profiler this
-// kernel takes 403, its tensor pipe busy 37 % of that, and the streaming form's two kernels, which find nothing to do, 7 and 72 (the merge has a CTA a row; for one
-// sequence of 2000 tokens with 128 query heads over 8 KV heads 340, 14 and 397). A pair of score tiles every 5000 clocks, where the products take 2048. Without the exponentials 443 of 457 us then: the chain of a half's scores, maxima,
+// 1000 tokens behind 3000 and 16000 keys, 8 KV heads of 128 channels, 4 query heads each: 435 us, 678 TFLOP/s, 41 % of the bf16 rate. Under the profiler this
+// kernel takes 393, its tensor pipe busy 38 % of that, and the streaming form's two kernels, which find nothing to do, 7 and 72 (the merge has a CTA a row; for one
+// sequence of 2000 tokens with 128 query heads over 8 KV heads 332, 14 and 397). A pair of score tiles every 5000 clocks, where the products take 2048. Without the exponentials 443 of 457 us then: the chain of a half's scores, maxima,
 // exponentials and store, on two warps a scheduler, and the last items' end (148 of 128 tiles' time on 148 SMs).
 // Polynomial exponentials on the FMA pipe, one in two to one in four: 463 to 479 us for 457.
 #include <algorithm>
