@@ -18,7 +18,7 @@
 // once otherwise): a NaN among V codes of a tile that some rows do not see all of (their zero probability times it is NaN), a V
 // scale of 2^126 or more, a scale that is a NaN, V scales more than 2^16
 // apart or below 2^-80 over codes that are not zero, V scales above 2^16 beside zeros under the least one or pages that are none, scores beyond 2^10.
-// 1000 tokens behind 3000 and 16000 keys, 8 KV heads of 128 channels, 4 query heads each: 435 us, 678 TFLOP/s, 41 % of the bf16 rate. Under the profiler this
+// 1000 tokens behind 3000 and 16000 keys, 8 KV heads of 128 channels, 4 query heads each: 438 us, 674 TFLOP/s, 41 % of the bf16 rate. Under the profiler this
 // kernel takes 393, its tensor pipe busy 38 % of that, and the streaming form's two kernels, which find nothing to do, 7 and 72 (the merge has a CTA a row; for one
 // sequence of 2000 tokens with 128 query heads over 8 KV heads 332, 14 and 397). A pair of score tiles every 5000 clocks, where the products take 2048. Without the exponentials 443 of 457 us then: the chain of a half's scores, maxima,
 // exponentials and store, on two warps a scheduler, and the last items' end (148 of 128 tiles' time on 148 SMs).
@@ -452,7 +452,9 @@ cache_sdpa_umma_kernel(const __grid_constant__ CachePrefillArgs args) {
             }
             const bool raise = top > r + kRaise || (r == -INFINITY && top > -INFINITY);
             if (__any_sync(0xffffffffu, raise)) {
-                const float next = raise ? rintf(top) : r, down = raise ? exp2_of(r - next) : 1.0f;   // (whole numbers: r - kUp and the difference of two are exact)
+                // (To 2^-13: r - kUp and the difference of two are exact up to kMostReference, and the largest weight's f16 is off by 2^-14, as next to exact as before. Of
+                // whole numbers it was off by up to 2^-12: errors of 2.9e-4 instead of 2.5e-4 with HALF outputs.)
+                const float next = raise ? rintf(top * 0x1p13f) * 0x1p-13f : r, down = raise ? exp2_of(r - next) : 1.0f;
                 r = next;
                 sum *= down;
                 if (h > 0) {   // (S of this half came behind the products with V of all halves but the last)
