@@ -19,7 +19,7 @@ constexpr int kMaxStages = 16;
 constexpr int kMaxSteps = DFGPU_MAX_EPILOGUE;
 constexpr int kSmemBudget = 227 * 1024 - 1024;   // (1 KB of slack aligns the tiles)
 
-enum Kind { kSixteen = 0, kCodes = 1, kScaled = 2, kPieces = 3, kSummed = 4, kScaledSummed = 5, kCodesSummed = 6, kPiecesSummed = 7 };
+enum Kind { kSixteen = 0, kCodes = 1, kScaled = 2, kPieces = 3, kSummed = 4, kScaledSummed = 5, kCodesSummed = 6, kPiecesSummed = 7, kIntegers = 8 };
 
 // One product as the kernel sees it; the descriptors alone decide everything but the pointers.
 struct Problem {
@@ -82,7 +82,7 @@ inline Shape choose_shape(const Problem& p, int operands) {
     const int64_t blocks = (p.K * p.in_bytes + kRowBytes - 1) / kRowBytes;
     constexpr int clusters_at_once[9] = {0, 148, 74, 45, 33, 26, 22, 15, 15};   // (cudaOccupancyMaxActiveClusters, by CTAs per cluster)
     const int sms = 148;   // (a function of the shape alone: the count this library is built for)
-    const bool former_only = p.out_dtype == DFGPU_F32 || has_pieces(p), both = p.kind == kCodes && !former_only;
+    const bool former_only = (p.out_dtype == DFGPU_F32 && p.kind != kIntegers) || has_pieces(p), both = p.kind == kCodes && !former_only;
     Shape best{0, 0, 0, 0, 0, 0, 0.0}, former_best = best, shapes[2 * 4 * 8];
     int count = 0;
     auto take = [](Shape& least, const Shape& shape) {

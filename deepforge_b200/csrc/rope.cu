@@ -2,8 +2,7 @@
 //
 // Bound by HBM: every value is read once and written once. The angles belong to a token, not to a head, so a CTA takes a few
 // tokens and a run of heads, works out the tokens' sines and cosines once into shared memory and turns all the heads' rows by them.
-// position * frequency passes 2^24 for far positions, where f32 has lost the angle: the product and its reduction to one turn are
-// made in f64 (one product, rint and difference a pair and token), the sine and cosine of what is left, within half a turn, in f32.
+// (turn_of() in rotary.cuh: reduced to one turn in f64.)
 // Next come the issue slots (two thirds taken): rows and units are stepped to, and a CTA's heads are of one pair of tensors (with the L2 flushed before
 // each pass 57.7 us for 60.4, the gradient below 22.9 for 25.6).
 // 2 x 8192 tokens, 32 + 8 heads of 128 bf16 channels: 56 to 59 us, 5.7 to 6.0 TB/s, 86 to 91 % of the copy rate; 3 x 1001 f32 tokens, 16 + 16 heads, half of each
@@ -13,6 +12,7 @@
 
 #include "common.cuh"
 #include "dfgpu_cache.h"
+#include "rotary.cuh"
 
 namespace dfgpu {
 namespace {
@@ -29,27 +29,12 @@ struct RopeSide {
 };
 struct RopeArgs {
     RopeSide side[2];
-    const void* positions;
-    const float* frequencies;
-    int64_t position_batch, position_token, frequency_stride;
-    int32_t positions_wide, seq, tiles, token_shift;   // a CTA's tokens: 1 << token_shift
+    Positions at;
+    int32_t seq, tiles, token_shift;   // a CTA's tokens: 1 << token_shift
     int32_t first_side, heads_per_cta, half, turning, units, pitch;   // first_side: runs of heads of the first pair of tensors; units of V pairs (half) or V channels (interleaved) a row; pitch: of a token in the table
     int32_t rows_on, units_on;                         // kRopeThreads units on: whole rows, and the units beyond
     FastDivisor by_units, by_tiles;
     float scale, sign;
-};
-
-__device__ __forceinline__ float widen(float v) { return v; }
-__device__ __forceinline__ float widen(__half v) { return __half2float(v); }
-__device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T> __device__ __forceinline__ T narrow(float v);
-template <> __device__ __forceinline__ float narrow<float>(float v) { return v; }
-template <> __device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-
-template <typename T, int V>
-struct alignas(sizeof(T) * V) Pack {
-    T v[V];
 };
 
 // One unit of a row: V pairs as two vectors (i and i + half), or with INTERLEAVED V channels as one (V = 1: one pair as two values).
@@ -116,13 +101,9 @@ rope_kernel(RopeArgs a) {
     for (int i = threadIdx.x; i < a.half << a.token_shift; i += kRopeThreads) {
         const int local = i & ((1 << a.token_shift) - 1), pair = i >> a.token_shift;
         if (token0 + local < a.seq) {
-            const int64_t at = batch_index * a.position_batch + (token0 + local) * a.position_token;
-            const int64_t position = a.positions_wide ? static_cast<const int64_t*>(a.positions)[at] : static_cast<int64_t>(static_cast<const int32_t*>(a.positions)[at]);
-            const double turns = static_cast<double>(position) * static_cast<double>(a.frequencies[pair * a.frequency_stride]) * 0.15915494309189533577;
-            float sine, cosine;
-            sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &sine, &cosine);
+            const float2 turn = turn_of(a.at, batch_index, token0 + local, pair);
             const int unit = pair / Unit::kPairs;
-            angles[local * a.pitch + (pair - unit * Unit::kPairs) * a.turning + unit] = make_float2(cosine * a.scale, sine * a.scale * a.sign);
+            angles[local * a.pitch + (pair - unit * Unit::kPairs) * a.turning + unit] = make_float2(turn.x * a.scale, turn.y * a.scale * a.sign);
         }
     }
     __syncthreads();
@@ -134,8 +115,6 @@ rope_kernel(RopeArgs a) {
         now = next;
     }
 }
-
-bool aligned(const void* pointer, int64_t bytes) { return (reinterpret_cast<uintptr_t>(pointer) & static_cast<uintptr_t>(bytes - 1)) == 0; }
 
 int check_side(const dfgpu_tensor& x, const dfgpu_tensor& y, const dfgpu_tensor& reference, const char* name) {
     if (!valid_tensor(x) || !valid_tensor(y) || x.rank != 4 || y.rank != 4) return fail(kInvalidShape, "ROPE: %s must have rank 4 and positive extents", name);
@@ -239,12 +218,8 @@ extern "C" int dfgpu_rope(const dfgpu_rope_params* p, void* const* tensors, void
         }
     }
     if (!aligned(tensors[2], p->positions.dtype == DFGPU_I64 ? 8 : 4) || !aligned(tensors[3], 4)) return fail(kInvalidArgument, "ROPE: positions or frequencies are not aligned to their type");
-    a.positions = tensors[2];
-    a.positions_wide = p->positions.dtype == DFGPU_I64;
-    a.position_batch = p->positions.dim[0] == 1 ? 0 : p->positions.stride[0];
-    a.position_token = p->positions.stride[2];
-    a.frequencies = static_cast<const float*>(tensors[3]);
-    a.frequency_stride = p->frequencies.stride[3];
+    a.at = Positions{tensors[2], static_cast<const float*>(tensors[3]), p->positions.dim[0] == 1 ? 0 : p->positions.stride[0], p->positions.stride[2], p->frequencies.stride[3],
+                     p->positions.dtype == DFGPU_I64};
     a.scale = p->scale;
     a.sign = p->inverse ? -1.0f : 1.0f;
     a.seq = static_cast<int>(p->x.dim[2]);

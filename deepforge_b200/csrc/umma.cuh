@@ -2,6 +2,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "dfgpu_decoder.h"
 
 namespace dfgpu {
 
@@ -101,6 +102,9 @@ int launch_matmul_umma(const dfgpu_matmul_params& p, void* const* tensors, int k
 bool matmul_fp8_umma_supported(const dfgpu_matmul_fp8_params& p);   // whole tiles: the kernel id's promise
 bool matmul_fp8_tiles_supported(const dfgpu_matmul_fp8_params& p);  // everything launch_matmul_fp8_umma() takes
 int launch_matmul_fp8_umma(const dfgpu_matmul_fp8_params& p, void* const* tensors, cudaStream_t stream);
+// MATMUL_INT8 of two matrices (rank 2): the scales of rows and columns and the bias applied in the epilogue.
+bool matmul_int8_umma_supported(const dfgpu_matmul_int8_params& p);
+int launch_matmul_int8_umma(const dfgpu_matmul_int8_params& p, void* const* tensors, cudaStream_t stream);
 int matmul_tiles_device_status(int* status);
 
 // SDPA forward on tcgen05 (bf16 or f16, head dimension 64 or 128, any lengths, causal and padding masks).

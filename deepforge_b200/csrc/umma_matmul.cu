@@ -79,6 +79,12 @@ struct TileArgs {
     // block scales: [M, K/32] and [K/32, N], one byte each
     const uint8_t* sfa;
     const uint8_t* sfb;
+    // kIntegers: value = sum * row_scale[row] * column_scale[column]; a step of 0 is one scale for all
+    const float* row_scale;
+    const float* column_scale;
+    int64_t row_step;
+    int64_t column_step;
+    int32_t column_vector;                // column_vector: 16-byte loads
     int64_t sfa_ld, sfb_ld;
     int32_t scale_blocks, sfa_words;  // K / 32; sfa rows are whole aligned words
 };
@@ -154,6 +160,8 @@ __device__ __forceinline__ void product(uint32_t d, uint64_t a, uint64_t b, uint
     if constexpr (sixteen && CG == 2) DFGPU_MMA("cta_group::2.kind::f16");
     if constexpr ((KIND == kCodes || KIND == kCodesSummed) && CG == 1) DFGPU_MMA("cta_group::1.kind::f8f6f4");
     if constexpr ((KIND == kCodes || KIND == kCodesSummed) && CG == 2) DFGPU_MMA("cta_group::2.kind::f8f6f4");
+    if constexpr (KIND == kIntegers && CG == 1) DFGPU_MMA("cta_group::1.kind::i8");
+    if constexpr (KIND == kIntegers && CG == 2) DFGPU_MMA("cta_group::2.kind::i8");
 #undef DFGPU_MMA
 #define DFGPU_MMA(FORM)                                                                                                   \
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma." FORM ".kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%5], [%6], p;\n\t}" \
@@ -255,6 +263,34 @@ __device__ __forceinline__ void add_operand(float (&v)[COUNT], const void* data,
 #pragma unroll
         for (int i = 0; i < BATCH; ++i) v[at + i] = __fadd_rn(v[at + i], x[i]);
     }
+}
+
+// kIntegers: the scales of COUNT neighbouring columns, all loads issued before the first use; columns past the last take any.
+template <int COUNT>
+__device__ __forceinline__ void load_column_scales(const TileArgs& args, float (&scale)[COUNT], int col0) {
+    const int live = args.n_total - col0;
+    if (args.column_vector && live >= COUNT) {
+#pragma unroll
+        for (int j = 0; j < COUNT / 4; ++j) {
+            const float4 q = reinterpret_cast<const float4*>(args.column_scale + col0)[j];
+            scale[4 * j] = q.x;
+            scale[4 * j + 1] = q.y;
+            scale[4 * j + 2] = q.z;
+            scale[4 * j + 3] = q.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < COUNT; ++i) scale[i] = i < live ? args.column_scale[static_cast<int64_t>(col0 + i) * args.column_step] : 0.0f;
+    }
+}
+__device__ __forceinline__ float row_scale_of(const TileArgs& args, int row, bool live) { return live ? args.row_scale[row * args.row_step] : 0.0f; }
+// The integers' f32, and the two products.
+template <int COUNT>
+__device__ __forceinline__ void scale_integers(float (&v)[COUNT], float row_scale, const float (&scale)[COUNT]) {
+    const uint64_t by_row = pack2(row_scale, row_scale);
+#pragma unroll
+    for (int e = 0; e < COUNT; e += 2)
+        unpack2(mul2(mul2(pack2(__int2float_rn(__float_as_int(v[e])), __int2float_rn(__float_as_int(v[e + 1]))), by_row), pack2(scale[e], scale[e + 1])), v[e], v[e + 1]);
 }
 
 struct Scalars {
@@ -366,6 +402,12 @@ template <bool CLUSTER>
 __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, int code) {
     if constexpr (CLUSTER) return mbar_wait_warp_cluster(bar, parity, code);
     else return mbar_wait_warp<true>(bar, parity, code);
+}
+
+// Partial sums of two CTAs: bits of integers where those are summed.
+template <int KIND>
+__device__ __forceinline__ float add_partial(float a, float b) {
+    return KIND == kIntegers ? __int_as_float(__float_as_int(a) + __float_as_int(b)) : __fadd_rn(a, b);
 }
 
 // kPieces: 32 columns of the products of the lower pieces onto those of the leading ones.
@@ -524,7 +566,7 @@ template <int KIND, int CG>
 __global__ void __launch_bounds__(thread_count<KIND>(), 1)
 umma_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const __grid_constant__ CUtensorMap map_c,
                    const __grid_constant__ TileArgs args) {
-    constexpr int kCode = KIND == kSixteen ? 0 : (KIND == kCodes || KIND == kCodesSummed ? 20 : (KIND == kScaled ? 40 : (kHasPieces<KIND> ? 60 : (KIND == kSummed ? 80 : 90))));
+    constexpr int kCode = KIND == kSixteen ? 0 : (KIND == kCodes || KIND == kCodesSummed ? 20 : (KIND == kScaled ? 40 : (kHasPieces<KIND> ? 60 : (KIND == kSummed ? 80 : (KIND == kIntegers ? 110 : 90)))));
     constexpr bool kSixteenBits = KIND == kSixteen || kHasPieces<KIND> || KIND == kSummed;
     constexpr int kPieceCount = kHasPieces<KIND> ? 3 : 1;
     constexpr bool kCodesOnly = KIND == kCodes || KIND == kCodesSummed;
@@ -734,6 +776,7 @@ umma_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
             int local = 0, status = 0;
             const bool ahead = (KIND == kSixteen || KIND == kPieces) && args.step_count > 0 && args.step_kind[0] != kStepRelu && args.step_dtype[0] != DFGPU_F32;
             uint32_t first_operand[16];
+            float columns_ahead[KIND == kIntegers ? 32 : 1], row_scale = 0.0f;
             for (int i = first_item; i < args.items; i += item_step, local += kInBlocks<KIND> ? 0 : 1) {
                 const int acc = local & args.acc_shift, use = local >> args.acc_shift;
                 const Item item = item_at(args, i);
@@ -742,6 +785,10 @@ umma_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                 // (the first operand of a part is loaded under the part before, of an item's first part under its products: waited for
                 // in its place it cost 700 clocks of every part's 2300)
                 if (ahead) load_ahead(args, first_operand, out_row, item.col0 + g * box_columns, row_live);
+                if constexpr (KIND == kIntegers) {
+                    row_scale = row_scale_of(args, out_row, row_live);
+                    load_column_scales<32>(args, columns_ahead, item.col0 + g * box_columns);
+                }
                 if constexpr (kInRegisters<KIND>) {
                     sum_blocks<CG>(sums, tmem_base + lane_base, args.acc_stride, item.width / 32, g, kb_end - kb_begin, local, acc_full(0), leader_bars + (acc_empty(0) - bar_base), lane, ok);
                 } else if constexpr (kInPlace<KIND>) {
@@ -790,6 +837,11 @@ umma_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
 #pragma unroll
                         for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(raw[e]);
                         const int col = col0 + part * 32;
+                        if constexpr (KIND == kIntegers) {
+                            scale_integers<32>(v, row_scale, columns_ahead);
+                            const bool same_box = part + 1 < box_columns / 32;
+                            if (same_box || b + 2 < boxes) load_column_scales<32>(args, columns_ahead, same_box ? col + 32 : item.col0 + (b + 2) * box_columns);
+                        }
                         if (ahead) {
                             uint32_t operand[16];
 #pragma unroll
@@ -922,7 +974,15 @@ umma_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                 load_words<4>(operand, static_cast<const uint16_t*>(args.step_data[0]) + (args.step_kind[0] == kStepBias ? 0 : (row0 + row_of(i)) * args.step_ld[0]) + col, args.n_total - col,
                               args.step_vector[0] != 0);
         };
+        float split_columns[4] = {}, split_row = 0.0f;
+        auto fetch_scales = [&](int i) {
+            const int col = column_of(i);
+            if (KIND != kIntegers || i >= count || col >= args.n_total) return;
+            load_column_scales<4>(args, split_columns, col);
+            split_row = row_scale_of(args, row0 + row_of(i), true);
+        };
         fetch(static_cast<int>(threadIdx.x));
+        fetch_scales(static_cast<int>(threadIdx.x));
         cluster_wait();
         const int status = ask_status();
         bool rare = false;
@@ -939,16 +999,18 @@ umma_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
 #pragma unroll
             for (int z = 1; z < kMost; ++z) {
                 if (z >= args.splits) break;
-                v[0] = __fadd_rn(v[0], part[z].x);
-                v[1] = __fadd_rn(v[1], part[z].y);
-                v[2] = __fadd_rn(v[2], part[z].z);
-                v[3] = __fadd_rn(v[3], part[z].w);
+                v[0] = add_partial<KIND>(v[0], part[z].x);
+                v[1] = add_partial<KIND>(v[1], part[z].y);
+                v[2] = add_partial<KIND>(v[2], part[z].z);
+                v[3] = add_partial<KIND>(v[3], part[z].w);
             }
             rare = rare || __float_as_uint(v[0]) == kRareSum;
+            if constexpr (KIND == kIntegers) scale_integers<4>(v, split_row, split_columns);
             if (ahead) apply_steps<kCodesOnly, 4, 4>(args, v, row0 + row, col, true, scalars, &operand);
             else apply_steps<kCodesOnly, 4, 4>(args, v, row0 + row, col, true, scalars);
             if (healthy_now(true, status)) store_four(args, v, row0 + row, col);
             fetch(i + static_cast<int>(blockDim.x));
+            fetch_scales(i + static_cast<int>(blockDim.x));
         }
         __syncwarp();
         cluster_arrive_behind_loads(rare);
@@ -1082,8 +1144,8 @@ int launch_problem(Problem p, TileArgs& args, const void* a, const void* b, void
     args.staging_offset = ring_bytes(args.stages, args.stage_bytes);   // (a split product parks its 128 x bn partial tile, at most 64 KB, in the ring)
     args.barrier_offset = args.staging_offset + staging;
     const int dynamic = args.barrier_offset + barriers + 1024;
-    // instruction descriptor: f32 accumulators (or E8M0 scales), the operand formats the caller has set, B's major, M (N is the item's)
-    args.idesc |= (scaled(p) ? 1u << 23 : 1u << 4) | (static_cast<uint32_t>(args.b_mn_major) << 16) |
+    // instruction descriptor: f32 accumulators (or E8M0 scales, or 32-bit integers), the operand formats the caller has set, B's major, M (N is the item's)
+    args.idesc |= (scaled(p) ? 1u << 23 : (p.kind == kIntegers ? 2u << 4 : 1u << 4)) | (static_cast<uint32_t>(args.b_mn_major) << 16) |
                   (static_cast<uint32_t>(kRows * shape.cg >> 4) << 24);
     const CUtensorMapDataType in_type = sixteen_bits(p) ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;   // (copied, never computed on)
     const uint32_t per_row = kRowBytes / p.in_bytes;
@@ -1101,6 +1163,7 @@ int launch_problem(Problem p, TileArgs& args, const void* a, const void* b, void
     const int64_t groups = shape.splits > 1 ? shape.tiles : std::min<int64_t>(shape.tiles, sm_count() / shape.cg);
     const int grid = static_cast<int>(groups * (shape.cg == 2 ? 2 : shape.splits));
     if (p.kind == kSixteen) return shape.cg == 2 ? launch_kernel<kSixteen, 2>(map_a, map_b, map_c, args, grid, dynamic, stream, what) : launch_kernel<kSixteen, 1>(map_a, map_b, map_c, args, grid, dynamic, stream, what);
+    if (p.kind == kIntegers) return shape.cg == 2 ? launch_kernel<kIntegers, 2>(map_a, map_b, map_c, args, grid, dynamic, stream, what) : launch_kernel<kIntegers, 1>(map_a, map_b, map_c, args, grid, dynamic, stream, what);
     if (p.kind == kCodesSummed) return shape.cg == 2 ? launch_kernel<kCodesSummed, 2>(map_a, map_b, map_c, args, grid, dynamic, stream, what) : launch_kernel<kCodesSummed, 1>(map_a, map_b, map_c, args, grid, dynamic, stream, what);
     if (p.kind == kCodes) return shape.cg == 2 ? launch_kernel<kCodes, 2>(map_a, map_b, map_c, args, grid, dynamic, stream, what) : launch_kernel<kCodes, 1>(map_a, map_b, map_c, args, grid, dynamic, stream, what);
     if (p.kind == kSummed) return shape.cg == 2 ? launch_kernel<kSummed, 2>(map_a, map_b, map_c, args, grid, dynamic, stream, what) : launch_kernel<kSummed, 1>(map_a, map_b, map_c, args, grid, dynamic, stream, what);
@@ -1277,6 +1340,37 @@ int launch_matmul_fp8_umma(const dfgpu_matmul_fp8_params& p, void* const* tensor
     args.descale_b = static_cast<const float*>(tensors[5]);
     args.scale_c = static_cast<const float*>(tensors[6]);
     return launch_problem(problem, args, tensors[0], tensors[1], tensors[2], stream, "MATMUL_FP8 (tcgen05)");
+}
+
+bool int8_problem(const dfgpu_matmul_int8_params& p, Problem& problem) {
+    if (p.c.rank != 2 || !describe(p.a, p.b, p.c, kIntegers, problem)) return false;
+    return !p.bias.rank || p.bias.stride[1] == 1 || p.bias.dim[1] == 1;
+}
+
+bool matmul_int8_umma_supported(const dfgpu_matmul_int8_params& p) {
+    Problem problem;
+    return int8_problem(p, problem);
+}
+
+int launch_matmul_int8_umma(const dfgpu_matmul_int8_params& p, void* const* tensors, cudaStream_t stream) {
+    Problem problem;
+    TileArgs args{};
+    if (!on16(tensors[0]) || !on16(tensors[1])) return fail(kInvalidArgument, "MATMUL_INT8: the tcgen05 kernel needs 16-byte aligned A and B");
+    if (!int8_problem(p, problem)) return fail(kUnsupported, "MATMUL_INT8: the tcgen05 kernel does not take these operands");
+    args.idesc = (1u << 7) | (1u << 10);   // signed bytes
+    args.row_scale = static_cast<const float*>(tensors[3]);
+    args.column_scale = static_cast<const float*>(tensors[4]);
+    args.row_step = p.a_scale.dim[0] == 1 ? 0 : p.a_scale.stride[0];
+    args.column_step = p.b_scale.dim[1] == 1 ? 0 : p.b_scale.stride[1];
+    args.column_vector = args.column_step == 1 && on16(args.column_scale) ? 1 : 0;
+    if (p.bias.rank) {
+        args.step_count = 1;
+        args.step_kind[0] = kStepBias;
+        args.step_data[0] = tensors[5];
+        args.step_dtype[0] = p.bias.dtype;
+        args.step_vector[0] = on16(tensors[5]) ? 1 : 0;
+    }
+    return launch_problem(problem, args, tensors[0], tensors[1], tensors[2], stream, "MATMUL_INT8 (tcgen05)");
 }
 
 int matmul_tiles_device_status(int* status) { return read_and_clear_device_status(status); }
