@@ -1,39 +1,46 @@
 // Beam search: the W best continuations of each batch entry over its beams and the vocabulary, and the states of the beams that go on.
 //
-// Selection, first kernel: the logits are read once, in chunks that a CTA holds in registers. Of 256 threads' largest values the W-th largest is a bound that W values
-// reach at least, and no more than W threads hold values that reach it: those few are sorted. (Equals are told apart by the number of
-// their 16-byte vector, so that this holds for constant rows too.) The exponentials are summed against the chunk's largest value, which is
-// known by then and counts as 1 exactly: the log-probability of a token that has nearly all of it is no rounding's leftover.
-// Second kernel: a CTA an entry. Each warp merges the lists of its beams' chunks, 32 lanes a list, and adds scores in 64 bits; one warp merges the beams.
+// Selection, first kernel: the logits are read once. A CTA takes a part of a row, each warp some blocks of 32 R vectors in a row with the next block on its way, and
+// sums exponentials against the largest value so far, which counts as 1 exactly: the log-probability of a token that has nearly all of it is no rounding's
+// leftover. Of the largest values of the CTA's lanes (32 of them, each over all warps) the W-th largest is a bound that W values reach at least, and hardly more than W lanes
+// of some warp: their vectors are looked through again (from the caches), and what reaches the bound is sorted, a lane an entry.
+// Second kernel: a CTA an entry, a warp a beam, which merges its parts' lists; scores are added in 64 bits, beams merged pair by pair.
 //
 // Reordering: a copy; HBM bounds it.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "common.cuh"
 #include "dfgpu_decoder.h"
 #include "ports.cuh"
 #include "rotary.cuh"
+#include "umma_ptx.cuh"
 
 namespace dfgpu {
 namespace {
 
-constexpr int kScanThreads = 256, kScanWarps = kScanThreads / 32;
+constexpr int kScanWarps = 16;
+constexpr int kCandidates = 64;   // of a CTA, that are sorted at once
 constexpr int kMaxBeams = 32;
 constexpr float kLog2e = 1.44269504088896341f;
 
-struct alignas(16) ChunkSum {
+struct alignas(16) PartSum {
     double sum;                // of exp(x - most)
     float most, unused;
 };
+struct Logits {
+    const void* data;
+    int64_t batch_stride, beam_stride;
+    int32_t beams, vocabulary, parts, blocks;   // parts of a row, blocks of a warp
+    PartSum* sums;                              // of a part
+    uint64_t* keys;                             // of a part: W, falling; 0: none
+};
 struct ScanArgs {
-    const void* logits;
+    Logits logits;
     const int32_t* finished;
-    ChunkSum* sums;            // of a chunk
-    uint64_t* keys;            // of a chunk: W, falling; 0: none
-    int64_t batch_stride, beam_stride, finished_batch, finished_beam;
-    int32_t beams, vocabulary, chunks;
-    FastDivisor by_chunks, by_beams;
+    int64_t finished_batch, finished_beam;
+    FastDivisor by_parts, by_beams;
 };
 
 // Floats as whole numbers in the same order (0 is below all of them).
@@ -46,6 +53,7 @@ __device__ __forceinline__ uint64_t ordered(double v) {
     const uint64_t bits = static_cast<uint64_t>(__double_as_longlong(v + 0.0));
     return bits ^ ((bits >> 63) ? ~0ull : 1ull << 63);
 }
+__device__ __forceinline__ double double_from_ordered(uint64_t o) { return __longlong_as_double(static_cast<long long>(o ^ ((o >> 63) ? 1ull << 63 : ~0ull))); }
 
 // An entry of a list: greater keys first, then lower places.
 struct Key {
@@ -100,17 +108,21 @@ __device__ __forceinline__ uint4 shifted(const uint4& lo, const uint4& hi, int s
     for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(w[k], w[k + 1], (shift & 2) * 8);
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
-// Vectors first, first + kScanThreads, ... of a row that starts `before` elements behind a 16-byte boundary; what lies past its end is -inf.
-// Nothing outside the row is read: vectors whose aligned halves are not all the row's come element by element.
+// Vectors first, first + 32, ... of a row that starts `before` elements behind a 16-byte boundary; what lies past its end is -inf.
+// Nothing outside the row is read (`first` is not negative): vectors whose aligned halves are not all the row's come element by element.
 template <typename T, int R>
 __device__ __forceinline__ void load_vectors(Pack<T, 16 / sizeof(T)> (&held)[R], const T* row, int first, int before, int length) {
     constexpr int VE = 16 / static_cast<int>(sizeof(T));
+    const int64_t last = static_cast<int64_t>(first + (R - 1) * 32 + 1) * VE;   // behind this lane's last vector
+    if (before == 0 && last <= length) {
+#pragma unroll
+        for (int j = 0; j < R; ++j) held[j] = *reinterpret_cast<const Pack<T, VE>*>(row + static_cast<int64_t>(first + j * 32) * VE);
+        return;
+    }
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-        const int64_t at = static_cast<int64_t>(first + j * kScanThreads) * VE;
-        if (before == 0 && at + VE <= length) {
-            held[j] = *reinterpret_cast<const Pack<T, VE>*>(row + at);
-        } else if (before != 0 && at > 0 && at + 2 * VE - before <= length) {
+        const int64_t at = static_cast<int64_t>(first + j * 32) * VE;
+        if (before != 0 && at > 0 && at + 2 * VE - before <= length) {
             const uint4* halves = reinterpret_cast<const uint4*>(row + at - before);
             *reinterpret_cast<uint4*>(&held[j]) = shifted(halves[0], halves[1], before * static_cast<int>(sizeof(T)));
         } else {
@@ -120,89 +132,223 @@ __device__ __forceinline__ void load_vectors(Pack<T, 16 / sizeof(T)> (&held)[R],
     }
 }
 
-// R vectors of 16 bytes a thread.
+// A key into a list in order, where it belongs; the last of 32 falls out.
+__device__ __forceinline__ void insert(Key& list, uint64_t key, int lane) {
+    const int place = __popc(__ballot_sync(0xffffffffu, list.key > key));
+    const uint64_t above = __shfl_up_sync(0xffffffffu, list.key, 1);
+    list.key = lane < place ? list.key : lane == place ? key : above;
+}
+
+// The largest of R vectors' values; a NaN is left out (the sum has it).
 template <typename T, int R>
-__global__ void __launch_bounds__(kScanThreads)
+__device__ __forceinline__ float largest_of(const Pack<T, 16 / sizeof(T)> (&v)[R]) {
+    if constexpr (sizeof(T) == 4) {
+        float most = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < R; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) most = fmaxf(most, v[j].v[i]);
+        return most;
+    } else {
+        using Two = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+        Two most = reinterpret_cast<const Two*>(&v[0])[0];
+#pragma unroll
+        for (int j = 0; j < R; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) most = __hmax2(most, reinterpret_cast<const Two*>(&v[j])[i]);
+        return fmaxf(fmaxf(widen(most.x), widen(most.y)), -INFINITY);
+    }
+}
+
+constexpr int kScanVectors = 4;   // of a lane and block
+template <typename T> constexpr int kVector = 16 / static_cast<int>(sizeof(T));
+// Vector `number` of a lane, counted from the row's beginning; `first`: the part's first.
+__device__ __forceinline__ int vector_at(int first, int number, int lane) { return first + (number / kScanVectors) * (32 * kScanVectors) + (number % kScanVectors) * 32 + lane; }
+
+// The lanes' values in falling order.
+__device__ __forceinline__ float in_order(float v, int lane) {
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+        for (int mask = size >> 1; mask > 0; mask >>= 1) {
+            const float other = __shfl_xor_sync(0xffffffffu, v, mask);
+            v = ((lane & size) == 0) == ((lane & mask) == 0) ? fmaxf(v, other) : fminf(v, other);
+        }
+    return v;
+}
+
+// A lane's vector of the row, and what it may add to a list: values above `least`, or equal to it and below `last_token`.
+template <typename T>
+struct Look {
+    uint4 words;
+    int vector;
+    __device__ __forceinline__ float value(int i) const {   // (`i` the same in all lanes, or known)
+        const int place = i * static_cast<int>(sizeof(T)) / 4;
+        const uint32_t word = place < 2 ? (place == 0 ? words.x : words.y) : (place == 2 ? words.z : words.w);
+        if constexpr (sizeof(T) == 4) {
+            return __uint_as_float(word);
+        } else {
+            const uint16_t half = static_cast<uint16_t>(i & 1 ? word >> 16 : word);
+            return widen(*reinterpret_cast<const T*>(&half));
+        }
+    }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(32 * kScanWarps, 2)
 beam_scan_kernel(const ScanArgs a) {
-    constexpr int VE = 16 / static_cast<int>(sizeof(T));
-    extern __shared__ uint64_t candidates[];            // W * R * VE
-    __shared__ uint64_t best[kScanWarps * kMaxBeams];   // the largest of each warp's threads
-    __shared__ uint64_t bound, top;
-    __shared__ double partial[kScanWarps];
+    constexpr int VE = kVector<T>, R = kScanVectors;
+    __shared__ float largest_of_warp[kScanWarps][32];
+    __shared__ double whole_of_warp[kScanWarps];
+    __shared__ float reference_of_warp[kScanWarps];
+    __shared__ uint64_t candidates[kCandidates];
     __shared__ int count;
-    const int row = static_cast<int>(fast_divide(blockIdx.x, a.by_chunks)), chunk = static_cast<int>(blockIdx.x) - row * a.chunks;
-    const int entry = static_cast<int>(fast_divide(static_cast<uint32_t>(row), a.by_beams)), beam = row - entry * a.beams;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const Logits& l = a.logits;
+    const int row = static_cast<int>(fast_divide(blockIdx.x, a.by_parts)), part = static_cast<int>(blockIdx.x) - row * l.parts;
+    const int entry = static_cast<int>(fast_divide(static_cast<uint32_t>(row), a.by_beams)), beam = row - entry * l.beams;
     if (threadIdx.x == 0) count = 0;
     chain_begin();
     if (a.finished && a.finished[entry * a.finished_batch + beam * a.finished_beam] != 0) return;
-    const T* logits = static_cast<const T*>(a.logits) + entry * a.batch_stride + beam * a.beam_stride;
-    // A thread's logits depend on their numbers alone, wherever the row starts, so that equal rows have equal sums.
+    const T* logits = static_cast<const T*>(l.data) + entry * l.batch_stride + beam * l.beam_stride;
+    // A lane's logits depend on their numbers alone, wherever the row starts, so that equal rows have equal sums.
     const int before = static_cast<int>((reinterpret_cast<uintptr_t>(logits) & 15u) / sizeof(T));
-    const int first_vector = chunk * (kScanThreads * R) + threadIdx.x;
-    Pack<T, VE> held[R];
-    float most[R], largest = -INFINITY;
-    load_vectors<T, R>(held, logits, first_vector, before, a.vocabulary);
+    const int of_lane = l.blocks * R, first_vector = (part * kScanWarps + warp) * of_lane * 32;
+    Pack<T, VE> held[R], next[R];
+    load_vectors<T, R>(held, logits, first_vector + lane, before, l.vocabulary);
+    float reference = 0.0f, largest = -INFINITY;   // reference: what exponentials are taken against, once there is `some` value
+    bool some = false;
+    uint64_t sums = 0;                             // of two halves, at most 64 terms each, before they go into `whole`
+    double whole = 0.0;
+    auto add_up = [&] {
+        float one, two;
+        unpack2(sums, one, two);
+        whole += static_cast<double>(one) + static_cast<double>(two);
+        sums = 0;
+    };
+#pragma unroll 1
+    for (int block = 0; block < l.blocks; ++block) {
+        if (block + 1 < l.blocks) load_vectors<T, R>(next, logits, first_vector + (block + 1) * (32 * R) + lane, before, l.vocabulary);
+        largest = fmaxf(largest, largest_of<T, R>(held));
+        if (__any_sync(0xffffffffu, largest > (some ? reference : -INFINITY))) {
+            const float top = from_ordered(__reduce_max_sync(0xffffffffu, ordered(largest)));
+            if (some) {
+                add_up();
+                whole *= static_cast<double>(power_of_two((reference - top) * kLog2e));
+            }
+            reference = top;
+            some = true;
+        }
+        const uint64_t away = pack2(-reference, -reference), by = pack2(kLog2e, kLog2e);
 #pragma unroll
-    for (int j = 0; j < R; ++j) {
-        most[j] = -INFINITY;
+        for (int j = 0; j < R; ++j)
 #pragma unroll
-        for (int i = 0; i < VE; ++i) most[j] = fmaxf(most[j], widen(held[j].v[i]));   // (a NaN is left out here; the sum has it)
-        largest = fmaxf(largest, most[j]);
+            for (int i = 0; i < VE; i += 2) {
+                float lo, hi;
+                unpack2(mul2(add2(pack2(widen(held[j].v[i]), widen(held[j].v[i + 1])), away), by), lo, hi);
+                sums = add2(sums, pack2(power_of_two(lo), power_of_two(hi)));
+            }
+        if ((block & 3) == 3) add_up();
+#pragma unroll
+        for (int j = 0; j < R; ++j) held[j] = next[j];
     }
-    int vector = 0;
-#pragma unroll
-    for (int j = R - 1; j >= 0; --j)
-        if (most[j] == largest) vector = first_vector + j * kScanThreads;
-    Key mine{static_cast<uint64_t>(ordered(largest)) << 32 | ~static_cast<uint32_t>(vector)};
-    sort_lanes(mine, lane);
-    if (lane < a.beams) best[warp * a.beams + lane] = mine.key;
-    __syncthreads();
-    for (int i = threadIdx.x; i < kScanWarps * a.beams; i += kScanThreads) {
-        const uint64_t own = best[i];
-        int rank = 0;
-        for (int o = 0; o < kScanWarps * a.beams; ++o) rank += best[o] > own ? 1 : 0;
-        if (rank == 0) top = own;
-        if (rank == a.beams - 1) bound = own;
+    add_up();
+    for (int o = 16; o > 0; o >>= 1) whole += __shfl_xor_sync(0xffffffffu, whole, o);
+    largest_of_warp[warp][lane] = largest;
+    if (lane == 0) {
+        whole_of_warp[warp] = whole;
+        reference_of_warp[warp] = some ? reference : -INFINITY;
     }
     __syncthreads();
-    const float least = from_ordered(static_cast<uint32_t>(bound >> 32)), most_of_all = from_ordered(static_cast<uint32_t>(top >> 32));
-    const uint32_t last_vector = ~static_cast<uint32_t>(bound);
-    const float reference = most_of_all == -INFINITY ? 0.0f : most_of_all;
-    float sum[2] = {0.0f, 0.0f};
+    float most = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < R; ++j) {
-#pragma unroll
-        for (int i = 0; i < VE; ++i) sum[i & 1] += power_of_two((widen(held[j].v[i]) - reference) * kLog2e);
-        if (most[j] >= least) {
-            const uint32_t number = static_cast<uint32_t>(first_vector + j * kScanThreads);
+    for (int w = 0; w < kScanWarps; ++w) most = fmaxf(most, largest_of_warp[w][lane]);
+    most = in_order(most, lane);
+    float least = __shfl_sync(0xffffffffu, most, l.beams - 1);
+    auto look = [&](int of_warp, int whose, int number) {
+        Pack<T, VE> own[1];
+        const bool there = number < of_lane;
+        const int vector = vector_at((part * kScanWarps + of_warp) * of_lane * 32, there ? number : 0, whose);
+        load_vectors<T, 1>(own, logits, vector, before, there ? l.vocabulary : 0);
+        return Look<T>{*reinterpret_cast<const uint4*>(&own[0]), there ? vector : -1};
+    };
+    // (Loops that are not unrolled: a warp comes by here once, and instructions that are run once are waited for.)
+#pragma unroll 1
+    for (uint32_t lanes = __ballot_sync(0xffffffffu, largest >= least); lanes != 0; lanes &= lanes - 1) {
+#pragma unroll 1
+        for (int from = 0; from < of_lane; from += 32) {
+            const Look<T> own = look(warp, __ffs(static_cast<int>(lanes)) - 1, from + lane);
+            if (own.vector < 0) continue;
+            const uint32_t token = static_cast<uint32_t>(own.vector) * VE;
 #pragma unroll
             for (int i = 0; i < VE; ++i) {
-                const float x = widen(held[j].v[i]);
-                const int64_t token = static_cast<int64_t>(number) * VE + i;
-                if ((x > least || (x == least && number <= last_vector)) && token < a.vocabulary)
-                    candidates[atomicAdd(&count, 1)] = static_cast<uint64_t>(ordered(x)) << 32 | ~static_cast<uint32_t>(token);   // (in any order: they are sorted)
+                const float x = own.value(i);
+                if (x >= least && token + i < static_cast<uint32_t>(l.vocabulary)) {
+                    const int at = atomicAdd(&count, 1);   // (in any order: they are sorted)
+                    if (at < kCandidates) candidates[at] = static_cast<uint64_t>(ordered(x)) << 32 | ~(token + i);
+                }
+            }
+        }
+        if (*static_cast<volatile int*>(&count) > kCandidates) break;
+    }
+    __syncthreads();
+    if (warp != 0) return;
+    Key list{0};
+    if (count <= kCandidates) {
+#pragma unroll 1
+        for (int from = 0; from < count; from += 32) {
+            Key more{from + lane < count ? candidates[from + lane] : 0};
+            sort_lanes(more, lane);
+            if (from == 0) list = more;
+            else merge_lanes(list, more, lane);
+        }
+    } else {
+        // Many equals: one after another. The list fills up with the lowest tokens, and vectors behind them are no candidates any more.
+        uint32_t last_token = 0xffffffffu;
+        uint64_t bound = static_cast<uint64_t>(ordered(least)) << 32;
+#pragma unroll 1
+        for (int w = 0; w < kScanWarps; ++w) {
+            const float value = largest_of_warp[w][lane];
+            const uint32_t first_token = static_cast<uint32_t>((part * kScanWarps + w) * of_lane * 32 + lane) * VE;
+#pragma unroll 1
+            for (uint32_t lanes = __ballot_sync(0xffffffffu, value > least || (value == least && first_token < last_token)); lanes != 0; lanes &= lanes - 1) {
+#pragma unroll 1
+                for (int from = 0; from < of_lane; from += 32) {
+                    const Look<T> own = look(w, __ffs(static_cast<int>(lanes)) - 1, from + lane);
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < VE; ++i) top = fmaxf(top, own.value(i));
+                    const bool reaches = own.vector >= 0 && (top > least || (top == least && static_cast<uint32_t>(own.vector) * VE < last_token));
+#pragma unroll 1
+                    for (uint32_t reaching = __ballot_sync(0xffffffffu, reaches); reaching != 0; reaching &= reaching - 1) {
+                        const int source = __ffs(static_cast<int>(reaching)) - 1;
+                        const uint32_t token = static_cast<uint32_t>(__shfl_sync(0xffffffffu, own.vector, source)) * VE;
+#pragma unroll 1
+                        for (int i = 0; i < VE; ++i) {
+                            const float x = __shfl_sync(0xffffffffu, own.value(i), source);
+                            const uint64_t key = static_cast<uint64_t>(ordered(x)) << 32 | ~(token + i);
+                            if (!(x >= least) || key <= bound || token + i >= static_cast<uint32_t>(l.vocabulary)) continue;
+                            insert(list, key, lane);
+                            const uint64_t last = list.from(l.beams - 1).key;
+                            if (last > bound) {
+                                bound = last;
+                                least = from_ordered(static_cast<uint32_t>(bound >> 32));
+                                last_token = ~static_cast<uint32_t>(bound);
+                            }
+                        }
+                    }
+                }
             }
         }
     }
-    double whole = static_cast<double>(sum[0]) + static_cast<double>(sum[1]);
-    for (int o = 16; o > 0; o >>= 1) whole += __shfl_xor_sync(0xffffffffu, whole, o);
-    if (lane == 0) partial[warp] = whole;
-    __syncthreads();
-    if (warp != 0) return;
-    const int found = count;
-    Key list{0};
-    for (int from = 0; from < found; from += 32) {
-        Key more{from + lane < found ? candidates[from + lane] : 0};
-        sort_lanes(more, lane);
-        merge_lanes(list, more, lane);
-    }
-    const int64_t at = blockIdx.x;
-    if (lane < a.beams) a.keys[at * a.beams + lane] = list.key;
-    if (lane == 0) {
-        for (int w = 1; w < kScanWarps; ++w) whole += partial[w];
-        a.sums[at] = ChunkSum{whole, reference, 0.0f};
-    }
+    if (lane < l.beams) l.keys[static_cast<int64_t>(blockIdx.x) * l.beams + lane] = list.key;
+    // the warps' sums against the CTA's largest value (a warp of -inf alone has no reference that means anything)
+    const float own_reference = lane < kScanWarps ? reference_of_warp[lane] : -INFINITY;
+    const float top = __shfl_sync(0xffffffffu, most, 0);
+    const double own_whole = lane < kScanWarps ? whole_of_warp[lane] : 0.0;
+    double sum = own_whole == 0.0 ? 0.0 : own_whole * (own_reference == top || own_reference == -INFINITY ? 1.0 : exp(static_cast<double>(own_reference) - static_cast<double>(top)));
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) l.sums[blockIdx.x] = PartSum{sum, top, 0.0f};
 }
 
 struct Ints {
@@ -211,100 +357,109 @@ struct Ints {
     __device__ __forceinline__ int32_t& at(int b, int w) const { return data[b * batch + w * beam]; }
 };
 struct MergeArgs {
-    const void* logits;
-    const ChunkSum* sums;
-    const uint64_t* keys;
-    int64_t batch_stride, beam_stride;
+    Logits logits;
     const float* scores;
     float* scores_out;
     int64_t scores_batch, scores_beam, out_batch, out_beam;
     Ints finished, lengths, tokens, parents, finished_out, lengths_out;
     int32_t* forks;
-    int32_t beams, vocabulary, chunks, logits_type, end, pad, source_base, target_base;
+    int32_t end, pad, source_base, target_base;
     float length_penalty;
 };
 
-__global__ void __launch_bounds__(kScanThreads)
+__global__ void __launch_bounds__(32 * kMaxBeams)
 beam_merge_kernel(const MergeArgs a) {
     __shared__ uint64_t keys[kMaxBeams][32];
     __shared__ uint32_t places[kMaxBeams][32];
-    __shared__ double normalisers[kMaxBeams];   // ln sum exp; NaN: all continuations at -inf
-    __shared__ float scores[kMaxBeams];
+    __shared__ double divisors[kMaxBeams];
     __shared__ int32_t finished[kMaxBeams], lengths[kMaxBeams];
-    const int entry = static_cast<int>(blockIdx.x), warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int entry = static_cast<int>(blockIdx.x), beam = threadIdx.x >> 5, lane = threadIdx.x & 31;   // (as many warps as beams)
+    const Logits& l = a.logits;
+    const int64_t first = (static_cast<int64_t>(entry) * l.beams + beam) * l.parts;
     chain_begin();
-    for (int beam = warp; beam < a.beams; beam += kScanWarps) {
-        const float score = a.scores[entry * a.scores_batch + beam * a.scores_beam];
-        const bool done = a.finished.data && a.finished.at(entry, beam) != 0;
-        int64_t length = a.lengths.data ? static_cast<int64_t>(a.lengths.at(entry, beam)) + (done ? 0 : 1) : 1;
+    // All that most rows need is on its way at once. (Of a finished beam it is whatever the scratch held.)
+    const float score = a.scores[entry * a.scores_batch + beam * a.scores_beam];
+    const bool done = a.finished.data && a.finished.at(entry, beam) != 0;
+    int64_t length = a.lengths.data ? static_cast<int64_t>(a.lengths.at(entry, beam)) + (done ? 0 : 1) : 1;
+    constexpr int kAhead = 4;
+    uint64_t ahead[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) ahead[i] = i < l.parts && lane < l.beams ? l.keys[(first + i) * l.beams + lane] : 0;
+    PartSum sums = lane < l.parts ? l.sums[first + lane] : PartSum{0.0, 0.0f, 0.0f};
+    Key list{ahead[0]};
+    if (!done) {
+#pragma unroll
+        for (int i = 1; i < kAhead; ++i)
+            if (i < l.parts && __shfl_sync(0xffffffffu, ahead[i], 0) > list.from(l.beams - 1).key) merge_lanes(list, Key{ahead[i]}, lane);
+        for (int from = kAhead; from < l.parts; from += 32) {
+            const uint64_t own = from + lane < l.parts ? l.keys[(first + from + lane) * l.beams] : 0;
+            for (uint32_t lists = __ballot_sync(0xffffffffu, own > list.from(l.beams - 1).key); lists != 0; lists &= lists - 1) {
+                const int i = __ffs(static_cast<int>(lists)) - 1;
+                if (__shfl_sync(0xffffffffu, own, i) <= list.from(l.beams - 1).key) continue;
+                merge_lanes(list, Key{lane < l.beams ? l.keys[(first + from + i) * l.beams + lane] : 0}, lane);
+            }
+        }
+    }
+    Place mine{0, 0xffffffffu};
+    {
         length = min(max(length, static_cast<int64_t>(1)), static_cast<int64_t>(0x7fffffff));
         const double divisor = a.lengths.data && a.length_penalty != 0.0f ? pow(static_cast<double>(length), static_cast<double>(a.length_penalty)) : 1.0;
         const bool alive = isfinite(score);
-        double normaliser = 0.0;
-        Place mine{0, 0xffffffffu};
-        const uint32_t row = static_cast<uint32_t>(beam) * static_cast<uint32_t>(a.vocabulary);
+        const uint32_t row = static_cast<uint32_t>(beam) * static_cast<uint32_t>(l.vocabulary);
         if (done) {
-            if (lane == 0) mine = Place{ordered(alive ? static_cast<double>(score) / divisor : -INFINITY), row + static_cast<uint32_t>(a.pad)};
+            if (lane == 0) mine = Place{ordered(alive ? static_cast<double>(score) / divisor : -static_cast<double>(INFINITY)), row + static_cast<uint32_t>(a.pad)};
         } else {
-            const int64_t first = (static_cast<int64_t>(entry) * a.beams + beam) * a.chunks;
-            float most = -INFINITY;
-            for (int i = lane; i < a.chunks; i += 32) {   // (a chunk of -inf alone has no largest value that means anything)
-                const ChunkSum part = a.sums[first + i];
-                if (part.sum != 0.0) most = fmaxf(most, part.most);
+            for (int from = 32; from < l.parts; from += 32) {   // a lane's parts against the largest of them
+                const PartSum more = from + lane < l.parts ? l.sums[first + from + lane] : PartSum{0.0, 0.0f, 0.0f};
+                if (more.sum == 0.0) continue;   // (of -inf alone: its reference means nothing)
+                const float top = sums.sum != 0.0 ? fmaxf(sums.most, more.most) : more.most;
+                sums.sum = (sums.sum != 0.0 ? sums.sum * exp(static_cast<double>(sums.most) - static_cast<double>(top)) : 0.0) + more.sum * exp(static_cast<double>(more.most) - static_cast<double>(top));
+                sums.most = top;
             }
+            float most = sums.sum != 0.0 ? sums.most : -INFINITY;
             for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-            double sum = 0.0;
-            for (int i = lane; i < a.chunks; i += 32) {
-                const ChunkSum part = a.sums[first + i];
-                if (part.sum != 0.0) sum += part.sum * exp(static_cast<double>(part.most) - static_cast<double>(most));
-            }
+            double sum = sums.sum != 0.0 ? sums.sum * (sums.most == most ? 1.0 : exp(static_cast<double>(sums.most) - static_cast<double>(most))) : 0.0;
             for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            normaliser = static_cast<double>(most) + log(sum);
-            if (!alive || !isfinite(normaliser)) normaliser = nan("");
-            Key list{0};
-            for (int i = 0; i < a.chunks; ++i) {
-                const Key more{lane < a.beams ? a.keys[(first + i) * a.beams + lane] : 0};
-                merge_lanes(list, more, lane);
-            }
-            if (normaliser != normaliser) {
-                if (lane < a.vocabulary) mine = Place{ordered(-static_cast<double>(INFINITY)), row + static_cast<uint32_t>(lane)};
+            const double normaliser = static_cast<double>(most) + log(sum);
+            if (!alive || !isfinite(normaliser)) {   // all continuations at -inf
+                if (lane < l.vocabulary) mine = Place{ordered(-static_cast<double>(INFINITY)), row + static_cast<uint32_t>(lane)};
             } else if (list.key != 0) {
                 const double logit = static_cast<double>(from_ordered(static_cast<uint32_t>(list.key >> 32)));
                 mine = Place{ordered((static_cast<double>(score) + (logit - normaliser)) / divisor), row + ~static_cast<uint32_t>(list.key)};
             }
-            if (lane >= a.beams) mine = Place{0, 0xffffffffu};
-            sort_lanes(mine, lane);   // (equal worths of different logits, where 64 bits do not tell them apart: by place)
+            if (lane >= l.beams) mine = Place{0, 0xffffffffu};
+            // (equal worths of different logits, where 64 bits do not tell them apart, may be out of order)
+            const Place above{__shfl_up_sync(0xffffffffu, mine.key, 1), __shfl_up_sync(0xffffffffu, mine.place, 1)};
+            if (__any_sync(0xffffffffu, lane > 0 && mine.before(above))) sort_lanes(mine, lane);
         }
         keys[beam][lane] = mine.key;
         places[beam][lane] = mine.place;
         if (lane == 0) {
-            normalisers[beam] = normaliser;
-            scores[beam] = alive ? score : -INFINITY;
+            divisors[beam] = divisor;
             finished[beam] = done;
             lengths[beam] = static_cast<int32_t>(length);
         }
     }
     __syncthreads();
-    if (warp != 0) return;
-    Place mine{keys[0][lane], places[0][lane]};
-    for (int beam = 1; beam < a.beams; ++beam) merge_lanes(mine, Place{keys[beam][lane], places[beam][lane]}, lane);
-    if (lane >= a.beams) return;
-    const int parent = static_cast<int>(mine.place / static_cast<uint32_t>(a.vocabulary)), token = static_cast<int>(mine.place - static_cast<uint32_t>(parent) * static_cast<uint32_t>(a.vocabulary));
-    float score = scores[parent];
-    if (!finished[parent]) {
-        const double normaliser = normalisers[parent];
-        const double logit = static_cast<double>(load_as_f32(a.logits, a.logits_type, entry * a.batch_stride + parent * a.beam_stride + token));
-        score = normaliser == normaliser ? static_cast<float>(static_cast<double>(score) + (logit - normaliser)) : -INFINITY;
+    for (int step = 1; step < l.beams; step <<= 1) {
+        if ((beam & (2 * step - 1)) == 0 && beam + step < l.beams) {
+            merge_lanes(mine, Place{keys[beam + step][lane], places[beam + step][lane]}, lane);
+            keys[beam][lane] = mine.key;
+            places[beam][lane] = mine.place;
+        }
+        __syncthreads();
     }
-    a.scores_out[entry * a.out_batch + lane * a.out_beam] = score;
+    if (beam != 0 || lane >= l.beams) return;
+    const int parent = static_cast<int>(mine.place / static_cast<uint32_t>(l.vocabulary)), token = static_cast<int>(mine.place - static_cast<uint32_t>(parent) * static_cast<uint32_t>(l.vocabulary));
+    a.scores_out[entry * a.out_batch + lane * a.out_beam] = static_cast<float>(double_from_ordered(mine.key) * divisors[parent]);
     a.tokens.at(entry, lane) = token;
     a.parents.at(entry, lane) = parent;
     if (a.finished_out.data) a.finished_out.at(entry, lane) = finished[parent] || (a.end >= 0 && token == a.end) ? 1 : 0;
     if (a.lengths_out.data) a.lengths_out.at(entry, lane) = lengths[parent];
     if (a.forks) {
-        int32_t* pair = a.forks + 2 * (static_cast<int64_t>(entry) * a.beams + lane);
-        pair[0] = a.source_base + entry * a.beams + parent;
-        pair[1] = a.target_base + entry * a.beams + lane;
+        int32_t* pair = a.forks + 2 * (static_cast<int64_t>(entry) * l.beams + lane);
+        pair[0] = a.source_base + entry * l.beams + parent;
+        pair[1] = a.target_base + entry * l.beams + lane;
     }
 }
 
@@ -376,8 +531,7 @@ int check_beams(const dfgpu_tensor& t, const dfgpu_beam_select_params& p, int dt
 }
 
 struct SelectCut {
-    int vectors;      // a thread
-    int64_t chunks;   // a row
+    int64_t parts, blocks;   // of a row; of a part
 };
 int check_select(const dfgpu_beam_select_params& p, SelectCut& cut) {
     if (!valid_tensor(p.logits) || p.logits.rank != 3) return fail(kInvalidShape, "BEAM_SELECT: logits must be [B, W, V] with positive extents");
@@ -403,27 +557,14 @@ int check_select(const dfgpu_beam_select_params& p, SelectCut& cut) {
         if (!is_packed_row_major(p.forks)) return fail(kInvalidLayout, "BEAM_SELECT: forks must be packed");
         if (p.source_base < 0 || p.target_base < 0 || p.source_base + rows > 0x7fffffff || p.target_base + rows > 0x7fffffff) return fail(kInvalidValue, "BEAM_SELECT: sequence numbers out of range");
     }
-    // As many vectors a thread as still give every SM two chunks.
-    const int width = 16 / dtype_bytes(p.logits.dtype);
-    const int64_t vectors = (p.logits.dim[2] + width - 1) / width;
-    for (cut.vectors = 8;; cut.vectors /= 2) {
-        cut.chunks = (vectors + kScanThreads * cut.vectors - 1) / (kScanThreads * cut.vectors);
-        if (cut.vectors == 1 || rows * cut.chunks >= 2 * 148) break;
-    }
-    if (rows * cut.chunks >= (1ll << 31)) return fail(kUnsupported, "BEAM_SELECT: too many tokens or entries");
+    // A block a warp, up to two CTAs for every SM, which run at once; then more blocks (16 x 8 beams, 128000 bf16 logits: 19.0 us; up to four CTAs 21.5, eight 28.8).
+    const int64_t values = 32 * kScanVectors * (16 / dtype_bytes(p.logits.dtype)), blocks = (p.logits.dim[2] + values - 1) / values;
+    cut.blocks = 1;
+    while (cut.parts = (blocks + kScanWarps * cut.blocks - 1) / (kScanWarps * cut.blocks), cut.parts > 1 && rows * cut.parts > 2 * 148) ++cut.blocks;
+    if (rows * cut.parts >= (1ll << 31)) return fail(kUnsupported, "BEAM_SELECT: too many tokens or entries");
     return kOk;
 }
-int64_t select_scratch(const dfgpu_beam_select_params& p, const SelectCut& cut) { return p.logits.dim[0] * p.logits.dim[1] * cut.chunks * (static_cast<int64_t>(sizeof(ChunkSum)) + 8 * p.logits.dim[1]); }
-
-template <typename T>
-void launch_scan(const ScanArgs& a, int vectors, int64_t chunks, cudaStream_t stream) {
-    const dim3 grid(static_cast<unsigned>(chunks));
-    const size_t shared = static_cast<size_t>(a.beams) * vectors * (16 / sizeof(T)) * sizeof(uint64_t);
-    if (vectors == 8) launch_chained(beam_scan_kernel<T, 8>, grid, dim3(kScanThreads), shared, stream, a);
-    else if (vectors == 4) launch_chained(beam_scan_kernel<T, 4>, grid, dim3(kScanThreads), shared, stream, a);
-    else if (vectors == 2) launch_chained(beam_scan_kernel<T, 2>, grid, dim3(kScanThreads), shared, stream, a);
-    else launch_chained(beam_scan_kernel<T, 1>, grid, dim3(kScanThreads), shared, stream, a);
-}
+int64_t select_scratch(const dfgpu_beam_select_params& p, const SelectCut& cut) { return p.logits.dim[0] * p.logits.dim[1] * cut.parts * (static_cast<int64_t>(sizeof(PartSum)) + 8 * p.logits.dim[1]); }
 
 int check_reorder(const dfgpu_beam_reorder_params& p) {
     if (!valid_tensor(p.parents) || p.parents.rank != 2) return fail(kInvalidShape, "BEAM_REORDER: parents must be [B, W] with positive extents");
@@ -494,25 +635,25 @@ extern "C" int dfgpu_beam_select(const dfgpu_beam_select_params* p, void* const*
             }
         }
     }
-    const int64_t entries = p->logits.dim[0], beams = p->logits.dim[1], chunks = entries * beams * cut.chunks;
+    const int64_t entries = p->logits.dim[0], beams = p->logits.dim[1], units = entries * beams * cut.parts;
     ScanArgs s{};
-    s.logits = port[0];
+    s.logits.data = port[0];
+    s.logits.batch_stride = p->logits.stride[0];
+    s.logits.beam_stride = p->logits.stride[1];
+    s.logits.beams = static_cast<int>(beams);
+    s.logits.vocabulary = static_cast<int>(p->logits.dim[2]);
+    s.logits.parts = static_cast<int>(cut.parts);
+    s.logits.blocks = static_cast<int>(cut.blocks);
+    s.logits.sums = static_cast<PartSum*>(scratch);
+    s.logits.keys = reinterpret_cast<uint64_t*>(s.logits.sums + units);
     s.finished = static_cast<const int32_t*>(port[2]);
-    s.sums = static_cast<ChunkSum*>(scratch);
-    s.keys = reinterpret_cast<uint64_t*>(s.sums + chunks);
-    s.batch_stride = p->logits.stride[0];
-    s.beam_stride = p->logits.stride[1];
     s.finished_batch = p->finished.rank ? p->finished.stride[0] : 0;
     s.finished_beam = p->finished.rank ? p->finished.stride[1] : 0;
-    s.beams = static_cast<int>(beams);
-    s.vocabulary = static_cast<int>(p->logits.dim[2]);
-    s.chunks = static_cast<int>(cut.chunks);
-    s.by_chunks = make_fast_divisor(static_cast<uint32_t>(cut.chunks));
+    s.by_parts = make_fast_divisor(static_cast<uint32_t>(cut.parts));
     s.by_beams = make_fast_divisor(static_cast<uint32_t>(beams));
     cudaStream_t on = as_stream(stream);
-    if (p->logits.dtype == DFGPU_F32) launch_scan<float>(s, cut.vectors, chunks, on);
-    else if (p->logits.dtype == DFGPU_F16) launch_scan<__half>(s, cut.vectors, chunks, on);
-    else launch_scan<__nv_bfloat16>(s, cut.vectors, chunks, on);
+    const dim3 grid(static_cast<unsigned>(units)), block(32 * kScanWarps);
+    launch_chained(p->logits.dtype == DFGPU_F32 ? beam_scan_kernel<float> : p->logits.dtype == DFGPU_F16 ? beam_scan_kernel<__half> : beam_scan_kernel<__nv_bfloat16>, grid, block, 0, on, s);
     status = check_launch("BEAM_SELECT");
     if (status) return status;
     MergeArgs m{};
@@ -520,10 +661,6 @@ extern "C" int dfgpu_beam_select(const dfgpu_beam_select_params* p, void* const*
         return Ints{static_cast<int32_t*>(port[i]), port[i] ? described[i]->stride[0] : 0, port[i] ? described[i]->stride[1] : 0};
     };
     m.logits = s.logits;
-    m.sums = s.sums;
-    m.keys = s.keys;
-    m.batch_stride = s.batch_stride;
-    m.beam_stride = s.beam_stride;
     m.scores = static_cast<const float*>(port[1]);
     m.scores_batch = p->scores.stride[0];
     m.scores_beam = p->scores.stride[1];
@@ -537,16 +674,12 @@ extern "C" int dfgpu_beam_select(const dfgpu_beam_select_params* p, void* const*
     m.finished_out = ints(7);
     m.lengths_out = ints(8);
     m.forks = static_cast<int32_t*>(port[9]);
-    m.beams = s.beams;
-    m.vocabulary = s.vocabulary;
-    m.chunks = s.chunks;
-    m.logits_type = p->logits.dtype;
     m.end = p->end;
     m.pad = p->pad;
     m.source_base = p->source_base;
     m.target_base = p->target_base;
     m.length_penalty = p->length_penalty;
-    launch_chained(beam_merge_kernel, dim3(static_cast<unsigned>(entries)), dim3(kScanThreads), 0, on, m);
+    launch_chained(beam_merge_kernel, dim3(static_cast<unsigned>(entries)), dim3(static_cast<unsigned>(32 * beams)), 0, on, m);
     return check_launch("BEAM_SELECT, join");
 }
 
