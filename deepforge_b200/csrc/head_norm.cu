@@ -9,13 +9,14 @@
 #include "dfgpu_decoder.h"
 #include "ports.cuh"
 #include "rotary.cuh"
+#include "umma_ptx.cuh"
 
 namespace dfgpu {
 namespace {
 
 constexpr int kNormThreads = 128, kNormWarps = kNormThreads / 32;
 constexpr int kNormTable = 2048;      // (cosine, sine) pairs of a CTA, forward: 16 KiB
-constexpr int kNormShared = 47 * 1024;   // gradient: the table and each warp's sums, in bytes
+constexpr int kNormShared = 14 * 1024, kNormSharedOfSixteen = 22 * 1024;   // bytes of a CTA's table, gradient: with the rows on their way within 48 KiB
 constexpr int64_t kNormMaxD = 1024;
 
 struct NormSide {
@@ -26,14 +27,14 @@ struct NormSide {
     float* partial;                   // (gradient: sums of dgain, null where it is not wanted)
     int64_t x_stride[3], dy_stride[3], out_stride[3];   // batch, head, token
     int64_t gain_head;
-    int32_t gain_type, heads, per_head;   // per_head: sums of dgain for each head
+    int32_t gain_type, heads, per_head;   // per_head: sums of dgain go out for each head
 };
 struct NormArgs {
     NormSide side[2];
     Positions at;
     int32_t seq, tokens, tiles, token_shift;   // tokens: of all sequences; a CTA's: 1 << token_shift
-    int32_t first_side, heads_per_cta;         // first_side: runs of heads of the first pair of tensors
-    int32_t d, half, turning, units, pitch;    // units of V pairs (half) or V channels (interleaved, or not turned) a row; pitch: of a token in the table
+    int32_t heads_per_cta, first_side;         // forward: of both pairs of tensors in a row; gradient: runs of the first pair are the first `first_side`
+    int32_t d, half, turning, units;           // units of V pairs (half) or V channels (interleaved, or not turned) a row
     int32_t group_shift;                       // lanes of a row: 1 << group_shift
     FastDivisor by_tiles, by_seq;
     float scale, epsilon, gain_offset, inverse_d;
@@ -46,23 +47,43 @@ __device__ __forceinline__ float gain_at(const NormSide& s, float offset, int64_
     return bf16_bits_to_f32(static_cast<const uint16_t*>(s.gain)[at]) + offset;
 }
 
-// One unit of a row in registers: V pairs as two vectors (i and i + half), or with INTERLEAVED V channels as one (V = 1: one pair as two values);
-// of channels that do not turn, V as one.
+__device__ __forceinline__ uint32_t narrow_two(__nv_bfloat16*, float lo, float hi) {
+    const __nv_bfloat162 pair = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&pair);
+}
+__device__ __forceinline__ uint32_t narrow_two(__half*, float lo, float hi) {
+    const __half2 pair = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&pair);
+}
+__device__ __forceinline__ uint64_t minus2(uint64_t v) { return v ^ 0x8000000080000000ull; }
+__device__ __forceinline__ float sum2(uint64_t v) {
+    float lo, hi;
+    unpack2(v, lo, hi);
+    return lo + hi;
+}
+
+// One unit of a row: V pairs as two vectors (i and i + half), or with INTERLEAVED V channels as one (V = 1: one pair as two values); of channels that do not
+// turn, V as one. In registers the pairs' first values are `one`, the second `two`, two neighbouring pairs to a register pair, which one instruction takes.
 template <typename T, int V, bool INTERLEAVED>
 struct NormUnit {
     static constexpr bool kTwo = !INTERLEAVED || V == 1;
-    static constexpr int kPairs = kTwo ? V : V / 2, kValues = kTwo ? 2 * V : V;
-    // places of pair p
-    static constexpr __device__ int one(int p) { return kTwo ? p : 2 * p; }
-    static constexpr __device__ int two(int p) { return kTwo ? V + p : 2 * p + 1; }
+    static constexpr int kPairs = kTwo ? V : V / 2, kPacks = (kPairs + 1) / 2, kQuad = kPairs < 4 ? kPairs : 4;
+    static constexpr int kPerLane = V == 1 ? 0 : 8 / kPairs;   // units that hold 16 values
     static __device__ __forceinline__ int channel(const NormArgs& a, int unit) {
         return unit < a.turning ? (INTERLEAVED ? unit * (V == 1 ? 2 : V) : unit * V) : 2 * a.half + (unit - a.turning) * V;
     }
     static __device__ __forceinline__ int apart(const NormArgs& a) { return INTERLEAVED ? 1 : a.half; }
+    // of value `half` (0, 1) of pack k: its place in a vector
+    static constexpr __device__ int place(int k, int half, bool second) { return kTwo ? 2 * k + half : 4 * k + 2 * half + (second ? 1 : 0); }
+};
+template <int PACKS>
+struct Values {
+    uint64_t one[PACKS], two[PACKS];
 };
 template <typename T, int V, bool INTERLEAVED>
 struct RawUnit {
     using Form = NormUnit<T, V, INTERLEAVED>;
+    using In = Values<Form::kPacks>;
     Pack<T, V> first, second;
     __device__ __forceinline__ void load(const T* from, int apart, bool live, bool turns) {
 #pragma unroll
@@ -70,372 +91,667 @@ struct RawUnit {
         if (live) first = *reinterpret_cast<const Pack<T, V>*>(from);
         if (Form::kTwo && live && turns) second = *reinterpret_cast<const Pack<T, V>*>(from + apart);
     }
-    __device__ __forceinline__ void values(float (&v)[Form::kValues]) const {
+    __device__ __forceinline__ In values() const {
+        In v;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            v[i] = widen(first.v[i]);
-            if constexpr (Form::kTwo) v[V + i] = widen(second.v[i]);
-        }
-    }
-    static __device__ __forceinline__ void store(T* to, int apart, bool turns, const float (&v)[Form::kValues]) {
-        Pack<T, V> out;
-#pragma unroll
-        for (int i = 0; i < V; ++i) out.v[i] = narrow<T>(v[i]);
-        *reinterpret_cast<Pack<T, V>*>(to) = out;
-        if constexpr (Form::kTwo) {
-            if (turns) {
-#pragma unroll
-                for (int i = 0; i < V; ++i) out.v[i] = narrow<T>(v[V + i]);
-                *reinterpret_cast<Pack<T, V>*>(to + apart) = out;
+        for (int k = 0; k < Form::kPacks; ++k) {
+            if constexpr (V == 1) {
+                v.one[k] = pack2(widen(first.v[0]), 0.0f);
+                v.two[k] = pack2(widen(second.v[0]), 0.0f);
+            } else if constexpr (Form::kTwo) {
+                v.one[k] = pack2(widen(first.v[2 * k]), widen(first.v[2 * k + 1]));
+                v.two[k] = pack2(widen(second.v[2 * k]), widen(second.v[2 * k + 1]));
+            } else {
+                v.one[k] = pack2(widen(first.v[4 * k]), widen(first.v[4 * k + 2]));
+                v.two[k] = pack2(widen(first.v[4 * k + 1]), widen(first.v[4 * k + 3]));
             }
+        }
+        return v;
+    }
+    static __device__ __forceinline__ void store(T* to, int apart, bool turns, const In& v) {
+        Pack<T, V> out[2];
+#pragma unroll
+        for (int k = 0; k < Form::kPacks; ++k) {
+            float a0, a1, b0, b1;
+            unpack2(v.one[k], a0, a1);
+            unpack2(v.two[k], b0, b1);
+            if constexpr (V == 1) {
+                out[0].v[0] = narrow<T>(a0);
+                out[1].v[0] = narrow<T>(b0);
+            } else if constexpr (sizeof(T) == 2) {
+                uint32_t* words[2] = {reinterpret_cast<uint32_t*>(&out[0]), reinterpret_cast<uint32_t*>(&out[1])};
+                if constexpr (Form::kTwo) {
+                    words[0][k] = narrow_two(static_cast<T*>(nullptr), a0, a1);
+                    words[1][k] = narrow_two(static_cast<T*>(nullptr), b0, b1);
+                } else {
+                    words[0][2 * k] = narrow_two(static_cast<T*>(nullptr), a0, b0);
+                    words[0][2 * k + 1] = narrow_two(static_cast<T*>(nullptr), a1, b1);
+                }
+            } else if constexpr (Form::kTwo) {
+                out[0].v[2 * k] = a0, out[0].v[2 * k + 1] = a1;
+                out[1].v[2 * k] = b0, out[1].v[2 * k + 1] = b1;
+            } else {
+                out[0].v[4 * k] = a0, out[0].v[4 * k + 1] = b0;
+                out[0].v[4 * k + 2] = a1, out[0].v[4 * k + 3] = b1;
+            }
+        }
+        *reinterpret_cast<Pack<T, V>*>(to) = out[0];
+        if constexpr (Form::kTwo) {
+            if (turns) *reinterpret_cast<Pack<T, V>*>(to + apart) = out[1];
         }
     }
 };
-template <typename Form>
-__device__ __forceinline__ void load_gains(const NormArgs& a, const NormSide& s, int head, int channel, bool live, bool turns, int apart, int v, float (&gain)[Form::kValues]) {
+template <typename Form, int V>
+__device__ __forceinline__ void load_gains(const NormArgs& a, const NormSide& s, int head, int channel, bool live, bool turns, Values<Form::kPacks>& gain) {
+    const int apart = Form::kTwo ? Form::apart(a) : 0;
+    const int64_t base = head * s.gain_head + channel;
 #pragma unroll
-    for (int i = 0; i < Form::kValues; ++i) {
-        const bool second = Form::kTwo && i >= v;
-        gain[i] = live && (!second || turns) ? gain_at(s, a.gain_offset, head * s.gain_head + channel + (second ? apart + i - v : i)) : 0.0f;
-    }
-}
-// The pairs of a unit by the angles at `table` (pair p of neighbouring units side by side); BACK: the other way.
-template <typename Form, bool BACK>
-__device__ __forceinline__ void turn_unit(const NormArgs& a, const float2* angles, int table, float (&v)[Form::kValues]) {
+    for (int k = 0; k < Form::kPacks; ++k) {
+        float g[2][2];
 #pragma unroll
-    for (int p = 0; p < Form::kPairs; ++p) {
-        const float2 cs = angles[table + p * a.turning];
-        const float x1 = v[Form::one(p)], x2 = v[Form::two(p)];
-        if (BACK) {
-            v[Form::one(p)] = __fmaf_rn(x1, cs.x, x2 * cs.y);
-            v[Form::two(p)] = __fmaf_rn(x2, cs.x, -(x1 * cs.y));
-        } else {
-            v[Form::one(p)] = __fmaf_rn(x1, cs.x, -(x2 * cs.y));
-            v[Form::two(p)] = __fmaf_rn(x2, cs.x, x1 * cs.y);
+        for (int half = 0; half < 2; ++half) {
+            const bool there = live && (V > 1 || half == 0);
+            g[0][half] = there ? gain_at(s, a.gain_offset, base + Form::place(k, half, false)) : 0.0f;
+            g[1][half] = there && (!Form::kTwo || turns) ? gain_at(s, a.gain_offset, base + apart + Form::place(k, half, true)) : 0.0f;
         }
+        gain.one[k] = pack2(g[0][0], g[0][1]);
+        gain.two[k] = pack2(g[1][0], g[1][1]);
     }
 }
+// The table of a token: cosines of all pairs, then sines, those of a unit's pairs in vectors of kQuad, vectors of neighbouring units side by side.
 template <typename Form>
-__device__ __forceinline__ void put_angle(const NormArgs& a, float2* angles, int local, int pair, float2 turn) {
-    const int unit = pair / Form::kPairs;
-    angles[local * a.pitch + (pair - unit * Form::kPairs) * a.turning + unit] = make_float2(turn.x * a.scale, turn.y * a.scale);
+__device__ __forceinline__ int angle_place(const NormArgs& a, int unit, int quad) { return (quad * a.turning + unit) * Form::kQuad; }
+template <typename Form, bool CLOSE>
+__device__ __forceinline__ void put_angle(const NormArgs& a, float* table, int pair, int64_t batch, int64_t token) {
+    float2 turn = turn_of<CLOSE>(a.at, batch, token, pair);
+    const int unit = pair / Form::kPairs, within = pair - unit * Form::kPairs, place = angle_place<Form>(a, unit, within / Form::kQuad) + within % Form::kQuad;
+    table[place] = turn.x * a.scale;
+    table[a.half + place] = turn.y * a.scale;
+}
+template <typename Form>
+__device__ __forceinline__ void get_angles(const float* table, int place, int step, uint64_t (&out)[Form::kPacks]) {
+    if constexpr (Form::kQuad == 4) {
+#pragma unroll
+        for (int q = 0; q < Form::kPacks / 2; ++q) {
+            const float4 four = *reinterpret_cast<const float4*>(table + place + q * step);
+            out[2 * q] = pack2(four.x, four.y);
+            out[2 * q + 1] = pack2(four.z, four.w);
+        }
+    } else if constexpr (Form::kQuad == 2) {
+        const float2 two = *reinterpret_cast<const float2*>(table + place);
+        out[0] = pack2(two.x, two.y);
+    } else {
+        out[0] = pack2(table[place], 0.0f);
+    }
+}
+// The pairs of a unit by a token's angles; BACK: the other way.
+template <typename Form, bool BACK>
+__device__ __forceinline__ void turn_unit(const NormArgs& a, const float* table, int unit, Values<Form::kPacks>& v) {
+    uint64_t cosine[Form::kPacks], sine[Form::kPacks];
+    const int place = angle_place<Form>(a, unit, 0), step = a.turning * Form::kQuad;
+    get_angles<Form>(table, place, step, cosine);
+    get_angles<Form>(table + a.half, place, step, sine);
+#pragma unroll
+    for (int k = 0; k < Form::kPacks; ++k) {
+        const uint64_t one = v.one[k], two = v.two[k], back = minus2(sine[k]);
+        v.one[k] = fma2(one, cosine[k], mul2(two, BACK ? sine[k] : back));
+        v.two[k] = fma2(two, cosine[k], mul2(one, BACK ? back : sine[k]));
+    }
 }
 __device__ __forceinline__ float sum_over(float v, int lanes) {
     for (int o = 1; o < lanes; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
 
-// ---- forward: a CTA takes a few tokens of one sequence and a run of heads --------------------------------------
-// U units a lane (1 or 2), or 0: a row is a whole warp's and read a second time (from the cache).
-template <typename T, int V, bool INTERLEAVED, int U>
-__global__ void __launch_bounds__(kNormThreads)
-head_norm_kernel(const NormArgs a) {
-    using Form = NormUnit<T, V, INTERLEAVED>;
-    using Raw = RawUnit<T, V, INTERLEAVED>;
-    extern __shared__ float2 angles[];
-    const int tile = static_cast<int>(blockIdx.x);
-    const int batch_index = static_cast<int>(fast_divide(static_cast<uint32_t>(tile), a.by_tiles));
-    const int token0 = (tile - batch_index * a.tiles) << a.token_shift;
-    const bool second_side = static_cast<int>(blockIdx.y) >= a.first_side;
-    const NormSide& s = second_side ? a.side[1] : a.side[0];
-    const int head0 = (static_cast<int>(blockIdx.y) - (second_side ? a.first_side : 0)) * a.heads_per_cta;
-    const int rows = min(a.heads_per_cta, s.heads - head0) << a.token_shift, tokens = a.seq - token0, mask = (1 << a.token_shift) - 1;
-    const T* x = static_cast<const T*>(s.x) + batch_index * s.x_stride[0] + head0 * s.x_stride[1] + token0 * s.x_stride[2];
-    T* y = static_cast<T*>(s.out) + batch_index * s.out_stride[0] + head0 * s.out_stride[1] + token0 * s.out_stride[2];
-    const int lanes = 1 << a.group_shift, lane = threadIdx.x & (lanes - 1), group = threadIdx.x >> a.group_shift, groups = kNormThreads >> a.group_shift;
-    const int apart = Form::apart(a);
-    auto fill_angles = [&] {
-        for (int i = threadIdx.x; i < a.half << a.token_shift; i += kNormThreads) {
-            const int local = i & mask, pair = i >> a.token_shift;
-            if (local < tokens) put_angle<Form>(a, angles, local, pair, turn_of(a.at, batch_index, token0 + local, pair));
-        }
-        __syncthreads();
-    };
-    chain_begin();
-    if constexpr (U > 0) {
-        int channel[U];
-        bool there[U], turns[U];
+template <typename T>
+__device__ __forceinline__ float inverse_root(float v) { return sizeof(T) == 4 ? __frsqrt_rn(v) : rsqrtf(v); }   // (the other is off by 2^-23 and a little, which 16 bits do not show)
+
+// What a lane has of every row: up to 16 values.
+template <typename Form, int U>
+struct Share {
+    int channel[U], unit[U];
+    bool there[U], turns[U];
+    __device__ __forceinline__ Share(const NormArgs& a, int lane) {
 #pragma unroll
         for (int j = 0; j < U; ++j) {
-            const int unit = lane + j * lanes;
-            there[j] = unit < a.units;
-            turns[j] = unit < a.turning;
-            channel[j] = Form::channel(a, unit);
+            unit[j] = lane + (j << a.group_shift);
+            there[j] = unit[j] < a.units;
+            turns[j] = unit[j] < a.turning;
+            channel[j] = Form::channel(a, unit[j]);
         }
-        Raw now[U], next[U];
-        auto load = [&](Raw (&raw)[U], int row) {
-            const int local = row & mask, head = row >> a.token_shift;
-            const bool live = row < rows && local < tokens;
-            const T* from = x + head * s.x_stride[1] + local * s.x_stride[2];
+    }
+};
+
+// Rows on their way: a thread copies its own vectors into shared memory (16 or 8 bytes each, asynchronously) and reads none but those, so nothing waits for
+// another thread, and what is in flight takes no registers. What is not wanted becomes zeros.
+template <typename T, int V, bool INTERLEAVED, int STAGES, int TENSORS>
+struct Ring {
+    using Form = NormUnit<T, V, INTERLEAVED>;
+    using Vector = Pack<T, V>;
+    static constexpr int U = Form::kPerLane, kSlots = (Form::kTwo ? 2 : 1) * U, kBytes = static_cast<int>(sizeof(Vector)) * kSlots * TENSORS * STAGES * kNormThreads;
+    Vector* own;   // [stage][tensor][slot][thread]
+    int filling = 0, reading = 0;
+    __device__ __forceinline__ explicit Ring(void* shared) : own(static_cast<Vector*>(shared) + threadIdx.x) {}
+    __device__ __forceinline__ Vector* slot(int stage, int tensor, int i) const { return own + ((stage * TENSORS + tensor) * kSlots + i) * kNormThreads; }
+    static __device__ __forceinline__ void copy(Vector* to, const T* from, bool wanted) {
+        const uint32_t bytes = wanted ? static_cast<uint32_t>(sizeof(Vector)) : 0u;
+        if constexpr (sizeof(Vector) == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(__cvta_generic_to_global(from)), "r"(bytes) : "memory");
+        else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(smem_u32(to)), "l"(__cvta_generic_to_global(from)), "r"(bytes) : "memory");
+    }
+    // One row of each tensor: `from` is an address that may be read, wanted or not.
+    __device__ __forceinline__ void fill(const Share<Form, U>& share, int apart, const T* const (&from)[TENSORS], bool wanted) {
 #pragma unroll
-            for (int j = 0; j < U; ++j) raw[j].load(from + channel[j], apart, live && there[j], turns[j]);
-        };
-        load(now, group);   // (on its way while the angles are worked out)
-        fill_angles();
-        float gain[U][Form::kValues];
-        int held = -1;      // the head whose gains these are
-        for (int base = 0; base < rows; base += groups) {   // (whole warps stay together)
-            const int row = base + group, local = row & mask, head = row >> a.token_shift;
-            load(next, row + groups);
-            const int wanted = s.gain_head ? head0 + min(head, s.heads - head0 - 1) : 0;
-            if (wanted != held) {
-#pragma unroll
-                for (int j = 0; j < U; ++j) load_gains<Form>(a, s, wanted, channel[j], there[j], turns[j], apart, V, gain[j]);
-                held = wanted;
-            }
-            float v[U][Form::kValues], squares = 0.0f;
+        for (int t = 0; t < TENSORS; ++t)
 #pragma unroll
             for (int j = 0; j < U; ++j) {
-                now[j].values(v[j]);
-#pragma unroll
-                for (int i = 0; i < Form::kValues; ++i) squares = __fmaf_rn(v[j][i], v[j][i], squares);
+                const bool first = wanted && share.there[j], second = first && share.turns[j];
+                copy(slot(filling, t, j), first ? from[t] + share.channel[j] : from[t], first);
+                if constexpr (Form::kTwo) copy(slot(filling, t, U + j), second ? from[t] + share.channel[j] + apart : from[t], second);
             }
-            const float r = rsqrtf(__fmaf_rn(sum_over(squares, lanes), a.inverse_d, a.epsilon));
-            if (row < rows && local < tokens) {
-                T* to = y + head * s.out_stride[1] + local * s.out_stride[2];
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        filling = filling + 1 == STAGES ? 0 : filling + 1;
+    }
+    // The oldest row that was not taken yet, of which STAGES - 1 are on their way.
+    __device__ __forceinline__ void take(RawUnit<T, V, INTERLEAVED> (&rows)[TENSORS][U]) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+#pragma unroll
+        for (int t = 0; t < TENSORS; ++t)
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                rows[t][j].first = *slot(reading, t, j);
+                if constexpr (Form::kTwo) rows[t][j].second = *slot(reading, t, U + j);
+            }
+        reading = reading + 1 == STAGES ? 0 : reading + 1;
+    }
+    __device__ __forceinline__ void drain() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+};
+template <typename T> constexpr int kForwardStages = sizeof(T) == 4 ? 3 : 4;
+template <typename T> constexpr int kGradientStages = sizeof(T) == 4 ? 2 : 3;
+
+// ---- forward: a CTA takes a few tokens of one sequence and a run of heads of both pairs of tensors, which share the tokens' angles -----------------------
+// A group of lanes has one token and walks the heads, so that the angles stay in registers, multiplied by the gains already.
+template <typename T, int V, bool INTERLEAVED>
+__global__ void __launch_bounds__(kNormThreads)
+head_norm_kernel(const __grid_constant__ NormArgs a) {
+    using Form = NormUnit<T, V, INTERLEAVED>;
+    using Raw = RawUnit<T, V, INTERLEAVED>;
+    constexpr int U = Form::kPerLane;
+    extern __shared__ __align__(16) float angles[];
+    const int tile = static_cast<int>(blockIdx.x);
+    const int batch_index = static_cast<int>(fast_divide(static_cast<uint32_t>(tile), a.by_tiles));
+    const int token0 = (tile - batch_index * a.tiles) << a.token_shift, tokens = a.seq - token0, mask = (1 << a.token_shift) - 1;
+    const int lanes = 1 << a.group_shift, group = threadIdx.x >> a.group_shift, groups = kNormThreads >> a.group_shift;
+    const int local = group & mask, first_head = group >> a.token_shift, step = groups >> a.token_shift;   // (no more tokens than groups)
+    const Share<Form, U> share(a, threadIdx.x & (lanes - 1));
+    const int apart = Form::apart(a), run0 = static_cast<int>(blockIdx.y) * a.heads_per_cta, run1 = run0 + a.heads_per_cta;
+    const bool live = local < tokens;
+    int which = run0 < a.side[0].heads ? 0 : 1, head = 0, heads = 0;   // of the pair of tensors that is at hand: heads of the run
+    const T* x = nullptr;
+    T* y = nullptr;
+    auto begin = [&] {
+        const NormSide& s = a.side[which];
+        const int before = which ? a.side[0].heads : 0, head0 = max(run0 - before, 0);
+        head = head0 + first_head;
+        heads = min(run1 - before, s.heads);
+        x = static_cast<const T*>(s.x) + batch_index * s.x_stride[0] + head * s.x_stride[1] + (token0 + local) * s.x_stride[2];
+        y = static_cast<T*>(s.out) + batch_index * s.out_stride[0] + head * s.out_stride[1] + (token0 + local) * s.out_stride[2];
+    };
+    Ring<T, V, INTERLEAVED, kForwardStages<T>, 1> ring(angles + ((2 * a.half) << a.token_shift));
+    int64_t x_step = 0;
+    auto start = [&] {   // the first rows of the pair of tensors at hand
+        x_step = step * a.side[which].x_stride[1];
+#pragma unroll
+        for (int i = 0; i + 1 < kForwardStages<T>; ++i) {
+            const bool wanted = live && head + i * step < heads;
+            const T* const from[1] = {wanted ? x + i * x_step : static_cast<const T*>(a.side[which].x)};
+            ring.fill(share, apart, from, wanted);
+        }
+    };
+    begin();
+    chain_begin();
+    start();   // (on their way while the angles are worked out)
+    for (int i = threadIdx.x; i < a.half << a.token_shift; i += kNormThreads) {
+        const int token = i & mask, pair = i >> a.token_shift;
+        if (token < tokens) put_angle<Form, sizeof(T) == 4>(a, angles + token * 2 * a.half, pair, batch_index, token0 + token);
+    }
+    __syncthreads();
+    for (;;) {
+        const NormSide& s = a.side[which];
+        const int64_t y_step = step * s.out_stride[1];
+        Values<Form::kPacks> along[U], across[U];   // what a pair's own value and the other one are multiplied by
+        int held = -1;                              // the head whose gains are in them
+        // (whole warps stay together: a warp's groups have heads side by side)
+        while (__any_sync(0xffffffffu, head < heads)) {
+            const bool own = live && head < heads, later = live && head + (kForwardStages<T> - 1) * step < heads;
+            Raw now[1][U];
+            ring.take(now);
+            const T* const from[1] = {later ? x + (kForwardStages<T> - 1) * x_step : static_cast<const T*>(s.x)};
+            ring.fill(share, apart, from, later);
+            const int wanted = s.gain_head ? min(head, s.heads - 1) : 0;
+            if (wanted != held) {
 #pragma unroll
                 for (int j = 0; j < U; ++j) {
-                    if (!there[j]) continue;
+                    Values<Form::kPacks> gain;
+                    load_gains<Form, V>(a, s, wanted, share.channel[j], share.there[j], share.turns[j], gain);
+                    along[j] = gain;
+                    across[j] = Values<Form::kPacks>{};
+                    if (!share.turns[j]) continue;
+                    uint64_t cosine[Form::kPacks], sine[Form::kPacks];
+                    const float* table = angles + local * 2 * a.half;
+                    const int place = angle_place<Form>(a, share.unit[j], 0), stride = a.turning * Form::kQuad;
+                    get_angles<Form>(table, place, stride, cosine);
+                    get_angles<Form>(table + a.half, place, stride, sine);
 #pragma unroll
-                    for (int i = 0; i < Form::kValues; ++i) v[j][i] = v[j][i] * r * gain[j][i];
-                    if (turns[j]) turn_unit<Form, false>(a, angles, local * a.pitch + lane + j * lanes, v[j]);
-                    Raw::store(to + channel[j], apart, turns[j], v[j]);
+                    for (int k = 0; k < Form::kPacks; ++k) {
+                        along[j].one[k] = mul2(gain.one[k], cosine[k]);
+                        along[j].two[k] = mul2(gain.two[k], cosine[k]);
+                        across[j].one[k] = minus2(mul2(gain.two[k], sine[k]));
+                        across[j].two[k] = mul2(gain.one[k], sine[k]);
+                    }
                 }
+                held = wanted;
             }
+            Values<Form::kPacks> v[U];
+            uint64_t squares = 0;
 #pragma unroll
-            for (int j = 0; j < U; ++j) now[j] = next[j];
+            for (int j = 0; j < U; ++j) {
+                v[j] = now[0][j].values();
+#pragma unroll
+                for (int k = 0; k < Form::kPacks; ++k) squares = fma2(v[j].two[k], v[j].two[k], fma2(v[j].one[k], v[j].one[k], squares));
+            }
+            const float r = inverse_root<T>(__fmaf_rn(sum_over(sum2(squares), lanes), a.inverse_d, a.epsilon));
+            const uint64_t both = pack2(r, r);
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+#pragma unroll
+                for (int k = 0; k < Form::kPacks; ++k) {
+                    const uint64_t one = mul2(v[j].one[k], both), two = mul2(v[j].two[k], both);
+                    v[j].one[k] = fma2(one, along[j].one[k], mul2(two, across[j].one[k]));
+                    v[j].two[k] = fma2(two, along[j].two[k], mul2(one, across[j].two[k]));
+                }
+                if (own && share.there[j]) Raw::store(y + share.channel[j], apart, share.turns[j], v[j]);
+            }
+            head += step;
+            x += x_step;
+            y += y_step;
         }
-    } else {
-        fill_angles();
-        for (int row = group; row < rows; row += groups) {
+        ring.drain();
+        if (which == 1 || run1 <= a.side[0].heads || a.side[1].heads == 0) return;
+        which = 1;
+        begin();
+        start();
+    }
+}
+
+// Single values, and rows longer than a warp's registers: a row is a whole warp's and read a second time (from the cache).
+template <typename T, int V, bool INTERLEAVED>
+__global__ void __launch_bounds__(kNormThreads)
+head_norm_long_kernel(const __grid_constant__ NormArgs a) {
+    using Form = NormUnit<T, V, INTERLEAVED>;
+    using Raw = RawUnit<T, V, INTERLEAVED>;
+    extern __shared__ __align__(16) float angles[];
+    const int tile = static_cast<int>(blockIdx.x);
+    const int batch_index = static_cast<int>(fast_divide(static_cast<uint32_t>(tile), a.by_tiles));
+    const int token0 = (tile - batch_index * a.tiles) << a.token_shift, tokens = a.seq - token0, mask = (1 << a.token_shift) - 1;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int apart = Form::apart(a), run0 = static_cast<int>(blockIdx.y) * a.heads_per_cta, run1 = run0 + a.heads_per_cta;
+    chain_begin();
+    for (int i = threadIdx.x; i < a.half << a.token_shift; i += kNormThreads) {
+        const int local = i & mask, pair = i >> a.token_shift;
+        if (local < tokens) put_angle<Form, sizeof(T) == 4>(a, angles + local * 2 * a.half, pair, batch_index, token0 + local);
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int which = 0; which < 2; ++which) {
+        const NormSide& s = a.side[which];
+        const int before = which ? a.side[0].heads : 0, head0 = max(run0 - before, 0), heads = min(run1 - before, s.heads) - head0;
+        if (heads <= 0) continue;
+        const T* x = static_cast<const T*>(s.x) + batch_index * s.x_stride[0] + head0 * s.x_stride[1] + token0 * s.x_stride[2];
+        T* y = static_cast<T*>(s.out) + batch_index * s.out_stride[0] + head0 * s.out_stride[1] + token0 * s.out_stride[2];
+        for (int row = warp; row < heads << a.token_shift; row += kNormWarps) {
             const int local = row & mask, head = row >> a.token_shift;
             if (local >= tokens) continue;   // (a whole warp's row)
             const T* from = x + head * s.x_stride[1] + local * s.x_stride[2];
             T* to = y + head * s.out_stride[1] + local * s.out_stride[2];
-            float squares = 0.0f;
+            uint64_t squares = 0;
             for (int unit = lane; unit < a.units; unit += 32) {
                 Raw raw;
-                float v[Form::kValues];
                 raw.load(from + Form::channel(a, unit), apart, true, unit < a.turning);
-                raw.values(v);
+                const Values<Form::kPacks> v = raw.values();
 #pragma unroll
-                for (int i = 0; i < Form::kValues; ++i) squares = __fmaf_rn(v[i], v[i], squares);
+                for (int k = 0; k < Form::kPacks; ++k) squares = fma2(v.two[k], v.two[k], fma2(v.one[k], v.one[k], squares));
             }
-            const float r = rsqrtf(__fmaf_rn(sum_over(squares, 32), a.inverse_d, a.epsilon));
+            const float r = inverse_root<T>(__fmaf_rn(sum_over(sum2(squares), 32), a.inverse_d, a.epsilon));
+            const uint64_t both = pack2(r, r);
             for (int unit = lane; unit < a.units; unit += 32) {
                 const bool turns = unit < a.turning;
                 const int channel = Form::channel(a, unit);
                 Raw raw;
-                float v[Form::kValues], gain[Form::kValues];
                 raw.load(from + channel, apart, true, turns);
-                raw.values(v);
-                load_gains<Form>(a, s, s.gain_head ? head0 + head : 0, channel, true, turns, apart, V, gain);
+                Values<Form::kPacks> v = raw.values(), gain;
+                load_gains<Form, V>(a, s, s.gain_head ? head0 + head : 0, channel, true, turns, gain);
 #pragma unroll
-                for (int i = 0; i < Form::kValues; ++i) v[i] = v[i] * r * gain[i];
-                if (turns) turn_unit<Form, false>(a, angles, local * a.pitch + unit, v);
+                for (int k = 0; k < Form::kPacks; ++k) {
+                    v.one[k] = mul2(mul2(v.one[k], both), gain.one[k]);
+                    v.two[k] = mul2(mul2(v.two[k], both), gain.two[k]);
+                }
+                if (turns) turn_unit<Form, false>(a, angles + local * 2 * a.half, unit, v);
                 Raw::store(to + channel, apart, turns, v);
             }
         }
     }
 }
 
-// ---- gradients: a CTA takes tokens of all sequences in a row and a run of heads; each warp has heads of its own, whose sums of dgain it keeps ----
-template <typename T, int V, bool INTERLEAVED, int U>
-__global__ void __launch_bounds__(kNormThreads)
-head_norm_grad_kernel(const NormArgs a) {
-    using Form = NormUnit<T, V, INTERLEAVED>;
-    using Raw = RawUnit<T, V, INTERLEAVED>;
-    extern __shared__ float2 angles[];                                // the table; where a lane keeps no sums, those of each warp behind it
-    __shared__ int64_t places[3][32];                                 // of the tokens in X, dY, dX
-    const int tile = static_cast<int>(blockIdx.x), token0 = tile << a.token_shift, tokens = min(a.tokens - token0, 1 << a.token_shift);
-    const bool second_side = static_cast<int>(blockIdx.y) >= a.first_side;
-    const NormSide& s = second_side ? a.side[1] : a.side[0];
-    const int run = static_cast<int>(blockIdx.y) - (second_side ? a.first_side : 0), runs = second_side ? static_cast<int>(gridDim.y) - a.first_side : a.first_side;
-    const int head0 = run * a.heads_per_cta, heads = min(a.heads_per_cta, s.heads - head0);
-    const int warp = threadIdx.x >> 5, lanes = 1 << a.group_shift, lane = threadIdx.x & (lanes - 1), group = (threadIdx.x & 31) >> a.group_shift, groups = 32 >> a.group_shift;
-    const int apart = Form::apart(a);
-    const bool sums_wanted = s.partial != nullptr;
-    if (threadIdx.x < tokens) {
-        const int token = token0 + threadIdx.x, b = static_cast<int>(fast_divide(static_cast<uint32_t>(token), a.by_seq)), t = token - b * a.seq;
-        places[0][threadIdx.x] = b * s.x_stride[0] + t * s.x_stride[2];
-        places[1][threadIdx.x] = b * s.dy_stride[0] + t * s.dy_stride[2];
-        places[2][threadIdx.x] = b * s.out_stride[0] + t * s.out_stride[2];
+// ---- gradients: a CTA takes tokens of all sequences in a row and a run of heads ------------------------------------------------------------------------
+// u turned back, squares and v x of a unit, added to the sums that the row needs.
+template <typename Form>
+__device__ __forceinline__ void add_unit(const Values<Form::kPacks>& x, const Values<Form::kPacks>& u, const Values<Form::kPacks>& gain, uint64_t& squares, uint64_t& product) {
+#pragma unroll
+    for (int k = 0; k < Form::kPacks; ++k) {
+        squares = fma2(x.two[k], x.two[k], fma2(x.one[k], x.one[k], squares));
+        product = fma2(mul2(u.two[k], gain.two[k]), x.two[k], fma2(mul2(u.one[k], gain.one[k]), x.one[k], product));
     }
-    chain_begin();
+}
+// dX of a unit in u's place, and the terms of dgain onto `sums`.
+template <typename Form>
+__device__ __forceinline__ void finish_unit(const Values<Form::kPacks>& x, Values<Form::kPacks>& u, const Values<Form::kPacks>& gain, float r, float along, Values<Form::kPacks>& sums) {
+    const uint64_t both = pack2(r, r), back = pack2(-along, -along);
+#pragma unroll
+    for (int k = 0; k < Form::kPacks; ++k) {
+        sums.one[k] = fma2(u.one[k], mul2(x.one[k], both), sums.one[k]);
+        sums.two[k] = fma2(u.two[k], mul2(x.two[k], both), sums.two[k]);
+        u.one[k] = mul2(both, fma2(x.one[k], back, mul2(u.one[k], gain.one[k])));
+        u.two[k] = mul2(both, fma2(x.two[k], back, mul2(u.two[k], gain.two[k])));
+    }
+}
+// A token's places in X, dY and dX.
+struct TokenPlaces {
+    int64_t x, dy, out;
+    __device__ __forceinline__ TokenPlaces(const NormArgs& a, const NormSide& s, int token) {
+        const int b = static_cast<int>(fast_divide(static_cast<uint32_t>(token), a.by_seq)), t = token - b * a.seq;
+        x = b * s.x_stride[0] + t * s.x_stride[2];
+        dy = b * s.dy_stride[0] + t * s.dy_stride[2];
+        out = b * s.out_stride[0] + t * s.out_stride[2];
+    }
+};
+template <typename Form, bool CLOSE>
+__device__ __forceinline__ void fill_angles(const NormArgs& a, float* angles, int token0, int tokens) {
     for (int i = threadIdx.x; i < a.half << a.token_shift; i += kNormThreads) {
         const int local = i & ((1 << a.token_shift) - 1), pair = i >> a.token_shift;
         if (local >= tokens) continue;
         const int token = token0 + local, b = static_cast<int>(fast_divide(static_cast<uint32_t>(token), a.by_seq));
-        put_angle<Form>(a, angles, local, pair, turn_of(a.at, b, token - b * a.seq, pair));
+        put_angle<Form, CLOSE>(a, angles + local * 2 * a.half, pair, b, token - b * a.seq);
     }
-    __syncthreads();
-    const T* x = static_cast<const T*>(s.x);
-    const T* dy = static_cast<const T*>(s.dy);
-    T* dx = static_cast<T*>(s.out);
-    float* of_tile = s.partial + (s.per_head ? (static_cast<int64_t>(tile) * s.heads) * a.d : (static_cast<int64_t>(tile) * runs + run) * a.d);
-    if constexpr (U > 0) {
-        int channel[U];
-        bool there[U], turns[U];
-        float gain[U][Form::kValues], sums[U][Form::kValues];
+}
+// The values of a lane's share, met over the groups of its warp, to channels at `to`.
+template <typename Form, int U, int V>
+__device__ __forceinline__ void put_sums(const NormArgs& a, const Share<Form, U>& share, const Values<Form::kPacks> (&sums)[U], float* to) {
+    const int lanes = 1 << a.group_shift;
+    const bool first_group = (threadIdx.x & 31) < lanes;
+    const int apart = Form::kTwo ? Form::apart(a) : 0;
+#pragma unroll
+    for (int j = 0; j < U; ++j)
+#pragma unroll
+        for (int k = 0; k < Form::kPacks; ++k) {
+            float v[2][2];
+            unpack2(sums[j].one[k], v[0][0], v[0][1]);
+            unpack2(sums[j].two[k], v[1][0], v[1][1]);
+#pragma unroll
+            for (int second = 0; second < 2; ++second)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    float sum = v[second][half];
+                    for (int o = lanes; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    if (first_group && share.there[j] && (!second || !Form::kTwo || share.turns[j])) to[share.channel[j] + (second ? apart : 0) + Form::place(k, half, second != 0)] = sum;
+                }
+        }
+}
+
+// PER_HEAD: each warp has heads of its own, with their gains, and walks the tokens, whose angles are in the table; the sums of dgain go out with each head.
+// Otherwise a group of lanes has one token, its angles in registers, and walks the heads; all have one sum.
+template <typename T, int V, bool INTERLEAVED, bool PER_HEAD>
+__global__ void __launch_bounds__(kNormThreads)
+head_norm_grad_kernel(const __grid_constant__ NormArgs a) {
+    using Form = NormUnit<T, V, INTERLEAVED>;
+    using Raw = RawUnit<T, V, INTERLEAVED>;
+    constexpr int U = Form::kPerLane;
+    extern __shared__ __align__(16) float angles[];                   // the table, and each warp's sums afterwards
+    __shared__ int64_t places[3][32];                                 // (PER_HEAD) of the tokens in X, dY, dX
+    const int tile = static_cast<int>(blockIdx.x), token0 = tile << a.token_shift, tokens = min(a.tokens - token0, 1 << a.token_shift);
+    const bool second_side = static_cast<int>(blockIdx.y) >= a.first_side;
+    const NormSide& s = a.side[second_side];
+    const int run = static_cast<int>(blockIdx.y) - (second_side ? a.first_side : 0), runs = second_side ? static_cast<int>(gridDim.y) - a.first_side : a.first_side;
+    const int head0 = run * a.heads_per_cta, heads = min(a.heads_per_cta, s.heads - head0);
+    const int warp = threadIdx.x >> 5, lanes = 1 << a.group_shift, apart = Form::apart(a);
+    const Share<Form, U> share(a, threadIdx.x & (lanes - 1));
+    const bool sums_wanted = s.partial != nullptr;
+    const int mask = (1 << a.token_shift) - 1;
+    const int group = PER_HEAD ? (threadIdx.x & 31) >> a.group_shift : threadIdx.x >> a.group_shift, groups = (PER_HEAD ? 32 : kNormThreads) >> a.group_shift;
+    const T* x = static_cast<const T*>(s.x) + head0 * s.x_stride[1];
+    const T* dy = static_cast<const T*>(s.dy) + head0 * s.dy_stride[1];
+    T* dx = static_cast<T*>(s.out) + head0 * s.out_stride[1];
+    Values<Form::kPacks> gain[U], sums[U], cosine[U], sine[U];   // (the angles, not PER_HEAD: `one` alone)
+#pragma unroll
+    for (int j = 0; j < U; ++j) sums[j] = Values<Form::kPacks>{};
+    Ring<T, V, INTERLEAVED, kGradientStages<T>, 2> ring(angles + ((2 * a.half) << a.token_shift));
+    auto fill = [&](const T* from_x, const T* from_dy, bool wanted) {
+        const T* const from[2] = {wanted ? from_x : static_cast<const T*>(s.x), wanted ? from_dy : static_cast<const T*>(s.dy)};
+        ring.fill(share, apart, from, wanted);
+    };
+    Raw rows[2][U];   // of X and dY, at hand
+    auto take_gains = [&](int head) {
+#pragma unroll
+        for (int j = 0; j < U; ++j) load_gains<Form, V>(a, s, head, share.channel[j], share.there[j], share.turns[j], gain[j]);
+    };
+    // The row at hand: u turned back, both sums, dX to `to`, and the terms of dgain.
+    auto row = [&](T* to, const float* table, bool live) {
+        Values<Form::kPacks> v[U], u[U];
+        uint64_t squares2 = 0, product2 = 0;
 #pragma unroll
         for (int j = 0; j < U; ++j) {
-            const int unit = lane + j * lanes;
-            there[j] = unit < a.units;
-            turns[j] = unit < a.turning;
-            channel[j] = Form::channel(a, unit);
+            v[j] = rows[0][j].values();
+            u[j] = rows[1][j].values();
+            if constexpr (PER_HEAD) {
+                if (share.turns[j]) turn_unit<Form, true>(a, table, share.unit[j], u[j]);
+            } else {
 #pragma unroll
-            for (int i = 0; i < Form::kValues; ++i) sums[j][i] = 0.0f;
-        }
-        // The groups' sums, met in one group's lanes, to channels at `to`.
-        auto put_sums = [&](float* to) {
-#pragma unroll
-            for (int j = 0; j < U; ++j)
-#pragma unroll
-                for (int i = 0; i < Form::kValues; ++i) {
-                    float v = sums[j][i];
-                    for (int o = lanes; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-                    const bool second = Form::kTwo && i >= V;
-                    if (group == 0 && there[j] && (!second || turns[j])) to[channel[j] + (second ? apart + i - V : i)] = v;
-                    sums[j][i] = 0.0f;
+                for (int k = 0; k < Form::kPacks; ++k) {
+                    const uint64_t one = u[j].one[k], two = u[j].two[k];
+                    u[j].one[k] = fma2(one, cosine[j].one[k], mul2(two, sine[j].one[k]));
+                    u[j].two[k] = fma2(two, cosine[j].one[k], mul2(one, minus2(sine[j].one[k])));
                 }
-        };
-        Raw x_now[U], dy_now[U], x_next[U], dy_next[U];
-        auto load = [&](Raw (&raw_x)[U], Raw (&raw_dy)[U], int head, int local) {
-            const bool live = head < heads && local < tokens;
-            const int at = live ? local : 0;
-            const T* from_x = x + (head0 + head) * s.x_stride[1] + places[0][at];
-            const T* from_dy = dy + (head0 + head) * s.dy_stride[1] + places[1][at];
+            }
+            add_unit<Form>(v[j], u[j], gain[j], squares2, product2);
+        }
+        float squares = sum2(squares2), product = sum2(product2);
+        for (int o = 1; o < lanes; o <<= 1) {
+            squares += __shfl_xor_sync(0xffffffffu, squares, o);
+            product += __shfl_xor_sync(0xffffffffu, product, o);
+        }
+        const float r = live ? inverse_root<T>(__fmaf_rn(squares, a.inverse_d, a.epsilon)) : 0.0f;
+        const float along = r * r * (product * a.inverse_d);
 #pragma unroll
-            for (int j = 0; j < U; ++j) {
-                raw_x[j].load(from_x + channel[j], apart, live && there[j], turns[j]);
-                raw_dy[j].load(from_dy + channel[j], apart, live && there[j], turns[j]);
+        for (int j = 0; j < U; ++j) {
+            finish_unit<Form>(v[j], u[j], gain[j], r, along, sums[j]);
+            if (live && share.there[j]) Raw::store(to + share.channel[j], apart, share.turns[j], u[j]);
+        }
+    };
+    if constexpr (PER_HEAD) {
+        if (threadIdx.x < tokens) {
+            const TokenPlaces of(a, s, token0 + static_cast<int>(threadIdx.x));
+            places[0][threadIdx.x] = of.x;
+            places[1][threadIdx.x] = of.dy;
+            places[2][threadIdx.x] = of.out;
+        }
+        chain_begin();
+        fill_angles<Form, sizeof(T) == 4>(a, angles, token0, tokens);
+        __syncthreads();
+        int head = warp, base = 0, ahead = warp, ahead_base = 0;   // at hand, and the next to be fetched
+        auto fetch = [&] {
+            const int local = ahead_base + group;
+            const bool wanted = ahead < heads && local < tokens;
+            const int at = wanted ? local : 0;
+            fill(x + ahead * s.x_stride[1] + places[0][at], dy + ahead * s.dy_stride[1] + places[1][at], wanted);
+            if ((ahead_base += groups) >= tokens) {
+                ahead_base = 0;
+                ahead += kNormWarps;
             }
         };
-        int head = warp, base = 0;
-        load(x_now, dy_now, head, group);
+#pragma unroll
+        for (int i = 0; i + 1 < kGradientStages<T>; ++i) fetch();
         bool fresh = true;
         while (head < heads) {
-            const int local = base + group;
-            const bool last = base + groups >= tokens;
-            const int next_head = last ? head + kNormWarps : head, next_base = last ? 0 : base + groups;
-            load(x_next, dy_next, next_head, next_base + group);
-            if (fresh) {
+            const int local = min(base + group, tokens - 1);
+            const bool live = base + group < tokens, last = base + groups >= tokens;
+            ring.take(rows);
+            fetch();
+            if (fresh) take_gains(s.gain_head ? head0 + head : 0);
+            fresh = last && s.gain_head != 0;
+            row(dx + head * s.out_stride[1] + places[2][local], angles + local * 2 * a.half, live);
+            if (last && sums_wanted) put_sums<Form, U, V>(a, share, sums, s.partial + (static_cast<int64_t>(tile) * s.heads + head0 + head) * a.d);
+            if (last) {
 #pragma unroll
-                for (int j = 0; j < U; ++j) load_gains<Form>(a, s, s.gain_head ? head0 + head : 0, channel[j], there[j], turns[j], apart, V, gain[j]);
-                fresh = false;
+                for (int j = 0; j < U; ++j) sums[j] = Values<Form::kPacks>{};
             }
-            const bool live = local < tokens;
-            float v[U][Form::kValues], u[U][Form::kValues], squares = 0.0f, product = 0.0f;
-#pragma unroll
-            for (int j = 0; j < U; ++j) {
-                x_now[j].values(v[j]);
-                dy_now[j].values(u[j]);
-                if (turns[j] && live) turn_unit<Form, true>(a, angles, local * a.pitch + lane + j * lanes, u[j]);
-#pragma unroll
-                for (int i = 0; i < Form::kValues; ++i) {
-                    squares = __fmaf_rn(v[j][i], v[j][i], squares);
-                    product = __fmaf_rn(u[j][i] * gain[j][i], v[j][i], product);
-                }
+            base += groups;
+            if (last) {
+                base = 0;
+                head += kNormWarps;
             }
-            for (int o = 1; o < lanes; o <<= 1) {
-                squares += __shfl_xor_sync(0xffffffffu, squares, o);
-                product += __shfl_xor_sync(0xffffffffu, product, o);
-            }
-            const float r = live ? rsqrtf(__fmaf_rn(squares, a.inverse_d, a.epsilon)) : 0.0f;
-            const float along = r * r * (product * a.inverse_d);
-#pragma unroll
-            for (int j = 0; j < U; ++j) {
-                float out[Form::kValues];
-#pragma unroll
-                for (int i = 0; i < Form::kValues; ++i) {
-                    sums[j][i] = __fmaf_rn(u[j][i], v[j][i] * r, sums[j][i]);
-                    out[i] = r * __fmaf_rn(-v[j][i], along, u[j][i] * gain[j][i]);
-                }
-                if (live && there[j]) Raw::store(dx + (head0 + head) * s.out_stride[1] + places[2][local] + channel[j], apart, turns[j], out);
-                x_now[j] = x_next[j];
-                dy_now[j] = dy_next[j];
-            }
-            if (last && s.per_head && sums_wanted) put_sums(of_tile + (head0 + head) * a.d);
-            if (last && s.gain_head) fresh = true;
-            head = next_head;
-            base = next_base;
         }
-        if (s.per_head || !sums_wanted) return;
-        __syncthreads();   // (the angles are not needed any more)
-        float* meeting = reinterpret_cast<float*>(angles);
-        put_sums(meeting + warp * a.d);
-        __syncthreads();
-        for (int c = threadIdx.x; c < a.d; c += kNormThreads) {
-            float sum = meeting[c];
-#pragma unroll
-            for (int w = 1; w < kNormWarps; ++w) sum += meeting[w * a.d + c];
-            of_tile[c] = sum;
-        }
+        ring.drain();
     } else {
-        float* meeting = reinterpret_cast<float*>(angles + (a.pitch << a.token_shift));
-        float* sums = meeting + warp * a.d;   // (a lane's channels are its own)
-        for (int c = threadIdx.x & 31; c < a.d; c += 32) sums[c] = 0.0f;
-        __syncwarp();
-        for (int head = warp; head < heads; head += kNormWarps) {
-            for (int local = 0; local < tokens; ++local) {
-                const T* from_x = x + (head0 + head) * s.x_stride[1] + places[0][local];
-                const T* from_dy = dy + (head0 + head) * s.dy_stride[1] + places[1][local];
-                T* to = dx + (head0 + head) * s.out_stride[1] + places[2][local];
-                float r = 0.0f, along = 0.0f, squares = 0.0f, product = 0.0f;
-                for (int pass = 0; pass < 2; ++pass) {
-                    for (int unit = lane; unit < a.units; unit += 32) {
-                        const bool turns = unit < a.turning;
-                        const int channel = Form::channel(a, unit);
-                        Raw raw_x, raw_dy;
-                        float v[Form::kValues], u[Form::kValues], gain[Form::kValues];
-                        raw_x.load(from_x + channel, apart, true, turns);
-                        raw_dy.load(from_dy + channel, apart, true, turns);
-                        raw_x.values(v);
-                        raw_dy.values(u);
-                        load_gains<Form>(a, s, s.gain_head ? head0 + head : 0, channel, true, turns, apart, V, gain);
-                        if (turns) turn_unit<Form, true>(a, angles, local * a.pitch + unit, u);
-                        if (pass == 0) {
+        const int local = group & mask, step = groups >> a.token_shift;   // (no more tokens than groups)
+        const bool live = local < tokens;
+        const TokenPlaces of(a, s, token0 + (live ? local : 0));
+        int head = group >> a.token_shift;
+        x += of.x + head * s.x_stride[1];
+        dy += of.dy + head * s.dy_stride[1];
+        dx += of.out + head * s.out_stride[1];
+        const int64_t x_step = step * s.x_stride[1], dy_step = step * s.dy_stride[1], dx_step = step * s.out_stride[1];
+        chain_begin();
 #pragma unroll
-                            for (int i = 0; i < Form::kValues; ++i) {
-                                squares = __fmaf_rn(v[i], v[i], squares);
-                                product = __fmaf_rn(u[i] * gain[i], v[i], product);
-                            }
-                        } else {
+        for (int i = 0; i + 1 < kGradientStages<T>; ++i) fill(x + i * x_step, dy + i * dy_step, live && head + i * step < heads);   // (on their way while the angles are worked out)
+        fill_angles<Form, sizeof(T) == 4>(a, angles, token0, tokens);
+        __syncthreads();
 #pragma unroll
-                            for (int i = 0; i < Form::kValues; ++i) {
-                                const bool second = Form::kTwo && i >= V;
-                                if (!second || turns) {
-                                    float& sum = sums[channel + (second ? apart + i - V : i)];
-                                    sum = __fmaf_rn(u[i], v[i] * r, sum);
-                                }
-                                u[i] = r * __fmaf_rn(-v[i], along, u[i] * gain[i]);
-                            }
-                            Raw::store(to + channel, apart, turns, u);
-                        }
-                    }
-                    if (pass == 0) {
-                        r = rsqrtf(__fmaf_rn(sum_over(squares, 32), a.inverse_d, a.epsilon));
-                        along = r * r * (sum_over(product, 32) * a.inverse_d);
-                    }
-                }
+        for (int j = 0; j < U; ++j) {
+#pragma unroll
+            for (int k = 0; k < Form::kPacks; ++k) {
+                cosine[j].one[k] = pack2(1.0f, 1.0f);
+                sine[j].one[k] = 0;
             }
-            if (s.per_head && sums_wanted) {
-                __syncwarp();
-                for (int c = threadIdx.x & 31; c < a.d; c += 32) {
-                    of_tile[(head0 + head) * static_cast<int64_t>(a.d) + c] = sums[c];
-                    sums[c] = 0.0f;
-                }
-                __syncwarp();
-            }
+            if (!share.turns[j]) continue;
+            const float* table = angles + local * 2 * a.half;
+            const int place = angle_place<Form>(a, share.unit[j], 0), stride = a.turning * Form::kQuad;
+            get_angles<Form>(table, place, stride, cosine[j].one);
+            get_angles<Form>(table + a.half, place, stride, sine[j].one);
         }
-        if (s.per_head || !sums_wanted) return;
+        if (!s.gain_head) take_gains(0);
+        while (__any_sync(0xffffffffu, head < heads)) {
+            if (s.gain_head) take_gains(head0 + min(head, heads - 1));
+            ring.take(rows);
+            fill(x + (kGradientStages<T> - 1) * x_step, dy + (kGradientStages<T> - 1) * dy_step, live && head + (kGradientStages<T> - 1) * step < heads);
+            row(dx, nullptr, live && head < heads);
+            head += step;
+            x += x_step;
+            dy += dy_step;
+            dx += dx_step;
+        }
+        ring.drain();
+        if (!sums_wanted) return;
+        __syncthreads();   // (the angles and rows are not needed any more)
+        put_sums<Form, U, V>(a, share, sums, angles + warp * a.d);
         __syncthreads();
         for (int c = threadIdx.x; c < a.d; c += kNormThreads) {
-            float sum = meeting[c];
+            float sum = angles[c];
 #pragma unroll
-            for (int w = 1; w < kNormWarps; ++w) sum += meeting[w * a.d + c];
-            of_tile[c] = sum;
+            for (int w = 1; w < kNormWarps; ++w) sum += angles[w * a.d + c];
+            s.partial[(static_cast<int64_t>(tile) * runs + run) * a.d + c] = sum;
         }
+    }
+}
+
+// Single values, and rows longer than a warp's registers: a row is a whole warp's and read a second time (from the caches); sums of dgain are in shared memory.
+template <typename T, int V, bool INTERLEAVED>
+__global__ void __launch_bounds__(kNormThreads)
+head_norm_grad_long_kernel(const __grid_constant__ NormArgs a) {
+    using Form = NormUnit<T, V, INTERLEAVED>;
+    using Raw = RawUnit<T, V, INTERLEAVED>;
+    extern __shared__ __align__(16) float angles[];                   // the table, and each warp's sums behind it
+    const int tile = static_cast<int>(blockIdx.x), token0 = tile << a.token_shift, tokens = min(a.tokens - token0, 1 << a.token_shift);
+    const bool second_side = static_cast<int>(blockIdx.y) >= a.first_side;
+    const NormSide& s = a.side[second_side];
+    const int run = static_cast<int>(blockIdx.y) - (second_side ? a.first_side : 0), runs = second_side ? static_cast<int>(gridDim.y) - a.first_side : a.first_side;
+    const int head0 = run * a.heads_per_cta, heads = min(a.heads_per_cta, s.heads - head0);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, apart = Form::apart(a);
+    const bool sums_wanted = s.partial != nullptr;
+    chain_begin();
+    fill_angles<Form, sizeof(T) == 4>(a, angles, token0, tokens);
+    __syncthreads();
+    float* meeting = angles + ((2 * a.half) << a.token_shift);
+    float* sums = meeting + warp * a.d;   // (a lane's channels are its own)
+    for (int c = lane; c < a.d; c += 32) sums[c] = 0.0f;
+    __syncwarp();
+    for (int head = warp; head < heads; head += kNormWarps) {
+        for (int local = 0; local < tokens; ++local) {
+            const TokenPlaces of(a, s, token0 + local);
+            const T* from_x = static_cast<const T*>(s.x) + (head0 + head) * s.x_stride[1] + of.x;
+            const T* from_dy = static_cast<const T*>(s.dy) + (head0 + head) * s.dy_stride[1] + of.dy;
+            T* to = static_cast<T*>(s.out) + (head0 + head) * s.out_stride[1] + of.out;
+            float r = 0.0f, along = 0.0f;
+            uint64_t squares = 0, product = 0;
+            for (int pass = 0; pass < 2; ++pass) {
+                for (int unit = lane; unit < a.units; unit += 32) {
+                    const bool turns = unit < a.turning;
+                    const int channel = Form::channel(a, unit);
+                    Raw raw_x, raw_dy;
+                    raw_x.load(from_x + channel, apart, true, turns);
+                    raw_dy.load(from_dy + channel, apart, true, turns);
+                    const Values<Form::kPacks> v = raw_x.values();
+                    Values<Form::kPacks> u = raw_dy.values(), gain, terms{};
+                    load_gains<Form, V>(a, s, s.gain_head ? head0 + head : 0, channel, true, turns, gain);
+                    if (turns) turn_unit<Form, true>(a, angles + local * 2 * a.half, unit, u);
+                    if (pass == 0) {
+                        add_unit<Form>(v, u, gain, squares, product);
+                        continue;
+                    }
+                    finish_unit<Form>(v, u, gain, r, along, terms);
+                    Raw::store(to + channel, apart, turns, u);
+#pragma unroll
+                    for (int k = 0; k < Form::kPacks; ++k) {
+                        float term[2][2];
+                        unpack2(terms.one[k], term[0][0], term[0][1]);
+                        unpack2(terms.two[k], term[1][0], term[1][1]);
+#pragma unroll
+                        for (int second = 0; second < 2; ++second)
+#pragma unroll
+                            for (int half = 0; half < 2; ++half)
+                                if ((!second || !Form::kTwo || turns) && (V > 1 || half == 0)) sums[channel + (second && Form::kTwo ? apart : 0) + Form::place(k, half, second != 0)] += term[second][half];
+                    }
+                }
+                if (pass == 0) {
+                    r = inverse_root<T>(__fmaf_rn(sum_over(sum2(squares), 32), a.inverse_d, a.epsilon));
+                    along = r * r * (sum_over(sum2(product), 32) * a.inverse_d);
+                }
+            }
+        }
+        if (s.per_head && sums_wanted) {
+            __syncwarp();
+            for (int c = lane; c < a.d; c += 32) {
+                s.partial[(static_cast<int64_t>(tile) * s.heads + head0 + head) * a.d + c] = sums[c];
+                sums[c] = 0.0f;
+            }
+            __syncwarp();
+        }
+    }
+    if (s.per_head || !sums_wanted) return;
+    __syncthreads();
+    for (int c = threadIdx.x; c < a.d; c += kNormThreads) {
+        float sum = meeting[c];
+#pragma unroll
+        for (int w = 1; w < kNormWarps; ++w) sum += meeting[w * a.d + c];
+        s.partial[(static_cast<int64_t>(tile) * runs + run) * a.d + c] = sum;
     }
 }
 
@@ -450,25 +766,31 @@ struct GainArgs {
     GainSide side[2];
     int32_t first_blocks;
 };
+// 16 columns a CTA, 64 rows at a time: what bounds it is the latency of a thread's loads, which are few and all on their way at once.
+constexpr int kGainColumns = 16;
 __global__ void __launch_bounds__(1024)
-gain_sums_kernel(const GainArgs a) {
+gain_sums_kernel(const __grid_constant__ GainArgs a) {
+    __shared__ double sums[32][kGainColumns];
+    const int which = static_cast<int>(blockIdx.x) >= a.first_blocks;
+    const GainSide& s = a.side[which];
+    const int tx = threadIdx.x % kGainColumns, ty = threadIdx.x / kGainColumns;
+    const int64_t column = (static_cast<int64_t>(blockIdx.x) - (which ? a.first_blocks : 0)) * kGainColumns + tx;
     chain_begin();
-    __shared__ double sums[32][33];
-    const bool second = static_cast<int>(blockIdx.x) >= a.first_blocks;
-    const GainSide& s = second ? a.side[1] : a.side[0];
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const int64_t column = (static_cast<int64_t>(blockIdx.x) - (second ? a.first_blocks : 0)) * 32 + tx;
     double sum = 0.0;
     if (column < s.columns) {
         const float* from = s.partial + column;
 #pragma unroll 8
-        for (int64_t row = ty; row < s.rows; row += 32) sum += static_cast<double>(from[row * s.columns]);
+        for (int64_t row = ty; row < s.rows; row += 1024 / kGainColumns) sum += static_cast<double>(from[row * s.columns]);
     }
-    sums[ty][tx] = sum;
+    sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+    if ((threadIdx.x & 16) == 0) sums[threadIdx.x >> 5][tx] = sum;
     __syncthreads();
-    if (ty != 0 || column >= s.columns) return;
+    if (threadIdx.x >= 32) return;
+    sum = 0.0;
 #pragma unroll
-    for (int i = 1; i < 32; ++i) sum += sums[i][tx];
+    for (int i = 0; i < 16; ++i) sum += sums[(threadIdx.x >> 4) * 16 + i][tx];
+    sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+    if (threadIdx.x >= 16 || column >= s.columns) return;
     const int64_t head = column / s.d;
     store_from_f32(s.out, s.type, head * s.out_head + (column - head * s.d), static_cast<float>(sum));
 }
@@ -572,7 +894,21 @@ int check_norm(NormProblem& p) {
     return kOk;
 }
 
-// Units a lane and lanes a row, the table, and the strides; `pointers`: of row[side][tensor], `positions` and `frequencies`.
+// As few lanes as hold a row, 16 values each; single values (width 1) and rows beyond a warp: a warp a row, read twice (per_lane 0).
+struct LaneForm {
+    int turning, units, per_lane, group_shift;
+};
+LaneForm lane_form(const NormProblem& p, int width) {
+    const int half = p.positions->rank ? static_cast<int>(p.frequencies->dim[3]) : 0, d = static_cast<int>(p.row[0][0]->dim[3]);
+    const int pairs = p.interleaved && width > 1 ? width / 2 : width;   // of a unit
+    LaneForm form{half / pairs, half / pairs + (d - 2 * half) / width, width == 1 ? 0 : 8 / pairs, 5};
+    if (form.units > 32 * form.per_lane) form.per_lane = 0;
+    if (form.per_lane)
+        for (form.group_shift = 0; (form.per_lane << form.group_shift) < form.units;) ++form.group_shift;
+    return form;
+}
+
+// The table, lanes and strides; `pointers`: of row[side][tensor], `positions` and `frequencies`.
 int build_norm(NormProblem& p, void* const (&pointers)[2][3], const void* positions, const void* frequencies, const void* const (&gains)[2], NormArgs& a, int& per_lane) {
     const dfgpu_tensor& x = *p.row[0][0];
     const int bytes = dtype_bytes(x.dtype), sides = p.two ? 2 : 1;
@@ -633,11 +969,12 @@ int build_norm(NormProblem& p, void* const (&pointers)[2][3], const void* positi
         side.gain_head = p.gain[s]->rank && p.gain[s]->dim[1] > 1 ? p.gain[s]->stride[1] : 0;
     }
     const int64_t d = x.dim[3];
-    const int pairs = p.interleaved && p.width > 1 ? p.width / 2 : p.width;   // of a unit
+    const LaneForm form = lane_form(p, p.width);
     a.d = static_cast<int>(d);
-    a.turning = a.half / pairs;
-    a.units = a.turning + (a.d - 2 * a.half) / p.width;
-    a.pitch = a.half + a.turning;   // (eight units of a token and the next token's do not meet in the same banks)
+    a.turning = form.turning;
+    a.units = form.units;
+    a.group_shift = form.group_shift;
+    per_lane = form.per_lane;
     a.seq = static_cast<int>(x.dim[2]);
     a.tokens = static_cast<int>(x.dim[0] * x.dim[2]);
     a.by_seq = make_fast_divisor(static_cast<uint32_t>(a.seq));
@@ -645,75 +982,80 @@ int build_norm(NormProblem& p, void* const (&pointers)[2][3], const void* positi
     a.epsilon = p.epsilon;
     a.gain_offset = p.gain_offset;
     a.inverse_d = static_cast<float>(1.0 / static_cast<double>(d));
-    // One unit a lane up to a warp's 32, two beyond; single values (V = 1) and longer rows: a warp a row, read twice.
-    per_lane = p.width == 1 || a.units > 64 ? 0 : (a.units > 32 ? 2 : 1);
-    a.group_shift = 5;
-    if (per_lane == 1)
-        for (a.group_shift = 0; (1 << a.group_shift) < a.units;) ++a.group_shift;
     return kOk;
 }
 
-template <bool GRAD, typename T, int V, bool INTERLEAVED, int U>
-void launch_norm(const NormArgs& a, dim3 grid, size_t shared, cudaStream_t stream) {
-    if constexpr (GRAD) {
-        launch_chained(head_norm_grad_kernel<T, V, INTERLEAVED, U>, grid, dim3(kNormThreads), shared, stream, a);
-    } else {
-        launch_chained(head_norm_kernel<T, V, INTERLEAVED, U>, grid, dim3(kNormThreads), shared, stream, a);
-    }
+// 16 values a thread (Ring::kBytes).
+size_t ring_bytes(const NormProblem& p, bool gradient) {
+    const int bytes = dtype_bytes(p.row[0][0]->dtype), stages = bytes == 4 ? (gradient ? 2 * kGradientStages<float> : kForwardStages<float>) : (gradient ? 2 * kGradientStages<__half> : kForwardStages<__half>);
+    return static_cast<size_t>(16 * bytes) * stages * kNormThreads;
 }
-template <bool GRAD, typename T, int V>
-void launch_norm(const NormArgs& a, bool interleaved, int per_lane, dim3 grid, size_t shared, cudaStream_t stream) {
+
+enum NormKernel { kForward, kForwardLong, kGradient, kGradientOfHeads, kGradientLong };
+template <typename T, int V, bool INTERLEAVED>
+void launch_norm(NormKernel kernel, const NormArgs& a, dim3 grid, size_t shared, cudaStream_t stream) {
+    void (*function)(const NormArgs) = head_norm_long_kernel<T, V, INTERLEAVED>;
+    if (kernel == kGradientLong) function = head_norm_grad_long_kernel<T, V, INTERLEAVED>;
     if constexpr (V > 1) {
-        if (per_lane == 1) return interleaved ? launch_norm<GRAD, T, V, true, 1>(a, grid, shared, stream) : launch_norm<GRAD, T, V, false, 1>(a, grid, shared, stream);
-        if (per_lane == 2) return interleaved ? launch_norm<GRAD, T, V, true, 2>(a, grid, shared, stream) : launch_norm<GRAD, T, V, false, 2>(a, grid, shared, stream);
+        if (kernel == kForward) function = head_norm_kernel<T, V, INTERLEAVED>;
+        if (kernel == kGradient) function = head_norm_grad_kernel<T, V, INTERLEAVED, false>;
+        if (kernel == kGradientOfHeads) function = head_norm_grad_kernel<T, V, INTERLEAVED, true>;
     }
-    interleaved ? launch_norm<GRAD, T, V, true, 0>(a, grid, shared, stream) : launch_norm<GRAD, T, V, false, 0>(a, grid, shared, stream);
+    launch_chained(function, grid, dim3(kNormThreads), shared, stream, a);
 }
-template <bool GRAD>
-void launch_norm(const NormArgs& a, int dtype, int width, bool interleaved, int per_lane, dim3 grid, size_t shared, cudaStream_t stream) {
+template <typename T, int V>
+void launch_norm(NormKernel kernel, const NormArgs& a, bool interleaved, dim3 grid, size_t shared, cudaStream_t stream) {
+    interleaved ? launch_norm<T, V, true>(kernel, a, grid, shared, stream) : launch_norm<T, V, false>(kernel, a, grid, shared, stream);
+}
+void launch_norm(NormKernel kernel, const NormArgs& a, int dtype, int width, bool interleaved, dim3 grid, size_t shared, cudaStream_t stream) {
     if (dtype == DFGPU_F32) {
-        if (width == 4) launch_norm<GRAD, float, 4>(a, interleaved, per_lane, grid, shared, stream);
-        else launch_norm<GRAD, float, 1>(a, interleaved, per_lane, grid, shared, stream);
+        if (width == 4) launch_norm<float, 4>(kernel, a, interleaved, grid, shared, stream);
+        else launch_norm<float, 1>(kernel, a, interleaved, grid, shared, stream);
     } else if (dtype == DFGPU_F16) {
-        if (width == 8) launch_norm<GRAD, __half, 8>(a, interleaved, per_lane, grid, shared, stream);
-        else if (width == 4) launch_norm<GRAD, __half, 4>(a, interleaved, per_lane, grid, shared, stream);
-        else launch_norm<GRAD, __half, 1>(a, interleaved, per_lane, grid, shared, stream);
+        if (width == 8) launch_norm<__half, 8>(kernel, a, interleaved, grid, shared, stream);
+        else if (width == 4) launch_norm<__half, 4>(kernel, a, interleaved, grid, shared, stream);
+        else launch_norm<__half, 1>(kernel, a, interleaved, grid, shared, stream);
     } else {
-        if (width == 8) launch_norm<GRAD, __nv_bfloat16, 8>(a, interleaved, per_lane, grid, shared, stream);
-        else if (width == 4) launch_norm<GRAD, __nv_bfloat16, 4>(a, interleaved, per_lane, grid, shared, stream);
-        else launch_norm<GRAD, __nv_bfloat16, 1>(a, interleaved, per_lane, grid, shared, stream);
+        if (width == 8) launch_norm<__nv_bfloat16, 8>(kernel, a, interleaved, grid, shared, stream);
+        else if (width == 4) launch_norm<__nv_bfloat16, 4>(kernel, a, interleaved, grid, shared, stream);
+        else launch_norm<__nv_bfloat16, 1>(kernel, a, interleaved, grid, shared, stream);
     }
 }
 
-// The gradient's cut: tokens a CTA (1 << shift) and heads a run. A function of the descriptors alone (the scratch depends on it): of the pitch of the widest
-// and of the scalar form alike, whichever the pointers allow.
+// The gradient's cut: tokens a CTA (1 << shift) and heads a run. A function of the descriptors alone: the scratch depends on it.
 struct GradCut {
     int shift, heads_per_cta;
     int64_t tiles, runs[2];
 };
+bool sums_of_heads(const dfgpu_tensor& dgain) { return dgain.rank && dgain.dim[1] > 1; }
+bool any_sums_of_heads(const NormProblem& p) { return sums_of_heads(*p.dgain[0]) || (p.two && sums_of_heads(*p.dgain[1])); }
 GradCut grad_cut(const NormProblem& p) {
     const dfgpu_tensor& x = *p.row[0][0];
-    const int64_t half = p.positions->rank ? p.frequencies->dim[3] : 0, pitch = 2 * half;   // (the largest: V = 1)
+    const int64_t half = p.positions->rank ? p.frequencies->dim[3] : 0;
     const int64_t tokens = x.dim[0] * x.dim[2], heads[2] = {x.dim[1], p.two ? p.row[1][0]->dim[1] : 0};
     GradCut cut{};
+    // With sums for each head 32 tokens, so that few sums go out; otherwise as many as there are groups of lanes.
     cut.shift = 5;
-    while (cut.shift > 0 && (8 * (pitch << cut.shift) + 16 * x.dim[3] > kNormShared)) --cut.shift;
-    cut.heads_per_cta = 16;
+    if (!any_sums_of_heads(p)) {
+        const LaneForm form = lane_form(p, p.width);
+        cut.shift = std::min(7 - form.group_shift, 5);
+    }
+    while (cut.shift > 0 && 8 * (half << cut.shift) > (dtype_bytes(x.dtype) == 4 ? kNormShared : kNormSharedOfSixteen)) --cut.shift;
+    cut.heads_per_cta = 32;
     auto ctas = [&] {
         cut.tiles = (tokens + (1ll << cut.shift) - 1) >> cut.shift;
         for (int s = 0; s < 2; ++s) cut.runs[s] = (heads[s] + cut.heads_per_cta - 1) / cut.heads_per_cta;
         return cut.tiles * (cut.runs[0] + cut.runs[1]);
     };
-    while (ctas() < 4 * 148 && cut.heads_per_cta > 4) cut.heads_per_cta /= 2;
+    while (ctas() < 6 * 148 && cut.heads_per_cta > 4) cut.heads_per_cta /= 2;
     while (ctas() < 4 * 148 && cut.shift > 2) --cut.shift;
     ctas();
     return cut;
 }
-bool sums_of_heads(const dfgpu_tensor& dgain) { return dgain.dim[1] > 1; }
 // Floats of partial sums of a side, none where no dgain is wanted.
 int64_t grad_partials(const NormProblem& p, const GradCut& cut, int s) {
     if ((s == 1 && !p.two) || p.dgain[s]->rank == 0) return 0;
-    return cut.tiles * p.row[s][0]->dim[3] * (sums_of_heads(*p.dgain[s]) ? p.row[s][0]->dim[1] : cut.runs[s]);
+    return cut.tiles * p.row[s][0]->dim[3] * (any_sums_of_heads(p) ? p.row[s][0]->dim[1] : cut.runs[s]);
 }
 
 }  // namespace
@@ -744,16 +1086,18 @@ extern "C" int dfgpu_head_norm(const dfgpu_head_norm_params* params, void* const
     const void* const gains[2] = {p.gain[0]->rank ? tensors[2] : nullptr, p.gain[1]->rank ? tensors[7] : nullptr};
     status = build_norm(p, rows, p.positions->rank ? tensors[3] : nullptr, p.positions->rank ? tensors[4] : nullptr, gains, a, per_lane);
     if (status) return status;
-    // Up to eight tokens a CTA, so that a long run of heads shares each token's sines; then as few heads as give each thread eight units.
-    while (a.token_shift < 3 && (1 << a.token_shift) < a.seq && (a.pitch << (a.token_shift + 1)) <= kNormTable) ++a.token_shift;
+    // A token a group of lanes (where the heads are to be shared out, several groups) and all heads, which share the tokens' angles; fewer heads where the CTAs would be few.
+    const int heads = a.side[0].heads + a.side[1].heads, groups = kNormThreads >> a.group_shift;
+    while (a.token_shift < 4 && (2 << a.token_shift) <= groups && (1 << a.token_shift) < a.seq && (a.half << (a.token_shift + 1)) <= kNormTable) ++a.token_shift;
     a.tiles = (a.seq + (1 << a.token_shift) - 1) >> a.token_shift;
     a.by_tiles = make_fast_divisor(static_cast<uint32_t>(a.tiles));
     const int64_t tiles = p.row[0][0]->dim[0] * a.tiles;
-    a.heads_per_cta = std::min(std::max(a.side[0].heads, a.side[1].heads), (8 * kNormThreads - 1) / (a.units << a.token_shift) + 1);
-    a.first_side = (a.side[0].heads + a.heads_per_cta - 1) / a.heads_per_cta;
-    const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(a.first_side + (a.side[1].heads + a.heads_per_cta - 1) / a.heads_per_cta));
-    const size_t shared = sizeof(float2) * static_cast<size_t>(a.pitch << a.token_shift);
-    launch_norm<false>(a, p.row[0][0]->dtype, p.width, p.interleaved != 0, per_lane, grid, shared, as_stream(stream));
+    a.heads_per_cta = heads;
+    auto runs = [&] { return (heads + a.heads_per_cta - 1) / a.heads_per_cta; };
+    while (tiles * runs() < 8 * 148 && (a.heads_per_cta << a.token_shift) > groups && a.heads_per_cta > 1) a.heads_per_cta = (a.heads_per_cta + 1) / 2;
+    const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(runs()));
+    const size_t shared = sizeof(float) * static_cast<size_t>((2 * a.half) << a.token_shift) + (per_lane ? ring_bytes(p, false) : 0);
+    launch_norm(per_lane ? kForward : kForwardLong, a, p.row[0][0]->dtype, p.width, p.interleaved != 0, grid, shared, as_stream(stream));
     return check_launch("HEAD_NORM");
 }
 
@@ -801,16 +1145,17 @@ extern "C" int dfgpu_head_norm_grad(const dfgpu_head_norm_grad_params* params, v
         }
         NormSide& side = a.side[s];
         side.partial = static_cast<float*>(scratch) + (s ? first_partials : 0);
-        side.per_head = sums_of_heads(dgain);
+        side.per_head = any_sums_of_heads(p);
+        const bool apart = sums_of_heads(dgain);   // (where only the other side's are, a side's heads meet in the second kernel)
         GainSide& sums = g.side[s];
         sums.partial = side.partial;
         sums.out = out;
         sums.d = a.d;
-        sums.rows = cut.tiles * (side.per_head ? 1 : cut.runs[s]);
-        sums.columns = side.per_head ? static_cast<int64_t>(side.heads) * a.d : a.d;
-        sums.out_head = side.per_head ? dgain.stride[1] : 0;
+        sums.rows = cut.tiles * (apart ? 1 : side.per_head ? side.heads : cut.runs[s]);
+        sums.columns = apart ? static_cast<int64_t>(side.heads) * a.d : a.d;
+        sums.out_head = apart ? dgain.stride[1] : 0;
         sums.type = dgain.dtype;
-        const int more = static_cast<int>((sums.columns + 31) / 32);
+        const int more = static_cast<int>((sums.columns + kGainColumns - 1) / kGainColumns);
         if (s == 0) g.first_blocks = more;
         blocks += more;
     }
@@ -818,8 +1163,13 @@ extern "C" int dfgpu_head_norm_grad(const dfgpu_head_norm_grad_params* params, v
     a.heads_per_cta = cut.heads_per_cta;
     a.first_side = static_cast<int>(cut.runs[0]);
     const dim3 grid(static_cast<unsigned>(cut.tiles), static_cast<unsigned>(cut.runs[0] + cut.runs[1]));
-    const size_t table = sizeof(float2) * static_cast<size_t>(a.pitch << a.token_shift), meeting = sizeof(float) * kNormWarps * static_cast<size_t>(a.d);
-    launch_norm<true>(a, p.row[0][0]->dtype, p.width, p.interleaved != 0, per_lane, grid, per_lane ? std::max(table, meeting) : table + meeting, as_stream(stream));
+    const size_t table = sizeof(float) * static_cast<size_t>((2 * a.half) << a.token_shift), meeting = sizeof(float) * kNormWarps * static_cast<size_t>(a.d);
+    // (the form for tokens a group needs as many groups as tokens; with narrower vectors than the cut had in mind a row may take more lanes)
+    const bool of_heads = any_sums_of_heads(p);
+    if (per_lane && !of_heads && (kNormThreads >> a.group_shift) < (1 << a.token_shift)) per_lane = 0;
+    launch_norm(!per_lane ? kGradientLong : of_heads ? kGradientOfHeads : kGradient, a, p.row[0][0]->dtype, p.width, p.interleaved != 0, grid,
+                per_lane ? std::max(table + ring_bytes(p, true), meeting) : table + meeting,
+                                as_stream(stream));
     status = check_launch("HEAD_NORM gradient");
     if (status || !blocks) return status;
     launch_chained(gain_sums_kernel, dim3(static_cast<unsigned>(blocks)), dim3(1024), 0, as_stream(stream), g);

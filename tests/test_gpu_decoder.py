@@ -245,6 +245,19 @@ def test_head_norm_gradient_against_differences():
     assert abs((values[0] - values[1]).sum() / (2 * h) - (double(dgain) * double(eg)).sum()) <= np.abs(values[0]).sum() * 60 * U / h
 
 
+def test_head_norm_gains_of_one_side_s_heads():
+    """Queries with a gain for each head, keys with one for all, and the other way round; a side without any."""
+    for order in (1, -1):
+        heads = Heads(15, 2, 6, 3, 45, 64, 32, F32)
+        whole = Heads(15, 2, 6, 3, 45, 64, 32, F32, per_head=True)
+        heads.gain = [whole.gain[0], heads.gain[1]] if order == 1 else [heads.gain[0], whole.gain[1]]
+        heads.check_forward(heads.forward())
+        heads.check_gradient(*heads.gradient())
+        heads.gain[0] = None
+        heads.check_forward(heads.forward())
+        heads.check_gradient(*heads.gradient())
+
+
 def test_head_norm_gradient_of_many_tokens():
     """Several runs of heads and tiles of tokens; the same call twice gives the same bits."""
     heads = Heads(14, 3, 40, 8, 500, 128, 128, BF16)
