@@ -16,7 +16,7 @@ namespace {
 
 constexpr int kNormThreads = 128, kNormWarps = kNormThreads / 32;
 constexpr int kNormTable = 2048;      // (cosine, sine) pairs of a CTA, forward: 16 KiB
-constexpr int kNormShared = 14 * 1024, kNormSharedOfSixteen = 22 * 1024;   // bytes of a CTA's table, gradient: with the rows on their way within 48 KiB
+constexpr int kNormShared = 18 * 1024;   // bytes of a CTA's table, gradient: with the rows on their way within 48 KiB
 constexpr int64_t kNormMaxD = 1024;
 
 struct NormSide {
@@ -68,7 +68,7 @@ template <typename T, int V, bool INTERLEAVED>
 struct NormUnit {
     static constexpr bool kTwo = !INTERLEAVED || V == 1;
     static constexpr int kPairs = kTwo ? V : V / 2, kPacks = (kPairs + 1) / 2, kQuad = kPairs < 4 ? kPairs : 4;
-    static constexpr int kPerLane = V == 1 ? 0 : 8 / kPairs;   // units that hold 16 values
+    static constexpr int kPerLane = V == 1 ? 0 : (16 / static_cast<int>(sizeof(T))) / kPairs;   // units that hold 32 bytes
     static __device__ __forceinline__ int channel(const NormArgs& a, int unit) {
         return unit < a.turning ? (INTERLEAVED ? unit * (V == 1 ? 2 : V) : unit * V) : 2 * a.half + (unit - a.turning) * V;
     }
@@ -158,15 +158,57 @@ __device__ __forceinline__ void load_gains(const NormArgs& a, const NormSide& s,
         gain.two[k] = pack2(g[1][0], g[1][1]);
     }
 }
+// A gain that all heads share, as f32 in shared memory (all threads; the barrier behind the angles' is its too), and a lane's part of it.
+__device__ __forceinline__ void fill_gains(const NormArgs& a, const NormSide& s, float* to) {
+    if (s.gain_head) return;
+    for (int c = threadIdx.x; c < a.d; c += kNormThreads) to[c] = gain_at(s, a.gain_offset, c);
+}
+template <typename Form, int V>
+__device__ __forceinline__ void take_gains(const NormArgs& a, const NormSide& s, const float* shared, int head, int channel, bool live, bool turns, Values<Form::kPacks>& gain) {
+    if (s.gain_head) return load_gains<Form, V>(a, s, head, channel, live, turns, gain);
+    gain = Values<Form::kPacks>{};
+    if (!live) return;
+    const float* first = shared + channel;
+#pragma unroll
+    for (int k = 0; k < Form::kPacks; ++k) {
+        if constexpr (Form::kTwo) {
+            gain.one[k] = reinterpret_cast<const uint64_t*>(first)[k];
+            if (turns) gain.two[k] = reinterpret_cast<const uint64_t*>(first + Form::apart(a))[k];
+        } else {
+            const float4 four = reinterpret_cast<const float4*>(first)[k];
+            gain.one[k] = pack2(four.x, four.z);
+            gain.two[k] = pack2(four.y, four.w);
+        }
+    }
+}
 // The table of a token: cosines of all pairs, then sines, those of a unit's pairs in vectors of kQuad, vectors of neighbouring units side by side.
 template <typename Form>
 __device__ __forceinline__ int angle_place(const NormArgs& a, int unit, int quad) { return (quad * a.turning + unit) * Form::kQuad; }
-template <typename Form, bool CLOSE>
-__device__ __forceinline__ void put_angle(const NormArgs& a, float* table, int pair, int64_t batch, int64_t token) {
-    float2 turn = turn_of<CLOSE>(a.at, batch, token, pair);
-    const int unit = pair / Form::kPairs, within = pair - unit * Form::kPairs, place = angle_place<Form>(a, unit, within / Form::kQuad) + within % Form::kQuad;
-    table[place] = turn.x * a.scale;
-    table[a.half + place] = turn.y * a.scale;
+// A thread's part of the tables of 1 << token_shift tokens: one token's, whose position it holds, pair by pair. The angle is reduced to one turn in 64 bits. f32 rows take sine
+// and cosine of the f32 nearest to it and what that leaves out; 16-bit ones those of the special function unit, which are off by 2^-21.4, and 1.9e-7 of the angle.
+template <typename T, typename Form>
+__device__ __forceinline__ void fill_angles(const NormArgs& a, float* angles, int local, bool live, int64_t batch, int64_t token) {
+    if (!live || a.half == 0) return;
+    const int64_t at = batch * a.at.batch + token * a.at.token;
+    const double position = a.at.wide ? static_cast<double>(static_cast<const int64_t*>(a.at.positions)[at]) : static_cast<double>(static_cast<const int32_t*>(a.at.positions)[at]);
+    float* table = angles + local * 2 * a.half;
+    for (int pair = threadIdx.x >> a.token_shift; pair < a.half; pair += kNormThreads >> a.token_shift) {
+        const double turns = position * static_cast<double>(a.at.frequencies[pair * a.at.frequency_stride]) * 0.15915494309189533577;
+        const double rest = turns - rint(turns);
+        float sine, cosine;
+        if constexpr (sizeof(T) == 4) {
+            const float halves = static_cast<float>(2.0 * rest), more = 3.14159265f * static_cast<float>(2.0 * rest - static_cast<double>(halves));
+            sincospif(halves, &sine, &cosine);
+            const float first = cosine;
+            cosine = __fmaf_rn(-sine, more, cosine);
+            sine = __fmaf_rn(first, more, sine);
+        } else {
+            __sincosf(static_cast<float>(6.283185307179586 * rest), &sine, &cosine);
+        }
+        const int unit = pair / Form::kPairs, within = pair - unit * Form::kPairs, place = angle_place<Form>(a, unit, within / Form::kQuad) + within % Form::kQuad;
+        table[place] = cosine * a.scale;
+        table[a.half + place] = sine * a.scale;
+    }
 }
 template <typename Form>
 __device__ __forceinline__ void get_angles(const float* table, int place, int step, uint64_t (&out)[Form::kPacks]) {
@@ -206,7 +248,7 @@ __device__ __forceinline__ float sum_over(float v, int lanes) {
 template <typename T>
 __device__ __forceinline__ float inverse_root(float v) { return sizeof(T) == 4 ? __frsqrt_rn(v) : rsqrtf(v); }   // (the other is off by 2^-23 and a little, which 16 bits do not show)
 
-// What a lane has of every row: up to 16 values.
+// What a lane has of every row: up to 32 bytes.
 template <typename Form, int U>
 struct Share {
     int channel[U], unit[U];
@@ -263,15 +305,18 @@ struct Ring {
             }
         reading = reading + 1 == STAGES ? 0 : reading + 1;
     }
-    __device__ __forceinline__ void drain() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+    // What is still on its way is waited for and not taken.
+    __device__ __forceinline__ void drain() {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        reading = filling;
+    }
 };
-template <typename T> constexpr int kForwardStages = sizeof(T) == 4 ? 3 : 4;
-template <typename T> constexpr int kGradientStages = sizeof(T) == 4 ? 2 : 3;
+constexpr int kForwardStages = 4, kGradientStages = 3;
 
 // ---- forward: a CTA takes a few tokens of one sequence and a run of heads of both pairs of tensors, which share the tokens' angles -----------------------
 // A group of lanes has one token and walks the heads, so that the angles stay in registers, multiplied by the gains already.
 template <typename T, int V, bool INTERLEAVED>
-__global__ void __launch_bounds__(kNormThreads)
+__global__ void __launch_bounds__(kNormThreads, 6)
 head_norm_kernel(const __grid_constant__ NormArgs a) {
     using Form = NormUnit<T, V, INTERLEAVED>;
     using Raw = RawUnit<T, V, INTERLEAVED>;
@@ -296,12 +341,13 @@ head_norm_kernel(const __grid_constant__ NormArgs a) {
         x = static_cast<const T*>(s.x) + batch_index * s.x_stride[0] + head * s.x_stride[1] + (token0 + local) * s.x_stride[2];
         y = static_cast<T*>(s.out) + batch_index * s.out_stride[0] + head * s.out_stride[1] + (token0 + local) * s.out_stride[2];
     };
-    Ring<T, V, INTERLEAVED, kForwardStages<T>, 1> ring(angles + ((2 * a.half) << a.token_shift));
+    float* gains = angles + ((2 * a.half) << a.token_shift);   // of both pairs of tensors
+    Ring<T, V, INTERLEAVED, kForwardStages, 1> ring(gains + 2 * a.d);
     int64_t x_step = 0;
     auto start = [&] {   // the first rows of the pair of tensors at hand
         x_step = step * a.side[which].x_stride[1];
 #pragma unroll
-        for (int i = 0; i + 1 < kForwardStages<T>; ++i) {
+        for (int i = 0; i + 1 < kForwardStages; ++i) {
             const bool wanted = live && head + i * step < heads;
             const T* const from[1] = {wanted ? x + i * x_step : static_cast<const T*>(a.side[which].x)};
             ring.fill(share, apart, from, wanted);
@@ -310,29 +356,28 @@ head_norm_kernel(const __grid_constant__ NormArgs a) {
     begin();
     chain_begin();
     start();   // (on their way while the angles are worked out)
-    for (int i = threadIdx.x; i < a.half << a.token_shift; i += kNormThreads) {
-        const int token = i & mask, pair = i >> a.token_shift;
-        if (token < tokens) put_angle<Form, sizeof(T) == 4>(a, angles + token * 2 * a.half, pair, batch_index, token0 + token);
-    }
+    fill_gains(a, a.side[0], gains);
+    if (a.side[1].heads) fill_gains(a, a.side[1], gains + a.d);
+    const int filled = threadIdx.x & mask;
+    fill_angles<T, Form>(a, angles, filled, filled < tokens, batch_index, token0 + filled);
     __syncthreads();
     for (;;) {
         const NormSide& s = a.side[which];
         const int64_t y_step = step * s.out_stride[1];
         Values<Form::kPacks> along[U], across[U];   // what a pair's own value and the other one are multiplied by
-        int held = -1;                              // the head whose gains are in them
+        bool fresh = false;                         // ... by the gains of the head at hand
         // (whole warps stay together: a warp's groups have heads side by side)
         while (__any_sync(0xffffffffu, head < heads)) {
-            const bool own = live && head < heads, later = live && head + (kForwardStages<T> - 1) * step < heads;
+            const bool own = live && head < heads, later = live && head + (kForwardStages - 1) * step < heads;
             Raw now[1][U];
             ring.take(now);
-            const T* const from[1] = {later ? x + (kForwardStages<T> - 1) * x_step : static_cast<const T*>(s.x)};
+            const T* const from[1] = {later ? x + (kForwardStages - 1) * x_step : static_cast<const T*>(s.x)};
             ring.fill(share, apart, from, later);
-            const int wanted = s.gain_head ? min(head, s.heads - 1) : 0;
-            if (wanted != held) {
+            if (!fresh) {
 #pragma unroll
                 for (int j = 0; j < U; ++j) {
                     Values<Form::kPacks> gain;
-                    load_gains<Form, V>(a, s, wanted, share.channel[j], share.there[j], share.turns[j], gain);
+                    take_gains<Form, V>(a, s, gains + which * a.d, min(head, s.heads - 1), share.channel[j], share.there[j], share.turns[j], gain);
                     along[j] = gain;
                     across[j] = Values<Form::kPacks>{};
                     if (!share.turns[j]) continue;
@@ -349,7 +394,7 @@ head_norm_kernel(const __grid_constant__ NormArgs a) {
                         across[j].two[k] = mul2(gain.one[k], sine[k]);
                     }
                 }
-                held = wanted;
+                fresh = s.gain_head == 0;
             }
             Values<Form::kPacks> v[U];
             uint64_t squares = 0;
@@ -396,10 +441,8 @@ head_norm_long_kernel(const __grid_constant__ NormArgs a) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int apart = Form::apart(a), run0 = static_cast<int>(blockIdx.y) * a.heads_per_cta, run1 = run0 + a.heads_per_cta;
     chain_begin();
-    for (int i = threadIdx.x; i < a.half << a.token_shift; i += kNormThreads) {
-        const int local = i & mask, pair = i >> a.token_shift;
-        if (local < tokens) put_angle<Form, sizeof(T) == 4>(a, angles + local * 2 * a.half, pair, batch_index, token0 + local);
-    }
+    const int filled = threadIdx.x & mask;
+    fill_angles<T, Form>(a, angles, filled, filled < tokens, batch_index, token0 + filled);
     __syncthreads();
 #pragma unroll 1
     for (int which = 0; which < 2; ++which) {
@@ -474,14 +517,11 @@ struct TokenPlaces {
         out = b * s.out_stride[0] + t * s.out_stride[2];
     }
 };
-template <typename Form, bool CLOSE>
-__device__ __forceinline__ void fill_angles(const NormArgs& a, float* angles, int token0, int tokens) {
-    for (int i = threadIdx.x; i < a.half << a.token_shift; i += kNormThreads) {
-        const int local = i & ((1 << a.token_shift) - 1), pair = i >> a.token_shift;
-        if (local >= tokens) continue;
-        const int token = token0 + local, b = static_cast<int>(fast_divide(static_cast<uint32_t>(token), a.by_seq));
-        put_angle<Form, CLOSE>(a, angles + local * 2 * a.half, pair, b, token - b * a.seq);
-    }
+// (gradient: tokens of all sequences in a row)
+template <typename T, typename Form>
+__device__ __forceinline__ void fill_angles_of(const NormArgs& a, float* angles, int token0, int tokens) {
+    const int local = threadIdx.x & ((1 << a.token_shift) - 1), token = token0 + min(local, tokens - 1), b = static_cast<int>(fast_divide(static_cast<uint32_t>(token), a.by_seq));
+    fill_angles<T, Form>(a, angles, local, local < tokens, b, token - b * a.seq);
 }
 // The values of a lane's share, met over the groups of its warp, to channels at `to`.
 template <typename Form, int U, int V>
@@ -533,15 +573,16 @@ head_norm_grad_kernel(const __grid_constant__ NormArgs a) {
     Values<Form::kPacks> gain[U], sums[U], cosine[U], sine[U];   // (the angles, not PER_HEAD: `one` alone)
 #pragma unroll
     for (int j = 0; j < U; ++j) sums[j] = Values<Form::kPacks>{};
-    Ring<T, V, INTERLEAVED, kGradientStages<T>, 2> ring(angles + ((2 * a.half) << a.token_shift));
+    float* gains = angles + ((2 * a.half) << a.token_shift);
+    Ring<T, V, INTERLEAVED, kGradientStages, 2> ring(gains + a.d);
     auto fill = [&](const T* from_x, const T* from_dy, bool wanted) {
         const T* const from[2] = {wanted ? from_x : static_cast<const T*>(s.x), wanted ? from_dy : static_cast<const T*>(s.dy)};
         ring.fill(share, apart, from, wanted);
     };
     Raw rows[2][U];   // of X and dY, at hand
-    auto take_gains = [&](int head) {
+    auto gains_of = [&](int head) {
 #pragma unroll
-        for (int j = 0; j < U; ++j) load_gains<Form, V>(a, s, head, share.channel[j], share.there[j], share.turns[j], gain[j]);
+        for (int j = 0; j < U; ++j) take_gains<Form, V>(a, s, gains, head, share.channel[j], share.there[j], share.turns[j], gain[j]);
     };
     // The row at hand: u turned back, both sums, dX to `to`, and the terms of dgain.
     auto row = [&](T* to, const float* table, bool live) {
@@ -584,7 +625,8 @@ head_norm_grad_kernel(const __grid_constant__ NormArgs a) {
             places[2][threadIdx.x] = of.out;
         }
         chain_begin();
-        fill_angles<Form, sizeof(T) == 4>(a, angles, token0, tokens);
+        fill_gains(a, s, gains);
+        fill_angles_of<T, Form>(a, angles, token0, tokens);
         __syncthreads();
         int head = warp, base = 0, ahead = warp, ahead_base = 0;   // at hand, and the next to be fetched
         auto fetch = [&] {
@@ -598,14 +640,14 @@ head_norm_grad_kernel(const __grid_constant__ NormArgs a) {
             }
         };
 #pragma unroll
-        for (int i = 0; i + 1 < kGradientStages<T>; ++i) fetch();
+        for (int i = 0; i + 1 < kGradientStages; ++i) fetch();
         bool fresh = true;
         while (head < heads) {
             const int local = min(base + group, tokens - 1);
             const bool live = base + group < tokens, last = base + groups >= tokens;
             ring.take(rows);
             fetch();
-            if (fresh) take_gains(s.gain_head ? head0 + head : 0);
+            if (fresh) gains_of(head0 + head);
             fresh = last && s.gain_head != 0;
             row(dx + head * s.out_stride[1] + places[2][local], angles + local * 2 * a.half, live);
             if (last && sums_wanted) put_sums<Form, U, V>(a, share, sums, s.partial + (static_cast<int64_t>(tile) * s.heads + head0 + head) * a.d);
@@ -631,8 +673,9 @@ head_norm_grad_kernel(const __grid_constant__ NormArgs a) {
         const int64_t x_step = step * s.x_stride[1], dy_step = step * s.dy_stride[1], dx_step = step * s.out_stride[1];
         chain_begin();
 #pragma unroll
-        for (int i = 0; i + 1 < kGradientStages<T>; ++i) fill(x + i * x_step, dy + i * dy_step, live && head + i * step < heads);   // (on their way while the angles are worked out)
-        fill_angles<Form, sizeof(T) == 4>(a, angles, token0, tokens);
+        for (int i = 0; i + 1 < kGradientStages; ++i) fill(x + i * x_step, dy + i * dy_step, live && head + i * step < heads);   // (on their way while the angles are worked out)
+        fill_gains(a, s, gains);
+        fill_angles_of<T, Form>(a, angles, token0, tokens);
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < U; ++j) {
@@ -647,11 +690,12 @@ head_norm_grad_kernel(const __grid_constant__ NormArgs a) {
             get_angles<Form>(table, place, stride, cosine[j].one);
             get_angles<Form>(table + a.half, place, stride, sine[j].one);
         }
-        if (!s.gain_head) take_gains(0);
+        bool fresh = true;
         while (__any_sync(0xffffffffu, head < heads)) {
-            if (s.gain_head) take_gains(head0 + min(head, heads - 1));
+            if (fresh) gains_of(head0 + min(head, heads - 1));
+            fresh = s.gain_head != 0;
             ring.take(rows);
-            fill(x + (kGradientStages<T> - 1) * x_step, dy + (kGradientStages<T> - 1) * dy_step, live && head + (kGradientStages<T> - 1) * step < heads);
+            fill(x + (kGradientStages - 1) * x_step, dy + (kGradientStages - 1) * dy_step, live && head + (kGradientStages - 1) * step < heads);
             row(dx, nullptr, live && head < heads);
             head += step;
             x += x_step;
@@ -687,7 +731,7 @@ head_norm_grad_long_kernel(const __grid_constant__ NormArgs a) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, apart = Form::apart(a);
     const bool sums_wanted = s.partial != nullptr;
     chain_begin();
-    fill_angles<Form, sizeof(T) == 4>(a, angles, token0, tokens);
+    fill_angles_of<T, Form>(a, angles, token0, tokens);
     __syncthreads();
     float* meeting = angles + ((2 * a.half) << a.token_shift);
     float* sums = meeting + warp * a.d;   // (a lane's channels are its own)
@@ -894,14 +938,14 @@ int check_norm(NormProblem& p) {
     return kOk;
 }
 
-// As few lanes as hold a row, 16 values each; single values (width 1) and rows beyond a warp: a warp a row, read twice (per_lane 0).
+// As few lanes as hold a row, 32 bytes each; single values (width 1) and rows beyond a warp: a warp a row, read twice (per_lane 0).
 struct LaneForm {
     int turning, units, per_lane, group_shift;
 };
 LaneForm lane_form(const NormProblem& p, int width) {
     const int half = p.positions->rank ? static_cast<int>(p.frequencies->dim[3]) : 0, d = static_cast<int>(p.row[0][0]->dim[3]);
     const int pairs = p.interleaved && width > 1 ? width / 2 : width;   // of a unit
-    LaneForm form{half / pairs, half / pairs + (d - 2 * half) / width, width == 1 ? 0 : 8 / pairs, 5};
+    LaneForm form{half / pairs, half / pairs + (d - 2 * half) / width, width == 1 ? 0 : 16 / dtype_bytes(p.row[0][0]->dtype) / pairs, 5};
     if (form.units > 32 * form.per_lane) form.per_lane = 0;
     if (form.per_lane)
         for (form.group_shift = 0; (form.per_lane << form.group_shift) < form.units;) ++form.group_shift;
@@ -985,11 +1029,8 @@ int build_norm(NormProblem& p, void* const (&pointers)[2][3], const void* positi
     return kOk;
 }
 
-// 16 values a thread (Ring::kBytes).
-size_t ring_bytes(const NormProblem& p, bool gradient) {
-    const int bytes = dtype_bytes(p.row[0][0]->dtype), stages = bytes == 4 ? (gradient ? 2 * kGradientStages<float> : kForwardStages<float>) : (gradient ? 2 * kGradientStages<__half> : kForwardStages<__half>);
-    return static_cast<size_t>(16 * bytes) * stages * kNormThreads;
-}
+// Ring::kBytes
+constexpr size_t ring_bytes(int stages, int tensors) { return static_cast<size_t>(32) * stages * tensors * kNormThreads; }
 
 enum NormKernel { kForward, kForwardLong, kGradient, kGradientOfHeads, kGradientLong };
 template <typename T, int V, bool INTERLEAVED>
@@ -1034,20 +1075,22 @@ GradCut grad_cut(const NormProblem& p) {
     const int64_t half = p.positions->rank ? p.frequencies->dim[3] : 0;
     const int64_t tokens = x.dim[0] * x.dim[2], heads[2] = {x.dim[1], p.two ? p.row[1][0]->dim[1] : 0};
     GradCut cut{};
-    // With sums for each head 32 tokens, so that few sums go out; otherwise as many as there are groups of lanes.
-    cut.shift = 5;
-    if (!any_sums_of_heads(p)) {
+    // With sums for each head 16 tokens and few heads (3 x 1001 f32 tokens of 32 heads: four heads 35.1 us, eight 38.6; 32 tokens 37.6 and 58.7, eight tokens 38.7 and 37.8); otherwise
+    // as many tokens as there are groups of lanes and many heads (4 x 2048 bf16 tokens of 32 + 8 heads: 32 heads 51.3 us, 16 57.1, 8 66.8; eight tokens 54.9, 64.5, 82.8).
+    const bool of_heads = any_sums_of_heads(p);
+    cut.shift = 4;
+    if (!of_heads) {
         const LaneForm form = lane_form(p, p.width);
         cut.shift = std::min(7 - form.group_shift, 5);
     }
-    while (cut.shift > 0 && 8 * (half << cut.shift) > (dtype_bytes(x.dtype) == 4 ? kNormShared : kNormSharedOfSixteen)) --cut.shift;
+    while (cut.shift > 0 && 8 * (half << cut.shift) > kNormShared) --cut.shift;
     cut.heads_per_cta = 32;
     auto ctas = [&] {
         cut.tiles = (tokens + (1ll << cut.shift) - 1) >> cut.shift;
         for (int s = 0; s < 2; ++s) cut.runs[s] = (heads[s] + cut.heads_per_cta - 1) / cut.heads_per_cta;
         return cut.tiles * (cut.runs[0] + cut.runs[1]);
     };
-    while (ctas() < 6 * 148 && cut.heads_per_cta > 4) cut.heads_per_cta /= 2;
+    while (ctas() < (of_heads ? 10 : 6) * 148 && cut.heads_per_cta > 4) cut.heads_per_cta /= 2;
     while (ctas() < 4 * 148 && cut.shift > 2) --cut.shift;
     ctas();
     return cut;
@@ -1086,9 +1129,10 @@ extern "C" int dfgpu_head_norm(const dfgpu_head_norm_params* params, void* const
     const void* const gains[2] = {p.gain[0]->rank ? tensors[2] : nullptr, p.gain[1]->rank ? tensors[7] : nullptr};
     status = build_norm(p, rows, p.positions->rank ? tensors[3] : nullptr, p.positions->rank ? tensors[4] : nullptr, gains, a, per_lane);
     if (status) return status;
-    // A token a group of lanes (where the heads are to be shared out, several groups) and all heads, which share the tokens' angles; fewer heads where the CTAs would be few.
+    // Up to eight tokens a CTA and all heads, which share the tokens' angles; fewer heads where the CTAs would be few. (2 x 8192 tokens of 40 heads of 128 bf16 channels: 60.7 us;
+    // sixteen tokens 66.7, four 64.2; the heads in two runs 61.9, in four 76.9.)
     const int heads = a.side[0].heads + a.side[1].heads, groups = kNormThreads >> a.group_shift;
-    while (a.token_shift < 4 && (2 << a.token_shift) <= groups && (1 << a.token_shift) < a.seq && (a.half << (a.token_shift + 1)) <= kNormTable) ++a.token_shift;
+    while (a.token_shift < 3 && (2 << a.token_shift) <= groups && (1 << a.token_shift) < a.seq && (a.half << (a.token_shift + 1)) <= kNormTable) ++a.token_shift;
     a.tiles = (a.seq + (1 << a.token_shift) - 1) >> a.token_shift;
     a.by_tiles = make_fast_divisor(static_cast<uint32_t>(a.tiles));
     const int64_t tiles = p.row[0][0]->dim[0] * a.tiles;
@@ -1096,7 +1140,7 @@ extern "C" int dfgpu_head_norm(const dfgpu_head_norm_params* params, void* const
     auto runs = [&] { return (heads + a.heads_per_cta - 1) / a.heads_per_cta; };
     while (tiles * runs() < 8 * 148 && (a.heads_per_cta << a.token_shift) > groups && a.heads_per_cta > 1) a.heads_per_cta = (a.heads_per_cta + 1) / 2;
     const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(runs()));
-    const size_t shared = sizeof(float) * static_cast<size_t>((2 * a.half) << a.token_shift) + (per_lane ? ring_bytes(p, false) : 0);
+    const size_t shared = sizeof(float) * static_cast<size_t>((2 * a.half) << a.token_shift) + (per_lane ? 8 * static_cast<size_t>(a.d) + ring_bytes(kForwardStages, 1) : 0);
     launch_norm(per_lane ? kForward : kForwardLong, a, p.row[0][0]->dtype, p.width, p.interleaved != 0, grid, shared, as_stream(stream));
     return check_launch("HEAD_NORM");
 }
@@ -1168,7 +1212,7 @@ extern "C" int dfgpu_head_norm_grad(const dfgpu_head_norm_grad_params* params, v
     const bool of_heads = any_sums_of_heads(p);
     if (per_lane && !of_heads && (kNormThreads >> a.group_shift) < (1 << a.token_shift)) per_lane = 0;
     launch_norm(!per_lane ? kGradientLong : of_heads ? kGradientOfHeads : kGradient, a, p.row[0][0]->dtype, p.width, p.interleaved != 0, grid,
-                per_lane ? std::max(table + ring_bytes(p, true), meeting) : table + meeting,
+                per_lane ? std::max(table + 4 * static_cast<size_t>(a.d) + ring_bytes(kGradientStages, 2), meeting) : table + meeting,
                                 as_stream(stream));
     status = check_launch("HEAD_NORM gradient");
     if (status || !blocks) return status;

@@ -28,23 +28,13 @@ struct Positions {
     int32_t wide;   // INT64
 };
 // (cosine, sine) of position * frequency. The product passes 2^24 for far positions, where f32 has lost the angle: it and its reduction to one turn
-// are made in f64, the sine and cosine of what is left, within half a turn, in f32. CLOSE: with what rounding the reduced angle to f32 leaves out, which
-// is off by up to 9e-8 and counts where results are f32.
-template <bool CLOSE = false>
+// are made in f64, the sine and cosine of what is left, within half a turn, in f32.
 __device__ __forceinline__ float2 turn_of(const Positions& p, int64_t batch, int64_t token, int64_t pair) {
     const int64_t at = batch * p.batch + token * p.token;
     const int64_t position = p.wide ? static_cast<const int64_t*>(p.positions)[at] : static_cast<int64_t>(static_cast<const int32_t*>(p.positions)[at]);
     const double turns = static_cast<double>(position) * static_cast<double>(p.frequencies[pair * p.frequency_stride]) * 0.15915494309189533577;
-    const double reduced = 2.0 * (turns - rint(turns));
-    const float halves = static_cast<float>(reduced);
     float sine, cosine;
-    sincospif(halves, &sine, &cosine);
-    if constexpr (CLOSE) {
-        const float rest = 3.14159265f * static_cast<float>(reduced - static_cast<double>(halves));
-        const float first = cosine;
-        cosine = __fmaf_rn(-sine, rest, cosine);
-        sine = __fmaf_rn(first, rest, sine);
-    }
+    sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &sine, &cosine);
     return make_float2(cosine, sine);
 }
 

@@ -106,21 +106,24 @@ class Heads:
         frequencies = np.zeros(0) if self.frequencies is None else self.frequencies.cpu().numpy()
         return x, gain, at, frequencies, half
 
+    def turn_error(self, half):
+        return 0 if half == 0 else 5e-7 if self.dtype == F32 else 7.5e-7
+
     def check_forward(self, y):
         """r: the sum of squares goes through at most 64 additions of a lane and 5 across, rounded up to 70 half steps, half of which reach r; the mean and epsilon
         2, rsqrtf 4: 41 U of r. x r gain: 3 more, the gain with its offset 1. A turn: 5e-7 of |n1| + |n2| (sines of a reduced angle, three roundings) and 2 U
-        for the scale. Then one rounding to the type."""
+        for the scale; in 16 bits sines and cosines are off by 2^-21.4 = 3.6e-7 and the angle by 1.9e-7 (pi 2^-24), with three roundings 7.5e-7. Then one rounding to the type."""
         for i, got in enumerate(y):
             x, gain, at, frequencies, half = self.parts(i)
             want = ref.head_norm(x, gain, at, frequencies, self.interleaved, self.scale, self.epsilon)
             n = ref.head_norm(x, gain, at, np.zeros(0), epsilon=self.epsilon)
             both = ref.both_of_pair(n, half, self.interleaved) * max(1.0, abs(self.scale))
-            bound = (47 * U + (5e-7 if half else 0)) * both + half_step(self.dtype) * np.abs(want) * 1.001 + (2.0 ** -25 if self.dtype == F16 else 0)
+            bound = (47 * U + self.turn_error(half)) * both + half_step(self.dtype) * np.abs(want) * 1.001 + (2.0 ** -25 if self.dtype == F16 else 0)
             error = np.abs(double(got) - want)
             assert np.all(error <= bound), np.max(error - bound)
 
     def check_gradient(self, dx, dgain, dgain_type=torch.float32):
-        """u: a turn, 5e-7 of |dy1| + |dy2| and 2 U. mean(v x): its terms 5e-7 of the pair's, 3 U, and a sum of 70 additions. r^2 twice 41 U, r once.
+        """u: a turn of |dy1| + |dy2| and 2 U. mean(v x): its terms that of the pair's, 3 U, and a sum of 70 additions. r^2 twice 41 U, r once.
         dgain: a term has u's error and 43 U; a CTA's sum at most 128 additions a lane, 5 across, 4 warps, and one rounding, the rest in 64 bits."""
         for i, got in enumerate(dx):
             x, gain, at, frequencies, half = self.parts(i)
@@ -128,7 +131,7 @@ class Heads:
             want, sums = ref.head_norm_grad(x, dy, gain, at, frequencies, self.interleaved, self.scale, self.epsilon)
             r = 1.0 / np.sqrt((x * x).mean(-1, keepdims=True) + self.epsilon)
             u = ref.both_of_pair(dy, half, self.interleaved) * max(1.0, abs(self.scale))
-            off = (5e-7 if half else 0) + 2 * U
+            off = self.turn_error(half) + 2 * U
             v = u * np.abs(gain)[None, :, None]
             mean = (v * np.abs(x)).mean(-1, keepdims=True)
             bound = r * v * (off + 45 * U) + np.abs(x) * r ** 3 * mean * (off + (75 + 3 * 41 + 6) * U)
@@ -256,6 +259,15 @@ def test_head_norm_gains_of_one_side_s_heads():
         heads.gain[0] = None
         heads.check_forward(heads.forward())
         heads.check_gradient(*heads.gradient())
+
+
+def test_head_norm_of_many_tokens():
+    """So many tokens that a CTA walks all heads of queries and keys, and runs that hold heads of both."""
+    for h, h2, s in ((32, 8, 3300), (13, 5, 1700), (3, 9, 700)):
+        heads = Heads(16, 3, h, h2, s, 64, 64, BF16)
+        heads.check_forward(heads.forward())
+        heads = Heads(17, 3, h, h2, s, 64, 32, F32, per_head=True)
+        heads.check_forward(heads.forward())
 
 
 def test_head_norm_gradient_of_many_tokens():
