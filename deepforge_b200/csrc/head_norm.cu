@@ -550,7 +550,7 @@ __device__ __forceinline__ void put_sums(const NormArgs& a, const Share<Form, U>
 // PER_HEAD: each warp has heads of its own, with their gains, and walks the tokens, whose angles are in the table; the sums of dgain go out with each head.
 // Otherwise a group of lanes has one token, its angles in registers, and walks the heads; all have one sum.
 template <typename T, int V, bool INTERLEAVED, bool PER_HEAD>
-__global__ void __launch_bounds__(kNormThreads)
+__global__ void __launch_bounds__(kNormThreads, sizeof(T) == 4 ? 6 : 4)
 head_norm_grad_kernel(const __grid_constant__ NormArgs a) {
     using Form = NormUnit<T, V, INTERLEAVED>;
     using Raw = RawUnit<T, V, INTERLEAVED>;
@@ -684,7 +684,7 @@ head_norm_grad_kernel(const __grid_constant__ NormArgs a) {
                 cosine[j].one[k] = pack2(1.0f, 1.0f);
                 sine[j].one[k] = 0;
             }
-            if (!share.turns[j]) continue;
+            if (!share.turns[j] || !live) continue;   // (behind the last token there are no angles: zeros stay zeros in the sums)
             const float* table = angles + local * 2 * a.half;
             const int place = angle_place<Form>(a, share.unit[j], 0), stride = a.turning * Form::kQuad;
             get_angles<Form>(table, place, stride, cosine[j].one);

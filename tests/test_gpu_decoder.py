@@ -270,6 +270,19 @@ def test_head_norm_of_many_tokens():
         heads.check_forward(heads.forward())
 
 
+@pytest.mark.parametrize("per_head", [False, True])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_head_norm_gradient_behind_the_last_token(interleaved, per_head):
+    """Tokens that do not fill the last CTA: what shared memory held before (here the NaN of a call with NaN frequencies on every SM) does not reach the sums."""
+    heads = Heads(18, 3, 8, 2, 1581, 80, 80, F32, interleaved=interleaved, per_head=per_head)
+    right = heads.frequencies
+    for _ in range(3):
+        heads.frequencies = torch.full_like(right, float("nan"))
+        heads.gradient()
+        heads.frequencies = right
+        heads.check_gradient(*heads.gradient())
+
+
 def test_head_norm_gradient_of_many_tokens():
     """Several runs of heads and tiles of tokens; the same call twice gives the same bits."""
     heads = Heads(14, 3, 40, 8, 500, 128, 128, BF16)
