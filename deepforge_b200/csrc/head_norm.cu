@@ -16,6 +16,7 @@ namespace {
 
 constexpr int kNormThreads = 128, kNormWarps = kNormThreads / 32;
 constexpr int kNormTable = 2048;      // (cosine, sine) pairs of a CTA, forward: 16 KiB
+constexpr int kNormGains = 8 * 1024;     // bytes of gains of heads, forward
 constexpr int kNormShared = 18 * 1024;   // bytes of a CTA's table, gradient: with the rows on their way within 48 KiB
 constexpr int64_t kNormMaxD = 1024;
 
@@ -28,15 +29,17 @@ struct NormSide {
     int64_t x_stride[3], dy_stride[3], out_stride[3];   // batch, head, token
     int64_t gain_head;
     int32_t gain_type, heads, per_head;   // per_head: sums of dgain go out for each head
+    int32_t runs, first_run;          // (gradient) of heads: those that hold some of these
 };
 struct NormArgs {
     NormSide side[2];
     Positions at;
     int32_t seq, tokens, tiles, token_shift;   // tokens: of all sequences; a CTA's: 1 << token_shift
-    int32_t heads_per_cta, first_side;         // forward: of both pairs of tensors in a row; gradient: runs of the first pair are the first `first_side`
+    int32_t heads_per_cta;                     // of both pairs of tensors in a row
+    int32_t gain_floats;                       // (forward) room for gains in shared memory
     int32_t d, half, turning, units;           // units of V pairs (half) or V channels (interleaved, or not turned) a row
     int32_t group_shift;                       // lanes of a row: 1 << group_shift
-    FastDivisor by_tiles, by_seq;
+    FastDivisor by_tiles, by_seq, by_d;
     float scale, epsilon, gain_offset, inverse_d;
 };
 
@@ -158,14 +161,19 @@ __device__ __forceinline__ void load_gains(const NormArgs& a, const NormSide& s,
         gain.two[k] = pack2(g[1][0], g[1][1]);
     }
 }
-// A gain that all heads share, as f32 in shared memory (all threads; the barrier behind the angles' is its too), and a lane's part of it.
-__device__ __forceinline__ void fill_gains(const NormArgs& a, const NormSide& s, float* to) {
-    if (s.gain_head) return;
-    for (int c = threadIdx.x; c < a.d; c += kNormThreads) to[c] = gain_at(s, a.gain_offset, c);
+// Gains as f32 in shared memory (by all threads; the barrier behind the angles' is its too): of all heads together, or of `heads` from head0 on. And a lane's part of
+// them: `shared` is the head's there, or null.
+__device__ __forceinline__ void fill_gains(const NormArgs& a, const NormSide& s, float* to, int head0, int heads) {
+    const int count = (s.gain_head ? heads : 1) * a.d;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < count; i += kNormThreads) {
+        const int head = static_cast<int>(fast_divide(static_cast<uint32_t>(i), a.by_d));
+        to[i] = gain_at(s, a.gain_offset, (head0 + head) * s.gain_head + (i - head * a.d));
+    }
 }
 template <typename Form, int V>
 __device__ __forceinline__ void take_gains(const NormArgs& a, const NormSide& s, const float* shared, int head, int channel, bool live, bool turns, Values<Form::kPacks>& gain) {
-    if (s.gain_head) return load_gains<Form, V>(a, s, head, channel, live, turns, gain);
+    if (!shared) return load_gains<Form, V>(a, s, head, channel, live, turns, gain);
     gain = Values<Form::kPacks>{};
     if (!live) return;
     const float* first = shared + channel;
@@ -315,7 +323,8 @@ constexpr int kForwardStages = 4, kGradientStages = 3;
 
 // ---- forward: a CTA takes a few tokens of one sequence and a run of heads of both pairs of tensors, which share the tokens' angles -----------------------
 // A group of lanes has one token and walks the heads, so that the angles stay in registers, multiplied by the gains already.
-template <typename T, int V, bool INTERLEAVED>
+// OF_HEADS: some gains are those of each head.
+template <typename T, int V, bool INTERLEAVED, bool OF_HEADS>
 __global__ void __launch_bounds__(kNormThreads, 6)
 head_norm_kernel(const __grid_constant__ NormArgs a) {
     using Form = NormUnit<T, V, INTERLEAVED>;
@@ -341,8 +350,11 @@ head_norm_kernel(const __grid_constant__ NormArgs a) {
         x = static_cast<const T*>(s.x) + batch_index * s.x_stride[0] + head * s.x_stride[1] + (token0 + local) * s.x_stride[2];
         y = static_cast<T*>(s.out) + batch_index * s.out_stride[0] + head * s.out_stride[1] + (token0 + local) * s.out_stride[2];
     };
-    float* gains = angles + ((2 * a.half) << a.token_shift);   // of both pairs of tensors
-    Ring<T, V, INTERLEAVED, kForwardStages, 1> ring(gains + 2 * a.d);
+    // gains of both pairs of tensors, of each the CTA's heads' or one
+    float* const first_gains = angles + ((2 * a.half) << a.token_shift);
+    const int first_heads = max(min(run1, a.side[0].heads) - run0, 0), second_head0 = max(run0 - a.side[0].heads, 0), second_heads = max(min(run1 - a.side[0].heads, a.side[1].heads) - second_head0, 0);
+    float* const second_gains = first_gains + (a.side[0].gain_head ? first_heads : 1) * a.d;
+    Ring<T, V, INTERLEAVED, kForwardStages, 1> ring(first_gains + a.gain_floats);
     int64_t x_step = 0;
     auto start = [&] {   // the first rows of the pair of tensors at hand
         x_step = step * a.side[which].x_stride[1];
@@ -356,8 +368,8 @@ head_norm_kernel(const __grid_constant__ NormArgs a) {
     begin();
     chain_begin();
     start();   // (on their way while the angles are worked out)
-    fill_gains(a, a.side[0], gains);
-    if (a.side[1].heads) fill_gains(a, a.side[1], gains + a.d);
+    fill_gains(a, a.side[0], first_gains, run0, first_heads);
+    if (second_heads) fill_gains(a, a.side[1], second_gains, second_head0, second_heads);
     const int filled = threadIdx.x & mask;
     fill_angles<T, Form>(a, angles, filled, filled < tokens, batch_index, token0 + filled);
     __syncthreads();
@@ -365,7 +377,28 @@ head_norm_kernel(const __grid_constant__ NormArgs a) {
         const NormSide& s = a.side[which];
         const int64_t y_step = step * s.out_stride[1];
         Values<Form::kPacks> along[U], across[U];   // what a pair's own value and the other one are multiplied by
-        bool fresh = false;                         // ... by the gains of the head at hand
+#pragma unroll
+        for (int j = 0; j < U; ++j) {               // (by the gains already, where all heads have the same)
+            Values<Form::kPacks> gain;
+#pragma unroll
+            for (int k = 0; k < Form::kPacks; ++k) gain.one[k] = gain.two[k] = pack2(1.0f, 1.0f);
+            if (!OF_HEADS || !s.gain_head) take_gains<Form, V>(a, s, which ? second_gains : first_gains, 0, share.channel[j], share.there[j], share.turns[j], gain);
+            along[j] = gain;
+            across[j] = Values<Form::kPacks>{};
+            if (!share.turns[j]) continue;
+            uint64_t cosine[Form::kPacks], sine[Form::kPacks];
+            const float* table = angles + local * 2 * a.half;
+            const int place = angle_place<Form>(a, share.unit[j], 0), stride = a.turning * Form::kQuad;
+            get_angles<Form>(table, place, stride, cosine);
+            get_angles<Form>(table + a.half, place, stride, sine);
+#pragma unroll
+            for (int k = 0; k < Form::kPacks; ++k) {
+                along[j].one[k] = mul2(gain.one[k], cosine[k]);
+                along[j].two[k] = mul2(gain.two[k], cosine[k]);
+                across[j].one[k] = minus2(mul2(gain.two[k], sine[k]));
+                across[j].two[k] = mul2(gain.one[k], sine[k]);
+            }
+        }
         // (whole warps stay together: a warp's groups have heads side by side)
         while (__any_sync(0xffffffffu, head < heads)) {
             const bool own = live && head < heads, later = live && head + (kForwardStages - 1) * step < heads;
@@ -373,29 +406,6 @@ head_norm_kernel(const __grid_constant__ NormArgs a) {
             ring.take(now);
             const T* const from[1] = {later ? x + (kForwardStages - 1) * x_step : static_cast<const T*>(s.x)};
             ring.fill(share, apart, from, later);
-            if (!fresh) {
-#pragma unroll
-                for (int j = 0; j < U; ++j) {
-                    Values<Form::kPacks> gain;
-                    take_gains<Form, V>(a, s, gains + which * a.d, min(head, s.heads - 1), share.channel[j], share.there[j], share.turns[j], gain);
-                    along[j] = gain;
-                    across[j] = Values<Form::kPacks>{};
-                    if (!share.turns[j]) continue;
-                    uint64_t cosine[Form::kPacks], sine[Form::kPacks];
-                    const float* table = angles + local * 2 * a.half;
-                    const int place = angle_place<Form>(a, share.unit[j], 0), stride = a.turning * Form::kQuad;
-                    get_angles<Form>(table, place, stride, cosine);
-                    get_angles<Form>(table + a.half, place, stride, sine);
-#pragma unroll
-                    for (int k = 0; k < Form::kPacks; ++k) {
-                        along[j].one[k] = mul2(gain.one[k], cosine[k]);
-                        along[j].two[k] = mul2(gain.two[k], cosine[k]);
-                        across[j].one[k] = minus2(mul2(gain.two[k], sine[k]));
-                        across[j].two[k] = mul2(gain.one[k], sine[k]);
-                    }
-                }
-                fresh = s.gain_head == 0;
-            }
             Values<Form::kPacks> v[U];
             uint64_t squares = 0;
 #pragma unroll
@@ -406,6 +416,19 @@ head_norm_kernel(const __grid_constant__ NormArgs a) {
             }
             const float r = inverse_root<T>(__fmaf_rn(sum_over(sum2(squares), lanes), a.inverse_d, a.epsilon));
             const uint64_t both = pack2(r, r);
+            if (OF_HEADS && s.gain_head) {
+                const float* of_head = (which ? second_gains - second_head0 * a.d : first_gains - run0 * a.d) + min(head, heads - 1) * a.d;
+#pragma unroll
+                for (int j = 0; j < U; ++j) {
+                    Values<Form::kPacks> gain;
+                    take_gains<Form, V>(a, s, of_head, 0, share.channel[j], share.there[j], share.turns[j], gain);
+#pragma unroll
+                    for (int k = 0; k < Form::kPacks; ++k) {
+                        v[j].one[k] = mul2(v[j].one[k], gain.one[k]);
+                        v[j].two[k] = mul2(v[j].two[k], gain.two[k]);
+                    }
+                }
+            }
 #pragma unroll
             for (int j = 0; j < U; ++j) {
 #pragma unroll
@@ -555,163 +578,174 @@ head_norm_grad_kernel(const __grid_constant__ NormArgs a) {
     using Form = NormUnit<T, V, INTERLEAVED>;
     using Raw = RawUnit<T, V, INTERLEAVED>;
     constexpr int U = Form::kPerLane;
-    extern __shared__ __align__(16) float angles[];                   // the table, and each warp's sums afterwards
+    extern __shared__ __align__(16) float angles[];
     __shared__ int64_t places[3][32];                                 // (PER_HEAD) of the tokens in X, dY, dX
     const int tile = static_cast<int>(blockIdx.x), token0 = tile << a.token_shift, tokens = min(a.tokens - token0, 1 << a.token_shift);
-    const bool second_side = static_cast<int>(blockIdx.y) >= a.first_side;
-    const NormSide& s = a.side[second_side];
-    const int run = static_cast<int>(blockIdx.y) - (second_side ? a.first_side : 0), runs = second_side ? static_cast<int>(gridDim.y) - a.first_side : a.first_side;
-    const int head0 = run * a.heads_per_cta, heads = min(a.heads_per_cta, s.heads - head0);
+    const int run0 = static_cast<int>(blockIdx.y) * a.heads_per_cta, run1 = run0 + a.heads_per_cta;
     const int warp = threadIdx.x >> 5, lanes = 1 << a.group_shift, apart = Form::apart(a);
     const Share<Form, U> share(a, threadIdx.x & (lanes - 1));
-    const bool sums_wanted = s.partial != nullptr;
-    const int mask = (1 << a.token_shift) - 1;
     const int group = PER_HEAD ? (threadIdx.x & 31) >> a.group_shift : threadIdx.x >> a.group_shift, groups = (PER_HEAD ? 32 : kNormThreads) >> a.group_shift;
-    const T* x = static_cast<const T*>(s.x) + head0 * s.x_stride[1];
-    const T* dy = static_cast<const T*>(s.dy) + head0 * s.dy_stride[1];
-    T* dx = static_cast<T*>(s.out) + head0 * s.out_stride[1];
-    Values<Form::kPacks> gain[U], sums[U], cosine[U], sine[U];   // (the angles, not PER_HEAD: `one` alone)
-#pragma unroll
-    for (int j = 0; j < U; ++j) sums[j] = Values<Form::kPacks>{};
-    float* gains = angles + ((2 * a.half) << a.token_shift);
-    Ring<T, V, INTERLEAVED, kGradientStages, 2> ring(gains + a.d);
-    auto fill = [&](const T* from_x, const T* from_dy, bool wanted) {
-        const T* const from[2] = {wanted ? from_x : static_cast<const T*>(s.x), wanted ? from_dy : static_cast<const T*>(s.dy)};
-        ring.fill(share, apart, from, wanted);
-    };
+    const int local = PER_HEAD ? 0 : group & ((1 << a.token_shift) - 1);   // (no more tokens than groups)
+    const bool own_token = local < tokens;
+    float* gains = angles + ((2 * a.half) << a.token_shift);   // of both pairs of tensors
+    float* meeting = gains + 2 * a.d;                          // where the rows are on their way, and the warps' sums afterwards
+    Ring<T, V, INTERLEAVED, kGradientStages, 2> ring(meeting);
     Raw rows[2][U];   // of X and dY, at hand
-    auto gains_of = [&](int head) {
+    Values<Form::kPacks> gain[U], sums[U], cosine[U], sine[U];   // (the angles, not PER_HEAD: `one` alone)
+    bool first = true;
+    chain_begin();
+#pragma unroll 1
+    for (int which = 0; which < 2; ++which) {
+        const NormSide& s = a.side[which];
+        const int before = which ? a.side[0].heads : 0, head0 = max(run0 - before, 0), heads = min(run1 - before, s.heads) - head0;
+        if (heads <= 0) continue;
+        const bool sums_wanted = s.partial != nullptr;
+        const T* x = static_cast<const T*>(s.x) + head0 * s.x_stride[1];
+        const T* dy = static_cast<const T*>(s.dy) + head0 * s.dy_stride[1];
+        T* dx = static_cast<T*>(s.out) + head0 * s.out_stride[1];
 #pragma unroll
-        for (int j = 0; j < U; ++j) take_gains<Form, V>(a, s, gains, head, share.channel[j], share.there[j], share.turns[j], gain[j]);
-    };
-    // The row at hand: u turned back, both sums, dX to `to`, and the terms of dgain.
-    auto row = [&](T* to, const float* table, bool live) {
-        Values<Form::kPacks> v[U], u[U];
-        uint64_t squares2 = 0, product2 = 0;
+        for (int j = 0; j < U; ++j) sums[j] = Values<Form::kPacks>{};
+        auto fill = [&](const T* from_x, const T* from_dy, bool wanted) {
+            const T* const from[2] = {wanted ? from_x : static_cast<const T*>(s.x), wanted ? from_dy : static_cast<const T*>(s.dy)};
+            ring.fill(share, apart, from, wanted);
+        };
+        auto gains_of = [&](int head) {
 #pragma unroll
-        for (int j = 0; j < U; ++j) {
-            v[j] = rows[0][j].values();
-            u[j] = rows[1][j].values();
-            if constexpr (PER_HEAD) {
-                if (share.turns[j]) turn_unit<Form, true>(a, table, share.unit[j], u[j]);
-            } else {
+            for (int j = 0; j < U; ++j) take_gains<Form, V>(a, s, s.gain_head ? nullptr : gains + which * a.d, head, share.channel[j], share.there[j], share.turns[j], gain[j]);
+        };
+        auto angles_and_gains = [&] {   // (once)
+            if (!first) return;
+            first = false;
+            for (int i = 0; i < 2; ++i)
+                if (a.side[i].heads && !a.side[i].gain_head) fill_gains(a, a.side[i], gains + i * a.d, 0, 1);
+            fill_angles_of<T, Form>(a, angles, token0, tokens);
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
 #pragma unroll
                 for (int k = 0; k < Form::kPacks; ++k) {
-                    const uint64_t one = u[j].one[k], two = u[j].two[k];
-                    u[j].one[k] = fma2(one, cosine[j].one[k], mul2(two, sine[j].one[k]));
-                    u[j].two[k] = fma2(two, cosine[j].one[k], mul2(one, minus2(sine[j].one[k])));
+                    cosine[j].one[k] = pack2(1.0f, 1.0f);
+                    sine[j].one[k] = 0;
                 }
-            }
-            add_unit<Form>(v[j], u[j], gain[j], squares2, product2);
-        }
-        float squares = sum2(squares2), product = sum2(product2);
-        for (int o = 1; o < lanes; o <<= 1) {
-            squares += __shfl_xor_sync(0xffffffffu, squares, o);
-            product += __shfl_xor_sync(0xffffffffu, product, o);
-        }
-        const float r = live ? inverse_root<T>(__fmaf_rn(squares, a.inverse_d, a.epsilon)) : 0.0f;
-        const float along = r * r * (product * a.inverse_d);
-#pragma unroll
-        for (int j = 0; j < U; ++j) {
-            finish_unit<Form>(v[j], u[j], gain[j], r, along, sums[j]);
-            if (live && share.there[j]) Raw::store(to + share.channel[j], apart, share.turns[j], u[j]);
-        }
-    };
-    if constexpr (PER_HEAD) {
-        if (threadIdx.x < tokens) {
-            const TokenPlaces of(a, s, token0 + static_cast<int>(threadIdx.x));
-            places[0][threadIdx.x] = of.x;
-            places[1][threadIdx.x] = of.dy;
-            places[2][threadIdx.x] = of.out;
-        }
-        chain_begin();
-        fill_gains(a, s, gains);
-        fill_angles_of<T, Form>(a, angles, token0, tokens);
-        __syncthreads();
-        int head = warp, base = 0, ahead = warp, ahead_base = 0;   // at hand, and the next to be fetched
-        auto fetch = [&] {
-            const int local = ahead_base + group;
-            const bool wanted = ahead < heads && local < tokens;
-            const int at = wanted ? local : 0;
-            fill(x + ahead * s.x_stride[1] + places[0][at], dy + ahead * s.dy_stride[1] + places[1][at], wanted);
-            if ((ahead_base += groups) >= tokens) {
-                ahead_base = 0;
-                ahead += kNormWarps;
+                if (PER_HEAD || !share.turns[j] || !own_token) continue;   // (behind the last token there are no angles: zeros stay zeros in the sums)
+                const float* table = angles + local * 2 * a.half;
+                const int place = angle_place<Form>(a, share.unit[j], 0), stride = a.turning * Form::kQuad;
+                get_angles<Form>(table, place, stride, cosine[j].one);
+                get_angles<Form>(table + a.half, place, stride, sine[j].one);
             }
         };
+        // The row at hand: u turned back, both sums, dX to `to`, and the terms of dgain.
+        auto row = [&](T* to, const float* table, bool live) {
+            Values<Form::kPacks> v[U], u[U];
+            uint64_t squares2 = 0, product2 = 0;
 #pragma unroll
-        for (int i = 0; i + 1 < kGradientStages; ++i) fetch();
+            for (int j = 0; j < U; ++j) {
+                v[j] = rows[0][j].values();
+                u[j] = rows[1][j].values();
+                if constexpr (PER_HEAD) {
+                    if (share.turns[j]) turn_unit<Form, true>(a, table, share.unit[j], u[j]);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < Form::kPacks; ++k) {
+                        const uint64_t one = u[j].one[k], two = u[j].two[k];
+                        u[j].one[k] = fma2(one, cosine[j].one[k], mul2(two, sine[j].one[k]));
+                        u[j].two[k] = fma2(two, cosine[j].one[k], mul2(one, minus2(sine[j].one[k])));
+                    }
+                }
+                add_unit<Form>(v[j], u[j], gain[j], squares2, product2);
+            }
+            float squares = sum2(squares2), product = sum2(product2);
+            for (int o = 1; o < lanes; o <<= 1) {
+                squares += __shfl_xor_sync(0xffffffffu, squares, o);
+                product += __shfl_xor_sync(0xffffffffu, product, o);
+            }
+            const float r = live ? inverse_root<T>(__fmaf_rn(squares, a.inverse_d, a.epsilon)) : 0.0f;
+            const float along = r * r * (product * a.inverse_d);
+#pragma unroll
+            for (int j = 0; j < U; ++j) {
+                finish_unit<Form>(v[j], u[j], gain[j], r, along, sums[j]);
+                if (live && share.there[j]) Raw::store(to + share.channel[j], apart, share.turns[j], u[j]);
+            }
+        };
         bool fresh = true;
-        while (head < heads) {
-            const int local = min(base + group, tokens - 1);
-            const bool live = base + group < tokens, last = base + groups >= tokens;
-            ring.take(rows);
-            fetch();
-            if (fresh) gains_of(head0 + head);
-            fresh = last && s.gain_head != 0;
-            row(dx + head * s.out_stride[1] + places[2][local], angles + local * 2 * a.half, live);
-            if (last && sums_wanted) put_sums<Form, U, V>(a, share, sums, s.partial + (static_cast<int64_t>(tile) * s.heads + head0 + head) * a.d);
-            if (last) {
-#pragma unroll
-                for (int j = 0; j < U; ++j) sums[j] = Values<Form::kPacks>{};
+        if constexpr (PER_HEAD) {
+            if (!first) __syncthreads();   // (the other pair's places are not needed any more)
+            if (threadIdx.x < tokens) {
+                const TokenPlaces of(a, s, token0 + static_cast<int>(threadIdx.x));
+                places[0][threadIdx.x] = of.x;
+                places[1][threadIdx.x] = of.dy;
+                places[2][threadIdx.x] = of.out;
             }
-            base += groups;
-            if (last) {
-                base = 0;
-                head += kNormWarps;
+            if (!first) __syncthreads();
+            angles_and_gains();
+            int head = warp, base = 0, ahead = warp, ahead_base = 0;   // at hand, and the next to be fetched
+            auto fetch = [&] {
+                const int token = ahead_base + group;
+                const bool wanted = ahead < heads && token < tokens;
+                const int at = wanted ? token : 0;
+                fill(x + ahead * s.x_stride[1] + places[0][at], dy + ahead * s.dy_stride[1] + places[1][at], wanted);
+                if ((ahead_base += groups) >= tokens) {
+                    ahead_base = 0;
+                    ahead += kNormWarps;
+                }
+            };
+#pragma unroll
+            for (int i = 0; i + 1 < kGradientStages; ++i) fetch();
+            while (head < heads) {
+                const int token = min(base + group, tokens - 1);
+                const bool live = base + group < tokens, last = base + groups >= tokens;
+                ring.take(rows);
+                fetch();
+                if (fresh) gains_of(head0 + head);
+                fresh = last && s.gain_head != 0;
+                row(dx + head * s.out_stride[1] + places[2][token], angles + token * 2 * a.half, live);
+                if (last && sums_wanted) put_sums<Form, U, V>(a, share, sums, s.partial + (static_cast<int64_t>(tile) * s.heads + head0 + head) * a.d);
+                if (last) {
+#pragma unroll
+                    for (int j = 0; j < U; ++j) sums[j] = Values<Form::kPacks>{};
+                }
+                base += groups;
+                if (last) {
+                    base = 0;
+                    head += kNormWarps;
+                }
             }
-        }
-        ring.drain();
-    } else {
-        const int local = group & mask, step = groups >> a.token_shift;   // (no more tokens than groups)
-        const bool live = local < tokens;
-        const TokenPlaces of(a, s, token0 + (live ? local : 0));
-        int head = group >> a.token_shift;
-        x += of.x + head * s.x_stride[1];
-        dy += of.dy + head * s.dy_stride[1];
-        dx += of.out + head * s.out_stride[1];
-        const int64_t x_step = step * s.x_stride[1], dy_step = step * s.dy_stride[1], dx_step = step * s.out_stride[1];
-        chain_begin();
+            ring.drain();
+        } else {
+            const int step = groups >> a.token_shift;
+            const TokenPlaces of(a, s, token0 + (own_token ? local : 0));
+            int head = group >> a.token_shift;
+            x += of.x + head * s.x_stride[1];
+            dy += of.dy + head * s.dy_stride[1];
+            dx += of.out + head * s.out_stride[1];
+            const int64_t x_step = step * s.x_stride[1], dy_step = step * s.dy_stride[1], dx_step = step * s.out_stride[1];
 #pragma unroll
-        for (int i = 0; i + 1 < kGradientStages; ++i) fill(x + i * x_step, dy + i * dy_step, live && head + i * step < heads);   // (on their way while the angles are worked out)
-        fill_gains(a, s, gains);
-        fill_angles_of<T, Form>(a, angles, token0, tokens);
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < U; ++j) {
-#pragma unroll
-            for (int k = 0; k < Form::kPacks; ++k) {
-                cosine[j].one[k] = pack2(1.0f, 1.0f);
-                sine[j].one[k] = 0;
+            for (int i = 0; i + 1 < kGradientStages; ++i) fill(x + i * x_step, dy + i * dy_step, own_token && head + i * step < heads);   // (on their way while the angles are worked out)
+            angles_and_gains();
+            while (__any_sync(0xffffffffu, head < heads)) {
+                if (fresh) gains_of(head0 + min(head, heads - 1));
+                fresh = s.gain_head != 0;
+                ring.take(rows);
+                fill(x + (kGradientStages - 1) * x_step, dy + (kGradientStages - 1) * dy_step, own_token && head + (kGradientStages - 1) * step < heads);
+                row(dx, nullptr, own_token && head < heads);
+                head += step;
+                x += x_step;
+                dy += dy_step;
+                dx += dx_step;
             }
-            if (!share.turns[j] || !live) continue;   // (behind the last token there are no angles: zeros stay zeros in the sums)
-            const float* table = angles + local * 2 * a.half;
-            const int place = angle_place<Form>(a, share.unit[j], 0), stride = a.turning * Form::kQuad;
-            get_angles<Form>(table, place, stride, cosine[j].one);
-            get_angles<Form>(table + a.half, place, stride, sine[j].one);
-        }
-        bool fresh = true;
-        while (__any_sync(0xffffffffu, head < heads)) {
-            if (fresh) gains_of(head0 + min(head, heads - 1));
-            fresh = s.gain_head != 0;
-            ring.take(rows);
-            fill(x + (kGradientStages - 1) * x_step, dy + (kGradientStages - 1) * dy_step, live && head + (kGradientStages - 1) * step < heads);
-            row(dx, nullptr, live && head < heads);
-            head += step;
-            x += x_step;
-            dy += dy_step;
-            dx += dx_step;
-        }
-        ring.drain();
-        if (!sums_wanted) return;
-        __syncthreads();   // (the angles and rows are not needed any more)
-        put_sums<Form, U, V>(a, share, sums, angles + warp * a.d);
-        __syncthreads();
-        for (int c = threadIdx.x; c < a.d; c += kNormThreads) {
-            float sum = angles[c];
+            ring.drain();
+            if (!sums_wanted) continue;
+            __syncthreads();   // (no rows are on their way any more)
+            put_sums<Form, U, V>(a, share, sums, meeting + warp * a.d);
+            __syncthreads();
+            const int64_t sum_row = static_cast<int64_t>(tile) * s.runs + (static_cast<int>(blockIdx.y) - s.first_run);
+            for (int c = threadIdx.x; c < a.d; c += kNormThreads) {
+                float sum = meeting[c];
 #pragma unroll
-            for (int w = 1; w < kNormWarps; ++w) sum += angles[w * a.d + c];
-            s.partial[(static_cast<int64_t>(tile) * runs + run) * a.d + c] = sum;
+                for (int w = 1; w < kNormWarps; ++w) sum += meeting[w * a.d + c];
+                s.partial[sum_row * a.d + c] = sum;
+            }
+            if (which == 0) __syncthreads();   // (before rows are on their way again)
         }
     }
 }
@@ -724,78 +758,83 @@ head_norm_grad_long_kernel(const __grid_constant__ NormArgs a) {
     using Raw = RawUnit<T, V, INTERLEAVED>;
     extern __shared__ __align__(16) float angles[];                   // the table, and each warp's sums behind it
     const int tile = static_cast<int>(blockIdx.x), token0 = tile << a.token_shift, tokens = min(a.tokens - token0, 1 << a.token_shift);
-    const bool second_side = static_cast<int>(blockIdx.y) >= a.first_side;
-    const NormSide& s = a.side[second_side];
-    const int run = static_cast<int>(blockIdx.y) - (second_side ? a.first_side : 0), runs = second_side ? static_cast<int>(gridDim.y) - a.first_side : a.first_side;
-    const int head0 = run * a.heads_per_cta, heads = min(a.heads_per_cta, s.heads - head0);
+    const int run0 = static_cast<int>(blockIdx.y) * a.heads_per_cta, run1 = run0 + a.heads_per_cta;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, apart = Form::apart(a);
-    const bool sums_wanted = s.partial != nullptr;
     chain_begin();
     fill_angles_of<T, Form>(a, angles, token0, tokens);
     __syncthreads();
     float* meeting = angles + ((2 * a.half) << a.token_shift);
     float* sums = meeting + warp * a.d;   // (a lane's channels are its own)
-    for (int c = lane; c < a.d; c += 32) sums[c] = 0.0f;
-    __syncwarp();
-    for (int head = warp; head < heads; head += kNormWarps) {
-        for (int local = 0; local < tokens; ++local) {
-            const TokenPlaces of(a, s, token0 + local);
-            const T* from_x = static_cast<const T*>(s.x) + (head0 + head) * s.x_stride[1] + of.x;
-            const T* from_dy = static_cast<const T*>(s.dy) + (head0 + head) * s.dy_stride[1] + of.dy;
-            T* to = static_cast<T*>(s.out) + (head0 + head) * s.out_stride[1] + of.out;
-            float r = 0.0f, along = 0.0f;
-            uint64_t squares = 0, product = 0;
-            for (int pass = 0; pass < 2; ++pass) {
-                for (int unit = lane; unit < a.units; unit += 32) {
-                    const bool turns = unit < a.turning;
-                    const int channel = Form::channel(a, unit);
-                    Raw raw_x, raw_dy;
-                    raw_x.load(from_x + channel, apart, true, turns);
-                    raw_dy.load(from_dy + channel, apart, true, turns);
-                    const Values<Form::kPacks> v = raw_x.values();
-                    Values<Form::kPacks> u = raw_dy.values(), gain, terms{};
-                    load_gains<Form, V>(a, s, s.gain_head ? head0 + head : 0, channel, true, turns, gain);
-                    if (turns) turn_unit<Form, true>(a, angles + local * 2 * a.half, unit, u);
+#pragma unroll 1
+    for (int which = 0; which < 2; ++which) {
+        const NormSide& s = a.side[which];
+        const int before = which ? a.side[0].heads : 0, head0 = max(run0 - before, 0), heads = min(run1 - before, s.heads) - head0;
+        if (heads <= 0) continue;
+        const bool sums_wanted = s.partial != nullptr;
+        for (int c = lane; c < a.d; c += 32) sums[c] = 0.0f;
+        __syncwarp();
+        for (int head = warp; head < heads; head += kNormWarps) {
+            for (int local = 0; local < tokens; ++local) {
+                const TokenPlaces of(a, s, token0 + local);
+                const T* from_x = static_cast<const T*>(s.x) + (head0 + head) * s.x_stride[1] + of.x;
+                const T* from_dy = static_cast<const T*>(s.dy) + (head0 + head) * s.dy_stride[1] + of.dy;
+                T* to = static_cast<T*>(s.out) + (head0 + head) * s.out_stride[1] + of.out;
+                float r = 0.0f, along = 0.0f;
+                uint64_t squares = 0, product = 0;
+                for (int pass = 0; pass < 2; ++pass) {
+                    for (int unit = lane; unit < a.units; unit += 32) {
+                        const bool turns = unit < a.turning;
+                        const int channel = Form::channel(a, unit);
+                        Raw raw_x, raw_dy;
+                        raw_x.load(from_x + channel, apart, true, turns);
+                        raw_dy.load(from_dy + channel, apart, true, turns);
+                        const Values<Form::kPacks> v = raw_x.values();
+                        Values<Form::kPacks> u = raw_dy.values(), gain, terms{};
+                        load_gains<Form, V>(a, s, s.gain_head ? head0 + head : 0, channel, true, turns, gain);
+                        if (turns) turn_unit<Form, true>(a, angles + local * 2 * a.half, unit, u);
+                        if (pass == 0) {
+                            add_unit<Form>(v, u, gain, squares, product);
+                            continue;
+                        }
+                        finish_unit<Form>(v, u, gain, r, along, terms);
+                        Raw::store(to + channel, apart, turns, u);
+#pragma unroll
+                        for (int k = 0; k < Form::kPacks; ++k) {
+                            float term[2][2];
+                            unpack2(terms.one[k], term[0][0], term[0][1]);
+                            unpack2(terms.two[k], term[1][0], term[1][1]);
+#pragma unroll
+                            for (int second = 0; second < 2; ++second)
+#pragma unroll
+                                for (int half = 0; half < 2; ++half)
+                                    if ((!second || !Form::kTwo || turns) && (V > 1 || half == 0)) sums[channel + (second && Form::kTwo ? apart : 0) + Form::place(k, half, second != 0)] += term[second][half];
+                        }
+                    }
                     if (pass == 0) {
-                        add_unit<Form>(v, u, gain, squares, product);
-                        continue;
-                    }
-                    finish_unit<Form>(v, u, gain, r, along, terms);
-                    Raw::store(to + channel, apart, turns, u);
-#pragma unroll
-                    for (int k = 0; k < Form::kPacks; ++k) {
-                        float term[2][2];
-                        unpack2(terms.one[k], term[0][0], term[0][1]);
-                        unpack2(terms.two[k], term[1][0], term[1][1]);
-#pragma unroll
-                        for (int second = 0; second < 2; ++second)
-#pragma unroll
-                            for (int half = 0; half < 2; ++half)
-                                if ((!second || !Form::kTwo || turns) && (V > 1 || half == 0)) sums[channel + (second && Form::kTwo ? apart : 0) + Form::place(k, half, second != 0)] += term[second][half];
+                        r = inverse_root<T>(__fmaf_rn(sum_over(sum2(squares), 32), a.inverse_d, a.epsilon));
+                        along = r * r * (sum_over(sum2(product), 32) * a.inverse_d);
                     }
                 }
-                if (pass == 0) {
-                    r = inverse_root<T>(__fmaf_rn(sum_over(sum2(squares), 32), a.inverse_d, a.epsilon));
-                    along = r * r * (sum_over(sum2(product), 32) * a.inverse_d);
+            }
+            if (s.per_head && sums_wanted) {
+                __syncwarp();
+                for (int c = lane; c < a.d; c += 32) {
+                    s.partial[(static_cast<int64_t>(tile) * s.heads + head0 + head) * a.d + c] = sums[c];
+                    sums[c] = 0.0f;
                 }
+                __syncwarp();
             }
         }
-        if (s.per_head && sums_wanted) {
-            __syncwarp();
-            for (int c = lane; c < a.d; c += 32) {
-                s.partial[(static_cast<int64_t>(tile) * s.heads + head0 + head) * a.d + c] = sums[c];
-                sums[c] = 0.0f;
-            }
-            __syncwarp();
-        }
-    }
-    if (s.per_head || !sums_wanted) return;
-    __syncthreads();
-    for (int c = threadIdx.x; c < a.d; c += kNormThreads) {
-        float sum = meeting[c];
+        if (s.per_head || !sums_wanted) continue;
+        __syncthreads();
+        const int64_t sum_row = static_cast<int64_t>(tile) * s.runs + (static_cast<int>(blockIdx.y) - s.first_run);
+        for (int c = threadIdx.x; c < a.d; c += kNormThreads) {
+            float sum = meeting[c];
 #pragma unroll
-        for (int w = 1; w < kNormWarps; ++w) sum += meeting[w * a.d + c];
-        s.partial[(static_cast<int64_t>(tile) * runs + run) * a.d + c] = sum;
+            for (int w = 1; w < kNormWarps; ++w) sum += meeting[w * a.d + c];
+            s.partial[sum_row * a.d + c] = sum;
+        }
+        __syncthreads();
     }
 }
 
@@ -808,33 +847,52 @@ struct GainSide {
 };
 struct GainArgs {
     GainSide side[2];
-    int32_t first_blocks;
+    int32_t first_blocks, cluster;   // cluster: CTAs that share a block's rows
 };
-// 16 columns a CTA, 64 rows at a time: what bounds it is the latency of a thread's loads, which are few and all on their way at once.
-constexpr int kGainColumns = 16;
+// 16 columns a CTA, 64 rows at a time: what bounds it is the latency of a thread's loads, which are few and all on their way at once. Many rows are shared out
+// over a cluster, whose sums meet in order (3518 + 3518 rows of 128 columns: 15 us by one CTA each).
+constexpr int kGainColumns = 16, kGainCluster = 8;
 __global__ void __launch_bounds__(1024)
 gain_sums_kernel(const __grid_constant__ GainArgs a) {
     __shared__ double sums[32][kGainColumns];
-    const int which = static_cast<int>(blockIdx.x) >= a.first_blocks;
+    __shared__ double whole[kGainColumns];
+    const int block = static_cast<int>(blockIdx.x) / a.cluster, rank = static_cast<int>(blockIdx.x) - block * a.cluster;
+    const int which = block >= a.first_blocks;
     const GainSide& s = a.side[which];
     const int tx = threadIdx.x % kGainColumns, ty = threadIdx.x / kGainColumns;
-    const int64_t column = (static_cast<int64_t>(blockIdx.x) - (which ? a.first_blocks : 0)) * kGainColumns + tx;
+    const int64_t column = (static_cast<int64_t>(block) - (which ? a.first_blocks : 0)) * kGainColumns + tx;
     chain_begin();
     double sum = 0.0;
     if (column < s.columns) {
         const float* from = s.partial + column;
+        const int step = a.cluster * (1024 / kGainColumns);
 #pragma unroll 8
-        for (int64_t row = ty; row < s.rows; row += 1024 / kGainColumns) sum += static_cast<double>(from[row * s.columns]);
+        for (int64_t row = rank * (1024 / kGainColumns) + ty; row < s.rows; row += step) sum += static_cast<double>(from[row * s.columns]);
     }
     sum += __shfl_xor_sync(0xffffffffu, sum, 16);
     if ((threadIdx.x & 16) == 0) sums[threadIdx.x >> 5][tx] = sum;
     __syncthreads();
-    if (threadIdx.x >= 32) return;
-    sum = 0.0;
+    if (threadIdx.x < 32) {
+        sum = 0.0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) sum += sums[(threadIdx.x >> 4) * 16 + i][tx];
-    sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-    if (threadIdx.x >= 16 || column >= s.columns) return;
+        for (int i = 0; i < 16; ++i) sum += sums[(threadIdx.x >> 4) * 16 + i][tx];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        if (threadIdx.x < 16) whole[tx] = sum;
+    }
+    if (a.cluster > 1) {
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        if (rank == 0 && threadIdx.x < 16) {
+            for (int r = 1; r < a.cluster; ++r) {
+                uint32_t remote;
+                double other;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(&whole[tx])), "r"(r));
+                asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(other) : "r"(remote) : "memory");
+                sum += other;
+            }
+        }
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");   // (no CTA leaves while its sums are read)
+    }
+    if (rank != 0 || threadIdx.x >= 16 || column >= s.columns) return;
     const int64_t head = column / s.d;
     store_from_f32(s.out, s.type, head * s.out_head + (column - head * s.d), static_cast<float>(sum));
 }
@@ -875,14 +933,19 @@ struct NormProblem {
     float scale, epsilon, gain_offset;
     bool two;
     int width;                        // values a vector
+    // (where nothing turns pairs may be anywhere: side by side a unit is one vector, all of which counts)
+    NormProblem without_pairs() {
+        if (positions->rank == 0) interleaved = 1;
+        return *this;
+    }
 };
 NormProblem problem_of(const dfgpu_head_norm_params& p) {
     return NormProblem{{{&p.x, &p.y, nullptr}, {&p.x2, &p.y2, nullptr}}, {&p.gain, &p.gain2}, {nullptr, nullptr}, &p.positions, &p.frequencies, 2, p.interleaved, p.kernel, p.scale,
-                       p.epsilon, p.gain_offset, p.x2.rank != 0 || p.y2.rank != 0, 1};
+                       p.epsilon, p.gain_offset, p.x2.rank != 0 || p.y2.rank != 0, 1}.without_pairs();
 }
 NormProblem problem_of(const dfgpu_head_norm_grad_params& p) {
     return NormProblem{{{&p.x, &p.dy, &p.dx}, {&p.x2, &p.dy2, &p.dx2}}, {&p.gain, &p.gain2}, {&p.dgain, &p.dgain2}, &p.positions, &p.frequencies, 3, p.interleaved, p.kernel, p.scale,
-                       p.epsilon, p.gain_offset, p.x2.rank != 0 || p.dy2.rank != 0 || p.dx2.rank != 0, 1};
+                       p.epsilon, p.gain_offset, p.x2.rank != 0 || p.dy2.rank != 0 || p.dx2.rank != 0, 1}.without_pairs();
 }
 // Values to a vector by the descriptors alone: 16 bytes, 8 (of 16-bit types), or one value.
 int norm_width(const NormProblem& p) {
@@ -1015,6 +1078,7 @@ int build_norm(NormProblem& p, void* const (&pointers)[2][3], const void* positi
     const int64_t d = x.dim[3];
     const LaneForm form = lane_form(p, p.width);
     a.d = static_cast<int>(d);
+    a.by_d = make_fast_divisor(static_cast<uint32_t>(d));
     a.turning = form.turning;
     a.units = form.units;
     a.group_shift = form.group_shift;
@@ -1032,13 +1096,14 @@ int build_norm(NormProblem& p, void* const (&pointers)[2][3], const void* positi
 // Ring::kBytes
 constexpr size_t ring_bytes(int stages, int tensors) { return static_cast<size_t>(32) * stages * tensors * kNormThreads; }
 
-enum NormKernel { kForward, kForwardLong, kGradient, kGradientOfHeads, kGradientLong };
+enum NormKernel { kForward, kForwardOfHeads, kForwardLong, kGradient, kGradientOfHeads, kGradientLong };
 template <typename T, int V, bool INTERLEAVED>
 void launch_norm(NormKernel kernel, const NormArgs& a, dim3 grid, size_t shared, cudaStream_t stream) {
     void (*function)(const NormArgs) = head_norm_long_kernel<T, V, INTERLEAVED>;
     if (kernel == kGradientLong) function = head_norm_grad_long_kernel<T, V, INTERLEAVED>;
     if constexpr (V > 1) {
-        if (kernel == kForward) function = head_norm_kernel<T, V, INTERLEAVED>;
+        if (kernel == kForward) function = head_norm_kernel<T, V, INTERLEAVED, false>;
+        if (kernel == kForwardOfHeads) function = head_norm_kernel<T, V, INTERLEAVED, true>;
         if (kernel == kGradient) function = head_norm_grad_kernel<T, V, INTERLEAVED, false>;
         if (kernel == kGradientOfHeads) function = head_norm_grad_kernel<T, V, INTERLEAVED, true>;
     }
@@ -1066,7 +1131,7 @@ void launch_norm(NormKernel kernel, const NormArgs& a, int dtype, int width, boo
 // The gradient's cut: tokens a CTA (1 << shift) and heads a run. A function of the descriptors alone: the scratch depends on it.
 struct GradCut {
     int shift, heads_per_cta;
-    int64_t tiles, runs[2];
+    int64_t tiles, runs, of_side[2], first_of_second;   // runs of heads: all, and those that hold some of a side's
 };
 bool sums_of_heads(const dfgpu_tensor& dgain) { return dgain.rank && dgain.dim[1] > 1; }
 bool any_sums_of_heads(const NormProblem& p) { return sums_of_heads(*p.dgain[0]) || (p.two && sums_of_heads(*p.dgain[1])); }
@@ -1075,8 +1140,8 @@ GradCut grad_cut(const NormProblem& p) {
     const int64_t half = p.positions->rank ? p.frequencies->dim[3] : 0;
     const int64_t tokens = x.dim[0] * x.dim[2], heads[2] = {x.dim[1], p.two ? p.row[1][0]->dim[1] : 0};
     GradCut cut{};
-    // With sums for each head 16 tokens and few heads (3 x 1001 f32 tokens of 32 heads: four heads 35.1 us, eight 38.6; 32 tokens 37.6 and 58.7, eight tokens 38.7 and 37.8); otherwise
-    // as many tokens as there are groups of lanes and many heads (4 x 2048 bf16 tokens of 32 + 8 heads: 32 heads 51.3 us, 16 57.1, 8 66.8; eight tokens 54.9, 64.5, 82.8).
+    // With sums for each head 16 tokens and few heads (3 x 1001 f32 tokens of 32 heads: four or eight heads 37.5 us, 16 61.8; eight tokens 43.9, 41.4 and 41.3); otherwise
+    // as many tokens as there are groups of lanes and many heads (4 x 2048 bf16 tokens of 32 + 8 heads: 40 heads 50.5 us, 32 50.4, 20 56.2, 10 61.0; eight tokens 51.4, 51.9, 58.3, 72.7).
     const bool of_heads = any_sums_of_heads(p);
     cut.shift = 4;
     if (!of_heads) {
@@ -1084,13 +1149,16 @@ GradCut grad_cut(const NormProblem& p) {
         cut.shift = std::min(7 - form.group_shift, 5);
     }
     while (cut.shift > 0 && 8 * (half << cut.shift) > kNormShared) --cut.shift;
-    cut.heads_per_cta = 32;
+    cut.heads_per_cta = static_cast<int>(std::min<int64_t>(heads[0] + heads[1], 40));
     auto ctas = [&] {
         cut.tiles = (tokens + (1ll << cut.shift) - 1) >> cut.shift;
-        for (int s = 0; s < 2; ++s) cut.runs[s] = (heads[s] + cut.heads_per_cta - 1) / cut.heads_per_cta;
-        return cut.tiles * (cut.runs[0] + cut.runs[1]);
+        cut.runs = (heads[0] + heads[1] + cut.heads_per_cta - 1) / cut.heads_per_cta;
+        cut.of_side[0] = (heads[0] + cut.heads_per_cta - 1) / cut.heads_per_cta;
+        cut.first_of_second = heads[0] / cut.heads_per_cta;
+        cut.of_side[1] = cut.runs - cut.first_of_second;
+        return cut.tiles * cut.runs;
     };
-    while (ctas() < (of_heads ? 10 : 6) * 148 && cut.heads_per_cta > 4) cut.heads_per_cta /= 2;
+    while (ctas() < (of_heads ? 10 : 3) * 148 && cut.heads_per_cta > 4) cut.heads_per_cta = (cut.heads_per_cta + 1) / 2;
     while (ctas() < 4 * 148 && cut.shift > 2) --cut.shift;
     ctas();
     return cut;
@@ -1098,7 +1166,7 @@ GradCut grad_cut(const NormProblem& p) {
 // Floats of partial sums of a side, none where no dgain is wanted.
 int64_t grad_partials(const NormProblem& p, const GradCut& cut, int s) {
     if ((s == 1 && !p.two) || p.dgain[s]->rank == 0) return 0;
-    return cut.tiles * p.row[s][0]->dim[3] * (any_sums_of_heads(p) ? p.row[s][0]->dim[1] : cut.runs[s]);
+    return cut.tiles * p.row[s][0]->dim[3] * (any_sums_of_heads(p) ? p.row[s][0]->dim[1] : cut.of_side[s]);
 }
 
 }  // namespace
@@ -1136,12 +1204,15 @@ extern "C" int dfgpu_head_norm(const dfgpu_head_norm_params* params, void* const
     a.tiles = (a.seq + (1 << a.token_shift) - 1) >> a.token_shift;
     a.by_tiles = make_fast_divisor(static_cast<uint32_t>(a.tiles));
     const int64_t tiles = p.row[0][0]->dim[0] * a.tiles;
-    a.heads_per_cta = heads;
+    // (gains of each head take 4 KiB of shared memory for eight heads of 128 channels)
+    const bool gains_of_heads = a.side[0].gain_head || a.side[1].gain_head;
+    a.heads_per_cta = gains_of_heads && per_lane ? std::min(heads, std::max(kNormGains / (4 * a.d), 1)) : heads;
     auto runs = [&] { return (heads + a.heads_per_cta - 1) / a.heads_per_cta; };
     while (tiles * runs() < 8 * 148 && (a.heads_per_cta << a.token_shift) > groups && a.heads_per_cta > 1) a.heads_per_cta = (a.heads_per_cta + 1) / 2;
     const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(runs()));
-    const size_t shared = sizeof(float) * static_cast<size_t>((2 * a.half) << a.token_shift) + (per_lane ? 8 * static_cast<size_t>(a.d) + ring_bytes(kForwardStages, 1) : 0);
-    launch_norm(per_lane ? kForward : kForwardLong, a, p.row[0][0]->dtype, p.width, p.interleaved != 0, grid, shared, as_stream(stream));
+    a.gain_floats = a.d * (gains_of_heads ? a.heads_per_cta + 1 : 2);
+    const size_t shared = sizeof(float) * static_cast<size_t>((2 * a.half) << a.token_shift) + (per_lane ? 4 * static_cast<size_t>(a.gain_floats) + ring_bytes(kForwardStages, 1) : 0);
+    launch_norm(!per_lane ? kForwardLong : gains_of_heads ? kForwardOfHeads : kForward, a, p.row[0][0]->dtype, p.width, p.interleaved != 0, grid, shared, as_stream(stream));
     return check_launch("HEAD_NORM");
 }
 
@@ -1195,7 +1266,7 @@ extern "C" int dfgpu_head_norm_grad(const dfgpu_head_norm_grad_params* params, v
         sums.partial = side.partial;
         sums.out = out;
         sums.d = a.d;
-        sums.rows = cut.tiles * (apart ? 1 : side.per_head ? side.heads : cut.runs[s]);
+        sums.rows = cut.tiles * (apart ? 1 : side.per_head ? side.heads : cut.of_side[s]);
         sums.columns = apart ? static_cast<int64_t>(side.heads) * a.d : a.d;
         sums.out_head = apart ? dgain.stride[1] : 0;
         sums.type = dgain.dtype;
@@ -1205,17 +1276,21 @@ extern "C" int dfgpu_head_norm_grad(const dfgpu_head_norm_grad_params* params, v
     }
     a.token_shift = cut.shift;
     a.heads_per_cta = cut.heads_per_cta;
-    a.first_side = static_cast<int>(cut.runs[0]);
-    const dim3 grid(static_cast<unsigned>(cut.tiles), static_cast<unsigned>(cut.runs[0] + cut.runs[1]));
+    for (int s = 0; s < 2; ++s) {
+        a.side[s].runs = static_cast<int>(cut.of_side[s]);
+        a.side[s].first_run = s ? static_cast<int>(cut.first_of_second) : 0;
+    }
+    const dim3 grid(static_cast<unsigned>(cut.tiles), static_cast<unsigned>(cut.runs));
     const size_t table = sizeof(float) * static_cast<size_t>((2 * a.half) << a.token_shift), meeting = sizeof(float) * kNormWarps * static_cast<size_t>(a.d);
     // (the form for tokens a group needs as many groups as tokens; with narrower vectors than the cut had in mind a row may take more lanes)
     const bool of_heads = any_sums_of_heads(p);
     if (per_lane && !of_heads && (kNormThreads >> a.group_shift) < (1 << a.token_shift)) per_lane = 0;
     launch_norm(!per_lane ? kGradientLong : of_heads ? kGradientOfHeads : kGradient, a, p.row[0][0]->dtype, p.width, p.interleaved != 0, grid,
-                per_lane ? std::max(table + 4 * static_cast<size_t>(a.d) + ring_bytes(kGradientStages, 2), meeting) : table + meeting,
+                table + (per_lane ? 8 * static_cast<size_t>(a.d) + std::max(ring_bytes(kGradientStages, 2), meeting) : meeting),
                                 as_stream(stream));
     status = check_launch("HEAD_NORM gradient");
     if (status || !blocks) return status;
-    launch_chained(gain_sums_kernel, dim3(static_cast<unsigned>(blocks)), dim3(1024), 0, as_stream(stream), g);
+    g.cluster = std::max(g.side[0].rows, g.side[1].rows) > 1024 ? kGainCluster : 1;
+    launch_chained_cluster(gain_sums_kernel, dim3(static_cast<unsigned>(blocks * g.cluster)), dim3(1024), g.cluster > 1 ? kGainCluster : 0u, 0, as_stream(stream), g);
     return check_launch("HEAD_NORM gradient, dgain");
 }
