@@ -21,7 +21,7 @@ namespace dfgpu {
 namespace {
 
 constexpr int kScanWarps = 16;
-constexpr int kCandidates = 64;   // of a CTA, that are sorted at once
+constexpr int kCandidates = 256;  // of a CTA, that are sorted at once (32 beams leave some 130)
 constexpr int kMaxBeams = 32;
 constexpr float kLog2e = 1.44269504088896341f;
 

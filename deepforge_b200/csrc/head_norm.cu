@@ -1234,13 +1234,13 @@ extern "C" int dfgpu_head_norm_grad(const dfgpu_head_norm_grad_params* params, v
     NormProblem p = problem_of(*params);
     int status = check_norm(p);
     if (status) return status;
+    const GradCut cut = grad_cut(p);   // (by the descriptors, as the query has it: places off the vectors' boundaries change the width below)
     NormArgs a{};
     int per_lane;
     void* const rows[2][3] = {{tensors[0], tensors[1], tensors[2]}, {p.two ? tensors[7] : nullptr, p.two ? tensors[8] : nullptr, p.two ? tensors[9] : nullptr}};
     const void* const gains[2] = {p.gain[0]->rank ? tensors[3] : nullptr, p.gain[1]->rank ? tensors[10] : nullptr};
     status = build_norm(p, rows, p.positions->rank ? tensors[5] : nullptr, p.positions->rank ? tensors[6] : nullptr, gains, a, per_lane);
     if (status) return status;
-    const GradCut cut = grad_cut(p);
     const int64_t first_partials = grad_partials(p, cut, 0), partials = first_partials + grad_partials(p, cut, 1);
     if (partials && (!scratch || !aligned(scratch, 4))) return fail(kInvalidArgument, "HEAD_NORM gradient: %s", scratch ? "the scratch is not aligned" : "scratch is needed for the sums of dgain");
     GainArgs g{};
@@ -1255,7 +1255,7 @@ extern "C" int dfgpu_head_norm_grad(const dfgpu_head_norm_grad_params* params, v
         for (int o = 0; o < (p.two ? 2 : 1); ++o) {
             for (int t = 0; t < 3; ++t)
                 if (overlaps(region, region_of(rows[o][t], *p.row[o][t]))) return fail(kInvalidArgument, "HEAD_NORM gradient: a dgain overlaps another tensor");
-            if (overlaps(region, region_of(gains[o], *p.gain[o])) || (o != s && overlaps(region, region_of(tensors[o ? 11 : 4], *p.dgain[o]))))
+            if (overlaps(region, region_of(gains[o], *p.gain[o])) || (o != s && p.dgain[o]->rank && overlaps(region, region_of(tensors[o ? 11 : 4], *p.dgain[o]))))
                 return fail(kInvalidArgument, "HEAD_NORM gradient: a dgain overlaps another gain");
         }
         NormSide& side = a.side[s];

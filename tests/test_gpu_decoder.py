@@ -91,12 +91,16 @@ class Heads:
                 dgain[i] = torch.full((1, x.shape[3]) if g is None else g.shape, 7.0, device="cuda", dtype=dgain_type)
                 setattr(p, "dgain" + n, self.gain_descriptor(dgain[i]))
         info = decoder.query("head_norm_grad", p)
+        room, behind = scratch, None
         if scratch is None:
-            scratch = torch.full((max(4, info.scratch_bytes),), 255, device="cuda", dtype=torch.uint8)
+            room = torch.full((info.scratch_bytes + (1 << 16),), 255, device="cuda", dtype=torch.uint8)
+            scratch, behind = room, room[info.scratch_bytes:]
         pointers = [address(self.x[0]), address(self.dy[0]), address(dx[0]), address(self.gain[0]), address(dgain[0]), address(self.positions), address(self.frequencies)]
         if len(dx) == 2:
             pointers += [address(self.x[1]), address(self.dy[1]), address(dx[1]), address(self.gain[1]), address(dgain[1])]
         decoder.head_norm_grad(p, pointers, scratch.data_ptr(), stream=stream)
+        if behind is not None:   # no more is written than the query said
+            assert torch.all(behind == 255)
         return dx, dgain
 
     def parts(self, i):
@@ -451,10 +455,14 @@ def select(logits, scores, finished=None, lengths=None, penalty=0.0, end=-1, pad
             setattr(p, name, describe(t))
     if bases is not None:
         p.source_base, p.target_base = bases
+    behind = None
     if scratch is None:
-        scratch = torch.full((decoder.query("beam_select", p).scratch_bytes,), 255, device="cuda", dtype=torch.uint8)
+        size = decoder.query("beam_select", p).scratch_bytes
+        scratch = torch.full((size + 4096,), 255, device="cuda", dtype=torch.uint8)
+        behind = scratch[size:]
     decoder.beam_select(p, [address(given[n]) for n in ("logits", "scores", "finished", "lengths", "scores_out", "tokens", "parents", "finished_out", "lengths_out", "forks")],
                         scratch.data_ptr(), stream=stream)
+    assert behind is None or torch.all(behind == 255)   # no more is written than the query said
     return out
 
 
