@@ -1,44 +1,64 @@
 // Rows to 8-bit integers with a scale each: scale = max |x| / 127, code = x / scale to the nearest whole number.
 //
-// HBM bounds it (2 or 4 bytes in, 1 out for a value); the scale has to be known before the first code, so a row's vectors stay in registers between the two
-// (what a row has beyond them is read again, from the cache).
+// HBM bounds it (2 or 4 bytes in, 1 out for a value), and close behind it the instructions of each value; the scale has to be known before the first code, so a row's
+// vectors stay in registers between the two (what a row has beyond them is read again, from the cache). Alone, with more data than the L2 holds, 8192 x 4096: 25 us from
+// bf16 (the bytes alone 15.4), 29 from f32 (25.7); 32 x 4096 2.1 to 2.6; rows of 4097 that are not whole vectors, 5000 of them, 33 (9.4), value by value.
 #include <algorithm>
 
 #include "common.cuh"
 #include "dfgpu_decoder.h"
 #include "ports.cuh"
 #include "rotary.cuh"
+#include "umma_ptx.cuh"
 
 namespace dfgpu {
 namespace {
-
-constexpr int kHeld = 8;          // vectors that a thread keeps
 
 struct QuantizeArgs {
     const void* x;
     int8_t* y;
     float* scale;
     int64_t x_stride[3], y_stride[3], scale_stride[3];   // the axes before K, the last of them first
-    int32_t k, vectors;                                  // of a row
+    int32_t k, vectors, flat;                            // of a row; flat: one axis before K
     int64_t rows;
     FastDivisor by[2];                                   // extents of the last two axes before K
 };
 
-// The largest |x|, ordered like whole numbers: a NaN is above all.
-template <typename T, int V>
-__device__ __forceinline__ uint32_t magnitude_bits(const Pack<T, V>& x, uint32_t bits) {
+// The largest |x|: without their signs floats are ordered like whole numbers, a NaN above all; of 16-bit values two at a time.
+template <typename T>
+struct Largest {
+    uint32_t bits = 0;
+    template <int V>
+    __device__ __forceinline__ void take(const Pack<T, V>& x) {
+        if constexpr (sizeof(T) == 2 && V > 1) {
+            const uint32_t* pairs = reinterpret_cast<const uint32_t*>(&x);
 #pragma unroll
-    for (int i = 0; i < V; ++i) bits = max(bits, __float_as_uint(widen(x.v[i])) & 0x7fffffffu);
-    return bits;
-}
+            for (int i = 0; i < V / 2; ++i) bits = __vmaxu2(bits, pairs[i] & 0x7fff7fffu);
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) bits = max(bits, whole(x.v[i]));
+        }
+    }
+    static __device__ __forceinline__ uint32_t whole(T v) {
+        if constexpr (sizeof(T) == 2) return *reinterpret_cast<const uint16_t*>(&v) & 0x7fffu;
+        else return __float_as_uint(v) & 0x7fffffffu;
+    }
+    __device__ __forceinline__ uint32_t as_f32() const {
+        if constexpr (sizeof(T) == 4) return bits;
+        const uint16_t top = static_cast<uint16_t>(max(bits & 0xffffu, bits >> 16));
+        return __float_as_uint(widen(*reinterpret_cast<const T*>(&top))) & 0x7fffffffu;
+    }
+};
 __device__ __forceinline__ int8_t exact_code(float x, float scale) {
     const float q = __fdiv_rn(x, scale);
     return q != q ? 0 : static_cast<int8_t>(__float2int_rn(fminf(fmaxf(q, -127.0f), 127.0f)));
 }
-// The codes of a vector. A division a value would cost three times the memory's time, so x times 1 / scale (each rounded: within 2^-23 of the quotient, 1.5e-5 of 127 codes
-// at most, and the f32 quotient 4e-6 more) is rounded by adding 1.5 * 2^23, whose low byte is the code; a vector with a product that close to a half, one in 1500 of
-// eight values, is divided after all, and so the code is always that of the f32 quotient.
-constexpr float kNear = 0.5f - 4e-5f;
+// The codes of a vector. A division a value would cost three times the memory's time, so x / scale is rounded as x times 1 / scale plus 1.5 * 2^23, one rounding whose low
+// byte is the code: the product of the rounded inverse is within 2^-24 of the quotient, 7.6e-6 of 127 codes at most, and the f32 quotient 4e-6 more. Of a product that
+// close to a half h (one in 500 normal bf16 values, most of them exact halves of what scale was rounded from) e = x - h scale is exact in f32, since so much cancels:
+// below half a step of f32 at h (times scale) the f32 quotient is h and goes to the even code, above it the sign of e decides, and only in between it is divided after all.
+// So the code is always that of the f32 quotient.
+constexpr float kNear = 0.5f - 4e-5f, kMove = 12582912.0f;
 template <typename T, int V>
 struct alignas(V) Codes {
     int8_t v[V];
@@ -46,34 +66,65 @@ struct alignas(V) Codes {
 template <typename T, int V>
 __device__ __forceinline__ Codes<T, V> encode(const Pack<T, V>& x, float scale, float inverse, bool plain) {
     Codes<T, V> codes;
-    float farthest = 0.5f;
     if (plain) {
-        farthest = 0.0f;
-        uint32_t bits[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float q = widen(x.v[i]) * inverse, moved = q + 12582912.0f;
-            bits[i] = __float_as_uint(moved);
-            farthest = fmaxf(farthest, fabsf(q - (moved - 12582912.0f)));
-        }
+        float farthest = 0.0f;
         if constexpr (V >= 4) {
+            uint32_t bits[V];
+            const uint64_t by = pack2(inverse, inverse), move = pack2(kMove, kMove), minus = pack2(-1.0f, -1.0f);
+#pragma unroll
+            for (int i = 0; i < V; i += 2) {
+                const uint64_t two = pack2(widen(x.v[i]), widen(x.v[i + 1])), moved = fma2(two, by, move);
+                const uint64_t rest = fma2(two, by, fma2(moved, minus, move));
+                float lo, hi;
+                unpack2(moved, lo, hi);
+                bits[i] = __float_as_uint(lo);
+                bits[i + 1] = __float_as_uint(hi);
+                unpack2(rest, lo, hi);
+                asm("max.abs.f32 %0, %0, %1, %2;" : "+f"(farthest) : "f"(lo), "f"(hi));
+            }
             uint32_t* words = reinterpret_cast<uint32_t*>(&codes);
 #pragma unroll
             for (int i = 0; i < V / 4; ++i) words[i] = __byte_perm(__byte_perm(bits[4 * i], bits[4 * i + 1], 0x0040), __byte_perm(bits[4 * i + 2], bits[4 * i + 3], 0x0040), 0x5410);
         } else {
 #pragma unroll
-            for (int i = 0; i < V; ++i) codes.v[i] = static_cast<int8_t>(bits[i]);
+            for (int i = 0; i < V; ++i) {
+                const float moved = __fmaf_rn(widen(x.v[i]), inverse, kMove);
+                codes.v[i] = static_cast<int8_t>(__float_as_uint(moved));
+                farthest = fmaxf(farthest, fabsf(__fmaf_rn(widen(x.v[i]), inverse, -(moved - kMove))));
+            }
         }
-    }
-    if (farthest >= kNear) {
+        if (farthest >= kNear) {
+            uint32_t near = 0;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                const float v = widen(x.v[i]);
+                if (fabsf(__fmaf_rn(v, inverse, kMove - __fmaf_rn(v, inverse, kMove))) >= kNear) near |= 1u << i;
+            }
+            for (; near != 0; near &= near - 1) {   // (hardly ever two)
+                const int at = __ffs(static_cast<int>(near)) - 1;
+                float v = 0.0f;
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (i == at) v = widen(x.v[i]);
+                const float whole = __fmaf_rn(v, inverse, kMove) - kMove, rest = __fmaf_rn(v, inverse, -whole);
+                const float half = whole + copysignf(0.5f, rest), e = __fmaf_rn(-half, scale, v);
+                const float step = __uint_as_float((__float_as_uint(half) & 0x7f800000u) - (24u << 23)) * scale;
+                const float decided = fabsf(e) < step ? half : e > 0.0f ? half + 0.5f : half - 0.5f;
+                const int8_t code = fabsf(e) == step ? exact_code(v, scale) : static_cast<int8_t>(__float_as_uint(decided + kMove));
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if (i == at) codes.v[i] = code;
+            }
+        }
+    } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) codes.v[i] = scale > 0.0f ? exact_code(widen(x.v[i]), scale) : 0;   // (0 for a NaN scale too)
     }
     return codes;
 }
 
-// A row is taken by `THREADS` threads: a warp (four rows a CTA) or a CTA.
-template <typename T, int V, int THREADS>
+// A row is taken by `THREADS` threads, a warp (four rows a CTA) or a CTA, which keep kHeld vectors each.
+template <typename T, int V, int THREADS, int kHeld>
 __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS)
 token_quantize_kernel(const QuantizeArgs a) {
     __shared__ uint32_t largest[THREADS / 32];
@@ -81,22 +132,26 @@ token_quantize_kernel(const QuantizeArgs a) {
     const int64_t row = THREADS == 32 ? static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5) : static_cast<int64_t>(blockIdx.x);
     chain_begin();
     if (row >= a.rows) return;
-    const uint32_t outer = fast_divide(static_cast<uint32_t>(row), a.by[0]), inner = static_cast<uint32_t>(row) - outer * a.by[0].divisor;
-    const uint32_t first = fast_divide(outer, a.by[1]), middle = outer - first * a.by[1].divisor;
-    const T* x = static_cast<const T*>(a.x) + inner * a.x_stride[0] + middle * a.x_stride[1] + first * a.x_stride[2];
-    int8_t* y = a.y + inner * a.y_stride[0] + middle * a.y_stride[1] + first * a.y_stride[2];
-    Pack<T, V> held[kHeld];
-    uint32_t bits = 0;
-#pragma unroll
-    for (int j = 0; j < kHeld; ++j) {
-        const int at = thread + j * THREADS;
-        if (at < a.vectors) held[j] = *reinterpret_cast<const Pack<T, V>*>(x + static_cast<int64_t>(at) * V);
+    int64_t axis[3] = {row, 0, 0};
+    if (!a.flat) {
+        const uint32_t outer = fast_divide(static_cast<uint32_t>(row), a.by[0]);
+        axis[0] = static_cast<uint32_t>(row) - outer * a.by[0].divisor;
+        axis[2] = fast_divide(outer, a.by[1]);
+        axis[1] = outer - static_cast<uint32_t>(axis[2]) * a.by[1].divisor;
     }
+    const T* x = static_cast<const T*>(a.x) + axis[0] * a.x_stride[0] + axis[1] * a.x_stride[1] + axis[2] * a.x_stride[2] + static_cast<int64_t>(thread) * V;
+    int8_t* y = a.y + axis[0] * a.y_stride[0] + axis[1] * a.y_stride[1] + axis[2] * a.y_stride[2] + static_cast<int64_t>(thread) * V;
+    Pack<T, V> held[kHeld];
+    Largest<T> most;
+    const int left = a.vectors - thread;   // vectors from this thread's first on
 #pragma unroll
     for (int j = 0; j < kHeld; ++j)
-        if (thread + j * THREADS < a.vectors) bits = magnitude_bits(held[j], bits);
-    for (int at = thread + kHeld * THREADS; at < a.vectors; at += THREADS) bits = magnitude_bits(*reinterpret_cast<const Pack<T, V>*>(x + static_cast<int64_t>(at) * V), bits);
-    bits = __reduce_max_sync(0xffffffffu, bits);
+        if (j * THREADS < left) held[j] = *reinterpret_cast<const Pack<T, V>*>(x + j * THREADS * V);
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j)
+        if (j * THREADS < left) most.take(held[j]);
+    for (int v = kHeld * THREADS; v < left; v += THREADS) most.take(*reinterpret_cast<const Pack<T, V>*>(x + static_cast<int64_t>(v) * V));
+    uint32_t bits = __reduce_max_sync(0xffffffffu, most.as_f32());
     if (THREADS > 32) {
         if ((thread & 31) == 0) largest[thread >> 5] = bits;
         __syncthreads();
@@ -104,15 +159,15 @@ token_quantize_kernel(const QuantizeArgs a) {
         for (int w = 0; w < THREADS / 32; ++w) bits = max(bits, largest[w]);
     }
     const float scale = __fdiv_rn(__uint_as_float(bits), 127.0f);
-    if (thread == 0) a.scale[inner * a.scale_stride[0] + middle * a.scale_stride[1] + first * a.scale_stride[2]] = scale;
-    // (products within 2^-23 of the quotients: a normal scale, whose inverse is one too)
+    if (thread == 0) a.scale[axis[0] * a.scale_stride[0] + axis[1] * a.scale_stride[1] + axis[2] * a.scale_stride[2]] = scale;
+    // (products within 2^-24 of the quotients: a normal scale, whose inverse is one too)
     const bool plain = scale >= 1e-30f && scale <= 1e30f;
-    const float inverse = __fdiv_rn(1.0f, scale);
+    const float inverse = __frcp_rn(scale);
 #pragma unroll
     for (int j = 0; j < kHeld; ++j)
-        if (thread + j * THREADS < a.vectors) *reinterpret_cast<Codes<T, V>*>(y + static_cast<int64_t>(thread + j * THREADS) * V) = encode<T, V>(held[j], scale, inverse, plain);
-    for (int at = thread + kHeld * THREADS; at < a.vectors; at += THREADS)
-        *reinterpret_cast<Codes<T, V>*>(y + static_cast<int64_t>(at) * V) = encode<T, V>(*reinterpret_cast<const Pack<T, V>*>(x + static_cast<int64_t>(at) * V), scale, inverse, plain);
+        if (j * THREADS < left) *reinterpret_cast<Codes<T, V>*>(y + j * THREADS * V) = encode<T, V>(held[j], scale, inverse, plain);
+    for (int v = kHeld * THREADS; v < left; v += THREADS)
+        *reinterpret_cast<Codes<T, V>*>(y + static_cast<int64_t>(v) * V) = encode<T, V>(*reinterpret_cast<const Pack<T, V>*>(x + static_cast<int64_t>(v) * V), scale, inverse, plain);
 }
 
 int check_quantize(const dfgpu_token_quantize_params& p, int& width) {
@@ -145,10 +200,16 @@ int check_quantize(const dfgpu_token_quantize_params& p, int& width) {
 
 template <typename T, int V>
 void launch_quantize(const QuantizeArgs& a, cudaStream_t stream) {
-    const unsigned rows = static_cast<unsigned>(a.rows);
-    if (a.vectors <= 64) launch_chained(token_quantize_kernel<T, V, 32>, dim3((rows + 3) / 4), dim3(128), 0, stream, a);
-    else if (a.vectors <= 128 * kHeld) launch_chained(token_quantize_kernel<T, V, 128>, dim3(rows), dim3(128), 0, stream, a);
-    else launch_chained(token_quantize_kernel<T, V, 512>, dim3(rows), dim3(512), 0, stream, a);
+    // Many rows: four vectors a thread, since eight cost registers and so warps (8192 x 4096 bf16 35 us, 25 with four) and a persistent grid whose warps load the next row ahead
+    // is slower yet (28 to 41). Up to two rows an SM there is nothing else to hide latency with, so that as many threads as there are take a row (32 x 4096 2.1 us, 2.7 with 128).
+    const unsigned rows = static_cast<unsigned>(a.rows), quarter = (rows + 3) / 4;
+    if (a.rows <= 2 * 148 && a.vectors > 64) launch_chained(token_quantize_kernel<T, V, 512, 2>, dim3(rows), dim3(512), 0, stream, a);
+    else if (a.vectors <= 64) launch_chained(token_quantize_kernel<T, V, 32, 2>, dim3(quarter), dim3(128), 0, stream, a);
+    else if (a.vectors <= 128) launch_chained(token_quantize_kernel<T, V, 32, 4>, dim3(quarter), dim3(128), 0, stream, a);
+    else if (a.vectors <= 256) launch_chained(token_quantize_kernel<T, V, 64, 4>, dim3(rows), dim3(64), 0, stream, a);
+    else if (a.vectors <= 512) launch_chained(token_quantize_kernel<T, V, 128, 4>, dim3(rows), dim3(128), 0, stream, a);
+    else if (a.vectors <= 1024) launch_chained(token_quantize_kernel<T, V, 256, 4>, dim3(rows), dim3(256), 0, stream, a);
+    else launch_chained(token_quantize_kernel<T, V, 512, 4>, dim3(rows), dim3(512), 0, stream, a);
 }
 
 }  // namespace
@@ -199,6 +260,7 @@ extern "C" int dfgpu_token_quantize(const dfgpu_token_quantize_params* p, void* 
     }
     a.k = static_cast<int>(p->x.dim[rank - 1]);
     a.vectors = a.k / width;
+    a.flat = rank == 2;
     cudaStream_t on = as_stream(stream);
     if (p->x.dtype == DFGPU_F32) width > 1 ? launch_quantize<float, 4>(a, on) : launch_quantize<float, 1>(a, on);
     else if (p->x.dtype == DFGPU_F16) width > 1 ? launch_quantize<__half, 8>(a, on) : launch_quantize<__half, 1>(a, on);
