@@ -68,10 +68,11 @@ struct Shape {
 // Splitting K divides the blocks and adds an exchange that grows with the partial tile, 800 + 0.31 x rows x bn (1000 more with block
 // scales, whose six loading warps also fall behind once they have more than a block each), and shares out the epilogue, which counts
 // for every column that a group of its warps takes: 14 clocks for a full operand that is not loaded ahead (`operands` of them), 20 for E4M3 codes, and 300 in
-// every round where a thread stores its row element by element, as K in splits is added up and stored by neighbouring threads side by side.
+// every round where C's rows are off the 16-byte boundaries (what they cost when a thread stored its row element by element; warps store them side by side now, but
+// other shapes would be other sums. Integers' sums are exact, so theirs is 40: 64 x 300 x 7777 to bf16 4.8 us, with 300 7.1; 333 x 1000 x 1111 with a bias to f16 6.1, 7.2).
 // Former costs -> these, in us: 777 x 4096 x 3072 bf16 [K, N] 26.9 (256 columns) -> 21.6 (192), 2050 x 1040 x 1040 13.0 -> 11.5, MXFP8
 // 15 x 1632 x 816 7.7 -> 6.3 (more splits). Where an exchange of 230 split K: 1 x 136 x 3648 bf16 4.0 whole, 5.0 in two. With bias, ReLU and a
-// full f32 operand, 128 x 384 x 384 f16: 6.0 in six, 7.5 whole; with a bf16 one 1059 x 368 x 104 6.4 and 7.7. With rows of C off the 16-byte boundaries 128 x 512 x 1280 f16 6.9 in splits, 12.9
+// full f32 operand, 128 x 384 x 384 f16: 6.0 in six, 7.5 whole; with a bf16 one 1059 x 368 x 104 6.4 and 7.7. With rows of C off the 16-byte boundaries, stored element by element, 128 x 512 x 1280 f16 6.9 in splits, 12.9
 // whole; FP8 128 x 1024 x 2688 to E5M2 10.2 and 29.2, 78 x 912 x 336 to E4M3 7.5 and 9.6.
 // f32 results and f32 operands (pieces) keep the former costs. Those split K more often, and an accumulator is off by 2^-24 of its value
 // for every block it takes, which a 16-bit result does not show and an f32 result does (128 x 640 x 3840 bf16 to f32: 1.7e-7 from
@@ -130,7 +131,7 @@ inline Shape choose_shape(const Problem& p, int operands) {
                     const double block = std::max({2.3 * bn, 0.9 * (2 * rows + bn / cg + columns), (rows + columns) * kRowBytes / rate});
                     const int box = p.direct_stores ? 32 : kRowBytes / p.out_bytes, serial = std::min(bn, (bn / box + 1) / 2 * box);   // (columns that one epilogue group takes)
                     const double exchange = splits > 1 ? 800.0 + 0.31 * std::min<double>(rows, static_cast<double>(p.M)) * bn + (scaled(p) ? 1000.0 : 0.0) : 0.0;
-                    const double stores = p.direct_stores ? 300.0 * std::ceil(rounds) : (p.out_dtype == DFGPU_E4M3 ? 20.0 : 0.0);
+                    const double stores = p.direct_stores ? (p.kind == kIntegers ? 40.0 : 300.0) * std::ceil(rounds) : (p.out_dtype == DFGPU_E4M3 ? 20.0 : 0.0);
                     const double epilogue = splits > 1 ? 0.0 : (14.0 * operands + stores) * serial;
                     shape.clocks = rounds * (k_per_split * block + (rounds > 1.0 ? 12.0 * bn : 0.0)) + 2000.0 + exchange + epilogue + (scaled(p) && k_per_split > 6 ? 450.0 : 0.0) + (cg == 2 ? 1480.0 : 0.0);
                     if (both) shapes[count++] = shape;

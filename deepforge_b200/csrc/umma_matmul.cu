@@ -28,7 +28,7 @@
 // Warps: 0 loads (TMA), 1 issues products, 4-11 are the epilogue (two groups of four, alternating 128-byte column boxes), and
 // with block scales 2, 3 and 12-15 gather them. Two accumulators in tensor memory, so that a tile's epilogue
 // runs under the next tile's products. Finished boxes leave through a swizzled staging tile by TMA; a thread's own row of
-// 64 bytes at a row's distance would jam the load/store unit.
+// 64 bytes at a row's distance would jam the load/store unit. (Rows off the 16-byte boundaries: a warp turns its values around there and stores row by row.)
 #include <algorithm>
 
 #include "matmul_shape.cuh"
@@ -874,11 +874,28 @@ umma_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                                 if (args.out_dtype == DFGPU_BF16) put(DFGPU_BF16);
                                 else put(DFGPU_F16);
                             }
-                        } else if (row_live && healthy_now(ok, status)) {
-                            const int64_t at = out_row * args.out_ld + col;
+                        } else {
+                            // Rows off the 16-byte boundaries: the warp's 32 x 32 values turn around in shared memory, so that its lanes store neighbours of one row
+                            // (4096 x 4096 x 4095 bf16 200 us -> 90, integers 179 -> 47; 4096 x 300 x 7777 integers to bf16 323 -> 38).
+                            const int quarter = row & 96, live_rows = min(32, args.m_total - row0 - quarter);
+                            float* turned = reinterpret_cast<float*>(generic_base + staging0) + quarter * 32;
+                            __syncwarp();
 #pragma unroll
-                            for (int e = 0; e < 32; ++e)
-                                if (col + e < args.n_total) store_from_f32(args.out, args.out_dtype, at + e, v[e]);
+                            for (int j = 0; j < 8; ++j)
+                                *reinterpret_cast<float4*>(turned + lane * 32 + ((j ^ (lane & 7)) << 2)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                            __syncwarp();
+                            if (col + lane < args.n_total && healthy_now(ok, status)) {
+                                const int64_t at = (row0 + quarter) * args.out_ld + col + lane;
+                                auto put = [&](int dtype) {   // (one branch for all)
+#pragma unroll 8
+                                    for (int r = 0; r < live_rows; ++r)
+                                        store_from_f32(args.out, dtype, at + r * args.out_ld, turned[r * 32 + (((lane >> 2) ^ (r & 7)) << 2) + (lane & 3)]);
+                                };
+                                if (args.out_dtype == DFGPU_BF16) put(DFGPU_BF16);
+                                else if (args.out_dtype == DFGPU_F16) put(DFGPU_F16);
+                                else if (args.out_dtype == DFGPU_F32) put(DFGPU_F32);
+                                else put(args.out_dtype);
+                            }
                         }
                     }
                     if (args.tma_store) {
@@ -1138,8 +1155,8 @@ int launch_problem(Problem p, TileArgs& args, const void* a, const void* b, void
     // the store before has been read, 400 clocks each. 2048 x 64 x 4096 bf16 with bias and ReLU, with the operands loaded ahead: 12.6 us -> 10.8; MXFP8 4096^3
     // with four stages for five: 0.9 % slower.)
     const bool many_boxes = shape.bn > 2 * box_columns || shape.tiles + shape.halved > sm_count() / shape.cg;
-    args.staging_boxes = many_boxes && stages_that_fit(args.stage_bytes, kSmemBudget - 4 * kStageBox - barriers) >= 5 ? 2 : 1;
-    const int staging = shape.splits > 1 || !args.tma_store ? 0 : 2 * args.staging_boxes * kStageBox;
+    args.staging_boxes = args.tma_store && many_boxes && stages_that_fit(args.stage_bytes, kSmemBudget - 4 * kStageBox - barriers) >= 5 ? 2 : 1;
+    const int staging = shape.splits > 1 ? 0 : 2 * args.staging_boxes * kStageBox;
     args.stages = stages_that_fit(args.stage_bytes, kSmemBudget - staging - barriers);
     args.staging_offset = ring_bytes(args.stages, args.stage_bytes);   // (a split product parks its 128 x bn partial tile, at most 64 KB, in the ring)
     args.barrier_offset = args.staging_offset + staging;

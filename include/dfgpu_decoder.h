@@ -46,8 +46,9 @@ int dfgpu_query_head_norm(const dfgpu_head_norm_params*, dfgpu_plan_info*);
 int dfgpu_head_norm(const dfgpu_head_norm_params*, void* const* tensors, void* scratch, void* stream);
 
 /* The gradients: with u the channels of dY turned back (times scale), v = u (gain + gain_offset) and m = mean(v x),
-   dX = r v - x r^3 m and dgain(i) = sum over the rows that share it of u(i) x(i) r. Partial sums of dgain are f32 over at most 512 rows each (a head's
-   32 tokens with gains of every head) and meet in 64 bits, always in the same order.
+   dX = r v - x r^3 m and dgain(i) = sum over the rows that share it of u(i) x(i) r. Partial sums of dgain are f32 over at most 1280 rows each (a head's
+   16 tokens with gains of every head) and meet in 64 bits, always in the same order.
+   A row whose squares pass f32's range has r = 0: its dX and its terms of dgain are zeros (NaN where the sum of v x passes it too).
    tensors: {X, dY, dX, gain or null, dgain or null, positions or null, frequencies or null, X2, dY2, dX2, gain2, dgain2 (null where absent)}.
    dX has X's extents and type and may be X or dY itself (same pointer, same strides); dX2 likewise. dgain has gain's extents, FLOAT, HALF or
    BFLOAT16, rank 0: not wanted; where gain is absent it may still be wanted, [1, 1 or H, 1, D]. Scratch holds the partial sums: none where no dgain is
