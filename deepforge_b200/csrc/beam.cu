@@ -292,6 +292,15 @@ beam_scan_kernel(const ScanArgs a) {
         if (*static_cast<volatile int*>(&count) > kCandidates) break;
     }
     __syncthreads();
+    if (warp == 1) {
+        // the warps' sums against the CTA's largest value (a warp of -inf alone has no reference that means anything)
+        const float own_reference = lane < kScanWarps ? reference_of_warp[lane] : -INFINITY;
+        const float top = __shfl_sync(0xffffffffu, most, 0);
+        const double own_whole = lane < kScanWarps ? whole_of_warp[lane] : 0.0;
+        double sum = own_whole == 0.0 ? 0.0 : own_whole * (own_reference == top || own_reference == -INFINITY ? 1.0 : exp(static_cast<double>(own_reference) - static_cast<double>(top)));
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0) l.sums[blockIdx.x] = PartSum{sum, top, 0.0f};
+    }
     if (warp != 0) return;
     Key list{0};
     if (count <= kCandidates) {
@@ -342,13 +351,6 @@ beam_scan_kernel(const ScanArgs a) {
         }
     }
     if (lane < l.beams) l.keys[static_cast<int64_t>(blockIdx.x) * l.beams + lane] = list.key;
-    // the warps' sums against the CTA's largest value (a warp of -inf alone has no reference that means anything)
-    const float own_reference = lane < kScanWarps ? reference_of_warp[lane] : -INFINITY;
-    const float top = __shfl_sync(0xffffffffu, most, 0);
-    const double own_whole = lane < kScanWarps ? whole_of_warp[lane] : 0.0;
-    double sum = own_whole == 0.0 ? 0.0 : own_whole * (own_reference == top || own_reference == -INFINITY ? 1.0 : exp(static_cast<double>(own_reference) - static_cast<double>(top)));
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) l.sums[blockIdx.x] = PartSum{sum, top, 0.0f};
 }
 
 struct Ints {
