@@ -1,7 +1,8 @@
 // C = (sum_k A B) a_scale b_scale + bias: 8-bit integers with a scale for each token (row of A) and each channel (column of B).
 //
-// The sums are exact in 32-bit integers, so every kernel gives the same bits; rows on 16-byte boundaries go to tcgen05 (umma_matmul.cu), everything else to the
-// CUDA cores here: 64 x 64 outputs a CTA, operands as words of four neighbours along K in shared memory, four products an instruction (dp4a).
+// The sums are exact in 32-bit integers, so every kernel gives the same bits; rows on 16-byte boundaries go to tcgen05 (umma_matmul.cu: 8192 x 4096 x 4096 86 us, 96 % of the rate)
+// or, few of them, to the second kernel here, everything else to the CUDA cores: 64 x 64 outputs a CTA, operands as words of four neighbours along K in shared memory, four products
+// an instruction (dp4a).
 #include <algorithm>
 
 #include "common.cuh"
@@ -9,6 +10,7 @@
 #include "ports.cuh"
 #include "rotary.cuh"
 #include "umma.cuh"
+#include "umma_ptx.cuh"
 
 namespace dfgpu {
 namespace {
@@ -101,6 +103,142 @@ matmul_int8_cores_kernel(const Int8Args g) {
     }
 }
 
+// ---- few tokens: bound by the weights, and by the latency of a launch ---------------------------------------------------------
+// A warp's product takes 16 columns of B x 32 of K and 32 of K x 8 tokens. Neighbouring lanes copy 64 bytes of K of a column, 16 each; a sum of integers has no order, so these bytes
+// stand for K in whichever order the instruction names it: two products. A CTA has 16 columns, its warps share K in blocks of 64, each with private copies on their way (no barrier until
+// their sums meet). 1 x 4096 x 4096 4.9 us (16.8 MB of weights: 2.6), 8 x 4096 x 4096 5.4, 1 x 4096 x 32000 21.9 (20.1). Loads straight into registers came out in any order (4.8 to 13 us).
+constexpr int kFewTokens = 16;
+
+// 16 bytes of a row from k on; what lies past its end counts as zeros.
+__device__ __noinline__ uint4 last_words(const int8_t* row, int k, int depth) {
+    uint32_t w[4] = {};
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        if (k + i < depth) w[i >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(row[k + i])) << (8 * (i & 3));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void multiply(int (&sums)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+r"(sums[0]), "+r"(sums[1]), "+r"(sums[2]), "+r"(sums[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <int TILES, int ROWS, int STAGES, int WARPS>
+struct Few {
+    static constexpr int kColumns = 16 * ROWS, kPitchOf = kColumns + 4, kThreads = 32 * WARPS, kOutputs = (8 * TILES * kColumns + kThreads - 1) / kThreads, kOfStage = 2 * ROWS + TILES;
+    static constexpr int kBytes = std::max(STAGES * kOfStage * 16 * kThreads, 4 * WARPS * 8 * TILES * kPitchOf);
+};
+template <int TILES, int ROWS, int STAGES, int WARPS>   // of 8 tokens; of 16 columns; blocks of a warp on their way
+__global__ void __launch_bounds__(32 * WARPS)
+matmul_int8_few_kernel(const __grid_constant__ Int8Args g) {
+    using F = Few<TILES, ROWS, STAGES, WARPS>;
+    extern __shared__ __align__(16) uint4 ring[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, eighth = lane >> 2, quarter = lane & 3;
+    const int64_t n0 = static_cast<int64_t>(blockIdx.x) * F::kColumns;
+    // Columns and tokens behind the last one are zeros, and nothing is read for them (many lanes that read one line of the L2 cache wait for one another).
+    const int8_t* from[F::kOfStage];
+    int bytes[F::kOfStage];
+#pragma unroll
+    for (int i = 0; i < F::kOfStage; ++i) {
+        const bool weights = i < 2 * ROWS;
+        const int64_t row = weights ? n0 + eighth + 8 * i : eighth + 8 * (i - 2 * ROWS), rows = weights ? g.n : g.m;
+        bytes[i] = row < rows ? 16 : 0;
+        from[i] = (weights ? g.b : g.a) + min(row, rows - 1) * (weights ? g.b_stride[1] : g.a_stride[0]) + quarter * 16;
+    }
+    int sums[TILES][ROWS][4] = {};
+    const int blocks = g.k / 64;
+    // A thread's copies are its own: it waits for them, and nobody else does.
+    auto fill = [&](int stage, int block) {
+        if (block < blocks) {
+#pragma unroll
+            for (int i = 0; i < F::kOfStage; ++i) {
+                const uint32_t to = smem_u32(ring + (stage * F::kOfStage + i) * F::kThreads + static_cast<int>(threadIdx.x));
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(__cvta_generic_to_global(from[i] + block * 64)), "r"(bytes[i]) : "memory");
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto add_up = [&](const uint4 (&at)[F::kOfStage]) {
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                const uint4 &one = at[2 * r], &two = at[2 * r + 1], &x = at[2 * ROWS + t];
+                multiply(sums[t][r], one.x, two.x, one.y, two.y, x.x, x.y);
+                multiply(sums[t][r], one.z, two.z, one.w, two.w, x.z, x.w);
+            }
+    };
+    chain_begin();
+#pragma unroll
+    for (int s = 0; s < STAGES; ++s) fill(s, warp + s * WARPS);
+    float a_scale[F::kOutputs], b_scale[F::kOutputs], bias[F::kOutputs];
+#pragma unroll
+    for (int o = 0; o < F::kOutputs; ++o) {
+        const int at = static_cast<int>(threadIdx.x) + o * F::kThreads, token = at / F::kColumns;
+        const int64_t n = n0 + at % F::kColumns;
+        const bool live = token < g.m && n < g.n;
+        a_scale[o] = live ? g.a_scale[token * g.a_scale_stride] : 0.0f;
+        b_scale[o] = live ? g.b_scale[n * g.b_scale_stride] : 0.0f;
+        bias[o] = live && g.bias ? load_as_f32(g.bias, g.bias_type, n * g.bias_stride) : 0.0f;
+    }
+    int stage = 0;
+    for (int block = warp; block < blocks; block += WARPS) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+        uint4 at[F::kOfStage];
+#pragma unroll
+        for (int i = 0; i < F::kOfStage; ++i) at[i] = ring[(stage * F::kOfStage + i) * F::kThreads + static_cast<int>(threadIdx.x)];
+        add_up(at);
+        fill(stage, block + STAGES * WARPS);   // (the products have what the stage held)
+        stage = stage + 1 == STAGES ? 0 : stage + 1;
+    }
+    if (g.k % 64 != 0 && warp == blocks % WARPS) {
+        uint4 at[F::kOfStage];
+#pragma unroll
+        for (int i = 0; i < F::kOfStage; ++i) at[i] = last_words(from[i], blocks * 64, g.k - quarter * 16);
+        __syncwarp();
+        add_up(at);
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();   // (nothing is on its way into the ring any more)
+    int32_t* partial = reinterpret_cast<int32_t*>(ring);
+#pragma unroll
+    for (int t = 0; t < TILES; ++t)
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) partial[(warp * 8 * TILES + 8 * t + 2 * quarter + (i & 1)) * F::kPitchOf + 16 * r + eighth + 8 * (i >> 1)] = sums[t][r][i];
+    __syncthreads();
+#pragma unroll
+    for (int o = 0; o < F::kOutputs; ++o) {
+        const int at = static_cast<int>(threadIdx.x) + o * F::kThreads, token = at / F::kColumns, column = at % F::kColumns;
+        const int64_t n = n0 + column;
+        if (token >= 8 * TILES || token >= g.m || n >= g.n) continue;
+        int sum = 0;
+#pragma unroll
+        for (int i = 0; i < WARPS; ++i) sum += partial[(i * 8 * TILES + token) * F::kPitchOf + column];
+        float value = __fmul_rn(__fmul_rn(__int2float_rn(sum), a_scale[o]), b_scale[o]);
+        if (g.bias) value = __fadd_rn(value, bias[o]);
+        store_from_f32(g.c, g.c_type, token * g.c_stride[0] + n * g.c_stride[1], value);
+    }
+}
+
+template <int TILES, int ROWS, int STAGES, int WARPS>
+int launch_few(const Int8Args& g, cudaStream_t stream) {
+    using F = Few<TILES, ROWS, STAGES, WARPS>;
+    if (F::kBytes > 48 * 1024) {
+        const cudaError_t error = cudaFuncSetAttribute(matmul_int8_few_kernel<TILES, ROWS, STAGES, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kBytes);
+        if (error != cudaSuccess) return fail(kExecutionFailed, "MATMUL_INT8: cannot reserve %d bytes of shared memory: %s", F::kBytes, cudaGetErrorString(error));
+    }
+    launch_chained(matmul_int8_few_kernel<TILES, ROWS, STAGES, WARPS>, dim3(static_cast<unsigned>((g.n + F::kColumns - 1) / F::kColumns)), dim3(F::kThreads), F::kBytes, stream, g);
+    return check_launch("MATMUL_INT8");
+}
+// Where the CTAs are few, twice the warps hide the latency (4096 x 4096 and 8 tokens 5.4 us, 7.3 with eight); where they are many, four CTAs of eight fit an SM (12288 columns of
+// 4096: 10.7, 11.8 with sixteen).
+int launch_few(const Int8Args& g, cudaStream_t stream) {
+    if (g.m > 8) return launch_few<2, 1, 4, 8>(g, stream);
+    return g.n <= 16 * 2 * 148 ? launch_few<1, 1, 4, 16>(g, stream) : launch_few<1, 1, 4, 8>(g, stream);
+}
+
 int check_int8(const dfgpu_matmul_int8_params& p) {
     const int rank = p.c.rank;
     if (!valid_tensor(p.a) || !valid_tensor(p.b) || !valid_tensor(p.c) || rank < 2 || p.a.rank != rank || p.b.rank != rank)
@@ -134,7 +272,7 @@ int check_int8(const dfgpu_matmul_int8_params& p) {
         if (!scale_ok(p.bias, 1, n, one) || p.bias.dim[rank - 1] != n) return fail(kInvalidShape, "MATMUL_INT8: the bias must be [..., 1, N]");
         if (p.bias.dtype != DFGPU_F32 && p.bias.dtype != DFGPU_F16 && p.bias.dtype != DFGPU_BF16) return fail(kUnsupported, "MATMUL_INT8: the bias must be FLOAT, HALF or BFLOAT16");
     }
-    if (p.kernel < DFGPU_MATMUL_INT8_AUTO || p.kernel > DFGPU_MATMUL_INT8_UMMA) return fail(kInvalidArgument, "MATMUL_INT8: unknown kernel id %d", p.kernel);
+    if (p.kernel < DFGPU_MATMUL_INT8_AUTO || p.kernel > DFGPU_MATMUL_INT8_FEW) return fail(kInvalidArgument, "MATMUL_INT8: unknown kernel id %d", p.kernel);
     return kOk;
 }
 
@@ -178,11 +316,53 @@ bool fold_batch(const dfgpu_matmul_int8_params& p, dfgpu_matmul_int8_params& fol
     return true;
 }
 
+// The kernel for few tokens takes any C and bias; rows of A and columns of B lie along K on 16-byte boundaries.
+bool few_tokens(const dfgpu_matmul_int8_params& folded) {
+    const dfgpu_tensor &a = folded.a, &b = folded.b;
+    return a.dim[0] <= kFewTokens && (a.dim[1] == 1 || (a.stride[1] == 1 && b.stride[0] == 1)) && (a.dim[0] == 1 || a.stride[0] % 16 == 0) && (b.dim[1] == 1 || b.stride[1] % 16 == 0);
+}
 int choose_int8(const dfgpu_matmul_int8_params& p, int& kernel, dfgpu_matmul_int8_params& folded) {
-    const bool tiles = fold_batch(p, folded) && matmul_int8_umma_supported(folded);
-    kernel = p.kernel == DFGPU_MATMUL_INT8_AUTO ? (tiles ? DFGPU_MATMUL_INT8_UMMA : DFGPU_MATMUL_INT8_CORES) : p.kernel;
+    const bool folds = fold_batch(p, folded), tiles = folds && matmul_int8_umma_supported(folded), few = folds && few_tokens(folded);
+    // Up to eight tokens the kernel for few of them is the quicker (1 x 4096 x 4096 4.9 us, tcgen05 6.8; x 12288 columns 10.7 and 13.1; 12288 x 4096 10.4 and 11.4; 4 x 1000 x 1111 3.0 and
+    // 4.2), up to sixteen where the weights are few (16 x 512 x 512 1.7 and 3.5, 16 x 1000 x 1111 3.7 and 4.2; 16 x 4096 x 4096 7.1 both, 16 x 12288 x 4096 15.7 and 11.7).
+    const bool quicker = few && (folded.c.dim[0] <= 8 || folded.a.dim[1] * folded.c.dim[1] <= 1 << 22);
+    kernel = p.kernel == DFGPU_MATMUL_INT8_AUTO ? (quicker ? DFGPU_MATMUL_INT8_FEW : tiles ? DFGPU_MATMUL_INT8_UMMA : DFGPU_MATMUL_INT8_CORES) : p.kernel;
+    if (kernel == DFGPU_MATMUL_INT8_FEW && !few) return fail(kUnsupported, "MATMUL_INT8: the kernel for few tokens does not cover this shape or layout");
     if (kernel == DFGPU_MATMUL_INT8_UMMA && !tiles) return fail(kUnsupported, "MATMUL_INT8: the tcgen05 kernel does not cover this shape or layout");
     return kOk;
+}
+
+Int8Args args_of(const dfgpu_matmul_int8_params& p, void* const* tensors) {
+    const int rank = p.c.rank;
+    Int8Args g{};
+    g.a = static_cast<const int8_t*>(tensors[0]);
+    g.b = static_cast<const int8_t*>(tensors[1]);
+    g.c = tensors[2];
+    g.a_scale = static_cast<const float*>(tensors[3]);
+    g.b_scale = static_cast<const float*>(tensors[4]);
+    g.bias = p.bias.rank ? tensors[5] : nullptr;
+    g.bias_type = p.bias.dtype;
+    g.c_type = p.c.dtype;
+    for (int i = 0; i < 2; ++i) {
+        g.a_stride[i] = p.a.stride[rank - 2 + i];
+        g.b_stride[i] = p.b.stride[rank - 2 + i];
+        g.c_stride[i] = p.c.stride[rank - 2 + i];
+    }
+    g.a_scale_stride = p.a_scale.dim[rank - 2] == 1 ? 0 : p.a_scale.stride[rank - 2];
+    g.b_scale_stride = p.b_scale.dim[rank - 1] == 1 ? 0 : p.b_scale.stride[rank - 1];
+    g.bias_stride = p.bias.rank ? p.bias.stride[rank - 1] : 0;
+    g.m = p.c.dim[rank - 2];
+    g.n = p.c.dim[rank - 1];
+    g.k = static_cast<int>(p.a.dim[rank - 1]);
+    g.batch_axes = rank - 2;
+    for (int i = 0; i < rank - 2; ++i) {
+        g.batch[i] = p.c.dim[i];
+        g.a_batch[i] = p.a.dim[i] == 1 ? 0 : p.a.stride[i];
+        g.b_batch[i] = p.b.dim[i] == 1 ? 0 : p.b.stride[i];
+        g.c_batch[i] = p.c.dim[i] == 1 ? 0 : p.c.stride[i];
+        g.a_scale_batch[i] = p.a_scale.dim[i] == 1 ? 0 : p.a_scale.stride[i];
+    }
+    return g;
 }
 
 }  // namespace
@@ -222,37 +402,15 @@ extern "C" int dfgpu_matmul_int8(const dfgpu_matmul_int8_params* p, void* const*
         if (aligned(tensors[0], 16) && aligned(tensors[1], 16)) return launch_matmul_int8_umma(folded, tensors, as_stream(stream));
         if (p->kernel == DFGPU_MATMUL_INT8_UMMA) return fail(kInvalidArgument, "MATMUL_INT8: the tcgen05 kernel needs A and B on 16-byte boundaries");
     }
-    const int rank = p->c.rank;
-    Int8Args g{};
-    g.a = static_cast<const int8_t*>(tensors[0]);
-    g.b = static_cast<const int8_t*>(tensors[1]);
-    g.c = tensors[2];
-    g.a_scale = static_cast<const float*>(tensors[3]);
-    g.b_scale = static_cast<const float*>(tensors[4]);
-    g.bias = p->bias.rank ? tensors[5] : nullptr;
-    g.bias_type = p->bias.dtype;
-    g.c_type = p->c.dtype;
-    for (int i = 0; i < 2; ++i) {
-        g.a_stride[i] = p->a.stride[rank - 2 + i];
-        g.b_stride[i] = p->b.stride[rank - 2 + i];
-        g.c_stride[i] = p->c.stride[rank - 2 + i];
+    if (kernel == DFGPU_MATMUL_INT8_FEW) {
+        if (aligned(tensors[0], 16) && aligned(tensors[1], 16)) {
+            return launch_few(args_of(folded, tensors), as_stream(stream));
+        }
+        if (p->kernel == DFGPU_MATMUL_INT8_FEW) return fail(kInvalidArgument, "MATMUL_INT8: the kernel for few tokens needs A and B on 16-byte boundaries");
     }
-    g.a_scale_stride = p->a_scale.dim[rank - 2] == 1 ? 0 : p->a_scale.stride[rank - 2];
-    g.b_scale_stride = p->b_scale.dim[rank - 1] == 1 ? 0 : p->b_scale.stride[rank - 1];
-    g.bias_stride = p->bias.rank ? p->bias.stride[rank - 1] : 0;
-    g.m = p->c.dim[rank - 2];
-    g.n = p->c.dim[rank - 1];
-    g.k = static_cast<int>(p->a.dim[rank - 1]);
-    g.batch_axes = rank - 2;
+    Int8Args g = args_of(*p, tensors);
     int64_t batches = 1;
-    for (int i = 0; i < rank - 2; ++i) {
-        g.batch[i] = p->c.dim[i];
-        g.a_batch[i] = p->a.dim[i] == 1 ? 0 : p->a.stride[i];
-        g.b_batch[i] = p->b.dim[i] == 1 ? 0 : p->b.stride[i];
-        g.c_batch[i] = p->c.dim[i] == 1 ? 0 : p->c.stride[i];
-        g.a_scale_batch[i] = p->a_scale.dim[i] == 1 ? 0 : p->a_scale.stride[i];
-        batches = std::min<int64_t>(batches * p->c.dim[i], 1ll << 31);
-    }
+    for (int i = 0; i < p->c.rank - 2; ++i) batches = std::min<int64_t>(batches * p->c.dim[i], 1ll << 31);
     g.m_tiles = (g.m + kTile - 1) / kTile;
     const int64_t tiles = g.m_tiles * ((g.n + kTile - 1) / kTile);
     if (batches > 65535 || tiles >= (1ll << 31)) return fail(kUnsupported, "MATMUL_INT8: more than 65535 matrices or 2^31 tiles on the CUDA cores");

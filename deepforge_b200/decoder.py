@@ -16,7 +16,7 @@ from .dfgpu import DfgpuError, PlanInfo, Tensor, tensor  # noqa: F401  (tensor: 
 I8 = 12
 HEAD_NORM_AUTO, HEAD_NORM_VECTOR, HEAD_NORM_SCALAR = range(3)
 TOKEN_QUANTIZE_AUTO, TOKEN_QUANTIZE_VECTOR, TOKEN_QUANTIZE_SCALAR = range(3)
-MATMUL_INT8_AUTO, MATMUL_INT8_CORES, MATMUL_INT8_UMMA = range(3)
+MATMUL_INT8_AUTO, MATMUL_INT8_CORES, MATMUL_INT8_UMMA, MATMUL_INT8_FEW = range(4)
 MAX_STATES = 8
 
 

@@ -84,9 +84,10 @@ int dfgpu_token_quantize(const dfgpu_token_quantize_params*, void* const* tensor
    tensors: {A, B, C, a_scale, b_scale, bias or null}. A INT8 [..., M, K], B INT8 [..., K, N], C FLOAT, HALF or BFLOAT16 [..., M, N], equal rank
    2 to 8; batch axes of A and B are C's or 1. a_scale FLOAT [..., M or 1, 1], b_scale FLOAT [..., 1, N or 1], bias FLOAT, HALF or BFLOAT16
    [..., 1, N], of the same rank, their batch axes 1 or (a_scale) A's. DFGPU_MATMUL_INT8_UMMA: tcgen05 (kind::i8); A with K contiguous, B with K or N
-   contiguous, their rows on 16-byte boundaries (any extents), C and the bias with N contiguous, batch axes that fold into M. AUTO takes it where it can;
-   everything else goes to the CUDA cores. */
-enum { DFGPU_MATMUL_INT8_AUTO = 0, DFGPU_MATMUL_INT8_CORES = 1, DFGPU_MATMUL_INT8_UMMA = 2 };
+   contiguous, their rows on 16-byte boundaries (any extents), C and the bias with N contiguous, batch axes that fold into M. DFGPU_MATMUL_INT8_FEW: at
+   most 16 rows of A, A and B with K contiguous on 16-byte boundaries, batch axes that fold into M, any C and bias: for a decoder's step, bound by B. AUTO takes the quicker of the two
+   where it can; everything else goes to the CUDA cores. The result does not depend on the kernel. */
+enum { DFGPU_MATMUL_INT8_AUTO = 0, DFGPU_MATMUL_INT8_CORES = 1, DFGPU_MATMUL_INT8_UMMA = 2, DFGPU_MATMUL_INT8_FEW = 3 };
 typedef struct dfgpu_matmul_int8_params {
     dfgpu_tensor a, b, c;
     dfgpu_tensor a_scale, b_scale, bias;

@@ -176,12 +176,18 @@ def int8_params(m=8, n=32, k=64, dtype=BF16, **change):
 
 
 def test_matmul_int8_refusals():
-    info = decoder.query("matmul_int8", int8_params())
+    info = decoder.query("matmul_int8", int8_params(m=32))
     assert (info.kernel, info.launches, info.scratch_bytes) == (decoder.MATMUL_INT8_UMMA, 1, 0)
+    few = decoder.MATMUL_INT8_FEW
+    for m, n, k, kernel in ((1, 32000, 4096, few), (8, 4096, 16384, few), (9, 4096, 4096, decoder.MATMUL_INT8_UMMA), (16, 1024, 1024, few), (17, 64, 64, decoder.MATMUL_INT8_UMMA)):
+        assert decoder.query("matmul_int8", int8_params(m=m, n=n, k=k)).kernel == kernel
+    assert decoder.query("matmul_int8", int8_params(c=tensor(BF16, [8, 32], [1, 8]), bias=tensor(F32, [1, 32], [64, 2]))).kernel == few   # any C and bias
+    for params in (int8_params(m=17, kernel=few), int8_params(k=65, kernel=few), int8_params(b=tensor(I8, [64, 32]), kernel=few)):
+        refused(20, "matmul_int8", params, "few tokens")
     assert decoder.query("matmul_int8", int8_params(k=65)).kernel == decoder.MATMUL_INT8_CORES
     assert decoder.query("matmul_int8", int8_params(b=tensor(I8, [64, 32]))).kernel == decoder.MATMUL_INT8_UMMA
     assert decoder.query("matmul_int8", int8_params(a=tensor(I8, [8, 64], [1, 8]))).kernel == decoder.MATMUL_INT8_CORES
-    assert decoder.query("matmul_int8", int8_params(a_scale=tensor(F32, [1, 1]), b_scale=tensor(F32, [1, 1]))).kernel == decoder.MATMUL_INT8_UMMA
+    assert decoder.query("matmul_int8", int8_params(m=32, a_scale=tensor(F32, [1, 1]), b_scale=tensor(F32, [1, 1]))).kernel == decoder.MATMUL_INT8_UMMA
     refused(20, "matmul_int8", int8_params(a=tensor(U8, [8, 64])))
     refused(20, "matmul_int8", int8_params(dtype=I32))
     refused(15, "matmul_int8", int8_params(b=tensor(I8, [63, 32])))
@@ -193,7 +199,7 @@ def test_matmul_int8_refusals():
     refused(14, "matmul_int8", int8_params(c=tensor(BF16, [8, 32], [0, 1])))
     refused(20, "matmul_int8", int8_params(k=131072), "32 bits")
     assert decoder.query("matmul_int8", int8_params(k=131071)).launches == 1
-    refused(1, "matmul_int8", int8_params(kernel=3))
+    refused(1, "matmul_int8", int8_params(kernel=4))
     refused(20, "matmul_int8", int8_params(kernel=decoder.MATMUL_INT8_UMMA, k=65))
 
     def batched(b_batch, strides=None, **change):
@@ -212,6 +218,7 @@ def test_matmul_int8_refusals():
     call_refused(1, decoder.matmul_int8, int8_params(), [far[0], far[1], far[2] + 1, *far[3:]], "aligned")
     call_refused(1, decoder.matmul_int8, int8_params(), [far[0], far[1], far[0] + 64, *far[3:]], "overlaps")
     call_refused(1, decoder.matmul_int8, int8_params(kernel=decoder.MATMUL_INT8_UMMA), [far[0] + 1, *far[1:]], "boundaries")
+    call_refused(1, decoder.matmul_int8, int8_params(kernel=few), [far[0], far[1] + 8, *far[2:]], "boundaries")
 
 
 # ---- beam search --------------------------------------------------------------------------------------

@@ -440,6 +440,28 @@ def test_matmul_int8_batches_and_extremes():
         check_product(product(wide, wide.T, unit, unit, F32, kernel=kernel), wide, wide.T, unit, unit)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 17, 15), (2, 16, 16), (7, 33, 63), (8, 130, 64), (9, 64, 65), (16, 15, 100), (11, 200, 1000), (15, 96, 511), (16, 1111, 513), (16, 40, 4100), (3, 4099, 2048), (1, 16, 131071)])
+def test_matmul_int8_of_few_tokens(dtype, m, n, k):
+    rng = np.random.default_rng(m + n + k)
+    a, b = rows16(int8s(rng, (m, k))), rows16(int8s(rng, (n, k))).T
+    a_scale, b_scale = scales(rng, (m, 1)), scales(rng, (1, n))
+    bias = randn(rng, (1, 2 * n), F32)[:, ::2]
+    few = decoder.MATMUL_INT8_FEW
+    wide = torch.full((m + 1, n + 3), 7.0, device="cuda", dtype=TORCH[dtype])
+    check_product(product(a, b, a_scale, b_scale, dtype, c=wide[:m, :n], kernel=few), a, b, a_scale, b_scale)
+    assert torch.all(wide[m] == 7.0) and torch.all(wide[:, n:] == 7.0)
+    check_product(product(a, b, a_scale, b_scale, dtype, bias, kernel=few), a, b, a_scale, b_scale, bias)
+    every, one = scales(rng, (2 * m, 3))[::2, :1], scales(rng, (1, 1))
+    check_product(product(a, b, every, one, dtype, kernel=few), a, b, every, one)
+    # an infinite scale (a row with an infinity) and that of a NaN reach their own row alone
+    a_scale[m - 1] = float("nan")
+    got = product(a, b, a_scale, b_scale, dtype, kernel=few)
+    assert torch.all(torch.isnan(got[m - 1]))
+    if m > 1:
+        check_product(got[: m - 1], a[: m - 1], b, a_scale[: m - 1], b_scale)
+
+
 # ---- beam search ---------------------------------------------------------------------------------------------
 
 def select(logits, scores, finished=None, lengths=None, penalty=0.0, end=-1, pad=0, bases=None, in_place=False, stream=None, scratch=None):
