@@ -203,6 +203,7 @@ beam_scan_kernel(const ScanArgs a) {
     __shared__ float reference_of_warp[kScanWarps];
     __shared__ uint64_t candidates[kCandidates];
     __shared__ int count;
+    __shared__ uint8_t lanes_of_warp[kScanWarps][32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const Logits& l = a.logits;
     const int row = static_cast<int>(fast_divide(blockIdx.x, a.by_parts)), part = static_cast<int>(blockIdx.x) - row * l.parts;
@@ -273,12 +274,17 @@ beam_scan_kernel(const ScanArgs a) {
         return Look<T>{*reinterpret_cast<const uint4*>(&own[0]), there ? vector : -1};
     };
     // (Loops that are not unrolled: a warp comes by here once, and instructions that are run once are waited for.)
+    // The lanes that reach the bound have their vectors looked through side by side, 32 at a time.
+    const uint32_t lanes = __ballot_sync(0xffffffffu, largest >= least);
+    if (largest >= least) lanes_of_warp[warp][__popc(lanes & ((1u << lane) - 1))] = static_cast<uint8_t>(lane);
+    __syncwarp();
+    const int vectors = __popc(lanes) * of_lane;
 #pragma unroll 1
-    for (uint32_t lanes = __ballot_sync(0xffffffffu, largest >= least); lanes != 0; lanes &= lanes - 1) {
-#pragma unroll 1
-        for (int from = 0; from < of_lane; from += 32) {
-            const Look<T> own = look(warp, __ffs(static_cast<int>(lanes)) - 1, from + lane);
-            if (own.vector < 0) continue;
+    for (int from = 0; from < vectors; from += 32) {
+        const int place = (from + lane) / of_lane;
+        const bool there = from + lane < vectors;
+        const Look<T> own = look(warp, there ? lanes_of_warp[warp][place] : 0, there ? from + lane - place * of_lane : of_lane);
+        if (own.vector >= 0) {
             const uint32_t token = static_cast<uint32_t>(own.vector) * VE;
 #pragma unroll
             for (int i = 0; i < VE; ++i) {
@@ -289,7 +295,7 @@ beam_scan_kernel(const ScanArgs a) {
                 }
             }
         }
-        if (*static_cast<volatile int*>(&count) > kCandidates) break;
+        if (__any_sync(0xffffffffu, *static_cast<volatile int*>(&count) > kCandidates)) break;   // (all lanes or none)
     }
     __syncthreads();
     if (warp == 1) {
