@@ -389,7 +389,7 @@ beam_merge_kernel(const MergeArgs a) {
     const float score = a.scores[entry * a.scores_batch + beam * a.scores_beam];
     const bool done = a.finished.data && a.finished.at(entry, beam) != 0;
     int64_t length = a.lengths.data ? static_cast<int64_t>(a.lengths.at(entry, beam)) + (done ? 0 : 1) : 1;
-    constexpr int kAhead = 4;
+    constexpr int kAhead = 8;
     uint64_t ahead[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) ahead[i] = i < l.parts && lane < l.beams ? l.keys[(first + i) * l.beams + lane] : 0;
