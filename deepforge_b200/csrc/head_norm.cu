@@ -1,7 +1,9 @@
 // RMS norms of query and key heads with their gains and rotary positions in one pass, and the gradients of all three.
 //
 // A row is one token's head, D channels. It is taken by a group of lanes that hold it in registers between its sum of squares and its result
-// (pairs that turn together lie in one lane), so that it is read once and written once: HBM is what bounds both kernels.
+// (pairs that turn together lie in one lane), so that it is read once and written once: HBM is what bounds both kernels, and close behind it the chain of instructions of
+// a row, which few warps hide (registers hold the angles and the gradients' sums). 2 x 8192 tokens of 32 + 8 heads of 128 bf16 channels 58 us (the bytes alone 51); gradients of
+// 4 x 2048 such tokens 51.5 (38.5), of 3 x 1001 f32 tokens with gains of every head 38 (22.6), the sums of dgain among them (6, half of it behind the first kernel's end).
 #include <algorithm>
 #include <cmath>
 
@@ -319,7 +321,7 @@ struct Ring {
         reading = filling;
     }
 };
-constexpr int kForwardStages = 4, kGradientStages = 3;
+constexpr int kForwardStages = 4, kGradientStages = 3;   // (gradients of 4 x 2048 bf16 tokens 51.8 us; two stages 61.2, four 52.2; of 3 x 1001 f32 tokens 38.0, 38.1 and 43.0)
 
 // ---- forward: a CTA takes a few tokens of one sequence and a run of heads of both pairs of tensors, which share the tokens' angles -----------------------
 // A group of lanes has one token and walks the heads, so that the angles stay in registers, multiplied by the gains already.
@@ -572,6 +574,7 @@ __device__ __forceinline__ void put_sums(const NormArgs& a, const Share<Form, U>
 
 // PER_HEAD: each warp has heads of its own, with their gains, and walks the tokens, whose angles are in the table; the sums of dgain go out with each head.
 // Otherwise a group of lanes has one token, its angles in registers, and walks the heads; all have one sum.
+// (CTAs on an SM, against registers: bf16 four 51.8 us, three 60.2, five 70.3 with spills; f32 six 38.0, five 40.5, four 40.6, seven 39.1)
 template <typename T, int V, bool INTERLEAVED, bool PER_HEAD>
 __global__ void __launch_bounds__(kNormThreads, sizeof(T) == 4 ? 6 : 4)
 head_norm_grad_kernel(const __grid_constant__ NormArgs a) {
