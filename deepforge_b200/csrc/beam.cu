@@ -5,8 +5,8 @@
 // leftover. Of the largest values of the CTA's lanes (32 of them, each over all warps) the W-th largest is a bound that W values reach at least, and hardly more than W lanes
 // of some warp: their vectors are looked through again (from the caches), and what reaches the bound is sorted, a lane an entry.
 // Second kernel: a CTA an entry, a warp a beam, which merges its parts' lists; scores are added in 64 bits, beams merged pair by pair.
-// What bounds it are the two kernels' chains, not the bytes: 16 x 8 beams over 128000 bf16 tokens 18.3 us (bytes 5.0, exponentials 3.6), of which the second look and the sorts
-// take 3 to 4 and the second kernel 4; one user's four beams over 32000 tokens 7.3; 7 x 5 over 50001 f32 tokens 9.8.
+// What bounds it are the two kernels' chains, not the bytes: 16 x 8 beams over 128000 bf16 tokens 18.8 us (bytes 5.0, exponentials 3.6), of which the second look and the sorts
+// take 3 to 4 and the second kernel 4; one user's four beams over 32000 tokens 7.6; 7 x 5 over 50001 f32 tokens 10.1.
 //
 // Reordering: a copy; HBM bounds it. 2 x 8 layers of 8 x 4 rows of 131072 bf16 values 35 us (134 MB each way; a part of it stays in the L2 cache), a token history of 1000 2.4.
 #include <algorithm>
@@ -134,6 +134,14 @@ __device__ __forceinline__ void load_vectors(Pack<T, 16 / sizeof(T)> (&held)[R],
     }
 }
 
+// (One copy: instructions that a warp runs once are waited for. 7 x 5 beams over 50001 f32 tokens 10.1 us, with a copy in each place 10.6.)
+template <typename T>
+__device__ __noinline__ uint4 one_vector(const T* row, int vector, int before, int length) {
+    Pack<T, 16 / sizeof(T)> own[1];
+    load_vectors<T, 1>(own, row, vector, before, length);
+    return *reinterpret_cast<const uint4*>(&own[0]);
+}
+
 // A key into a list in order, where it belongs; the last of 32 falls out.
 __device__ __forceinline__ void insert(Key& list, uint64_t key, int lane) {
     const int place = __popc(__ballot_sync(0xffffffffu, list.key > key));
@@ -182,6 +190,7 @@ __device__ __forceinline__ float in_order(float v, int lane) {
 // A lane's vector of the row, and what it may add to a list: values above `least`, or equal to it and below `last_token`.
 template <typename T>
 struct Look {
+    static constexpr int kValues = kVector<T>;
     uint4 words;
     int vector;
     __device__ __forceinline__ float value(int i) const {   // (`i` the same in all lanes, or known)
@@ -196,6 +205,69 @@ struct Look {
     }
 };
 
+// A CTA's candidates.
+struct Found {
+    uint64_t candidates[kCandidates];
+    uint32_t first_equals[kScanWarps][kMaxBeams];
+    int equals[kScanWarps], count;
+    uint8_t lanes[kScanWarps][32];
+    __device__ __forceinline__ void add(float value, uint32_t token) {
+        const int at = atomicAdd(&count, 1);   // (in any order: they are sorted)
+        if (at < kCandidates) candidates[at] = static_cast<uint64_t>(ordered(value)) << 32 | ~token;
+    }
+    template <typename L>
+    __device__ __forceinline__ void take(const L& own, float bound, int vocabulary) {
+        if (own.vector < 0) return;
+        const uint32_t token = static_cast<uint32_t>(own.vector) * L::kValues;
+#pragma unroll
+        for (int i = 0; i < L::kValues; ++i) {
+            const float x = own.value(i);
+            if (x >= bound && token + i < static_cast<uint32_t>(vocabulary)) add(x, token + i);
+        }
+    }
+};
+// Where too many values equal the bound (masks, equal logits) for the candidates' room: what passes it, and of the equals each warp's first W, of which the first W of all are taken.
+// By all threads; the candidates are complete when it returns. (16 x 8 beams over 128000 tokens, all but five masked: 20 us; value by value through the list 48.)
+template <typename T>
+__device__ __noinline__ void collect_again(Found& found, const T* logits, int first_vector, int of_lane, int before, int vocabulary, int beams, float largest, float least) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    auto look = [&](int whose, int number) {
+        const bool there = number < of_lane;
+        const int vector = vector_at(first_vector, there ? number : 0, whose);
+        return Look<T>{one_vector(logits, vector, before, there ? vocabulary : 0), there ? vector : -1};
+    };
+    __syncthreads();   // (all have seen the count)
+    if (threadIdx.x == 0) found.count = 0;
+    int equal = 0;
+#pragma unroll 1
+    for (int number = 0; number < of_lane && equal < beams; ++number) {   // (a warp's tokens in their order)
+        const Look<T> own = look(lane, number);
+        const uint32_t token = static_cast<uint32_t>(own.vector) * Look<T>::kValues;
+        uint32_t equals = 0;
+#pragma unroll
+        for (int i = 0; i < Look<T>::kValues; ++i) equals |= static_cast<uint32_t>(own.value(i) == least && token + i < static_cast<uint32_t>(vocabulary)) << i;
+        int upto = __popc(equals);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int below = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += below;
+        }
+        for (int at = equal + upto - __popc(equals); equals != 0 && at < beams; ++at, equals &= equals - 1) found.first_equals[warp][at] = token + __ffs(static_cast<int>(equals)) - 1;
+        equal += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    if (lane == 0) found.equals[warp] = min(equal, beams);
+    __syncthreads();
+    const int before_own = __reduce_add_sync(0xffffffffu, lane < warp ? found.equals[lane] : 0);
+    if (lane < min(beams - before_own, found.equals[warp])) found.add(least, found.first_equals[warp][lane]);
+    const float bound = from_ordered(ordered(least) + 1);   // (the next value; a NaN behind infinity, which none reaches)
+    for (uint32_t lanes = __ballot_sync(0xffffffffu, largest >= bound); lanes != 0; lanes &= lanes - 1) {
+#pragma unroll 1
+        for (int from = 0; from < of_lane; from += 32) found.take(look(__ffs(static_cast<int>(lanes)) - 1, from + lane), bound, vocabulary);
+        if (__any_sync(0xffffffffu, *static_cast<volatile int*>(&found.count) > kCandidates)) break;   // (all lanes or none)
+    }
+    __syncthreads();
+}
+
 template <typename T>
 __global__ void __launch_bounds__(32 * kScanWarps, 2)
 beam_scan_kernel(const ScanArgs a) {
@@ -203,14 +275,12 @@ beam_scan_kernel(const ScanArgs a) {
     __shared__ float largest_of_warp[kScanWarps][32];
     __shared__ double whole_of_warp[kScanWarps];
     __shared__ float reference_of_warp[kScanWarps];
-    __shared__ uint64_t candidates[kCandidates];
-    __shared__ int count;
-    __shared__ uint8_t lanes_of_warp[kScanWarps][32];
+    __shared__ Found found;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const Logits& l = a.logits;
     const int row = static_cast<int>(fast_divide(blockIdx.x, a.by_parts)), part = static_cast<int>(blockIdx.x) - row * l.parts;
     const int entry = static_cast<int>(fast_divide(static_cast<uint32_t>(row), a.by_beams)), beam = row - entry * l.beams;
-    if (threadIdx.x == 0) count = 0;
+    if (threadIdx.x == 0) found.count = 0;
     chain_begin();
     if (a.finished && a.finished[entry * a.finished_batch + beam * a.finished_beam] != 0) return;
     const T* logits = static_cast<const T*>(l.data) + entry * l.batch_stride + beam * l.beam_stride;
@@ -269,37 +339,29 @@ beam_scan_kernel(const ScanArgs a) {
     most = in_order(most, lane);
     float least = __shfl_sync(0xffffffffu, most, l.beams - 1);
     auto look = [&](int of_warp, int whose, int number) {
-        Pack<T, VE> own[1];
         const bool there = number < of_lane;
         const int vector = vector_at((part * kScanWarps + of_warp) * of_lane * 32, there ? number : 0, whose);
-        load_vectors<T, 1>(own, logits, vector, before, there ? l.vocabulary : 0);
-        return Look<T>{*reinterpret_cast<const uint4*>(&own[0]), there ? vector : -1};
+        return Look<T>{one_vector(logits, vector, before, there ? l.vocabulary : 0), there ? vector : -1};
     };
     // (Loops that are not unrolled: a warp comes by here once, and instructions that are run once are waited for.)
     // The lanes that reach the bound have their vectors looked through side by side, 32 at a time.
     const uint32_t lanes = __ballot_sync(0xffffffffu, largest >= least);
-    if (largest >= least) lanes_of_warp[warp][__popc(lanes & ((1u << lane) - 1))] = static_cast<uint8_t>(lane);
+    if (largest >= least) found.lanes[warp][__popc(lanes & ((1u << lane) - 1))] = static_cast<uint8_t>(lane);
     __syncwarp();
-    const int vectors = __popc(lanes) * of_lane;
+    int vectors = __popc(lanes) * of_lane;
+    if (lanes == 0xffffffffu) {   // (masks, equal logits: the second turn's)
+        vectors = 0;
+        if (lane == 0) atomicAdd(&found.count, kCandidates + 1);
+    }
 #pragma unroll 1
     for (int from = 0; from < vectors; from += 32) {
         const int place = (from + lane) / of_lane;
         const bool there = from + lane < vectors;
-        const Look<T> own = look(warp, there ? lanes_of_warp[warp][place] : 0, there ? from + lane - place * of_lane : of_lane);
-        if (own.vector >= 0) {
-            const uint32_t token = static_cast<uint32_t>(own.vector) * VE;
-#pragma unroll
-            for (int i = 0; i < VE; ++i) {
-                const float x = own.value(i);
-                if (x >= least && token + i < static_cast<uint32_t>(l.vocabulary)) {
-                    const int at = atomicAdd(&count, 1);   // (in any order: they are sorted)
-                    if (at < kCandidates) candidates[at] = static_cast<uint64_t>(ordered(x)) << 32 | ~(token + i);
-                }
-            }
-        }
-        if (__any_sync(0xffffffffu, *static_cast<volatile int*>(&count) > kCandidates)) break;   // (all lanes or none)
+        found.take(look(warp, there ? found.lanes[warp][place] : 0, there ? from + lane - place * of_lane : of_lane), least, l.vocabulary);
+        if (__any_sync(0xffffffffu, *static_cast<volatile int*>(&found.count) > kCandidates)) break;   // (all lanes or none)
     }
     __syncthreads();
+    if (__builtin_expect(found.count > kCandidates, 0)) collect_again<T>(found, logits, first_vector, of_lane, before, l.vocabulary, l.beams, largest, least);
     if (warp == 1) {
         // the warps' sums against the CTA's largest value (a warp of -inf alone has no reference that means anything)
         const float own_reference = lane < kScanWarps ? reference_of_warp[lane] : -INFINITY;
@@ -311,16 +373,16 @@ beam_scan_kernel(const ScanArgs a) {
     }
     if (warp != 0) return;
     Key list{0};
-    if (count <= kCandidates) {
+    if (found.count <= kCandidates) {
 #pragma unroll 1
-        for (int from = 0; from < count; from += 32) {
-            Key more{from + lane < count ? candidates[from + lane] : 0};
+        for (int from = 0; from < found.count; from += 32) {
+            Key more{from + lane < found.count ? found.candidates[from + lane] : 0};
             sort_lanes(more, lane);
             if (from == 0) list = more;
             else merge_lanes(list, more, lane);
         }
     } else {
-        // Many equals: one after another. The list fills up with the lowest tokens, and vectors behind them are no candidates any more.
+        // Many that pass the bound, all in few lanes: one after another. The list fills up with the lowest tokens, and vectors behind them are no candidates any more.
         uint32_t last_token = 0xffffffffu;
         uint64_t bound = static_cast<uint64_t>(ordered(least)) << 32;
 #pragma unroll 1

@@ -544,6 +544,38 @@ def test_beam_select_equals_and_masks(dtype):
     check_select(select(largest, torch.zeros(1, 2, device="cuda")), largest, torch.zeros(1, 2, device="cuda"))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("b,w,v", [(9, 4, 40001), (2, 32, 40001), (45, 8, 20001), (9, 1, 3000), (300, 2, 9000)])
+def test_beam_select_of_few_values_that_count(dtype, b, w, v):
+    """Masks that leave next to nothing, equal rows, and large values in few lanes: the bound is reached by far more values than are wanted."""
+    rng = np.random.default_rng(b * w)
+    logits, scores = randn(rng, (b, w, v), dtype), randn(rng, (b, w), F32)
+    token = torch.arange(v, device="cuda")
+    for entry in range(b):
+        x, kind = logits[entry], entry % 9 if b > 2 else 5 * entry
+        keep = torch.from_numpy(rng.random((w, v)) < 5 / v).cuda()
+        if kind == 0:
+            x.masked_fill_(~keep, -float("inf"))
+        elif kind == 1:
+            x.masked_fill_(~keep, torch.finfo(x.dtype).min)
+        elif kind == 2:
+            x.fill_(1.0)
+        elif kind == 3:
+            x.fill_(-2.0)
+            x[:, -10:] = 2.0
+        elif kind == 4:
+            x.copy_(torch.round(x))
+        elif kind == 5:   # two lanes of a warp have all the large ones
+            x[:, (token * x.element_size() // 16 % 32 == 3) | (token * x.element_size() // 16 % 32 == 17)] += 8.0
+        elif kind == 6:
+            x.masked_fill_(torch.from_numpy(rng.random((w, v)) < 0.5).cuda(), -float("inf"))
+        elif kind == 7:
+            x.copy_(torch.where(x > 0, 0.0, -0.0))
+        else:
+            x.masked_fill_(token != v - 1, -float("inf"))
+    check_select(select(logits, scores), logits, scores)
+
+
 def test_beam_select_strides_and_forks():
     rng = np.random.default_rng(6)
     b, w, v = 3, 5, 700
