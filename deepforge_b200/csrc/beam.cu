@@ -29,7 +29,8 @@ constexpr float kLog2e = 1.44269504088896341f;
 
 struct alignas(16) PartSum {
     double sum;                // of exp(x - most)
-    float most, unused;
+    double divisor;            // of the row's worths; of its first part only
+    float most;
 };
 struct Logits {
     const void* data;
@@ -38,12 +39,22 @@ struct Logits {
     PartSum* sums;                              // of a part
     uint64_t* keys;                             // of a part: W, falling; 0: none
 };
+struct Ints {
+    int32_t* data;              // null: absent
+    int64_t batch, beam;
+    __device__ __forceinline__ int32_t& at(int b, int w) const { return data[b * batch + w * beam]; }
+};
 struct ScanArgs {
     Logits logits;
-    const int32_t* finished;
-    int64_t finished_batch, finished_beam;
+    Ints finished, lengths;
+    float length_penalty;
     FastDivisor by_parts, by_beams;
 };
+
+// What a row's scores are divided by; n counts the token to come.
+__device__ __noinline__ double divisor_of(int length, bool done, float penalty) {
+    return pow(static_cast<double>(min(max(static_cast<int64_t>(length) + (done ? 0 : 1), static_cast<int64_t>(1)), static_cast<int64_t>(0x7fffffff))), static_cast<double>(penalty));
+}
 
 // Floats as whole numbers in the same order (0 is below all of them).
 __device__ __forceinline__ uint32_t ordered(float v) {
@@ -282,13 +293,18 @@ beam_scan_kernel(const ScanArgs a) {
     const int entry = static_cast<int>(fast_divide(static_cast<uint32_t>(row), a.by_beams)), beam = row - entry * l.beams;
     if (threadIdx.x == 0) found.count = 0;
     chain_begin();
-    if (a.finished && a.finished[entry * a.finished_batch + beam * a.finished_beam] != 0) return;
+    const bool done = a.finished.data && a.finished.at(entry, beam) != 0;   // (on its way with the first logits)
+    const bool divides = part == 0 && a.lengths.data && a.length_penalty != 0.0f;
     const T* logits = static_cast<const T*>(l.data) + entry * l.batch_stride + beam * l.beam_stride;
     // A lane's logits depend on their numbers alone, wherever the row starts, so that equal rows have equal sums.
     const int before = static_cast<int>((reinterpret_cast<uintptr_t>(logits) & 15u) / sizeof(T));
     const int of_lane = l.blocks * R, first_vector = (part * kScanWarps + warp) * of_lane * 32;
     Pack<T, VE> held[R], next[R];
     load_vectors<T, R>(held, logits, first_vector + lane, before, l.vocabulary);
+    if (done) {
+        if (divides && threadIdx.x == 0) l.sums[blockIdx.x].divisor = divisor_of(a.lengths.at(entry, beam), true, a.length_penalty);
+        return;
+    }
     float reference = 0.0f, largest = -INFINITY;   // reference: what exponentials are taken against, once there is `some` value
     bool some = false;
     uint64_t sums = 0;                             // of two halves, at most 64 terms each, before they go into `whole`
@@ -369,8 +385,12 @@ beam_scan_kernel(const ScanArgs a) {
         const double own_whole = lane < kScanWarps ? whole_of_warp[lane] : 0.0;
         double sum = own_whole == 0.0 ? 0.0 : own_whole * (own_reference == top || own_reference == -INFINITY ? 1.0 : exp(static_cast<double>(own_reference) - static_cast<double>(top)));
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0) l.sums[blockIdx.x] = PartSum{sum, top, 0.0f};
+        if (lane == 0) {
+            l.sums[blockIdx.x].sum = sum;
+            l.sums[blockIdx.x].most = top;
+        }
     }
+    if (warp == 2 && lane == 0 && divides) l.sums[blockIdx.x].divisor = divisor_of(a.lengths.at(entry, beam), false, a.length_penalty);   // (a power takes as long as the sort)
     if (warp != 0) return;
     Key list{0};
     if (found.count <= kCandidates) {
@@ -423,11 +443,6 @@ beam_scan_kernel(const ScanArgs a) {
     if (lane < l.beams) l.keys[static_cast<int64_t>(blockIdx.x) * l.beams + lane] = list.key;
 }
 
-struct Ints {
-    int32_t* data;              // null: absent
-    int64_t batch, beam;
-    __device__ __forceinline__ int32_t& at(int b, int w) const { return data[b * batch + w * beam]; }
-};
 struct MergeArgs {
     Logits logits;
     const float* scores;
@@ -457,32 +472,32 @@ beam_merge_kernel(const MergeArgs a) {
     uint64_t ahead[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) ahead[i] = i < l.parts && lane < l.beams ? l.keys[(first + i) * l.beams + lane] : 0;
-    PartSum sums = lane < l.parts ? l.sums[first + lane] : PartSum{0.0, 0.0f, 0.0f};
+    PartSum sums = lane < l.parts ? l.sums[first + lane] : PartSum{0.0, 1.0, 0.0f};
+    const bool divides = a.lengths.data && a.length_penalty != 0.0f;
+    const double divisor = divides ? __shfl_sync(0xffffffffu, sums.divisor, 0) : 1.0;
     Key list{ahead[0]};
     if (!done) {
+#pragma unroll 1
+        for (int from = 0; from < l.parts; from += kAhead) {
+            if (from > 0) {
 #pragma unroll
-        for (int i = 1; i < kAhead; ++i)
-            if (i < l.parts && __shfl_sync(0xffffffffu, ahead[i], 0) > list.from(l.beams - 1).key) merge_lanes(list, Key{ahead[i]}, lane);
-        for (int from = kAhead; from < l.parts; from += 32) {
-            const uint64_t own = from + lane < l.parts ? l.keys[(first + from + lane) * l.beams] : 0;
-            for (uint32_t lists = __ballot_sync(0xffffffffu, own > list.from(l.beams - 1).key); lists != 0; lists &= lists - 1) {
-                const int i = __ffs(static_cast<int>(lists)) - 1;
-                if (__shfl_sync(0xffffffffu, own, i) <= list.from(l.beams - 1).key) continue;
-                merge_lanes(list, Key{lane < l.beams ? l.keys[(first + from + i) * l.beams + lane] : 0}, lane);
+                for (int i = 0; i < kAhead; ++i) ahead[i] = from + i < l.parts && lane < l.beams ? l.keys[(first + from + i) * l.beams + lane] : 0;
             }
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i)
+                if (from + i > 0 && from + i < l.parts && __shfl_sync(0xffffffffu, ahead[i], 0) > list.from(l.beams - 1).key) merge_lanes(list, Key{ahead[i]}, lane);
         }
     }
     Place mine{0, 0xffffffffu};
     {
         length = min(max(length, static_cast<int64_t>(1)), static_cast<int64_t>(0x7fffffff));
-        const double divisor = a.lengths.data && a.length_penalty != 0.0f ? pow(static_cast<double>(length), static_cast<double>(a.length_penalty)) : 1.0;
         const bool alive = isfinite(score);
         const uint32_t row = static_cast<uint32_t>(beam) * static_cast<uint32_t>(l.vocabulary);
         if (done) {
-            if (lane == 0) mine = Place{ordered(alive ? static_cast<double>(score) / divisor : -static_cast<double>(INFINITY)), row + static_cast<uint32_t>(a.pad)};
+            if (lane == 0) mine = Place{ordered(!alive ? -static_cast<double>(INFINITY) : divides ? static_cast<double>(score) / divisor : static_cast<double>(score)), row + static_cast<uint32_t>(a.pad)};
         } else {
             for (int from = 32; from < l.parts; from += 32) {   // a lane's parts against the largest of them
-                const PartSum more = from + lane < l.parts ? l.sums[first + from + lane] : PartSum{0.0, 0.0f, 0.0f};
+                const PartSum more = from + lane < l.parts ? l.sums[first + from + lane] : PartSum{0.0, 1.0, 0.0f};
                 if (more.sum == 0.0) continue;   // (of -inf alone: its reference means nothing)
                 const float top = sums.sum != 0.0 ? fmaxf(sums.most, more.most) : more.most;
                 sums.sum = (sums.sum != 0.0 ? sums.sum * exp(static_cast<double>(sums.most) - static_cast<double>(top)) : 0.0) + more.sum * exp(static_cast<double>(more.most) - static_cast<double>(top));
@@ -497,7 +512,8 @@ beam_merge_kernel(const MergeArgs a) {
                 if (lane < l.vocabulary) mine = Place{ordered(-static_cast<double>(INFINITY)), row + static_cast<uint32_t>(lane)};
             } else if (list.key != 0) {
                 const double logit = static_cast<double>(from_ordered(static_cast<uint32_t>(list.key >> 32)));
-                mine = Place{ordered((static_cast<double>(score) + (logit - normaliser)) / divisor), row + ~static_cast<uint32_t>(list.key)};
+                const double worth = static_cast<double>(score) + (logit - normaliser);
+                mine = Place{ordered(divides ? worth / divisor : worth), row + ~static_cast<uint32_t>(list.key)};
             }
             if (lane >= l.beams) mine = Place{0, 0xffffffffu};
             // (equal worths of different logits, where 64 bits do not tell them apart, may be out of order)
@@ -718,9 +734,12 @@ extern "C" int dfgpu_beam_select(const dfgpu_beam_select_params* p, void* const*
     s.logits.blocks = static_cast<int>(cut.blocks);
     s.logits.sums = static_cast<PartSum*>(scratch);
     s.logits.keys = reinterpret_cast<uint64_t*>(s.logits.sums + units);
-    s.finished = static_cast<const int32_t*>(port[2]);
-    s.finished_batch = p->finished.rank ? p->finished.stride[0] : 0;
-    s.finished_beam = p->finished.rank ? p->finished.stride[1] : 0;
+    auto ints = [&](int i) {
+        return Ints{static_cast<int32_t*>(port[i]), port[i] ? described[i]->stride[0] : 0, port[i] ? described[i]->stride[1] : 0};
+    };
+    s.finished = ints(2);
+    s.lengths = ints(3);
+    s.length_penalty = p->length_penalty;
     s.by_parts = make_fast_divisor(static_cast<uint32_t>(cut.parts));
     s.by_beams = make_fast_divisor(static_cast<uint32_t>(beams));
     cudaStream_t on = as_stream(stream);
@@ -729,9 +748,6 @@ extern "C" int dfgpu_beam_select(const dfgpu_beam_select_params* p, void* const*
     status = check_launch("BEAM_SELECT");
     if (status) return status;
     MergeArgs m{};
-    auto ints = [&](int i) {
-        return Ints{static_cast<int32_t*>(port[i]), port[i] ? described[i]->stride[0] : 0, port[i] ? described[i]->stride[1] : 0};
-    };
     m.logits = s.logits;
     m.scores = static_cast<const float*>(port[1]);
     m.scores_batch = p->scores.stride[0];
