@@ -22,7 +22,6 @@
 namespace dfgpu {
 namespace {
 
-constexpr int kScanWarps = 16;
 constexpr int kCandidates = 256;  // of a CTA, that are sorted at once (32 beams leave some 130)
 constexpr int kMaxBeams = 32;
 constexpr float kLog2e = 1.44269504088896341f;
@@ -217,11 +216,12 @@ struct Look {
 };
 
 // A CTA's candidates.
+template <int WARPS>
 struct Found {
     uint64_t candidates[kCandidates];
-    uint32_t first_equals[kScanWarps][kMaxBeams];
-    int equals[kScanWarps], count;
-    uint8_t lanes[kScanWarps][32];
+    uint32_t first_equals[WARPS][kMaxBeams];
+    int equals[WARPS], count;
+    uint8_t lanes[WARPS][32];
     __device__ __forceinline__ void add(float value, uint32_t token) {
         const int at = atomicAdd(&count, 1);   // (in any order: they are sorted)
         if (at < kCandidates) candidates[at] = static_cast<uint64_t>(ordered(value)) << 32 | ~token;
@@ -239,8 +239,8 @@ struct Found {
 };
 // Where too many values equal the bound (masks, equal logits) for the candidates' room: what passes it, and of the equals each warp's first W, of which the first W of all are taken.
 // By all threads; the candidates are complete when it returns. (16 x 8 beams over 128000 tokens, all but five masked: 20 us; value by value through the list 48.)
-template <typename T>
-__device__ __noinline__ void collect_again(Found& found, const T* logits, int first_vector, int of_lane, int before, int vocabulary, int beams, float largest, float least) {
+template <typename T, int WARPS>
+__device__ __noinline__ void collect_again(Found<WARPS>& found, const T* logits, int first_vector, int of_lane, int before, int vocabulary, int beams, float largest, float least) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     auto look = [&](int whose, int number) {
         const bool there = number < of_lane;
@@ -279,14 +279,14 @@ __device__ __noinline__ void collect_again(Found& found, const T* logits, int fi
     __syncthreads();
 }
 
-template <typename T>
-__global__ void __launch_bounds__(32 * kScanWarps, 2)
+template <typename T, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS, 32 / WARPS)
 beam_scan_kernel(const ScanArgs a) {
     constexpr int VE = kVector<T>, R = kScanVectors;
-    __shared__ float largest_of_warp[kScanWarps][32];
-    __shared__ double whole_of_warp[kScanWarps];
-    __shared__ float reference_of_warp[kScanWarps];
-    __shared__ Found found;
+    __shared__ float largest_of_warp[WARPS][32];
+    __shared__ double whole_of_warp[WARPS];
+    __shared__ float reference_of_warp[WARPS];
+    __shared__ Found<WARPS> found;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const Logits& l = a.logits;
     const int row = static_cast<int>(fast_divide(blockIdx.x, a.by_parts)), part = static_cast<int>(blockIdx.x) - row * l.parts;
@@ -298,7 +298,7 @@ beam_scan_kernel(const ScanArgs a) {
     const T* logits = static_cast<const T*>(l.data) + entry * l.batch_stride + beam * l.beam_stride;
     // A lane's logits depend on their numbers alone, wherever the row starts, so that equal rows have equal sums.
     const int before = static_cast<int>((reinterpret_cast<uintptr_t>(logits) & 15u) / sizeof(T));
-    const int of_lane = l.blocks * R, first_vector = (part * kScanWarps + warp) * of_lane * 32;
+    const int of_lane = l.blocks * R, first_vector = (part * WARPS + warp) * of_lane * 32;
     Pack<T, VE> held[R], next[R];
     load_vectors<T, R>(held, logits, first_vector + lane, before, l.vocabulary);
     if (done) {
@@ -351,12 +351,12 @@ beam_scan_kernel(const ScanArgs a) {
     __syncthreads();
     float most = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kScanWarps; ++w) most = fmaxf(most, largest_of_warp[w][lane]);
+    for (int w = 0; w < WARPS; ++w) most = fmaxf(most, largest_of_warp[w][lane]);
     most = in_order(most, lane);
     float least = __shfl_sync(0xffffffffu, most, l.beams - 1);
     auto look = [&](int of_warp, int whose, int number) {
         const bool there = number < of_lane;
-        const int vector = vector_at((part * kScanWarps + of_warp) * of_lane * 32, there ? number : 0, whose);
+        const int vector = vector_at((part * WARPS + of_warp) * of_lane * 32, there ? number : 0, whose);
         return Look<T>{one_vector(logits, vector, before, there ? l.vocabulary : 0), there ? vector : -1};
     };
     // (Loops that are not unrolled: a warp comes by here once, and instructions that are run once are waited for.)
@@ -377,12 +377,12 @@ beam_scan_kernel(const ScanArgs a) {
         if (__any_sync(0xffffffffu, *static_cast<volatile int*>(&found.count) > kCandidates)) break;   // (all lanes or none)
     }
     __syncthreads();
-    if (__builtin_expect(found.count > kCandidates, 0)) collect_again<T>(found, logits, first_vector, of_lane, before, l.vocabulary, l.beams, largest, least);
+    if (__builtin_expect(found.count > kCandidates, 0)) collect_again<T, WARPS>(found, logits, first_vector, of_lane, before, l.vocabulary, l.beams, largest, least);
     if (warp == 1) {
         // the warps' sums against the CTA's largest value (a warp of -inf alone has no reference that means anything)
-        const float own_reference = lane < kScanWarps ? reference_of_warp[lane] : -INFINITY;
+        const float own_reference = lane < WARPS ? reference_of_warp[lane] : -INFINITY;
         const float top = __shfl_sync(0xffffffffu, most, 0);
-        const double own_whole = lane < kScanWarps ? whole_of_warp[lane] : 0.0;
+        const double own_whole = lane < WARPS ? whole_of_warp[lane] : 0.0;
         double sum = own_whole == 0.0 ? 0.0 : own_whole * (own_reference == top || own_reference == -INFINITY ? 1.0 : exp(static_cast<double>(own_reference) - static_cast<double>(top)));
         for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) {
@@ -406,9 +406,9 @@ beam_scan_kernel(const ScanArgs a) {
         uint32_t last_token = 0xffffffffu;
         uint64_t bound = static_cast<uint64_t>(ordered(least)) << 32;
 #pragma unroll 1
-        for (int w = 0; w < kScanWarps; ++w) {
+        for (int w = 0; w < WARPS; ++w) {
             const float value = largest_of_warp[w][lane];
-            const uint32_t first_token = static_cast<uint32_t>((part * kScanWarps + w) * of_lane * 32 + lane) * VE;
+            const uint32_t first_token = static_cast<uint32_t>((part * WARPS + w) * of_lane * 32 + lane) * VE;
 #pragma unroll 1
             for (uint32_t lanes = __ballot_sync(0xffffffffu, value > least || (value == least && first_token < last_token)); lanes != 0; lanes &= lanes - 1) {
 #pragma unroll 1
@@ -620,6 +620,7 @@ int check_beams(const dfgpu_tensor& t, const dfgpu_beam_select_params& p, int dt
 
 struct SelectCut {
     int64_t parts, blocks;   // of a row; of a part
+    int warps;               // of a CTA
 };
 int check_select(const dfgpu_beam_select_params& p, SelectCut& cut) {
     if (!valid_tensor(p.logits) || p.logits.rank != 3) return fail(kInvalidShape, "BEAM_SELECT: logits must be [B, W, V] with positive extents");
@@ -645,10 +646,13 @@ int check_select(const dfgpu_beam_select_params& p, SelectCut& cut) {
         if (!is_packed_row_major(p.forks)) return fail(kInvalidLayout, "BEAM_SELECT: forks must be packed");
         if (p.source_base < 0 || p.target_base < 0 || p.source_base + rows > 0x7fffffff || p.target_base + rows > 0x7fffffff) return fail(kInvalidValue, "BEAM_SELECT: sequence numbers out of range");
     }
-    // A block a warp, up to two CTAs for every SM, which run at once; then more blocks (16 x 8 beams, 128000 bf16 logits: 19.0 us; up to four CTAs 21.5, eight 28.8).
+    // A block a warp, up to 32 warps for every SM, which run at once; then more blocks (16 x 8 beams, 128000 bf16 logits: 19.0 us; up to four CTAs of 16 warps 21.5, eight 28.8).
     const int64_t values = 32 * kScanVectors * (16 / dtype_bytes(p.logits.dtype)), blocks = (p.logits.dim[2] + values - 1) / values;
+    // Sixteen warps a CTA; four where the rows are more than two CTAs an SM, whose second look and sorts then run under the others' loads (45 x 8 beams, 20001 bf16 logits: 22.9 us and 16.6;
+    // 26 x 12, 306 f32 ones 13.8 and 9.0), or short (2 x 15, 2024 f16 ones 10.1 and 9.4). With 256 rows of 32000 sixteen are the quicker, 13.5 and 15.3, with 7 x 5 of 50001 11.1 and 14.0.
+    cut.warps = rows > 2 * 148 || blocks <= 4 ? 4 : 16;
     cut.blocks = 1;
-    while (cut.parts = (blocks + kScanWarps * cut.blocks - 1) / (kScanWarps * cut.blocks), cut.parts > 1 && rows * cut.parts > 2 * 148) ++cut.blocks;
+    while (cut.parts = (blocks + cut.warps * cut.blocks - 1) / (cut.warps * cut.blocks), cut.parts > 1 && rows * cut.parts > 32 / cut.warps * 148) ++cut.blocks;
     if (rows * cut.parts >= (1ll << 31)) return fail(kUnsupported, "BEAM_SELECT: too many tokens or entries");
     return kOk;
 }
@@ -743,8 +747,12 @@ extern "C" int dfgpu_beam_select(const dfgpu_beam_select_params* p, void* const*
     s.by_parts = make_fast_divisor(static_cast<uint32_t>(cut.parts));
     s.by_beams = make_fast_divisor(static_cast<uint32_t>(beams));
     cudaStream_t on = as_stream(stream);
-    const dim3 grid(static_cast<unsigned>(units)), block(32 * kScanWarps);
-    launch_chained(p->logits.dtype == DFGPU_F32 ? beam_scan_kernel<float> : p->logits.dtype == DFGPU_F16 ? beam_scan_kernel<__half> : beam_scan_kernel<__nv_bfloat16>, grid, block, 0, on, s);
+    const dim3 grid(static_cast<unsigned>(units)), block(static_cast<unsigned>(32 * cut.warps));
+    void (*scan)(const ScanArgs) = beam_scan_kernel<__nv_bfloat16, 16>;
+    if (p->logits.dtype == DFGPU_F32) scan = cut.warps == 4 ? beam_scan_kernel<float, 4> : beam_scan_kernel<float, 16>;
+    else if (p->logits.dtype == DFGPU_F16) scan = cut.warps == 4 ? beam_scan_kernel<__half, 4> : beam_scan_kernel<__half, 16>;
+    else if (cut.warps == 4) scan = beam_scan_kernel<__nv_bfloat16, 4>;
+    launch_chained(scan, grid, block, 0, on, s);
     status = check_launch("BEAM_SELECT");
     if (status) return status;
     MergeArgs m{};
