@@ -18,6 +18,7 @@
 #include "ports.cuh"
 #include "rotary.cuh"
 #include "umma_ptx.cuh"
+#include "unaligned.cuh"
 
 namespace dfgpu {
 namespace {
@@ -109,17 +110,6 @@ __device__ __forceinline__ float power_of_two(float x) {
     return y;
 }
 
-// The 16 bytes that start `shift` bytes (a multiple of 2 or 4) into two aligned vectors.
-__device__ __forceinline__ uint4 shifted(const uint4& lo, const uint4& hi, int shift) {
-    uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-#pragma unroll
-    for (int k = 0; k < 6; ++k) w[k] = shift & 8 ? w[k + 2] : w[k];
-#pragma unroll
-    for (int k = 0; k < 5; ++k) w[k] = shift & 4 ? w[k + 1] : w[k];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) w[k] = __funnelshift_r(w[k], w[k + 1], (shift & 2) * 8);
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
 // Vectors first, first + 32, ... of a row that starts `before` elements behind a 16-byte boundary; what lies past its end is -inf.
 // Nothing outside the row is read (`first` is not negative): vectors whose aligned halves are not all the row's come element by element.
 template <typename T, int R>

@@ -2,7 +2,7 @@
 //
 // HBM bounds it (2 or 4 bytes in, 1 out for a value), and close behind it the instructions of each value; the scale has to be known before the first code, so a row's
 // vectors stay in registers between the two (what a row has beyond them is read again, from the cache). Alone, with more data than the L2 holds, 8192 x 4096: 25 us from
-// bf16 (the bytes alone 15.4), 29 from f32 (25.7); 32 x 4096 2.1 to 2.6; rows of 4097 that are not whole vectors, 5000 of them, 33 (9.4), value by value.
+// bf16 (the bytes alone 15.4), 29 from f32 (25.7); 32 x 4096 2.1 to 2.6. Rows that start anywhere come as aligned vectors shifted together: 3498 x 3451 bf16 20 (5.5; value by value 29), 20000 x 333 f16 13 (3.1; 21).
 #include <algorithm>
 
 #include "common.cuh"
@@ -10,6 +10,7 @@
 #include "ports.cuh"
 #include "rotary.cuh"
 #include "umma_ptx.cuh"
+#include "unaligned.cuh"
 
 namespace dfgpu {
 namespace {
@@ -124,9 +125,11 @@ __device__ __forceinline__ Codes<T, V> encode(const Pack<T, V>& x, float scale, 
 }
 
 // A row is taken by `THREADS` threads, a warp (four rows a CTA) or a CTA, which keep kHeld vectors each.
-template <typename T, int V, int THREADS, int kHeld>
+// ANYWHERE: rows that are no whole vectors, or do not start on their boundaries.
+template <typename T, bool ANYWHERE, int THREADS, int kHeld>
 __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS)
 token_quantize_kernel(const QuantizeArgs a) {
+    constexpr int V = 16 / static_cast<int>(sizeof(T));
     __shared__ uint32_t largest[THREADS / 32];
     const int thread = THREADS == 32 ? static_cast<int>(threadIdx.x & 31) : static_cast<int>(threadIdx.x);
     const int64_t row = THREADS == 32 ? static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5) : static_cast<int64_t>(blockIdx.x);
@@ -139,18 +142,51 @@ token_quantize_kernel(const QuantizeArgs a) {
         axis[2] = fast_divide(outer, a.by[1]);
         axis[1] = outer - static_cast<uint32_t>(axis[2]) * a.by[1].divisor;
     }
-    const T* x = static_cast<const T*>(a.x) + axis[0] * a.x_stride[0] + axis[1] * a.x_stride[1] + axis[2] * a.x_stride[2] + static_cast<int64_t>(thread) * V;
-    int8_t* y = a.y + axis[0] * a.y_stride[0] + axis[1] * a.y_stride[1] + axis[2] * a.y_stride[2] + static_cast<int64_t>(thread) * V;
+    const T* x = static_cast<const T*>(a.x) + axis[0] * a.x_stride[0] + axis[1] * a.x_stride[1] + axis[2] * a.x_stride[2];
+    int8_t* y = a.y + axis[0] * a.y_stride[0] + axis[1] * a.y_stride[1] + axis[2] * a.y_stride[2];
+    const int before = ANYWHERE ? static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T)) : 0;
+    const bool whole_codes = !ANYWHERE || (reinterpret_cast<uintptr_t>(y) & (V - 1)) == 0;
+    const T* own_x = x + static_cast<int64_t>(thread) * V;
+    int8_t* own_y = y + static_cast<int64_t>(thread) * V;
+    const int left = a.vectors - thread;   // vectors from this thread's first on
+    auto load = [&](int v) { return ANYWHERE ? vector_of<T>(x, (thread + v) * V, before, a.k) : *reinterpret_cast<const Pack<T, V>*>(own_x + v * V); };
+    auto store = [&](int from, const Codes<T, V>& codes) {
+        const int v = thread + from;
+        if (whole_codes && (!ANYWHERE || (v + 1) * V <= a.k)) {
+            *reinterpret_cast<Codes<T, V>*>(own_y + from * V) = codes;
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (v * V + i < a.k) y[v * V + i] = codes.v[i];
+        }
+    };
     Pack<T, V> held[kHeld];
     Largest<T> most;
-    const int left = a.vectors - thread;   // vectors from this thread's first on
+    if constexpr (ANYWHERE) {   // (all loads before the first is shifted)
+        uint4 halves[kHeld][2];
 #pragma unroll
-    for (int j = 0; j < kHeld; ++j)
-        if (j * THREADS < left) held[j] = *reinterpret_cast<const Pack<T, V>*>(x + j * THREADS * V);
+        for (int j = 0; j < kHeld; ++j) {
+            const int at = (thread + j * THREADS) * V;
+            if (!halves_inside<T>(at, before, a.k)) continue;
+            halves[j][0] = *reinterpret_cast<const uint4*>(x + at - before);
+            halves[j][1] = *reinterpret_cast<const uint4*>(x + at - before + V);
+        }
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j) {
+            const int at = (thread + j * THREADS) * V;
+            uint4 row = shifted(halves[j][0], halves[j][1], before * static_cast<int>(sizeof(T)));
+            if (at < a.k && !halves_inside<T>(at, before, a.k)) row = edge_vector<T>(x, at, a.k);
+            held[j] = *reinterpret_cast<const Pack<T, V>*>(&row);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j)
+            if (j * THREADS < left) held[j] = load(j * THREADS);
+    }
 #pragma unroll
     for (int j = 0; j < kHeld; ++j)
         if (j * THREADS < left) most.take(held[j]);
-    for (int v = kHeld * THREADS; v < left; v += THREADS) most.take(*reinterpret_cast<const Pack<T, V>*>(x + static_cast<int64_t>(v) * V));
+    for (int v = kHeld * THREADS; v < left; v += THREADS) most.take(load(v));
     uint32_t bits = __reduce_max_sync(0xffffffffu, most.as_f32());
     if (THREADS > 32) {
         if ((thread & 31) == 0) largest[thread >> 5] = bits;
@@ -165,9 +201,8 @@ token_quantize_kernel(const QuantizeArgs a) {
     const float inverse = __frcp_rn(scale);
 #pragma unroll
     for (int j = 0; j < kHeld; ++j)
-        if (j * THREADS < left) *reinterpret_cast<Codes<T, V>*>(y + j * THREADS * V) = encode<T, V>(held[j], scale, inverse, plain);
-    for (int v = kHeld * THREADS; v < left; v += THREADS)
-        *reinterpret_cast<Codes<T, V>*>(y + static_cast<int64_t>(v) * V) = encode<T, V>(*reinterpret_cast<const Pack<T, V>*>(x + static_cast<int64_t>(v) * V), scale, inverse, plain);
+        if (j * THREADS < left) store(j * THREADS, encode<T, V>(held[j], scale, inverse, plain));
+    for (int v = kHeld * THREADS; v < left; v += THREADS) store(v, encode<T, V>(load(v), scale, inverse, plain));
 }
 
 int check_quantize(const dfgpu_token_quantize_params& p, int& width) {
@@ -198,18 +233,19 @@ int check_quantize(const dfgpu_token_quantize_params& p, int& width) {
     return kOk;
 }
 
-template <typename T, int V>
+template <typename T, bool ANYWHERE>
 void launch_quantize(const QuantizeArgs& a, cudaStream_t stream) {
     // Many rows: four vectors a thread, since eight cost registers and so warps (8192 x 4096 bf16 35 us, 25 with four) and a persistent grid whose warps load the next row ahead
     // is slower yet (28 to 41). Up to two rows an SM there is nothing else to hide latency with, so that as many threads as there are take a row (32 x 4096 2.1 us, 2.7 with 128).
+    // A few vectors beyond what the threads keep are read again: half of twice the threads would have nothing to do.
     const unsigned rows = static_cast<unsigned>(a.rows), quarter = (rows + 3) / 4;
-    if (a.rows <= 2 * 148 && a.vectors > 64) launch_chained(token_quantize_kernel<T, V, 512, 2>, dim3(rows), dim3(512), 0, stream, a);
-    else if (a.vectors <= 64) launch_chained(token_quantize_kernel<T, V, 32, 2>, dim3(quarter), dim3(128), 0, stream, a);
-    else if (a.vectors <= 128) launch_chained(token_quantize_kernel<T, V, 32, 4>, dim3(quarter), dim3(128), 0, stream, a);
-    else if (a.vectors <= 256) launch_chained(token_quantize_kernel<T, V, 64, 4>, dim3(rows), dim3(64), 0, stream, a);
-    else if (a.vectors <= 512) launch_chained(token_quantize_kernel<T, V, 128, 4>, dim3(rows), dim3(128), 0, stream, a);
-    else if (a.vectors <= 1024) launch_chained(token_quantize_kernel<T, V, 256, 4>, dim3(rows), dim3(256), 0, stream, a);
-    else launch_chained(token_quantize_kernel<T, V, 512, 4>, dim3(rows), dim3(512), 0, stream, a);
+    if (a.rows <= 2 * 148 && a.vectors > 64) launch_chained(token_quantize_kernel<T, ANYWHERE, 512, 2>, dim3(rows), dim3(512), 0, stream, a);
+    else if (a.vectors <= 72) launch_chained(token_quantize_kernel<T, ANYWHERE, 32, 2>, dim3(quarter), dim3(128), 0, stream, a);
+    else if (a.vectors <= 144) launch_chained(token_quantize_kernel<T, ANYWHERE, 32, 4>, dim3(quarter), dim3(128), 0, stream, a);
+    else if (a.vectors <= 288) launch_chained(token_quantize_kernel<T, ANYWHERE, 64, 4>, dim3(rows), dim3(64), 0, stream, a);
+    else if (a.vectors <= 576) launch_chained(token_quantize_kernel<T, ANYWHERE, 128, 4>, dim3(rows), dim3(128), 0, stream, a);
+    else if (a.vectors <= 1152) launch_chained(token_quantize_kernel<T, ANYWHERE, 256, 4>, dim3(rows), dim3(256), 0, stream, a);
+    else launch_chained(token_quantize_kernel<T, ANYWHERE, 512, 4>, dim3(rows), dim3(512), 0, stream, a);
 }
 
 }  // namespace
@@ -259,11 +295,12 @@ extern "C" int dfgpu_token_quantize(const dfgpu_token_quantize_params* p, void* 
         a.rows *= p->x.dim[axis];
     }
     a.k = static_cast<int>(p->x.dim[rank - 1]);
-    a.vectors = a.k / width;
+    const int of_vector = 16 / dtype_bytes(p->x.dtype);
+    a.vectors = (a.k - 1) / of_vector + 1;
     a.flat = rank == 2;
     cudaStream_t on = as_stream(stream);
-    if (p->x.dtype == DFGPU_F32) width > 1 ? launch_quantize<float, 4>(a, on) : launch_quantize<float, 1>(a, on);
-    else if (p->x.dtype == DFGPU_F16) width > 1 ? launch_quantize<__half, 8>(a, on) : launch_quantize<__half, 1>(a, on);
-    else width > 1 ? launch_quantize<__nv_bfloat16, 8>(a, on) : launch_quantize<__nv_bfloat16, 1>(a, on);
+    if (p->x.dtype == DFGPU_F32) width > 1 ? launch_quantize<float, false>(a, on) : launch_quantize<float, true>(a, on);
+    else if (p->x.dtype == DFGPU_F16) width > 1 ? launch_quantize<__half, false>(a, on) : launch_quantize<__half, true>(a, on);
+    else width > 1 ? launch_quantize<__nv_bfloat16, false>(a, on) : launch_quantize<__nv_bfloat16, true>(a, on);
     return check_launch("TOKEN_QUANTIZE");
 }

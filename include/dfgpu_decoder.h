@@ -70,7 +70,8 @@ int dfgpu_head_norm_grad(const dfgpu_head_norm_grad_params*, void* const* tensor
    rounded once, so codes are the same wherever they are computed. A row of zeros (or below 2^-143) has scale 0 and codes 0; one with an infinity has an
    infinite scale and codes 0, one with a NaN a NaN scale and codes 0: its products are NaN.
    tensors: {X, Y, scale}. X FLOAT, HALF or BFLOAT16 [..., M, K], rank 2 to 4, K contiguous; Y INT8 of the same extents, K contiguous; scale
-   FLOAT [..., M, 1]. Weights [N, K] are quantised channel by channel in the same way. */
+   FLOAT [..., M, 1]. Weights [N, K] are quantised channel by channel in the same way. DFGPU_TOKEN_QUANTIZE_VECTOR: rows of whole 16-byte vectors on their
+   boundaries; DFGPU_TOKEN_QUANTIZE_SCALAR: any rows. */
 enum { DFGPU_TOKEN_QUANTIZE_AUTO = 0, DFGPU_TOKEN_QUANTIZE_VECTOR = 1, DFGPU_TOKEN_QUANTIZE_SCALAR = 2 };
 typedef struct dfgpu_token_quantize_params {
     dfgpu_tensor x, y, scale;

@@ -233,7 +233,7 @@ def select_params(b=2, w=4, v=100, dtype=BF16, **change):
 
 def test_beam_select_refusals():
     info = decoder.query("beam_select", select_params())
-    assert info.launches == 2 and info.scratch_bytes == 2 * 4 * 1 * (16 + 8 * 4)
+    assert info.launches == 2 and info.scratch_bytes == 2 * 4 * 1 * (32 + 8 * 4)
     ints = tensor(I32, [2, 4])
     assert decoder.query("beam_select", select_params(finished=ints, lengths=ints, finished_out=ints, lengths_out=ints, forks=tensor(I32, [8, 2]))).launches == 2
     refused(15, "beam_select", select_params(logits=tensor(BF16, [2, 4])))
