@@ -679,8 +679,7 @@ head_norm_grad_kernel(const __grid_constant__ NormArgs a) {
                 places[1][threadIdx.x] = of.dy;
                 places[2][threadIdx.x] = of.out;
             }
-            if (!first) __syncthreads();
-            angles_and_gains();
+            __syncthreads();
             int head = warp, base = 0, ahead = warp, ahead_base = 0;   // at hand, and the next to be fetched
             auto fetch = [&] {
                 const int token = ahead_base + group;
@@ -693,7 +692,8 @@ head_norm_grad_kernel(const __grid_constant__ NormArgs a) {
                 }
             };
 #pragma unroll
-            for (int i = 0; i + 1 < kGradientStages; ++i) fetch();
+            for (int i = 0; i + 1 < kGradientStages; ++i) fetch();   // (on their way while the angles are worked out)
+            angles_and_gains();
             while (head < heads) {
                 const int token = min(base + group, tokens - 1);
                 const bool live = base + group < tokens, last = base + groups >= tokens;
