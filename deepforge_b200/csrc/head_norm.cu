@@ -1161,8 +1161,21 @@ GradCut grad_cut(const NormProblem& p) {
         cut.of_side[1] = cut.runs - cut.first_of_second;
         return cut.tiles * cut.runs;
     };
-    while (ctas() < (of_heads ? 10 : 3) * 148 && cut.heads_per_cta > 4) cut.heads_per_cta = (cut.heads_per_cta + 1) / 2;
-    while (ctas() < 4 * 148 && cut.shift > 2) --cut.shift;
+    // Few tokens: runs of heads that fill the SMs once, since a CTA's own chain (places, angles, first rows, sums) is most of what it takes, fewer tokens and heads only where half the SMs would be left
+    // (3 x 2167 tokens of 1 + 1 heads of 80: 17.3 us by three CTAs an SM and any rest, 12.5 so; 4 x 67 of 2 + 2 of 64 13.3, 8.6; 1 x 411 of 56 + 8 of 128 19.8, 17.2; 8 x 26 of 47 + 8 of 96 15.1, 11.9).
+    const int64_t all = heads[0] + heads[1], slots = (x.dtype == DFGPU_F32 ? 6 : 4) * 148;   // CTAs that run at once
+    auto spread = [&] {
+        if (!of_heads) {   // runs that fill the slots once
+            ctas();
+            const int64_t runs = std::max<int64_t>(1, std::min(all, slots / cut.tiles));
+            cut.heads_per_cta = static_cast<int>(std::min<int64_t>(40, (all + runs - 1) / runs));
+        }
+        return ctas();
+    };
+    if (of_heads)
+        while (ctas() < 10 * 148 && cut.heads_per_cta > 4) cut.heads_per_cta = (cut.heads_per_cta + 1) / 2;
+    while (2 * spread() <= slots && cut.shift > 2) --cut.shift;
+    while (2 * ctas() <= slots && cut.heads_per_cta > 1) cut.heads_per_cta = (cut.heads_per_cta + 1) / 2;
     ctas();
     return cut;
 }
