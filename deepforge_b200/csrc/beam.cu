@@ -5,8 +5,8 @@
 // leftover. Of the largest values of the CTA's lanes (32 of them, each over all warps) the W-th largest is a bound that W values reach at least, and hardly more than W lanes
 // of some warp: their vectors are looked through again (from the caches), and what reaches the bound is sorted, a lane an entry.
 // Second kernel: a CTA an entry, a warp a beam, which merges its parts' lists; scores are added in 64 bits, beams merged pair by pair.
-// What bounds it are the two kernels' chains, not the bytes: 16 x 8 beams over 128000 bf16 tokens 18.8 us (bytes 5.0, exponentials 3.6), of which the second look and the sorts
-// take 3 to 4 and the second kernel 4; one user's four beams over 32000 tokens 7.6; 7 x 5 over 50001 f32 tokens 10.1.
+// What bounds it are the two kernels' chains, not the bytes: 16 x 8 beams over 128000 bf16 tokens 17.8 us (bytes 5.0, exponentials 3.6), of which the second look and the sorts
+// take 3 to 4 and the second kernel 4; one user's four beams over 32000 tokens 7.5; 7 x 5 over 50001 f32 tokens 10.1.
 //
 // Reordering: a copy; HBM bounds it. 2 x 8 layers of 8 x 4 rows of 131072 bf16 values 35 us (134 MB each way; a part of it stays in the L2 cache), a token history of 1000 2.4.
 #include <algorithm>

@@ -3,7 +3,7 @@
 // A row is one token's head, D channels. It is taken by a group of lanes that hold it in registers between its sum of squares and its result
 // (pairs that turn together lie in one lane), so that it is read once and written once: HBM is what bounds both kernels, and close behind it the chain of instructions of
 // a row, which few warps hide (registers hold the angles and the gradients' sums). 2 x 8192 tokens of 32 + 8 heads of 128 bf16 channels 58 us (the bytes alone 51); gradients of
-// 4 x 2048 such tokens 51.5 (38.5), of 3 x 1001 f32 tokens with gains of every head 38 (22.6), the sums of dgain among them (6, half of it behind the first kernel's end).
+// 4 x 2048 such tokens 51.5 (38.5), of 3 x 1001 f32 tokens with gains of every head 37.5 (22.6), the sums of dgain among them (6, half of it behind the first kernel's end).
 #include <algorithm>
 #include <cmath>
 

@@ -350,6 +350,24 @@ def test_token_quantize_strides():
     check_codes(flat[1:].view(3, 128), *quantize(flat[1:].view(3, 128)))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("rows,k", [(3, 40001), (300, 4097), (301, 577), (400, 9), (2, 15), (310, 2305), (299, 1)])
+def test_token_quantize_of_rows_anywhere(dtype, rows, k):
+    """Rows that start on any element and end inside a vector, codes that start on any byte; what lies around them stays and is not looked at."""
+    rng = np.random.default_rng(k)
+    for shift, codes_shift, pitch in ((0, 0, k), (1, 0, (k + 15) // 16 * 16 + 16), (3, 5, k + 2), (2, 3, k)):
+        base = torch.full((rows * pitch + 8,), float("nan"), device="cuda", dtype=TORCH[dtype])
+        x = base[shift:].as_strided((rows, k), (pitch, 1))
+        x.copy_(randn(rng, (rows, k), dtype, 3.0))
+        around = torch.full((rows * (k + 3) + 8,), 99, device="cuda", dtype=torch.int8)
+        y = around[codes_shift:].as_strided((rows, k), (k + 3, 1))
+        got, scale = quantize(x, y)
+        check_codes(x.contiguous(), got, scale)
+        mask = torch.ones_like(around, dtype=torch.bool)
+        mask[codes_shift:].as_strided((rows, k), (k + 3, 1)).fill_(False)
+        assert torch.all(around[mask] == 99)
+
+
 def int8s(rng, shape):
     return torch.from_numpy(rng.integers(-128, 128, shape).astype(np.int8)).cuda()
 
@@ -454,6 +472,8 @@ def test_matmul_int8_of_few_tokens(dtype, m, n, k):
     check_product(product(a, b, a_scale, b_scale, dtype, bias, kernel=few), a, b, a_scale, b_scale, bias)
     every, one = scales(rng, (2 * m, 3))[::2, :1], scales(rng, (1, 1))
     check_product(product(a, b, every, one, dtype, kernel=few), a, b, every, one)
+    turned = torch.full((n, m), 7.0, device="cuda", dtype=TORCH[dtype]).T
+    check_product(product(a, b, a_scale, b_scale, dtype, c=turned, kernel=few), a, b, a_scale, b_scale)
     # an infinite scale (a row with an infinity) and that of a NaN reach their own row alone
     a_scale[m - 1] = float("nan")
     got = product(a, b, a_scale, b_scale, dtype, kernel=few)
