@@ -1,8 +1,8 @@
 // Matrix products on the 5th-generation tensor cores for every extent: C = steps(A B), A [M, K] with K contiguous, B with
 // K or N contiguous, 16-bit floats (bf16, f16), FP8 codes (MATMUL_FP8), FP8 codes with E8M0 block scales (MXFP8) or 8-bit integers (MATMUL_INT8).
 //
-// kIntegers: sums in 32-bit integers, exact in any order and shape; partial tiles of a split K are added as integers. The scales of a row and of 32 columns at a time are loaded under the
-// products and multiplied in the epilogue. 8192 x 4096 x 4096 to bf16 86 us (96 % of twice the bf16 rate), 32 x 4096 x 4096 7.2 (16.8 MB of weights: 2.6).
+// kIntegers: sums in 32-bit integers, exact in any order and shape; partial tiles of a split K are added as integers. The scales of a row and of 32 columns at a time, and a 16-bit bias, are loaded under the
+// part before and applied in the epilogue (a bias waited for in its place: 2394 x 256 x 14016 41.5 us, 33.4 so). 8192 x 4096 x 4096 to bf16 86 us (96 % of twice the bf16 rate), 32 x 4096 x 4096 7.2 (16.8 MB of weights: 2.6).
 //
 // kPieces: f32 operands as three bf16 pieces each (split_f32.cu), six products of a K block's tiles per stage: every piece is copied
 // once for two products (six-fold deep copies moved and stored twice as much: 1183 x 1888 x 5360 154 us then, 128 now, 87 of
@@ -777,7 +777,7 @@ umma_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
             Scalars scalars = load_scalars<kCodesOnly>(args);
             int stored = 0;   // boxes this group has sent off
             int local = 0, status = 0;
-            const bool ahead = (KIND == kSixteen || KIND == kPieces) && args.step_count > 0 && args.step_kind[0] != kStepRelu && args.step_dtype[0] != DFGPU_F32;
+            const bool ahead = (KIND == kSixteen || KIND == kPieces || KIND == kIntegers) && args.step_count > 0 && args.step_kind[0] != kStepRelu && args.step_dtype[0] != DFGPU_F32;
             uint32_t first_operand[16];
             float columns_ahead[KIND == kIntegers ? 32 : 1], row_scale = 0.0f;
             for (int i = first_item; i < args.items; i += item_step, local += kInBlocks<KIND> ? 0 : 1) {
@@ -845,7 +845,15 @@ umma_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                             const bool same_box = part + 1 < box_columns / 32;
                             if (same_box || b + 2 < boxes) load_column_scales<32>(args, columns_ahead, same_box ? col + 32 : item.col0 + (b + 2) * box_columns);
                         }
-                        if (ahead) {
+                        if constexpr (KIND == kIntegers) {   // (a bias at most)
+                            if (ahead) {
+                                add_words<32>(v, first_operand, args.step_dtype[0]);
+                                const bool same_box = part + 1 < box_columns / 32;
+                                if (same_box || b + 2 < boxes) load_ahead(args, first_operand, out_row, same_box ? col + 32 : item.col0 + (b + 2) * box_columns, row_live);
+                            } else if (args.step_count > 0) {
+                                add_operand<32, 32>(v, args.step_data[0], args.step_dtype[0], col, args.n_total - col, args.step_vector[0] != 0);
+                            }
+                        } else if (ahead) {
                             uint32_t operand[16];
 #pragma unroll
                             for (int e = 0; e < 16; ++e) operand[e] = first_operand[e];
