@@ -1224,7 +1224,26 @@ extern "C" int dfgpu_head_norm(const dfgpu_head_norm_params* params, void* const
     const bool gains_of_heads = a.side[0].gain_head || a.side[1].gain_head;
     a.heads_per_cta = gains_of_heads && per_lane ? std::min(heads, std::max(kNormGains / (4 * a.d), 1)) : heads;
     auto runs = [&] { return (heads + a.heads_per_cta - 1) / a.heads_per_cta; };
-    while (tiles * runs() < 8 * 148 && (a.heads_per_cta << a.token_shift) > groups && a.heads_per_cta > 1) a.heads_per_cta = (a.heads_per_cta + 1) / 2;
+    // Runs of heads by what they would take: as many rounds as the CTAs need of the six an SM holds, three quarters of one lost beyond the first, each six steps of a CTA's own chain and its rows' (4 x 2048 tokens of 32 + 8 heads 31.3 us in
+    // two runs, 34.7 in one; 1 x 1024 9.6 in four, 12.0 in more; 1 x 411 of 56 + 8 7.2 in 16, 9.6 in 32). f32 rows take more runs (7 x 281 tokens of 10 + 8 heads 14.6 in six, 15.8 in two).
+    if (p.row[0][0]->dtype == DFGPU_F32) {
+        while (tiles * runs() < 8 * 148 && (a.heads_per_cta << a.token_shift) > groups && a.heads_per_cta > 1) a.heads_per_cta = (a.heads_per_cta + 1) / 2;
+    } else {
+        auto cost = [&] {
+            const double rounds = static_cast<double>(tiles * runs()) / (6 * 148);
+            return (rounds <= 1.0 ? 1.0 : rounds + 0.75) * (6 + ((a.heads_per_cta << a.token_shift) + groups - 1) / groups);
+        };
+        int best = a.heads_per_cta;
+        double least = cost();
+        while ((a.heads_per_cta << a.token_shift) > groups && a.heads_per_cta > 1) {
+            a.heads_per_cta = (a.heads_per_cta + 1) / 2;
+            if (cost() < least) {
+                least = cost();
+                best = a.heads_per_cta;
+            }
+        }
+        a.heads_per_cta = best;
+    }
     const dim3 grid(static_cast<unsigned>(tiles), static_cast<unsigned>(runs()));
     a.gain_floats = a.d * (gains_of_heads ? a.heads_per_cta + 1 : 2);
     const size_t shared = sizeof(float) * static_cast<size_t>((2 * a.half) << a.token_shift) + (per_lane ? 4 * static_cast<size_t>(a.gain_floats) + ring_bytes(kForwardStages, 1) : 0);
