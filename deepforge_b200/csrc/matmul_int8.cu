@@ -321,6 +321,13 @@ bool few_tokens(const dfgpu_matmul_int8_params& folded) {
     const dfgpu_tensor &a = folded.a, &b = folded.b;
     return a.dim[0] <= kFewTokens && (a.dim[1] == 1 || (a.stride[1] == 1 && b.stride[0] == 1)) && (a.dim[0] == 1 || a.stride[0] % 16 == 0) && (b.dim[1] == 1 || b.stride[1] % 16 == 0);
 }
+int check_cores(const dfgpu_matmul_int8_params& p) {
+    int64_t batches = 1;
+    for (int i = 0; i < p.c.rank - 2; ++i) batches = std::min<int64_t>(batches * p.c.dim[i], 1ll << 31);
+    const int64_t tiles = ((p.c.dim[p.c.rank - 2] + kTile - 1) / kTile) * ((p.c.dim[p.c.rank - 1] + kTile - 1) / kTile);
+    if (batches > 65535 || tiles >= (1ll << 31)) return fail(kUnsupported, "MATMUL_INT8: more than 65535 matrices or 2^31 tiles on the CUDA cores");
+    return kOk;
+}
 int choose_int8(const dfgpu_matmul_int8_params& p, int& kernel, dfgpu_matmul_int8_params& folded) {
     const bool folds = fold_batch(p, folded), tiles = folds && matmul_int8_umma_supported(folded), few = folds && few_tokens(folded);
     // Up to eight tokens the kernel for few of them is the quicker (1 x 4096 x 4096 4.9 us, tcgen05 6.8; x 12288 columns 10.7 and 13.1; 12288 x 4096 10.4 and 11.4; 4 x 1000 x 1111 3.0 and
@@ -329,7 +336,7 @@ int choose_int8(const dfgpu_matmul_int8_params& p, int& kernel, dfgpu_matmul_int
     kernel = p.kernel == DFGPU_MATMUL_INT8_AUTO ? (quicker ? DFGPU_MATMUL_INT8_FEW : tiles ? DFGPU_MATMUL_INT8_UMMA : DFGPU_MATMUL_INT8_CORES) : p.kernel;
     if (kernel == DFGPU_MATMUL_INT8_FEW && !few) return fail(kUnsupported, "MATMUL_INT8: the kernel for few tokens does not cover this shape or layout");
     if (kernel == DFGPU_MATMUL_INT8_UMMA && !tiles) return fail(kUnsupported, "MATMUL_INT8: the tcgen05 kernel does not cover this shape or layout");
-    return kOk;
+    return kernel == DFGPU_MATMUL_INT8_CORES ? check_cores(p) : kOk;
 }
 
 Int8Args args_of(const dfgpu_matmul_int8_params& p, void* const* tensors) {
@@ -408,12 +415,13 @@ extern "C" int dfgpu_matmul_int8(const dfgpu_matmul_int8_params* p, void* const*
         }
         if (p->kernel == DFGPU_MATMUL_INT8_FEW) return fail(kInvalidArgument, "MATMUL_INT8: the kernel for few tokens needs A and B on 16-byte boundaries");
     }
+    status = check_cores(*p);   // (another kernel's rows may be off their boundaries only now)
+    if (status) return status;
     Int8Args g = args_of(*p, tensors);
     int64_t batches = 1;
-    for (int i = 0; i < p->c.rank - 2; ++i) batches = std::min<int64_t>(batches * p->c.dim[i], 1ll << 31);
+    for (int i = 0; i < p->c.rank - 2; ++i) batches *= p->c.dim[i];
     g.m_tiles = (g.m + kTile - 1) / kTile;
     const int64_t tiles = g.m_tiles * ((g.n + kTile - 1) / kTile);
-    if (batches > 65535 || tiles >= (1ll << 31)) return fail(kUnsupported, "MATMUL_INT8: more than 65535 matrices or 2^31 tiles on the CUDA cores");
     launch_chained(matmul_int8_cores_kernel, dim3(static_cast<unsigned>(tiles), 1, static_cast<unsigned>(batches)), dim3(256), 0, as_stream(stream), g);
     return check_launch("MATMUL_INT8");
 }

@@ -212,6 +212,10 @@ def test_matmul_int8_refusals():
     assert decoder.query("matmul_int8", batched(3)).kernel == decoder.MATMUL_INT8_CORES
     assert decoder.query("matmul_int8", batched(1, a_scale=tensor(F32, [3, 1, 1]))).kernel == decoder.MATMUL_INT8_CORES
     refused(15, "matmul_int8", batched(2))
+    many = decoder.MatmulInt8Params()                                                                                                   # a matrix for each of 65536
+    many.a, many.b, many.c = tensor(I8, [65536, 1, 64]), tensor(I8, [65536, 64, 2]), tensor(BF16, [65536, 1, 2])
+    many.a_scale, many.b_scale = tensor(F32, [65536, 1, 1]), tensor(F32, [1, 1, 2])
+    refused(20, "matmul_int8", many, "65535")
     far = [(i + 1) << 20 for i in range(5)]
     call_refused(1, decoder.matmul_int8, int8_params(), [*far[:4], None], "null")
     call_refused(1, decoder.matmul_int8, int8_params(bias=tensor(F32, [1, 32])), far, "null")
