@@ -43,9 +43,6 @@ struct PagesArgs {
     int32_t batch, slots, pages, entries, block;
 };
 
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 // Once at the kernel's beginning, the two halves apart: nobody writes into another CTA's shared memory before that CTA is running.
 __device__ __forceinline__ void cluster_arrive_first() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait_first() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
@@ -94,7 +91,7 @@ __device__ __forceinline__ int2 cluster_scan(PagesShared& shared, int turn, int2
         asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(address) : "r"(own_address), "r"(to));
         asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(address), "r"(which ? all.y : all.x) : "memory");
     }
-    cluster_sync();
+    cluster_barrier();
     total = make_int2(0, 0);
     int2 base = make_int2(0, 0);
 #pragma unroll
@@ -144,13 +141,13 @@ cache_pages_kernel(PagesArgs a) {
             // the first entry that names a target; the lengths, which a target's new one may go over before its source's is asked for
             for (int i = thread; i < a.batch; i += kPagesAll) a.sequence_a[i] = 0x7fffffff, a.sequence_b[i] = length_of(a, i);
             copy_ints(a.lengths_out, a.lengths, a.batch, thread);
-            cluster_sync();
+            cluster_barrier();
             for (int i = thread; i < a.entries; i += kPagesAll) {
                 const int source = a.list[2 * i], target = a.list[2 * i + 1];
                 const bool fine = source >= 0 && source < a.batch && target >= 0 && target < a.batch && source != target && length_of(a, target) == 0;
                 if (fine) atomicMin(&a.sequence_a[target], i);
             }
-            cluster_sync();
+            cluster_barrier();
         }
         // Free pages before this thread's, and demand before this thread's sequences or entries.
         int page0, page1, from, until;
@@ -257,14 +254,14 @@ cache_pages_kernel(PagesArgs a) {
     } else if constexpr (OP == DFGPU_CACHE_PAGES_FREE) {
         for (int i = thread; i < a.batch; i += kPagesAll) a.sequence_a[i] = 0;
         copy_ints(a.refs_out, a.refs, a.pages, thread);
-        cluster_sync();
+        cluster_barrier();
         int2 mine = make_int2(0, 0);   // pages given back, refused
         for (int i = thread; i < a.entries; i += kPagesAll) {
             const int sequence = a.list[i];
             if (sequence >= 0 && sequence < a.batch) a.sequence_a[sequence] = 1;
             else mine.y += sequence >= a.batch;
         }
-        cluster_sync();
+        cluster_barrier();
         for (int i = warp; i < a.batch; i += kPagesAll / 32) {
             const bool drop = a.sequence_a[i] != 0;
             if (!drop && a.table == a.table_out) continue;
@@ -312,7 +309,7 @@ cache_pages_kernel(PagesArgs a) {
         int hole = before.y;
         for (int i = page0; i < min(page1, live); ++i)
             if (a.refs[i] <= 0) a.pages_a[hole++] = i;
-        cluster_sync();
+        cluster_barrier();
         int mover = before.x;
         for (int i = page0; i < page1; ++i) {
             int to = i;
@@ -330,7 +327,7 @@ cache_pages_kernel(PagesArgs a) {
             }
             a.pages_b[i] = to;
         }
-        cluster_sync();
+        cluster_barrier();
         for (int i = warp; i < a.batch; i += kPagesAll / 32) {
             const int used = slots_of(a, length_of(a, i));
             for (int s = lane; s < a.slots; s += 32) {
@@ -357,10 +354,10 @@ cache_pages_kernel(PagesArgs a) {
         int source, target;
         for (int i = thread; i < a.entries; i += kPagesAll)
             if (valid(i, source, target)) a.pages_a[source] = a.pages_a[target] = -1;   // the last entry that names a target
-        cluster_sync();
+        cluster_barrier();
         for (int i = thread; i < a.entries; i += kPagesAll)
             if (valid(i, source, target)) atomicMax(&a.pages_a[target], i);
-        cluster_sync();
+        cluster_barrier();
         int2 mine = make_int2(0, 0);   // copied, refused
         for (int i = thread; i < a.entries; i += kPagesAll) {
             const bool fine = valid(i, source, target);

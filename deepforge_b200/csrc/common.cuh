@@ -92,6 +92,12 @@ __device__ __forceinline__ void cluster_arrive_behind_loads(bool rare_sum_loaded
     if (__any_sync(0xffffffffu, rare_sum_loaded)) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     else asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
 }
+// A barrier of the cluster behind which its CTAs see one another's shared memory. `aligned` wants all threads of a warp at it together, which a branch or loop
+// before it does not see to by itself.
+__device__ __forceinline__ void cluster_barrier() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 // The pointer again, but known only from here on: a load through a const __restrict__ pointer counts as independent of
 // memory barriers, so only a data dependence keeps the compiler from moving it above the wait. The address passes through
 // as a global one: a pointer of unknown space would make generic loads of what were global ones (22 % on the CUDA-core MATMUL).

@@ -883,7 +883,7 @@ gain_sums_kernel(const __grid_constant__ GainArgs a) {
         if (threadIdx.x < 16) whole[tx] = sum;
     }
     if (a.cluster > 1) {
-        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        cluster_barrier();
         if (rank == 0 && threadIdx.x < 16) {
             for (int r = 1; r < a.cluster; ++r) {
                 uint32_t remote;
@@ -893,7 +893,7 @@ gain_sums_kernel(const __grid_constant__ GainArgs a) {
                 sum += other;
             }
         }
-        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");   // (no CTA leaves while its sums are read)
+        cluster_barrier();   // (no CTA leaves while its sums are read)
     }
     if (rank != 0 || threadIdx.x >= 16 || column >= s.columns) return;
     const int64_t head = column / s.d;

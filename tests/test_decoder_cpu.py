@@ -301,3 +301,19 @@ def test_beam_reorder_refusals():
     call_refused(1, decoder.beam_reorder, reorder_params(2), [far[0], far[1], far[2], far[3], far[1] + 32], "overlaps")
     call_refused(1, decoder.beam_reorder, reorder_params(2), [far[0], far[1], far[2], far[3], far[2]], "overlaps")
     call_refused(1, decoder.beam_reorder, reorder_params(), [far[0], far[1], far[0] - 16], "parents")
+
+
+# ---- barriers of clusters ---------------------------------------------------------------------------------
+
+def test_barriers_of_clusters_come_behind_a_converged_warp():
+    """`aligned` wants all threads of a warp at the barrier together, which a branch or loop before it does not see to: where such code stands before it, the barrier is the helper's, which has a __syncwarp()."""
+    sources = ROOT / "deepforge_b200" / "csrc"
+    helper = re.search(r"void cluster_barrier\(\) \{(.*?)\n\}", (sources / "common.cuh").read_text(), re.S)
+    assert helper and re.search(r"__syncwarp\(\);.*barrier\.cluster\.arrive\.release\.aligned.*barrier\.cluster\.wait\.acquire\.aligned", helper.group(1), re.S)
+    head_norm, pages = ((sources / name).read_text() for name in ("head_norm.cu", "cache_pages.cu"))
+    assert "barrier.cluster" not in head_norm and head_norm.count("cluster_barrier();") == 2
+    matmul = (sources / "umma_matmul.cu").read_text()
+    helpers = re.findall(r"void (\w+)\(\) \{\n    __syncwarp\(\);\n    asm volatile\(\"barrier\.cluster", matmul)
+    assert helpers == ["cluster_arrive", "cluster_arrive_relaxed", "cluster_wait"] and matmul.count("barrier.cluster") == 3
+    # (the pages' kernel: its first arrival and wait, before any branch, are its own)
+    assert re.findall(r"void (\w+)\(\) \{[^}]*barrier\.cluster", pages) == ["cluster_arrive_first", "cluster_wait_first"] and pages.count("barrier.cluster") == 2
