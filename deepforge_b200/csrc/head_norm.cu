@@ -418,24 +418,19 @@ head_norm_kernel(const __grid_constant__ NormArgs a) {
             }
             const float r = inverse_root<T>(__fmaf_rn(sum_over(sum2(squares), lanes), a.inverse_d, a.epsilon));
             const uint64_t both = pack2(r, r);
-            if (OF_HEADS && s.gain_head) {
-                const float* of_head = (which ? second_gains - second_head0 * a.d : first_gains - run0 * a.d) + min(head, heads - 1) * a.d;
-#pragma unroll
-                for (int j = 0; j < U; ++j) {
-                    Values<Form::kPacks> gain;
-                    take_gains<Form, V>(a, s, of_head, 0, share.channel[j], share.there[j], share.turns[j], gain);
-#pragma unroll
-                    for (int k = 0; k < Form::kPacks; ++k) {
-                        v[j].one[k] = mul2(v[j].one[k], gain.one[k]);
-                        v[j].two[k] = mul2(v[j].two[k], gain.two[k]);
-                    }
-                }
-            }
+            // (r first: a gain may take a row past f32's range whose r is 0)
+            const float* of_head = OF_HEADS && s.gain_head ? (which ? second_gains - second_head0 * a.d : first_gains - run0 * a.d) + min(head, heads - 1) * a.d : nullptr;
 #pragma unroll
             for (int j = 0; j < U; ++j) {
+                Values<Form::kPacks> gain;
+                if (of_head) take_gains<Form, V>(a, s, of_head, 0, share.channel[j], share.there[j], share.turns[j], gain);
 #pragma unroll
                 for (int k = 0; k < Form::kPacks; ++k) {
-                    const uint64_t one = mul2(v[j].one[k], both), two = mul2(v[j].two[k], both);
+                    uint64_t one = mul2(v[j].one[k], both), two = mul2(v[j].two[k], both);
+                    if (of_head) {
+                        one = mul2(one, gain.one[k]);
+                        two = mul2(two, gain.two[k]);
+                    }
                     v[j].one[k] = fma2(one, along[j].one[k], mul2(two, across[j].one[k]));
                     v[j].two[k] = fma2(two, along[j].two[k], mul2(one, across[j].two[k]));
                 }

@@ -296,6 +296,38 @@ def test_head_norm_gradient_of_many_tokens():
     assert all(torch.equal(a, b) for a, b in zip(dx + dgain, again[0] + again[1]))
 
 
+def rows_of(heads, i=0):
+    """X and dY of one side, to be changed."""
+    return heads.x[i], heads.dy[i]
+
+
+KERNELS = [decoder.HEAD_NORM_VECTOR, decoder.HEAD_NORM_SCALAR]
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("per_head", [False, True])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_head_norm_of_rows_whose_squares_pass_the_range(kernel, per_head, interleaved, dtype):
+    """Finite rows whose squares have no f32 sum give zeros, whatever the gain makes of their values before r; so do their gradients where the sum of v x is finite."""
+    heads = Heads(23, 2, 3, 2, 5, 64, 32, dtype, per_head=per_head, interleaved=interleaved, kernel=kernel)
+    for i in range(2):
+        x, _ = rows_of(heads, i)
+        heads.gain[i] = 2.0 + heads.gain[i]
+        signs = torch.sign(x[0, 1, 2]) + (x[0, 1, 2] == 0)
+        x[0, 1, 2], x[1, 0, 4] = 2e38 * signs, 1e20 * signs
+    for y in heads.forward():
+        assert torch.all(y[0, 1, 2] == 0) and torch.all(y[1, 0, 4] == 0) and torch.isfinite(y).all()
+    for i in range(2):
+        rows_of(heads, i)[0][0, 1, 2] = 1e20
+    dx, dgain = heads.gradient()
+    for i in range(2):
+        assert torch.all(dx[i][0, 1, 2] == 0) and torch.all(dx[i][1, 0, 4] == 0) and torch.isfinite(dx[i]).all()
+        rows_of(heads, i)[1][0, 1, 2] = rows_of(heads, i)[1][1, 0, 4] = 0
+    without = heads.gradient()[1]
+    assert all(torch.equal(a, b) for a, b in zip(dgain, without))   # (their terms are zeros)
+
+
 # ---- 8-bit integers ------------------------------------------------------------------------------------------
 
 def quantize(x, y=None, kernel=0, stream=None):
