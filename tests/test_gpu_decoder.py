@@ -328,6 +328,55 @@ def test_head_norm_of_rows_whose_squares_pass_the_range(kernel, per_head, interl
     assert all(torch.equal(a, b) for a, b in zip(dgain, without))   # (their terms are zeros)
 
 
+@pytest.mark.parametrize("kernel", KERNELS)
+@pytest.mark.parametrize("per_head", [False, True])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("rotary", [0, 32])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_head_norm_infinities_stay_in_channels_that_do_not_turn(kernel, per_head, interleaved, rotary, dtype):
+    """A channel that no position turns has no partner: an infinity in it is its own NaN (inf * 0) in Y and dgain, and every other value is what the definition says."""
+    def fresh():
+        return Heads(24, 2, 3, 2, 5, 64, rotary, dtype, per_head=per_head, interleaved=interleaved, kernel=kernel)
+    places = [(0, 1, 2, 41), (1, 2, 4, 62)]                          # rows of queries: of either half of a pair's place, head 1 and 2
+    channels = torch.arange(64, device="cuda")
+    heads, plain = fresh(), fresh()
+    for b, h, s, c in places:
+        heads.x[0][b, h, s, c] = float("inf")
+    y, want = heads.forward(), plain.forward()
+    (dx, dgain), still = heads.gradient(), fresh()
+    for b, h, s, c in places:
+        assert torch.equal(torch.isnan(y[0][b, h, s]), channels == c) and torch.all(y[0][b, h, s][channels != c] == 0)
+        assert torch.isnan(dx[0][b, h, s]).all()                    # (r^3 of 0 times a mean of infinity)
+        y[0][b, h, s] = want[0][b, h, s]
+        still.dy[0][b, h, s] = 0
+    assert torch.equal(y[0], want[0]) and torch.equal(y[1], want[1])
+    rest = still.gradient()[1]                                       # the other channels' terms of these rows are u x 0 = 0
+    hit = torch.zeros_like(dgain[0], dtype=torch.bool)
+    for _, h, _, c in places:
+        hit[h if per_head else 0, c] = True
+    assert torch.equal(torch.isnan(dgain[0]), hit) and torch.equal(dgain[0][~hit], rest[0][~hit]) and torch.equal(dgain[1], rest[1])
+    # an infinity in dY: the mean of v x is one, so dX of its row is -x times it, NaN in its own channel; dgain has it in its channel alone
+    heads = fresh()
+    for b, h, s, c in places:
+        heads.dy[0][b, h, s, c] = float("inf")
+    (dx, dgain), (want, _) = heads.gradient(), fresh().gradient()
+    for b, h, s, c in places:
+        x = heads.x[0][b, h, s].float()
+        sign = torch.sign(x) * torch.sign(x[c])
+        others = (channels != c) & (x != 0)
+        assert torch.isnan(dx[0][b, h, s, c]) and torch.equal(dx[0][b, h, s][others].float(), -float("inf") * sign[others])
+        dx[0][b, h, s] = want[0][b, h, s]
+    assert torch.equal(dx[0], want[0]) and torch.equal(dx[1], want[1])
+    assert torch.equal(torch.isinf(dgain[0]), hit) and torch.isfinite(dgain[0][~hit]).all() and torch.isfinite(dgain[1]).all()
+    x, gain, at, frequencies, half = heads.parts(0)
+    finite = np.where(np.isinf(double(heads.dy[0])), 0.0, double(heads.dy[0]))
+    sums = ref.head_norm_grad(x, finite, gain, at, frequencies, interleaved)[1]
+    terms = (ref.both_of_pair(finite, half, interleaved) * np.abs(x) / np.sqrt((x * x).mean(-1, keepdims=True) + 1e-6)).sum((0, 2))
+    terms = terms if per_head else terms.sum(0, keepdims=True)
+    keep = ~hit.cpu().numpy()
+    assert np.all((np.abs(double(dgain[0]) - sums) <= terms * (heads.turn_error(half) + 185 * U))[keep])   # (as in check_gradient(), for f32 sums)
+
+
 # ---- 8-bit integers ------------------------------------------------------------------------------------------
 
 def quantize(x, y=None, kernel=0, stream=None):
