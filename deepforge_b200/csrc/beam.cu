@@ -25,6 +25,7 @@ namespace {
 
 constexpr int kCandidates = 256;  // of a CTA, that are sorted at once (32 beams leave some 130)
 constexpr int kMaxBeams = 32;
+constexpr float kMaxPenalty = 28.0f;
 constexpr float kLog2e = 1.44269504088896341f;
 
 struct alignas(16) PartSum {
@@ -628,7 +629,8 @@ int check_select(const dfgpu_beam_select_params& p, SelectCut& cut) {
     if (!status && p.lengths_out.rank) status = check_beams(p.lengths_out, p, DFGPU_I32, "lengths_out", true);
     if (status) return status;
     if (p.lengths_out.rank && !p.lengths.rank) return fail(kInvalidArgument, "BEAM_SELECT: lengths_out without lengths");
-    if (p.lengths.rank && !std::isfinite(p.length_penalty)) return fail(kInvalidValue, "BEAM_SELECT: the length penalty must be finite");
+    // (n^28 is at most 2^868: what f32 scores are over it and times it stays within 64 bits, where worths are compared and scores come back from them)
+    if (p.lengths.rank && !(std::fabs(p.length_penalty) <= kMaxPenalty)) return fail(kInvalidValue, "BEAM_SELECT: the length penalty must be within -28 and 28");
     if (p.finished.rank && (p.pad < 0 || p.pad >= p.logits.dim[2])) return fail(kInvalidValue, "BEAM_SELECT: pad is no token");
     const int64_t rows = p.logits.dim[0] * p.logits.dim[1];
     if (p.forks.rank) {

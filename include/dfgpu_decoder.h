@@ -100,7 +100,8 @@ int dfgpu_matmul_int8(const dfgpu_matmul_int8_params*, void* const* tensors, voi
 /* ---- beam search -------------------------------------------------------------------------------
    A batch entry has W beams (at most 32). Beam w that is not finished continues with each of the V tokens t, at score(w) + logits(w, t) - ln sum exp logits(w, .); one that
    is finished with the token `pad` alone, at score(w). The W continuations of the greatest worth are kept, in falling order; equals go to the lower
-   beam, then the lower token. Worth is the score; with lengths, score / n^length_penalty, where n = max(1, lengths(w) + 1), for a finished beam max(1, lengths(w)).
+   beam, then the lower token. Worth is the score; with lengths, score / n^length_penalty, where n = max(1, lengths(w) + 1), for a finished beam max(1, lengths(w));
+   length_penalty is within -28 and 28.
    Sums of exponentials are f32 over at most 64 terms of a thread and meet in 64 bits, where scores are added and compared. A beam whose score is not
    finite, or whose logits have no finite sum of exponentials (a NaN, +inf, all -inf), continues at -inf: with its tokens 0, 1, ...,
    which are kept only where fewer than W others are finite; the same holds for logits of -inf.

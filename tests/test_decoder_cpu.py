@@ -317,3 +317,13 @@ def test_barriers_of_clusters_come_behind_a_converged_warp():
     assert helpers == ["cluster_arrive", "cluster_arrive_relaxed", "cluster_wait"] and matmul.count("barrier.cluster") == 3
     # (the pages' kernel: its first arrival and wait, before any branch, are its own)
     assert re.findall(r"void (\w+)\(\) \{[^}]*barrier\.cluster", pages) == ["cluster_arrive_first", "cluster_wait_first"] and pages.count("barrier.cluster") == 2
+
+
+def test_beam_select_refuses_penalties_whose_powers_have_no_place():
+    """Worths are scores over n^penalty in 64 bits, n up to 2^31 - 1: 2^(31 * 28) = 2^868 leaves room for f32 scores (2^-149 to 2^128) on either side of what 64 bits hold (2^-1022 to 2^1024)."""
+    ints = tensor(I32, [2, 4])
+    for penalty in (28.5, -28.5, 400.0, -400.0, 3e38, float("nan"), -float("inf")):
+        refused(8, "beam_select", select_params(lengths=ints, length_penalty=penalty), "penalty")
+        assert decoder.query("beam_select", select_params(length_penalty=penalty)).launches == 2   # (read only with lengths)
+    for penalty in (28.0, -28.0, 0.0):
+        assert decoder.query("beam_select", select_params(lengths=ints, length_penalty=penalty)).launches == 2

@@ -720,6 +720,22 @@ def test_beam_reorder_leaves_rows_of_bad_parents():
     assert torch.equal(target, want)
 
 
+@pytest.mark.parametrize("penalty", [28.0, -28.0])
+def test_beam_select_penalties_at_the_ends(penalty):
+    """The largest penalties with the longest lengths: worths stay within 64 bits, and scores come out of them whole; finished beams of score 0 too."""
+    rng = np.random.default_rng(8)
+    logits, scores = randn(rng, (4, 3, 50), F32, 3.0), randn(rng, (4, 3), F32) - 5
+    scores[0], scores[1, 0], scores[2] = 0.0, -3e38, -1e-38
+    lengths, finished = ints([[0x7FFFFFFF, 0x7FFFFFFE, 1], [2, 3, 4], [0x7FFFFFFF] * 3, [-5, 0, 100]]), ints([[1, 0, 1], [0, 0, 1], [1, 1, 0], [0, 0, 0]])
+    more = dict(finished=finished, lengths=lengths, penalty=penalty, end=7, pad=3)
+    out = select(logits, scores, **more)
+    assert torch.isfinite(out["scores_out"]).all()
+    want = ref.beam_select(double(logits), double(scores), finished.cpu().numpy(), lengths.cpu().numpy(), penalty, 7, 3)
+    assert np.array_equal(out["tokens"].cpu().numpy(), want[1]) and np.array_equal(out["parents"].cpu().numpy(), want[2])
+    # (as in check_select(), with three roundings of 64 bits for quotient, power and product)
+    assert np.all(np.abs(double(out["scores_out"]) - want[0]) <= 75 * U + 1.001 * U * np.abs(want[0]))
+
+
 # ---- streams and graphs -------------------------------------------------------------------------------------------
 
 def test_two_streams_and_graphs():
