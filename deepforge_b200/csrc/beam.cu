@@ -550,7 +550,7 @@ struct StateSide {
     uint8_t* target;
     int64_t source_stride[3], target_stride[3];   // layer, entry, beam, in bytes
     int64_t row_bytes;
-    int32_t width, layers, first_unit;            // bytes of a vector; the state's first unit
+    int32_t width, first_unit;                    // bytes of a vector; the state's first unit
     FastDivisor by_segments;
 };
 struct ReorderArgs {
@@ -802,7 +802,6 @@ extern "C" int dfgpu_beam_reorder(const dfgpu_beam_reorder_params* p, void* cons
         StateSide& side = a.state[i];
         side.source = static_cast<const uint8_t*>(tensors[1 + 2 * i]);
         side.target = static_cast<uint8_t*>(tensors[2 + 2 * i]);
-        side.layers = static_cast<int>(s.dim[0]);
         side.row_bytes = s.dim[3] * bytes;
         side.width = 16;
         uint64_t places = reinterpret_cast<uintptr_t>(side.source) | reinterpret_cast<uintptr_t>(side.target) | static_cast<uint64_t>(side.row_bytes);

@@ -90,11 +90,11 @@ struct RawUnit {
     using Form = NormUnit<T, V, INTERLEAVED>;
     using In = Values<Form::kPacks>;
     Pack<T, V> first, second;
-    __device__ __forceinline__ void load(const T* from, int apart, bool live, bool turns) {
+    __device__ __forceinline__ void load(const T* from, int apart, bool turns) {
+        first = *reinterpret_cast<const Pack<T, V>*>(from);
 #pragma unroll
-        for (int i = 0; i < V; ++i) first.v[i] = second.v[i] = narrow<T>(0.0f);
-        if (live) first = *reinterpret_cast<const Pack<T, V>*>(from);
-        if (Form::kTwo && live && turns) second = *reinterpret_cast<const Pack<T, V>*>(from + apart);
+        for (int i = 0; i < V; ++i) second.v[i] = narrow<T>(0.0f);
+        if (Form::kTwo && turns) second = *reinterpret_cast<const Pack<T, V>*>(from + apart);
     }
     __device__ __forceinline__ In values() const {
         In v;
@@ -504,7 +504,7 @@ head_norm_long_kernel(const __grid_constant__ NormArgs a) {
             uint64_t squares = 0;
             for (int unit = lane; unit < a.units; unit += 32) {
                 Raw raw;
-                raw.load(from + Form::channel(a, unit), apart, true, unit < a.turning);
+                raw.load(from + Form::channel(a, unit), apart, unit < a.turning);
                 const Values<Form::kPacks> v = raw.values();
 #pragma unroll
                 for (int k = 0; k < Form::kPacks; ++k) squares = fma2(v.two[k], v.two[k], fma2(v.one[k], v.one[k], squares));
@@ -515,7 +515,7 @@ head_norm_long_kernel(const __grid_constant__ NormArgs a) {
                 const bool turns = unit < a.turning;
                 const int channel = Form::channel(a, unit);
                 Raw raw;
-                raw.load(from + channel, apart, true, turns);
+                raw.load(from + channel, apart, turns);
                 Values<Form::kPacks> v = raw.values(), gain;
                 load_gains<Form, V>(a, s, s.gain_head ? head0 + head : 0, channel, true, turns, gain);
 #pragma unroll
@@ -809,8 +809,8 @@ head_norm_grad_long_kernel(const __grid_constant__ NormArgs a) {
                         const bool turns = unit < a.turning;
                         const int channel = Form::channel(a, unit);
                         Raw raw_x, raw_dy;
-                        raw_x.load(from_x + channel, apart, true, turns);
-                        raw_dy.load(from_dy + channel, apart, true, turns);
+                        raw_x.load(from_x + channel, apart, turns);
+                        raw_dy.load(from_dy + channel, apart, turns);
                         const Values<Form::kPacks> v = raw_x.values();
                         Values<Form::kPacks> u = raw_dy.values(), gain, terms{};
                         load_gains<Form, V>(a, s, s.gain_head ? head0 + head : 0, channel, true, turns, gain);
@@ -1337,9 +1337,9 @@ extern "C" int dfgpu_head_norm_grad(const dfgpu_head_norm_grad_params* params, v
     }
     const dim3 grid(static_cast<unsigned>(cut.tiles), static_cast<unsigned>(cut.runs));
     const size_t table = sizeof(float) * static_cast<size_t>((2 * a.half) << a.token_shift), meeting = sizeof(float) * kNormWarps * static_cast<size_t>(a.d);
-    // (the form for tokens a group needs as many groups as tokens; with narrower vectors than the cut had in mind a row may take more lanes)
+    // (The form for tokens a group needs as many groups as tokens, and has them where the vectors are narrower than the cut had in mind too: a row of half as long vectors has twice the units, of
+    // which a lane has twice as many; single values are a warp's.)
     const bool of_heads = any_sums_of_heads(p);
-    if (per_lane && !of_heads && (kNormThreads >> a.group_shift) < (1 << a.token_shift)) per_lane = 0;
     launch_norm(!per_lane ? kGradientLong : of_heads ? kGradientOfHeads : kGradient, a, p.row[0][0]->dtype, p.width, p.interleaved != 0, grid,
                 table + (per_lane ? 8 * static_cast<size_t>(a.d) + std::max(ring_bytes(kGradientStages, 2), meeting) : meeting),
                                 as_stream(stream));

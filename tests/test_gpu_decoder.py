@@ -377,6 +377,30 @@ def test_head_norm_infinities_stay_in_channels_that_do_not_turn(kernel, per_head
     assert np.all((np.abs(double(dgain[0]) - sums) <= terms * (heads.turn_error(half) + 185 * U))[keep])   # (as in check_gradient(), for f32 sums)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("per_head", [False, True])
+@pytest.mark.parametrize("d,rotary", [(64, 32), (128, 128), (256, 0), (512, 256)])
+def test_head_norm_on_8_byte_boundaries(dtype, interleaved, per_head, d, rotary):
+    """Rows of 16-bit values that start 8 bytes behind a 16-byte boundary: the launch takes shorter vectors than the scratch was cut for."""
+    def moved(t, places):
+        flat = torch.full((t.numel() + 8,), 7.0, device="cuda", dtype=t.dtype)
+        view = flat[places:places + t.numel()].view(t.shape)
+        view.copy_(t)
+        return view
+    heads = Heads(25, 3, 5, 2, 37, d, rotary, dtype, per_head=per_head, interleaved=interleaved)
+    want, (want_dx, want_dgain) = heads.forward(), heads.gradient()
+    for tensors in ("x", "dy", "out"):
+        again = Heads(25, 3, 5, 2, 37, d, rotary, dtype, per_head=per_head, interleaved=interleaved)
+        out = [moved(torch.zeros_like(x), 4 if tensors == "out" else 0) for x in again.x]
+        if tensors != "out":
+            setattr(again, tensors, [moved(t, 4) for t in getattr(again, tensors)])
+        again.kernel = decoder.HEAD_NORM_VECTOR
+        again.check_forward(again.forward(out=out))
+        again.check_gradient(*again.gradient(out=out))
+    assert want[0].shape == want_dx[0].shape and want_dgain[0].shape[1] == d
+
+
 # ---- 8-bit integers ------------------------------------------------------------------------------------------
 
 def quantize(x, y=None, kernel=0, stream=None):
