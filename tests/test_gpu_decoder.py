@@ -587,6 +587,21 @@ def test_matmul_int8_of_few_tokens(dtype, m, n, k):
         check_product(got[: m - 1], a[: m - 1], b, a_scale[: m - 1], b_scale)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("m,n,k", [(20, 70, 100), (130, 300, 384), (64, 1111, 2048), (600, 1040, 200)])
+def test_matmul_int8_scales_of_the_tensor_cores_anywhere(dtype, m, n, k):
+    """tcgen05 with scales of rows and columns that lie apart, that start on any float, and one for all of either side; whole and split K."""
+    rng = np.random.default_rng(m * n)
+    a, b = rows16(int8s(rng, (m, k))), rows16(int8s(rng, (n, k))).T
+    every_row, every_column = scales(rng, (3 * m, 2))[::3, 1:], scales(rng, (1, 2 * n + 1))[:, 1::2]
+    row, column = scales(rng, (m + 1, 1))[1:], scales(rng, (1, n + 1))[:, 1:]
+    one = scales(rng, (1, 1))
+    bias = randn(rng, (1, n + 1), dtype)[:, 1:]
+    for a_scale, b_scale in ((every_row, every_column), (row, column), (every_row, one), (one, every_column), (row, every_column), (every_row, column)):
+        for more in (None, bias):
+            check_product(product(a, b, a_scale, b_scale, dtype, more, kernel=decoder.MATMUL_INT8_UMMA), a, b, a_scale, b_scale, more)
+
+
 # ---- beam search ---------------------------------------------------------------------------------------------
 
 def select(logits, scores, finished=None, lengths=None, penalty=0.0, end=-1, pad=0, bases=None, in_place=False, stream=None, scratch=None):
@@ -712,6 +727,21 @@ def test_beam_select_strides_and_forks():
     forks = out["forks"].view(b, w, 2)
     at = torch.arange(b, device="cuda")[:, None] * w
     assert torch.equal(forks[..., 0], 100 + at + out["parents"]) and torch.equal(forks[..., 1], 7 + at + torch.arange(w, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("b,w,v", [(2, 3, 7), (3, 4, 5001), (40, 8, 3001)])
+def test_beam_select_lengths_and_finished_apart(dtype, b, w, v):
+    """Lengths without flags of what is finished, and flags without lengths; in place too."""
+    rng = np.random.default_rng(b * v)
+    logits, scores = randn(rng, (b, w, v), dtype, 3.0), randn(rng, (b, w), F32, 4.0) - 20
+    finished, lengths = ints(rng.integers(0, 3, (b, w)) == 0), ints(rng.integers(0, 60, (b, w)))
+    for more in (dict(lengths=lengths, penalty=0.7, end=v // 2), dict(lengths=lengths), dict(finished=finished, end=v // 2, pad=v - 1)):
+        want = select(logits, scores, **more)
+        check_select(want, logits, scores, **more)
+        held = {n: t.clone() if torch.is_tensor(t) else t for n, t in more.items()}
+        got = select(logits, scores.clone(), in_place=True, **held)
+        assert all(torch.equal(got[n], want[n]) for n in want if want[n] is not None)
 
 
 @pytest.mark.parametrize("dtype", [torch.uint8, torch.bfloat16, torch.float32, torch.int64])
