@@ -8,7 +8,9 @@
 // What bounds it are the two kernels' chains, not the bytes: 16 x 8 beams over 128000 bf16 tokens 17.8 us (bytes 5.0, exponentials 3.6), of which the second look and the sorts
 // take 3 to 4 and the second kernel 4; one user's four beams over 32000 tokens 7.5; 7 x 5 over 50001 f32 tokens 10.1.
 //
-// Reordering: a copy; HBM bounds it. 2 x 8 layers of 8 x 4 rows of 131072 bf16 values 35 us (134 MB each way; a part of it stays in the L2 cache), a token history of 1000 2.4.
+// Reordering: a copy, by the widest vectors that divide all of a state's places and its rows' bytes. HBM bounds it from 8-byte vectors up: 2 x 8 layers of 8 x 4 rows of 131072 bf16 values 36 us (134 MB
+// each way; a part of it stays in the L2 cache), of 131076 36. Below that the loads' number does: of 131074 (4 bytes) 45, 131071 (2) 77, 262143 single bytes 153; 2 x 32 layers of 33333 f32 values 89,
+// 33332 67. A token history of 1000 2.5.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>

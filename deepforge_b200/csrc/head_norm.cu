@@ -3,7 +3,10 @@
 // A row is one token's head, D channels. It is taken by a group of lanes that hold it in registers between its sum of squares and its result
 // (pairs that turn together lie in one lane), so that it is read once and written once: HBM is what bounds both kernels, and close behind it the chain of instructions of
 // a row, which few warps hide (registers hold the angles and the gradients' sums). 2 x 8192 tokens of 32 + 8 heads of 128 bf16 channels 58 us (the bytes alone 51); gradients of
-// 4 x 2048 such tokens 51.5 (38.5), of 3 x 1001 f32 tokens with gains of every head 37.5 (22.6), the sums of dgain among them (6, half of it behind the first kernel's end).
+// 4 x 2048 such tokens 51.5 (38.5), of 3 x 1001 f32 tokens with gains of every head 37.3 (22.6), the sums of dgain among them (6, half of it behind the first kernel's end).
+// Token by token as slices of one buffer 60 and 52; with 16-bit gains 60; f32 rows 57 (51). With gains of every head, which a row takes from shared memory, 79 (f32 rows 61) and gradients 105; half of
+// a head turned as halves apart, where a unit of what stays has half the bytes, 86 and 82. Outside the vectors a warp takes a row value by value or twice: 2 x 2048 tokens of 66 channels 79 (6.6), of 128 off
+// the boundaries 83 (12.8), gradients 146 and 271; of 4 + 1 heads of 1024 channels 38 (12.8), gradients 159.
 #include <algorithm>
 #include <cmath>
 

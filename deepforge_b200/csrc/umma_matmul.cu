@@ -2,7 +2,7 @@
 // K or N contiguous, 16-bit floats (bf16, f16), FP8 codes (MATMUL_FP8), FP8 codes with E8M0 block scales (MXFP8) or 8-bit integers (MATMUL_INT8).
 //
 // kIntegers: sums in 32-bit integers, exact in any order and shape; partial tiles of a split K are added as integers. The scales of a row and of 32 columns at a time, and a 16-bit bias, are loaded under the
-// part before and applied in the epilogue (a bias waited for in its place: 2394 x 256 x 14016 41.5 us, 33.4 so). 8192 x 4096 x 4096 to bf16 86 us (96 % of twice the bf16 rate), 32 x 4096 x 4096 7.2 (16.8 MB of weights: 2.6).
+// part before and applied in the epilogue (a bias waited for in its place: 2394 x 256 x 14016 41.5 us, 33.5 so, 30.0 without one; an f32 bias is waited for: 42.4). 8192 x 4096 x 4096 to bf16 86 us (96 % of twice the bf16 rate), 32 x 4096 x 4096 7.2 (16.8 MB of weights: 2.6).
 //
 // kPieces: f32 operands as three bf16 pieces each (split_f32.cu), six products of a K block's tiles per stage: every piece is copied
 // once for two products (six-fold deep copies moved and stored twice as much: 1183 x 1888 x 5360 154 us then, 128 now, 87 of
@@ -905,7 +905,9 @@ umma_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                             if (col + lane < args.n_total && healthy_now(ok, status)) {
                                 const int64_t at = (row0 + quarter) * args.out_ld + col + lane;
                                 constexpr bool kF32Only = kInRegisters<KIND> || KIND == kScaledSummed;
-                                constexpr int kRowsAtOnce = kInRegisters<KIND> || KIND == kPieces ? 4 : 8;   // (the others have no registers to spare)
+                                // (The former have no registers to spare: three forms of those that hold sums in registers spill 8 to 32 bytes, which costs no time that could be measured; 65 products of all
+                                // types, with rows on and off the boundaries, were nowhere more than 1.8 % slower than before they stored so, 11 % quicker in f16 4096^3 to f32.)
+                                constexpr int kRowsAtOnce = kInRegisters<KIND> || KIND == kPieces ? 4 : 8;
                                 auto put = [&](int dtype) {   // (one branch for all)
 #pragma unroll kRowsAtOnce
                                     for (int r = 0; r < live_rows; ++r)
