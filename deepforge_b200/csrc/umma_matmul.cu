@@ -905,7 +905,7 @@ umma_matmul_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_const
                             if (col + lane < args.n_total && healthy_now(ok, status)) {
                                 const int64_t at = (row0 + quarter) * args.out_ld + col + lane;
                                 constexpr bool kF32Only = kInRegisters<KIND> || KIND == kScaledSummed;
-                                // (The former have no registers to spare: three forms of those that hold sums in registers spill 8 to 32 bytes, which costs no time that could be measured; 65 products of all
+                                // (The former have no registers to spare: three forms of those that hold sums in registers spill 8 to 32 bytes, which costs no time that could be measured; 84 products of all
                                 // types, with rows on and off the boundaries, were nowhere more than 1.8 % slower than before they stored so, 11 % quicker in f16 4096^3 to f32.)
                                 constexpr int kRowsAtOnce = kInRegisters<KIND> || KIND == kPieces ? 4 : 8;
                                 auto put = [&](int dtype) {   // (one branch for all)

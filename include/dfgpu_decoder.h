@@ -87,8 +87,8 @@ int dfgpu_token_quantize(const dfgpu_token_quantize_params*, void* const* tensor
    [..., 1, N], of the same rank, their batch axes 1 or (a_scale) A's. DFGPU_MATMUL_INT8_UMMA: tcgen05 (kind::i8); A with K contiguous, B with K or N
    contiguous, their rows on 16-byte boundaries (any extents), C and the bias with N contiguous, batch axes that fold into M. DFGPU_MATMUL_INT8_FEW: at
    most 16 rows of A, A and B with K contiguous on 16-byte boundaries, batch axes that fold into M, any C and bias: for a decoder's step, bound by B. AUTO takes the quicker of the two
-   where it can; everything else goes to the CUDA cores, which take any layout at 20 to 75 times the time: rows or columns off the 16-byte boundaries, K contiguous
-   in neither, a B for each batch entry, and batches whose rows do not lie evenly (a padded buffer: call once an entry instead). The result does not depend on the kernel. */
+   where it can; everything else goes to the CUDA cores, which take any layout at 20 to 75 times the time: rows or columns off the 16-byte boundaries, an A whose K
+   is not contiguous, a B for each batch entry, and batches whose rows do not lie evenly (a padded buffer: call once an entry instead). The result does not depend on the kernel. */
 enum { DFGPU_MATMUL_INT8_AUTO = 0, DFGPU_MATMUL_INT8_CORES = 1, DFGPU_MATMUL_INT8_UMMA = 2, DFGPU_MATMUL_INT8_FEW = 3 };
 typedef struct dfgpu_matmul_int8_params {
     dfgpu_tensor a, b, c;
